@@ -1,0 +1,965 @@
+// The 8-bit key/value cache (gfx950 / CDNA4): its write, its read-back and the
+// attention rows over it.
+//
+// One layer's cache holds e4m3 codes with a power-of-two scale for each block
+// of 64 tokens, kv head and tensor; value = code * scale.
+//   k       [B, Hkv, cap, D]            a token's row is D bytes
+//   v       [B, Hkv, cap / 64, D, 64]   a block's tokens for one column together;
+//                                       token 16 t + 4 g + r (t, g, r in 0..3)
+//                                       at place 16 g + 4 t + r
+//   scales  [B, Hkv, cap / 64] fp32     2^e, e in [E_MIN, E_MAX]
+//
+// Why powers of two: e4m3 is a floating format, so a finer scale would gain no
+// relative precision, while with 2^e every value code * scale is exact in bf16,
+// and a block's codes move to a larger scale (when a later token of the block
+// needs one) without a second rounding, apart from those that become subnormal.
+//
+// Why this place order of the values: the attention rows form S^T = K Q^T and
+// O^T = V^T P^T with 16x16x32 MFMAs. A lane (column c = lane % 16, group g =
+// lane / 16) then holds the probabilities of tokens 16 t + 4 g + r of its row c,
+// which is the second product's right operand as it stands, if the left operand
+// V^T holds the same tokens in the same lane: 16 consecutive bytes of a column
+// of the cache. Neither product needs LDS or a transpose.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "capi_common.h"
+#include "delta_attn.h"
+#include "device_common.h"
+
+namespace da {
+namespace {
+
+constexpr int KB = 64;               // tokens per block
+constexpr int MAX_CAP = 1 << 30;     // tokens of a sequence (row numbers and limits stay inside 32 bits)
+constexpr int E_MIN = -117;          // 2^-9 * 2^-117 (the smallest code's value) is a normal float
+constexpr int E_MAX = 120;           // 448 * 2^120 reaches the largest bf16
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+template <typename T> struct Half;   // 16-bit element: bits of infinity, largest value
+template <> struct Half<__bf16> {
+  static constexpr uint32_t inf = 0x7f80;
+  static constexpr float max = 3.3895313892515355e38f;
+};
+template <> struct Half<_Float16> {
+  static constexpr uint32_t inf = 0x7c00;
+  static constexpr float max = 65504.f;
+};
+
+// Token of place p of a block's values, and the other way round.
+__host__ __device__ constexpr int token_of(int p) { return (p % 16 / 4) * 16 + (p / 16) * 4 + p % 4; }
+
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// The smallest e with amax <= 448 * 2^e, in [E_MIN, E_MAX]: 448 = 1.75 * 2^8.
+__device__ __forceinline__ int block_exponent(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u);
+  return min(max(e, E_MIN), E_MAX);
+}
+
+// Exponent of a stored scale (any bits give one in range).
+__device__ __forceinline__ int scale_exponent(float s) {
+  return min(max((int)((__float_as_uint(s) >> 23) & 0xff) - 127, E_MIN), E_MAX);
+}
+
+// Four codes times f, rounded to codes again.
+__device__ __forceinline__ uint32_t move4(uint32_t w, float f) {
+  const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a.x * f, a.y * f, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(b.x * f, b.y * f, r, true);
+}
+
+// Byte i of the result is 0xff where bit i of `bits` is set.
+__device__ __forceinline__ uint32_t byte_mask(uint32_t bits) {
+  return ((bits & 1) * 0xffu) | ((bits >> 1 & 1) * 0xff00u) | ((bits >> 2 & 1) * 0xff0000u) |
+         ((bits >> 3 & 1) * 0xff000000u);
+}
+
+struct Cache {
+  uint8_t *k, *v;
+  float *ks, *vs;
+  int64_t k_b, k_h, v_b, v_h, ks_b, ks_h, vs_b, vs_h;   // batch and head strides
+  int cap;
+};
+
+// ---------------------------------------------------------------------------
+// write: one wave per block, head and tensor. A lane holds 8 columns of D / 8
+// tokens, those of consecutive places, so that keys (8 bytes of a row) and
+// values (D / 8 bytes of a column) are both packed inside the lane; only the
+// block's largest magnitude crosses lanes.
+struct WriteArgs {
+  Cache c;
+  const void *k, *v;
+  int64_t kx_b, kx_s, kx_h, vx_b, vx_s, vx_h;
+  const int64_t* pos_dev;
+  int64_t pos;
+  const int* counts;
+  int pos_step, counts_step;   // 1: an entry per sequence, 0: one for all
+  int B, Hkv, S, n_blk;
+  int64_t units;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
+  using E = Elt<T>;
+  constexpr int DG = D / 8, TPL = D / 8;       // lanes across a row, tokens per lane
+  const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (unit >= a.units) return;
+  const int lane = threadIdx.x % 64;
+  const bool is_v = unit & 1;
+  int64_t u = unit >> 1;
+  const int h = (int)(u % a.Hkv);
+  u /= a.Hkv;
+  const int j = (int)(u % a.n_blk);
+  const int b = (int)(u / a.n_blk);
+  const int64_t pos = a.pos_dev ? a.pos_dev[(int64_t)b * a.pos_step] : a.pos;
+  const int count = a.counts ? min(max(a.counts[(int64_t)b * a.counts_step], 0), a.S) : a.S;
+  if (pos < 0 || pos > (int64_t)a.c.cap - count) return;
+  const int blk = (int)(pos / KB) + j;
+  const int base = blk * KB;
+  const int r0 = max((int)pos - base, 0), r1 = min((int)pos + count - base, KB);   // its new rows
+  if (r1 <= r0) return;
+  const bool full = r0 == 0 && r1 == KB;
+
+  const int dg = lane % DG, p0 = lane / DG * TPL;
+  const T* src = is_v ? (const T*)a.v + b * a.vx_b + h * a.vx_h : (const T*)a.k + b * a.kx_b + h * a.kx_h;
+  const int64_t step = is_v ? a.vx_s : a.kx_s;
+  src += (int64_t)(base - (int)pos) * step + dg * 8;
+  u32x4 x[TPL];
+  uint32_t fresh = 0, older = 0;               // bit i: token i of this lane is new, or holds an earlier token
+#pragma unroll
+  for (int i = 0; i < TPL; ++i) {
+    const int r = token_of(p0 + i);
+    x[i] = *(const u32x4*)(src + (int64_t)min(max(r, r0), r1 - 1) * step);
+    fresh |= (uint32_t)(r >= r0 && r < r1) << i;
+    older |= (uint32_t)(r < r0) << i;
+  }
+  u16x2 m = {0, 0};
+#pragma unroll
+  for (int i = 0; i < TPL; ++i) {
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[i][w] & 0x7fff7fffu));
+  }
+  uint32_t top = max((uint32_t)m.x, (uint32_t)m.y);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+  const bool odd = top >= Half<T>::inf;        // infinities or NaN among them
+  if (odd) {
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < TPL; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t lo = x[i][w] & 0x7fffu, hi = x[i][w] >> 16 & 0x7fffu;
+        top = max(top, max(lo < Half<T>::inf ? lo : 0u, hi < Half<T>::inf ? hi : 0u));
+      }
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
+  }
+  int e = block_exponent(E::lo(top));
+  float* scale = (is_v ? a.c.vs + b * a.c.vs_b + h * a.c.vs_h : a.c.ks + b * a.c.ks_b + h * a.c.ks_h) + blk;
+  bool grown = false;
+  float f = 1.f;
+  if (r0 > 0) {
+    const int eo = scale_exponent(*scale);
+    grown = e > eo;
+    if (grown) f = pow2(eo) * pow2(-e);        // (0 where that is below the floats: so are the values)
+    e = max(e, eo);
+  }
+  const float inv = pow2(-e);
+  if (lane == 0) *scale = pow2(e);
+  // a finite value is at most 448 after the scale; the others become NaN
+  auto val = [&](uint32_t w, bool hi) __attribute__((always_inline)) {
+    const float y = (hi ? E::hi(w) : E::lo(w)) * inv;
+    return odd && !(fabsf(y) < 512.f) ? __builtin_nanf("") : y;
+  };
+  if (!is_v) {
+    uint8_t* dst = a.c.k + b * a.c.k_b + h * a.c.k_h + (int64_t)base * D + dg * 8;
+#pragma unroll
+    for (int i = 0; i < TPL; ++i) {
+      u32x2 w;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(val(x[i][2 * n], false), val(x[i][2 * n], true), 0, false);
+        w[n] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(val(x[i][2 * n + 1], false), val(x[i][2 * n + 1], true), c, true);
+      }
+      u32x2* row = (u32x2*)(dst + token_of(p0 + i) * D);
+      if (full || (fresh >> i & 1)) {
+        *row = w;
+      } else if (grown && (older >> i & 1)) {
+        const u32x2 o = *row;
+        *row = (u32x2){move4(o[0], f), move4(o[1], f)};
+      }
+    }
+  } else {
+    uint8_t* dst = a.c.v + b * a.c.v_b + h * a.c.v_h + (int64_t)blk * KB * D + dg * 8 * KB + p0;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      uint32_t* run = (uint32_t*)(dst + n * KB);
+      uint32_t w[TPL / 4];
+#pragma unroll
+      for (int q = 0; q < TPL / 4; ++q) {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(val(x[4 * q][n / 2], n & 1), val(x[4 * q + 1][n / 2], n & 1), 0, false);
+        w[q] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(val(x[4 * q + 2][n / 2], n & 1), val(x[4 * q + 3][n / 2], n & 1), c, true);
+        if (!full) {
+          const uint32_t o = run[q];
+          const uint32_t nm = byte_mask(fresh >> 4 * q), om = grown ? byte_mask(older >> 4 * q) : 0;
+          w[q] = (w[q] & nm) | (move4(o, f) & om) | (o & ~(nm | om));
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < TPL / 4; ++q) run[q] = w[q];
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// read: the write's lanes the other way round.
+struct ReadArgs {
+  Cache c;
+  void *k, *v;
+  int64_t ko_b, ko_h, ko_s, vo_b, vo_h, vo_s;
+  const int* n_keys;
+  int n_step;
+  int B, Hkv, start, n, n_blk;
+  int64_t units;
+};
+
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
+  using E = Elt<T>;
+  constexpr int DG = D / 8, TPL = D / 8;
+  const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
+  if (unit >= a.units) return;
+  const int lane = threadIdx.x % 64;
+  const bool is_v = unit & 1;
+  int64_t u = unit >> 1;
+  const int h = (int)(u % a.Hkv);
+  u /= a.Hkv;
+  const int blk = a.start / KB + (int)(u % a.n_blk);
+  const int b = (int)(u / a.n_blk);
+  const int live = a.n_keys ? a.n_keys[(int64_t)b * a.n_step] : a.c.cap;
+  const int dg = lane % DG, p0 = lane / DG * TPL;
+  const float s = (is_v ? a.c.vs + b * a.c.vs_b + h * a.c.vs_h : a.c.ks + b * a.c.ks_b + h * a.c.ks_h)[blk];
+  const bool sat = 448.f * s > Half<T>::max;   // (also where the product is infinite)
+  auto fix = [&](float y) __attribute__((always_inline)) {
+    return sat && y == y ? fminf(fmaxf(y, -Half<T>::max), Half<T>::max) : y;
+  };
+  T* dst = is_v ? (T*)a.v + b * a.vo_b + h * a.vo_h : (T*)a.k + b * a.ko_b + h * a.ko_h;
+  const int64_t step = is_v ? a.vo_s : a.ko_s;
+  auto put = [&](int r, u32x4 w) __attribute__((always_inline)) {
+    const int row = blk * KB + r;
+    if (row < a.start || row >= a.start + a.n) return;
+    if (row >= live) w = (u32x4){0, 0, 0, 0};
+    *(u32x4*)(dst + (int64_t)(row - a.start) * step + dg * 8) = w;
+  };
+  if (!is_v) {
+    const uint8_t* src = a.c.k + b * a.c.k_b + h * a.c.k_h + (int64_t)blk * KB * D + dg * 8;
+#pragma unroll
+    for (int i = 0; i < TPL; ++i) {
+      const int r = token_of(p0 + i);
+      const u32x2 w = *(const u32x2*)(src + r * D);
+      u32x4 o;
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[n], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[n], true);
+        o[2 * n] = E::pack2(fix(lo.x * s), fix(lo.y * s));
+        o[2 * n + 1] = E::pack2(fix(hi.x * s), fix(hi.y * s));
+      }
+      put(r, o);
+    }
+  } else {
+    const uint8_t* src = a.c.v + b * a.c.v_b + h * a.c.v_h + (int64_t)blk * KB * D + dg * 8 * KB + p0;
+#pragma unroll
+    for (int q = 0; q < TPL / 4; ++q) {
+      float y[4][8];
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const uint32_t w = *(const uint32_t*)(src + n * KB + 4 * q);
+        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+        y[0][n] = fix(lo.x * s);
+        y[1][n] = fix(lo.y * s);
+        y[2][n] = fix(hi.x * s);
+        y[3][n] = fix(hi.y * s);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        put(token_of(p0 + 4 * q + r), (u32x4){E::pack2(y[r][0], y[r][1]), E::pack2(y[r][2], y[r][3]),
+                                              E::pack2(y[r][4], y[r][5]), E::pack2(y[r][6], y[r][7])});
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// attention rows at the end of each sequence's cache
+struct RowsArgs {
+  Cache c;
+  const void* q;
+  int64_t q_b, q_h, q_s;
+  void* o;
+  int64_t o_b, o_h, o_s;
+  const void* add;
+  int64_t add_b, add_h, add_s;
+  const int* n_dev;         // key counts on the device (entry b * n_step), or NULL: `n`
+  int n_step, n;
+  int B, Hkv, G, s;         // G query heads per kv head, s rows at the end of each sequence
+  int n_rt, rows;           // row tiles of `rows` rows (flattened row i * G + head) per sequence and kv head
+  int window, sink;
+  float scale_log2;         // sm_scale * log2(e)
+  int target;               // items asked for
+  float* part;              // per item: rows x D sums, then rows references, rows weights
+  int64_t pitch;            // floats per item
+};
+
+constexpr float NO_KEYS = -1e30f;
+// Probabilities are held relative to a row reference that may lag its maximum
+// by up to LAG (log2), times 2^BIAS: at most 2^14, inside fp16, and fp16 ends
+// 2^-32 below the reference.
+constexpr float LAG = 6.f, BIAS = 8.f;
+
+// The blocks that a sequence's rows see: those of the sinks, then [lo, hi).
+struct Blocks {
+  int first, lo, n;         // sink blocks, first block after them, all together
+  __device__ __forceinline__ int at(int i) const { return i < first ? i : lo + i - first; }
+};
+
+__device__ __forceinline__ int keys_of(const RowsArgs& a, int b) {
+  const int n = a.n_dev ? a.n_dev[(int64_t)b * a.n_step] : a.n;
+  return min(max(n, 0), a.c.cap);
+}
+
+__device__ __forceinline__ Blocks blocks_of(const RowsArgs& a, int n) {
+  Blocks l;
+  l.lo = a.window > 0 ? max(n - a.s - a.window + 1, 0) / KB : 0;
+  l.first = a.window > 0 ? min((a.sink + KB - 1) / KB, l.lo) : 0;
+  l.n = l.first + (n + KB - 1) / KB - l.lo;
+  return l;
+}
+
+constexpr int WAVES = 4;
+
+// Splits: every item takes `chunk` blocks of one (sequence, kv head, row tile);
+// chunk is the launch's blocks over the items asked for, so that sequences of
+// different lengths give items of one size. An item's place is found by each
+// wave for itself: the sequences' item counts, summed over 64 lanes.
+struct Place {
+  int b, unit, split, n_split, chunk, slot0;   // unit: kv head * n_rt + row tile; slot0: its first item
+};
+
+__device__ __forceinline__ int chunk_of(int64_t blocks, int target) {
+  const int64_t c = (blocks + target - 1) / target;
+  return (int)((c + WAVES - 1) / WAVES) * WAVES;
+}
+
+__device__ __forceinline__ int wave_sum(int x) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+  return x;
+}
+
+// ITEM: `i` counts items, otherwise (sequence, unit) pairs.
+template <bool ITEM>
+__device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
+  const int lane = threadIdx.x % 64;
+  const int units = a.Hkv * a.n_rt;
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int n = b0 + lane < a.B ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
+    total += wave_sum(n);
+  }
+  p.chunk = max(chunk_of(total * units, a.target), WAVES);
+  int before = 0;           // items of the sequences before
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const bool in = b0 + lane < a.B;
+    const int n = in ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
+    const int mine = in ? max((n + p.chunk - 1) / p.chunk, 1) : 0;
+    int upto = mine;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int x = __shfl_up(upto, off);
+      if (lane >= off) upto += x;
+    }
+    const int have = ITEM ? i - before : i - b0 * units;     // in this batch of sequences
+    const int end = ITEM ? upto * units : (lane + 1) * units;
+    const uint64_t past = __ballot(in && end > have);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      const int start = __shfl(upto - mine, l) * units;
+      p.n_split = __shfl(mine, l);
+      p.b = b0 + l;
+      if (ITEM) {
+        const int rest = have - start;
+        p.unit = rest / p.n_split;
+        p.split = rest % p.n_split;
+      } else {
+        p.unit = have - l * units;
+        p.split = 0;
+      }
+      p.slot0 = before + start + p.unit * p.n_split;
+      return true;
+    }
+    before += __shfl(upto, 63) * units;
+  }
+  return false;
+}
+
+__device__ __forceinline__ float group_max(float x) {   // over the four lanes of one row
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
+template <typename T> struct Dot;    // 16x16x32 products of Q's type
+template <> struct Dot<__bf16> {
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ u32x4 codes(uint32_t lo, uint32_t hi) {
+    return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true))};
+  }
+};
+template <> struct Dot<_Float16> {
+  static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ u32x4 codes(uint32_t lo, uint32_t hi) {
+    return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, true))};
+  }
+};
+
+// Stores a finished row's four columns: rnd(o), or rnd(rnd(o) + add).
+template <typename T>
+__device__ __forceinline__ void store4(const RowsArgs& a, int b, int h, int i, int d, f32x4 o) {
+  using E = Elt<T>;
+  u32x2 w = {E::pack2(o[0], o[1]), E::pack2(o[2], o[3])};
+  if (a.add) {
+    const u32x2 x = *(const u32x2*)((const T*)a.add + b * a.add_b + h * a.add_h + i * a.add_s + d);
+    w = (u32x2){E::pack2(E::lo(w[0]) + E::lo(x[0]), E::hi(w[0]) + E::hi(x[0])),
+                E::pack2(E::lo(w[1]) + E::lo(x[1]), E::hi(w[1]) + E::hi(x[1]))};
+  }
+  *(u32x2*)((T*)a.o + b * a.o_b + h * a.o_h + i * a.o_s + d) = w;
+}
+
+// MT: 16-row tiles per wave. The P V product is formed in fp16 whatever Q's
+// type: the codes are exact in it, and its 11 bits keep the probabilities'
+// rounding below that of a bf16 result.
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(64 * WAVES) void kv8_rows_kernel(RowsArgs a) {
+  constexpr int KS = D / 32;                 // steps of the Q K product
+  constexpr int KW = D >= 64 ? D / 64 : 1;   // loads of a key's row per lane
+  constexpr int DT = D / 16;
+  using P = Dot<_Float16>;
+  Place p;
+  if (!locate<true>(a, blockIdx.x, p)) return;
+  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int c = lane % 16, g = lane / 16;
+  const int b = p.b, hk = p.unit / a.n_rt, m0 = p.unit % a.n_rt * a.rows;
+  const int n = keys_of(a, b);
+  const Blocks list = blocks_of(a, n);
+  const int n_rows = min(a.rows, a.s * a.G - m0);
+
+  // Q as the product's right operand, its columns in the order of the keys'
+  // loads: step 2 w + u holds columns 64 w + 16 g + 8 u .. + 7
+  u32x4 qf[MT][KS];
+  int lim[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int m = m0 + mt * 16 + c;
+    const bool in = mt * 16 + c < n_rows;
+    const int i = m / a.G;
+    lim[mt] = in ? n - a.s + i : -1;
+    const T* src = (const T*)a.q + b * a.q_b + (int64_t)(hk * a.G + m % a.G) * a.q_h + i * a.q_s;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int d = D >= 64 ? k / 2 * 64 + g * 16 + k % 2 * 8 : g * 8;
+      qf[mt][k] = in ? *(const u32x4*)(src + d) : (u32x4){0, 0, 0, 0};
+    }
+  }
+  const uint8_t* kc = a.c.k + b * a.c.k_b + hk * a.c.k_h;
+  const uint8_t* vc = a.c.v + b * a.c.v_b + hk * a.c.v_h;
+  const float* ksc = a.c.ks + b * a.c.ks_b + hk * a.c.ks_h;
+  const float* vsc = a.c.vs + b * a.c.vs_b + hk * a.c.vs_h;
+
+  f32x4 acc[MT][DT], sum[MT];
+  float ref[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    ref[mt] = NO_KEYS;
+    sum[mt] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[mt][t] = (f32x4){0, 0, 0, 0};
+  }
+  const uint32_t one = 0x3c003c00u;
+  const u32x4 ones = {one, one, one, one};
+  // rows m0 / G .. of the tile: the first's and the last's limits
+  const int lim_lo = n - a.s + m0 / a.G, lim_hi = n - a.s + (m0 + n_rows - 1) / a.G;
+
+  const int end = min((p.split + 1) * p.chunk, list.n);
+  for (int x = p.split * p.chunk + wave; x < end; x += WAVES) {
+    const int blk = __builtin_amdgcn_readfirstlane(list.at(x));
+    const int key0 = blk * KB;
+    if (key0 > lim_hi) continue;
+    // every row sees every key of the block?
+    const bool whole = key0 + KB - 1 <= lim_lo &&
+        (a.window == 0 || key0 > lim_hi - a.window || key0 + KB <= a.sink);
+    const uint8_t* kb = kc + (int64_t)key0 * D;
+    const uint8_t* vb = vc + (int64_t)key0 * D;
+    u32x4 kf[4][KW], vf[DT];
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int w = 0; w < KW; ++w) {
+        const uint8_t* src = kb + (t * 16 + c) * D;
+        if constexpr (D >= 64) {
+          kf[t][w] = *(const u32x4*)(src + w * 64 + g * 16);
+        } else {
+          const u32x2 y = *(const u32x2*)(src + g * 8);
+          kf[t][w] = (u32x4){y[0], y[1], 0, 0};
+        }
+      }
+#pragma unroll
+    for (int t = 0; t < DT; ++t) vf[t] = *(const u32x4*)(vb + (t * 16 + c) * KB + g * 16);
+    const float sc = ksc[blk] * a.scale_log2;
+    const float vs = vsc[blk];
+
+    u32x4 pf[MT][2];
+    uint32_t seen[MT];                        // bit 4 t + r: the row sees token 16 t + 4 g + r
+    {
+      f32x4 s[MT][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][t] = (f32x4){0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          const u32x4 af = Dot<T>::codes(kf[t][k / 2][k % 2 * 2], kf[t][k / 2][k % 2 * 2 + 1]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) s[mt][t] = Dot<T>::mfma(af, qf[mt][k], s[mt][t]);
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        seen[mt] = 0xffffu;
+        if (!whole) {
+          seen[mt] = 0;
+          const int lo = a.window > 0 ? lim[mt] - a.window : -1;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = key0 + e / 4 * 16 + g * 4 + e % 4;
+            seen[mt] |= (uint32_t)(key <= lim[mt] && (key > lo || key < a.sink)) << e;
+          }
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          float y = s[mt][e / 4][e % 4] * sc;
+          if (!whole) y = seen[mt] >> e & 1 ? y : -INFINITY;
+          s[mt][e / 4][e % 4] = y;
+          top = fmaxf(top, y);
+        }
+        top = group_max(top);
+        if (__any(top > ref[mt] + LAG)) {
+          const float to = fmaxf(ref[mt], top);
+          const float alpha = fast_exp2(ref[mt] - to);
+          ref[mt] = to;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[mt][r] *= alpha;
+#pragma unroll
+          for (int t = 0; t < DT; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc[mt][t][r] *= alpha;
+        }
+        const float off = BIAS - ref[mt];
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int t = 2 * u + w / 2, r = w % 2 * 2;
+            float y0 = fast_exp2(s[mt][t][r] + off), y1 = fast_exp2(s[mt][t][r + 1] + off);
+            if (!whole) {
+              y0 = seen[mt] >> (4 * t + r) & 1 ? y0 : 0.f;
+              y1 = seen[mt] >> (4 * t + r + 1) & 1 ? y1 : 0.f;
+            }
+            pf[mt][u][w] = Elt<_Float16>::pack2(y0, y1);
+          }
+      }
+    }
+    if (!whole) {
+      // A NaN code of a token that a row does not see (rows behind the last
+      // key, or outside the row's window) must not reach it through 0 * NaN:
+      // the codes are taken as zero, and the rows that do see one get theirs
+      // from a product of the codes' and the rows' marks.
+      uint32_t bad = 0;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) bad |= (vf[t][w] & 0x7f7f7f7fu) + 0x01010101u;
+      if (__any((bad & 0x80808080u) != 0)) {
+        u32x4 mark[MT][2];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const uint32_t two = seen[mt] >> (8 * u + 2 * w) & 3;
+              mark[mt][u][w] = (two & 1 ? 0x3c00u : 0u) | (two & 2 ? 0x3c000000u : 0u);
+            }
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          u32x4 nan;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t hit = ((vf[t][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // bit 7 of NaN bytes
+            nan[w] = (hit >> 7) * 0x38u;                                                    // 1.0 there
+            vf[t][w] &= ~((hit >> 7) * 0xffu);
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            f32x4 hits = {0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) hits = P::mfma(P::codes(nan[2 * u], nan[2 * u + 1]), mark[mt][u], hits);
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (hits[r] > 0.f) acc[mt][t][r] = __builtin_nanf("");
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) sum[mt] = P::mfma(ones, pf[mt][u], sum[mt]);
+#pragma unroll
+    for (int t = 0; t < DT; ++t) {
+      const u32x4 v0 = P::codes(vf[t][0], vf[t][1]), v1 = P::codes(vf[t][2], vf[t][3]);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        f32x4 y = P::mfma(v0, pf[mt][0], (f32x4){0, 0, 0, 0});
+        y = P::mfma(v1, pf[mt][1], y);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[mt][t][r] = fmaf(y[r], vs, acc[mt][t][r]);
+      }
+    }
+  }
+
+  // join the waves, one 16-row tile after the other
+  constexpr int LD = D + 4;                    // row pitch: the 16 rows of a column spread over the banks
+  __shared__ float s_o[WAVES][16][LD];
+  __shared__ float s_m[WAVES][16], s_l[WAVES][16];
+  float* part = a.part + (int64_t)(p.slot0 + p.split) * a.pitch;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    if (mt > 0) __syncthreads();
+#pragma unroll
+    for (int t = 0; t < DT; ++t) *(f32x4*)&s_o[wave][c][t * 16 + g * 4] = acc[mt][t];
+    if (g == 0) {
+      s_m[wave][c] = ref[mt];
+      s_l[wave][c] = sum[mt][0];
+    }
+    __syncthreads();
+    for (int task = threadIdx.x; task < 16 * (D / 4); task += 64 * WAVES) {
+      const int r = task / (D / 4), d = task % (D / 4) * 4, row = mt * 16 + r;
+      if (row >= n_rows) break;
+      float M = s_m[0][r];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) M = fmaxf(M, s_m[w][r]);
+      float L = 0.f;
+      f32x4 o = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        const float k = fast_exp2(s_m[w][r] - M);
+        const f32x4 y = *(const f32x4*)&s_o[w][r][d];
+        L = fmaf(s_l[w][r], k, L);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], k, o[e]);
+      }
+      if (p.n_split == 1) {
+        const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] *= inv;
+        const int m = m0 + row;
+        store4<T>(a, b, hk * a.G + m % a.G, m / a.G, d, o);
+      } else {
+        *(f32x4*)(part + row * D + d) = o;
+        if (d == 0) {
+          part[a.rows * D + row] = M;
+          part[a.rows * (D + 1) + row] = L;
+        }
+      }
+    }
+  }
+}
+
+// Joins the items of one (sequence, kv head, row tile): a workgroup per row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void kv8_join_kernel(RowsArgs a) {
+  constexpr int CT = D / 4, SG = 256 / CT;     // threads across a row, splits taken side by side
+  __shared__ float s_w[SG][3];
+  __shared__ f32x4 s_o[SG][CT];
+  const int row = blockIdx.y;
+  Place p;
+  if (!locate<false>(a, blockIdx.x, p) || p.n_split == 1) return;
+  const int m = p.unit % a.n_rt * a.rows + row;
+  if (m >= a.s * a.G) return;
+  const int t = threadIdx.x % CT, sg = threadIdx.x / CT;
+  const float* part = a.part + p.slot0 * a.pitch;
+  float M = NO_KEYS, L = 0.f;
+  f32x4 o = {0, 0, 0, 0};
+  for (int i = sg; i < p.n_split; i += SG) {
+    const float* src = part + i * a.pitch;
+    const float mi = src[a.rows * D + row], li = src[a.rows * (D + 1) + row];
+    const f32x4 y = *(const f32x4*)(src + row * D + t * 4);
+    const float to = fmaxf(M, mi);
+    const float k0 = fast_exp2(M - to), k1 = fast_exp2(mi - to);
+    M = to;
+    L = L * k0 + li * k1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * k0 + y[e] * k1;
+  }
+  s_o[sg][t] = o;
+  if (t == 0) {
+    s_w[sg][0] = M;
+    s_w[sg][1] = L;
+  }
+  __syncthreads();
+  if (sg > 0) return;
+#pragma unroll
+  for (int i = 1; i < SG; ++i) M = fmaxf(M, s_w[i][0]);
+  L = 0.f;
+  o = (f32x4){0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < SG; ++i) {
+    const float k = fast_exp2(s_w[i][0] - M);
+    const f32x4 y = s_o[i][t];
+    L = fmaf(s_w[i][1], k, L);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], k, o[e]);
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] *= inv;
+  store4<T>(a, p.b, p.unit / a.n_rt * a.G + m % a.G, m / a.G, t * 4, o);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+
+// Row tiles: as many 16-row tiles per wave as the rows fill, up to what the
+// registers hold.
+struct RowsPlan {
+  int mt, rows, n_rt;
+  int64_t pairs, items;     // (sequence, kv head, row tile) triples; item slots
+  int64_t pitch;            // floats of an item's partial sums (a multiple of 4)
+  int target;
+  size_t bytes;
+};
+
+RowsPlan plan_rows(int B, int Hkv, int G, int s, int D, int64_t max_keys, int window, int sink) {
+  RowsPlan p{};
+  const int64_t m = (int64_t)G * s;
+  p.mt = m <= 16 ? 1 : m <= 32 || D == 256 ? 2 : 4;
+  p.rows = (int)(m < 16 * p.mt ? m : 16 * p.mt);
+  const int64_t rt = (m + 16 * p.mt - 1) / (16 * p.mt);
+  p.n_rt = (int)rt;
+  p.pairs = (int64_t)B * Hkv * rt;
+  int64_t blocks = (max_keys + KB - 1) / KB;
+  if (window > 0) {
+    const int64_t near = ((int64_t)window + s + 2 * KB - 2) / KB + ((int64_t)sink + KB - 1) / KB;
+    if (near < blocks) blocks = near;
+  }
+  p.target = 1024;
+  // no more items than chunks of WAVES blocks: one for each pair at least
+  const int64_t chunks = (blocks + WAVES - 1) / WAVES;
+  const int64_t most = p.pairs * (chunks > 1 ? chunks : 1);
+  p.items = p.target + p.pairs < most ? p.target + p.pairs : most;
+  p.pitch = (int64_t)p.rows * D + (2 * p.rows + 3) / 4 * 4;
+  p.bytes = chunks <= 1 ? 0 : (size_t)(p.items * p.pitch) * sizeof(float);
+  return p;
+}
+
+bool kv8_cache(Cache& c, const void* k, const void* v, const float* ks, const float* vs,
+               const int64_t st[8], int cap) {
+  c = Cache{(uint8_t*)k, (uint8_t*)v, (float*)ks, (float*)vs, st[0], st[1], st[2], st[3],
+            st[4], st[5], st[6], st[7], cap};
+  return aligned16(k) && aligned16(v) && ((uintptr_t)ks & 3) == 0 && ((uintptr_t)vs & 3) == 0 &&
+         st[0] % 16 == 0 && st[1] % 16 == 0 && st[2] % 16 == 0 && st[3] % 16 == 0;
+}
+
+int check_cache(const void* k, const void* v, const float* ks, const float* vs, const int64_t* st,
+                int cap, int B, int Hkv, int D, int dtype) {
+  if (dtype != DA_BF16 && dtype != DA_FP16) return DA_ERR_DTYPE;
+  if (!head_dim_ok(D)) return DA_ERR_HEAD_DIM;
+  if (B < 0 || Hkv < 1 || cap < 0 || cap > MAX_CAP || cap % KB != 0 || !st) return DA_ERR_INVALID_ARG;
+  if (!k || !v || !ks || !vs) return DA_ERR_INVALID_ARG;
+  return DA_OK;
+}
+
+template <typename T, int D>
+void launch_rows(const RowsArgs& a, const RowsPlan& p, hipStream_t st) {
+  const dim3 grid((unsigned)p.items), block(64 * WAVES);
+  if (p.mt == 1) {
+    hipLaunchKernelGGL((kv8_rows_kernel<T, D, 1>), grid, block, 0, st, a);
+  } else if (p.mt == 2) {
+    hipLaunchKernelGGL((kv8_rows_kernel<T, D, 2>), grid, block, 0, st, a);
+  } else if constexpr (D < 256) {
+    hipLaunchKernelGGL((kv8_rows_kernel<T, D, 4>), grid, block, 0, st, a);
+  }
+  if (p.bytes > 0)
+    hipLaunchKernelGGL((kv8_join_kernel<T, D>), dim3((unsigned)p.pairs, (unsigned)p.rows), dim3(256), 0, st, a);
+}
+
+template <typename T> struct Tag { using type = T; };
+
+// f(Tag<element>, std::integral_constant<int, head dim>)
+template <typename F>
+void by_type(int dtype, int D, F&& f) {
+  auto dims = [&](auto t) {
+    if (D == 32) f(t, std::integral_constant<int, 32>{});
+    else if (D == 64) f(t, std::integral_constant<int, 64>{});
+    else if (D == 128) f(t, std::integral_constant<int, 128>{});
+    else f(t, std::integral_constant<int, 256>{});
+  };
+  if (dtype == DA_BF16) dims(Tag<__bf16>{});
+  else dims(Tag<_Float16>{});
+}
+
+int launched() { return hipGetLastError() == hipSuccess ? DA_OK : DA_ERR_LAUNCH; }
+
+}  // namespace
+}  // namespace da
+
+using namespace da;
+
+extern "C" int da_kv8_write(const void* k, const int64_t k_str[3], const void* v, const int64_t v_str[3],
+                            int B, int S, int Hkv, int D,
+                            void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                            const int64_t c_str[8], int cap,
+                            const int64_t* pos_dev, int pos_per_seq, int64_t pos,
+                            const int32_t* counts_dev, int counts_per_seq, int dtype, void* stream) {
+  int rc = check_cache(k_codes, v_codes, k_scale, v_scale, c_str, cap, B, Hkv, D, dtype);
+  if (rc != DA_OK) return rc;
+  if (S < 0 || !k_str || !v_str) return DA_ERR_INVALID_ARG;
+  if (!pos_dev && (pos < 0 || pos + S > cap)) return DA_ERR_INVALID_ARG;
+  if (S == 0 || B == 0) return DA_OK;
+  if (!k || !v) return DA_ERR_INVALID_ARG;
+  WriteArgs a{};
+  if (!kv8_cache(a.c, k_codes, v_codes, k_scale, v_scale, c_str, cap) || !aligned16(k) || !aligned16(v) ||
+      !strides8(k_str) || !strides8(v_str) || ((uintptr_t)pos_dev & 7) || ((uintptr_t)counts_dev & 3))
+    return DA_ERR_ALIGNMENT;
+  a.k = k;
+  a.v = v;
+  a.kx_b = k_str[0], a.kx_s = k_str[1], a.kx_h = k_str[2];
+  a.vx_b = v_str[0], a.vx_s = v_str[1], a.vx_h = v_str[2];
+  a.pos_dev = pos_dev;
+  a.pos = pos;
+  a.counts = counts_dev;
+  a.pos_step = pos_per_seq ? 1 : 0;
+  a.counts_step = counts_per_seq ? 1 : 0;
+  a.B = B, a.Hkv = Hkv, a.S = S;
+  // blocks that S tokens touch: from a known row, or from any
+  a.n_blk = pos_dev ? (int)(((int64_t)S + KB - 2) / KB + 1) : (int)((pos + S + KB - 1) / KB - pos / KB);
+  a.units = (int64_t)B * a.n_blk * Hkv * 2;
+  if ((a.units + 3) / 4 > 0x7fffffff) return DA_ERR_INVALID_ARG;
+  by_type(dtype, D, [&](auto t, auto d) {
+    hipLaunchKernelGGL((kv8_write_kernel<typename decltype(t)::type, decltype(d)::value>), dim3((unsigned)((a.units + 3) / 4)),
+                       dim3(256), 0, (hipStream_t)stream, a);
+  });
+  return launched();
+}
+
+extern "C" int da_kv8_read(const void* k_codes, const void* v_codes, const float* k_scale,
+                           const float* v_scale, const int64_t c_str[8], int cap,
+                           int B, int Hkv, int D, int start, int n,
+                           const int32_t* n_keys_dev, int n_keys_per_seq,
+                           void* k_out, const int64_t ko_str[3], void* v_out, const int64_t vo_str[3],
+                           int dtype, void* stream) {
+  int rc = check_cache(k_codes, v_codes, k_scale, v_scale, c_str, cap, B, Hkv, D, dtype);
+  if (rc != DA_OK) return rc;
+  if (start < 0 || n < 0 || (int64_t)start + n > cap || !ko_str || !vo_str) return DA_ERR_INVALID_ARG;
+  if (n == 0 || B == 0) return DA_OK;
+  if (!k_out || !v_out) return DA_ERR_INVALID_ARG;
+  ReadArgs a{};
+  if (!kv8_cache(a.c, k_codes, v_codes, k_scale, v_scale, c_str, cap) || !aligned16(k_out) || !aligned16(v_out) ||
+      !strides8(ko_str) || !strides8(vo_str) || ((uintptr_t)n_keys_dev & 3))
+    return DA_ERR_ALIGNMENT;
+  a.k = k_out;
+  a.v = v_out;
+  a.ko_b = ko_str[0], a.ko_h = ko_str[1], a.ko_s = ko_str[2];
+  a.vo_b = vo_str[0], a.vo_h = vo_str[1], a.vo_s = vo_str[2];
+  a.n_keys = n_keys_dev;
+  a.n_step = n_keys_per_seq ? 1 : 0;
+  a.B = B, a.Hkv = Hkv, a.start = start, a.n = n;
+  a.n_blk = (int)(((int64_t)start + n + KB - 1) / KB - start / KB);
+  a.units = (int64_t)B * a.n_blk * Hkv * 2;
+  if ((a.units + 3) / 4 > 0x7fffffff) return DA_ERR_INVALID_ARG;
+  by_type(dtype, D, [&](auto t, auto d) {
+    hipLaunchKernelGGL((kv8_read_kernel<typename decltype(t)::type, decltype(d)::value>), dim3((unsigned)((a.units + 3) / 4)),
+                       dim3(256), 0, (hipStream_t)stream, a);
+  });
+  return launched();
+}
+
+extern "C" size_t da_kv8_attn_workspace_bytes(int B, int Hq, int Hkv, int s, int D, int max_keys,
+                                              int window, int sink) {
+  if (B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv != 0 || s < 1 || !head_dim_ok(D) || max_keys < 0 ||
+      window < 0 || sink < 0)
+    return 0;
+  return plan_rows(B, Hkv, Hq / Hkv, s, D, max_keys, window, sink).bytes;
+}
+
+extern "C" int da_kv8_attn_fwd(const void* q, const int64_t q_str[3], const void* k_codes,
+                               const void* v_codes, const float* k_scale, const float* v_scale,
+                               const int64_t c_str[8], int cap, void* out, const int64_t o_str[3],
+                               int B, int Hq, int Hkv, int s, int D,
+                               const int32_t* n_keys_dev, int n_keys_per_seq, int n_keys,
+                               int window, int sink, float sm_scale,
+                               const void* addend, const int64_t add_str[3],
+                               void* workspace, size_t workspace_bytes, int dtype, void* stream) {
+  int rc = check_cache(k_codes, v_codes, k_scale, v_scale, c_str, cap, B, Hkv, D, dtype);
+  if (rc != DA_OK) return rc;
+  if (Hq < 1 || Hq % Hkv != 0 || s < 0 || window < 0 || sink < 0 || !q_str || !o_str) return DA_ERR_INVALID_ARG;
+  if (!n_keys_dev && (n_keys < 0 || n_keys > cap)) return DA_ERR_INVALID_ARG;
+  if (s == 0 || B == 0) return DA_OK;
+  if (!q || !out || (addend && !add_str)) return DA_ERR_INVALID_ARG;
+  RowsArgs a{};
+  if (!kv8_cache(a.c, k_codes, v_codes, k_scale, v_scale, c_str, cap) || !aligned16(q) || !aligned16(out) ||
+      !strides8(q_str) || !strides8(o_str) || ((uintptr_t)n_keys_dev & 3) ||
+      (addend && (!aligned16(addend) || !strides8(add_str))))
+    return DA_ERR_ALIGNMENT;
+  // (a window or sinks past the capacity are every key)
+  window = window < cap ? window : cap;
+  sink = sink < cap ? sink : cap;
+  const RowsPlan p = plan_rows(B, Hkv, Hq / Hkv, s, D, n_keys_dev ? cap : n_keys, window, sink);
+  if ((int64_t)Hq / Hkv * s > 0x7fffffff || p.pairs > 0x7fffff || p.items * 256 > 0x7fffffffll) return DA_ERR_INVALID_ARG;
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return DA_ERR_WORKSPACE;
+  if (!aligned16(workspace)) return DA_ERR_ALIGNMENT;
+  a.q = q;
+  a.q_b = q_str[0], a.q_h = q_str[1], a.q_s = q_str[2];
+  a.o = out;
+  a.o_b = o_str[0], a.o_h = o_str[1], a.o_s = o_str[2];
+  a.add = addend;
+  if (addend) a.add_b = add_str[0], a.add_h = add_str[1], a.add_s = add_str[2];
+  a.n_dev = n_keys_dev;
+  a.n_step = n_keys_per_seq ? 1 : 0;
+  a.n = n_keys;
+  a.B = B, a.Hkv = Hkv, a.G = Hq / Hkv, a.s = s;
+  a.n_rt = p.n_rt, a.rows = p.rows;
+  a.window = window, a.sink = sink;
+  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.target = p.target;
+  a.part = (float*)workspace;
+  a.pitch = p.pitch;
+  by_type(dtype, D, [&](auto t, auto d) {
+    launch_rows<typename decltype(t)::type, decltype(d)::value>(a, p, (hipStream_t)stream);
+  });
+  return launched();
+}

@@ -64,6 +64,10 @@ EXPORTS = (
     "da_set_sparse_rows_per_wave",
     "da_sparse_rows_per_wave",
     "da_set_bwd_rows_per_chunk",
+    "da_kv8_write",
+    "da_kv8_read",
+    "da_kv8_attn_workspace_bytes",
+    "da_kv8_attn_fwd",
 )
 
 _ERR_TEXT = {
@@ -85,6 +89,7 @@ _lib = None
 _lib_lock = threading.Lock()
 
 I64x3 = ctypes.c_int64 * 3
+I64x8 = ctypes.c_int64 * 8
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -216,6 +221,18 @@ def _load() -> ctypes.CDLL:
                                      _p3, _p3, _p3, _p3, _i, _i, _i, _f,
                                      _i, _i, _i, _i, _i, _i, _d, _d, _d,
                                      _vp, _vp, _vp, _vp, _i, _vp, _sz, _i, _vp, _vp]
+    L.da_kv8_write.restype = _i
+    L.da_kv8_write.argtypes = [_vp, _p3, _vp, _p3, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _p3, _i,
+                               _vp, _i, _i64, _vp, _i, _i, _vp]
+    L.da_kv8_read.restype = _i
+    L.da_kv8_read.argtypes = [_vp, _vp, _vp, _vp, _p3, _i, _i, _i, _i, _i, _i, _vp, _i,
+                              _vp, _p3, _vp, _p3, _i, _vp]
+    L.da_kv8_attn_workspace_bytes.restype = _sz
+    L.da_kv8_attn_workspace_bytes.argtypes = [_i, _i, _i, _i, _i, _i, _i, _i]
+    L.da_kv8_attn_fwd.restype = _i
+    L.da_kv8_attn_fwd.argtypes = [_vp, _p3, _vp, _vp, _vp, _vp, _p3, _i, _vp, _p3,
+                                  _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _f, _vp, _p3,
+                                  _vp, _sz, _i, _vp]
     L.da_build_target.restype = ctypes.c_char_p
     L.da_build_target.argtypes = []
     return L

@@ -11,7 +11,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import functools
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 import torch
 
@@ -587,6 +587,178 @@ def decode_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
                 None if add is None else _s3(add, 0, 1, 2),
                 _ptr(ws), nbytes, _code(q), _stream(dev))
     L.check(rc, "da_decode_attn_fwd" if n_keys is None else "da_decode_attn_fwd_dev")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# the 8-bit key/value cache
+
+KV8_BLOCK = 64    # tokens that share a scale
+
+
+class KV8(NamedTuple):
+    """One layer's 8-bit cache: e4m3 codes and a power-of-two scale for each
+    block of 64 tokens, kv head and tensor; value = code * scale.
+
+    k [B, Hkv, cap, D] and v [B, Hkv, cap / 64, D, 64] (torch.float8_e4m3fn;
+    token 16 t + 4 g + r of a block, t, g, r in 0..3, stands at place
+    16 g + 4 t + r), k_scale / v_scale [B, Hkv, cap / 64] float32. Slices over
+    sequences and heads are caches too. Made by kv8_empty."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+
+
+def kv8_empty(B: int, Hkv: int, max_len: int, D: int, device="cuda") -> KV8:
+    """A cache for max_len tokens per sequence (rounded up to whole blocks)
+    that holds none yet."""
+    assert D in (32, 64, 128, 256), f"unsupported head_dim {D}"
+    assert B >= 0 and Hkv >= 1 and 1 <= max_len <= 1 << 30, (B, Hkv, max_len)
+    nb = -(-int(max_len) // KV8_BLOCK)
+    kw = dict(device=device, dtype=torch.float8_e4m3fn)
+    scale = torch.full((2, B, Hkv, nb), 2.0 ** -117, device=device, dtype=torch.float32)
+    return KV8(torch.empty((B, Hkv, nb * KV8_BLOCK, D), **kw), torch.empty((B, Hkv, nb, D, KV8_BLOCK), **kw),
+               scale[0], scale[1])
+
+
+def _kv8(c: KV8):
+    """Checks a cache's tensors -> (B, Hkv, cap, D, strides of the C ABI)."""
+    k, v, ks, vs = c
+    B, Hkv, cap, D = k.shape
+    nb = cap // KV8_BLOCK
+    assert cap % KV8_BLOCK == 0 and v.shape == (B, Hkv, nb, D, KV8_BLOCK), (k.shape, v.shape)
+    assert ks.shape == (B, Hkv, nb) and vs.shape == ks.shape, (ks.shape, vs.shape, nb)
+    assert k.dtype == v.dtype == torch.float8_e4m3fn and ks.dtype == vs.dtype == torch.float32, (
+        k.dtype, v.dtype, ks.dtype, vs.dtype)
+    a, b, d, e = k.stride(), v.stride(), ks.stride(), vs.stride()
+    assert a[2:] == (D, 1) and b[2:] == (D * KV8_BLOCK, KV8_BLOCK, 1) and d[2] == e[2] == 1, (
+        "a cache's tokens, blocks and scales must be contiguous within a head")
+    return B, Hkv, cap, D, L.I64x8(a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1])
+
+
+def _per_seq(t: torch.Tensor, B: int, dtype: torch.dtype, dev: torch.device, what: str) -> int:
+    """Checks a device tensor of one entry, or one per sequence -> 0 or 1."""
+    assert t.dtype == dtype and t.device == dev and t.dim() <= 1 and t.numel() in (1, B) and t.is_contiguous(), (
+        f"{what}: a contiguous {dtype} tensor of 1 or {B} entries on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
+    return int(t.numel() == B)
+
+
+def kv8_write(cache: KV8, k: torch.Tensor, v: torch.Tensor, pos, *,
+              counts: Optional[torch.Tensor] = None) -> None:
+    """Appends tokens to an 8-bit cache, rounding each block of 64 to e4m3 with
+    one scale per head (da_kv8_write): k/v [B, S, Hkv, D] (projection layout,
+    any batch/seq/head strides), token t of a sequence to its row pos + t.
+
+    pos: an int, or an int64 device tensor of one entry or one per sequence,
+    read when the kernel runs. counts: optional int32 device tensor (one entry
+    or one per sequence), the tokens of each right-padded sequence. Rows behind
+    the written ones keep their bytes but hold nothing any more. With device
+    positions, a sequence whose rows do not fit is left unchanged."""
+    B, Hkv, cap, D, cs = _kv8(cache)
+    assert k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype, (k.shape, v.shape, k.dtype, v.dtype)
+    S = k.shape[1]
+    assert k.shape == (B, S, Hkv, D), (k.shape, (B, S, Hkv, D))
+    dev = _on_gpu(k, v, *cache)
+    code = _code(k)
+    pos_dev = pos_b = counts_b = 0
+    if isinstance(pos, torch.Tensor):
+        pos_b, pos_dev, pos = _per_seq(pos, B, torch.int64, dev, "pos"), pos.data_ptr(), 0
+    else:
+        pos = int(pos)
+        assert 0 <= pos and pos + S <= cap, f"rows {pos} .. {pos + S} do not fit a cache of {cap}"
+    if counts is not None:
+        counts_b = _per_seq(counts, B, torch.int32, dev, "counts")
+    if B == 0 or S == 0:
+        return
+    k, v = _ready(k), _ready(v)
+    with _device(dev):
+        rc = L.lib().da_kv8_write(
+            k.data_ptr(), _s3(k, 0, 1, 2), v.data_ptr(), _s3(v, 0, 1, 2), B, S, Hkv, D,
+            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+            cs, cap, pos_dev or None, pos_b, pos, _ptr(counts), counts_b, code, _stream(dev))
+    L.check(rc, "da_kv8_write")
+
+
+def kv8_read(cache: KV8, start: int, n: int, *, n_keys: Optional[torch.Tensor] = None,
+             dtype: torch.dtype = torch.bfloat16, out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+             ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows start .. start + n - 1 of an 8-bit cache in a 16-bit dtype
+    (da_kv8_read) -> (k, v) [B, Hkv, n, D], exact in bfloat16; finite values
+    beyond float16's largest saturate. n_keys: optional int32 device tensor
+    (one entry or one per sequence); rows at or past it are zero. out: the two
+    tensors to write."""
+    B, Hkv, cap, D, cs = _kv8(cache)
+    start, n = int(start), int(n)
+    assert start >= 0 and n >= 0 and start + n <= cap, f"rows {start} .. {start + n} of a cache of {cap}"
+    dev = _on_gpu(*cache)
+    n_b = 0 if n_keys is None else _per_seq(n_keys, B, torch.int32, dev, "n_keys")
+    if out is None:
+        out = tuple(torch.empty((2, B, Hkv, n, D), device=dev, dtype=dtype))
+    k, v = out
+    assert k.shape == v.shape == (B, Hkv, n, D) and k.dtype == v.dtype and k.device == v.device == dev, (k.shape, v.shape)
+    code = _code(k)
+    if B == 0 or n == 0:
+        return k, v
+    assert k.stride(-1) == 1 and v.stride(-1) == 1
+    with _device(dev):
+        rc = L.lib().da_kv8_read(
+            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cs,
+            cap, B, Hkv, D, start, n, _ptr(n_keys), n_b,
+            k.data_ptr(), _s3(k, 0, 1, 2), v.data_ptr(), _s3(v, 0, 1, 2), code, _stream(dev))
+    L.check(rc, "da_kv8_read")
+    return k, v
+
+
+@functools.lru_cache(maxsize=256)
+def _kv8_ws_bytes(B: int, H: int, Hkv: int, s: int, D: int, n: int, window: int, sink: int) -> int:
+    return int(L.lib().da_kv8_attn_workspace_bytes(B, H, Hkv, s, D, n, window, sink))
+
+
+def kv8_attention(q: torch.Tensor, cache: KV8, *, n_keys, window: int = 0, sink: int = 0,
+                  sm_scale: float, out: Optional[torch.Tensor] = None,
+                  add: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The last s rows of each sequence against its 8-bit cache
+    (da_kv8_attn_fwd): q [B, H, s, D] -> [B, H, s, D]. With n keys, row i
+    stands at n - s + i and sees the keys up to itself: all of them, or with
+    window > 0 the first `sink` and its last `window` (decode_attention's rows,
+    which s = 1 are). Rows before the sequence's start (n < s) are zero.
+
+    n_keys: an int, or an int32 device tensor of one entry or one per sequence,
+    read when the kernels run (a recorded call serves every length; counts are
+    clamped to the capacity). add: a tensor like q; rnd(rnd(row) + add)."""
+    B, Hkv, cap, D, cs = _kv8(cache)
+    assert q.dim() == 4 and q.shape[0] == B and q.shape[3] == D, (q.shape, cache.k.shape)
+    H, s = q.shape[1], q.shape[2]
+    assert H % Hkv == 0 and H > 0, (H, Hkv)
+    dev = _on_gpu(q, *cache)
+    code = _code(q)
+    q = _ready(q)
+    if out is None:
+        out = torch.empty((B, H, s, D), device=dev, dtype=q.dtype)
+    assert out.shape == (B, H, s, D) and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == dev
+    w, sk = max(int(window), 0), max(int(sink), 0)
+    nk_dev, nk_b, n = None, 0, cap
+    if isinstance(n_keys, torch.Tensor):
+        nk_b, nk_dev = _per_seq(n_keys, B, torch.int32, dev, "n_keys"), n_keys.data_ptr()
+    else:
+        n = int(n_keys)
+        assert 0 <= n <= cap, f"{n} keys in a cache of {cap}"
+    if add is not None:
+        assert add.shape == q.shape and add.dtype == q.dtype and add.device == dev
+        add = _ready(add)
+    if B == 0 or s == 0:
+        return out
+    nbytes = _kv8_ws_bytes(B, H, Hkv, s, D, n, min(w, cap), min(sk, cap))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    with _device(dev):
+        rc = L.lib().da_kv8_attn_fwd(
+            q.data_ptr(), _s3(q, 0, 1, 2), cache.k.data_ptr(), cache.v.data_ptr(),
+            cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cs, cap,
+            out.data_ptr(), _s3(out, 0, 1, 2), B, H, Hkv, s, D, nk_dev, nk_b, n, min(w, cap), min(sk, cap),
+            float(sm_scale), _ptr(add), None if add is None else _s3(add, 0, 1, 2),
+            _ptr(ws), nbytes, code, _stream(dev))
+    L.check(rc, "da_kv8_attn_fwd")
     return out
 
 

@@ -260,6 +260,83 @@ int da_decode_attn_fwd_dev_noalloc(const void* q, const void* k, const void* v, 
                                    int dtype, void* stream);
 
 /*
+ * The 8-bit key/value cache. One layer's cache holds e4m3 codes (OCP e4m3fn)
+ * with a power-of-two fp32 scale per block of 64 tokens, kv head and tensor;
+ * value = code * scale:
+ *   k_codes  [B, Hkv, cap, D] bytes (a token's D codes contiguous, tokens D apart)
+ *   v_codes  [B, Hkv, cap / 64, D, 64] bytes (contiguous from the block on): a
+ *            block's 64 tokens stand together for each column, token
+ *            16 t + 4 g + r (t, g, r in 0..3) at place 16 g + 4 t + r
+ *   k_scale, v_scale  [B, Hkv, cap / 64] fp32 (blocks contiguous), 2^e with e in
+ *            [-117, 120]
+ *   c_str    {k batch, k head, v batch, v head (bytes, multiples of 16), k_scale
+ *            batch, head, v_scale batch, head (elements)}
+ *   cap      tokens per sequence, a multiple of 64 up to 2^30.
+ * D is 32, 64, 128 or 256; `dtype` is that of the 16-bit tensors beside the
+ * cache. Rows of a cache that were not written may hold any bytes: they reach no
+ * result. No counterpart in the reference (its cache is the model's dtype).
+ */
+
+/*
+ * Appends to an 8-bit cache: token t of k / v [B, S, Hkv, D] (strides {batch,
+ * seq, head}) goes to row pos + t of its sequence. pos is pos_dev[b] (or
+ * pos_dev[0] for every sequence when pos_per_seq is 0), read when the kernel
+ * runs, or the host's `pos` when pos_dev is NULL. counts_dev (optional; one
+ * entry, or one per sequence): only the first counts tokens (clamped to [0, S])
+ * are written, for right-padded batches.
+ * A block's exponent is the smallest e with |x| <= 448 * 2^e over its finite new
+ * values; a block that also holds rows before pos takes the larger of that and
+ * its present e, and if that grew their codes are rounded to it. Codes are
+ * x / 2^e rounded to nearest even; infinities and NaN become NaN. Rows from
+ * pos + count on keep their bytes; they stand for nothing any more where their
+ * block was written. A sequence whose rows do not fit ([pos, pos + count) not in
+ * [0, cap)) keeps its cache unchanged (DA_ERR_INVALID_ARG for a host pos).
+ */
+int da_kv8_write(const void* k, const int64_t k_str[3], const void* v, const int64_t v_str[3],
+                 int B, int S, int Hkv, int D,
+                 void* k_codes, void* v_codes, float* k_scale, float* v_scale,
+                 const int64_t c_str[8], int cap,
+                 const int64_t* pos_dev, int pos_per_seq, int64_t pos,
+                 const int32_t* counts_dev, int counts_per_seq, int dtype, void* stream);
+
+/*
+ * Rows start .. start + n - 1 of an 8-bit cache in `dtype`: k_out / v_out
+ * [B, Hkv, n, D] (strides {batch, head, row}) = code * scale, one rounding
+ * (exact in bf16), finite values beyond the type's largest one saturated. With
+ * n_keys_dev (int32, one entry or one per sequence) rows at or past a sequence's
+ * count are zero.
+ */
+int da_kv8_read(const void* k_codes, const void* v_codes, const float* k_scale,
+                const float* v_scale, const int64_t c_str[8], int cap,
+                int B, int Hkv, int D, int start, int n,
+                const int32_t* n_keys_dev, int n_keys_per_seq,
+                void* k_out, const int64_t ko_str[3], void* v_out, const int64_t vo_str[3],
+                int dtype, void* stream);
+
+/*
+ * Attention of the last s rows of each sequence over its 8-bit cache: with n
+ * keys, row i of q [B, Hq, s, D] (strides {batch, head, row}) stands at r = n - s
+ * + i and sees the keys j <= r, with window > 0 only those with j < sink or
+ * j > r - window (the decode rows of da_decode_attn_fwd, window 0: every key).
+ * out [B, Hq, s, D] = softmax(sm_scale q k) v in fp32, rounded once; rows that
+ * see no key (r < 0) are zero. addend (optional, like q): out = rnd(rnd(row) +
+ * addend). n is n_keys_dev[b] (or n_keys_dev[0] when n_keys_per_seq is 0) read
+ * when the kernels run and clamped to [0, cap], or the host's n_keys.
+ * Workspace: da_kv8_attn_workspace_bytes(..., max_keys = cap with a device
+ * count, else n_keys) bytes, which may be 0.
+ */
+size_t da_kv8_attn_workspace_bytes(int B, int Hq, int Hkv, int s, int D, int max_keys,
+                                   int window, int sink);
+int da_kv8_attn_fwd(const void* q, const int64_t q_str[3], const void* k_codes,
+                    const void* v_codes, const float* k_scale, const float* v_scale,
+                    const int64_t c_str[8], int cap, void* out, const int64_t o_str[3],
+                    int B, int Hq, int Hkv, int s, int D,
+                    const int32_t* n_keys_dev, int n_keys_per_seq, int n_keys,
+                    int window, int sink, float sm_scale,
+                    const void* addend, const int64_t add_str[3],
+                    void* workspace, size_t workspace_bytes, int dtype, void* stream);
+
+/*
  * Kernel (3): delta broadcast-add over rows 0 .. s_p-1.
  * Replaces the torch broadcast at delta_attention/llama.py:740-755 (uniform
  * stride) and delta_attention/stride.py:26-40 (`apply_delta_variable`).

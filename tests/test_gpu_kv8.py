@@ -1,0 +1,435 @@
+"""GPU parity of the 8-bit key/value cache (ops.kv8_write / kv8_read /
+kv8_attention) with the float64 oracle: codes and scales bit for bit, read rows
+bit for bit, attention rows within the bound of kv8_helpers.tolerance."""
+
+import numpy as np
+import pytest
+import torch
+
+from helpers import np64
+from kv8_helpers import place, same, to_oracle, tolerance
+from oracle import kv8_oracle as K8
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def tokens(B, S, Hkv, D, dtype, seed, spread=True):
+    """Tokens whose magnitude varies over heads and rows (so do the scales)."""
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(B, S, Hkv, D, generator=g)
+    if spread:
+        x = x * torch.exp2(torch.randint(-6, 7, (B, S, Hkv, 1), generator=g).float())
+    return x.to(dtype).cuda()
+
+
+def garbage(c, seed):
+    """Every byte and scale of a new cache set to noise, NaN codes among them."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    for t in (c.k, c.v):
+        t.view(torch.uint8).random_(0, 256, generator=g)
+    for t in (c.k_scale, c.v_scale):
+        t.copy_(torch.exp2(torch.randint(-100, 100, t.shape, device="cuda", generator=g).float()))
+    return c
+
+
+def check_cache(c, ref, live):
+    """Codes and scales of the first live[b] rows equal the oracle's."""
+    got = to_oracle(c)
+    for b, n in enumerate(live):
+        nb = -(-n // 64)
+        for x in ("k", "v"):
+            assert same(got[x][b, :, :n], ref[x][b, :, :n]), (b, x)
+        for x in ("ke", "ve"):
+            assert np.array_equal(got[x][b, :, :nb], ref[x][b, :, :nb]), (b, x)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,Hkv,D,cap,pos,S", [
+    (1, 1, 128, 64, 0, 64),        # one whole block
+    (1, 2, 128, 128, 0, 1),        # the first token
+    (2, 3, 64, 256, 0, 130),       # whole blocks and a part
+    (1, 2, 32, 320, 5, 200),       # from inside a block
+    (2, 2, 256, 192, 63, 66),      # the last row of a block, one of the next but one
+    (1, 8, 128, 1024, 127, 777),
+])
+def test_write_codes_and_scales(gpu, B, Hkv, D, cap, pos, S, dtype):
+    from delta_attention import ops
+    c = garbage(ops.kv8_empty(B, Hkv, cap, D), 1)
+    ref = K8.new_cache(B, Hkv, cap, D)
+    if pos:
+        k0, v0 = (tokens(B, pos, Hkv, D, DT[dtype], s) for s in (2, 3))
+        ops.kv8_write(c, k0, v0, 0)
+        K8.write(ref, np64(k0), np64(v0), [0] * B)
+    k, v = (tokens(B, S, Hkv, D, DT[dtype], s) for s in (4, 5))
+    before = to_oracle_bytes(c)
+    ops.kv8_write(c, k, v, pos)
+    torch.cuda.synchronize()
+    K8.write(ref, np64(k), np64(v), [pos] * B)
+    check_cache(c, ref, [pos + S] * B)
+    # rows behind the last one keep their bytes, blocks behind it their scales
+    after = to_oracle_bytes(c)
+    end = pos + S
+    assert np.array_equal(after[0][:, :, end:], before[0][:, :, end:])
+    assert np.array_equal(after[1][:, :, end:], before[1][:, :, end:])
+    nb = -(-end // 64)
+    for x, y in zip(after[2:], before[2:]):
+        assert np.array_equal(x[:, :, nb:], y[:, :, nb:])
+
+
+def to_oracle_bytes(c):
+    """Raw bytes in token order, and the scales."""
+    B, Hkv, cap, D = c.k.shape
+    v = c.v.view(torch.uint8).cpu().numpy()[..., place()].transpose(0, 1, 2, 4, 3).reshape(B, Hkv, cap, D)
+    return c.k.view(torch.uint8).cpu().numpy(), v, c.k_scale.cpu().numpy(), c.v_scale.cpu().numpy()
+
+
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_write_token_by_token(gpu, D):
+    """Tokens appended one at a time, each larger than the last by up to 2^12:
+    a block's earlier codes move to its larger scales, into the subnormals."""
+    from delta_attention import ops
+    B, Hkv, cap = 2, 2, 128
+    c, ref = garbage(ops.kv8_empty(B, Hkv, cap, D), 7), K8.new_cache(B, Hkv, cap, D)
+    for i in range(70):
+        k, v = (tokens(B, 1, Hkv, D, torch.bfloat16, 100 + 2 * i + s, False) * 2.0 ** ((i * 5) % 13) for s in (0, 1))
+        pos = torch.tensor([i, i + 3], device="cuda") if i else torch.zeros(2, dtype=torch.int64, device="cuda")
+        if i == 1:    # the second sequence stands three rows further from here on
+            k3, v3 = (tokens(1, 3, Hkv, D, torch.bfloat16, s) for s in (8, 9))
+            ops.kv8_write(ops.KV8(*(t[1:] for t in c)), k3, v3, 1)
+            one = {x: y[1:] for x, y in ref.items()}
+            K8.write(one, np64(k3), np64(v3), [1])
+        ops.kv8_write(c, k, v, pos)
+        K8.write(ref, np64(k), np64(v), pos.tolist())
+    check_cache(c, ref, [70, 73])
+
+
+def test_write_special_values(gpu):
+    """Zeros, the type's extremes and subnormals, infinities and NaN: the scale
+    comes from the finite values, what has no code becomes NaN, and no other
+    block or value is touched by it."""
+    from delta_attention import ops
+    for dtype in (torch.bfloat16, torch.float16):
+        fi = torch.finfo(dtype)
+        x = torch.zeros(1, 64 * 8, 1, 128, dtype=dtype)
+        x[0, 64:128] = fi.max                                            # the largest
+        x[0, 128:192] = fi.tiny * fi.eps                                 # the smallest subnormal
+        x[0, 192:256] = torch.randn(64, 1, 128) * fi.tiny                # around the normal range's end
+        x[0, 256:320] = torch.randn(64, 1, 128)
+        x[0, 256, 0, :5] = torch.tensor([float("inf"), -float("inf"), float("nan"), -0.0, 447.9])
+        x[0, 320:384] = float("inf")                                     # nothing finite
+        x[0, 384:448] = torch.linspace(-448, 448, 64 * 128).view(64, 1, 128)
+        x[0, 448:] = 2.0 ** (torch.arange(64 * 128) % 30 - 20).float().view(64, 1, 128)
+        x = x.cuda()
+        c, ref = ops.kv8_empty(1, 1, 512, 128), K8.new_cache(1, 1, 512, 128)
+        ops.kv8_write(c, x, -x, 0)
+        K8.write(ref, np64(x), np64(-x), [0])
+        check_cache(c, ref, [512])
+        # one more inside a block of moderate values: only the finite ones move the scale
+        y = torch.full((1, 1, 1, 128), float("nan"), dtype=dtype, device="cuda")
+        y[..., 3] = 1e4
+        ops.kv8_write(c, y, y, 300)
+        K8.write(ref, np64(y), np64(y), [300])
+        check_cache(c, ref, [301])
+
+
+def test_write_padded_and_refused_rows(gpu):
+    """Counts per sequence (clamped to [0, S]); device positions whose rows do
+    not fit leave their sequence unchanged."""
+    from delta_attention import ops
+    B, Hkv, D, cap, S = 6, 2, 64, 256, 90
+    c = garbage(ops.kv8_empty(B, Hkv, cap, D), 3)
+    before = [t.clone() for t in c]
+    k, v = (tokens(B, S, Hkv, D, torch.float16, s) for s in (1, 2))
+    pos = torch.tensor([0, 64, 0, 192, -1, 166], device="cuda")
+    counts = torch.tensor([90, 33, -5, 70, 4, 1000], dtype=torch.int32, device="cuda")
+    ops.kv8_write(c, k, v, pos, counts=counts)
+    ref = K8.new_cache(B, Hkv, cap, D)
+    K8.write(ref, np64(k), np64(v), pos.tolist(), counts.tolist())
+    got = to_oracle(c)
+    for b, (a, n) in enumerate(((0, 90), (64, 33), (166, 90))):
+        b = (0, 1, 5)[b]
+        if b == 5:     # its first block already held rows: their (noise) scale may stay the larger
+            continue
+        for x in ("k", "v"):
+            assert same(got[x][b, :, a:a + n], ref[x][b, :, a:a + n])
+    for b in (2, 3, 4):
+        for t, u in zip(c, before):
+            assert torch.equal(t[b].view(torch.uint8), u[b].view(torch.uint8)), b
+    # one position and one count for all
+    c2, c3 = ops.kv8_empty(B, Hkv, cap, D), ops.kv8_empty(B, Hkv, cap, D)
+    ops.kv8_write(c2, k, v, torch.tensor([7], device="cuda"), counts=torch.tensor([50], dtype=torch.int32, device="cuda"))
+    ops.kv8_write(c3, k[:, :50], v[:, :50], 7)
+    for x in ("k", "v"):
+        assert same(to_oracle(c2)[x][:, :, 7:57], to_oracle(c3)[x][:, :, 7:57])
+
+
+def test_write_strides(gpu):
+    """Strided tokens (views of one fused projection), and a cache that is a
+    slice of a larger one over sequences and heads."""
+    from delta_attention import ops
+    B, S, Hkv, D = 2, 100, 2, 64
+    big = tokens(B, S, 7, D, torch.bfloat16, 4)
+    k, v = big[:, :, 2:4], big[:, :, 4:6]
+    whole = garbage(ops.kv8_empty(5, 6, 128, D), 5)
+    keep = [t.clone() for t in whole]
+    part = ops.KV8(*(t[1:5:2, 3:5] for t in whole))
+    ops.kv8_write(part, k, v, 9)
+    kk, vv = ops.kv8_read(part, 64, 45)                      # a block written whole: no noise in its scale
+    o = K8.new_cache(B, Hkv, 128, D)
+    K8.write(o, np64(k), np64(v), [9] * B)
+    ok, ov = K8.values(o, 64, 45)
+    assert same(np64(kk), ok) and same(np64(vv), ov)
+    for t, u in zip(whole, keep):
+        for b in range(5):
+            for h in range(6):
+                if b not in (1, 3) or h not in (3, 4):
+                    assert torch.equal(t[b, h].view(torch.uint8), u[b, h].view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,Hkv,D,cap,start,n", [
+    (1, 1, 128, 64, 0, 64), (1, 2, 64, 192, 1, 1), (2, 2, 32, 256, 63, 130), (1, 3, 256, 320, 100, 217),
+    (1, 8, 128, 2048, 5, 2043),
+])
+def test_read(gpu, B, Hkv, D, cap, start, n, dtype):
+    from delta_attention import ops
+    c, ref = ops.kv8_empty(B, Hkv, cap, D), K8.new_cache(B, Hkv, cap, D)
+    k, v = (tokens(B, cap, Hkv, D, torch.bfloat16, s) for s in (1, 2))
+    k[0, min(70, cap - 1), 0, 3] = float("nan")
+    k[:, : cap // 2] *= 2.0 ** 10                     # past float16's largest for some
+    v[:, : cap // 2] *= 2.0 ** -14                    # into float16's subnormals
+    ops.kv8_write(c, k, v, 0)
+    K8.write(ref, np64(k), np64(v), [0] * B)
+    want = []
+    for x in K8.values(ref, start, n):
+        top = float(torch.finfo(DT[dtype]).max)
+        want.append(torch.from_numpy(np.clip(x, -top, top)).to(DT[dtype]))
+    got = ops.kv8_read(c, start, n, dtype=DT[dtype])
+    for x, y in zip(got, want):
+        assert x.shape == (B, Hkv, n, D) and same(np64(x), np64(y))
+    # rows behind each sequence's end are zero; strided outputs keep their other rows
+    live = torch.tensor([start + n // 2 + b for b in range(B)], dtype=torch.int32, device="cuda")
+    buf = torch.full((2, B, n + 3, Hkv, D), 7.0, dtype=DT[dtype], device="cuda")
+    out = tuple(buf[i, :, 2:n + 2].transpose(1, 2) for i in (0, 1))
+    ops.kv8_read(c, start, n, n_keys=live, out=out)
+    for x, y in zip(out, want):
+        y = np64(y)
+        for b in range(B):
+            y[b, :, max(int(live[b]) - start, 0):] = 0
+        assert same(np64(x), y)
+    assert (buf[:, :, :2] == 7).all() and (buf[:, :, n + 2:] == 7).all()
+
+
+def filled(B, Hkv, cap, D, n, dtype, seed, scale=1.0):
+    """A cache of noise with n[b] tokens of N(0, 1) times a varying factor."""
+    from delta_attention import ops
+    c, ref = garbage(ops.kv8_empty(B, Hkv, cap, D), seed), K8.new_cache(B, Hkv, cap, D)
+    g = torch.Generator().manual_seed(seed + 1)
+    k, v = ((torch.randn(B, max(max(n), 1), Hkv, D, generator=g)
+             * torch.exp2(torch.randint(-1, 2, (B, 1, Hkv, 1), generator=g).float()) * scale).to(dtype).cuda() for _ in (0, 1))
+    counts = torch.tensor(n, dtype=torch.int32, device="cuda")
+    ops.kv8_write(c, k, v, 0, counts=counts)
+    K8.write(ref, np64(k), np64(v), [0] * B, n)
+    return c, ref, counts
+
+
+def check_rows(got, q, ref, n, window, sink, scale, add=None, what=""):
+    kk, vv = K8.values(ref)
+    want, spread = K8.rows(np64(q), kk, vv, n, window, sink, scale)
+    a = None if add is None else np64(add)
+    tol = tolerance(want, spread, q.shape[3], max(max(n), 1), q.dtype, a)
+    if a is not None:
+        want = want + a
+    d = np.abs(np64(got) - want)
+    worst = float((d / tol).max())
+    print(f"{what}: worst {worst:.3f} of the bound", flush=True)
+    assert np.isfinite(np64(got)).all() and worst <= 1.0, (what, worst)
+
+
+ROWS = [
+    # B, Hkv, G, D, cap, n, s, window, sink
+    (1, 1, 1, 128, 64, [1], 1, 0, 0),
+    (1, 2, 4, 128, 64, [64], 1, 0, 0),
+    (1, 2, 4, 128, 128, [65], 1, 0, 0),
+    (2, 2, 4, 64, 1024, [1000, 3], 1, 0, 0),
+    (3, 1, 5, 128, 2048, [0, 1, 2047], 1, 0, 0),              # an empty sequence
+    (1, 2, 4, 128, 4096, [4001], 1, 512, 64),                 # sinks and a window
+    (2, 2, 2, 32, 1024, [1021, 300], 1, 100, 7),
+    (1, 1, 8, 256, 1024, [999], 1, 0, 0),
+    (1, 2, 1, 256, 1024, [999], 1, 333, 20),
+    (2, 2, 4, 128, 512, [500, 2], 6, 0, 0),                   # more rows than keys in one
+    (1, 2, 4, 64, 2048, [2000], 5, 200, 33),
+    (1, 1, 8, 128, 512, [400], 4, 0, 0),                      # 32 rows
+    (1, 1, 12, 64, 512, [400], 5, 130, 3),                    # 60 rows
+    (1, 2, 4, 256, 512, [300], 7, 0, 0),                      # 28 rows, head_dim 256
+    (1, 1, 4, 128, 512, [290], 100, 0, 0),                    # 400 rows: several row tiles
+    (1, 1, 8, 256, 256, [200], 9, 64, 10),                    # 72 rows, head_dim 256
+    (70, 1, 2, 32, 128, [(i * 37) % 129 for i in range(70)], 1, 0, 0),   # more sequences than lanes
+    (1, 1, 4, 128, 20480, [20001], 1, 0, 0),                  # a long one: many splits
+    (2, 1, 20, 128, 8192, [8192, 100], 1, 1000, 5000),        # sinks past the window's start
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("B,Hkv,G,D,cap,n,s,window,sink", ROWS)
+def test_rows(gpu, B, Hkv, G, D, cap, n, s, window, sink, dtype):
+    from delta_attention import ops
+    c, ref, counts = filled(B, Hkv, cap, D, n, DT[dtype], 17 * B + cap + s)
+    q = tokens(B, s, Hkv * G, D, DT[dtype], 5, False).transpose(1, 2)
+    scale = D ** -0.5
+    got = ops.kv8_attention(q, c, n_keys=counts, window=window, sink=sink, sm_scale=scale)
+    assert got.shape == q.shape and got.dtype == q.dtype
+    what = f"B{B} H{Hkv * G}/{Hkv} D{D} n{n[:3]} s{s} w{window} k{sink} {dtype}"
+    check_rows(got, q, ref, n, window, sink, scale, what=what)
+    add = tokens(B, s, Hkv * G, D, DT[dtype], 6, False).transpose(1, 2)
+    got = ops.kv8_attention(q, c, n_keys=counts, window=window, sink=sink, sm_scale=scale, add=add)
+    check_rows(got, q, ref, n, window, sink, scale, add, what=what + " add")
+    if len(set(n)) == 1:     # the host's count
+        got = ops.kv8_attention(q, c, n_keys=n[0], window=window, sink=sink, sm_scale=scale)
+        check_rows(got, q, ref, n, window, sink, scale, what=what + " host count")
+
+
+def test_rows_large_scores(gpu):
+    """Scores from -300 to 300 with the largest late: the running reference
+    moves up many times, and rows end with one key's value."""
+    from delta_attention import ops
+    B, Hkv, G, D, n = 1, 1, 4, 128, 1500
+    c, ref, counts = filled(B, Hkv, 1536, D, [n], torch.float16, 3, scale=3.0)
+    q = tokens(B, 1, G, D, torch.float16, 5, False).transpose(1, 2) * 8
+    got = ops.kv8_attention(q, c, n_keys=counts, sm_scale=1.0)
+    check_rows(got, q, ref, [n], 0, 0, 1.0, what="large scores")
+
+
+def test_rows_nan_in_masked_places(gpu):
+    """NaN keys and values that a row does not see (behind the last key, before
+    its window, of later rows) do not reach it; the rows that see one are NaN
+    in its columns."""
+    from delta_attention import ops
+    B, Hkv, G, D, cap, n, s, window, sink = 1, 1, 2, 64, 512, 300, 4, 70, 5
+    for at, tensor in ((298, "v"), (229, "v"), (100, "v"), (3, "v"), (6, "v"), (298, "k"), (150, "k")):
+        k, v = (tokens(B, n, Hkv, D, torch.bfloat16, x, False) for x in (1, 2))
+        (k if tensor == "k" else v)[0, at, 0, 9] = float("nan")
+        c = garbage(ops.kv8_empty(B, Hkv, cap, D), at)
+        ops.kv8_write(c, k, v, 0)
+        q = tokens(B, s, G, D, torch.bfloat16, 3, False).transpose(1, 2)
+        got = np64(ops.kv8_attention(q, c, n_keys=n, window=window, sink=sink, sm_scale=0.125))
+        for i in range(s):
+            r = n - s + i
+            sees = at <= r and (at < sink or at > r - window)
+            bad = np.isnan(got[0, :, i])
+            want = np.zeros_like(bad)
+            if sees and tensor == "k":
+                want[:] = True
+            elif sees:
+                want[:, 9] = True
+            assert np.array_equal(bad, want), (at, tensor, i)
+
+
+def test_rows_strides_and_outputs(gpu):
+    """Strided queries and outputs (other rows kept), a sliced cache."""
+    from delta_attention import ops
+    B, Hkv, G, D, n = 2, 2, 3, 64, [200, 131]
+    c, ref, counts = filled(B, Hkv, 256, D, n, torch.bfloat16, 8)
+    big = tokens(B, 3, 2 * Hkv * G, D, torch.bfloat16, 9, False)
+    q = big[:, 1:3, Hkv * G:].transpose(1, 2)
+    buf = torch.full((B, 4, Hkv * G, D), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = buf[:, 1:3].transpose(1, 2)
+    got = ops.kv8_attention(q, c, n_keys=counts, sm_scale=0.1, out=out)
+    assert got is out
+    check_rows(out, q, ref, n, 0, 0, 0.1, what="strided")
+    assert (buf[:, 0] == 7).all() and (buf[:, 3] == 7).all()
+    part = ops.KV8(*(t[:, 1:] for t in c))
+    one = ops.kv8_attention(q[:, G:], part, n_keys=counts, sm_scale=0.1)
+    check_rows(one, q[:, G:], {x: y[:, 1:] for x, y in ref.items()}, n, 0, 0, 0.1, what="one head's cache")
+
+
+def test_rows_repeat_and_streams(gpu):
+    """The same call twice, on another stream and beside another call gives the
+    same bits."""
+    from delta_attention import ops
+    c, ref, counts = filled(2, 2, 4096, 128, [4001, 977], torch.bfloat16, 21)
+    q = tokens(2, 1, 8, 128, torch.bfloat16, 22, False).transpose(1, 2)
+    call = lambda: ops.kv8_attention(q, c, n_keys=counts, sm_scale=0.09)
+    a = call()
+    torch.cuda.synchronize()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(s1):
+        b = [call() for _ in range(3)]
+    with torch.cuda.stream(s2):
+        d = [call() for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, x) for x in b + d)
+
+
+def test_append_and_rows_in_a_graph(gpu):
+    """A decode step (append one token per sequence, attend) recorded once and
+    replayed while positions and counts advance on the device, against the
+    same steps run eagerly on a second cache: every replay's bits."""
+    from delta_attention import ops
+    B, Hkv, G, D, cap = 2, 2, 4, 128, 320
+    n0 = [62, 130]
+    caches = [filled(B, Hkv, cap, D, n0, torch.bfloat16, 31)[0] for _ in (0, 1)]
+    src = [tokens(B, 80, Hkv, D, torch.bfloat16, s) for s in (1, 2)]
+    qs = tokens(B, 80, Hkv * G, D, torch.bfloat16, 3, False)
+    k, v = (torch.empty(B, 1, Hkv, D, dtype=torch.bfloat16, device="cuda") for _ in (0, 1))
+    q = torch.empty(B, Hkv * G, 1, D, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty_like(q)
+
+    def step(c, pos, counts):
+        ops.kv8_write(c, k, v, pos)
+        ops.kv8_attention(q, c, n_keys=counts, window=100, sink=9, sm_scale=0.09, out=out)
+        pos.add_(1)
+        counts.add_(1)
+
+    def load(i):
+        k.copy_(src[0][:, i:i + 1])
+        v.copy_(src[1][:, i:i + 1])
+        q.copy_(qs[:, i:i + 1].transpose(1, 2))
+
+    pos = [torch.tensor(n0, device="cuda") for _ in (0, 1)]
+    cnt = [(p + 1).to(torch.int32) for p in pos]
+    load(0)
+    for j in (0, 1):
+        step(caches[j], pos[j], cnt[j])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(caches[0], pos[0], cnt[0])
+    for i in range(1, 80):
+        load(i)
+        g.replay()
+        got = out.clone()
+        step(caches[1], pos[1], cnt[1])
+        assert torch.equal(got, out), i
+    # both sequences' last rows against the rows recomputed from the whole history
+    for a, b in zip(to_oracle(caches[0]).values(), to_oracle(caches[1]).values()):
+        assert same(a, b)
+
+
+def test_prompt_chunk_token_run(gpu):
+    """Used together: a padded prompt, a chunk behind it, tokens one by one, rows
+    after each; the read-back through the framework's rows kernel agrees with the
+    cache's own rows."""
+    from delta_attention import ops
+    from delta_attention.delta_kernel import attention as rows_attention
+    B, Hkv, G, D, cap = 2, 2, 4, 128, 512
+    c, ref = ops.kv8_empty(B, Hkv, cap, D), K8.new_cache(B, Hkv, cap, D)
+    n = [0, 0]
+    scale = D ** -0.5
+    for step, (S, cnt) in enumerate([(200, [200, 151]), (70, [70, 70]), (1, [1, 1]), (1, [1, 1])]):
+        k, v = (tokens(B, S, Hkv, D, torch.bfloat16, 50 + 2 * step + s, False) for s in (0, 1))
+        ops.kv8_write(c, k, v, torch.tensor(n, device="cuda"),
+                      counts=torch.tensor(cnt, dtype=torch.int32, device="cuda"))
+        K8.write(ref, np64(k), np64(v), n, cnt)
+        n = [a + b for a, b in zip(n, cnt)]
+        check_cache(c, ref, n)
+        q = tokens(B, 3, Hkv * G, D, torch.bfloat16, 60 + step, False).transpose(1, 2)
+        got = ops.kv8_attention(q, c, n_keys=torch.tensor(n, dtype=torch.int32, device="cuda"), sm_scale=scale)
+        check_rows(got, q, ref, n, 0, 0, scale, what=f"step {step}")
+    for b in range(B):
+        one = ops.KV8(*(t[b:b + 1] for t in c))
+        kk, vv = ops.kv8_read(one, 0, n[b])
+        mask = torch.arange(n[b] - 3, n[b], device="cuda")[None]
+        rows = rows_attention(q[b:b + 1].contiguous(), kk, vv, mask, scale)
+        assert (rows.float() - got[b:b + 1].float()).abs().max().item() < 2e-2

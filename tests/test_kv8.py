@@ -1,0 +1,176 @@
+"""CPU checks of the 8-bit key/value cache: its oracle against torch's e4m3
+casts, its argument checks at the C entry points and in ops, its layout."""
+
+import ctypes
+import os
+
+import numpy as np
+import pytest
+import torch
+
+import conftest  # noqa: F401  (paths)
+from delta_attention import _lib as L
+from delta_attention import ops
+from kv8_helpers import place, same
+from oracle import kv8_oracle as K8
+
+
+@pytest.fixture(scope="module")
+def lib():
+    if not os.path.exists(L.LIB_PATH):
+        import build_lib
+        build_lib.build()
+    return L.lib()
+
+
+def test_oracle_rounding_is_torchs():
+    x = torch.cat([torch.randn(20000) * 2.0 ** s for s in (-12, -8, -4, 0, 4, 6)]).clamp(-448, 448)
+    x = torch.cat([x, torch.tensor([0.0, 448.0, 2.0 ** -9, 2.0 ** -10, 3 * 2.0 ** -10, 17.0, 19.0, 0.017578125])])
+    assert same(K8.round_e4m3(x.numpy()), x.to(torch.float8_e4m3fn).double().numpy())
+    assert np.isnan(K8.round_e4m3([np.nan, np.inf, -np.inf])).all()
+
+
+def test_oracle_exponent():
+    for e in (-117, -30, 0, 7, 120):
+        assert K8.block_exponent(np.array([np.ldexp(448.0, e), np.inf, np.nan])) == e
+        if e < 120:
+            assert K8.block_exponent(np.array([np.ldexp(448.0, e) * (1 + 2.0 ** -40)])) == e + 1
+    assert K8.block_exponent(np.zeros(3)) == K8.block_exponent(np.array([np.nan])) == K8.E_MIN
+    assert K8.block_exponent(np.array([float(torch.finfo(torch.bfloat16).max)])) == K8.E_MAX
+
+
+def test_oracle_growth_is_one_rounding_in_the_normal_range():
+    """Codes that move to a larger power of two keep their values, but for
+    those that become subnormal."""
+    rng = np.random.default_rng(0)
+    B, D = 1, 4
+    c = K8.new_cache(B, 1, 64, D)
+    x = rng.standard_normal((1, 8, 1, D))
+    K8.write(c, x, x, [0])
+    before, _ = K8.values(c, 0, 8)
+    y = np.full((1, 1, 1, D), 100.0)
+    K8.write(c, y, y, [8])
+    after, _ = K8.values(c, 0, 9)
+    scale = 2.0 ** int(c["ke"][0, 0, 0])
+    normal = np.abs(before) >= scale * 2.0 ** -6
+    assert normal.any() and np.array_equal(after[:, :, :8][normal], before[normal])
+    assert np.abs(after[:, :, :8] - before).max() <= scale * 2.0 ** -10
+    assert np.abs(after[0, 0, 8] - 100.0).max() <= 100 * 2.0 ** -4
+
+
+def test_place_is_a_permutation_of_a_block():
+    p = place()
+    assert sorted(p) == list(range(64)) and p[0] == 0 and p[1] == 1 and p[4] == 16 and p[16] == 4 and p[63] == 63
+
+
+def test_empty_cache_and_its_slices():
+    c = ops.kv8_empty(2, 3, 100, 64, "cpu")
+    assert c.k.shape == (2, 3, 128, 64) and c.v.shape == (2, 3, 2, 64, 64)
+    assert c.k_scale.shape == c.v_scale.shape == (2, 3, 2) and (c.k_scale == 2.0 ** -117).all()
+    B, H, cap, D, st = ops._kv8(c)
+    assert (B, H, cap, D) == (2, 3, 128, 64) and list(st)[:2] == [3 * 128 * 64, 128 * 64]
+    part = ops.KV8(*(t[:, 1:] for t in c))
+    assert ops._kv8(part)[:4] == (2, 2, 128, 64)
+    for bad in (dict(D=96), dict(max_len=0), dict(max_len=(1 << 30) + 1), dict(Hkv=0)):
+        with pytest.raises(AssertionError):
+            ops.kv8_empty(**{**dict(B=1, Hkv=1, max_len=64, D=64, device="cpu"), **bad})
+
+
+def test_ops_refuse_caches_that_are_not_laid_out_so():
+    c = ops.kv8_empty(1, 2, 128, 64, "cpu")
+    for bad in (c._replace(k=c.k[:, :, ::2]), c._replace(k=c.k[:, :, :100]), c._replace(v=c.v[:, :, :1]),
+                c._replace(v=c.v.transpose(3, 4)), c._replace(k_scale=c.k_scale[..., :1]),
+                c._replace(k=c.k.view(torch.uint8)), c._replace(v_scale=c.v_scale.double()),
+                c._replace(k_scale=c.k_scale[..., 0:1].expand(1, 2, 2))):
+        with pytest.raises(AssertionError):
+            ops._kv8(bad)
+
+
+def test_ops_refuse_arguments_on_the_cpu():
+    c = ops.kv8_empty(1, 2, 128, 64, "cpu")
+    k = torch.zeros(1, 3, 2, 64, dtype=torch.bfloat16)
+    q = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError, match="GPU tensors"):
+        ops.kv8_write(c, k, k, 0)
+    with pytest.raises(AssertionError):
+        ops.kv8_write(c, k[..., :32], k[..., :32], 0)
+    with pytest.raises(AssertionError):
+        ops.kv8_write(c, k, k.half(), 0)
+    with pytest.raises(AssertionError, match="GPU tensors"):
+        ops.kv8_attention(q, c, n_keys=1, sm_scale=1.0)
+    with pytest.raises(AssertionError):
+        ops.kv8_attention(q[:, :3], c, n_keys=1, sm_scale=1.0)
+    with pytest.raises(AssertionError):
+        ops.kv8_read(c, 100, 29)
+
+
+def _write(lib, **kw):
+    a = dict(k=16, v=16, ks=(3 * 128, 128, 64), vs=(3 * 128, 128, 64), B=1, S=3, Hkv=2, D=64, kc=16, vc=16,
+             sk=16, sv=16, cs=(128 * 128, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2), cap=128, pos=0, pos_dev=0,
+             counts=0, dtype=L.DA_BF16)
+    a.update(kw)
+    p = ctypes.c_void_p
+    return lib.da_kv8_write(p(a["k"]), L.strides3(*a["ks"]), p(a["v"]), L.strides3(*a["vs"]), a["B"], a["S"],
+                            a["Hkv"], a["D"], p(a["kc"]), p(a["vc"]), p(a["sk"]), p(a["sv"]), L.I64x8(*a["cs"]),
+                            a["cap"], p(a["pos_dev"]), 0, a["pos"], p(a["counts"]), 0, a["dtype"], None)
+
+
+def test_c_write_refusals(lib):
+    assert _write(lib, dtype=5) == L.DA_ERR_DTYPE
+    assert _write(lib, D=96) == L.DA_ERR_HEAD_DIM
+    for bad in (dict(cap=100), dict(cap=-64), dict(cap=(1 << 30) + 64), dict(Hkv=0), dict(B=-1), dict(S=-1),
+                dict(k=0), dict(v=0), dict(kc=0), dict(vc=0), dict(sk=0), dict(sv=0), dict(pos=-1), dict(pos=126),
+                dict(S=129), dict(pos=2 ** 62)):
+        assert _write(lib, **bad) == L.DA_ERR_INVALID_ARG, bad
+    for bad in (dict(k=24), dict(vc=24), dict(sk=18), dict(ks=(3 * 128, 129, 64)), dict(pos_dev=20), dict(counts=18),
+                dict(cs=(128 * 128 + 8, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2))):
+        assert _write(lib, **bad) == L.DA_ERR_ALIGNMENT, bad
+    assert _write(lib, S=0) == L.DA_OK and _write(lib, B=0) == L.DA_OK       # nothing launched
+
+
+def test_c_read_refusals(lib):
+    def call(**kw):
+        a = dict(kc=16, vc=16, sk=16, sv=16, cap=128, B=1, Hkv=2, D=64, start=0, n=5, nk=0, ko=16, vo=16,
+                 st=(2 * 5 * 64, 5 * 64, 64), dtype=L.DA_FP16)
+        a.update(kw)
+        p = ctypes.c_void_p
+        return lib.da_kv8_read(p(a["kc"]), p(a["vc"]), p(a["sk"]), p(a["sv"]),
+                               L.I64x8(128 * 128, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2), a["cap"], a["B"],
+                               a["Hkv"], a["D"], a["start"], a["n"], p(a["nk"]), 0, p(a["ko"]),
+                               L.strides3(*a["st"]), p(a["vo"]), L.strides3(*a["st"]), a["dtype"], None)
+    assert call(dtype=2) == L.DA_ERR_DTYPE and call(D=48) == L.DA_ERR_HEAD_DIM
+    for bad in (dict(start=-1), dict(n=-1), dict(start=124), dict(start=2 ** 31 - 1, n=2 ** 31 - 1), dict(ko=0),
+                dict(kc=0), dict(cap=65)):
+        assert call(**bad) == L.DA_ERR_INVALID_ARG, bad
+    for bad in (dict(ko=24), dict(st=(640, 321, 64)), dict(nk=2)):
+        assert call(**bad) == L.DA_ERR_ALIGNMENT, bad
+    assert call(n=0) == L.DA_OK and call(B=0) == L.DA_OK
+
+
+def test_c_rows_refusals_and_workspace(lib):
+    ws = lib.da_kv8_attn_workspace_bytes
+    assert ws(1, 32, 8, 1, 128, 131072, 0, 0) > 0
+    assert ws(1, 32, 8, 1, 128, 131072, 2048, 128) <= ws(1, 32, 8, 1, 128, 131072, 0, 0)
+    assert ws(1, 32, 8, 1, 128, 64, 0, 0) == 0                 # one block: nothing to join
+    assert ws(1, 32, 8, 1, 96, 131072, 0, 0) == 0 and ws(1, 30, 8, 1, 128, 131072, 0, 0) == 0
+    assert ws(1, 32, 8, 0, 128, 131072, 0, 0) == 0 and ws(1, 32, 8, 1, 128, -1, 0, 0) == 0
+
+    def call(**kw):
+        a = dict(q=16, qs=(8 * 64, 64, 64), kc=16, vc=16, sk=16, sv=16, cap=1024, out=16, B=1, Hq=8, Hkv=2, s=1, D=64,
+                 nk=0, n=1000, window=0, sink=0, add=0, ws=16, nb=1 << 30, dtype=L.DA_BF16)
+        a.update(kw)
+        p = ctypes.c_void_p
+        return lib.da_kv8_attn_fwd(p(a["q"]), L.strides3(*a["qs"]), p(a["kc"]), p(a["vc"]), p(a["sk"]), p(a["sv"]),
+                                   L.I64x8(128 * 1024, 64 * 1024, 128 * 1024, 64 * 1024, 32, 16, 32, 16), a["cap"],
+                                   p(a["out"]), L.strides3(8 * 64, 64, 64), a["B"], a["Hq"], a["Hkv"], a["s"], a["D"],
+                                   p(a["nk"]), 0, a["n"], a["window"], a["sink"], 0.1, p(a["add"]), None, p(a["ws"]),
+                                   a["nb"], a["dtype"], None)
+    assert call(dtype=3) == L.DA_ERR_DTYPE and call(D=512) == L.DA_ERR_HEAD_DIM
+    for bad in (dict(Hq=9), dict(Hq=0), dict(s=-1), dict(window=-1), dict(sink=-1), dict(n=-1), dict(n=1025), dict(q=0),
+                dict(out=0), dict(kc=0), dict(cap=1000), dict(add=16), dict(s=1 << 30)):
+        assert call(**bad) == L.DA_ERR_INVALID_ARG, bad
+    need = ws(1, 8, 2, 1, 64, 1000, 0, 0)
+    assert need > 0 and call(nb=need - 1) == L.DA_ERR_WORKSPACE and call(ws=0) == L.DA_ERR_WORKSPACE
+    for bad in (dict(q=24), dict(out=24), dict(qs=(512, 65, 64)), dict(nk=18), dict(ws=24)):
+        assert call(**bad) == L.DA_ERR_ALIGNMENT, bad
+    assert call(s=0) == L.DA_OK and call(B=0) == L.DA_OK
