@@ -309,7 +309,9 @@ struct RowsArgs {
   int n_rt, rows;           // row tiles of `rows` rows (flattened row i * G + head) per sequence and kv head
   int window, sink;
   float scale_log2;         // sm_scale * log2(e)
-  int target;               // items asked for
+  int slots;                // workgroups that are resident together
+  FastDiv round;            // blocks that they take at most: slots * CHUNK
+  FastDiv units, tiles, heads;   // Hkv * n_rt, n_rt, G
   float* part;              // per item: rows x D sums, then rows references, rows weights
   int64_t pitch;            // floats per item
 };
@@ -339,61 +341,105 @@ __device__ __forceinline__ Blocks blocks_of(const RowsArgs& a, int n) {
   return l;
 }
 
-constexpr int WAVES = 4;
+#ifndef KV8_WAVES
+#define KV8_WAVES 4
+#endif
+#ifndef KV8_CMAX
+#define KV8_CMAX 64
+#endif
+#ifndef KV8_NT
+#define KV8_NT 0
+#endif
+#ifndef KV8_W128
+#define KV8_W128 2
+#endif
+constexpr int WAVES = KV8_WAVES;
+// Waves per SIMD of the rows kernel: what the registers of a block's codes, the
+// sums and MT tiles of probabilities leave room for.
+__host__ __device__ constexpr int rows_waves(int D, int mt) {
+  return D * mt <= 64 ? (mt == 1 ? 4 : mt == 2 ? 3 : 2) : D * mt <= 128 ? (D == 128 ? KV8_W128 : 2) : 1;
+}
+constexpr int CHUNK = KV8_CMAX;              // blocks of an item at most, where there are many
 
 // Splits: every item takes `chunk` blocks of one (sequence, kv head, row tile);
 // chunk is the launch's blocks over the items asked for, so that sequences of
 // different lengths give items of one size. An item's place is found by each
 // wave for itself: the sequences' item counts, summed over 64 lanes.
+// `blocks`: all sequences', kv heads' and row tiles' together (below 2^31).
+__host__ __device__ __forceinline__ int item_budget(int blocks, int slots, const FastDiv& round) {
+  return slots * (int)(fdiv(blocks + round.d - 1, round));
+}
+
 struct Place {
   int b, unit, split, n_split, chunk, slot0;   // unit: kv head * n_rt + row tile; slot0: its first item
 };
 
-__device__ __forceinline__ int chunk_of(int64_t blocks, int target) {
-  const int64_t c = (blocks + target - 1) / target;
-  return (int)((c + WAVES - 1) / WAVES) * WAVES;
-}
-
-__device__ __forceinline__ int wave_sum(int x) {
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor(x, off);
+// Inclusive sum over the lanes up to this one.
+__device__ __forceinline__ int scan64(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);    // row_shr 1, 2, 4, 8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);   // row 0's total to row 1, 2's to 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);   // rows 0 and 1's to rows 2 and 3
   return x;
 }
 
 // ITEM: `i` counts items, otherwise (sequence, unit) pairs.
 template <bool ITEM>
 __device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
-  const int lane = threadIdx.x % 64;
-  const int units = a.Hkv * a.n_rt;
-  int64_t total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int n = b0 + lane < a.B ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
-    total += wave_sum(n);
+  const int units = a.units.d;
+  if (a.B == 1 || !a.n_dev || a.n_step == 0) {     // one count for all sequences
+    const int n = blocks_of(a, __builtin_amdgcn_readfirstlane(keys_of(a, 0))).n;
+    const int pairs = a.B * units;
+    const int splits = max(item_budget(n * pairs, a.slots, a.round) / pairs, 1);
+    p.chunk = max((n + splits - 1) / splits, WAVES);
+    p.n_split = max((n + p.chunk - 1) / p.chunk, 1);
+    const int pair = ITEM ? i / p.n_split : i;
+    p.split = ITEM ? i - pair * p.n_split : 0;
+    p.b = fdiv(pair, a.units);
+    p.unit = pair - p.b * units;
+    p.slot0 = pair * p.n_split;
+    return p.b < a.B;
   }
-  p.chunk = max(chunk_of(total * units, a.target), WAVES);
+  const int lane = threadIdx.x % 64;
+  // the counts of the first 64 sequences stay in a register
+  const int n0 = lane < a.B ? blocks_of(a, keys_of(a, lane)).n : 0;
+  int total = __builtin_amdgcn_readlane(scan64(n0), 63);
+  for (int b0 = 64; b0 < a.B; b0 += 64) {
+    const int n = b0 + lane < a.B ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
+    total += __builtin_amdgcn_readlane(scan64(n), 63);
+  }
+  const int budget = item_budget(total * units, a.slots, a.round);
+  p.chunk = max((total * units + budget - 1) / max(budget, 1), WAVES);
+  // the sequences' last items are short: longer ones, until all fit the budget
+  for (int tries = 0; tries < 4; ++tries) {
+    int items = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {
+      const bool in = b0 + lane < a.B;
+      const int n = b0 == 0 ? n0 : in ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
+      items += __builtin_amdgcn_readlane(scan64(in ? max((n + p.chunk - 1) / p.chunk, 1) : 0), 63) * units;
+    }
+    if (items <= budget || a.B * units >= budget) break;
+    p.chunk += max((p.chunk * (items - budget)) / budget, 1);
+  }
   int before = 0;           // items of the sequences before
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const bool in = b0 + lane < a.B;
-    const int n = in ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
+    const int n = b0 == 0 ? n0 : in ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
     const int mine = in ? max((n + p.chunk - 1) / p.chunk, 1) : 0;
-    int upto = mine;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int x = __shfl_up(upto, off);
-      if (lane >= off) upto += x;
-    }
+    const int upto = scan64(mine);
     const int have = ITEM ? i - before : i - b0 * units;     // in this batch of sequences
-    const int end = ITEM ? upto * units : (lane + 1) * units;
-    const uint64_t past = __ballot(in && end > have);
+    const uint64_t past = __ballot(in && (ITEM ? upto : lane + 1) * units > have);
     if (past) {
       const int l = __ffsll((unsigned long long)past) - 1;
-      const int start = __shfl(upto - mine, l) * units;
-      p.n_split = __shfl(mine, l);
+      p.n_split = __builtin_amdgcn_readlane(mine, l);
+      const int start = (__builtin_amdgcn_readlane(upto, l) - p.n_split) * units;
       p.b = b0 + l;
       if (ITEM) {
         const int rest = have - start;
         p.unit = rest / p.n_split;
-        p.split = rest % p.n_split;
+        p.split = rest - p.unit * p.n_split;
       } else {
         p.unit = have - l * units;
         p.split = 0;
@@ -401,7 +447,7 @@ __device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
       p.slot0 = before + start + p.unit * p.n_split;
       return true;
     }
-    before += __shfl(upto, 63) * units;
+    before += __builtin_amdgcn_readlane(upto, 63) * units;
   }
   return false;
 }
@@ -452,17 +498,24 @@ __device__ __forceinline__ void store4(const RowsArgs& a, int b, int h, int i, i
 // type: the codes are exact in it, and its 11 bits keep the probabilities'
 // rounding below that of a bf16 result.
 template <typename T, int D, int MT>
-__global__ __launch_bounds__(64 * WAVES) void kv8_rows_kernel(RowsArgs a) {
+__global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel(RowsArgs a) {
   constexpr int KS = D / 32;                 // steps of the Q K product
   constexpr int KW = D >= 64 ? D / 64 : 1;   // loads of a key's row per lane
   constexpr int DT = D / 16;
   using P = Dot<_Float16>;
   Place p;
   if (!locate<true>(a, blockIdx.x, p)) return;
-  const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  // (all of it is the wave's: scalar registers)
+  p.b = __builtin_amdgcn_readfirstlane(p.b);
+  p.unit = __builtin_amdgcn_readfirstlane(p.unit);
+  p.split = __builtin_amdgcn_readfirstlane(p.split);
+  p.chunk = __builtin_amdgcn_readfirstlane(p.chunk);
+  p.n_split = __builtin_amdgcn_readfirstlane(p.n_split);
+  p.slot0 = __builtin_amdgcn_readfirstlane(p.slot0);
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int c = lane % 16, g = lane / 16;
-  const int b = p.b, hk = p.unit / a.n_rt, m0 = p.unit % a.n_rt * a.rows;
-  const int n = keys_of(a, b);
+  const int b = p.b, hk = fdiv(p.unit, a.tiles), m0 = (p.unit - hk * a.n_rt) * a.rows;
+  const int n = __builtin_amdgcn_readfirstlane(keys_of(a, b));
   const Blocks list = blocks_of(a, n);
   const int n_rows = min(a.rows, a.s * a.G - m0);
 
@@ -472,16 +525,13 @@ __global__ __launch_bounds__(64 * WAVES) void kv8_rows_kernel(RowsArgs a) {
   int lim[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int m = m0 + mt * 16 + c;
-    const bool in = mt * 16 + c < n_rows;
-    const int i = m / a.G;
-    lim[mt] = in ? n - a.s + i : -1;
-    const T* src = (const T*)a.q + b * a.q_b + (int64_t)(hk * a.G + m % a.G) * a.q_h + i * a.q_s;
+    // (columns behind the last row repeat it; nothing is made of them)
+    const int m = m0 + min(mt * 16 + c, n_rows - 1);
+    const int i = fdiv(m, a.heads);
+    lim[mt] = n - a.s + i;
+    const T* src = (const T*)a.q + b * a.q_b + (int64_t)(hk * a.G + m - i * a.G) * a.q_h + i * a.q_s;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      const int d = D >= 64 ? k / 2 * 64 + g * 16 + k % 2 * 8 : g * 8;
-      qf[mt][k] = in ? *(const u32x4*)(src + d) : (u32x4){0, 0, 0, 0};
-    }
+    for (int k = 0; k < KS; ++k) qf[mt][k] = *(const u32x4*)(src + (D >= 64 ? k / 2 * 64 + g * 16 + k % 2 * 8 : g * 8));
   }
   const uint8_t* kc = a.c.k + b * a.c.k_b + hk * a.c.k_h;
   const uint8_t* vc = a.c.v + b * a.c.v_b + hk * a.c.v_h;
@@ -500,137 +550,156 @@ __global__ __launch_bounds__(64 * WAVES) void kv8_rows_kernel(RowsArgs a) {
   const uint32_t one = 0x3c003c00u;
   const u32x4 ones = {one, one, one, one};
   // rows m0 / G .. of the tile: the first's and the last's limits
-  const int lim_lo = n - a.s + m0 / a.G, lim_hi = n - a.s + (m0 + n_rows - 1) / a.G;
+  const int lim_lo = n - a.s + (int)fdiv(m0, a.heads), lim_hi = n - a.s + (int)fdiv(m0 + n_rows - 1, a.heads);
 
-  const int end = min((p.split + 1) * p.chunk, list.n);
-  for (int x = p.split * p.chunk + wave; x < end; x += WAVES) {
-    const int blk = __builtin_amdgcn_readfirstlane(list.at(x));
-    const int key0 = blk * KB;
-    if (key0 > lim_hi) continue;
-    // every row sees every key of the block?
-    const bool whole = key0 + KB - 1 <= lim_lo &&
-        (a.window == 0 || key0 > lim_hi - a.window || key0 + KB <= a.sink);
-    const uint8_t* kb = kc + (int64_t)key0 * D;
-    const uint8_t* vb = vc + (int64_t)key0 * D;
-    u32x4 kf[4][KW], vf[DT];
+  // this wave's blocks of the list: one in WAVES, up to the tile's last key
+  int end = min((p.split + 1) * p.chunk, list.n);
+  end = min(end, lim_hi < 0 ? 0 : list.first + lim_hi / KB + 1 - list.lo);
+  int x = p.split * p.chunk + wave;
+  u32x4 kf[4][KW], vf[DT];
+  float sk, sv;
+  // a block's loads; none are made (zeros) where there is no block
+  const uint32_t k_off = c * D + g * (D >= 64 ? 16 : 8), v_off = c * KB + g * 16;
+  auto load_k = [&](int blk, bool any) __attribute__((always_inline)) {
+    const auto r = make_rsrc(kc + (int64_t)blk * (KB * D), any ? KB * D : 0);
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
-        const uint8_t* src = kb + (t * 16 + c) * D;
         if constexpr (D >= 64) {
-          kf[t][w] = *(const u32x4*)(src + w * 64 + g * 16);
+          kf[t][w] = __builtin_amdgcn_raw_buffer_load_b128(r, k_off, t * 16 * D + w * 64, KV8_NT ? 2 : 0);
         } else {
-          const u32x2 y = *(const u32x2*)(src + g * 8);
+          const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(r, k_off, t * 16 * D, KV8_NT ? 2 : 0);
           kf[t][w] = (u32x4){y[0], y[1], 0, 0};
         }
       }
+    sk = ksc[blk];
+  };
+  auto load_v = [&](int blk, bool any) __attribute__((always_inline)) {
+    const auto r = make_rsrc(vc + (int64_t)blk * (KB * D), any ? KB * D : 0);
 #pragma unroll
-    for (int t = 0; t < DT; ++t) vf[t] = *(const u32x4*)(vb + (t * 16 + c) * KB + g * 16);
-    const float sc = ksc[blk] * a.scale_log2;
-    const float vs = vsc[blk];
-
-    u32x4 pf[MT][2];
-    uint32_t seen[MT];                        // bit 4 t + r: the row sees token 16 t + 4 g + r
-    {
-      f32x4 s[MT][4];
+    for (int t = 0; t < DT; ++t) vf[t] = __builtin_amdgcn_raw_buffer_load_b128(r, v_off, t * 16 * KB, KV8_NT ? 2 : 0);
+    sv = vsc[blk];
+  };
+  int blk = x < end ? list.at(x) : 0;
+  load_k(blk, x < end);
+  __builtin_amdgcn_sched_barrier(0);          // (the keys are waited for first)
+  load_v(blk, x < end);
+  while (x < end) {
+    const int key0 = blk * KB;
+    x += WAVES;
+    const bool more = x < end;
+    blk = more ? list.at(x) : 0;
+    // every row sees every key of the block?
+    const bool whole = key0 + KB - 1 <= lim_lo &&
+        (a.window == 0 || key0 > lim_hi - a.window || key0 + KB <= a.sink);
+    // bit 4 t + r: the row sees token 16 t + 4 g + r of the block
+    auto seen = [&](int mt) __attribute__((always_inline)) {
+      const int hi = lim[mt] - key0 - g * 4, lo = a.window > 0 ? hi - a.window : -1, sink = a.sink - key0 - g * 4;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int at = e / 4 * 16 + e % 4;
+        bits |= (uint32_t)(at <= hi && (at > lo || at < sink)) << e;
+      }
+      return bits;
+    };
+    f32x4 s[MT][4];
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
+        const u32x4 af = Dot<T>::codes(kf[t][k / 2][k % 2 * 2], kf[t][k / 2][k % 2 * 2 + 1]);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) s[mt][t] = (f32x4){0, 0, 0, 0};
-#pragma unroll
-        for (int k = 0; k < KS; ++k) {
-          const u32x4 af = Dot<T>::codes(kf[t][k / 2][k % 2 * 2], kf[t][k / 2][k % 2 * 2 + 1]);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) s[mt][t] = Dot<T>::mfma(af, qf[mt][k], s[mt][t]);
-        }
+        for (int mt = 0; mt < MT; ++mt)
+          s[mt][t] = Dot<T>::mfma(af, qf[mt][k], k == 0 ? (f32x4){0, 0, 0, 0} : s[mt][t]);
       }
+      __builtin_amdgcn_sched_barrier(0);      // (the conversions stay beside their products: fewer registers)
+    }
+    const float sc = sk * a.scale_log2;
+    load_k(blk, more);                        // the keys' registers are free from here on
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[mt][e / 4][e % 4] *= sc;
+    if (!whole) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        seen[mt] = 0xffffu;
-        if (!whole) {
-          seen[mt] = 0;
-          const int lo = a.window > 0 ? lim[mt] - a.window : -1;
+        const uint32_t bits = seen(mt);
 #pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = key0 + e / 4 * 16 + g * 4 + e % 4;
-            seen[mt] |= (uint32_t)(key <= lim[mt] && (key > lo || key < a.sink)) << e;
-          }
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          float y = s[mt][e / 4][e % 4] * sc;
-          if (!whole) y = seen[mt] >> e & 1 ? y : -INFINITY;
-          s[mt][e / 4][e % 4] = y;
-          top = fmaxf(top, y);
-        }
-        top = group_max(top);
-        if (__any(top > ref[mt] + LAG)) {
-          const float to = fmaxf(ref[mt], top);
-          const float alpha = fast_exp2(ref[mt] - to);
-          ref[mt] = to;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) sum[mt][r] *= alpha;
-#pragma unroll
-          for (int t = 0; t < DT; ++t)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc[mt][t][r] *= alpha;
-        }
-        const float off = BIAS - ref[mt];
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int t = 2 * u + w / 2, r = w % 2 * 2;
-            float y0 = fast_exp2(s[mt][t][r] + off), y1 = fast_exp2(s[mt][t][r + 1] + off);
-            if (!whole) {
-              y0 = seen[mt] >> (4 * t + r) & 1 ? y0 : 0.f;
-              y1 = seen[mt] >> (4 * t + r + 1) & 1 ? y1 : 0.f;
-            }
-            pf[mt][u][w] = Elt<_Float16>::pack2(y0, y1);
-          }
+        for (int e = 0; e < 16; ++e) s[mt][e / 4][e % 4] = bits >> e & 1 ? s[mt][e / 4][e % 4] : -INFINITY;
       }
     }
+    u32x4 pf[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float top = s[mt][0][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[mt][e / 4][e % 4]);
+      top = group_max(top);
+      if (__any(top > ref[mt] + LAG)) {
+        const float to = fmaxf(ref[mt], top);
+        const float alpha = fast_exp2(ref[mt] - to);
+        ref[mt] = to;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum[mt][r] *= alpha;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[mt][t][r] *= alpha;
+      }
+      const float off = BIAS - ref[mt];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int t = 2 * u + w / 2, r = w % 2 * 2;
+          pf[mt][u][w] = Elt<_Float16>::pack2(fast_exp2(s[mt][t][r] + off), fast_exp2(s[mt][t][r + 1] + off));
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);
     if (!whole) {
-      // A NaN code of a token that a row does not see (rows behind the last
-      // key, or outside the row's window) must not reach it through 0 * NaN:
-      // the codes are taken as zero, and the rows that do see one get theirs
-      // from a product of the codes' and the rows' marks.
+      // A NaN code of a token that a row does not see (behind the last key,
+      // outside the row's window) must not reach it through 0 * NaN: the code
+      // is taken as zero, and the rows that do see one get theirs from a
+      // product of the codes' and the rows' marks.
+      auto nans = [&](uint32_t w) __attribute__((always_inline)) {      // bit 0 of its NaN bytes
+        return ((w & 0x7f7f7f7fu) + 0x01010101u) >> 7 & 0x01010101u;
+      };
       uint32_t bad = 0;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) bad |= (vf[t][w] & 0x7f7f7f7fu) + 0x01010101u;
-      if (__any((bad & 0x80808080u) != 0)) {
+        for (int w = 0; w < 4; ++w) bad |= nans(vf[t][w]);
+      if (__any(bad != 0)) {
         u32x4 mark[MT][2];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt) {
+          const uint32_t bits = seen(mt);
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const uint32_t two = seen[mt] >> (8 * u + 2 * w) & 3;
-              mark[mt][u][w] = (two & 1 ? 0x3c00u : 0u) | (two & 2 ? 0x3c000000u : 0u);
-            }
+          for (int w = 0; w < 8; ++w) {
+            const uint32_t two = bits >> 2 * w & 3;
+            mark[mt][w / 4][w % 4] = (two & 1) * 0x3c00u | (two >> 1) * 0x3c000000u;
+          }
+        }
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
-          u32x4 nan;
+          uint32_t hit[4];
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t hit = ((vf[t][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;   // bit 7 of NaN bytes
-            nan[w] = (hit >> 7) * 0x38u;                                                    // 1.0 there
-            vf[t][w] &= ~((hit >> 7) * 0xffu);
+            hit[w] = nans(vf[t][w]);
+            vf[t][w] &= ~(hit[w] * 0xffu);
+            hit[w] *= 0x38u;                                            // the code of 1
           }
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            f32x4 hits = {0, 0, 0, 0};
+            f32x4 hits = P::mfma(P::codes(hit[0], hit[1]), mark[mt][0], (f32x4){0, 0, 0, 0});
+            hits = P::mfma(P::codes(hit[2], hit[3]), mark[mt][1], hits);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) hits = P::mfma(P::codes(nan[2 * u], nan[2 * u + 1]), mark[mt][u], hits);
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (hits[r] > 0.f) acc[mt][t][r] = __builtin_nanf("");
+            for (int r = 0; r < 4; ++r) acc[mt][t][r] = hits[r] > 0.f ? __builtin_nanf("") : acc[mt][t][r];
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     }
@@ -646,9 +715,12 @@ __global__ __launch_bounds__(64 * WAVES) void kv8_rows_kernel(RowsArgs a) {
         f32x4 y = P::mfma(v0, pf[mt][0], (f32x4){0, 0, 0, 0});
         y = P::mfma(v1, pf[mt][1], y);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) acc[mt][t][r] = fmaf(y[r], vs, acc[mt][t][r]);
+        for (int r = 0; r < 4; ++r) acc[mt][t][r] = fmaf(y[r], sv, acc[mt][t][r]);
       }
+      if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
+    load_v(blk, more);
+    __builtin_amdgcn_sched_barrier(0);
   }
 
   // join the waves, one 16-row tile after the other
@@ -686,8 +758,8 @@ __global__ __launch_bounds__(64 * WAVES) void kv8_rows_kernel(RowsArgs a) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] *= inv;
-        const int m = m0 + row;
-        store4<T>(a, b, hk * a.G + m % a.G, m / a.G, d, o);
+        const int m = m0 + row, i = fdiv(m, a.heads);
+        store4<T>(a, b, hk * a.G + m - i * a.G, i, d, o);
       } else {
         *(f32x4*)(part + row * D + d) = o;
         if (d == 0) {
@@ -708,22 +780,35 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(RowsArgs a) {
   const int row = blockIdx.y;
   Place p;
   if (!locate<false>(a, blockIdx.x, p) || p.n_split == 1) return;
-  const int m = p.unit % a.n_rt * a.rows + row;
+  const int hk = fdiv(p.unit, a.tiles), m = (p.unit - hk * a.n_rt) * a.rows + row;
   if (m >= a.s * a.G) return;
+  const int qi = fdiv(m, a.heads);
   const int t = threadIdx.x % CT, sg = threadIdx.x / CT;
   const float* part = a.part + p.slot0 * a.pitch;
   float M = NO_KEYS, L = 0.f;
   f32x4 o = {0, 0, 0, 0};
-  for (int i = sg; i < p.n_split; i += SG) {
-    const float* src = part + i * a.pitch;
-    const float mi = src[a.rows * D + row], li = src[a.rows * (D + 1) + row];
-    const f32x4 y = *(const f32x4*)(src + row * D + t * 4);
-    const float to = fmaxf(M, mi);
-    const float k0 = fast_exp2(M - to), k1 = fast_exp2(mi - to);
-    M = to;
-    L = L * k0 + li * k1;
+  constexpr int U = 4;                         // items whose loads are in flight together
+  for (int i0 = sg; i0 < p.n_split; i0 += U * SG) {
+    float mi[U], li[U];
+    f32x4 y[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * k0 + y[e] * k1;
+    for (int u = 0; u < U; ++u) {
+      const int i = min(i0 + u * SG, p.n_split - 1);
+      const float* src = part + i * a.pitch;
+      mi[u] = src[a.rows * D + row];
+      li[u] = src[a.rows * (D + 1) + row];
+      y[u] = *(const f32x4*)(src + row * D + t * 4);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i0 + u * SG >= p.n_split) break;
+      const float to = fmaxf(M, mi[u]);
+      const float k0 = fast_exp2(M - to), k1 = fast_exp2(mi[u] - to);
+      M = to;
+      L = L * k0 + li[u] * k1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = o[e] * k0 + y[u][e] * k1;
+    }
   }
   s_o[sg][t] = o;
   if (t == 0) {
@@ -747,7 +832,7 @@ __global__ __launch_bounds__(256) void kv8_join_kernel(RowsArgs a) {
   const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= inv;
-  store4<T>(a, p.b, p.unit / a.n_rt * a.G + m % a.G, m / a.G, t * 4, o);
+  store4<T>(a, p.b, hk * a.G + m - qi * a.G, qi, t * 4, o);
 }
 
 // ---------------------------------------------------------------------------
@@ -759,7 +844,8 @@ struct RowsPlan {
   int mt, rows, n_rt;
   int64_t pairs, items;     // (sequence, kv head, row tile) triples; item slots
   int64_t pitch;            // floats of an item's partial sums (a multiple of 4)
-  int target;
+  int slots;
+  FastDiv round;
   size_t bytes;
 };
 
@@ -776,11 +862,17 @@ RowsPlan plan_rows(int B, int Hkv, int G, int s, int D, int64_t max_keys, int wi
     const int64_t near = ((int64_t)window + s + 2 * KB - 2) / KB + ((int64_t)sink + KB - 1) / KB;
     if (near < blocks) blocks = near;
   }
-  p.target = 1024;
-  // no more items than chunks of WAVES blocks: one for each pair at least
+  p.slots = 256 * 4 * rows_waves(D, p.mt) / WAVES;
+  // an upper bound of the items, whatever the lengths: the budget of the longest
+  // ones and one short item a pair, but no more than items of WAVES blocks
   const int64_t chunks = (blocks + WAVES - 1) / WAVES;
   const int64_t most = p.pairs * (chunks > 1 ? chunks : 1);
-  p.items = p.target + p.pairs < most ? p.target + p.pairs : most;
+  p.round = make_fastdiv(p.slots * CHUNK);
+  p.items = most;
+  if (blocks * p.pairs < 0x7fffffff - p.slots * CHUNK) {
+    const int64_t some = item_budget((int)(blocks * p.pairs), p.slots, p.round) + p.pairs;
+    if (some < most) p.items = some;
+  }
   p.pitch = (int64_t)p.rows * D + (2 * p.rows + 3) / 4 * 4;
   p.bytes = chunks <= 1 ? 0 : (size_t)(p.items * p.pitch) * sizeof(float);
   return p;
@@ -939,7 +1031,9 @@ extern "C" int da_kv8_attn_fwd(const void* q, const int64_t q_str[3], const void
   window = window < cap ? window : cap;
   sink = sink < cap ? sink : cap;
   const RowsPlan p = plan_rows(B, Hkv, Hq / Hkv, s, D, n_keys_dev ? cap : n_keys, window, sink);
-  if ((int64_t)Hq / Hkv * s > 0x7fffffff || p.pairs > 0x7fffff || p.items * 256 > 0x7fffffffll) return DA_ERR_INVALID_ARG;
+  if ((int64_t)Hq / Hkv * s > 0x7fffffff || p.pairs > 0x7fffff || p.items * 256 > 0x7fffffffll ||
+      p.pairs * ((cap + KB - 1) / KB) > 0x70000000ll)
+    return DA_ERR_INVALID_ARG;
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return DA_ERR_WORKSPACE;
   if (!aligned16(workspace)) return DA_ERR_ALIGNMENT;
   a.q = q;
@@ -955,7 +1049,11 @@ extern "C" int da_kv8_attn_fwd(const void* q, const int64_t q_str[3], const void
   a.n_rt = p.n_rt, a.rows = p.rows;
   a.window = window, a.sink = sink;
   a.scale_log2 = sm_scale * 1.4426950408889634f;
-  a.target = p.target;
+  a.slots = p.slots;
+  a.round = p.round;
+  a.units = make_fastdiv(Hkv * p.n_rt);
+  a.tiles = make_fastdiv(p.n_rt);
+  a.heads = make_fastdiv(a.G);
   a.part = (float*)workspace;
   a.pitch = p.pitch;
   by_type(dtype, D, [&](auto t, auto d) {
