@@ -103,19 +103,39 @@ struct Cache {
 
 template <int N> struct alignas(N < 4 ? 4 * N : 16) Words { uint32_t w[N]; };
 
-// One wave per (sequence, block, head, tensor), heads next to each other.
+// One wave per (sequence, block, head, tensor), four to a workgroup.
 struct Units {
-  FastDiv per_blk, per_seq;    // waves of a block (2 Hkv), of a sequence
-  uint32_t n;
+  FastDiv inner, per_seq;      // waves of a block or of a head's tensor, of a sequence
+  uint32_t n, heads;
 };
 
-__device__ __forceinline__ bool unit_of(const Units& u, int& b, int& j, int& h, bool& is_v) {
+// Writes: heads innermost (a token's heads lie together in the input), and each
+// eighth of the waves on one XCD (workgroup x runs on XCD x % 8; the grid is a
+// multiple of 8), with non-temporal loads of the input: a prompt of 131072
+// tokens takes 145 us so, 157 in launch order, 151 with ordinary loads.
+__device__ __forceinline__ bool write_unit(const Units& u, int& b, int& j, int& h, bool& is_v) {
+  const uint32_t x = blockIdx.x, wg = x % 8 * (gridDim.x / 8) + x / 8;
+  const uint32_t i = wg * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  if (i >= u.n) return false;
+  b = fdiv(i, u.per_seq);
+  const uint32_t rest = i - b * u.per_seq.d;
+  j = fdiv(rest, u.inner);
+  const uint32_t w = rest - j * u.inner.d;
+  is_v = w >= u.heads;
+  h = w - (is_v ? u.heads : 0);
+  return true;
+}
+
+// Reads: a head's blocks innermost (both sides are contiguous along them), with
+// non-temporal stores: 131072 rows take 145 us so, 167 with heads innermost,
+// 174 with ordinary stores too.
+__device__ __forceinline__ bool read_unit(const Units& u, int& b, int& j, int& h, bool& is_v) {
   const uint32_t i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   if (i >= u.n) return false;
   b = fdiv(i, u.per_seq);
   const uint32_t rest = i - b * u.per_seq.d;
-  j = fdiv(rest, u.per_blk);
-  const uint32_t w = rest - j * u.per_blk.d;
+  const uint32_t w = fdiv(rest, u.inner);
+  j = rest - w * u.inner.d;
   h = w >> 1;
   is_v = w & 1;
   return true;
@@ -145,7 +165,7 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
   using Run = Words<TPL / 4>;
   int b, j, h;
   bool is_v;
-  if (!unit_of(a.units, b, j, h, is_v)) return;
+  if (!write_unit(a.units, b, j, h, is_v)) return;
   const int lane = threadIdx.x % 64;
   const int64_t pos = a.pos_dev ? a.pos_dev[(int64_t)b * a.pos_step] : a.pos;
   const int count = a.counts ? min(max(a.counts[(int64_t)b * a.counts_step], 0), a.S) : a.S;
@@ -165,7 +185,7 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
 #pragma unroll
   for (int i = 0; i < TPL; ++i) {
     const int r = token_of(p0 + i);
-    x[i] = *(const u32x4*)(src + (int64_t)min(max(r, r0), r1 - 1) * step);
+    x[i] = ld_nt4(src + (int64_t)min(max(r, r0), r1 - 1) * step);
     fresh |= (uint32_t)(r >= r0 && r < r1) << i;
     older |= (uint32_t)(r < r0) << i;
   }
@@ -253,14 +273,15 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
 // tensor, a lane 8 columns of the token. The block's other tokens are touched
 // only where the token needs a larger scale than theirs. What counts is the
 // chain position -> token -> its largest magnitude -> stores; the block-sized
-// kernel above, which also loads the block's runs, takes MEASURED_APPEND.
+// kernel above, which also loads the block's runs, takes 4 us more (10.7 us to 2.7
+// in a captured step's launch, before it loaded them early).
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(WriteArgs a) {
   using E = Elt<T>;
   constexpr int DG = D / 8;
   int b, j, h;
   bool is_v;
-  if (!unit_of(a.units, b, j, h, is_v)) return;
+  if (!write_unit(a.units, b, j, h, is_v)) return;
   const int lane = threadIdx.x % 64, dg = lane % DG;
   const T* src = is_v ? (const T*)a.v + b * a.vx_b + h * a.vx_h : (const T*)a.k + b * a.kx_b + h * a.kx_h;
   const u32x4 x = *(const u32x4*)(src + dg * 8);
@@ -356,7 +377,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
   using Run = Words<TPL / 4>;
   int b, j, h;
   bool is_v;
-  if (!unit_of(a.units, b, j, h, is_v)) return;
+  if (!read_unit(a.units, b, j, h, is_v)) return;
   const int lane = threadIdx.x % 64;
   const int blk = a.start / KB + j;
   const int live = a.n_keys ? a.n_keys[(int64_t)b * a.n_step] : a.c.cap;
@@ -372,7 +393,7 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
     const int row = blk * KB + r;
     if (row < a.start || row >= a.start + a.n) return;
     if (row >= live) w = (u32x4){0, 0, 0, 0};
-    *(u32x4*)(dst + (int64_t)(row - a.start) * step + dg * 8) = w;
+    st_nt4(dst + (int64_t)(row - a.start) * step + dg * 8, w);
   };
   if (!is_v) {
     const uint8_t* src = a.c.k + b * a.c.k_b + h * a.c.k_h + (int64_t)blk * KB * D + dg * 8;
@@ -1051,12 +1072,15 @@ void by_type(int dtype, int D, F&& f) {
 }
 
 // Waves of a write or read (below 2^31).
-bool units_for(Units& u, int B, int n_blk, int Hkv) {
+bool units_for(Units& u, int B, int n_blk, int Hkv, bool read) {
   const int64_t n = (int64_t)B * n_blk * 2 * Hkv;
-  if ((int64_t)n_blk * 2 * Hkv > 0x7ffffff0 || n > 0x7ffffff0) return false;
-  u = Units{make_fastdiv(2 * Hkv), make_fastdiv(n_blk * 2 * Hkv), (uint32_t)n};
+  if ((int64_t)n_blk * 2 * Hkv > 0x7fffff00 || n > 0x7fffff00) return false;
+  u = Units{make_fastdiv(read ? n_blk : 2 * Hkv), make_fastdiv(n_blk * 2 * Hkv), (uint32_t)n, (uint32_t)Hkv};
   return true;
 }
+
+// Workgroups of four waves, a multiple of eight.
+unsigned units_grid(const Units& u) { return (u.n + 31) / 32 * 8; }
 
 int launched() { return hipGetLastError() == hipSuccess ? DA_OK : DA_ERR_LAUNCH; }
 
@@ -1093,10 +1117,10 @@ extern "C" int da_kv8_write(const void* k, const int64_t k_str[3], const void* v
   a.S = S;
   // blocks that S tokens touch: from a known row, or from any
   const int n_blk = pos_dev ? (int)(((int64_t)S + KB - 2) / KB + 1) : (int)((pos + S + KB - 1) / KB - pos / KB);
-  if (!units_for(a.units, B, n_blk, Hkv)) return DA_ERR_INVALID_ARG;
+  if (!units_for(a.units, B, n_blk, Hkv, false)) return DA_ERR_INVALID_ARG;
   by_type(dtype, D, [&](auto t, auto d) {
     using E = typename decltype(t)::type;
-    const dim3 grid((a.units.n + 3) / 4), block(256);
+    const dim3 grid(units_grid(a.units)), block(256);
     if (S == 1) hipLaunchKernelGGL((kv8_append_kernel<E, decltype(d)::value>), grid, block, 0, (hipStream_t)stream, a);
     else hipLaunchKernelGGL((kv8_write_kernel<E, decltype(d)::value>), grid, block, 0, (hipStream_t)stream, a);
   });
@@ -1126,9 +1150,9 @@ extern "C" int da_kv8_read(const void* k_codes, const void* v_codes, const float
   a.n_step = n_keys_per_seq ? 1 : 0;
   a.start = start, a.n = n;
   const int n_blk = (int)(((int64_t)start + n + KB - 1) / KB - start / KB);
-  if (!units_for(a.units, B, n_blk, Hkv)) return DA_ERR_INVALID_ARG;
+  if (!units_for(a.units, B, n_blk, Hkv, true)) return DA_ERR_INVALID_ARG;
   by_type(dtype, D, [&](auto t, auto d) {
-    hipLaunchKernelGGL((kv8_read_kernel<typename decltype(t)::type, decltype(d)::value>), dim3((a.units.n + 3) / 4),
+    hipLaunchKernelGGL((kv8_read_kernel<typename decltype(t)::type, decltype(d)::value>), dim3(units_grid(a.units)),
                        dim3(256), 0, (hipStream_t)stream, a);
   });
   return launched();
