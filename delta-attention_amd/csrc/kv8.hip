@@ -1020,20 +1020,16 @@ RowsPlan plan_rows(int B, int Hkv, int G, int s, int D, int64_t max_keys, int wi
   return p;
 }
 
-bool kv8_cache(Cache& c, const void* k, const void* v, const float* ks, const float* vs,
-               const int64_t st[8], int cap) {
-  c = Cache{(uint8_t*)k, (uint8_t*)v, (float*)ks, (float*)vs, st[0], st[1], st[2], st[3],
-            st[4], st[5], st[6], st[7], cap};
-  return aligned16(k) && aligned16(v) && ((uintptr_t)ks & 3) == 0 && ((uintptr_t)vs & 3) == 0 &&
-         st[0] % 16 == 0 && st[1] % 16 == 0 && st[2] % 16 == 0 && st[3] % 16 == 0;
-}
-
-int check_cache(const void* k, const void* v, const float* ks, const float* vs, const int64_t* st,
-                int cap, int B, int Hkv, int D, int dtype) {
+int take_cache(Cache& c, const da_kv8_cache& x, int dtype) {
   if (dtype != DA_BF16 && dtype != DA_FP16) return DA_ERR_DTYPE;
-  if (!head_dim_ok(D)) return DA_ERR_HEAD_DIM;
-  if (B < 0 || Hkv < 1 || cap < 0 || cap > MAX_CAP || cap % KB != 0 || !st) return DA_ERR_INVALID_ARG;
-  if (!k || !v || !ks || !vs) return DA_ERR_INVALID_ARG;
+  if (!head_dim_ok(x.D)) return DA_ERR_HEAD_DIM;
+  if (x.B < 0 || x.Hkv < 1 || x.cap < KB || x.cap > MAX_CAP || x.cap % KB != 0) return DA_ERR_INVALID_ARG;
+  if (x.B > 0 && (!x.k || !x.v || !x.k_scale || !x.v_scale)) return DA_ERR_INVALID_ARG;
+  if (!aligned16(x.k) || !aligned16(x.v) || ((uintptr_t)x.k_scale & 3) || ((uintptr_t)x.v_scale & 3) ||
+      x.k_str[0] % 16 || x.k_str[1] % 16 || x.v_str[0] % 16 || x.v_str[1] % 16)
+    return DA_ERR_ALIGNMENT;
+  c = Cache{(uint8_t*)x.k, (uint8_t*)x.v, x.k_scale, x.v_scale, x.k_str[0], x.k_str[1], x.v_str[0], x.v_str[1],
+            x.k_scale_str[0], x.k_scale_str[1], x.v_scale_str[0], x.v_scale_str[1], x.cap};
   return DA_OK;
 }
 
@@ -1089,36 +1085,32 @@ int launched() { return hipGetLastError() == hipSuccess ? DA_OK : DA_ERR_LAUNCH;
 
 using namespace da;
 
-extern "C" int da_kv8_write(const void* k, const int64_t k_str[3], const void* v, const int64_t v_str[3],
-                            int B, int S, int Hkv, int D,
-                            void* k_codes, void* v_codes, float* k_scale, float* v_scale,
-                            const int64_t c_str[8], int cap,
-                            const int64_t* pos_dev, int pos_per_seq, int64_t pos,
-                            const int32_t* counts_dev, int counts_per_seq, int dtype, void* stream) {
-  int rc = check_cache(k_codes, v_codes, k_scale, v_scale, c_str, cap, B, Hkv, D, dtype);
-  if (rc != DA_OK) return rc;
-  if (S < 0 || !k_str || !v_str) return DA_ERR_INVALID_ARG;
-  if (!pos_dev && (pos < 0 || pos + S > cap)) return DA_ERR_INVALID_ARG;
-  if (S == 0 || B == 0) return DA_OK;
-  if (!k || !v) return DA_ERR_INVALID_ARG;
+extern "C" int da_kv8_write(const da_kv8_write_args* x, void* stream) {
+  if (!x) return DA_ERR_INVALID_ARG;
   WriteArgs a{};
-  if (!kv8_cache(a.c, k_codes, v_codes, k_scale, v_scale, c_str, cap) || !aligned16(k) || !aligned16(v) ||
-      !strides8(k_str) || !strides8(v_str) || ((uintptr_t)pos_dev & 7) || ((uintptr_t)counts_dev & 3))
+  const int rc = take_cache(a.c, x->cache, x->dtype);
+  if (rc != DA_OK) return rc;
+  const int B = x->cache.B, Hkv = x->cache.Hkv, cap = x->cache.cap, S = x->S;
+  if (S < 0 || (!x->pos_dev && (x->pos < 0 || x->pos > cap - (int64_t)S))) return DA_ERR_INVALID_ARG;
+  if (S == 0 || B == 0) return DA_OK;
+  if (!x->k || !x->v) return DA_ERR_INVALID_ARG;
+  if (!aligned16(x->k) || !aligned16(x->v) || !strides8(x->k_str) || !strides8(x->v_str) ||
+      ((uintptr_t)x->pos_dev & 7) || ((uintptr_t)x->counts_dev & 3))
     return DA_ERR_ALIGNMENT;
-  a.k = k;
-  a.v = v;
-  a.kx_b = k_str[0], a.kx_s = k_str[1], a.kx_h = k_str[2];
-  a.vx_b = v_str[0], a.vx_s = v_str[1], a.vx_h = v_str[2];
-  a.pos_dev = pos_dev;
-  a.pos = pos;
-  a.counts = counts_dev;
-  a.pos_step = pos_per_seq ? 1 : 0;
-  a.counts_step = counts_per_seq ? 1 : 0;
+  a.k = x->k;
+  a.v = x->v;
+  a.kx_b = x->k_str[0], a.kx_s = x->k_str[1], a.kx_h = x->k_str[2];
+  a.vx_b = x->v_str[0], a.vx_s = x->v_str[1], a.vx_h = x->v_str[2];
+  a.pos_dev = x->pos_dev;
+  a.pos = x->pos;
+  a.counts = x->counts_dev;
+  a.pos_step = x->pos_per_seq ? 1 : 0;
+  a.counts_step = x->counts_per_seq ? 1 : 0;
   a.S = S;
   // blocks that S tokens touch: from a known row, or from any
-  const int n_blk = pos_dev ? (int)(((int64_t)S + KB - 2) / KB + 1) : (int)((pos + S + KB - 1) / KB - pos / KB);
+  const int n_blk = x->pos_dev ? (int)(((int64_t)S + KB - 2) / KB + 1) : (int)((x->pos + S + KB - 1) / KB - x->pos / KB);
   if (!units_for(a.units, B, n_blk, Hkv, false)) return DA_ERR_INVALID_ARG;
-  by_type(dtype, D, [&](auto t, auto d) {
+  by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     using E = typename decltype(t)::type;
     const dim3 grid(units_grid(a.units)), block(256);
     if (S == 1) hipLaunchKernelGGL((kv8_append_kernel<E, decltype(d)::value>), grid, block, 0, (hipStream_t)stream, a);
@@ -1127,31 +1119,28 @@ extern "C" int da_kv8_write(const void* k, const int64_t k_str[3], const void* v
   return launched();
 }
 
-extern "C" int da_kv8_read(const void* k_codes, const void* v_codes, const float* k_scale,
-                           const float* v_scale, const int64_t c_str[8], int cap,
-                           int B, int Hkv, int D, int start, int n,
-                           const int32_t* n_keys_dev, int n_keys_per_seq,
-                           void* k_out, const int64_t ko_str[3], void* v_out, const int64_t vo_str[3],
-                           int dtype, void* stream) {
-  int rc = check_cache(k_codes, v_codes, k_scale, v_scale, c_str, cap, B, Hkv, D, dtype);
-  if (rc != DA_OK) return rc;
-  if (start < 0 || n < 0 || (int64_t)start + n > cap || !ko_str || !vo_str) return DA_ERR_INVALID_ARG;
-  if (n == 0 || B == 0) return DA_OK;
-  if (!k_out || !v_out) return DA_ERR_INVALID_ARG;
+extern "C" int da_kv8_read(const da_kv8_read_args* x, void* stream) {
+  if (!x) return DA_ERR_INVALID_ARG;
   ReadArgs a{};
-  if (!kv8_cache(a.c, k_codes, v_codes, k_scale, v_scale, c_str, cap) || !aligned16(k_out) || !aligned16(v_out) ||
-      !strides8(ko_str) || !strides8(vo_str) || ((uintptr_t)n_keys_dev & 3))
+  const int rc = take_cache(a.c, x->cache, x->dtype);
+  if (rc != DA_OK) return rc;
+  const int B = x->cache.B, start = x->start, n = x->n;
+  if (start < 0 || n < 0 || (int64_t)start + n > x->cache.cap) return DA_ERR_INVALID_ARG;
+  if (n == 0 || B == 0) return DA_OK;
+  if (!x->k || !x->v) return DA_ERR_INVALID_ARG;
+  if (!aligned16(x->k) || !aligned16(x->v) || !strides8(x->k_str) || !strides8(x->v_str) ||
+      ((uintptr_t)x->n_keys_dev & 3))
     return DA_ERR_ALIGNMENT;
-  a.k = k_out;
-  a.v = v_out;
-  a.ko_b = ko_str[0], a.ko_h = ko_str[1], a.ko_s = ko_str[2];
-  a.vo_b = vo_str[0], a.vo_h = vo_str[1], a.vo_s = vo_str[2];
-  a.n_keys = n_keys_dev;
-  a.n_step = n_keys_per_seq ? 1 : 0;
+  a.k = x->k;
+  a.v = x->v;
+  a.ko_b = x->k_str[0], a.ko_h = x->k_str[1], a.ko_s = x->k_str[2];
+  a.vo_b = x->v_str[0], a.vo_h = x->v_str[1], a.vo_s = x->v_str[2];
+  a.n_keys = x->n_keys_dev;
+  a.n_step = x->n_keys_per_seq ? 1 : 0;
   a.start = start, a.n = n;
   const int n_blk = (int)(((int64_t)start + n + KB - 1) / KB - start / KB);
-  if (!units_for(a.units, B, n_blk, Hkv, true)) return DA_ERR_INVALID_ARG;
-  by_type(dtype, D, [&](auto t, auto d) {
+  if (!units_for(a.units, B, n_blk, x->cache.Hkv, true)) return DA_ERR_INVALID_ARG;
+  by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     hipLaunchKernelGGL((kv8_read_kernel<typename decltype(t)::type, decltype(d)::value>), dim3(units_grid(a.units)),
                        dim3(256), 0, (hipStream_t)stream, a);
   });
@@ -1166,55 +1155,48 @@ extern "C" size_t da_kv8_attn_workspace_bytes(int B, int Hq, int Hkv, int s, int
   return plan_rows(B, Hkv, Hq / Hkv, s, D, max_keys, window, sink).bytes;
 }
 
-extern "C" int da_kv8_attn_fwd(const void* q, const int64_t q_str[3], const void* k_codes,
-                               const void* v_codes, const float* k_scale, const float* v_scale,
-                               const int64_t c_str[8], int cap, void* out, const int64_t o_str[3],
-                               int B, int Hq, int Hkv, int s, int D,
-                               const int32_t* n_keys_dev, int n_keys_per_seq, int n_keys,
-                               int window, int sink, float sm_scale,
-                               const void* addend, const int64_t add_str[3],
-                               void* workspace, size_t workspace_bytes, int dtype, void* stream) {
-  int rc = check_cache(k_codes, v_codes, k_scale, v_scale, c_str, cap, B, Hkv, D, dtype);
-  if (rc != DA_OK) return rc;
-  if (Hq < 1 || Hq % Hkv != 0 || s < 0 || window < 0 || sink < 0 || !q_str || !o_str) return DA_ERR_INVALID_ARG;
-  if (!n_keys_dev && (n_keys < 0 || n_keys > cap)) return DA_ERR_INVALID_ARG;
-  if (s == 0 || B == 0) return DA_OK;
-  if (!q || !out || (addend && !add_str)) return DA_ERR_INVALID_ARG;
+extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
+  if (!x) return DA_ERR_INVALID_ARG;
   RowsArgs a{};
-  if (!kv8_cache(a.c, k_codes, v_codes, k_scale, v_scale, c_str, cap) || !aligned16(q) || !aligned16(out) ||
-      !strides8(q_str) || !strides8(o_str) || ((uintptr_t)n_keys_dev & 3) ||
-      (addend && (!aligned16(addend) || !strides8(add_str))))
+  const int rc = take_cache(a.c, x->cache, x->dtype);
+  if (rc != DA_OK) return rc;
+  const int B = x->cache.B, Hkv = x->cache.Hkv, cap = x->cache.cap, Hq = x->Hq, s = x->s;
+  if (Hq < 1 || Hq % Hkv != 0 || s < 0 || x->window < 0 || x->sink < 0) return DA_ERR_INVALID_ARG;
+  if (!x->n_keys_dev && (x->n_keys < 0 || x->n_keys > cap)) return DA_ERR_INVALID_ARG;
+  if (s == 0 || B == 0) return DA_OK;
+  if (!x->q || !x->out) return DA_ERR_INVALID_ARG;
+  if (!aligned16(x->q) || !aligned16(x->out) || !strides8(x->q_str) || !strides8(x->o_str) ||
+      ((uintptr_t)x->n_keys_dev & 3) || (x->addend && (!aligned16(x->addend) || !strides8(x->add_str))))
     return DA_ERR_ALIGNMENT;
   // (a window or sinks past the capacity are every key)
-  window = window < cap ? window : cap;
-  sink = sink < cap ? sink : cap;
-  const RowsPlan p = plan_rows(B, Hkv, Hq / Hkv, s, D, n_keys_dev ? cap : n_keys, window, sink);
-  if ((int64_t)Hq / Hkv * s > 0x7fffffff || p.pairs > 0x7fffff || p.items * 256 > 0x7fffffffll ||
-      p.pairs * ((cap + KB - 1) / KB) > 0x70000000ll)
+  a.window = x->window < cap ? x->window : cap;
+  a.sink = x->sink < cap ? x->sink : cap;
+  if ((int64_t)Hq / Hkv * s > 1 << 28) return DA_ERR_INVALID_ARG;
+  const RowsPlan p = plan_rows(B, Hkv, Hq / Hkv, s, x->cache.D, x->n_keys_dev ? cap : x->n_keys, a.window, a.sink);
+  if (p.pairs > 0x7fffff || p.items * 256 > 0x7fffffffll || p.pairs * (cap / KB) > 0x70000000ll)
     return DA_ERR_INVALID_ARG;
-  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes)) return DA_ERR_WORKSPACE;
-  if (!aligned16(workspace)) return DA_ERR_ALIGNMENT;
-  a.q = q;
-  a.q_b = q_str[0], a.q_h = q_str[1], a.q_s = q_str[2];
-  a.o = out;
-  a.o_b = o_str[0], a.o_h = o_str[1], a.o_s = o_str[2];
-  a.add = addend;
-  if (addend) a.add_b = add_str[0], a.add_h = add_str[1], a.add_s = add_str[2];
-  a.n_dev = n_keys_dev;
-  a.n_step = n_keys_per_seq ? 1 : 0;
-  a.n = n_keys;
+  if (p.bytes > 0 && (!x->workspace || x->workspace_bytes < (int64_t)p.bytes)) return DA_ERR_WORKSPACE;
+  if (!aligned16(x->workspace)) return DA_ERR_ALIGNMENT;
+  a.q = x->q;
+  a.q_b = x->q_str[0], a.q_h = x->q_str[1], a.q_s = x->q_str[2];
+  a.o = x->out;
+  a.o_b = x->o_str[0], a.o_h = x->o_str[1], a.o_s = x->o_str[2];
+  a.add = x->addend;
+  a.add_b = x->add_str[0], a.add_h = x->add_str[1], a.add_s = x->add_str[2];
+  a.n_dev = x->n_keys_dev;
+  a.n_step = x->n_keys_per_seq ? 1 : 0;
+  a.n = x->n_keys;
   a.B = B, a.Hkv = Hkv, a.G = Hq / Hkv, a.s = s;
   a.n_rt = p.n_rt, a.rows = p.rows;
-  a.window = window, a.sink = sink;
-  a.scale_log2 = sm_scale * 1.4426950408889634f;
+  a.scale_log2 = x->sm_scale * 1.4426950408889634f;
   a.slots = p.slots;
   a.round = p.round;
   a.units = make_fastdiv(Hkv * p.n_rt);
   a.tiles = make_fastdiv(p.n_rt);
   a.heads = make_fastdiv(a.G);
-  a.part = (float*)workspace;
+  a.part = (float*)x->workspace;
   a.pitch = p.pitch;
-  by_type(dtype, D, [&](auto t, auto d) {
+  by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     launch_rows<typename decltype(t)::type, decltype(d)::value>(a, p, (hipStream_t)stream);
   });
   return launched();

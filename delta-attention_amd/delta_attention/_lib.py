@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -89,7 +90,6 @@ _lib = None
 _lib_lock = threading.Lock()
 
 I64x3 = ctypes.c_int64 * 3
-I64x8 = ctypes.c_int64 * 8
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -221,18 +221,12 @@ def _load() -> ctypes.CDLL:
                                      _p3, _p3, _p3, _p3, _i, _i, _i, _f,
                                      _i, _i, _i, _i, _i, _i, _d, _d, _d,
                                      _vp, _vp, _vp, _vp, _i, _vp, _sz, _i, _vp, _vp]
-    L.da_kv8_write.restype = _i
-    L.da_kv8_write.argtypes = [_vp, _p3, _vp, _p3, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _p3, _i,
-                               _vp, _i, _i64, _vp, _i, _i, _vp]
-    L.da_kv8_read.restype = _i
-    L.da_kv8_read.argtypes = [_vp, _vp, _vp, _vp, _p3, _i, _i, _i, _i, _i, _i, _vp, _i,
-                              _vp, _p3, _vp, _p3, _i, _vp]
+    # (these take one struct, packed by the caller: see KV8_WRITE below)
+    for f in (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd):
+        f.restype = _i
+        f.argtypes = [ctypes.c_char_p, _vp]
     L.da_kv8_attn_workspace_bytes.restype = _sz
     L.da_kv8_attn_workspace_bytes.argtypes = [_i, _i, _i, _i, _i, _i, _i, _i]
-    L.da_kv8_attn_fwd.restype = _i
-    L.da_kv8_attn_fwd.argtypes = [_vp, _p3, _vp, _vp, _vp, _vp, _p3, _i, _vp, _p3,
-                                  _i, _i, _i, _i, _i, _vp, _i, _i, _i, _i, _f, _vp, _p3,
-                                  _vp, _sz, _i, _vp]
     L.da_build_target.restype = ctypes.c_char_p
     L.da_build_target.argtypes = []
     return L
@@ -248,6 +242,15 @@ def check(rc: int, what: str) -> None:
     if rc == DA_ERR_LAUNCH:
         raise RuntimeError(msg)
     raise AssertionError(msg)
+
+
+# The structs of the 8-bit cache's calls (native alignment), in the header's
+# order: one pack is a fifth of the time of as many ctypes arguments.
+_KV8_CACHE = "4P8q4i"      # k, v, k_scale, v_scale; their {batch, head} strides; B, Hkv, cap, D
+KV8_WRITE = struct.Struct(_KV8_CACHE + "4P7q4i")      # k, v, pos_dev, counts_dev; strides, pos; S, 2 flags, dtype
+KV8_READ = struct.Struct(_KV8_CACHE + "3P6q4i")       # k, v, n_keys_dev; strides; start, n, flag, dtype
+KV8_ATTN = struct.Struct(_KV8_CACHE + "5P10q7if")     # q, out, addend, n_keys_dev, workspace; its bytes, strides;
+                                                      # Hq, s, flag, n_keys, window, sink, dtype; sm_scale
 
 
 def strides3(*s: int):

@@ -622,26 +622,34 @@ def kv8_empty(B: int, Hkv: int, max_len: int, D: int, device="cuda") -> KV8:
                scale[0], scale[1])
 
 
-def _kv8(c: KV8):
-    """Checks a cache's tensors -> (B, Hkv, cap, D, strides of the C ABI)."""
+_F8, _F32, _I32, _I64 = torch.float8_e4m3fn, torch.float32, torch.int32, torch.int64
+
+
+def _kv8(c: KV8, dev: torch.device):
+    """Checks a cache's tensors -> the head of the C ABI's structs (pointers,
+    strides, B, Hkv, cap, D)."""
     k, v, ks, vs = c
     B, Hkv, cap, D = k.shape
     nb = cap // KV8_BLOCK
-    assert cap % KV8_BLOCK == 0 and v.shape == (B, Hkv, nb, D, KV8_BLOCK), (k.shape, v.shape)
-    assert ks.shape == (B, Hkv, nb) and vs.shape == ks.shape, (ks.shape, vs.shape, nb)
-    assert k.dtype == v.dtype == torch.float8_e4m3fn and ks.dtype == vs.dtype == torch.float32, (
-        k.dtype, v.dtype, ks.dtype, vs.dtype)
     a, b, d, e = k.stride(), v.stride(), ks.stride(), vs.stride()
+    assert cap % KV8_BLOCK == 0 and v.shape == (B, Hkv, nb, D, KV8_BLOCK) and ks.shape == vs.shape == (B, Hkv, nb), (
+        k.shape, v.shape, ks.shape, vs.shape)
+    assert k.dtype is _F8 and v.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32, (
+        k.dtype, v.dtype, ks.dtype, vs.dtype)
     assert a[2:] == (D, 1) and b[2:] == (D * KV8_BLOCK, KV8_BLOCK, 1) and d[2] == e[2] == 1, (
         "a cache's tokens, blocks and scales must be contiguous within a head")
-    return B, Hkv, cap, D, L.I64x8(a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1])
+    assert k.device == v.device == ks.device == vs.device == dev, "all tensors must be on one device"
+    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
+            a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1], B, Hkv, cap, D)
 
 
-def _per_seq(t: torch.Tensor, B: int, dtype: torch.dtype, dev: torch.device, what: str) -> int:
-    """Checks a device tensor of one entry, or one per sequence -> 0 or 1."""
-    assert t.dtype == dtype and t.device == dev and t.dim() <= 1 and t.numel() in (1, B) and t.is_contiguous(), (
+def _per_seq(t: torch.Tensor, B: int, dtype: torch.dtype, dev: torch.device, what: str) -> bool:
+    """Checks a device tensor of one entry, or one per sequence -> whether the
+    latter."""
+    n = t.numel()
+    assert t.dtype is dtype and t.device == dev and (n == B or n == 1) and t.dim() <= 1 and t.is_contiguous(), (
         f"{what}: a contiguous {dtype} tensor of 1 or {B} entries on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return int(t.numel() == B)
+    return n == B
 
 
 def kv8_write(cache: KV8, k: torch.Tensor, v: torch.Tensor, pos, *,
@@ -655,28 +663,28 @@ def kv8_write(cache: KV8, k: torch.Tensor, v: torch.Tensor, pos, *,
     or one per sequence), the tokens of each right-padded sequence. Rows behind
     the written ones keep their bytes but hold nothing any more. With device
     positions, a sequence whose rows do not fit is left unchanged."""
-    B, Hkv, cap, D, cs = _kv8(cache)
-    assert k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype, (k.shape, v.shape, k.dtype, v.dtype)
+    dev = k.device
+    head = _kv8(cache, dev)
+    B, Hkv, cap, D = head[12:]
     S = k.shape[1]
-    assert k.shape == (B, S, Hkv, D), (k.shape, (B, S, Hkv, D))
-    dev = _on_gpu(k, v, *cache)
+    assert k.shape == v.shape == (B, S, Hkv, D) and k.dtype is v.dtype, (k.shape, v.shape, (B, S, Hkv, D), k.dtype, v.dtype)
     code = _code(k)
-    pos_dev = pos_b = counts_b = 0
+    assert dev.type == "cuda" and v.device == dev, "delta-attention kernels need GPU tensors, all on one device"
+    p_dev = c_dev = p_b = c_b = 0
     if isinstance(pos, torch.Tensor):
-        pos_b, pos_dev, pos = _per_seq(pos, B, torch.int64, dev, "pos"), pos.data_ptr(), 0
+        p_b, p_dev, pos = _per_seq(pos, B, _I64, dev, "pos"), pos.data_ptr(), 0
     else:
         pos = int(pos)
-        assert 0 <= pos and pos + S <= cap, f"rows {pos} .. {pos + S} do not fit a cache of {cap}"
+        assert 0 <= pos <= cap - S, f"rows {pos} .. {pos + S} do not fit a cache of {cap}"
     if counts is not None:
-        counts_b = _per_seq(counts, B, torch.int32, dev, "counts")
+        c_b, c_dev = _per_seq(counts, B, _I32, dev, "counts"), counts.data_ptr()
     if B == 0 or S == 0:
         return
     k, v = _ready(k), _ready(v)
+    args = L.KV8_WRITE.pack(*head, k.data_ptr(), v.data_ptr(), p_dev, c_dev, *k.stride()[:3], *v.stride()[:3],
+                            pos, S, p_b, c_b, code)
     with _device(dev):
-        rc = L.lib().da_kv8_write(
-            k.data_ptr(), _s3(k, 0, 1, 2), v.data_ptr(), _s3(v, 0, 1, 2), B, S, Hkv, D,
-            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-            cs, cap, pos_dev or None, pos_b, pos, _ptr(counts), counts_b, code, _stream(dev))
+        rc = L.lib().da_kv8_write(args, _stream(dev))
     L.check(rc, "da_kv8_write")
 
 
@@ -688,24 +696,27 @@ def kv8_read(cache: KV8, start: int, n: int, *, n_keys: Optional[torch.Tensor] =
     beyond float16's largest saturate. n_keys: optional int32 device tensor
     (one entry or one per sequence); rows at or past it are zero. out: the two
     tensors to write."""
-    B, Hkv, cap, D, cs = _kv8(cache)
+    dev = cache.k.device
+    head = _kv8(cache, dev)
+    B, Hkv, cap, D = head[12:]
     start, n = int(start), int(n)
-    assert start >= 0 and n >= 0 and start + n <= cap, f"rows {start} .. {start + n} of a cache of {cap}"
-    dev = _on_gpu(*cache)
-    n_b = 0 if n_keys is None else _per_seq(n_keys, B, torch.int32, dev, "n_keys")
+    assert 0 <= start and 0 <= n <= cap - start, f"rows {start} .. {start + n} of a cache of {cap}"
+    assert dev.type == "cuda", "delta-attention kernels need GPU tensors"
+    n_dev = n_b = 0
+    if n_keys is not None:
+        n_b, n_dev = _per_seq(n_keys, B, _I32, dev, "n_keys"), n_keys.data_ptr()
     if out is None:
         out = tuple(torch.empty((2, B, Hkv, n, D), device=dev, dtype=dtype))
     k, v = out
-    assert k.shape == v.shape == (B, Hkv, n, D) and k.dtype == v.dtype and k.device == v.device == dev, (k.shape, v.shape)
+    assert k.shape == v.shape == (B, Hkv, n, D) and k.dtype is v.dtype and k.device == v.device == dev, (k.shape, v.shape)
+    assert k.stride(-1) == 1 and v.stride(-1) == 1
     code = _code(k)
     if B == 0 or n == 0:
         return k, v
-    assert k.stride(-1) == 1 and v.stride(-1) == 1
+    args = L.KV8_READ.pack(*head, k.data_ptr(), v.data_ptr(), n_dev, *k.stride()[:3], *v.stride()[:3],
+                           start, n, n_b, code)
     with _device(dev):
-        rc = L.lib().da_kv8_read(
-            cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cs,
-            cap, B, Hkv, D, start, n, _ptr(n_keys), n_b,
-            k.data_ptr(), _s3(k, 0, 1, 2), v.data_ptr(), _s3(v, 0, 1, 2), code, _stream(dev))
+        rc = L.lib().da_kv8_read(args, _stream(dev))
     L.check(rc, "da_kv8_read")
     return k, v
 
@@ -726,38 +737,41 @@ def kv8_attention(q: torch.Tensor, cache: KV8, *, n_keys, window: int = 0, sink:
 
     n_keys: an int, or an int32 device tensor of one entry or one per sequence,
     read when the kernels run (a recorded call serves every length; counts are
-    clamped to the capacity). add: a tensor like q; rnd(rnd(row) + add)."""
-    B, Hkv, cap, D, cs = _kv8(cache)
-    assert q.dim() == 4 and q.shape[0] == B and q.shape[3] == D, (q.shape, cache.k.shape)
-    H, s = q.shape[1], q.shape[2]
-    assert H % Hkv == 0 and H > 0, (H, Hkv)
-    dev = _on_gpu(q, *cache)
+    clamped to the capacity). add: a tensor like q; rnd(rnd(row) + add). A new
+    result has q's strides where q is dense."""
+    dev = q.device
+    head = _kv8(cache, dev)
+    B, Hkv, cap, D = head[12:]
+    Bq, H, s, Dq = q.shape
+    assert Bq == B and Dq == D and H > 0 and H % Hkv == 0, (q.shape, cache.k.shape)
     code = _code(q)
+    assert dev.type == "cuda", "delta-attention kernels need GPU tensors"
     q = _ready(q)
     if out is None:
-        out = torch.empty((B, H, s, D), device=dev, dtype=q.dtype)
-    assert out.shape == (B, H, s, D) and out.dtype == q.dtype and out.stride(-1) == 1 and out.device == dev
-    w, sk = max(int(window), 0), max(int(sink), 0)
-    nk_dev, nk_b, n = None, 0, cap
+        out = torch.empty_like(q)
+    else:
+        assert out.shape == q.shape and out.dtype is q.dtype and out.stride(-1) == 1 and out.device == dev
+    window, sink = min(max(int(window), 0), cap), min(max(int(sink), 0), cap)
+    n_dev, n_b, n = 0, False, cap
     if isinstance(n_keys, torch.Tensor):
-        nk_b, nk_dev = _per_seq(n_keys, B, torch.int32, dev, "n_keys"), n_keys.data_ptr()
+        n_b, n_dev = _per_seq(n_keys, B, _I32, dev, "n_keys"), n_keys.data_ptr()
     else:
         n = int(n_keys)
         assert 0 <= n <= cap, f"{n} keys in a cache of {cap}"
+    a_ptr, a_str = 0, (0, 0, 0)
     if add is not None:
-        assert add.shape == q.shape and add.dtype == q.dtype and add.device == dev
+        assert add.shape == q.shape and add.dtype is q.dtype and add.device == dev
         add = _ready(add)
+        a_ptr, a_str = add.data_ptr(), add.stride()[:3]
     if B == 0 or s == 0:
         return out
-    nbytes = _kv8_ws_bytes(B, H, Hkv, s, D, n, min(w, cap), min(sk, cap))
+    nbytes = _kv8_ws_bytes(B, H, Hkv, s, D, n, window, sink)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    args = L.KV8_ATTN.pack(*head, q.data_ptr(), out.data_ptr(), a_ptr, n_dev, 0 if ws is None else ws.data_ptr(),
+                           nbytes, *q.stride()[:3], *out.stride()[:3], *a_str, H, s, n_b, n, window, sink,
+                           code, sm_scale)
     with _device(dev):
-        rc = L.lib().da_kv8_attn_fwd(
-            q.data_ptr(), _s3(q, 0, 1, 2), cache.k.data_ptr(), cache.v.data_ptr(),
-            cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cs, cap,
-            out.data_ptr(), _s3(out, 0, 1, 2), B, H, Hkv, s, D, nk_dev, nk_b, n, min(w, cap), min(sk, cap),
-            float(sm_scale), _ptr(add), None if add is None else _s3(add, 0, 1, 2),
-            _ptr(ws), nbytes, code, _stream(dev))
+        rc = L.lib().da_kv8_attn_fwd(args, _stream(dev))
     L.check(rc, "da_kv8_attn_fwd")
     return out
 

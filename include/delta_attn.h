@@ -263,19 +263,25 @@ int da_decode_attn_fwd_dev_noalloc(const void* q, const void* k, const void* v, 
  * The 8-bit key/value cache. One layer's cache holds e4m3 codes (OCP e4m3fn)
  * with a power-of-two fp32 scale per block of 64 tokens, kv head and tensor;
  * value = code * scale:
- *   k_codes  [B, Hkv, cap, D] bytes (a token's D codes contiguous, tokens D apart)
- *   v_codes  [B, Hkv, cap / 64, D, 64] bytes (contiguous from the block on): a
+ *   k        [B, Hkv, cap, D] bytes (a token's D codes contiguous, tokens D apart)
+ *   v        [B, Hkv, cap / 64, D, 64] bytes (contiguous from the block on): a
  *            block's 64 tokens stand together for each column, token
  *            16 t + 4 g + r (t, g, r in 0..3) at place 16 g + 4 t + r
  *   k_scale, v_scale  [B, Hkv, cap / 64] fp32 (blocks contiguous), 2^e with e in
  *            [-117, 120]
- *   c_str    {k batch, k head, v batch, v head (bytes, multiples of 16), k_scale
- *            batch, head, v_scale batch, head (elements)}
- *   cap      tokens per sequence, a multiple of 64 up to 2^30.
- * D is 32, 64, 128 or 256; `dtype` is that of the 16-bit tensors beside the
- * cache. Rows of a cache that were not written may hold any bytes: they reach no
+ * Strides are {batch, head}: bytes for the codes (multiples of 16), elements for
+ * the scales. cap is a multiple of 64 up to 2^30; D is 32, 64, 128 or 256.
+ * Rows of a cache that were not written may hold any bytes: they reach no
  * result. No counterpart in the reference (its cache is the model's dtype).
+ * The calls take their arguments as one struct, which they read before they
+ * return; `dtype` is that of the 16-bit tensors beside the cache.
  */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale;
+  int64_t k_str[2], v_str[2], k_scale_str[2], v_scale_str[2];
+  int32_t B, Hkv, cap, D;
+} da_kv8_cache;
 
 /*
  * Appends to an 8-bit cache: token t of k / v [B, S, Hkv, D] (strides {batch,
@@ -292,26 +298,30 @@ int da_decode_attn_fwd_dev_noalloc(const void* q, const void* k, const void* v, 
  * block was written. A sequence whose rows do not fit ([pos, pos + count) not in
  * [0, cap)) keeps its cache unchanged (DA_ERR_INVALID_ARG for a host pos).
  */
-int da_kv8_write(const void* k, const int64_t k_str[3], const void* v, const int64_t v_str[3],
-                 int B, int S, int Hkv, int D,
-                 void* k_codes, void* v_codes, float* k_scale, float* v_scale,
-                 const int64_t c_str[8], int cap,
-                 const int64_t* pos_dev, int pos_per_seq, int64_t pos,
-                 const int32_t* counts_dev, int counts_per_seq, int dtype, void* stream);
+typedef struct {
+  da_kv8_cache cache;
+  const void *k, *v;
+  const int64_t* pos_dev;
+  const int32_t* counts_dev;
+  int64_t k_str[3], v_str[3], pos;
+  int32_t S, pos_per_seq, counts_per_seq, dtype;
+} da_kv8_write_args;
+int da_kv8_write(const da_kv8_write_args* args, void* stream);
 
 /*
- * Rows start .. start + n - 1 of an 8-bit cache in `dtype`: k_out / v_out
- * [B, Hkv, n, D] (strides {batch, head, row}) = code * scale, one rounding
- * (exact in bf16), finite values beyond the type's largest one saturated. With
- * n_keys_dev (int32, one entry or one per sequence) rows at or past a sequence's
- * count are zero.
+ * Rows start .. start + n - 1 of an 8-bit cache in `dtype`: k / v [B, Hkv, n, D]
+ * (strides {batch, head, row}) = code * scale, one rounding (exact in bf16),
+ * finite values beyond the type's largest one saturated. With n_keys_dev (int32,
+ * one entry or one per sequence) rows at or past a sequence's count are zero.
  */
-int da_kv8_read(const void* k_codes, const void* v_codes, const float* k_scale,
-                const float* v_scale, const int64_t c_str[8], int cap,
-                int B, int Hkv, int D, int start, int n,
-                const int32_t* n_keys_dev, int n_keys_per_seq,
-                void* k_out, const int64_t ko_str[3], void* v_out, const int64_t vo_str[3],
-                int dtype, void* stream);
+typedef struct {
+  da_kv8_cache cache;
+  void *k, *v;
+  const int32_t* n_keys_dev;
+  int64_t k_str[3], v_str[3];
+  int32_t start, n, n_keys_per_seq, dtype;
+} da_kv8_read_args;
+int da_kv8_read(const da_kv8_read_args* args, void* stream);
 
 /*
  * Attention of the last s rows of each sequence over its 8-bit cache: with n
@@ -325,16 +335,21 @@ int da_kv8_read(const void* k_codes, const void* v_codes, const float* k_scale,
  * Workspace: da_kv8_attn_workspace_bytes(..., max_keys = cap with a device
  * count, else n_keys) bytes, which may be 0.
  */
+typedef struct {
+  da_kv8_cache cache;
+  const void* q;
+  void* out;
+  const void* addend;
+  const int32_t* n_keys_dev;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_str[3], o_str[3], add_str[3];
+  int32_t Hq, s, n_keys_per_seq, n_keys, window, sink, dtype;
+  float sm_scale;
+} da_kv8_attn_args;
 size_t da_kv8_attn_workspace_bytes(int B, int Hq, int Hkv, int s, int D, int max_keys,
                                    int window, int sink);
-int da_kv8_attn_fwd(const void* q, const int64_t q_str[3], const void* k_codes,
-                    const void* v_codes, const float* k_scale, const float* v_scale,
-                    const int64_t c_str[8], int cap, void* out, const int64_t o_str[3],
-                    int B, int Hq, int Hkv, int s, int D,
-                    const int32_t* n_keys_dev, int n_keys_per_seq, int n_keys,
-                    int window, int sink, float sm_scale,
-                    const void* addend, const int64_t add_str[3],
-                    void* workspace, size_t workspace_bytes, int dtype, void* stream);
+int da_kv8_attn_fwd(const da_kv8_attn_args* args, void* stream);
 
 /*
  * Kernel (3): delta broadcast-add over rows 0 .. s_p-1.

@@ -1,7 +1,6 @@
 """CPU checks of the 8-bit key/value cache: its oracle against torch's e4m3
 casts, its argument checks at the C entry points and in ops, its layout."""
 
-import ctypes
 import os
 
 import numpy as np
@@ -67,10 +66,10 @@ def test_empty_cache_and_its_slices():
     c = ops.kv8_empty(2, 3, 100, 64, "cpu")
     assert c.k.shape == (2, 3, 128, 64) and c.v.shape == (2, 3, 2, 64, 64)
     assert c.k_scale.shape == c.v_scale.shape == (2, 3, 2) and (c.k_scale == 2.0 ** -117).all()
-    B, H, cap, D, st = ops._kv8(c)
-    assert (B, H, cap, D) == (2, 3, 128, 64) and list(st)[:2] == [3 * 128 * 64, 128 * 64]
+    head = ops._kv8(c, c.k.device)
+    assert head[12:] == (2, 3, 128, 64) and head[4:6] == (3 * 128 * 64, 128 * 64)
     part = ops.KV8(*(t[:, 1:] for t in c))
-    assert ops._kv8(part)[:4] == (2, 2, 128, 64)
+    assert ops._kv8(part, c.k.device)[12:] == (2, 2, 128, 64)
     for bad in (dict(D=96), dict(max_len=0), dict(max_len=(1 << 30) + 1), dict(Hkv=0)):
         with pytest.raises(AssertionError):
             ops.kv8_empty(**{**dict(B=1, Hkv=1, max_len=64, D=64, device="cpu"), **bad})
@@ -83,7 +82,7 @@ def test_ops_refuse_caches_that_are_not_laid_out_so():
                 c._replace(k=c.k.view(torch.uint8)), c._replace(v_scale=c.v_scale.double()),
                 c._replace(k_scale=c.k_scale[..., 0:1].expand(1, 2, 2))):
         with pytest.raises(AssertionError):
-            ops._kv8(bad)
+            ops._kv8(bad, c.k.device)
 
 
 def test_ops_refuse_arguments_on_the_cpu():
@@ -104,40 +103,47 @@ def test_ops_refuse_arguments_on_the_cpu():
         ops.kv8_read(c, 100, 29)
 
 
-def _write(lib, **kw):
-    a = dict(k=16, v=16, ks=(3 * 128, 128, 64), vs=(3 * 128, 128, 64), B=1, S=3, Hkv=2, D=64, kc=16, vc=16,
-             sk=16, sv=16, cs=(128 * 128, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2), cap=128, pos=0, pos_dev=0,
-             counts=0, dtype=L.DA_BF16)
-    a.update(kw)
-    p = ctypes.c_void_p
-    return lib.da_kv8_write(p(a["k"]), L.strides3(*a["ks"]), p(a["v"]), L.strides3(*a["vs"]), a["B"], a["S"],
-                            a["Hkv"], a["D"], p(a["kc"]), p(a["vc"]), p(a["sk"]), p(a["sv"]), L.I64x8(*a["cs"]),
-                            a["cap"], p(a["pos_dev"]), 0, a["pos"], p(a["counts"]), 0, a["dtype"], None)
+CACHE = dict(kc=16, vc=16, sk=16, sv=16, cs=(128 * 128, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2), B=1, Hkv=2,
+             cap=128, D=64)
+
+
+def _head(a):
+    return (a["kc"], a["vc"], a["sk"], a["sv"], *a["cs"], a["B"], a["Hkv"], a["cap"], a["D"])
+
+
+def test_struct_sizes():
+    """The packed structs are the header's: fields in order, native alignment."""
+    assert L.KV8_WRITE.size == 112 + 4 * 8 + 7 * 8 + 16
+    assert L.KV8_READ.size == 112 + 3 * 8 + 6 * 8 + 16
+    assert L.KV8_ATTN.size == 112 + 5 * 8 + 10 * 8 + 32
 
 
 def test_c_write_refusals(lib):
-    assert _write(lib, dtype=5) == L.DA_ERR_DTYPE
-    assert _write(lib, D=96) == L.DA_ERR_HEAD_DIM
-    for bad in (dict(cap=100), dict(cap=-64), dict(cap=(1 << 30) + 64), dict(Hkv=0), dict(B=-1), dict(S=-1),
+    def call(**kw):
+        a = dict(CACHE, k=16, v=16, ks=(3 * 128, 128, 64), vs=(3 * 128, 128, 64), S=3, pos=0, pos_dev=0, counts=0,
+                 dtype=L.DA_BF16)
+        a.update(kw)
+        return lib.da_kv8_write(L.KV8_WRITE.pack(*_head(a), a["k"], a["v"], a["pos_dev"], a["counts"], *a["ks"],
+                                                 *a["vs"], a["pos"], a["S"], 0, 0, a["dtype"]), None)
+    assert call(dtype=5) == L.DA_ERR_DTYPE
+    assert call(D=96) == L.DA_ERR_HEAD_DIM
+    for bad in (dict(cap=100), dict(cap=0), dict(cap=-64), dict(cap=(1 << 30) + 64), dict(Hkv=0), dict(B=-1), dict(S=-1),
                 dict(k=0), dict(v=0), dict(kc=0), dict(vc=0), dict(sk=0), dict(sv=0), dict(pos=-1), dict(pos=126),
-                dict(S=129), dict(pos=2 ** 62)):
-        assert _write(lib, **bad) == L.DA_ERR_INVALID_ARG, bad
+                dict(S=129), dict(pos=2 ** 62), dict(Hkv=2 ** 30)):
+        assert call(**bad) == L.DA_ERR_INVALID_ARG, bad
     for bad in (dict(k=24), dict(vc=24), dict(sk=18), dict(ks=(3 * 128, 129, 64)), dict(pos_dev=20), dict(counts=18),
                 dict(cs=(128 * 128 + 8, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2))):
-        assert _write(lib, **bad) == L.DA_ERR_ALIGNMENT, bad
-    assert _write(lib, S=0) == L.DA_OK and _write(lib, B=0) == L.DA_OK       # nothing launched
+        assert call(**bad) == L.DA_ERR_ALIGNMENT, bad
+    assert call(S=0) == L.DA_OK and call(B=0) == L.DA_OK       # nothing launched
+    assert lib.da_kv8_write(None, None) == L.DA_ERR_INVALID_ARG
 
 
 def test_c_read_refusals(lib):
     def call(**kw):
-        a = dict(kc=16, vc=16, sk=16, sv=16, cap=128, B=1, Hkv=2, D=64, start=0, n=5, nk=0, ko=16, vo=16,
-                 st=(2 * 5 * 64, 5 * 64, 64), dtype=L.DA_FP16)
+        a = dict(CACHE, start=0, n=5, nk=0, ko=16, vo=16, st=(2 * 5 * 64, 5 * 64, 64), dtype=L.DA_FP16)
         a.update(kw)
-        p = ctypes.c_void_p
-        return lib.da_kv8_read(p(a["kc"]), p(a["vc"]), p(a["sk"]), p(a["sv"]),
-                               L.I64x8(128 * 128, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2), a["cap"], a["B"],
-                               a["Hkv"], a["D"], a["start"], a["n"], p(a["nk"]), 0, p(a["ko"]),
-                               L.strides3(*a["st"]), p(a["vo"]), L.strides3(*a["st"]), a["dtype"], None)
+        return lib.da_kv8_read(L.KV8_READ.pack(*_head(a), a["ko"], a["vo"], a["nk"], *a["st"], *a["st"], a["start"],
+                                               a["n"], 0, a["dtype"]), None)
     assert call(dtype=2) == L.DA_ERR_DTYPE and call(D=48) == L.DA_ERR_HEAD_DIM
     for bad in (dict(start=-1), dict(n=-1), dict(start=124), dict(start=2 ** 31 - 1, n=2 ** 31 - 1), dict(ko=0),
                 dict(kc=0), dict(cap=65)):
@@ -145,6 +151,7 @@ def test_c_read_refusals(lib):
     for bad in (dict(ko=24), dict(st=(640, 321, 64)), dict(nk=2)):
         assert call(**bad) == L.DA_ERR_ALIGNMENT, bad
     assert call(n=0) == L.DA_OK and call(B=0) == L.DA_OK
+    assert lib.da_kv8_read(None, None) == L.DA_ERR_INVALID_ARG
 
 
 def test_c_rows_refusals_and_workspace(lib):
@@ -156,21 +163,20 @@ def test_c_rows_refusals_and_workspace(lib):
     assert ws(1, 32, 8, 0, 128, 131072, 0, 0) == 0 and ws(1, 32, 8, 1, 128, -1, 0, 0) == 0
 
     def call(**kw):
-        a = dict(q=16, qs=(8 * 64, 64, 64), kc=16, vc=16, sk=16, sv=16, cap=1024, out=16, B=1, Hq=8, Hkv=2, s=1, D=64,
-                 nk=0, n=1000, window=0, sink=0, add=0, ws=16, nb=1 << 30, dtype=L.DA_BF16)
+        a = dict(CACHE, cap=1024, q=16, qs=(8 * 64, 64, 64), out=16, Hq=8, s=1, nk=0, n=1000, window=0, sink=0, add=0,
+                 as_=(8, 8, 8), ws=16, nb=1 << 30, dtype=L.DA_BF16)
         a.update(kw)
-        p = ctypes.c_void_p
-        return lib.da_kv8_attn_fwd(p(a["q"]), L.strides3(*a["qs"]), p(a["kc"]), p(a["vc"]), p(a["sk"]), p(a["sv"]),
-                                   L.I64x8(128 * 1024, 64 * 1024, 128 * 1024, 64 * 1024, 32, 16, 32, 16), a["cap"],
-                                   p(a["out"]), L.strides3(8 * 64, 64, 64), a["B"], a["Hq"], a["Hkv"], a["s"], a["D"],
-                                   p(a["nk"]), 0, a["n"], a["window"], a["sink"], 0.1, p(a["add"]), None, p(a["ws"]),
-                                   a["nb"], a["dtype"], None)
+        return lib.da_kv8_attn_fwd(L.KV8_ATTN.pack(*_head(a), a["q"], a["out"], a["add"], a["nk"], a["ws"], a["nb"],
+                                                   *a["qs"], 8 * 64, 64, 64, *a["as_"], a["Hq"], a["s"], 0, a["n"],
+                                                   a["window"], a["sink"], a["dtype"], 0.1), None)
     assert call(dtype=3) == L.DA_ERR_DTYPE and call(D=512) == L.DA_ERR_HEAD_DIM
     for bad in (dict(Hq=9), dict(Hq=0), dict(s=-1), dict(window=-1), dict(sink=-1), dict(n=-1), dict(n=1025), dict(q=0),
-                dict(out=0), dict(kc=0), dict(cap=1000), dict(add=16), dict(s=1 << 30)):
+                dict(out=0), dict(kc=0), dict(cap=1000), dict(s=1 << 30)):
         assert call(**bad) == L.DA_ERR_INVALID_ARG, bad
     need = ws(1, 8, 2, 1, 64, 1000, 0, 0)
     assert need > 0 and call(nb=need - 1) == L.DA_ERR_WORKSPACE and call(ws=0) == L.DA_ERR_WORKSPACE
-    for bad in (dict(q=24), dict(out=24), dict(qs=(512, 65, 64)), dict(nk=18), dict(ws=24)):
+    for bad in (dict(q=24), dict(out=24), dict(qs=(512, 65, 64)), dict(nk=18), dict(ws=24), dict(add=24),
+                dict(add=16, as_=(8, 8, 4))):
         assert call(**bad) == L.DA_ERR_ALIGNMENT, bad
     assert call(s=0) == L.DA_OK and call(B=0) == L.DA_OK
+    assert lib.da_kv8_attn_fwd(None, None) == L.DA_ERR_INVALID_ARG
