@@ -509,8 +509,11 @@ __host__ __device__ __forceinline__ int item_budget(int blocks, int slots, const
   return slots * (int)(fdiv(blocks + round.d - 1, round));
 }
 
+// Within a sequence the items lie by kv head, split, row tile: the tiles of one
+// split, which read the same codes, are next to each other.
 struct Place {
-  int b, unit, split, n_split, chunk, slot0;   // unit: kv head * n_rt + row tile; slot0: its first item
+  int b, head, tile, split, n_split, chunk;
+  int slot;                 // the item, or a tile's first one (the others n_rt apart)
 };
 
 // Inclusive sum over the lanes up to this one.
@@ -524,71 +527,84 @@ __device__ __forceinline__ int scan64(int x) {
   return x;
 }
 
-// ITEM: `i` counts items, otherwise (sequence, unit) pairs.
+// locate() among sequences of different lengths: 64 sequences to a lane each;
+// those of the first KEPT rounds stay in registers.
+template <bool ITEM, int KEPT>
+__device__ __forceinline__ bool among(const RowsArgs& a, int i, Place& p, int& rest, int& first) {
+  const int lane = threadIdx.x % 64, units = a.units.d, nu = KEPT == 1 ? 1 : (a.B + 63) / 64;
+  auto load = [&](int u) __attribute__((always_inline)) {
+    const int b = u * 64 + lane;
+    return b < a.B ? blocks_of(a, keys_of(a, b)).n : -1;
+  };
+  int kept[KEPT];
+#pragma unroll
+  for (int u = 0; u < KEPT; ++u) kept[u] = u < nu ? load(u) : -1;
+  auto blocks = [&](int u) __attribute__((always_inline)) {   // -1 past the last sequence
+    if constexpr (KEPT == 1) return kept[0];
+    else return u == 0 ? kept[0] : u == 1 ? kept[1] : u == 2 ? kept[2] : u == 3 ? kept[3] : load(u);
+  };
+  auto items = [&](int u) __attribute__((always_inline)) {
+    const int n = blocks(u);
+    return n < 0 ? 0 : max((n + p.chunk - 1) / p.chunk, 1);
+  };
+  int total = 0;
+  for (int u = 0; u < nu; ++u) total += __builtin_amdgcn_readlane(scan64(max(blocks(u), 0)), 63);
+  const int budget = item_budget(total * units, a.slots, a.round);
+  p.chunk = max((total * units + budget - 1) / max(budget, 1), WAVES);
+  // the sequences' last items are short: longer ones, until all fit the budget
+  for (int tries = 0; tries < 4 && a.B * units < budget; ++tries) {
+    int all = 0;
+    for (int u = 0; u < nu; ++u) all += __builtin_amdgcn_readlane(scan64(items(u)), 63) * units;
+    if (all <= budget) break;
+    p.chunk += max((p.chunk * (all - budget)) / budget, 1);
+  }
+  first = 0;
+  for (int u = 0, have = i; u < nu; ++u) {
+    const int mine = items(u), upto = scan64(mine);
+    const uint64_t past = __ballot(mine > 0 && (ITEM ? upto : lane + 1) * units > have);
+    if (past) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      p.n_split = __builtin_amdgcn_readlane(mine, l);
+      const int before = (__builtin_amdgcn_readlane(upto, l) - p.n_split) * units;
+      p.b = u * 64 + l;
+      first += before;
+      rest = have - (ITEM ? before : l * units);
+      return true;
+    }
+    const int here = __builtin_amdgcn_readlane(upto, 63) * units;
+    first += here;
+    have -= ITEM ? here : 64 * units;
+  }
+  return false;
+}
+
+// The place of item `i`, or (ITEM false) of (sequence, kv head, row tile) `i`;
+// false past the last.
 template <bool ITEM>
 __device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
   const int units = a.units.d;
+  int rest, first;          // `i` and the first item, within the sequence
   if (a.B == 1 || !a.n_dev || a.n_step == 0) {     // one count for all sequences
     const int n = blocks_of(a, __builtin_amdgcn_readfirstlane(keys_of(a, 0))).n;
     const int pairs = a.B * units;
     const int splits = max(item_budget(n * pairs, a.slots, a.round) / pairs, 1);
     p.chunk = max((n + splits - 1) / splits, WAVES);
     p.n_split = max((n + p.chunk - 1) / p.chunk, 1);
-    const int pair = ITEM ? i / p.n_split : i;
-    p.split = ITEM ? i - pair * p.n_split : 0;
-    p.b = fdiv(pair, a.units);
-    p.unit = pair - p.b * units;
-    p.slot0 = pair * p.n_split;
-    return p.b < a.B;
+    const int per_seq = ITEM ? units * p.n_split : units;
+    p.b = a.B == 1 ? 0 : i / per_seq;
+    rest = i - p.b * per_seq;
+    if (p.b >= a.B || rest >= per_seq) return false;
+    first = p.b * units * p.n_split;
+  } else {
+    // (a separate copy for up to 64 sequences, one to a lane)
+    if (!(a.B <= 64 ? among<ITEM, 1>(a, i, p, rest, first) : among<ITEM, 4>(a, i, p, rest, first))) return false;
   }
-  const int lane = threadIdx.x % 64;
-  // the counts of the first 64 sequences stay in a register
-  const int n0 = lane < a.B ? blocks_of(a, keys_of(a, lane)).n : 0;
-  int total = __builtin_amdgcn_readlane(scan64(n0), 63);
-  for (int b0 = 64; b0 < a.B; b0 += 64) {
-    const int n = b0 + lane < a.B ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
-    total += __builtin_amdgcn_readlane(scan64(n), 63);
-  }
-  const int budget = item_budget(total * units, a.slots, a.round);
-  p.chunk = max((total * units + budget - 1) / max(budget, 1), WAVES);
-  // the sequences' last items are short: longer ones, until all fit the budget
-  for (int tries = 0; tries < 4; ++tries) {
-    int items = 0;
-    for (int b0 = 0; b0 < a.B; b0 += 64) {
-      const bool in = b0 + lane < a.B;
-      const int n = b0 == 0 ? n0 : in ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
-      items += __builtin_amdgcn_readlane(scan64(in ? max((n + p.chunk - 1) / p.chunk, 1) : 0), 63) * units;
-    }
-    if (items <= budget || a.B * units >= budget) break;
-    p.chunk += max((p.chunk * (items - budget)) / budget, 1);
-  }
-  int before = 0;           // items of the sequences before
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const bool in = b0 + lane < a.B;
-    const int n = b0 == 0 ? n0 : in ? blocks_of(a, keys_of(a, b0 + lane)).n : 0;
-    const int mine = in ? max((n + p.chunk - 1) / p.chunk, 1) : 0;
-    const int upto = scan64(mine);
-    const int have = ITEM ? i - before : i - b0 * units;     // in this batch of sequences
-    const uint64_t past = __ballot(in && (ITEM ? upto : lane + 1) * units > have);
-    if (past) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      p.n_split = __builtin_amdgcn_readlane(mine, l);
-      const int start = (__builtin_amdgcn_readlane(upto, l) - p.n_split) * units;
-      p.b = b0 + l;
-      if (ITEM) {
-        const int rest = have - start;
-        p.unit = rest / p.n_split;
-        p.split = rest - p.unit * p.n_split;
-      } else {
-        p.unit = have - l * units;
-        p.split = 0;
-      }
-      p.slot0 = before + start + p.unit * p.n_split;
-      return true;
-    }
-    before += __builtin_amdgcn_readlane(upto, 63) * units;
-  }
-  return false;
+  const int group = fdiv(rest, a.tiles);            // (kv head, split), or the kv head
+  p.tile = rest - group * a.n_rt;
+  p.head = ITEM ? group / p.n_split : group;
+  p.split = ITEM ? group - p.head * p.n_split : 0;
+  p.slot = first + (p.head * p.n_split + p.split) * a.n_rt + p.tile;
+  return true;
 }
 
 __device__ __forceinline__ float group_max(float x) {   // over the four lanes of one row
@@ -643,17 +659,25 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
   constexpr int DT = D / 16;
   using P = Dot<_Float16>;
   Place p;
-  if (!locate<true>(a, blockIdx.x, p)) return;
+  // The row tiles of one split run on one XCD (workgroup x runs on XCD x % 8):
+  // its L2 holds the codes that they share.
+  int item = blockIdx.x;
+  if (a.n_rt > 1) {
+    const int q = item / 8, k = fdiv(q, a.tiles);
+    item = (k * 8 + item % 8) * a.n_rt + q - k * a.n_rt;
+  }
+  if (!locate<true>(a, item, p)) return;
   // (all of it is the wave's: scalar registers)
   p.b = __builtin_amdgcn_readfirstlane(p.b);
-  p.unit = __builtin_amdgcn_readfirstlane(p.unit);
+  p.head = __builtin_amdgcn_readfirstlane(p.head);
+  p.tile = __builtin_amdgcn_readfirstlane(p.tile);
   p.split = __builtin_amdgcn_readfirstlane(p.split);
   p.chunk = __builtin_amdgcn_readfirstlane(p.chunk);
   p.n_split = __builtin_amdgcn_readfirstlane(p.n_split);
-  p.slot0 = __builtin_amdgcn_readfirstlane(p.slot0);
+  p.slot = __builtin_amdgcn_readfirstlane(p.slot);
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int c = lane % 16, g = lane / 16;
-  const int b = p.b, hk = fdiv(p.unit, a.tiles), m0 = (p.unit - hk * a.n_rt) * a.rows;
+  const int b = p.b, hk = p.head, m0 = p.tile * a.rows;
   const int n = __builtin_amdgcn_readfirstlane(keys_of(a, b));
   const Blocks list = blocks_of(a, n);
   const int n_rows = min(a.rows, a.s * a.G - m0);
@@ -700,7 +724,9 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
   // A block's loads; none are made (zeros) where there is no block. Non-temporal:
   // a decode step's other layers and weights pass between two reads of a cache.
   // Caches of 2 GB together, 4 to 268 MB a call: 9.3 -> 8.5 to 54.2 -> 48.0 us; a
-  // single cache of 34 to 268 MB read again and again: up to 5 % slower.
+  // single cache of 34 to 268 MB read again and again: up to 5 % slower. (The
+  // most rows a wave holds may be one of several row tiles, which share codes.)
+  constexpr int STREAM = MT == (D == 256 ? 2 : 4) ? 0 : 2;
   const uint32_t k_off = c * D + g * (D >= 64 ? 16 : 8), v_off = c * KB + g * 16;
   auto load_k = [&](int blk, bool any) __attribute__((always_inline)) {
     const auto r = make_rsrc(kc + (int64_t)blk * (KB * D), any ? KB * D : 0);
@@ -709,9 +735,9 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
 #pragma unroll
       for (int w = 0; w < KW; ++w) {
         if constexpr (D >= 64) {
-          kf[t][w] = __builtin_amdgcn_raw_buffer_load_b128(r, k_off, t * 16 * D + w * 64, 2);
+          kf[t][w] = __builtin_amdgcn_raw_buffer_load_b128(r, k_off, t * 16 * D + w * 64, STREAM);
         } else {
-          const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(r, k_off, t * 16 * D, 2);
+          const u32x2 y = __builtin_amdgcn_raw_buffer_load_b64(r, k_off, t * 16 * D, STREAM);
           kf[t][w] = (u32x4){y[0], y[1], 0, 0};
         }
       }
@@ -720,7 +746,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
   auto load_v = [&](int blk, bool any) __attribute__((always_inline)) {
     const auto r = make_rsrc(vc + (int64_t)blk * (KB * D), any ? KB * D : 0);
 #pragma unroll
-    for (int t = 0; t < DT; ++t) vf[t] = __builtin_amdgcn_raw_buffer_load_b128(r, v_off, t * 16 * KB, 2);
+    for (int t = 0; t < DT; ++t) vf[t] = __builtin_amdgcn_raw_buffer_load_b128(r, v_off, t * 16 * KB, STREAM);
     sv = vsc[blk];
   };
   int blk = x < end ? list.at(x) : 0;
@@ -869,7 +895,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
   constexpr int LD = D + 4;                    // row pitch: the 16 rows of a column spread over the banks
   __shared__ float s_o[WAVES][16][LD];
   __shared__ float s_m[WAVES][16], s_l[WAVES][16];
-  float* part = a.part + (int64_t)(p.slot0 + p.split) * a.pitch;
+  float* part = a.part + (int64_t)p.slot * a.pitch;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     if (mt > 0) __syncthreads();
@@ -922,11 +948,12 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
   const int row = blockIdx.y;
   Place p;
   if (!locate<false>(a, blockIdx.x, p) || p.n_split == 1) return;
-  const int hk = fdiv(p.unit, a.tiles), m = (p.unit - hk * a.n_rt) * a.rows + row;
+  const int hk = p.head, m = p.tile * a.rows + row;
   if (m >= a.s * a.G) return;
   const int qi = fdiv(m, a.heads);
   const int t = threadIdx.x % CT, sg = threadIdx.x / CT;
-  const float* part = a.part + p.slot0 * a.pitch;
+  const float* part = a.part + (int64_t)p.slot * a.pitch;
+  const int64_t pitch = a.pitch * a.n_rt;
   float M = NO_KEYS, L = 0.f;
   f32x4 o = {0, 0, 0, 0};
   constexpr int U = 4;                         // items whose loads are in flight together
@@ -936,7 +963,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int i = min(i0 + u * SG, p.n_split - 1);
-      const float* src = part + i * a.pitch;
+      const float* src = part + i * pitch;
       mi[u] = src[a.rows * D + row];
       li[u] = src[a.rows * (D + 1) + row];
       y[u] = *(const f32x4*)(src + row * D + t * 4);
@@ -1035,7 +1062,9 @@ int take_cache(Cache& c, const da_kv8_cache& x, int dtype) {
 
 template <typename T, int D>
 void launch_rows(const RowsArgs& a, const RowsPlan& p, hipStream_t st) {
-  const dim3 grid((unsigned)p.items), block(64 * WAVES);
+  // (with several row tiles a multiple of 8 of them, as the items are dealt to the XCDs)
+  const int64_t group = p.n_rt > 1 ? 8 * (int64_t)p.n_rt : 1;
+  const dim3 grid((unsigned)((p.items + group - 1) / group * group)), block(64 * WAVES);
   if (p.mt == 1) {
     hipLaunchKernelGGL((kv8_rows_kernel<T, D, 1>), grid, block, 0, st, a);
   } else if (p.mt == 2) {
