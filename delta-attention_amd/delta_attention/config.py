@@ -4,7 +4,8 @@
 prefill path reads, plus `sink_tokens`: the reference hard-codes 1024 sink
 tokens (llama.py:415, config.py:128, flex_delta.py:101); here it is a knob
 with that default, and it is part of PIPELINE_FIELDS so that init code copies
-it onto model.config with the others.
+it onto model.config with the others. `kv_cache` (no counterpart there) names
+the decode cache: the model's dtype, or 8-bit codes.
 """
 
 from __future__ import annotations
@@ -52,6 +53,7 @@ class Config:
     drift_threshold: float = 0.95
     drift_k: float = 2.0
     gamma_dec_max: int = 128
+    kv_cache: str = "model"         # decode cache: model (16-bit) | fp8 (model.KVCache8)
 
     hip_attention_dense_layers: List[int] = field(default_factory=lambda: [0, 1, 2])
     hip_attention_last_dense: int = 64
@@ -78,7 +80,7 @@ PIPELINE_FIELDS = (
     "stride_policy", "gamma_min", "gamma_max", "adapt_chunk",
     "adapt_threshold", "stride_trigger", "adapt_k",
     "decode_mode", "gamma_dec", "refresh_policy", "drift_threshold",
-    "drift_k", "gamma_dec_max",
+    "drift_k", "gamma_dec_max", "kv_cache",
 )
 
 

@@ -16,7 +16,7 @@ pipeline knobs of `config.PIPELINE_FIELDS`.
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
 from torch import nn
@@ -25,6 +25,23 @@ from . import _lib as L
 from . import ops
 from .delta_kernel import attention as qsa_kernel
 from .timing import region
+
+
+class CachedKeys8(NamedTuple):
+    """What an 8-bit cache hands to the attention in the place of the key
+    states (the value states are then None): one layer's codes and scales, and
+    their key count (an int, or in recorded decode steps an int32 device
+    tensor)."""
+    cache: ops.KV8
+    n_keys: Union[int, torch.Tensor]
+
+
+# Rows (tokens times query heads per kv head) up to which a pass over an 8-bit
+# cache reads its codes (ops.kv8_attention); more rows read the keys back into
+# 16 bits first and run the rows kernel. 32 query heads over 32768 / 131072
+# keys: 256 rows 66 / 260 us so, 91 / 297 by the read-back; 512 rows 127 / 513
+# us, 117 / 412 by the read-back.
+DIRECT_ROWS8 = 256
 
 
 # per-device side streams of the adaptive path (LlamaAttention._side_stream)
@@ -415,12 +432,15 @@ class LlamaAttention(nn.Module):
             return self.delta_decode_forward(module, query_states, key_states, value_states,
                                              scaling=scaling, **kwargs)
         q, k, v = self._half(query_states, key_states, value_states)
-        n = k.size(2)
         if s == 1:
-            out = ops.decode_attention(q, k, v, window=0, sink=0, sm_scale=float(scaling),
-                                       n_keys=n_keys)
+            out = self._decode_row(q, k, v, scaling, n_keys=n_keys)
+        elif isinstance(k, CachedKeys8) and s * self.num_key_value_groups <= DIRECT_ROWS8:
+            out = ops.kv8_attention(q, k.cache, n_keys=k.n_keys, sm_scale=float(scaling))
         else:
             assert n_keys is None, "a device key count serves one-row decode steps"
+            if isinstance(k, CachedKeys8):
+                k, v = ops.kv8_read(k.cache, 0, k.n_keys, dtype=q.dtype)
+            n = k.size(2)
             mask = torch.arange(n - s, n, device=q.device, dtype=torch.int64)[None]
             out = qsa_kernel(q, k, v, mask, float(scaling))
         return out.transpose(1, 2).contiguous().to(query_states.dtype), None
@@ -428,15 +448,27 @@ class LlamaAttention(nn.Module):
     @staticmethod
     def _half(q, k, v):
         if q.dtype == torch.float32:
+            if isinstance(k, CachedKeys8):
+                return q.to(torch.bfloat16), k, v
             return q.to(torch.bfloat16), k.to(torch.bfloat16), v.to(torch.bfloat16)
         return q, k, v
 
-    def _decode_sparse_row(self, q, k, v, scaling, n_keys=None):
+    @staticmethod
+    def _decode_row(q, k, v, scaling, *, window: int = 0, sink: int = 0, n_keys=None, add=None):
+        """One decode row over the cache's keys, 16-bit or 8-bit (k then a
+        CachedKeys8)."""
+        if isinstance(k, CachedKeys8):
+            return ops.kv8_attention(q, k.cache, n_keys=k.n_keys, window=window, sink=sink,
+                                     sm_scale=float(scaling), add=add)
+        return ops.decode_attention(q, k, v, window=window, sink=sink, sm_scale=float(scaling),
+                                    n_keys=n_keys, add=add)
+
+    def _decode_sparse_row(self, q, k, v, scaling, n_keys=None, add=None):
         """One decode row over the sink tokens + the last sliding_window keys of
         the cache, softmax over exactly that set (llama.py:537-549; every key
         when the cache holds at most sink + window keys). GQA native."""
-        return ops.decode_attention(q, k, v, window=int(self.config.sliding_window),
-                                    sink=self._sink(), sm_scale=float(scaling), n_keys=n_keys)
+        return self._decode_row(q, k, v, scaling, window=int(self.config.sliding_window),
+                                sink=self._sink(), n_keys=n_keys, add=add)
 
     def _delta_decode_recorded(self, q, k, v, scaling, n_keys, anchor: bool, out_dtype):
         """delta_decode_forward's fixed-policy step in the form a recorded
@@ -448,16 +480,13 @@ class LlamaAttention(nn.Module):
             st = getattr(self, "_dec_static", None)
             assert st is not None, "a delta decode step needs an anchor step first"
             # the sparse row and the cached delta's add in one launch
-            out = ops.decode_attention(q, k, v, window=int(self.config.sliding_window),
-                                       sink=self._sink(), sm_scale=float(scaling),
-                                       n_keys=n_keys, add=st["last_delta"])
+            out = self._decode_sparse_row(q, k, v, scaling, n_keys, add=st["last_delta"])
             return out.transpose(1, 2).contiguous().to(out_dtype), None
         sparse_out = self._decode_sparse_row(q, k, v, scaling, n_keys)
         if self.config.decode_mode == "sparse":
             out = sparse_out
         elif anchor:
-            dense_out = ops.decode_attention(q, k, v, window=0, sink=0, sm_scale=float(scaling),
-                                             n_keys=n_keys)
+            dense_out = self._decode_row(q, k, v, scaling, n_keys=n_keys)
             st = getattr(self, "_dec_static", None)
             if st is None:    # first anchor step (run eagerly before any recording)
                 st = self._dec_static = {"last_delta": torch.empty_like(dense_out)}
@@ -493,8 +522,7 @@ class LlamaAttention(nn.Module):
         logging = bool(getattr(self.config, "log_drift", False))
         sparse = self._decode_sparse_row(q, k, v, scaling)
         anchor, since = rule.decide(state, sparse)
-        dense = (ops.decode_attention(q, k, v, window=0, sink=0, sm_scale=float(scaling))
-                 if anchor or logging else None)
+        dense = self._decode_row(q, k, v, scaling) if anchor or logging else None
         out = dense if anchor else sparse + state["last_delta"]
         dp.commit(state, anchor, since, sparse, dense, out)
         if logging:
@@ -561,7 +589,12 @@ class LlamaAttention(nn.Module):
         hidden_shape = (*input_shape, -1, self.head_dim)
         cos, sin = position_embeddings
         timer = kwargs.get("timer")
+        if (self.config._attn_implementation == "window" and getattr(past_key_value, "eight_bit", False)
+                and past_key_value.len[self.layer_idx] > 0):
+            raise NotImplementedError("the delta prefill takes a whole prompt, and the 8-bit cache already "
+                                      "holds tokens (continue with 'sdpa_rectangle')")
         static = (past_key_value is not None and getattr(past_key_value, "static", False)
+                  and not getattr(past_key_value, "eight_bit", False)
                   and hidden_states.dtype in (torch.bfloat16, torch.float16))
         query_states, key_states, value_states = self._qkv_rope(
             hidden_states, hidden_shape, cos, sin, timer, append=past_key_value if static else None)

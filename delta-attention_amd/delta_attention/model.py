@@ -22,7 +22,8 @@ import torch
 from torch import nn
 
 from . import ops
-from .llama import LlamaAttention, LlamaRMSNorm, fuse_linears, fused_params, rope_cos_sin
+from .llama import (CachedKeys8, LlamaAttention, LlamaRMSNorm, fuse_linears, fused_params,
+                    rope_cos_sin)
 from .timing import Timer, region as _region
 
 
@@ -66,6 +67,8 @@ class LlamaConfig:
     drift_threshold: float = 0.95
     drift_k: float = 2.0
     gamma_dec_max: int = 128
+    # decode cache: "model" (16-bit, the model's dtype) or "fp8" (KVCache8)
+    kv_cache: str = "model"
 
 
 class KVCache:
@@ -73,12 +76,13 @@ class KVCache:
     projection layout, so appending is one strided copy); `update` appends
     and returns [B, Hkv, len, D] views, which the kernels read in place."""
 
+    # whether keys and values are codes (the attention then gets CachedKeys8, and
+    # static appends run in a launch of their own, not in RoPE's)
+    eight_bit = False
+
     def __init__(self, config, batch: int, max_len: int, device, dtype):
-        shape = (batch, max_len, config.num_key_value_heads, config.head_dim)
-        n = config.num_hidden_layers
-        self.k = [torch.empty(shape, device=device, dtype=dtype) for _ in range(n)]
-        self.v = [torch.empty(shape, device=device, dtype=dtype) for _ in range(n)]
-        self.len = [0] * n
+        self._allocate(config, batch, max_len, device, dtype)
+        self.len = [0] * config.num_hidden_layers
         self.max_len = max_len
         # static mode (decode steps recorded in a HIP graph): the appended row
         # and the key count live on the device and advance there
@@ -86,6 +90,12 @@ class KVCache:
         self.pos = None        # int64 [1]: row of the next append
         self.n_keys = None     # int32 [1]: keys after that append
         self.anchor = False    # delta decode: whether the recorded step is an anchor step
+
+    def _allocate(self, config, batch, max_len, device, dtype):
+        shape = (batch, max_len, config.num_key_value_heads, config.head_dim)
+        n = config.num_hidden_layers
+        self.k = [torch.empty(shape, device=device, dtype=dtype) for _ in range(n)]
+        self.v = [torch.empty(shape, device=device, dtype=dtype) for _ in range(n)]
 
     def start_static(self):
         """Switch to device-side positions: one-token appends go to row
@@ -129,6 +139,51 @@ class KVCache:
 
     def seq_len(self) -> int:
         return self.len[0]
+
+
+class KVCache8(KVCache):
+    """The cache in 8 bits (ops.KV8 per layer): e4m3 codes with a power-of-two
+    scale per block of 64 tokens and head, half the memory and half the bytes of
+    every decode row. A prompt's own pass attends its unrounded keys and values
+    (`update` of an empty cache returns them); later passes get the codes
+    (CachedKeys8): decode rows and short passes read them directly, longer
+    passes read them back into 16 bits."""
+
+    eight_bit = True
+
+    def _allocate(self, config, batch, max_len, device, dtype):
+        self.layers = [ops.kv8_empty(batch, config.num_key_value_heads, max_len, config.head_dim, device)
+                       for _ in range(config.num_hidden_layers)]
+        self.k = [c.k for c in self.layers]
+        self.v = [c.v for c in self.layers]
+
+    def views(self, layer_idx: int):
+        assert self.static
+        return CachedKeys8(self.layers[layer_idx], self.n_keys), None
+
+    def update(self, key_states, value_states, layer_idx: int, cache_kwargs=None):
+        s = key_states.shape[2]
+        k, v = key_states, value_states
+        if k.dtype == torch.float32:
+            k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+        c = self.layers[layer_idx]
+        if self.static:
+            assert s == 1, "static mode appends one token per step"
+            ops.kv8_write(c, k.transpose(1, 2), v.transpose(1, 2), self.pos)
+            return CachedKeys8(c, self.n_keys), None
+        l0 = self.len[layer_idx]
+        assert l0 + s <= self.max_len, (l0, s, self.max_len)
+        ops.kv8_write(c, k.transpose(1, 2), v.transpose(1, 2), l0)
+        self.len[layer_idx] = l0 + s
+        return (key_states, value_states) if l0 == 0 else (CachedKeys8(c, l0 + s), None)
+
+
+def new_cache(config, batch: int, max_len: int, device, dtype) -> KVCache:
+    """The cache that config.kv_cache names."""
+    kind = getattr(config, "kv_cache", "model")
+    if kind not in ("model", "fp8"):
+        raise ValueError(f"kv_cache {kind!r} (built: model, fp8)")
+    return (KVCache8 if kind == "fp8" else KVCache)(config, batch, max_len, device, dtype)
 
 
 class LlamaMLP(nn.Module):
@@ -371,7 +426,7 @@ class LlamaForCausalLM(nn.Module):
             ids = [eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id)
             eos = torch.tensor(ids, dtype=torch.int64, device=input_ids.device)
         b, s = input_ids.shape
-        cache = KVCache(cfg, b, s + max_new_tokens, input_ids.device, self.lm_head.weight.dtype)
+        cache = new_cache(cfg, b, s + max_new_tokens, input_ids.device, self.lm_head.weight.dtype)
         self.reset_decode_state()
         impl = cfg._attn_implementation
         out = []
