@@ -1,14 +1,20 @@
-"""Build libdelta_attn.so (the C-ABI library) for gfx950 with hipcc.
+"""Build libdelta_attn.so (the C-ABI library) for gfx950 with hipcc, and the
+extension module of the 8-bit cache's Python calls with g++.
 
-Run as a script or call ``build()``. The library lands next to the Python
-package (delta_attention/libdelta_attn.so) so that it travels with the tree.
+Run as a script or call ``build()``. Both land next to the Python package
+(delta_attention/libdelta_attn.so, _kv8_ext.so) so that they travel with the
+tree.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -18,6 +24,8 @@ OUT = os.path.join(HERE, "delta_attention", "libdelta_attn.so")
 SOURCES = ["attn_kernels.hip", "attn_bwd.hip", "delta_add.hip", "rope.hip", "norm.hip",
            "anchor_cos.hip", "adapt_loop.hip", "kv8.hip"]
 ARCH = "gfx950"
+EXT_SOURCE = "kv8_bind.cpp"
+EXT_OUT = os.path.join(HERE, "delta_attention", "_kv8_ext.so")
 
 # Packed fp32 VALU ops are disabled: they are not used by hand and must not be
 # formed by the compiler either.
@@ -44,9 +52,12 @@ def hipcc() -> str:
     return path if os.path.exists(path) else "hipcc"
 
 
-def build(verbose: bool = False, out: str = OUT) -> str:
-    cmd = [hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}",
-           *[os.path.join(CSRC, s) for s in SOURCES], "-o", out + ".tmp"]
+def torch_dir() -> str:
+    """The installed torch package's folder (found without importing it)."""
+    return importlib.util.find_spec("torch").submodule_search_locations[0]
+
+
+def _run(cmd, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)
@@ -54,9 +65,40 @@ def build(verbose: bool = False, out: str = OUT) -> str:
     warn = "\n".join(l for l in res.stderr.splitlines()
                      if "packed-fp32-ops" not in l and l.strip())
     if res.returncode != 0:
-        raise RuntimeError(f"hipcc failed ({res.returncode}):\n{warn}")
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({res.returncode}):\n{warn}")
     if warn and verbose:
         print(warn, file=sys.stderr)
+
+
+def build_ext(verbose: bool = False, out: str = EXT_OUT) -> str:
+    """The extension module of the 8-bit cache's calls (host code, against the
+    installed torch)."""
+    t = torch_dir()
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          f"-I{INCLUDE}", f"-I{sysconfig.get_paths()['include']}", "-isystem", os.path.join(t, "include"),
+          "-isystem", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+          "-isystem", os.path.join(rocm, "include"), os.path.join(CSRC, EXT_SOURCE), "-o", out + ".tmp",
+          f"-L{t}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-lamdhip64",
+          f"-Wl,-rpath,{t}/lib"], verbose)
+    os.replace(out + ".tmp", out)
+    return out
+
+
+def build(verbose: bool = False, out: str = OUT) -> str:
+    """Every source at once (each an object of its own), then the library; the
+    extension beside it when the library is the package's."""
+    compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(SOURCES) + 1) as pool:
+        objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        jobs = [pool.submit(_run, [hipcc(), *compile_flags, f"-I{INCLUDE}", f"-I{CSRC}", "-c",
+                                   os.path.join(CSRC, s), "-o", o], verbose)
+                for s, o in zip(SOURCES, objs)]
+        if out == OUT:
+            jobs.append(pool.submit(build_ext, verbose))
+        for j in jobs:
+            j.result()
+        _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *objs, "-o", out + ".tmp"], verbose)
     os.replace(out + ".tmp", out)
     return out
 

@@ -7,12 +7,14 @@ or fails to load, every op raises ExtensionMissing.
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import os
-import struct
 import threading
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libdelta_attn.so")
+EXT_PATH = os.path.join(HERE, "_kv8_ext.so")
 
 DA_OK = 0
 DA_ERR_INVALID_ARG = -1
@@ -87,6 +89,7 @@ class ExtensionMissing(RuntimeError):
 
 
 _lib = None
+_kv8_ext = None
 _lib_lock = threading.Lock()
 
 I64x3 = ctypes.c_int64 * 3
@@ -221,7 +224,7 @@ def _load() -> ctypes.CDLL:
                                      _p3, _p3, _p3, _p3, _i, _i, _i, _f,
                                      _i, _i, _i, _i, _i, _i, _d, _d, _d,
                                      _vp, _vp, _vp, _vp, _i, _vp, _sz, _i, _vp, _vp]
-    # (these take one struct, packed by the caller: see KV8_WRITE below)
+    # (these take one struct; kv8_ext's functions pack it)
     for f in (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd):
         f.restype = _i
         f.argtypes = [ctypes.c_char_p, _vp]
@@ -244,13 +247,30 @@ def check(rc: int, what: str) -> None:
     raise AssertionError(msg)
 
 
-# The structs of the 8-bit cache's calls (native alignment), in the header's
-# order: one pack is a fifth of the time of as many ctypes arguments.
-_KV8_CACHE = "4P8q4i"      # k, v, k_scale, v_scale; their {batch, head} strides; B, Hkv, cap, D
-KV8_WRITE = struct.Struct(_KV8_CACHE + "4P7q4i")      # k, v, pos_dev, counts_dev; strides, pos; S, 2 flags, dtype
-KV8_READ = struct.Struct(_KV8_CACHE + "3P6q4i")       # k, v, n_keys_dev; strides; start, n, flag, dtype
-KV8_ATTN = struct.Struct(_KV8_CACHE + "5P10q7if")     # q, out, addend, n_keys_dev, workspace; its bytes, strides;
-                                                      # Hq, s, flag, n_keys, window, sink, dtype; sm_scale
+def kv8_ext():
+    """The extension module of the 8-bit cache's calls (csrc/kv8_bind.cpp),
+    loaded once and bound to the library's functions."""
+    global _kv8_ext
+    if _kv8_ext is not None:
+        return _kv8_ext
+    L = lib()
+    with _lib_lock:
+        if _kv8_ext is None:
+            import torch  # noqa: F401  (its libraries are the extension's)
+            if not os.path.exists(EXT_PATH):
+                raise ExtensionMissing(
+                    f"{EXT_PATH} is not built: run `python delta-attention_amd/build_lib.py` "
+                    "(or __graft_entry__.build()) first")
+            loader = importlib.machinery.ExtensionFileLoader(f"{__package__}._kv8_ext", EXT_PATH)
+            try:
+                m = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+                loader.exec_module(m)
+            except ImportError as e:  # pragma: no cover - depends on the machine
+                raise ExtensionMissing(f"cannot load {EXT_PATH}: {e}") from e
+            m.bind(*(ctypes.cast(f, _vp).value for f in (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd,
+                                                         L.da_kv8_attn_workspace_bytes)), check)
+            _kv8_ext = m
+    return _kv8_ext
 
 
 def strides3(*s: int):

@@ -622,35 +622,8 @@ def kv8_empty(B: int, Hkv: int, max_len: int, D: int, device="cuda") -> KV8:
                scale[0], scale[1])
 
 
-_F8, _F32, _I32, _I64 = torch.float8_e4m3fn, torch.float32, torch.int32, torch.int64
-
-
-def _kv8(c: KV8, dev: torch.device):
-    """Checks a cache's tensors -> the head of the C ABI's structs (pointers,
-    strides, B, Hkv, cap, D)."""
-    k, v, ks, vs = c
-    B, Hkv, cap, D = k.shape
-    nb = cap // KV8_BLOCK
-    a, b, d, e = k.stride(), v.stride(), ks.stride(), vs.stride()
-    assert cap % KV8_BLOCK == 0 and v.shape == (B, Hkv, nb, D, KV8_BLOCK) and ks.shape == vs.shape == (B, Hkv, nb), (
-        k.shape, v.shape, ks.shape, vs.shape)
-    assert k.dtype is _F8 and v.dtype is _F8 and ks.dtype is _F32 and vs.dtype is _F32, (
-        k.dtype, v.dtype, ks.dtype, vs.dtype)
-    assert a[2:] == (D, 1) and b[2:] == (D * KV8_BLOCK, KV8_BLOCK, 1) and d[2] == e[2] == 1, (
-        "a cache's tokens, blocks and scales must be contiguous within a head")
-    assert k.device == v.device == ks.device == vs.device == dev, "all tensors must be on one device"
-    return (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(),
-            a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1], B, Hkv, cap, D)
-
-
-def _per_seq(t: torch.Tensor, B: int, dtype: torch.dtype, dev: torch.device, what: str) -> bool:
-    """Checks a device tensor of one entry, or one per sequence -> whether the
-    latter."""
-    n = t.numel()
-    assert t.dtype is dtype and t.device == dev and (n == B or n == 1) and t.dim() <= 1 and t.is_contiguous(), (
-        f"{what}: a contiguous {dtype} tensor of 1 or {B} entries on {dev}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return n == B
-
+# (the checks and launches of the calls below are csrc/kv8_bind.cpp's: a decode
+# step's are shorter on the GPU than in Python)
 
 def kv8_write(cache: KV8, k: torch.Tensor, v: torch.Tensor, pos, *,
               counts: Optional[torch.Tensor] = None) -> None:
@@ -663,29 +636,7 @@ def kv8_write(cache: KV8, k: torch.Tensor, v: torch.Tensor, pos, *,
     or one per sequence), the tokens of each right-padded sequence. Rows behind
     the written ones keep their bytes but hold nothing any more. With device
     positions, a sequence whose rows do not fit is left unchanged."""
-    dev = k.device
-    head = _kv8(cache, dev)
-    B, Hkv, cap, D = head[12:]
-    S = k.shape[1]
-    assert k.shape == v.shape == (B, S, Hkv, D) and k.dtype is v.dtype, (k.shape, v.shape, (B, S, Hkv, D), k.dtype, v.dtype)
-    code = _code(k)
-    assert dev.type == "cuda" and v.device == dev, "delta-attention kernels need GPU tensors, all on one device"
-    p_dev = c_dev = p_b = c_b = 0
-    if isinstance(pos, torch.Tensor):
-        p_b, p_dev, pos = _per_seq(pos, B, _I64, dev, "pos"), pos.data_ptr(), 0
-    else:
-        pos = int(pos)
-        assert 0 <= pos <= cap - S, f"rows {pos} .. {pos + S} do not fit a cache of {cap}"
-    if counts is not None:
-        c_b, c_dev = _per_seq(counts, B, _I32, dev, "counts"), counts.data_ptr()
-    if B == 0 or S == 0:
-        return
-    k, v = _ready(k), _ready(v)
-    args = L.KV8_WRITE.pack(*head, k.data_ptr(), v.data_ptr(), p_dev, c_dev, *k.stride()[:3], *v.stride()[:3],
-                            pos, S, p_b, c_b, code)
-    with _device(dev):
-        rc = L.lib().da_kv8_write(args, _stream(dev))
-    L.check(rc, "da_kv8_write")
+    L.kv8_ext().write(cache, k, v, pos, counts)
 
 
 def kv8_read(cache: KV8, start: int, n: int, *, n_keys: Optional[torch.Tensor] = None,
@@ -696,34 +647,13 @@ def kv8_read(cache: KV8, start: int, n: int, *, n_keys: Optional[torch.Tensor] =
     beyond float16's largest saturate. n_keys: optional int32 device tensor
     (one entry or one per sequence); rows at or past it are zero. out: the two
     tensors to write."""
-    dev = cache.k.device
-    head = _kv8(cache, dev)
-    B, Hkv, cap, D = head[12:]
-    start, n = int(start), int(n)
-    assert 0 <= start and 0 <= n <= cap - start, f"rows {start} .. {start + n} of a cache of {cap}"
-    assert dev.type == "cuda", "delta-attention kernels need GPU tensors"
-    n_dev = n_b = 0
-    if n_keys is not None:
-        n_b, n_dev = _per_seq(n_keys, B, _I32, dev, "n_keys"), n_keys.data_ptr()
     if out is None:
-        out = tuple(torch.empty((2, B, Hkv, n, D), device=dev, dtype=dtype))
+        B, Hkv, cap, D = cache.k.shape
+        assert 0 <= start and 0 <= n <= cap - start, f"rows {start} .. {start + n} of a cache of {cap}"
+        out = torch.empty((2, B, Hkv, n, D), device=cache.k.device, dtype=dtype).unbind(0)
     k, v = out
-    assert k.shape == v.shape == (B, Hkv, n, D) and k.dtype is v.dtype and k.device == v.device == dev, (k.shape, v.shape)
-    assert k.stride(-1) == 1 and v.stride(-1) == 1
-    code = _code(k)
-    if B == 0 or n == 0:
-        return k, v
-    args = L.KV8_READ.pack(*head, k.data_ptr(), v.data_ptr(), n_dev, *k.stride()[:3], *v.stride()[:3],
-                           start, n, n_b, code)
-    with _device(dev):
-        rc = L.lib().da_kv8_read(args, _stream(dev))
-    L.check(rc, "da_kv8_read")
+    L.kv8_ext().read(cache, start, n, n_keys, k, v)
     return k, v
-
-
-@functools.lru_cache(maxsize=256)
-def _kv8_ws_bytes(B: int, H: int, Hkv: int, s: int, D: int, n: int, window: int, sink: int) -> int:
-    return int(L.lib().da_kv8_attn_workspace_bytes(B, H, Hkv, s, D, n, window, sink))
 
 
 def kv8_attention(q: torch.Tensor, cache: KV8, *, n_keys, window: int = 0, sink: int = 0,
@@ -739,41 +669,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8, *, n_keys, window: int = 0, sink:
     read when the kernels run (a recorded call serves every length; counts are
     clamped to the capacity). add: a tensor like q; rnd(rnd(row) + add). A new
     result has q's strides where q is dense."""
-    dev = q.device
-    head = _kv8(cache, dev)
-    B, Hkv, cap, D = head[12:]
-    Bq, H, s, Dq = q.shape
-    assert Bq == B and Dq == D and H > 0 and H % Hkv == 0, (q.shape, cache.k.shape)
-    code = _code(q)
-    assert dev.type == "cuda", "delta-attention kernels need GPU tensors"
-    q = _ready(q)
-    if out is None:
-        out = torch.empty_like(q)
-    else:
-        assert out.shape == q.shape and out.dtype is q.dtype and out.stride(-1) == 1 and out.device == dev
-    window, sink = min(max(int(window), 0), cap), min(max(int(sink), 0), cap)
-    n_dev, n_b, n = 0, False, cap
-    if isinstance(n_keys, torch.Tensor):
-        n_b, n_dev = _per_seq(n_keys, B, _I32, dev, "n_keys"), n_keys.data_ptr()
-    else:
-        n = int(n_keys)
-        assert 0 <= n <= cap, f"{n} keys in a cache of {cap}"
-    a_ptr, a_str = 0, (0, 0, 0)
-    if add is not None:
-        assert add.shape == q.shape and add.dtype is q.dtype and add.device == dev
-        add = _ready(add)
-        a_ptr, a_str = add.data_ptr(), add.stride()[:3]
-    if B == 0 or s == 0:
-        return out
-    nbytes = _kv8_ws_bytes(B, H, Hkv, s, D, n, window, sink)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    args = L.KV8_ATTN.pack(*head, q.data_ptr(), out.data_ptr(), a_ptr, n_dev, 0 if ws is None else ws.data_ptr(),
-                           nbytes, *q.stride()[:3], *out.stride()[:3], *a_str, H, s, n_b, n, window, sink,
-                           code, sm_scale)
-    with _device(dev):
-        rc = L.lib().da_kv8_attn_fwd(args, _stream(dev))
-    L.check(rc, "da_kv8_attn_fwd")
-    return out
+    return L.kv8_ext().attention(q, cache, n_keys, window, sink, sm_scale, out, add)
 
 
 # ---------------------------------------------------------------------------

@@ -2,6 +2,7 @@
 casts, its argument checks at the C entry points and in ops, its layout."""
 
 import os
+import struct
 
 import numpy as np
 import pytest
@@ -66,10 +67,9 @@ def test_empty_cache_and_its_slices():
     c = ops.kv8_empty(2, 3, 100, 64, "cpu")
     assert c.k.shape == (2, 3, 128, 64) and c.v.shape == (2, 3, 2, 64, 64)
     assert c.k_scale.shape == c.v_scale.shape == (2, 3, 2) and (c.k_scale == 2.0 ** -117).all()
-    head = ops._kv8(c, c.k.device)
-    assert head[12:] == (2, 3, 128, 64) and head[4:6] == (3 * 128 * 64, 128 * 64)
-    part = ops.KV8(*(t[:, 1:] for t in c))
-    assert ops._kv8(part, c.k.device)[12:] == (2, 2, 128, 64)
+    for cache in (c, ops.KV8(*(t[:, 1:] for t in c))):       # (its layout passes: only the GPU is missing)
+        with pytest.raises(AssertionError, match="GPU tensors"):
+            ops.kv8_read(cache, 0, 5)
     for bad in (dict(D=96), dict(max_len=0), dict(max_len=(1 << 30) + 1), dict(Hkv=0)):
         with pytest.raises(AssertionError):
             ops.kv8_empty(**{**dict(B=1, Hkv=1, max_len=64, D=64, device="cpu"), **bad})
@@ -81,8 +81,11 @@ def test_ops_refuse_caches_that_are_not_laid_out_so():
                 c._replace(v=c.v.transpose(3, 4)), c._replace(k_scale=c.k_scale[..., :1]),
                 c._replace(k=c.k.view(torch.uint8)), c._replace(v_scale=c.v_scale.double()),
                 c._replace(k_scale=c.k_scale[..., 0:1].expand(1, 2, 2))):
-        with pytest.raises(AssertionError):
-            ops._kv8(bad, c.k.device)
+        with pytest.raises(AssertionError, match="belong together|contiguous|float8|dimensions"):
+            ops.kv8_read(bad, 0, 5)
+    for bad in (tuple(c)[:3], None, [*c]):
+        with pytest.raises(AssertionError, match="KV8 cache"):
+            L.kv8_ext().read(bad, 0, 5, None, torch.zeros(1, 2, 5, 64), torch.zeros(1, 2, 5, 64))
 
 
 def test_ops_refuse_arguments_on_the_cpu():
@@ -91,18 +94,31 @@ def test_ops_refuse_arguments_on_the_cpu():
     q = torch.zeros(1, 4, 1, 64, dtype=torch.bfloat16)
     with pytest.raises(AssertionError, match="GPU tensors"):
         ops.kv8_write(c, k, k, 0)
-    with pytest.raises(AssertionError):
+    with pytest.raises(AssertionError, match="k and v are"):
         ops.kv8_write(c, k[..., :32], k[..., :32], 0)
-    with pytest.raises(AssertionError):
+    with pytest.raises(AssertionError, match="different types"):
         ops.kv8_write(c, k, k.half(), 0)
+    with pytest.raises(AssertionError, match="not supported"):
+        ops.kv8_write(c, k.float(), k.float(), 0)
+    with pytest.raises(AssertionError, match="a tensor is needed"):
+        ops.kv8_write(c, None, k, 0)
+    with pytest.raises(TypeError):
+        L.kv8_ext().write(c, k)
     with pytest.raises(AssertionError, match="GPU tensors"):
         ops.kv8_attention(q, c, n_keys=1, sm_scale=1.0)
-    with pytest.raises(AssertionError):
+    with pytest.raises(AssertionError, match="multiple of 2"):
         ops.kv8_attention(q[:, :3], c, n_keys=1, sm_scale=1.0)
-    with pytest.raises(AssertionError):
-        ops.kv8_read(c, 100, 29)
+    for start, n in ((100, 29), (-1, 2), (0, -1)):
+        with pytest.raises(AssertionError, match="rows"):
+            ops.kv8_read(c, start, n)
 
 
+# the header's structs, in native alignment
+_CACHE = "4P8q4i"                                # k, v, k_scale, v_scale; {batch, head} strides; B, Hkv, cap, D
+WRITE = struct.Struct(_CACHE + "4P7q4i")         # k, v, pos_dev, counts_dev; strides, pos; S, 2 flags, dtype
+READ = struct.Struct(_CACHE + "3P6q4i")          # k, v, n_keys_dev; strides; start, n, flag, dtype
+ATTN = struct.Struct(_CACHE + "5P10q7if")        # q, out, addend, n_keys_dev, workspace; its bytes, strides;
+                                                 # Hq, s, flag, n_keys, window, sink, dtype; sm_scale
 CACHE = dict(kc=16, vc=16, sk=16, sv=16, cs=(128 * 128, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2), B=1, Hkv=2,
              cap=128, D=64)
 
@@ -111,19 +127,12 @@ def _head(a):
     return (a["kc"], a["vc"], a["sk"], a["sv"], *a["cs"], a["B"], a["Hkv"], a["cap"], a["D"])
 
 
-def test_struct_sizes():
-    """The packed structs are the header's: fields in order, native alignment."""
-    assert L.KV8_WRITE.size == 112 + 4 * 8 + 7 * 8 + 16
-    assert L.KV8_READ.size == 112 + 3 * 8 + 6 * 8 + 16
-    assert L.KV8_ATTN.size == 112 + 5 * 8 + 10 * 8 + 32
-
-
 def test_c_write_refusals(lib):
     def call(**kw):
         a = dict(CACHE, k=16, v=16, ks=(3 * 128, 128, 64), vs=(3 * 128, 128, 64), S=3, pos=0, pos_dev=0, counts=0,
                  dtype=L.DA_BF16)
         a.update(kw)
-        return lib.da_kv8_write(L.KV8_WRITE.pack(*_head(a), a["k"], a["v"], a["pos_dev"], a["counts"], *a["ks"],
+        return lib.da_kv8_write(WRITE.pack(*_head(a), a["k"], a["v"], a["pos_dev"], a["counts"], *a["ks"],
                                                  *a["vs"], a["pos"], a["S"], 0, 0, a["dtype"]), None)
     assert call(dtype=5) == L.DA_ERR_DTYPE
     assert call(D=96) == L.DA_ERR_HEAD_DIM
@@ -142,7 +151,7 @@ def test_c_read_refusals(lib):
     def call(**kw):
         a = dict(CACHE, start=0, n=5, nk=0, ko=16, vo=16, st=(2 * 5 * 64, 5 * 64, 64), dtype=L.DA_FP16)
         a.update(kw)
-        return lib.da_kv8_read(L.KV8_READ.pack(*_head(a), a["ko"], a["vo"], a["nk"], *a["st"], *a["st"], a["start"],
+        return lib.da_kv8_read(READ.pack(*_head(a), a["ko"], a["vo"], a["nk"], *a["st"], *a["st"], a["start"],
                                                a["n"], 0, a["dtype"]), None)
     assert call(dtype=2) == L.DA_ERR_DTYPE and call(D=48) == L.DA_ERR_HEAD_DIM
     for bad in (dict(start=-1), dict(n=-1), dict(start=124), dict(start=2 ** 31 - 1, n=2 ** 31 - 1), dict(ko=0),
@@ -166,7 +175,7 @@ def test_c_rows_refusals_and_workspace(lib):
         a = dict(CACHE, cap=1024, q=16, qs=(8 * 64, 64, 64), out=16, Hq=8, s=1, nk=0, n=1000, window=0, sink=0, add=0,
                  as_=(8, 8, 8), ws=16, nb=1 << 30, dtype=L.DA_BF16)
         a.update(kw)
-        return lib.da_kv8_attn_fwd(L.KV8_ATTN.pack(*_head(a), a["q"], a["out"], a["add"], a["nk"], a["ws"], a["nb"],
+        return lib.da_kv8_attn_fwd(ATTN.pack(*_head(a), a["q"], a["out"], a["add"], a["nk"], a["ws"], a["nb"],
                                                    *a["qs"], 8 * 64, 64, 64, *a["as_"], a["Hq"], a["s"], 0, a["n"],
                                                    a["window"], a["sink"], a["dtype"], 0.1), None)
     assert call(dtype=3) == L.DA_ERR_DTYPE and call(D=512) == L.DA_ERR_HEAD_DIM
