@@ -78,6 +78,9 @@ def parse():
     p.add_argument("--decode-tokens", type=int, default=0,
                    help="with --model: also generate this many tokens after the prefill, with "
                         "dense and with delta decode, and report ms per decode token")
+    p.add_argument("--kv-cache", choices=("model", "fp8"), default="model",
+                   help="decode cache of --model --decode-tokens: 16-bit, or 8-bit codes with a "
+                        "scale per block of 64 tokens and head")
     p.add_argument("--train", action="store_true",
                    help="time delta_forward_train's forward and backward (the training "
                         "path) at --seq/--gamma/--window/--sink instead of the prefill")
@@ -463,7 +466,7 @@ def model_prefill(a, dev):
         dec = {}
         for mode in ("dense", "delta"):
             for graph in (False, True):
-                cfg.decode_mode, cfg.gamma_dec = mode, a.gamma_dec
+                cfg.decode_mode, cfg.gamma_dec, cfg.kv_cache = mode, a.gamma_dec, a.kv_cache
                 steps_ms = []
                 toks = model.generate_greedy(ids, a.decode_tokens, step_ms=steps_ms, graph=graph)
                 later = steps_ms[2:] or steps_ms     # graphs: the first step of each kind records
@@ -471,7 +474,7 @@ def model_prefill(a, dev):
                     "ms_per_token": round(float(np.median(steps_ms)), 3),
                     "mean_ms_after_step2": round(float(np.mean(later)), 3),
                     "tokens": int(toks.shape[1])}
-        line["decode"] = dict(dec, gamma_dec=a.gamma_dec, context=S,
+        line["decode"] = dict(dec, gamma_dec=a.gamma_dec, context=S, kv_cache=a.kv_cache,
                               note="median wall time of one decode step (all layers + lm_head); "
                                    "_graph: each step kind recorded once and replayed")
     print(json.dumps(line), flush=True)

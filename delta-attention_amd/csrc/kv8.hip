@@ -20,7 +20,9 @@
 // which is the second product's right operand as it stands, if the left operand
 // V^T holds the same tokens in the same lane: 16 consecutive bytes of a column
 // of the cache. Neither product needs LDS or a transpose.
+#include <float.h>
 #include <hip/hip_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "capi_common.h"
@@ -450,7 +452,8 @@ struct RowsArgs {
   int B, Hkv, G, s;         // G query heads per kv head, s rows at the end of each sequence
   int n_rt, rows;           // row tiles of `rows` rows (flattened row i * G + head) per sequence and kv head
   int window, sink;
-  float scale_log2;         // sm_scale * log2(e)
+  float scale_log2;         // |sm_scale| * log2(e), above zero
+  uint32_t flip;            // the sign bits of Q where sm_scale is negative
   int slots;                // workgroups that are resident together
   FastDiv round;            // blocks that they take at most: slots * CHUNK
   FastDiv units, tiles, heads;   // Hkv * n_rt, n_rt, G
@@ -458,10 +461,11 @@ struct RowsArgs {
   int64_t pitch;            // floats per item
 };
 
-constexpr float NO_KEYS = -1e30f;
-// Probabilities are held relative to a row reference that may lag its maximum
-// by up to LAG (log2), times 2^BIAS: at most 2^14, inside fp16, and fp16 ends
-// 2^-32 below the reference.
+constexpr float NO_KEYS = -3.4028234664e38f;   // the reference of a row without keys yet: below every finite score
+// Probabilities are held relative to a row reference (a score q k, not yet times
+// sm_scale: differences are taken before anything can overflow) that may lag its
+// maximum by up to LAG (log2), times 2^BIAS: at most 2^14, inside fp16, and fp16
+// ends 2^-32 below the reference.
 constexpr float LAG = 6.f, BIAS = 8.f;
 
 // The blocks that a sequence's rows see: those of the sinks, then [lo, hi).
@@ -612,23 +616,28 @@ __device__ __forceinline__ float group_max(float x) {   // over the four lanes o
   return max32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 
-template <typename T> struct Dot;    // 16x16x32 products of Q's type
+// 16x16x32 products of one type, and eight codes as its left operand. SCALED:
+// the conversion applies the block's scale, exactly (bf16 has float's range:
+// scores then overflow only where they would anyway); fp16 takes the codes alone.
+template <typename T> struct Dot;
 template <> struct Dot<__bf16> {
+  static constexpr bool SCALED = true;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ u32x4 codes(uint32_t lo, uint32_t hi) {
-    return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false)),
-                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true))};
+  static __device__ __forceinline__ u32x4 codes(uint32_t lo, uint32_t hi, float scale) {
+    return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true))};
   }
 };
 template <> struct Dot<_Float16> {
+  static constexpr bool SCALED = false;
   static __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
   }
-  static __device__ __forceinline__ u32x4 codes(uint32_t lo, uint32_t hi) {
+  static __device__ __forceinline__ u32x4 codes(uint32_t lo, uint32_t hi, float = 1.f) {
     return (u32x4){__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, false)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, 1.f, true)),
                    __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, 1.f, false)),
@@ -694,7 +703,8 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
     lim[mt] = n - a.s + i;
     const T* src = (const T*)a.q + b * a.q_b + (int64_t)(hk * a.G + m - i * a.G) * a.q_h + i * a.q_s;
 #pragma unroll
-    for (int k = 0; k < KS; ++k) qf[mt][k] = *(const u32x4*)(src + (D >= 64 ? k / 2 * 64 + g * 16 + k % 2 * 8 : g * 8));
+    for (int k = 0; k < KS; ++k)
+      qf[mt][k] = *(const u32x4*)(src + (D >= 64 ? k / 2 * 64 + g * 16 + k % 2 * 8 : g * 8)) ^ a.flip;
   }
   const uint8_t* kc = a.c.k + b * a.c.k_b + hk * a.c.k_h;
   const uint8_t* vc = a.c.v + b * a.c.v_b + hk * a.c.v_h;
@@ -777,20 +787,22 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
     for (int k = 0; k < KS; ++k) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const u32x4 af = Dot<T>::codes(kf[t][k / 2][k % 2 * 2], kf[t][k / 2][k % 2 * 2 + 1]);
+        const u32x4 af = Dot<T>::codes(kf[t][k / 2][k % 2 * 2], kf[t][k / 2][k % 2 * 2 + 1], sk);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
           s[mt][t] = Dot<T>::mfma(af, qf[mt][k], k == 0 ? (f32x4){0, 0, 0, 0} : s[mt][t]);
       }
       __builtin_amdgcn_sched_barrier(0);      // (the conversions stay beside their products: fewer registers)
     }
-    const float sc = sk * a.scale_log2;
+    const float unit = sk;
     load_k(blk, more);                        // the keys' registers are free from here on
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (!Dot<T>::SCALED) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[mt][e / 4][e % 4] *= sc;
+        for (int e = 0; e < 16; ++e) s[mt][e / 4][e % 4] *= unit;
+    }
     if (!whole) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
@@ -806,9 +818,9 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, s[mt][e / 4][e % 4]);
       top = group_max(top);
-      if (__any(top > ref[mt] + LAG)) {
+      if (__any((top - ref[mt]) * a.scale_log2 > LAG)) {
         const float to = fmaxf(ref[mt], top);
-        const float alpha = fast_exp2(ref[mt] - to);
+        const float alpha = ref[mt] == NO_KEYS ? 0.f : fast_exp2((ref[mt] - to) * a.scale_log2);
         ref[mt] = to;
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum[mt][r] *= alpha;
@@ -817,13 +829,15 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[mt][t][r] *= alpha;
       }
-      const float off = BIAS - ref[mt];
+      auto weight = [&](float y) __attribute__((always_inline)) {
+        return fast_exp2(fmaf(y - ref[mt], a.scale_log2, BIAS));
+      };
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int t = 2 * u + w / 2, r = w % 2 * 2;
-          pf[mt][u][w] = Elt<_Float16>::pack2(fast_exp2(s[mt][t][r] + off), fast_exp2(s[mt][t][r + 1] + off));
+          pf[mt][u][w] = Elt<_Float16>::pack2(weight(s[mt][t][r]), weight(s[mt][t][r + 1]));
         }
     }
     __builtin_amdgcn_sched_barrier(0);
@@ -916,7 +930,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
       f32x4 o = {0, 0, 0, 0};
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
-        const float k = fast_exp2(s_m[w][r] - M);
+        const float k = fast_exp2((s_m[w][r] - M) * a.scale_log2);
         const f32x4 y = *(const f32x4*)&s_o[w][r][d];
         L = fmaf(s_l[w][r], k, L);
 #pragma unroll
@@ -972,7 +986,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
     for (int u = 0; u < U; ++u) {
       if (i0 + u * SG >= p.n_split) break;
       const float to = fmaxf(M, mi[u]);
-      const float k0 = fast_exp2(M - to), k1 = fast_exp2(mi[u] - to);
+      const float k0 = fast_exp2((M - to) * a.scale_log2), k1 = fast_exp2((mi[u] - to) * a.scale_log2);
       M = to;
       L = L * k0 + li[u] * k1;
 #pragma unroll
@@ -992,7 +1006,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
   o = (f32x4){0, 0, 0, 0};
 #pragma unroll 4
   for (int i = 0; i < used; ++i) {
-    const float k = fast_exp2(s_w[i][0] - M);
+    const float k = fast_exp2((s_w[i][0] - M) * a.scale_log2);
     const f32x4 y = s_o[i][t];
     L = fmaf(s_w[i][1], k, L);
 #pragma unroll
@@ -1123,6 +1137,11 @@ extern "C" int da_kv8_write(const da_kv8_write_args* x, void* stream) {
   if (S < 0 || (!x->pos_dev && (x->pos < 0 || x->pos > cap - (int64_t)S))) return DA_ERR_INVALID_ARG;
   if (S == 0 || B == 0) return DA_OK;
   if (!x->k || !x->v) return DA_ERR_INVALID_ARG;
+  // a cache that repeats itself over sequences or heads has no one value to write
+  const da_kv8_cache& c = x->cache;
+  if ((B > 1 && (!c.k_str[0] || !c.v_str[0] || !c.k_scale_str[0] || !c.v_scale_str[0])) ||
+      (Hkv > 1 && (!c.k_str[1] || !c.v_str[1] || !c.k_scale_str[1] || !c.v_scale_str[1])))
+    return DA_ERR_INVALID_ARG;
   if (!aligned16(x->k) || !aligned16(x->v) || !strides8(x->k_str) || !strides8(x->v_str) ||
       ((uintptr_t)x->pos_dev & 7) || ((uintptr_t)x->counts_dev & 3))
     return DA_ERR_ALIGNMENT;
@@ -1192,6 +1211,7 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   const int B = x->cache.B, Hkv = x->cache.Hkv, cap = x->cache.cap, Hq = x->Hq, s = x->s;
   if (Hq < 1 || Hq % Hkv != 0 || s < 0 || x->window < 0 || x->sink < 0) return DA_ERR_INVALID_ARG;
   if (!x->n_keys_dev && (x->n_keys < 0 || x->n_keys > cap)) return DA_ERR_INVALID_ARG;
+  if (!(fabsf(x->sm_scale) <= FLT_MAX)) return DA_ERR_INVALID_ARG;
   if (s == 0 || B == 0) return DA_OK;
   if (!x->q || !x->out) return DA_ERR_INVALID_ARG;
   if (!aligned16(x->q) || !aligned16(x->out) || !strides8(x->q_str) || !strides8(x->o_str) ||
@@ -1217,7 +1237,9 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   a.n = x->n_keys;
   a.B = B, a.Hkv = Hkv, a.G = Hq / Hkv, a.s = s;
   a.n_rt = p.n_rt, a.rows = p.rows;
-  a.scale_log2 = x->sm_scale * 1.4426950408889634f;
+  // (a scale of zero, which weighs every key alike, as the smallest one)
+  a.scale_log2 = fminf(fmaxf(fabsf(x->sm_scale) * 1.4426950408889634f, FLT_MIN), FLT_MAX);
+  a.flip = x->sm_scale < 0.f ? 0x80008000u : 0;
   a.slots = p.slots;
   a.round = p.round;
   a.units = make_fastdiv(Hkv * p.n_rt);

@@ -296,7 +296,8 @@ typedef struct {
  * x / 2^e rounded to nearest even; infinities and NaN become NaN. Rows from
  * pos + count on keep their bytes; they stand for nothing any more where their
  * block was written. A sequence whose rows do not fit ([pos, pos + count) not in
- * [0, cap)) keeps its cache unchanged (DA_ERR_INVALID_ARG for a host pos).
+ * [0, cap)) keeps its cache unchanged (DA_ERR_INVALID_ARG for a host pos, and
+ * for a cache with a zero stride over its sequences or heads).
  */
 typedef struct {
   da_kv8_cache cache;
@@ -328,7 +329,8 @@ int da_kv8_read(const da_kv8_read_args* args, void* stream);
  * keys, row i of q [B, Hq, s, D] (strides {batch, head, row}) stands at r = n - s
  * + i and sees the keys j <= r, with window > 0 only those with j < sink or
  * j > r - window (the decode rows of da_decode_attn_fwd, window 0: every key).
- * out [B, Hq, s, D] = softmax(sm_scale q k) v in fp32, rounded once; rows that
+ * out [B, Hq, s, D] = softmax(sm_scale q k) v in fp32, rounded once (sums of
+ * values are held times up to 2^14 a key: right for |v| up to 2^90); rows that
  * see no key (r < 0) are zero. addend (optional, like q): out = rnd(rnd(row) +
  * addend). n is n_keys_dev[b] (or n_keys_dev[0] when n_keys_per_seq is 0) read
  * when the kernels run and clamped to [0, cap], or the host's n_keys.

@@ -269,6 +269,10 @@ ROWS = [
     (70, 1, 2, 32, 128, [(i * 37) % 129 for i in range(70)], 1, 0, 0),   # more sequences than lanes
     (1, 1, 4, 128, 20480, [20001], 1, 0, 0),                  # a long one: many splits
     (2, 1, 20, 128, 8192, [8192, 100], 1, 1000, 5000),        # sinks past the window's start
+    (300, 1, 1, 32, 192, [(i * 53) % 193 for i in range(300)], 1, 0, 0),  # more than are kept in registers
+    (3, 2, 8, 64, 1024, [1000, 0, 513], 40, 100, 70),         # several row tiles, ragged, windows
+    (1, 1, 1, 128, 131072, [70], 1, 0, 0),                    # a few keys of a large capacity
+    (2, 1, 16, 32, 256, [256, 3], 4, 0, 0),                   # 64 rows, more rows than keys
 ]
 
 
@@ -300,6 +304,116 @@ def test_rows_large_scores(gpu):
     q = tokens(B, 1, G, D, torch.float16, 5, False).transpose(1, 2) * 8
     got = ops.kv8_attention(q, c, n_keys=counts, sm_scale=1.0)
     check_rows(got, q, ref, [n], 0, 0, 1.0, what="large scores")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_rows_other_scales(gpu, dtype):
+    """A negative scale, and zero (every key weighs alike)."""
+    from delta_attention import ops
+    n = [700, 64]
+    c, ref, counts = filled(2, 2, 1024, 64, n, DT[dtype], 40)
+    q = tokens(2, 2, 6, 64, DT[dtype], 41, False).transpose(1, 2)
+    for scale in (-0.2, 0.0, 1e-30):
+        got = ops.kv8_attention(q, c, n_keys=counts, window=200, sink=3, sm_scale=scale)
+        check_rows(got, q, ref, n, 200, 3, scale, what=f"scale {scale}")
+    for bad in (float("nan"), float("inf"), 1e39):
+        with pytest.raises(AssertionError):
+            ops.kv8_attention(q, c, n_keys=counts, sm_scale=bad)
+
+
+def test_rows_huge_scores_and_infinite_queries(gpu):
+    """Scores near float32's ends (finite bf16 inputs) pick the largest; a query
+    with an infinity or NaN gives its own row NaN and no other."""
+    from delta_attention import ops
+    D, n = 64, 130
+    k = torch.zeros(1, n, 1, D, dtype=torch.bfloat16, device="cuda")
+    k[0, :, 0, 0] = torch.linspace(-1, 1, n)
+    v = tokens(1, n, 1, D, torch.bfloat16, 2, False)
+    c = ops.kv8_empty(1, 1, 192, D)
+    ops.kv8_write(c, k, v, 0)
+    q = torch.zeros(1, 4, 1, D, dtype=torch.bfloat16, device="cuda")
+    q[0, 0, 0, 0], q[0, 1, 0, 0] = 1e38, -1e38
+    q[0, 2, 0, 0] = float("inf")
+    q[0, 3, 0, 1] = 1.0
+    got = ops.kv8_attention(q, c, n_keys=n, sm_scale=1.0)
+    kk, vv = ops.kv8_read(c, 0, n)
+    for h, at in ((0, kk[0, 0, :, 0].argmax()), (1, kk[0, 0, :, 0].argmin())):
+        same_k = kk[0, 0, :, 0] == kk[0, 0, at, 0]            # (codes tie: the row is their mean)
+        want = vv[0, 0, same_k].float().mean(0)
+        assert (got[0, h, 0].float() - want).abs().max() <= 2.0 ** -7 * max(1.0, want.abs().max().item())
+    assert got[0, 2].isnan().all()
+    want = vv[0, 0].float().mean(0)
+    assert (got[0, 3, 0].float() - want).abs().max() <= 2.0 ** -8
+    low = ops.kv8_attention(-q[:, :1].abs() * 3, c, n_keys=1, sm_scale=1.0)   # one key, its score +3e38
+    assert torch.equal(low[0, 0, 0], vv[0, 0, 0])
+
+
+def test_rows_shared_prefix_and_refused_writes(gpu):
+    """One sequence's cache expanded over a batch serves its rows (a shared
+    prompt); writing through the expansion is refused."""
+    from delta_attention import ops
+    c, ref, _ = filled(1, 2, 512, 64, [400], torch.bfloat16, 12)
+    many = ops.KV8(*(t.expand(5, *t.shape[1:]) for t in c))
+    q = tokens(5, 2, 6, 64, torch.bfloat16, 13, False).transpose(1, 2)
+    got = ops.kv8_attention(q, many, n_keys=torch.tensor([400], dtype=torch.int32, device="cuda"), sm_scale=0.125)
+    check_rows(got, q, {x: np.repeat(y, 5, 0) for x, y in ref.items()}, [400] * 5, 0, 0, 0.125, what="shared")
+    with pytest.raises(AssertionError, match="invalid"):
+        ops.kv8_write(many, tokens(5, 1, 2, 64, torch.bfloat16, 1), tokens(5, 1, 2, 64, torch.bfloat16, 2), 400)
+
+
+def test_gpu_refusals(gpu):
+    """Arguments that only fail with GPU tensors: counts and positions of the
+    wrong type, size or device; keys past the capacity; results unlike q."""
+    from delta_attention import ops
+    c = ops.kv8_empty(2, 2, 128, 64)
+    k = tokens(2, 3, 2, 64, torch.bfloat16, 1)
+    q = tokens(2, 1, 4, 64, torch.bfloat16, 2).transpose(1, 2)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    for bad in (i32(0, 1), torch.tensor([0, 1, 2], device="cuda"), torch.tensor([0, 1]), torch.tensor([[0, 1]], device="cuda"),
+                torch.arange(4, device="cuda")[::2], -1, 126):
+        with pytest.raises(AssertionError):
+            ops.kv8_write(c, k, k, bad)
+    with pytest.raises(AssertionError):
+        ops.kv8_write(c, k, k, 0, counts=torch.tensor([1, 2], device="cuda"))
+    with pytest.raises(AssertionError):
+        ops.kv8_write(c, k.cpu(), k, 0)
+    for bad in (129, -1, i32(1, 2, 3), torch.tensor([1, 2], device="cuda")):
+        with pytest.raises(AssertionError):
+            ops.kv8_attention(q, c, n_keys=bad, sm_scale=1.0)
+    with pytest.raises(AssertionError):
+        ops.kv8_attention(q, c, n_keys=1, sm_scale=1.0, out=torch.empty(2, 4, 1, 64, dtype=torch.float16, device="cuda"))
+    with pytest.raises(AssertionError):
+        ops.kv8_attention(q, c, n_keys=1, sm_scale=1.0, add=q[:, :2])
+    with pytest.raises(AssertionError):
+        ops.kv8_read(c, 0, 5, dtype=torch.float32)
+    # nothing to do is no error
+    assert ops.kv8_attention(q[:, :, :0], c, n_keys=1, sm_scale=1.0).shape == (2, 4, 0, 64)
+    assert ops.kv8_read(c, 7, 0)[0].shape == (2, 2, 0, 64)
+    ops.kv8_write(c, k[:, :0], k[:, :0], 128)
+
+
+def test_rows_in_place_and_unaligned(gpu):
+    """The result written over q; q and the tokens at addresses and strides that
+    are not 16-byte aligned."""
+    from delta_attention import ops
+    c, ref, counts = filled(2, 1, 1024, 64, [1000, 70], torch.bfloat16, 14)
+    q = tokens(2, 2, 4, 64, torch.bfloat16, 15, False).transpose(1, 2)
+    want = ops.kv8_attention(q, c, n_keys=counts, sm_scale=0.1)
+    raw = torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")[1:]
+    odd = raw.view(2, 4, 2, 64).copy_(q)
+    assert odd.data_ptr() % 16 and torch.equal(ops.kv8_attention(odd, c, n_keys=counts, sm_scale=0.1), want)
+    k = tokens(2, 5, 1, 64, torch.bfloat16, 16)
+    wide = torch.zeros(2, 5, 1, 67, dtype=k.dtype, device="cuda")
+    wide[..., 2:66] = k
+    c2 = ops.KV8(*(t.clone() for t in c))
+    ops.kv8_write(c, k, k, 1000)
+    ops.kv8_write(c2, wide[..., 2:66], wide[..., 2:66], 1000)
+    for a, b in zip(c, c2):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    qq = q.clone()
+    counts = counts.clone()
+    ops.kv8_attention(qq, c, n_keys=counts, sm_scale=0.1, out=qq)
+    assert torch.equal(qq, want)
 
 
 def test_rows_nan_in_masked_places(gpu):

@@ -138,7 +138,8 @@ def test_c_write_refusals(lib):
     assert call(D=96) == L.DA_ERR_HEAD_DIM
     for bad in (dict(cap=100), dict(cap=0), dict(cap=-64), dict(cap=(1 << 30) + 64), dict(Hkv=0), dict(B=-1), dict(S=-1),
                 dict(k=0), dict(v=0), dict(kc=0), dict(vc=0), dict(sk=0), dict(sv=0), dict(pos=-1), dict(pos=126),
-                dict(S=129), dict(pos=2 ** 62), dict(Hkv=2 ** 30)):
+                dict(S=129), dict(pos=2 ** 62), dict(Hkv=2 ** 30), dict(B=2, cs=(0, 64 * 128, 0, 64 * 128, 0, 2, 0, 2)),
+                dict(cs=(128 * 128, 64 * 128, 128 * 128, 64 * 128, 4, 0, 4, 2))):
         assert call(**bad) == L.DA_ERR_INVALID_ARG, bad
     for bad in (dict(k=24), dict(vc=24), dict(sk=18), dict(ks=(3 * 128, 129, 64)), dict(pos_dev=20), dict(counts=18),
                 dict(cs=(128 * 128 + 8, 64 * 128, 128 * 128, 64 * 128, 4, 2, 4, 2))):
