@@ -487,25 +487,18 @@ __device__ __forceinline__ Blocks blocks_of(const RowsArgs& a, int n) {
   return l;
 }
 
-#ifndef KV8_WAVES
-#define KV8_WAVES 4
-#endif
-#ifndef KV8_CMAX
-#define KV8_CMAX 64
-#endif
-#ifndef KV8_W128
-#define KV8_W128 2
-#endif
-constexpr int WAVES = KV8_WAVES;
+constexpr int WAVES = 4;
 // Waves per SIMD of the rows kernel: what the registers of a block's codes, the
 // sums and MT tiles of probabilities leave room for.
 __host__ __device__ constexpr int rows_waves(int D, int mt) {
-  return D * mt <= 64 ? (mt == 1 ? 4 : mt == 2 ? 3 : 2) : D * mt <= 128 ? (D == 128 ? KV8_W128 : 2) : 1;
+  return D * mt <= 64 ? (mt == 1 ? 4 : mt == 2 ? 3 : 2) : D * mt <= 128 ? 2 : 1;
 }
-constexpr int CHUNK = KV8_CMAX;              // blocks of an item at most, where there are many
+constexpr int CHUNK = 64;                    // blocks of an item at most, where there are many
 
-// Splits: every item takes `chunk` blocks of one (sequence, kv head, row tile);
-// chunk is the launch's blocks over the items asked for, so that sequences of
+// Splits: every item takes `chunk` blocks of one (sequence, kv head, row tile).
+// There are as many items as workgroups are resident together, or some rounds of
+// them where an item would exceed CHUNK blocks (eight sequences of 98K-131K keys
+// take 283 us at 64 blocks, 304 at 24, 320 at 16, 371 at 8); sequences of
 // different lengths give items of one size. An item's place is found by each
 // wave for itself: the sequences' item counts, summed over 64 lanes.
 // `blocks`: all sequences', kv heads' and row tiles' together (below 2^31).
@@ -531,8 +524,8 @@ __device__ __forceinline__ int scan64(int x) {
   return x;
 }
 
-// locate() among sequences of different lengths: 64 sequences to a lane each;
-// those of the first KEPT rounds stay in registers.
+// locate() among sequences of different lengths, 64 at a time with one to a
+// lane; the counts of the first KEPT rounds stay in registers.
 template <bool ITEM, int KEPT>
 __device__ __forceinline__ bool among(const RowsArgs& a, int i, Place& p, int& rest, int& first) {
   const int lane = threadIdx.x % 64, units = a.units.d, nu = KEPT == 1 ? 1 : (a.B + 63) / 64;
@@ -658,9 +651,22 @@ __device__ __forceinline__ void store4(const RowsArgs& a, int b, int h, int i, i
   *(u32x2*)((T*)a.o + b * a.o_b + h * a.o_h + i * a.o_s + d) = w;
 }
 
+// One item: its waves take its blocks in turn and are joined through LDS. A block
+// is one pass of S^T = K Q^T, the probabilities with a running reference, O^T =
+// V^T P^T; a block's codes go straight to registers, the next block's keys loaded
+// when the first product has read this one's, its values after the second.
+//
+// What bounds it: memory, where there is enough of it (a dense row of 32 / 8 heads
+// over 131072 keys 43.8 us, 6.1 TB/s with the first loads; eight sequences of that
+// length 6.65 TB/s); else a launch (1.9 us) and the loads that wait for each other
+// (arguments, count, codes: 5.2 us for a single block). Registers, not MFMA or
+// conversions, limit the waves (201 at head_dim 128 and one row tile).
+//
 // MT: 16-row tiles per wave. The P V product is formed in fp16 whatever Q's
 // type: the codes are exact in it, and its 11 bits keep the probabilities'
-// rounding below that of a bf16 result.
+// rounding below that of a bf16 result (bf16 probabilities would add as much
+// again to the result's own rounding error). Each tile's weights are summed by an
+// MFMA with ones, from the same rounded probabilities.
 template <typename T, int D, int MT>
 __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel(RowsArgs a) {
   constexpr int KS = D / 32;                 // steps of the Q K product
@@ -953,7 +959,9 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
   }
 }
 
-// Joins the items of one (sequence, kv head, row tile): a workgroup per row.
+// Joins the items of one (sequence, kv head, row tile): a workgroup per row, some
+// items side by side and four loads of each in flight. Launch and three dependent
+// loads: 3.5 us for 32 rows of 9 items, 5.2 for 32 of 64.
 template <typename T, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
   constexpr int CT = D / 4, SG = THREADS / CT; // threads across a row, items taken side by side
@@ -1088,8 +1096,9 @@ void launch_rows(const RowsArgs& a, const RowsPlan& p, hipStream_t st) {
   }
   if (p.bytes > 0) {
     const dim3 rows((unsigned)p.pairs, (unsigned)p.rows);
-    // wide workgroups where few rows have many items each (32 rows of 64: 5.6 us
-    // against 5.2, of 32 at head_dim 256 5.2 against 4.5; 768 rows of 16: 7.4 against 4.4)
+    // Wide workgroups where few rows have many items each: 32 rows of 64 items take
+    // 5.2 us (5.6 with 256 threads), 16 rows of 32 at head_dim 256 4.5 (5.2), but 768
+    // rows of 16 7.7 (4.4).
     if (p.items > 16 * p.pairs && p.pairs * p.rows <= 256) hipLaunchKernelGGL((kv8_join_kernel<T, D, 1024>), rows, dim3(1024), 0, st, a);
     else hipLaunchKernelGGL((kv8_join_kernel<T, D, 256>), rows, dim3(256), 0, st, a);
   }

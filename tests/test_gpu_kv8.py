@@ -295,6 +295,47 @@ def test_rows(gpu, B, Hkv, G, D, cap, n, s, window, sink, dtype):
         check_rows(got, q, ref, n, window, sink, scale, what=what + " host count")
 
 
+@pytest.mark.parametrize("seed", range(24))
+def test_random_runs(gpu, seed):
+    """Random shapes, types and lengths: a padded prompt, a chunk and tokens into
+    a cache of noise, then rows over it and a stretch read back."""
+    import random
+    from delta_attention import ops
+    r = random.Random(1000 + seed)
+    B, Hkv, G, D = r.choice([1, 1, 2, 3, 5]), r.choice([1, 2, 3]), r.choice([1, 2, 3, 4, 7, 9]), r.choice([32, 64, 128, 256])
+    dtype = DT[r.choice(["bf16", "fp16"])]
+    cap = 64 * r.randint(1, 9)
+    c, ref = garbage(ops.kv8_empty(B, Hkv, cap, D), seed), K8.new_cache(B, Hkv, cap, D)
+    n = [0] * B
+    print(f"seed {seed}: B{B} H{Hkv * G}/{Hkv} D{D} cap {cap} {dtype}", flush=True)
+    for step in range(r.randint(1, 4)):
+        S = min(r.choice([1, 1, r.randint(1, 40), r.randint(1, cap)]), cap - max(n))
+        if S < 1:
+            break
+        cnt = [S] * B if r.random() < 0.5 else [r.randint(0, S) for _ in range(B)]
+        k, v = (tokens(B, S, Hkv, D, dtype, seed * 50 + 2 * step + i) for i in (0, 1))
+        ops.kv8_write(c, k, v, torch.tensor(n, device="cuda"), counts=torch.tensor(cnt, dtype=torch.int32, device="cuda"))
+        K8.write(ref, np64(k), np64(v), n, cnt)
+        n = [a + b for a, b in zip(n, cnt)]
+    check_cache(c, ref, n)
+    s = r.choice([1, 1, 2, r.randint(1, 12), 33])
+    window = r.choice([0, 0, r.randint(1, cap), 2 ** 31 - 1])
+    sink = r.choice([0, r.randint(0, 130)])
+    scale = r.choice([D ** -0.5, 0.3, -0.05])
+    q = tokens(B, s, Hkv * G, D, dtype, seed, False).transpose(1, 2)
+    live = {x: np.nan_to_num(y) if x in ("k", "v") else y for x, y in ref.items()}   # (no key past n is looked at)
+    got = ops.kv8_attention(q, c, n_keys=torch.tensor(n, dtype=torch.int32, device="cuda"), window=window, sink=sink,
+                            sm_scale=scale)
+    check_rows(got, q, live, n, window, sink, scale, what=f"seed {seed} n{n} s{s} w{window} k{sink} scale {scale:.3f}")
+    a = r.randint(0, cap - 1)
+    m = r.randint(1, cap - a)
+    kk, vv = ops.kv8_read(c, a, m, n_keys=torch.tensor(n, dtype=torch.int32, device="cuda"), dtype=dtype)
+    for x, y in zip((kk, vv), K8.values(live, a, m)):
+        for b in range(B):
+            y[b, :, max(n[b] - a, 0):] = 0
+        assert same(np64(x), np64(torch.from_numpy(y).to(dtype)))
+
+
 def test_rows_large_scores(gpu):
     """Scores from -300 to 300 with the largest late: the running reference
     moves up many times, and rows end with one key's value."""
