@@ -1167,6 +1167,7 @@ extern "C" int da_kv8_write(const da_kv8_write_args* x, void* stream) {
   // blocks that S tokens touch: from a known row, or from any
   const int n_blk = x->pos_dev ? (int)(((int64_t)S + KB - 2) / KB + 1) : (int)((x->pos + S + KB - 1) / KB - x->pos / KB);
   if (!units_for(a.units, B, n_blk, Hkv, false)) return DA_ERR_INVALID_ARG;
+  (void)hipGetLastError();
   by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     using E = typename decltype(t)::type;
     const dim3 grid(units_grid(a.units)), block(256);
@@ -1197,6 +1198,7 @@ extern "C" int da_kv8_read(const da_kv8_read_args* x, void* stream) {
   a.start = start, a.n = n;
   const int n_blk = (int)(((int64_t)start + n + KB - 1) / KB - start / KB);
   if (!units_for(a.units, B, n_blk, x->cache.Hkv, true)) return DA_ERR_INVALID_ARG;
+  (void)hipGetLastError();
   by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     hipLaunchKernelGGL((kv8_read_kernel<typename decltype(t)::type, decltype(d)::value>), dim3(units_grid(a.units)),
                        dim3(256), 0, (hipStream_t)stream, a);
@@ -1256,6 +1258,7 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   a.heads = make_fastdiv(a.G);
   a.part = (float*)x->workspace;
   a.pitch = p.pitch;
+  (void)hipGetLastError();
   by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     launch_rows<typename decltype(t)::type, decltype(d)::value>(a, p, (hipStream_t)stream);
   });
