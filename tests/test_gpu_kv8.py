@@ -336,6 +336,31 @@ def test_random_runs(gpu, seed):
         assert same(np64(x), np64(torch.from_numpy(y).to(dtype)))
 
 
+def test_offsets_past_32_bits(gpu):
+    """Sequences of 16M tokens at head_dim 256: codes 4 GiB into a head, the
+    second sequence past them; tokens at both ends, a window's rows, a read."""
+    from delta_attention import ops
+    cap, D = 1 << 24, 256
+    c = ops.kv8_empty(2, 1, cap, D)
+    head = [tokens(2, 70, 1, D, torch.bfloat16, x, False) for x in (1, 2)]
+    tail = [tokens(2, 203, 1, D, torch.bfloat16, x, False) for x in (3, 4)]
+    ops.kv8_write(c, *head, 0)
+    at = cap - 204
+    ops.kv8_write(c, *tail, torch.tensor([at, at], device="cuda"))
+    one = [tokens(2, 1, 1, D, torch.bfloat16, x, False) for x in (5, 6)]
+    ops.kv8_write(c, *one, cap - 1)
+    # the same tokens in a short cache whose blocks lie alike: 70 at the start, 204 to the end
+    short = ops.kv8_empty(2, 1, 384, D)
+    ops.kv8_write(short, *head, 0)
+    ops.kv8_write(short, *tail, 384 - 204)
+    ops.kv8_write(short, *one, 383)
+    for x, y in zip(ops.kv8_read(c, at, 204), ops.kv8_read(short, 180, 204)):
+        assert torch.equal(x, y)
+    q = tokens(2, 2, 4, D, torch.bfloat16, 7, False).transpose(1, 2)
+    kw = dict(window=150, sink=70, sm_scale=0.06)
+    assert torch.equal(ops.kv8_attention(q, c, n_keys=cap, **kw), ops.kv8_attention(q, short, n_keys=384, **kw))
+
+
 def test_rows_large_scores(gpu):
     """Scores from -300 to 300 with the largest late: the running reference
     moves up many times, and rows end with one key's value."""
