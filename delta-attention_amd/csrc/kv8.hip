@@ -452,7 +452,7 @@ struct RowsArgs {
   int B, Hkv, G, s;         // G query heads per kv head, s rows at the end of each sequence
   int n_rt, rows;           // row tiles of `rows` rows (flattened row i * G + head) per sequence and kv head
   int window, sink;
-  float scale_log2;         // |sm_scale| * log2(e), above zero
+  float scale2;             // 2 |sm_scale| log2(e), above zero: references and differences are halves
   uint32_t flip;            // the sign bits of Q where sm_scale is negative
   int slots;                // workgroups that are resident together
   FastDiv round;            // blocks that they take at most: slots * CHUNK
@@ -461,11 +461,11 @@ struct RowsArgs {
   int64_t pitch;            // floats per item
 };
 
-constexpr float NO_KEYS = -3.4028234664e38f;   // the reference of a row without keys yet: below every finite score
-// Probabilities are held relative to a row reference (a score q k, not yet times
-// sm_scale: differences are taken before anything can overflow) that may lag its
-// maximum by up to LAG (log2), times 2^BIAS: at most 2^14, inside fp16, and fp16
-// ends 2^-32 below the reference.
+// Probabilities are held relative to a row reference (half a score q k, not yet
+// times sm_scale: half the difference of two finite scores is finite) that may lag
+// its maximum by up to LAG (log2), times 2^BIAS: at most 2^14, inside fp16, and
+// fp16 ends 2^-32 below the reference.
+constexpr float NO_KEYS = -FLT_MAX / 2;        // the reference of a row without keys yet: half the lowest score
 constexpr float LAG = 6.f, BIAS = 8.f;
 
 // The blocks that a sequence's rows see: those of the sinks, then [lo, hi).
@@ -824,9 +824,9 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, s[mt][e / 4][e % 4]);
       top = group_max(top);
-      if (__any((top - ref[mt]) * a.scale_log2 > LAG)) {
-        const float to = fmaxf(ref[mt], top);
-        const float alpha = ref[mt] == NO_KEYS ? 0.f : fast_exp2((ref[mt] - to) * a.scale_log2);
+      if (__any(fmaf(top, 0.5f, -ref[mt]) * a.scale2 > LAG)) {
+        const float to = fmaxf(ref[mt], top * 0.5f);
+        const float alpha = fast_exp2((ref[mt] - to) * a.scale2);
         ref[mt] = to;
 #pragma unroll
         for (int r = 0; r < 4; ++r) sum[mt][r] *= alpha;
@@ -836,7 +836,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
           for (int r = 0; r < 4; ++r) acc[mt][t][r] *= alpha;
       }
       auto weight = [&](float y) __attribute__((always_inline)) {
-        return fast_exp2(fmaf(y - ref[mt], a.scale_log2, BIAS));
+        return fast_exp2(fmaf(fmaf(y, 0.5f, -ref[mt]), a.scale2, BIAS));
       };
 #pragma unroll
       for (int u = 0; u < 2; ++u)
@@ -936,7 +936,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
       f32x4 o = {0, 0, 0, 0};
 #pragma unroll
       for (int w = 0; w < WAVES; ++w) {
-        const float k = fast_exp2((s_m[w][r] - M) * a.scale_log2);
+        const float k = fast_exp2((s_m[w][r] - M) * a.scale2);
         const f32x4 y = *(const f32x4*)&s_o[w][r][d];
         L = fmaf(s_l[w][r], k, L);
 #pragma unroll
@@ -994,7 +994,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
     for (int u = 0; u < U; ++u) {
       if (i0 + u * SG >= p.n_split) break;
       const float to = fmaxf(M, mi[u]);
-      const float k0 = fast_exp2((M - to) * a.scale_log2), k1 = fast_exp2((mi[u] - to) * a.scale_log2);
+      const float k0 = fast_exp2((M - to) * a.scale2), k1 = fast_exp2((mi[u] - to) * a.scale2);
       M = to;
       L = L * k0 + li[u] * k1;
 #pragma unroll
@@ -1014,7 +1014,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
   o = (f32x4){0, 0, 0, 0};
 #pragma unroll 4
   for (int i = 0; i < used; ++i) {
-    const float k = fast_exp2((s_w[i][0] - M) * a.scale_log2);
+    const float k = fast_exp2((s_w[i][0] - M) * a.scale2);
     const f32x4 y = s_o[i][t];
     L = fmaf(s_w[i][1], k, L);
 #pragma unroll
@@ -1248,8 +1248,9 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   a.n = x->n_keys;
   a.B = B, a.Hkv = Hkv, a.G = Hq / Hkv, a.s = s;
   a.n_rt = p.n_rt, a.rows = p.rows;
-  // (a scale of zero, which weighs every key alike, as the smallest one)
-  a.scale_log2 = fminf(fmaxf(fabsf(x->sm_scale) * 1.4426950408889634f, FLT_MIN), FLT_MAX);
+  // (a scale of zero, which weighs every key alike, as the smallest one: it moves
+  // no weight by more than 2^-20, and a masked score's -inf stays -inf)
+  a.scale2 = fminf(fmaxf(fabsf(x->sm_scale) * (2 * 1.4426950408889634f), FLT_TRUE_MIN), FLT_MAX);
   a.flip = x->sm_scale < 0.f ? 0x80008000u : 0;
   a.slots = p.slots;
   a.round = p.round;

@@ -414,6 +414,26 @@ def test_rows_huge_scores_and_infinite_queries(gpu):
     assert torch.equal(low[0, 0, 0], vv[0, 0, 0])
 
 
+@pytest.mark.parametrize("early,late,scale", [(-3e38, -9e37, 2e-38), (-3e38, 3e38, 1.2e-38), (3e38, -3e38, 1.2e-38)])
+def test_rows_scores_of_floats_ends(gpu, early, late, scale):
+    """Scores near float32's ends under a scale near its smallest: a wave's
+    first blocks, which such a scale leaves within reach of a row without keys,
+    still count when later blocks move the row's reference, and so do keys
+    further from the largest score than float32 reaches."""
+    from delta_attention import ops
+    B, Hkv, n, D = 64, 16, 1024, 32                   # one item per head, four blocks a wave
+    k = torch.zeros(B, n, Hkv, D, dtype=torch.bfloat16, device="cuda")
+    k[..., 0] = early / 2e19
+    k[:, -64:, :, 0] = late / 2e19
+    v = tokens(B, n, Hkv, D, torch.bfloat16, 3, False)
+    c = ops.kv8_empty(B, Hkv, n, D)
+    ops.kv8_write(c, k, v, 0)
+    q = torch.zeros(B, Hkv, 1, D, dtype=torch.bfloat16, device="cuda")
+    q[..., 0] = 2e19
+    got = ops.kv8_attention(q, c, n_keys=n, sm_scale=scale)
+    check_rows(got, q, to_oracle(c), [n] * B, 0, 0, float(np.float32(scale)), what=f"scores {early} then {late}")
+
+
 def test_rows_shared_prefix_and_refused_writes(gpu):
     """One sequence's cache expanded over a batch serves its rows (a shared
     prompt); writing through the expansion is refused."""
