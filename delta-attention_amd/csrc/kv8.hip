@@ -105,19 +105,24 @@ struct Cache {
 
 template <int N> struct alignas(N < 4 ? 4 * N : 16) Words { uint32_t w[N]; };
 
-// One wave per (sequence, block, head, tensor), four to a workgroup.
+// The (sequence, block, head, tensor) of a workgroup or wave.
 struct Units {
-  FastDiv inner, per_seq;      // waves of a block or of a head's tensor, of a sequence
+  FastDiv inner, per_seq;      // of a block or of a head's tensor, of a sequence
   uint32_t n, heads;
 };
 
-// Writes: heads innermost (a token's heads lie together in the input), and each
-// eighth of the waves on one XCD (workgroup x runs on XCD x % 8; the grid is a
-// multiple of 8), with non-temporal loads of the input: a prompt of 131072
-// tokens takes 145 us so, 157 in launch order, 151 with ordinary loads.
+// Writes: heads innermost (a token's heads lie together in the input), 16
+// workgroups beside each other on one XCD (workgroup x runs on XCD x % 8), the
+// XCDs beside each other too. A prompt of 131072 tokens takes 143 us so, 168 in
+// launch order, 149 with an eighth of the write to each XCD; 32 x 4000 tokens of
+// 8 heads of 128 118, 111 and 118 us.
+constexpr int WRITE_GROUP = 16;
+
+template <int PER_WG>
 __device__ __forceinline__ bool write_unit(const Units& u, int& b, int& j, int& h, bool& is_v) {
-  const uint32_t x = blockIdx.x, wg = x % 8 * (gridDim.x / 8) + x / 8;
-  const uint32_t i = wg * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t x = blockIdx.x, first = x / (8 * WRITE_GROUP) * (8 * WRITE_GROUP);
+  const uint32_t wg = first + 8 * WRITE_GROUP <= gridDim.x ? first + x % 8 * WRITE_GROUP + x / 8 % WRITE_GROUP : x;
+  const uint32_t i = wg * PER_WG + (PER_WG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
   if (i >= u.n) return false;
   b = fdiv(i, u.per_seq);
   const uint32_t rest = i - b * u.per_seq.d;
@@ -144,10 +149,18 @@ __device__ __forceinline__ bool read_unit(const Units& u, int& b, int& j, int& h
 }
 
 // ---------------------------------------------------------------------------
-// write: one wave per block, head and tensor. A lane holds 8 columns of D / 8
-// tokens, those of consecutive places, so that keys (8 bytes of a row) and
-// values (D / 8 bytes of a column) are both packed inside the lane; only the
-// block's largest magnitude crosses lanes.
+// write: a workgroup of D / 32 waves per block, head and tensor. A lane holds 8
+// columns of 4 tokens of consecutive places, so that keys (8 bytes of a row) and
+// values (4 bytes of a column) are both packed inside the lane; only the block's
+// largest magnitude crosses lanes, and waves through LDS.
+//
+// Memory bounds long writes (5.6 TB/s), one block's chain of loads, maximum and
+// stores short ones: the more waves share a block, the shorter. One wave for all
+// of it (D / 8 tokens a lane) took 8.1 us for a block of 8 heads of 128 and 14.5
+// of 256 (3.7 and 4.3 so), 8 tokens a lane 5.7 and 6.2; 32 x 2000 tokens of 8
+// heads of 256 take 109 us so, 154 and 127.
+constexpr int TPL = 4;                         // tokens per lane
+
 struct WriteArgs {
   Cache c;
   const void *k, *v;
@@ -160,15 +173,22 @@ struct WriteArgs {
   Units units;
 };
 
+template <int D> struct WriteShape {
+  static constexpr int W = D / 8 / TPL;        // waves of a block
+  static constexpr int PER_WG = W == 1 ? 4 : 1;
+  static constexpr int THREADS = 64 * W * PER_WG;
+};
+
 template <typename T, int D>
-__global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
+__global__ __launch_bounds__(WriteShape<D>::THREADS) void kv8_write_kernel(WriteArgs a) {
   using E = Elt<T>;
-  constexpr int DG = D / 8, TPL = D / 8;       // lanes across a row, tokens per lane
-  using Run = Words<TPL / 4>;
+  constexpr int DG = D / 8, W = WriteShape<D>::W;   // lanes across a row, waves of the block
+  __shared__ uint32_t s_top[2][W];
+  __shared__ int s_e;
   int b, j, h;
   bool is_v;
-  if (!write_unit(a.units, b, j, h, is_v)) return;
-  const int lane = threadIdx.x % 64;
+  if (!write_unit<WriteShape<D>::PER_WG>(a.units, b, j, h, is_v)) return;
+  const int lane = threadIdx.x % 64, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int64_t pos = a.pos_dev ? a.pos_dev[(int64_t)b * a.pos_step] : a.pos;
   const int count = a.counts ? min(max(a.counts[(int64_t)b * a.counts_step], 0), a.S) : a.S;
   if (pos < 0 || pos > (int64_t)a.c.cap - count) return;
@@ -178,18 +198,33 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
   if (r1 <= r0) return;
   const bool full = r0 == 0 && r1 == KB;
 
-  const int dg = lane % DG, p0 = lane / DG * TPL;
+  // Keys: the waves share out the tokens. Values: the columns, so that runs of 64
+  // bytes are stored whole (by tokens a block of 8 heads of 256 takes 6.4 us, not
+  // 4.3, 32 x 2000 tokens 158, not 115).
+  const int dg = is_v ? wave * TPL + lane % TPL : lane % DG;
+  const int p0 = (is_v ? lane / TPL : (wave * 64 + lane) / DG) * TPL;
   const T* src = is_v ? (const T*)a.v + b * a.vx_b + h * a.vx_h : (const T*)a.k + b * a.kx_b + h * a.kx_h;
   const int64_t step = is_v ? a.vx_s : a.kx_s;
   src += (int64_t)(base - (int)pos) * step + dg * 8;
+  float* scale = (is_v ? a.c.vs + b * a.c.vs_b + h * a.c.vs_h : a.c.ks + b * a.c.ks_b + h * a.c.ks_h) + blk;
   u32x4 x[TPL];
   uint32_t fresh = 0, older = 0;               // bit i: token i of this lane is new, or holds an earlier token
 #pragma unroll
   for (int i = 0; i < TPL; ++i) {
     const int r = token_of(p0 + i);
-    x[i] = ld_nt4(src + (int64_t)min(max(r, r0), r1 - 1) * step);
+    // non-temporal where the loads are whole lines, else ordinary (32 x 2000 tokens
+    // of 8 heads of 32: 14.7 us, 23.0 non-temporal)
+    const T* at = src + (int64_t)min(max(r, r0), r1 - 1) * step;
+    x[i] = (is_v ? TPL : DG) * 16 < 128 ? *(const u32x4*)at : ld_nt4(at);
     fresh |= (uint32_t)(r >= r0 && r < r1) << i;
     older |= (uint32_t)(r < r0) << i;
+  }
+  const float before = r0 > 0 && wave == 0 ? *scale : 0.f;
+  uint32_t was[8];                             // a part block's other tokens share its values' words
+  uint8_t* vdst = a.c.v + b * a.c.v_b + h * a.c.v_h + (int64_t)blk * KB * D + dg * 8 * KB + p0;
+  if (is_v && !full) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) was[n] = *(const uint32_t*)(vdst + n * KB);
   }
   u16x2 m = {0, 0};
 #pragma unroll
@@ -198,7 +233,19 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
     for (int w = 0; w < 4; ++w)
       m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[i][w] & 0x7fff7fffu));
   }
-  uint32_t top = wave_max(max((uint32_t)m.x, (uint32_t)m.y));
+  // the largest of all the waves'
+  auto joined = [&](uint32_t x, int i) __attribute__((always_inline)) {
+    x = wave_max(x);
+    if constexpr (W > 1) {
+      if (lane == 0) s_top[i][wave] = x;
+      if (i == 0 && wave == 0 && lane == 0) s_e = scale_exponent(before);
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; ++w) x = max(x, s_top[i][w]);
+    }
+    return x;
+  };
+  uint32_t top = joined(max((uint32_t)m.x, (uint32_t)m.y), 0);
   const bool odd = top >= Half<T>::inf;        // infinities or NaN among them
   if (odd) {
     top = 0;
@@ -209,20 +256,19 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
         const uint32_t lo = x[i][w] & 0x7fffu, hi = x[i][w] >> 16 & 0x7fffu;
         top = max(top, max(lo < Half<T>::inf ? lo : 0u, hi < Half<T>::inf ? hi : 0u));
       }
-    top = wave_max(top);
+    top = joined(top, 1);
   }
   int e = block_exponent(E::lo(top));
-  float* scale = (is_v ? a.c.vs + b * a.c.vs_b + h * a.c.vs_h : a.c.ks + b * a.c.ks_b + h * a.c.ks_h) + blk;
   bool grown = false;
   float f = 1.f;
   if (r0 > 0) {
-    const int eo = scale_exponent(*scale);
+    const int eo = W > 1 ? s_e : scale_exponent(before);
     grown = e > eo;
     if (grown) f = pow2(eo) * pow2(-e);        // (0 where that is below the floats: so are the values)
     e = max(e, eo);
   }
   const float inv = pow2(-e);
-  if (lane == 0) *scale = pow2(e);
+  if (wave == 0 && lane == 0) *scale = pow2(e);
   // a finite value is at most 448 after the scale; the others become NaN
   auto val = [&](uint32_t w, bool hi) __attribute__((always_inline)) {
     const float y = (hi ? E::hi(w) : E::lo(w)) * inv;
@@ -247,76 +293,83 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(WriteArgs a) {
       }
     }
   } else {
-    uint8_t* dst = a.c.v + b * a.c.v_b + h * a.c.v_h + (int64_t)blk * KB * D + dg * 8 * KB + p0;
-    Run was[8];                                // a part block's other tokens share its runs
-    if (!full) {
-#pragma unroll
-      for (int n = 0; n < 8; ++n) was[n] = *(const Run*)(dst + n * KB);
-    }
+    const uint32_t nm = byte_mask(fresh), om = grown ? byte_mask(older) : 0;
 #pragma unroll
     for (int n = 0; n < 8; ++n) {
-      Run w;
-#pragma unroll
-      for (int q = 0; q < TPL / 4; ++q) {
-        int c = __builtin_amdgcn_cvt_pk_fp8_f32(val(x[4 * q][n / 2], n & 1), val(x[4 * q + 1][n / 2], n & 1), 0, false);
-        w.w[q] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(val(x[4 * q + 2][n / 2], n & 1), val(x[4 * q + 3][n / 2], n & 1), c, true);
-        if (!full) {
-          const uint32_t o = was[n].w[q];
-          const uint32_t nm = byte_mask(fresh >> 4 * q), om = grown ? byte_mask(older >> 4 * q) : 0;
-          w.w[q] = (w.w[q] & nm) | (move4(o, f) & om) | (o & ~(nm | om));
-        }
-      }
-      *(Run*)(dst + n * KB) = w;
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(val(x[0][n / 2], n & 1), val(x[1][n / 2], n & 1), 0, false);
+      uint32_t w = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(val(x[2][n / 2], n & 1), val(x[3][n / 2], n & 1), c, true);
+      if (!full) w = (w & nm) | (move4(was[n], f) & om) | (was[n] & ~(nm | om));
+      *(uint32_t*)(vdst + n * KB) = w;
     }
   }
 }
 
-// One token per sequence (a decode step): one wave per sequence, head and
-// tensor, a lane 8 columns of the token. The block's other tokens are touched
-// only where the token needs a larger scale than theirs. What counts is the
-// chain position -> token -> its largest magnitude -> stores; the block-sized
-// kernel above, which also loads the block's runs, takes 4 us more (10.7 us to 2.7
-// in a captured step's launch, before it loaded them early).
-template <typename T, int D>
+// A few tokens per sequence (a decode step's one, drafted ones): one wave per
+// sequence, block, head and tensor, a lane 8 columns of NP tokens. The block's
+// other tokens are touched only where the new ones need a larger scale than
+// theirs, and the tokens' loads wait for nothing. 4 tokens of 32 sequences of 8
+// heads of 256 take 5.1 us (by the kernel above 8.8), 8 of 128 4.8 (5.9), 16 of 64
+// 3.8 (4.5). With four passes 8 tokens of 256 take 7.1 (8.9), but those of a single
+// sequence 6.2 (4.3): two at most.
+// ONE: a single token, which every lane group then holds (2.8 us, 3.0 without).
+template <typename T, int D, int NP, bool ONE>
 __global__ __launch_bounds__(256) void kv8_append_kernel(WriteArgs a) {
   using E = Elt<T>;
-  constexpr int DG = D / 8;
+  constexpr int DG = D / 8, AT_ONCE = 64 / DG;  // lanes across a token, tokens side by side
   int b, j, h;
   bool is_v;
-  if (!write_unit(a.units, b, j, h, is_v)) return;
-  const int lane = threadIdx.x % 64, dg = lane % DG;
+  if (!write_unit<4>(a.units, b, j, h, is_v)) return;
+  const int lane = threadIdx.x % 64, dg = lane % DG, t0 = lane / DG;
   const T* src = is_v ? (const T*)a.v + b * a.vx_b + h * a.vx_h : (const T*)a.k + b * a.kx_b + h * a.kx_h;
-  const u32x4 x = *(const u32x4*)(src + dg * 8);
+  const int64_t step = is_v ? a.vx_s : a.kx_s;
+  u32x4 x[NP];
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int t = i * AT_ONCE + t0;
+    x[i] = *(const u32x4*)(ONE ? src + dg * 8 : src + min(t, a.S - 1) * step + dg * 8);
+  }
   const int64_t pos = a.pos_dev ? a.pos_dev[(int64_t)b * a.pos_step] : a.pos;
-  const int count = a.counts ? a.counts[(int64_t)b * a.counts_step] : 1;
-  if (pos < 0 || pos >= a.c.cap || count < 1) return;
-  const int blk = (int)(pos / KB), r = (int)(pos % KB);
+  const int S = ONE ? 1 : a.S, count = a.counts ? min(max(a.counts[(int64_t)b * a.counts_step], 0), S) : S;
+  if (pos < 0 || pos > (int64_t)a.c.cap - count) return;
+  if (ONE) j = 0;                              // (its only block)
+  const int blk = (int)(pos / KB) + j, r0 = j == 0 ? (int)(pos % KB) : 0;   // the first new row's
+  const int lo = j == 0 ? 0 : blk * KB - (int)pos, hi = min(count, (blk + 1) * KB - (int)pos);
+  if (ONE ? count < 1 : hi <= lo) return;      // tokens lo .. hi - 1 are this block's
+  auto mine = [&](int i) __attribute__((always_inline)) {
+    const int t = i * AT_ONCE + t0;
+    return ONE || (t >= lo && t < hi);         // (one token: every lane group holds it)
+  };
   float* scale = (is_v ? a.c.vs + b * a.c.vs_b + h * a.c.vs_h : a.c.ks + b * a.c.ks_b + h * a.c.ks_h) + blk;
   const float before = *scale;
 
   u16x2 m = {0, 0};
 #pragma unroll
-  for (int w = 0; w < 4; ++w) m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, x[w] & 0x7fff7fffu));
+  for (int i = 0; i < NP; ++i)
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, mine(i) ? x[i][w] & 0x7fff7fffu : 0u));
   uint32_t top = wave_max(max((uint32_t)m.x, (uint32_t)m.y));
   const bool odd = top >= Half<T>::inf;        // infinities or NaN among them
   if (odd) {
     top = 0;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const uint32_t lo = x[w] & 0x7fffu, hi = x[w] >> 16 & 0x7fffu;
-      top = max(top, max(lo < Half<T>::inf ? lo : 0u, hi < Half<T>::inf ? hi : 0u));
-    }
+    for (int i = 0; i < NP; ++i)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t y = mine(i) ? x[i][w] : 0u, even = y & 0x7fffu, next = y >> 16 & 0x7fffu;
+        top = max(top, max(even < Half<T>::inf ? even : 0u, next < Half<T>::inf ? next : 0u));
+      }
     top = wave_max(top);
   }
   int e = block_exponent(E::lo(top));
   uint8_t* block = is_v ? a.c.v + b * a.c.v_b + h * a.c.v_h + (int64_t)blk * KB * D
                         : a.c.k + b * a.c.k_b + h * a.c.k_h + (int64_t)blk * KB * D;
-  if (r > 0) {
+  if (r0 > 0) {
     const int eo = scale_exponent(before);
     if (e > eo) {                              // the earlier tokens' codes move to the new scale
       const float f = pow2(eo) * pow2(-e);
       if (!is_v) {
-        for (int i = lane; i < r * D / 16; i += 64) {
+        for (int i = lane; i < r0 * D / 16; i += 64) {
           u32x4* c = (u32x4*)block + i;
           const u32x4 w = *c;
           *c = (u32x4){move4(w[0], f), move4(w[1], f), move4(w[2], f), move4(w[3], f)};
@@ -327,13 +380,13 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(WriteArgs a) {
           u32x4 w = *c;
 #pragma unroll
           for (int t = 0; t < 4; ++t) {        // tokens 16 t + 4 (i % 4) + 0 .. 3
-            const int n = min(max(r - 16 * t - 4 * (i % 4), 0), 4);
+            const int n = min(max(r0 - 16 * t - 4 * (i % 4), 0), 4);
             const uint32_t om = n == 4 ? 0xffffffffu : (1u << 8 * n) - 1;
             w[t] = (move4(w[t], f) & om) | (w[t] & ~om);
           }
           *c = w;
         }
-        __threadfence_block();                 // the token's bytes below lie in these words
+        __threadfence_block();                 // the new tokens' bytes below lie in these words
       }
     }
     e = max(e, eo);
@@ -344,19 +397,23 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(WriteArgs a) {
     const float y = (hi ? E::hi(w) : E::lo(w)) * inv;
     return odd && !(fabsf(y) < 512.f) ? __builtin_nanf("") : y;
   };
-  if (lane >= DG) return;
-  u32x2 c;
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(val(x[2 * n], false), val(x[2 * n], true), 0, false);
-    c[n] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(val(x[2 * n + 1], false), val(x[2 * n + 1], true), lo, true);
-  }
-  if (!is_v) {
-    *(u32x2*)(block + r * D + dg * 8) = c;
-  } else {
-    uint8_t* dst = block + dg * 8 * KB + place_of(r);
+  for (int i = 0; i < NP; ++i) {
+    if (ONE ? t0 > 0 : !mine(i)) continue;
+    const int r = ONE ? r0 : r0 + i * AT_ONCE + t0 - lo;
+    u32x2 c;
 #pragma unroll
-    for (int n = 0; n < 8; ++n) dst[n * KB] = (uint8_t)(c[n / 4] >> 8 * (n % 4));
+    for (int n = 0; n < 2; ++n) {
+      const int lo2 = __builtin_amdgcn_cvt_pk_fp8_f32(val(x[i][2 * n], false), val(x[i][2 * n], true), 0, false);
+      c[n] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(val(x[i][2 * n + 1], false), val(x[i][2 * n + 1], true), lo2, true);
+    }
+    if (!is_v) {
+      *(u32x2*)(block + r * D + dg * 8) = c;
+    } else {
+      uint8_t* dst = block + dg * 8 * KB + place_of(r);
+#pragma unroll
+      for (int n = 0; n < 8; ++n) dst[n * KB] = (uint8_t)(c[n / 4] >> 8 * (n % 4));
+    }
   }
 }
 
@@ -1119,10 +1176,11 @@ void by_type(int dtype, int D, F&& f) {
   else dims(Tag<_Float16>{});
 }
 
-// Waves of a write or read (below 2^31).
-bool units_for(Units& u, int B, int n_blk, int Hkv, bool read) {
-  const int64_t n = (int64_t)B * n_blk * 2 * Hkv;
-  if ((int64_t)n_blk * 2 * Hkv > 0x7fffff00 || n > 0x7fffff00) return false;
+// Blocks of a write or read, of `waves` waves each.
+bool units_for(Units& u, int B, int n_blk, int Hkv, int waves, bool read) {
+  const int64_t per_seq = (int64_t)n_blk * 2 * Hkv, most = 0x3ffff00 / waves;   // (threads of a grid: below 2^32)
+  if (per_seq > most || per_seq * B > most) return false;
+  const int64_t n = per_seq * B;
   u = Units{make_fastdiv(read ? n_blk : 2 * Hkv), make_fastdiv(n_blk * 2 * Hkv), (uint32_t)n, (uint32_t)Hkv};
   return true;
 }
@@ -1166,13 +1224,17 @@ extern "C" int da_kv8_write(const da_kv8_write_args* x, void* stream) {
   a.S = S;
   // blocks that S tokens touch: from a known row, or from any
   const int n_blk = x->pos_dev ? (int)(((int64_t)S + KB - 2) / KB + 1) : (int)((x->pos + S + KB - 1) / KB - x->pos / KB);
-  if (!units_for(a.units, B, n_blk, Hkv, false)) return DA_ERR_INVALID_ARG;
+  if (!units_for(a.units, B, n_blk, Hkv, x->cache.D / (8 * TPL), false)) return DA_ERR_INVALID_ARG;
   (void)hipGetLastError();
   by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     using E = typename decltype(t)::type;
-    const dim3 grid(units_grid(a.units)), block(256);
-    if (S == 1) hipLaunchKernelGGL((kv8_append_kernel<E, decltype(d)::value>), grid, block, 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((kv8_write_kernel<E, decltype(d)::value>), grid, block, 0, (hipStream_t)stream, a);
+    constexpr int DIM = decltype(d)::value, AT_ONCE = 512 / DIM;
+    using Shape = WriteShape<DIM>;
+    const auto grid = [&](int per_wg) { return dim3((a.units.n + per_wg - 1) / per_wg); };
+    if (S == 1) hipLaunchKernelGGL((kv8_append_kernel<E, DIM, 1, true>), grid(4), dim3(256), 0, (hipStream_t)stream, a);
+    else if (S <= AT_ONCE) hipLaunchKernelGGL((kv8_append_kernel<E, DIM, 1, false>), grid(4), dim3(256), 0, (hipStream_t)stream, a);
+    else if (S <= 2 * AT_ONCE) hipLaunchKernelGGL((kv8_append_kernel<E, DIM, 2, false>), grid(4), dim3(256), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((kv8_write_kernel<E, DIM>), grid(Shape::PER_WG), dim3(Shape::THREADS), 0, (hipStream_t)stream, a);
   });
   return launched();
 }
@@ -1197,7 +1259,7 @@ extern "C" int da_kv8_read(const da_kv8_read_args* x, void* stream) {
   a.n_step = x->n_keys_per_seq ? 1 : 0;
   a.start = start, a.n = n;
   const int n_blk = (int)(((int64_t)start + n + KB - 1) / KB - start / KB);
-  if (!units_for(a.units, B, n_blk, x->cache.Hkv, true)) return DA_ERR_INVALID_ARG;
+  if (!units_for(a.units, B, n_blk, x->cache.Hkv, 1, true)) return DA_ERR_INVALID_ARG;
   (void)hipGetLastError();
   by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     hipLaunchKernelGGL((kv8_read_kernel<typename decltype(t)::type, decltype(d)::value>), dim3(units_grid(a.units)),

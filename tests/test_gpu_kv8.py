@@ -85,6 +85,35 @@ def to_oracle_bytes(c):
     return c.k.view(torch.uint8).cpu().numpy(), v, c.k_scale.cpu().numpy(), c.v_scale.cpu().numpy()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_write_few_tokens(gpu, D, dtype):
+    """A few tokens behind others, from two to more than the calls for few
+    tokens take: inside a block, across two, at a block's first and last row,
+    right-padded (to none in one sequence), with larger scales than the block's
+    and with infinities and NaN."""
+    from delta_attention import ops
+    B, Hkv, cap, at_once = 5, 3, 192, 512 // D
+    for S in (2, 3, at_once, at_once + 1, 2 * at_once, 2 * at_once + 1, 3 * at_once + 2, 64):
+        c, ref = garbage(ops.kv8_empty(B, Hkv, cap, D), S), K8.new_cache(B, Hkv, cap, D)
+        pos = [7, 64 - S // 2, 64, 127, 128 - S]
+        k0, v0 = (tokens(B, 128, Hkv, D, DT[dtype], 50 + S + s) * 0.25 for s in (0, 1))
+        counts = torch.tensor(pos, dtype=torch.int32, device="cuda")
+        ops.kv8_write(c, k0, v0, 0, counts=counts)
+        K8.write(ref, np64(k0), np64(v0), [0] * B, pos)
+        for ragged, new in ((False, [S] * B), (True, [S, S - 1, 1, 0, S // 2 + 1])):
+            k, v = (tokens(B, S, Hkv, D, DT[dtype], 70 + S + s) for s in (0, 1))
+            k[0, S // 2, 1, 3], v[1, 0, 2, 5], v[2, 0, 0, 1] = float("inf"), float("nan"), 300.0
+            given = torch.tensor(new, dtype=torch.int32, device="cuda") if ragged else None
+            was = to_oracle_bytes(c)[:2]
+            ops.kv8_write(c, k, v, torch.tensor(pos, device="cuda"), counts=given)
+            K8.write(ref, np64(k), np64(v), pos, new)
+            check_cache(c, ref, [a + n for a, n in zip(pos, new)])
+            now = to_oracle_bytes(c)[:2]
+            for b, (a, n) in enumerate(zip(pos, new)):     # rows behind keep their bytes
+                assert all(same(x[b, :, a + n:], y[b, :, a + n:]) for x, y in zip(was, now)), (S, b)
+
+
 @pytest.mark.parametrize("D", [32, 64, 128, 256])
 def test_write_token_by_token(gpu, D):
     """Tokens appended one at a time, each larger than the last by up to 2^12:
