@@ -103,7 +103,14 @@ struct Cache {
   int cap;
 };
 
-template <int N> struct alignas(N < 4 ? 4 * N : 16) Words { uint32_t w[N]; };
+// Writes and reads deal groups of G workgroups beside each other to the XCDs in
+// turn (workgroup x runs on XCD x % 8), so that the XCDs work beside each other
+// too; a last, incomplete round stays in launch order.
+template <int G>
+__device__ __forceinline__ uint32_t dealt() {
+  const uint32_t x = blockIdx.x, first = x / (8 * G) * (8 * G);
+  return first + 8 * G <= gridDim.x ? first + x % 8 * G + x / 8 % G : x;
+}
 
 // The (sequence, block, head, tensor) of a workgroup or wave.
 struct Units {
@@ -111,18 +118,13 @@ struct Units {
   uint32_t n, heads;
 };
 
-// Writes: heads innermost (a token's heads lie together in the input), 16
-// workgroups beside each other on one XCD (workgroup x runs on XCD x % 8), the
-// XCDs beside each other too. A prompt of 131072 tokens takes 143 us so, 168 in
-// launch order, 149 with an eighth of the write to each XCD; 32 x 4000 tokens of
-// 8 heads of 128 118, 111 and 118 us.
-constexpr int WRITE_GROUP = 16;
-
+// Writes: heads innermost (a token's heads lie together in the input). A prompt
+// of 131072 tokens takes 143 us in groups of 16, 166 of 8, 168 in launch order,
+// 149 with an eighth of the write to each XCD; 32 x 4000 tokens of 8 heads of 128
+// 118, 117, 111 and 118 us.
 template <int PER_WG>
 __device__ __forceinline__ bool write_unit(const Units& u, int& b, int& j, int& h, bool& is_v) {
-  const uint32_t x = blockIdx.x, first = x / (8 * WRITE_GROUP) * (8 * WRITE_GROUP);
-  const uint32_t wg = first + 8 * WRITE_GROUP <= gridDim.x ? first + x % 8 * WRITE_GROUP + x / 8 % WRITE_GROUP : x;
-  const uint32_t i = wg * PER_WG + (PER_WG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
+  const uint32_t i = dealt<16>() * PER_WG + (PER_WG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x / 64) : 0);
   if (i >= u.n) return false;
   b = fdiv(i, u.per_seq);
   const uint32_t rest = i - b * u.per_seq.d;
@@ -133,11 +135,14 @@ __device__ __forceinline__ bool write_unit(const Units& u, int& b, int& j, int& 
   return true;
 }
 
-// Reads: a head's blocks innermost (both sides are contiguous along them), with
-// non-temporal stores: 131072 rows take 145 us so, 167 with heads innermost,
-// 174 with ordinary stores too.
-__device__ __forceinline__ bool read_unit(const Units& u, int& b, int& j, int& h, bool& is_v) {
-  const uint32_t i = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+// Reads: a head's blocks innermost (both sides are contiguous along them), each
+// of W waves. 131072 rows of 8 heads of 256 take 267 us in groups of 8, 276 of 4,
+// 257 of 16, 270 in launch order; 32 x 200 14.7, 15.3, 15.1 and 19.3, 32 x 4000
+// of 128 132, 132, 140 and 132.
+template <int W>
+__device__ __forceinline__ bool read_unit(const Units& u, int& b, int& j, int& h, bool& is_v, int& part) {
+  const uint32_t k = dealt<8>() * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x / 64), i = k / W;
+  part = k % W;
   if (i >= u.n) return false;
   b = fdiv(i, u.per_seq);
   const uint32_t rest = i - b * u.per_seq.d;
@@ -173,21 +178,21 @@ struct WriteArgs {
   Units units;
 };
 
-template <int D> struct WriteShape {
+template <int D> struct Shape {
   static constexpr int W = D / 8 / TPL;        // waves of a block
-  static constexpr int PER_WG = W == 1 ? 4 : 1;
+  static constexpr int PER_WG = W == 1 ? 4 : 1;   // blocks of a writing workgroup
   static constexpr int THREADS = 64 * W * PER_WG;
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(WriteShape<D>::THREADS) void kv8_write_kernel(WriteArgs a) {
+__global__ __launch_bounds__(Shape<D>::THREADS) void kv8_write_kernel(WriteArgs a) {
   using E = Elt<T>;
-  constexpr int DG = D / 8, W = WriteShape<D>::W;   // lanes across a row, waves of the block
+  constexpr int DG = D / 8, W = Shape<D>::W;   // lanes across a row, waves of the block
   __shared__ uint32_t s_top[2][W];
   __shared__ int s_e;
   int b, j, h;
   bool is_v;
-  if (!write_unit<WriteShape<D>::PER_WG>(a.units, b, j, h, is_v)) return;
+  if (!write_unit<Shape<D>::PER_WG>(a.units, b, j, h, is_v)) return;
   const int lane = threadIdx.x % 64, wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int64_t pos = a.pos_dev ? a.pos_dev[(int64_t)b * a.pos_step] : a.pos;
   const int count = a.counts ? min(max(a.counts[(int64_t)b * a.counts_step], 0), a.S) : a.S;
@@ -418,7 +423,12 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(WriteArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// read: the write's lanes the other way round.
+// read: the write's lanes the other way round, without a maximum to share: D / 32
+// waves a block, each by itself, with non-temporal stores (131072 rows: 144 us,
+// 174 with ordinary ones, by one wave a block). A wave of the values covers 64
+// columns of half the tokens, so that its stores are whole lines of 128 bytes:
+// 131072 rows of 8 heads of 128 take 133 us so, 149 with half lines, 143 with
+// twice as long ones; one wave a block took 144, and 500 rows 5.7 us (3.3 so).
 struct ReadArgs {
   Cache c;
   void *k, *v;
@@ -432,15 +442,16 @@ struct ReadArgs {
 template <typename T, int D>
 __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
   using E = Elt<T>;
-  constexpr int DG = D / 8, TPL = D / 8;
-  using Run = Words<TPL / 4>;
-  int b, j, h;
+  constexpr int DG = D / 8, W = Shape<D>::W;
+  constexpr int AC = DG < 8 ? DG : 8, CG = DG / AC;   // lanes across the values' columns, waves across them
+  int b, j, h, part;
   bool is_v;
-  if (!read_unit(a.units, b, j, h, is_v)) return;
+  if (!read_unit<W>(a.units, b, j, h, is_v, part)) return;
   const int lane = threadIdx.x % 64;
   const int blk = a.start / KB + j;
   const int live = a.n_keys ? a.n_keys[(int64_t)b * a.n_step] : a.c.cap;
-  const int dg = lane % DG, p0 = lane / DG * TPL;
+  const int dg = is_v ? part % CG * AC + lane % AC : lane % DG;
+  const int p0 = (is_v ? part / CG * (64 / AC) + lane / AC : (part * 64 + lane) / DG) * TPL;
   const float s = (is_v ? a.c.vs + b * a.c.vs_b + h * a.c.vs_h : a.c.ks + b * a.c.ks_b + h * a.c.ks_h)[blk];
   const bool sat = 448.f * s > Half<T>::max;   // (also where the product is infinite)
   auto fix = [&](float y) __attribute__((always_inline)) {
@@ -472,25 +483,22 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
     }
   } else {
     const uint8_t* src = a.c.v + b * a.c.v_b + h * a.c.v_h + (int64_t)blk * KB * D + dg * 8 * KB + p0;
-    Run x[8];
+    uint32_t x[8];
 #pragma unroll
-    for (int n = 0; n < 8; ++n) x[n] = *(const Run*)(src + n * KB);
+    for (int n = 0; n < 8; ++n) x[n] = *(const uint32_t*)(src + n * KB);
+    float y[4][8];
 #pragma unroll
-    for (int q = 0; q < TPL / 4; ++q) {
-      float y[4][8];
-#pragma unroll
-      for (int n = 0; n < 8; ++n) {
-        const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(x[n].w[q], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(x[n].w[q], true);
-        y[0][n] = fix(lo.x * s);
-        y[1][n] = fix(lo.y * s);
-        y[2][n] = fix(hi.x * s);
-        y[3][n] = fix(hi.y * s);
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        put(token_of(p0 + 4 * q + r), (u32x4){E::pack2(y[r][0], y[r][1]), E::pack2(y[r][2], y[r][3]),
-                                              E::pack2(y[r][4], y[r][5]), E::pack2(y[r][6], y[r][7])});
+    for (int n = 0; n < 8; ++n) {
+      const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8(x[n], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(x[n], true);
+      y[0][n] = fix(lo.x * s);
+      y[1][n] = fix(lo.y * s);
+      y[2][n] = fix(hi.x * s);
+      y[3][n] = fix(hi.y * s);
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      put(token_of(p0 + r), (u32x4){E::pack2(y[r][0], y[r][1]), E::pack2(y[r][2], y[r][3]),
+                                    E::pack2(y[r][4], y[r][5]), E::pack2(y[r][6], y[r][7])});
   }
 }
 
@@ -1176,17 +1184,14 @@ void by_type(int dtype, int D, F&& f) {
   else dims(Tag<_Float16>{});
 }
 
-// Blocks of a write or read, of `waves` waves each.
-bool units_for(Units& u, int B, int n_blk, int Hkv, int waves, bool read) {
-  const int64_t per_seq = (int64_t)n_blk * 2 * Hkv, most = 0x3ffff00 / waves;   // (threads of a grid: below 2^32)
+// Blocks of a write or read, of D / 32 waves each.
+bool units_for(Units& u, int B, int n_blk, int Hkv, int D, bool read) {
+  const int64_t per_seq = (int64_t)n_blk * 2 * Hkv, most = 0x3ffff00 / (D / 32);   // (threads of a grid: below 2^32)
   if (per_seq > most || per_seq * B > most) return false;
   const int64_t n = per_seq * B;
   u = Units{make_fastdiv(read ? n_blk : 2 * Hkv), make_fastdiv(n_blk * 2 * Hkv), (uint32_t)n, (uint32_t)Hkv};
   return true;
 }
-
-// Workgroups of four waves, a multiple of eight.
-unsigned units_grid(const Units& u) { return (u.n + 31) / 32 * 8; }
 
 int launched() { return hipGetLastError() == hipSuccess ? DA_OK : DA_ERR_LAUNCH; }
 
@@ -1224,17 +1229,16 @@ extern "C" int da_kv8_write(const da_kv8_write_args* x, void* stream) {
   a.S = S;
   // blocks that S tokens touch: from a known row, or from any
   const int n_blk = x->pos_dev ? (int)(((int64_t)S + KB - 2) / KB + 1) : (int)((x->pos + S + KB - 1) / KB - x->pos / KB);
-  if (!units_for(a.units, B, n_blk, Hkv, x->cache.D / (8 * TPL), false)) return DA_ERR_INVALID_ARG;
+  if (!units_for(a.units, B, n_blk, Hkv, x->cache.D, false)) return DA_ERR_INVALID_ARG;
   (void)hipGetLastError();
   by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
     using E = typename decltype(t)::type;
     constexpr int DIM = decltype(d)::value, AT_ONCE = 512 / DIM;
-    using Shape = WriteShape<DIM>;
     const auto grid = [&](int per_wg) { return dim3((a.units.n + per_wg - 1) / per_wg); };
     if (S == 1) hipLaunchKernelGGL((kv8_append_kernel<E, DIM, 1, true>), grid(4), dim3(256), 0, (hipStream_t)stream, a);
     else if (S <= AT_ONCE) hipLaunchKernelGGL((kv8_append_kernel<E, DIM, 1, false>), grid(4), dim3(256), 0, (hipStream_t)stream, a);
     else if (S <= 2 * AT_ONCE) hipLaunchKernelGGL((kv8_append_kernel<E, DIM, 2, false>), grid(4), dim3(256), 0, (hipStream_t)stream, a);
-    else hipLaunchKernelGGL((kv8_write_kernel<E, DIM>), grid(Shape::PER_WG), dim3(Shape::THREADS), 0, (hipStream_t)stream, a);
+    else hipLaunchKernelGGL((kv8_write_kernel<E, DIM>), grid(Shape<DIM>::PER_WG), dim3(Shape<DIM>::THREADS), 0, (hipStream_t)stream, a);
   });
   return launched();
 }
@@ -1259,11 +1263,12 @@ extern "C" int da_kv8_read(const da_kv8_read_args* x, void* stream) {
   a.n_step = x->n_keys_per_seq ? 1 : 0;
   a.start = start, a.n = n;
   const int n_blk = (int)(((int64_t)start + n + KB - 1) / KB - start / KB);
-  if (!units_for(a.units, B, n_blk, x->cache.Hkv, 1, true)) return DA_ERR_INVALID_ARG;
+  if (!units_for(a.units, B, n_blk, x->cache.Hkv, x->cache.D, true)) return DA_ERR_INVALID_ARG;
   (void)hipGetLastError();
   by_type(x->dtype, x->cache.D, [&](auto t, auto d) {
-    hipLaunchKernelGGL((kv8_read_kernel<typename decltype(t)::type, decltype(d)::value>), dim3(units_grid(a.units)),
-                       dim3(256), 0, (hipStream_t)stream, a);
+    constexpr int DIM = decltype(d)::value, W = Shape<DIM>::W;
+    hipLaunchKernelGGL((kv8_read_kernel<typename decltype(t)::type, DIM>), dim3((a.units.n * W + 3) / 4), dim3(256), 0,
+                       (hipStream_t)stream, a);
   });
   return launched();
 }

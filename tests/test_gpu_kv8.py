@@ -251,6 +251,29 @@ def test_read(gpu, B, Hkv, D, cap, start, n, dtype):
     assert (buf[:, :, :2] == 7).all() and (buf[:, :, n + 2:] == 7).all()
 
 
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+def test_write_and_read_many_blocks(gpu, D):
+    """More workgroups than some rounds of the XCDs take, the last one not whole:
+    every block of a padded batch is written and read once."""
+    from delta_attention import ops
+    B, Hkv, cap, S = 3, 3, 3200, 3111
+    c, ref = garbage(ops.kv8_empty(B, Hkv, cap, D), D), K8.new_cache(B, Hkv, cap, D)
+    k0, v0 = (tokens(B, 5, Hkv, D, torch.bfloat16, s) for s in (1, 2))
+    k, v = (tokens(B, S, Hkv, D, torch.bfloat16, s) for s in (3, 4))
+    new = [S, 2990, 64]
+    ops.kv8_write(c, k0, v0, 0)
+    ops.kv8_write(c, k, v, 5, counts=torch.tensor(new, dtype=torch.int32, device="cuda"))
+    K8.write(ref, np64(k0), np64(v0), [0] * B)
+    K8.write(ref, np64(k), np64(v), [5] * B, new)
+    check_cache(c, ref, [5 + n for n in new])
+    live = torch.tensor([5 + n for n in new], dtype=torch.int32, device="cuda")
+    for start, n in ((0, cap), (61, 2999)):
+        for x, y in zip(ops.kv8_read(c, start, n, n_keys=live), K8.values(ref, start, n)):
+            for b, m in enumerate(new):
+                y[b, :, max(5 + m - start, 0):] = 0
+            assert same(np64(x), y), (start, n)
+
+
 def filled(B, Hkv, cap, D, n, dtype, seed, scale=1.0):
     """A cache of noise with n[b] tokens of N(0, 1) times a varying factor."""
     from delta_attention import ops
