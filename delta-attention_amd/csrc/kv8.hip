@@ -519,6 +519,7 @@ struct RowsArgs {
   int window, sink;
   float scale2;             // 2 |sm_scale| log2(e), above zero: references and differences are halves
   uint32_t flip;            // the sign bits of Q where sm_scale is negative
+  int whole;                // above zero: no list is split, and none has more blocks
   int slots;                // workgroups that are resident together
   FastDiv round;            // blocks that they take at most: slots * CHUNK
   FastDiv units, tiles, heads;   // Hkv * n_rt, n_rt, G
@@ -559,6 +560,19 @@ __host__ __device__ constexpr int rows_waves(int D, int mt) {
   return D * mt <= 64 ? (mt == 1 ? 4 : mt == 2 ? 3 : 2) : D * mt <= 128 ? 2 : 1;
 }
 constexpr int CHUNK = 64;                    // blocks of an item at most, where there are many
+
+// Lists stay whole, an item each, where no list's own chain of blocks (a
+// workgroup takes D * 3.7 ns a block beside 5 us of start and end) is longer than
+// a split's second launch and join, or where there are so many lists that their
+// blocks keep memory busy together. One row each, 12 blocks of 128 columns in 8
+// lists 7.4 us whole and 7.6 split, 16 9.4 and 8.0; 32 blocks, all full / of 1 to
+// 32, in 128 lists 21 / 19 and 18 / 15, in 256 25 / 21 and 29 / 22, in 512 43 / 31
+// and 46 / 35; six rows each in 384 lists of 24 blocks of 64 columns 17 / 13 and 28
+// / 31. Four row tiles take twice as long a block: 8 blocks 17 and 17, 12 20 and 17.
+__host__ __device__ constexpr bool stays_whole(int64_t blocks, int64_t lists, int D, int mt) {
+  const int64_t few = mt < 4 ? 1280 : 1024;
+  return blocks <= WAVES || (blocks <= CHUNK && blocks * D <= (few > 16 * lists ? few : 16 * lists));
+}
 
 // Splits: every item takes `chunk` blocks of one (sequence, kv head, row tile).
 // There are as many items as workgroups are resident together, or some rounds of
@@ -646,12 +660,17 @@ template <bool ITEM>
 __device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
   const int units = a.units.d;
   int rest, first;          // `i` and the first item, within the sequence
-  if (a.B == 1 || !a.n_dev || a.n_step == 0) {     // one count for all sequences
-    const int n = blocks_of(a, __builtin_amdgcn_readfirstlane(keys_of(a, 0))).n;
-    const int pairs = a.B * units;
-    const int splits = max(item_budget(n * pairs, a.slots, a.round) / pairs, 1);
-    p.chunk = max((n + splits - 1) / splits, WAVES);
-    p.n_split = max((n + p.chunk - 1) / p.chunk, 1);
+  if (a.whole > 0 || a.B == 1 || !a.n_dev || a.n_step == 0) {     // all sequences alike
+    if (a.whole > 0) {
+      p.chunk = a.whole;
+      p.n_split = 1;
+    } else {
+      const int n = blocks_of(a, __builtin_amdgcn_readfirstlane(keys_of(a, 0))).n;
+      const int pairs = a.B * units;
+      const int splits = max(item_budget(n * pairs, a.slots, a.round) / pairs, 1);
+      p.chunk = max((n + splits - 1) / splits, WAVES);
+      p.n_split = max((n + p.chunk - 1) / p.chunk, 1);
+    }
     const int per_seq = ITEM ? units * p.n_split : units;
     p.b = a.B == 1 ? 0 : i / per_seq;
     rest = i - p.b * per_seq;
@@ -1100,7 +1119,7 @@ struct RowsPlan {
   int mt, rows, n_rt;
   int64_t pairs, items;     // (sequence, kv head, row tile) triples; item slots
   int64_t pitch;            // floats of an item's partial sums (a multiple of 4)
-  int slots;
+  int slots, whole;
   FastDiv round;
   size_t bytes;
 };
@@ -1119,18 +1138,22 @@ RowsPlan plan_rows(int B, int Hkv, int G, int s, int D, int64_t max_keys, int wi
     if (near < blocks) blocks = near;
   }
   p.slots = 256 * 4 * rows_waves(D, p.mt) / WAVES;
-  // an upper bound of the items, whatever the lengths: the budget of the longest
-  // ones and one short item a pair, but no more than items of WAVES blocks
-  const int64_t chunks = (blocks + WAVES - 1) / WAVES;
-  const int64_t most = p.pairs * (chunks > 1 ? chunks : 1);
   p.round = make_fastdiv(p.slots * CHUNK);
-  p.items = most;
-  if (blocks * p.pairs < 0x7fffffff - p.slots * CHUNK) {
-    const int64_t some = item_budget((int)(blocks * p.pairs), p.slots, p.round) + p.pairs;
-    if (some < most) p.items = some;
+  p.items = p.pairs;
+  p.whole = 0;
+  if (stays_whole(blocks, p.pairs, D, p.mt)) {
+    p.whole = (int)(blocks > 1 ? blocks : 1);
+  } else {
+    // an upper bound of the items, whatever the lengths: the budget of the longest
+    // ones and one short item a pair, but no more than items of WAVES blocks
+    p.items *= (blocks + WAVES - 1) / WAVES;
+    if (blocks * p.pairs < 0x7fffffff - p.slots * CHUNK) {
+      const int64_t some = item_budget((int)(blocks * p.pairs), p.slots, p.round) + p.pairs;
+      if (some < p.items) p.items = some;
+    }
   }
   p.pitch = (int64_t)p.rows * D + (2 * p.rows + 3) / 4 * 4;
-  p.bytes = chunks <= 1 ? 0 : (size_t)(p.items * p.pitch) * sizeof(float);
+  p.bytes = p.whole > 0 ? 0 : (size_t)(p.items * p.pitch) * sizeof(float);
   return p;
 }
 
@@ -1319,6 +1342,7 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   // no weight by more than 2^-20, and a masked score's -inf stays -inf)
   a.scale2 = fminf(fmaxf(fabsf(x->sm_scale) * (2 * 1.4426950408889634f), FLT_TRUE_MIN), FLT_MAX);
   a.flip = x->sm_scale < 0.f ? 0x80008000u : 0;
+  a.whole = p.whole;
   a.slots = p.slots;
   a.round = p.round;
   a.units = make_fastdiv(Hkv * p.n_rt);

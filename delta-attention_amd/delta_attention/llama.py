@@ -39,8 +39,8 @@ class CachedKeys8(NamedTuple):
 # Rows (tokens times query heads per kv head) up to which a pass over an 8-bit
 # cache reads its codes (ops.kv8_attention); more rows read the keys back into
 # 16 bits first and run the rows kernel. 32 query heads over 32768 / 131072
-# keys: 256 rows 66 / 260 us so, 91 / 297 by the read-back; 512 rows 127 / 513
-# us, 117 / 412 by the read-back.
+# keys: 256 rows 66 / 219 us so, 91 / 276 by the read-back; 512 rows 115 / 433
+# us, 115 / 391 by the read-back.
 DIRECT_ROWS8 = 256
 
 

@@ -325,6 +325,13 @@ ROWS = [
     (3, 2, 8, 64, 1024, [1000, 0, 513], 40, 100, 70),         # several row tiles, ragged, windows
     (1, 1, 1, 128, 131072, [70], 1, 0, 0),                    # a few keys of a large capacity
     (2, 1, 16, 32, 256, [256, 3], 4, 0, 0),                   # 64 rows, more rows than keys
+    (70, 1, 2, 32, 4224, [4200 if i % 23 == 5 else (i * 37) % 300 for i in range(70)], 1, 0, 0),    # as above, split
+    (260, 1, 1, 32, 4160, [4160 if i in (3, 258) else (i * 53) % 400 for i in range(260)], 1, 0, 0),
+    (66, 1, 3, 64, 4224, [(i * 997) % 4225 for i in range(66)], 2, 4100, 100),                      # and with a window
+    (5, 2, 4, 128, 640, [640, 0, 1, 333, 577], 1, 0, 0),      # the longest lists that stay whole,
+    (5, 2, 4, 128, 704, [704, 0, 1, 333, 577], 1, 0, 0),      # and one block more
+    (24, 4, 2, 64, 1536, [(i * 611) % 1537 for i in range(24)], 5, 0, 0),       # whole for their number
+    (40, 8, 1, 128, 3008, [(i * 733) % 2561 for i in range(40)], 1, 2300, 150), # whole by their windows
 ]
 
 
@@ -548,8 +555,9 @@ def test_rows_in_place_and_unaligned(gpu):
     ops.kv8_write(c2, wide[..., 2:66], wide[..., 2:66], 1000)
     for a, b in zip(c, c2):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    # (the write moved the earlier codes of its block to a larger scale)
+    want = ops.kv8_attention(q, c, n_keys=counts, sm_scale=0.1)
     qq = q.clone()
-    counts = counts.clone()
     ops.kv8_attention(qq, c, n_keys=counts, sm_scale=0.1, out=qq)
     assert torch.equal(qq, want)
 

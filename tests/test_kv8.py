@@ -183,8 +183,9 @@ def test_c_rows_refusals_and_workspace(lib):
     for bad in (dict(Hq=9), dict(Hq=0), dict(s=-1), dict(window=-1), dict(sink=-1), dict(n=-1), dict(n=1025), dict(q=0),
                 dict(out=0), dict(kc=0), dict(cap=1000), dict(s=1 << 30)):
         assert call(**bad) == L.DA_ERR_INVALID_ARG, bad
-    need = ws(1, 8, 2, 1, 64, 1000, 0, 0)
-    assert need > 0 and call(nb=need - 1) == L.DA_ERR_WORKSPACE and call(ws=0) == L.DA_ERR_WORKSPACE
+    assert ws(1, 8, 2, 1, 64, 1000, 0, 0) == 0                 # short lists stay whole
+    need, long = ws(1, 8, 2, 1, 64, 4000, 0, 0), dict(cap=4096, n=4000)
+    assert need > 0 and call(nb=need - 1, **long) == L.DA_ERR_WORKSPACE and call(ws=0, **long) == L.DA_ERR_WORKSPACE
     for bad in (dict(q=24), dict(out=24), dict(qs=(512, 65, 64)), dict(nk=18), dict(ws=24), dict(add=24),
                 dict(add=16, as_=(8, 8, 4))):
         assert call(**bad) == L.DA_ERR_ALIGNMENT, bad
