@@ -519,6 +519,7 @@ struct RowsArgs {
   int window, sink;
   float scale2;             // 2 |sm_scale| log2(e), above zero: references and differences are halves
   uint32_t flip;            // the sign bits of Q where sm_scale is negative
+  int alike;                // every sequence splits alike: one count for all, or
   int whole;                // above zero: no list is split, and none has more blocks
   int slots;                // workgroups that are resident together
   FastDiv round;            // blocks that they take at most: slots * CHUNK
@@ -660,7 +661,7 @@ template <bool ITEM>
 __device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
   const int units = a.units.d;
   int rest, first;          // `i` and the first item, within the sequence
-  if (a.whole > 0 || a.B == 1 || !a.n_dev || a.n_step == 0) {     // all sequences alike
+  if (a.alike) {
     if (a.whole > 0) {
       p.chunk = a.whole;
       p.n_split = 1;
@@ -1343,6 +1344,7 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   a.scale2 = fminf(fmaxf(fabsf(x->sm_scale) * (2 * 1.4426950408889634f), FLT_TRUE_MIN), FLT_MAX);
   a.flip = x->sm_scale < 0.f ? 0x80008000u : 0;
   a.whole = p.whole;
+  a.alike = p.whole > 0 || B == 1 || !a.n_dev || a.n_step == 0;
   a.slots = p.slots;
   a.round = p.round;
   a.units = make_fastdiv(Hkv * p.n_rt);
