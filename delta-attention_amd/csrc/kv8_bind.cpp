@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <limits>
@@ -169,30 +170,52 @@ PyObject* write(PyObject* const* a) {
   Py_RETURN_NONE;
 }
 
-// (cache, start, n, n_keys, k out, v out)
+// (cache, start, n, n_keys, dtype, (k out, v out) or None) -> (k, v)
 PyObject* read(PyObject* const* a) {
-  const at::Tensor &k = tensor(a[4], "k"), &v = tensor(a[5], "v");
-  const c10::Device dev = k.device();
+  const bool given = a[5] != Py_None;
+  REQUIRE(PyTuple_Check(a[0]) && PyTuple_GET_SIZE(a[0]) == 4, "an ops.KV8 cache is needed");
+  const c10::Device dev = tensor(PyTuple_GET_ITEM(a[0], 0), "cache.k").device();
   da_kv8_read_args x{};
   x.cache = cache_of(a[0], dev);
   const int64_t start = integer(a[1]), n = integer(a[2]), B = x.cache.B;
   REQUIRE(start >= 0 && n >= 0 && start <= x.cache.cap - n, "rows ", start, " .. ", start, " + ", n, " of a cache of ", x.cache.cap);
-  REQUIRE(k.sizes() == at::IntArrayRef({B, (int64_t)x.cache.Hkv, n, (int64_t)x.cache.D}) && v.sizes() == k.sizes() &&
-              k.scalar_type() == v.scalar_type() && v.device() == dev && k.stride(3) == 1 && v.stride(3) == 1,
-          "the results are two [", B, ", ", x.cache.Hkv, ", ", n, ", ", x.cache.D, "] tensors of one type, got ", k.sizes(), v.sizes());
-  x.dtype = dtype_code(k.scalar_type());
-  on_gpu(dev);
+  at::Tensor k, v;
+  if (given) {
+    REQUIRE(PyTuple_Check(a[5]) && PyTuple_GET_SIZE(a[5]) == 2, "out: two tensors are needed");
+    k = tensor(PyTuple_GET_ITEM(a[5], 0), "k");
+    v = tensor(PyTuple_GET_ITEM(a[5], 1), "v");
+    REQUIRE(k.sizes() == at::IntArrayRef({B, (int64_t)x.cache.Hkv, n, (int64_t)x.cache.D}) && v.sizes() == k.sizes() &&
+                k.scalar_type() == v.scalar_type() && k.stride(3) == 1 && v.stride(3) == 1,
+            "the results are two [", B, ", ", x.cache.Hkv, ", ", n, ", ", x.cache.D, "] tensors of one type, got ", k.sizes(), v.sizes());
+    REQUIRE(k.device() == dev && v.device() == dev, "all tensors must be on one device");
+    x.dtype = dtype_code(k.scalar_type());
+    on_gpu(dev);
+  } else {
+    REQUIRE(THPDtype_Check(a[4]), "dtype: a torch.dtype is needed");
+    const at::ScalarType type = ((THPDtype*)a[4])->scalar_type;
+    x.dtype = dtype_code(type);
+    on_gpu(dev);
+    const at::Tensor both = at::empty({2, B, x.cache.Hkv, n, x.cache.D}, at::TensorOptions().dtype(type).device(dev));
+    k = both.select(0, 0);
+    v = both.select(0, 1);
+  }
   x.n_keys_dev = entries<int32_t>(a[3], B, at::kInt, dev, "n_keys", x.n_keys_per_seq);
-  if (B == 0 || n == 0) Py_RETURN_NONE;
-  x.start = (int32_t)start;
-  x.n = (int32_t)n;
-  x.k = k.data_ptr();
-  x.v = v.data_ptr();
-  strides3(x.k_str, k);
-  strides3(x.v_str, v);
-  const On on(dev);
-  check(g_read(&x, on.stream()), "da_kv8_read");
-  Py_RETURN_NONE;
+  if (B > 0 && n > 0) {
+    x.start = (int32_t)start;
+    x.n = (int32_t)n;
+    x.k = k.data_ptr();
+    x.v = v.data_ptr();
+    strides3(x.k_str, k);
+    strides3(x.v_str, v);
+    const On on(dev);
+    check(g_read(&x, on.stream()), "da_kv8_read");
+  }
+  if (given) return Py_NewRef(a[5]);
+  PyObject* result = PyTuple_New(2);
+  if (!result) throw PythonError();
+  PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(std::move(k)));
+  PyTuple_SET_ITEM(result, 1, THPVariable_Wrap(std::move(v)));
+  return result;
 }
 
 // (q, cache, n_keys, window, sink, sm_scale, out or None, add or None) -> out

@@ -647,13 +647,7 @@ def kv8_read(cache: KV8, start: int, n: int, *, n_keys: Optional[torch.Tensor] =
     beyond float16's largest saturate. n_keys: optional int32 device tensor
     (one entry or one per sequence); rows at or past it are zero. out: the two
     tensors to write."""
-    if out is None:
-        B, Hkv, cap, D = cache.k.shape
-        assert 0 <= start and 0 <= n <= cap - start, f"rows {start} .. {start + n} of a cache of {cap}"
-        out = torch.empty((2, B, Hkv, n, D), device=cache.k.device, dtype=dtype).unbind(0)
-    k, v = out
-    L.kv8_ext().read(cache, start, n, n_keys, k, v)
-    return k, v
+    return L.kv8_ext().read(cache, start, n, n_keys, dtype, out if out is None else tuple(out))
 
 
 def kv8_attention(q: torch.Tensor, cache: KV8, *, n_keys, window: int = 0, sink: int = 0,
