@@ -521,6 +521,7 @@ struct RowsArgs {
   uint32_t flip;            // the sign bits of Q where sm_scale is negative
   int alike;                // every sequence splits alike: one count for all, or
   int whole;                // above zero: no list is split, and none has more blocks
+  int most;                 // splits at most, where the sequences split alike
   int slots;                // workgroups that are resident together
   FastDiv round;            // blocks that they take at most: slots * CHUNK
   FastDiv units, tiles, heads;   // Hkv * n_rt, n_rt, G
@@ -655,37 +656,56 @@ __device__ __forceinline__ bool among(const RowsArgs& a, int i, Place& p, int& r
   return false;
 }
 
-// The place of item `i`, or (ITEM false) of (sequence, kv head, row tile) `i`;
-// false past the last.
-template <bool ITEM>
-__device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
-  const int units = a.units.d;
-  int rest, first;          // `i` and the first item, within the sequence
-  if (a.alike) {
-    if (a.whole > 0) {
-      p.chunk = a.whole;
-      p.n_split = 1;
-    } else {
-      const int n = blocks_of(a, __builtin_amdgcn_readfirstlane(keys_of(a, 0))).n;
-      const int pairs = a.B * units;
-      const int splits = max(item_budget(n * pairs, a.slots, a.round) / pairs, 1);
-      p.chunk = max((n + splits - 1) / splits, WAVES);
-      p.n_split = max((n + p.chunk - 1) / p.chunk, 1);
-    }
-    const int per_seq = ITEM ? units * p.n_split : units;
-    p.b = a.B == 1 ? 0 : i / per_seq;
-    rest = i - p.b * per_seq;
-    if (p.b >= a.B || rest >= per_seq) return false;
-    first = p.b * units * p.n_split;
+// The splits of every sequence where they split alike.
+__device__ __forceinline__ void split_alike(const RowsArgs& a, Place& p) {
+  if (a.whole > 0) {
+    p.chunk = a.whole;
+    p.n_split = 1;
   } else {
-    // (a separate copy for up to 64 sequences, one to a lane)
-    if (!(a.B <= 64 ? among<ITEM, 1>(a, i, p, rest, first) : among<ITEM, 4>(a, i, p, rest, first))) return false;
+    const int n = blocks_of(a, __builtin_amdgcn_readfirstlane(keys_of(a, 0))).n, pairs = a.B * (int)a.units.d;
+    const int splits = max(item_budget(n * pairs, a.slots, a.round) / pairs, 1);
+    p.chunk = max((n + splits - 1) / splits, WAVES);
+    p.n_split = max((n + p.chunk - 1) / p.chunk, 1);
   }
+}
+
+// Tile, head and split of the `rest`th item (ITEM false: pair of head and tile)
+// of a sequence whose items have slots from `first` on, `room` a pair.
+template <bool ITEM>
+__device__ __forceinline__ void place(const RowsArgs& a, Place& p, int rest, int first, int room) {
   const int group = fdiv(rest, a.tiles);            // (kv head, split), or the kv head
   p.tile = rest - group * a.n_rt;
   p.head = ITEM ? group / p.n_split : group;
   p.split = ITEM ? group - p.head * p.n_split : 0;
-  p.slot = first + (p.head * p.n_split + p.split) * a.n_rt + p.tile;
+  p.slot = first + (p.head * room + p.split) * a.n_rt + p.tile;
+}
+
+// Where the sequences split alike, a pair's slots depend on no count.
+__device__ __forceinline__ bool place_alike(const RowsArgs& a, int i, Place& p) {
+  const int units = a.units.d;
+  p.b = a.B == 1 ? 0 : fdiv(i, a.units);
+  if (p.b >= a.B || i - p.b * units >= units) return false;
+  place<false>(a, p, i - p.b * units, p.b * units * a.most, a.most);
+  return true;
+}
+
+// The place of item `i`, or (ITEM false, sequences of different lengths) of
+// (sequence, kv head, row tile) `i`; false past the last.
+template <bool ITEM>
+__device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
+  int rest, first;          // `i` and the first item, within the sequence
+  if (ITEM && a.alike) {
+    split_alike(a, p);
+    const int units = a.units.d, per_seq = units * p.n_split;
+    p.b = a.B == 1 ? 0 : i / per_seq;
+    rest = i - p.b * per_seq;
+    if (p.b >= a.B || rest >= per_seq) return false;
+    place<ITEM>(a, p, rest, p.b * units * a.most, a.most);
+    return true;
+  }
+  // (a separate copy for up to 64 sequences, one to a lane)
+  if (!(a.B <= 64 ? among<ITEM, 1>(a, i, p, rest, first) : among<ITEM, 4>(a, i, p, rest, first))) return false;
+  place<ITEM>(a, p, rest, first, p.n_split);
   return true;
 }
 
@@ -1054,7 +1074,12 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
   __shared__ f32x4 s_o[SG][CT];
   const int row = blockIdx.y;
   Place p;
-  if (!locate<false>(a, blockIdx.x, p) || p.n_split == 1) return;
+  if (a.alike) {
+    if (!place_alike(a, blockIdx.x, p)) return;
+  } else {
+    if (!locate<false>(a, blockIdx.x, p)) return;
+  }
+  const int room = a.alike ? a.most : p.n_split;    // slots of this pair
   const int hk = p.head, m = p.tile * a.rows + row;
   if (m >= a.s * a.G) return;
   const int qi = fdiv(m, a.heads);
@@ -1064,16 +1089,19 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
   float M = NO_KEYS, L = 0.f;
   f32x4 o = {0, 0, 0, 0};
   constexpr int U = 4;                         // items whose loads are in flight together
-  for (int i0 = sg; i0 < p.n_split; i0 += U * SG) {
+  for (int i0 = sg; ; i0 += U * SG) {
     float mi[U], li[U];
     f32x4 y[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = min(i0 + u * SG, p.n_split - 1);
-      const float* src = part + i * pitch;
+    for (int u = 0; u < U; ++u) {              // (past the last item: not used)
+      const float* src = part + min(i0 + u * SG, room - 1) * pitch;
       mi[u] = src[a.rows * D + row];
       li[u] = src[a.rows * (D + 1) + row];
       y[u] = *(const f32x4*)(src + row * D + t * 4);
+    }
+    if (i0 == sg) {                            // the first loads wait for no count
+      if (a.alike) split_alike(a, p);
+      if (p.n_split == 1) return;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -1085,6 +1113,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = o[e] * k0 + y[u][e] * k1;
     }
+    if (i0 + U * SG >= p.n_split) break;
   }
   s_o[sg][t] = o;
   if (t == 0) {
@@ -1120,7 +1149,7 @@ struct RowsPlan {
   int mt, rows, n_rt;
   int64_t pairs, items;     // (sequence, kv head, row tile) triples; item slots
   int64_t pitch;            // floats of an item's partial sums (a multiple of 4)
-  int slots, whole;
+  int slots, whole, most;
   FastDiv round;
   size_t bytes;
 };
@@ -1142,15 +1171,19 @@ RowsPlan plan_rows(int B, int Hkv, int G, int s, int D, int64_t max_keys, int wi
   p.round = make_fastdiv(p.slots * CHUNK);
   p.items = p.pairs;
   p.whole = 0;
+  p.most = 1;
   if (stays_whole(blocks, p.pairs, D, p.mt)) {
     p.whole = (int)(blocks > 1 ? blocks : 1);
   } else {
     // an upper bound of the items, whatever the lengths: the budget of the longest
     // ones and one short item a pair, but no more than items of WAVES blocks
-    p.items *= (blocks + WAVES - 1) / WAVES;
+    const int64_t most = (blocks + WAVES - 1) / WAVES;
+    p.most = (int)most;
+    p.items *= most;
     if (blocks * p.pairs < 0x7fffffff - p.slots * CHUNK) {
-      const int64_t some = item_budget((int)(blocks * p.pairs), p.slots, p.round) + p.pairs;
-      if (some < p.items) p.items = some;
+      const int64_t budget = item_budget((int)(blocks * p.pairs), p.slots, p.round), each = budget / p.pairs;
+      if (each < most) p.most = (int)(each > 1 ? each : 1);
+      if (budget + p.pairs < p.items) p.items = budget + p.pairs;
     }
   }
   p.pitch = (int64_t)p.rows * D + (2 * p.rows + 3) / 4 * 4;
@@ -1344,6 +1377,7 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   a.scale2 = fminf(fmaxf(fabsf(x->sm_scale) * (2 * 1.4426950408889634f), FLT_TRUE_MIN), FLT_MAX);
   a.flip = x->sm_scale < 0.f ? 0x80008000u : 0;
   a.whole = p.whole;
+  a.most = p.most;
   a.alike = p.whole > 0 || B == 1 || !a.n_dev || a.n_step == 0;
   a.slots = p.slots;
   a.round = p.round;
