@@ -1065,8 +1065,9 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
 }
 
 // Joins the items of one (sequence, kv head, row tile): a workgroup per row, some
-// items side by side and four loads of each in flight. Launch and three dependent
-// loads: 3.5 us for 32 rows of 9 items, 5.2 for 32 of 64.
+// items side by side and four loads of each in flight. Launch and dependent loads
+// (arguments, count, partials; where the sequences split alike the first partials
+// do not wait for the count): 3.5 us for 32 rows of 9 items, 4.9 for 32 of 64.
 template <typename T, int D, int THREADS>
 __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
   constexpr int CT = D / 4, SG = THREADS / CT; // threads across a row, items taken side by side
