@@ -395,6 +395,44 @@ def test_random_runs(gpu, seed):
         assert same(np64(x), np64(torch.from_numpy(y).to(dtype)))
 
 
+@pytest.mark.parametrize("seed", range(16))
+def test_random_split_rows(gpu, seed):
+    """Random shapes at capacities whose lists are split or just not: the count
+    given by the host, by one device entry and by one per sequence, and a
+    recorded call of the last two that serves other lengths."""
+    import random
+    from delta_attention import ops
+    r = random.Random(7000 + seed)
+    B, Hkv, G, D = r.choice([1, 1, 2, 3, 6, 67]), r.choice([1, 2, 4]), r.choice([1, 2, 4, 9]), r.choice([32, 64, 128, 256])
+    dtype, s = DT[r.choice(["bf16", "fp16"])], r.choice([1, 1, 2, 5, 12])
+    most = max(4, min(90, 2 ** 21 // (64 * B * Hkv * D)))
+    cap = 64 * r.randint(most // 2, most)
+    window = r.choice([0, 0, r.randint(1, cap)])
+    sink, scale = r.choice([0, r.randint(0, 200)]), r.choice([D ** -0.5, -0.05])
+    c, ref, _ = filled(B, Hkv, cap, D, [cap] * B, dtype, 90 + seed)
+    q = tokens(B, s, Hkv * G, D, dtype, 91 + seed, False).transpose(1, 2)
+    what = f"seed {seed}: B{B} H{Hkv * G}/{Hkv} D{D} cap {cap} s{s} w{window} k{sink}"
+
+    def rows(n_keys):
+        return ops.kv8_attention(q, c, n_keys=n_keys, window=window, sink=sink, sm_scale=scale)
+
+    n = r.randint(1, cap)
+    check_rows(rows(n), q, ref, [n] * B, window, sink, scale, what=what + " host")
+    for form in ("one", "each"):
+        now = torch.zeros(1 if form == "one" else B, dtype=torch.int32, device="cuda")
+        rows(now)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = rows(now)
+        for n in (cap, r.randint(1, cap), 0, 1, r.randint(cap // 2, cap)):
+            lens = [n] * B if form == "one" else [r.randint(0, n) if b else n for b in range(B)]
+            now.copy_(torch.tensor(lens[:now.numel()], dtype=torch.int32))
+            graph.replay()
+            assert torch.equal(out, rows(now)), (what, form, lens[:4])
+            check_rows(out, q, ref, lens, window, sink, scale, what=f"{what} {form} {lens[:3]}")
+
+
 def test_offsets_past_32_bits(gpu):
     """Sequences of 16M tokens at head_dim 256: codes 4 GiB into a head, the
     second sequence past them; tokens at both ends, a window's rows, a read."""
