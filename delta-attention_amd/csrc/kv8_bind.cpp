@@ -67,6 +67,7 @@ da_kv8_cache cache_of(PyObject* o, c10::Device dev) {
                    &ks = tensor(PyTuple_GET_ITEM(o, 2), "cache.k_scale"), &vs = tensor(PyTuple_GET_ITEM(o, 3), "cache.v_scale");
   REQUIRE(k.dim() == 4 && v.dim() == 5 && ks.dim() == 3 && vs.dim() == 3, "a cache's tensors have 4, 5, 3 and 3 dimensions");
   const int64_t B = k.size(0), H = k.size(1), cap = k.size(2), D = k.size(3), nb = cap / 64;
+  REQUIRE(H >= 1, "a cache has one kv head at least");
   REQUIRE(cap % 64 == 0 && v.sizes() == at::IntArrayRef({B, H, nb, D, 64}) && ks.sizes() == at::IntArrayRef({B, H, nb}) &&
               vs.sizes() == ks.sizes(), "a cache's shapes do not belong together: ", k.sizes(), v.sizes(), ks.sizes(), vs.sizes());
   REQUIRE(k.scalar_type() == at::kFloat8_e4m3fn && v.scalar_type() == at::kFloat8_e4m3fn && ks.scalar_type() == at::kFloat &&

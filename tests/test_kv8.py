@@ -113,6 +113,16 @@ def test_ops_refuse_arguments_on_the_cpu():
             ops.kv8_read(c, start, n)
 
 
+def test_ops_refuse_a_cache_without_heads():
+    """An empty slice over the heads is no cache, whatever the call."""
+    c = ops.KV8(*(t[:, :0] for t in ops.kv8_empty(1, 2, 128, 64, "cpu")))
+    k = torch.zeros(1, 3, 0, 64, dtype=torch.bfloat16)
+    for call in (lambda: ops.kv8_write(c, k, k, 0), lambda: ops.kv8_read(c, 0, 5),
+                 lambda: ops.kv8_attention(torch.zeros(1, 2, 1, 64, dtype=torch.bfloat16), c, n_keys=1, sm_scale=1.0)):
+        with pytest.raises(AssertionError, match="kv head"):
+            call()
+
+
 # the header's structs, in native alignment
 _CACHE = "4P8q4i"                                # k, v, k_scale, v_scale; {batch, head} strides; B, Hkv, cap, D
 WRITE = struct.Struct(_CACHE + "4P7q4i")         # k, v, pos_dev, counts_dev; strides, pos; S, 2 flags, dtype
