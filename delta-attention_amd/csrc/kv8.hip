@@ -1155,14 +1155,18 @@ struct RowsPlan {
   size_t bytes;
 };
 
-RowsPlan plan_rows(int B, int Hkv, int G, int s, int D, int64_t max_keys, int window, int sink) {
-  RowsPlan p{};
+// False for more (sequence, kv head, row tile) triples, or rows, than a launch takes.
+bool plan_rows(RowsPlan& p, int B, int Hkv, int G, int s, int D, int64_t max_keys, int window, int sink) {
+  constexpr int64_t MAX_PAIRS = 0x7fffff;
+  p = RowsPlan{};
   const int64_t m = (int64_t)G * s;
+  if (m > 1 << 28 || (int64_t)B * Hkv > MAX_PAIRS) return false;   // (the products below stay inside 64 bits)
   p.mt = m <= 16 ? 1 : m <= 32 || D == 256 ? 2 : 4;
   p.rows = (int)(m < 16 * p.mt ? m : 16 * p.mt);
   const int64_t rt = (m + 16 * p.mt - 1) / (16 * p.mt);
   p.n_rt = (int)rt;
   p.pairs = (int64_t)B * Hkv * rt;
+  if (p.pairs > MAX_PAIRS) return false;
   int64_t blocks = (max_keys + KB - 1) / KB;
   if (window > 0) {
     const int64_t near = ((int64_t)window + s + 2 * KB - 2) / KB + ((int64_t)sink + KB - 1) / KB;
@@ -1189,7 +1193,7 @@ RowsPlan plan_rows(int B, int Hkv, int G, int s, int D, int64_t max_keys, int wi
   }
   p.pitch = (int64_t)p.rows * D + (2 * p.rows + 3) / 4 * 4;
   p.bytes = p.whole > 0 ? 0 : (size_t)(p.items * p.pitch) * sizeof(float);
-  return p;
+  return true;
 }
 
 int take_cache(Cache& c, const da_kv8_cache& x, int dtype) {
@@ -1336,7 +1340,8 @@ extern "C" size_t da_kv8_attn_workspace_bytes(int B, int Hq, int Hkv, int s, int
   if (B < 1 || Hq < 1 || Hkv < 1 || Hq % Hkv != 0 || s < 1 || !head_dim_ok(D) || max_keys < 0 ||
       window < 0 || sink < 0)
     return 0;
-  return plan_rows(B, Hkv, Hq / Hkv, s, D, max_keys, window, sink).bytes;
+  RowsPlan p;
+  return plan_rows(p, B, Hkv, Hq / Hkv, s, D, max_keys, window, sink) ? p.bytes : 0;
 }
 
 extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
@@ -1356,9 +1361,9 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   // (a window or sinks past the capacity are every key)
   a.window = x->window < cap ? x->window : cap;
   a.sink = x->sink < cap ? x->sink : cap;
-  if ((int64_t)Hq / Hkv * s > 1 << 28) return DA_ERR_INVALID_ARG;
-  const RowsPlan p = plan_rows(B, Hkv, Hq / Hkv, s, x->cache.D, x->n_keys_dev ? cap : x->n_keys, a.window, a.sink);
-  if (p.pairs > 0x7fffff || p.items * 256 > 0x7fffffffll || p.pairs * (cap / KB) > 0x70000000ll)
+  RowsPlan p;
+  if (!plan_rows(p, B, Hkv, Hq / Hkv, s, x->cache.D, x->n_keys_dev ? cap : x->n_keys, a.window, a.sink) ||
+      p.items * 256 > 0x7fffffffll || p.pairs * (cap / KB) > 0x70000000ll)
     return DA_ERR_INVALID_ARG;
   if (p.bytes > 0 && (!x->workspace || x->workspace_bytes < (int64_t)p.bytes)) return DA_ERR_WORKSPACE;
   if (!aligned16(x->workspace)) return DA_ERR_ALIGNMENT;

@@ -201,3 +201,16 @@ def test_c_rows_refusals_and_workspace(lib):
         assert call(**bad) == L.DA_ERR_ALIGNMENT, bad
     assert call(s=0) == L.DA_OK and call(B=0) == L.DA_OK
     assert lib.da_kv8_attn_fwd(None, None) == L.DA_ERR_INVALID_ARG
+
+
+def test_c_rows_of_sizes_past_any_launch(lib):
+    """Products of sequences, heads and row tiles that pass 64 bits (2^64 = 0)
+    are refused, and have no workspace."""
+    big = 1 << 30
+    for B, Hkv, G, s, keys in ((big, big, 1, 1024, 1000000), (big, big, 1, 1, 64), (1, 1, big, big, 1000000),
+                               (1, 1, 1, 2 ** 31 - 1, 2 ** 31 - 1), (1 << 23, 1, 1, 1, 4096)):
+        assert lib.da_kv8_attn_workspace_bytes(B, Hkv * G, Hkv, s, 32, keys, 0, 0) == 0
+        a = dict(CACHE, B=B, Hkv=Hkv, cap=1 << 20, D=32)
+        rc = lib.da_kv8_attn_fwd(ATTN.pack(*_head(a), 16, 16, 0, 16, 16, 1 << 40, *((32,) * 6), *((0,) * 3), Hkv * G, s, 0,
+                                           0, 0, 0, L.DA_BF16, 0.1), None)
+        assert rc == L.DA_ERR_INVALID_ARG, (B, Hkv, G, s)
