@@ -1255,6 +1255,12 @@ bool units_for(Units& u, int B, int n_blk, int Hkv, int D, bool read) {
   return true;
 }
 
+// Results [B, H, rows, D] by their strides: false where some share their place
+// (a stride of zero over more than one entry), which leaves none of them right.
+bool apart(const int64_t str[3], int B, int H, int rows) {
+  return (B <= 1 || str[0]) && (H <= 1 || str[1]) && (rows <= 1 || str[2]);
+}
+
 int launched() { return hipGetLastError() == hipSuccess ? DA_OK : DA_ERR_LAUNCH; }
 
 }  // namespace
@@ -1313,7 +1319,8 @@ extern "C" int da_kv8_read(const da_kv8_read_args* x, void* stream) {
   const int B = x->cache.B, start = x->start, n = x->n;
   if (start < 0 || n < 0 || (int64_t)start + n > x->cache.cap) return DA_ERR_INVALID_ARG;
   if (n == 0 || B == 0) return DA_OK;
-  if (!x->k || !x->v) return DA_ERR_INVALID_ARG;
+  if (!x->k || !x->v || !apart(x->k_str, B, x->cache.Hkv, n) || !apart(x->v_str, B, x->cache.Hkv, n))
+    return DA_ERR_INVALID_ARG;
   if (!aligned16(x->k) || !aligned16(x->v) || !strides8(x->k_str) || !strides8(x->v_str) ||
       ((uintptr_t)x->n_keys_dev & 3))
     return DA_ERR_ALIGNMENT;
@@ -1354,7 +1361,7 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   if (!x->n_keys_dev && (x->n_keys < 0 || x->n_keys > cap)) return DA_ERR_INVALID_ARG;
   if (!(fabsf(x->sm_scale) <= FLT_MAX)) return DA_ERR_INVALID_ARG;
   if (s == 0 || B == 0) return DA_OK;
-  if (!x->q || !x->out) return DA_ERR_INVALID_ARG;
+  if (!x->q || !x->out || !apart(x->o_str, B, Hq, s)) return DA_ERR_INVALID_ARG;
   if (!aligned16(x->q) || !aligned16(x->out) || !strides8(x->q_str) || !strides8(x->o_str) ||
       ((uintptr_t)x->n_keys_dev & 3) || (x->addend && (!aligned16(x->addend) || !strides8(x->add_str))))
     return DA_ERR_ALIGNMENT;

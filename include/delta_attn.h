@@ -314,6 +314,7 @@ int da_kv8_write(const da_kv8_write_args* args, void* stream);
  * (strides {batch, head, row}) = code * scale, one rounding (exact in bf16),
  * finite values beyond the type's largest one saturated. With n_keys_dev (int32,
  * one entry or one per sequence) rows at or past a sequence's count are zero.
+ * DA_ERR_INVALID_ARG for results with a zero stride over more than one entry.
  */
 typedef struct {
   da_kv8_cache cache;
@@ -334,6 +335,7 @@ int da_kv8_read(const da_kv8_read_args* args, void* stream);
  * see no key (r < 0) are zero. addend (optional, like q): out = rnd(rnd(row) +
  * addend). n is n_keys_dev[b] (or n_keys_dev[0] when n_keys_per_seq is 0) read
  * when the kernels run and clamped to [0, cap], or the host's n_keys.
+ * DA_ERR_INVALID_ARG for an out with a zero stride over more than one entry.
  * Workspace: da_kv8_attn_workspace_bytes(..., max_keys = cap with a device
  * count, else n_keys) bytes, which may be 0.
  */

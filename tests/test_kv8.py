@@ -214,3 +214,22 @@ def test_c_rows_of_sizes_past_any_launch(lib):
         rc = lib.da_kv8_attn_fwd(ATTN.pack(*_head(a), 16, 16, 0, 16, 16, 1 << 40, *((32,) * 6), *((0,) * 3), Hkv * G, s, 0,
                                            0, 0, 0, L.DA_BF16, 0.1), None)
         assert rc == L.DA_ERR_INVALID_ARG, (B, Hkv, G, s)
+
+
+def test_c_results_that_share_their_place(lib):
+    """Results with a zero stride over sequences, heads or rows are refused;
+    over a single entry a stride counts for nothing (no launch: n or s = 0)."""
+    def read(ks, vs, B=2, n=5):
+        a = dict(CACHE, B=B)
+        return lib.da_kv8_read(READ.pack(*_head(a), 16, 16, 0, *ks, *vs, 0, n, 0, L.DA_BF16), None)
+
+    def rows(os, B=2, Hq=4, s=3):
+        a = dict(CACHE, B=B)
+        return lib.da_kv8_attn_fwd(ATTN.pack(*_head(a), 16, 16, 0, 0, 16, 1 << 30, 3 * 256, 64, 256, *os, 0, 0, 0, Hq, s, 0,
+                                             100, 0, 0, L.DA_BF16, 0.1), None)
+    good = (640, 320, 64)
+    for i in range(3):
+        bad = tuple(0 if j == i else x for j, x in enumerate(good))
+        assert read(bad, good) == read(good, bad) == L.DA_ERR_INVALID_ARG, bad
+        assert rows(bad) == L.DA_ERR_INVALID_ARG, bad
+    assert read((0, 0, 0), (0, 0, 0), n=0) == rows((0, 0, 0), s=0) == L.DA_OK
