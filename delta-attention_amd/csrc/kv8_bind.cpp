@@ -11,8 +11,10 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <exception>
 #include <limits>
 #include <stdexcept>
 #include <string>
@@ -305,10 +307,8 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   } catch (const PythonError&) {
   } catch (const Refused& e) {
     PyErr_SetString(PyExc_AssertionError, e.what());
-  } catch (const c10::Error& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {            // torch's own errors keep their types (out of memory)
+    torch::translate_exception_to_python(std::current_exception());
   }
   return nullptr;
 }

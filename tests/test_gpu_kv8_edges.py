@@ -36,3 +36,12 @@ def test_results_that_share_their_place_are_refused(gpu):
     out = torch.empty(4, 64, device="cuda").bfloat16().as_strided((1, 4, 1, 64), (0, 64, 0, 1))
     ops.kv8_attention(q[:1, :, :1], ops.KV8(*(t[:1] for t in c)), n_keys=100, sm_scale=0.1, out=out)
     assert torch.equal(out, want)
+
+
+def test_out_of_memory_is_torchs(gpu):
+    """Results past the card's memory raise torch's own error: a long cache
+    expanded over sequences asks for 2 TB."""
+    from delta_attention import ops
+    c = ops.KV8(*(t.expand(1 << 28, *t.shape[1:]) for t in ops.kv8_empty(1, 1, 64, 32)))
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.kv8_read(c, 0, 64)
