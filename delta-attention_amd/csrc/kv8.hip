@@ -1295,8 +1295,11 @@ extern "C" int da_kv8_write(const da_kv8_write_args* x, void* stream) {
   a.pos_step = x->pos_per_seq ? 1 : 0;
   a.counts_step = x->counts_per_seq ? 1 : 0;
   a.S = S;
-  // blocks that S tokens touch: from a known row, or from any
-  const int n_blk = x->pos_dev ? (int)(((int64_t)S + KB - 2) / KB + 1) : (int)((x->pos + S + KB - 1) / KB - x->pos / KB);
+  // Blocks that S tokens touch, from a known row or from any: no more than the
+  // capacity's, however far a padded length passes it (a block's first row, up to
+  // twice the capacity, then fits 32 bits).
+  const int from_any = (int)(((int64_t)S + KB - 2) / KB + 1);
+  const int n_blk = x->pos_dev ? (from_any < cap / KB ? from_any : cap / KB) : (int)((x->pos + S + KB - 1) / KB - x->pos / KB);
   if (!units_for(a.units, B, n_blk, Hkv, x->cache.D, false)) return DA_ERR_INVALID_ARG;
   (void)hipGetLastError();
   by_type(x->dtype, x->cache.D, [&](auto t, auto d) {

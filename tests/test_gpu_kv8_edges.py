@@ -45,3 +45,30 @@ def test_out_of_memory_is_torchs(gpu):
     c = ops.KV8(*(t.expand(1 << 28, *t.shape[1:]) for t in ops.kv8_empty(1, 1, 64, 32)))
     with pytest.raises(torch.OutOfMemoryError):
         ops.kv8_read(c, 0, 64)
+
+
+def test_write_padded_past_the_capacity(gpu):
+    """A padded length past the capacity, up to the largest int32, with counts
+    that fit: the counts' tokens are written, and nothing else."""
+    from delta_attention import ops
+    B, Hkv, D, cap = 2, 2, 64, 256
+    for S in (300, 2 ** 31 - 1):
+        k, v = (torch.randn(B, 1, Hkv, D, device="cuda").bfloat16() for _ in (0, 1))
+        c, ref = ops.kv8_empty(B, Hkv, cap, D), K8.new_cache(B, Hkv, cap, D)
+        for t in c[:2]:
+            t.view(torch.uint8).fill_(0x55)
+        counts, pos = [90, 7], [100, 249]
+        first = torch.randn(B, 256, Hkv, D, device="cuda").bfloat16()
+        ops.kv8_write(c, first, first, 0, counts=torch.tensor(pos, dtype=torch.int32, device="cuda"))
+        K8.write(ref, np64(first), np64(first), [0, 0], pos)
+        ops.kv8_write(c, k.expand(B, S, Hkv, D), v.expand(B, S, Hkv, D), torch.tensor(pos, device="cuda"),
+                      counts=torch.tensor(counts, dtype=torch.int32, device="cuda"))
+        K8.write(ref, *(np64(x.expand(B, 90, Hkv, D)) for x in (k, v)), pos, counts)
+        got = to_oracle(c)
+        for b in range(B):
+            n = pos[b] + counts[b]
+            for x in ("k", "v"):
+                assert np.array_equal(got[x][b, :, :n], ref[x][b, :, :n]), (S, b, x)
+                assert (got[x][b, :, n:] == 13.0).all()            # (0x55)
+            for x in ("ke", "ve"):
+                assert np.array_equal(got[x][b, :, :-(-n // 64)], ref[x][b, :, :-(-n // 64)]), (S, b, x)
