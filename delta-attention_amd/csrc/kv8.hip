@@ -716,7 +716,8 @@ __device__ __forceinline__ float group_max(float x) {   // over the four lanes o
 
 // 16x16x32 products of one type, and eight codes as its left operand. SCALED:
 // the conversion applies the block's scale, exactly (bf16 has float's range:
-// scores then overflow only where they would anyway); fp16 takes the codes alone.
+// scores then overflow only where they would anyway; half of it where a code may
+// reach 256 * 2^120, past both types' largest); fp16 takes the codes alone.
 template <typename T> struct Dot;
 template <> struct Dot<__bf16> {
   static constexpr bool SCALED = true;
@@ -765,7 +766,7 @@ __device__ __forceinline__ void store4(const RowsArgs& a, int b, int h, int i, i
 // over 131072 keys 43.8 us, 6.1 TB/s with the first loads; eight sequences of that
 // length 6.65 TB/s); else a launch (1.9 us) and the loads that wait for each other
 // (arguments, count, codes: 5.2 us for a single block). Registers, not MFMA or
-// conversions, limit the waves (201 at head_dim 128 and one row tile).
+// conversions, limit the waves (203 at head_dim 128 and one row tile).
 //
 // MT: 16-row tiles per wave. The P V product is formed in fp16 whatever Q's
 // type: the codes are exact in it, and its 11 bits keep the probabilities'
@@ -893,12 +894,15 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
       }
       return bits;
     };
+    // s holds the scores, or (the largest scale) half of them: s * half is half a score
+    const bool far = Dot<T>::SCALED && sk > pow2(E_MAX - 1);
+    const float by = far ? pow2(E_MAX - 1) : sk, half = far ? 1.f : 0.5f;
     f32x4 s[MT][4];
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        const u32x4 af = Dot<T>::codes(kf[t][k / 2][k % 2 * 2], kf[t][k / 2][k % 2 * 2 + 1], sk);
+        const u32x4 af = Dot<T>::codes(kf[t][k / 2][k % 2 * 2], kf[t][k / 2][k % 2 * 2 + 1], by);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
           s[mt][t] = Dot<T>::mfma(af, qf[mt][k], k == 0 ? (f32x4){0, 0, 0, 0} : s[mt][t]);
@@ -929,8 +933,8 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
 #pragma unroll
       for (int e = 1; e < 16; ++e) top = fmaxf(top, s[mt][e / 4][e % 4]);
       top = group_max(top);
-      if (__any(fmaf(top, 0.5f, -ref[mt]) * a.scale2 > LAG)) {
-        const float to = fmaxf(ref[mt], top * 0.5f);
+      if (__any(fmaf(top, half, -ref[mt]) * a.scale2 > LAG)) {
+        const float to = fmaxf(ref[mt], top * half);
         const float alpha = fast_exp2((ref[mt] - to) * a.scale2);
         ref[mt] = to;
 #pragma unroll
@@ -941,7 +945,7 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
           for (int r = 0; r < 4; ++r) acc[mt][t][r] *= alpha;
       }
       auto weight = [&](float y) __attribute__((always_inline)) {
-        return fast_exp2(fmaf(fmaf(y, 0.5f, -ref[mt]), a.scale2, BIAS));
+        return fast_exp2(fmaf(fmaf(y, half, -ref[mt]), a.scale2, BIAS));
       };
 #pragma unroll
       for (int u = 0; u < 2; ++u)

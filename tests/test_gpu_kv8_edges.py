@@ -72,3 +72,37 @@ def test_write_padded_past_the_capacity(gpu):
                 assert (got[x][b, :, n:] == 13.0).all()            # (0x55)
             for x in ("ke", "ve"):
                 assert np.array_equal(got[x][b, :, :-(-n // 64)], ref[x][b, :, :-(-n // 64)]), (S, b, x)
+
+
+@pytest.mark.parametrize("D,G,s,n", [
+    (32, 1, 1, 100), (64, 4, 1, 4000), (128, 4, 1, 100), (128, 4, 1, 20001), (256, 2, 1, 3000),   # one row tile a wave
+    (64, 4, 6, 2000), (128, 8, 4, 500), (256, 8, 4, 500),                                         # two
+    (32, 8, 8, 700), (128, 8, 8, 700), (128, 4, 40, 500),                                         # four, and several
+])
+def test_rows_of_the_largest_keys(gpu, D, G, s, n):
+    """Keys up to bfloat16's largest: their codes reach 256 * 2^120, which no
+    bfloat16 and no float32 holds, though their scores are ordinary."""
+    from delta_attention import ops
+    g = torch.Generator().manual_seed(D + n)
+    top = torch.finfo(torch.bfloat16).max
+    k = torch.randn(1, n, 2, D, generator=g) * 2.0 ** 126
+    k[0, ::7, :, 3] = float(top)
+    k[0, 5::11, 1, 0] = -float(top)
+    k = k.clamp(-float(top), float(top)).to(torch.bfloat16)
+    k[0, n // 2:n // 2 + 70] *= 2.0 ** -8                # (and a block or two of a smaller scale)
+    v = torch.randn(1, n, 2, D, generator=g).to(torch.bfloat16)
+    q = (1 + torch.rand(1, 2 * G, s, D, generator=g)) * 2.0 ** -125
+    q = (q * (torch.randint(0, 2, q.shape, generator=g) * 2 - 1)).to(torch.bfloat16)
+    c, ref = ops.kv8_empty(1, 2, n, D), K8.new_cache(1, 2, -(-n // 64) * 64, D)
+    for t in c[:2]:
+        t.view(torch.uint8).fill_(0x7f)
+    ops.kv8_write(c, k.cuda(), v.cuda(), 0)
+    K8.write(ref, np64(k), np64(v), [0])
+    assert ref["ke"].max() == 120 and np.nanmax(np.abs(ref["k"])) >= 256
+    kk, vv = K8.values(ref)
+    for scale in (D ** -0.5, -0.02):
+        got = ops.kv8_attention(q.cuda(), c, n_keys=n, sm_scale=scale)
+        want, spread = K8.rows(np64(q), kk, vv, [n], 0, 0, scale)
+        tol = tolerance(want, spread, D, n, torch.bfloat16)
+        d = np.abs(np64(got) - want)
+        assert np.isfinite(np64(got)).all() and (d <= tol).all(), float((d / tol).max())
