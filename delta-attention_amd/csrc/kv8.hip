@@ -709,6 +709,11 @@ __device__ __forceinline__ bool locate(const RowsArgs& a, int i, Place& p) {
   return true;
 }
 
+// What a row's sums are divided by: a row without keys (standing before the
+// sequence's start) is zero; one whose every score is -inf has no weight either,
+// and no softmax: NaN.
+__device__ __forceinline__ float inverse(float weight, int row) { return row < 0 ? 0.f : 1.f / weight; }
+
 __device__ __forceinline__ float group_max(float x) {   // over the four lanes of one row
   const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return max32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
@@ -1052,10 +1057,10 @@ __global__ __launch_bounds__(64 * WAVES, rows_waves(D, MT)) void kv8_rows_kernel
         for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], k, o[e]);
       }
       if (p.n_split == 1) {
-        const float inv = L == 0.f ? 0.f : 1.f / L;
+        const int m = m0 + row, i = fdiv(m, a.heads);
+        const float inv = inverse(L, n - a.s + i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] *= inv;
-        const int m = m0 + row, i = fdiv(m, a.heads);
         store4<T>(a, b, hk * a.G + m - i * a.G, i, d, o);
       } else {
         *(f32x4*)(part + row * D + d) = o;
@@ -1091,6 +1096,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
   const int t = threadIdx.x % CT, sg = threadIdx.x / CT;
   const float* part = a.part + (int64_t)p.slot * a.pitch;
   const int64_t pitch = a.pitch * a.n_rt;
+  const int n = keys_of(a, p.b);
   float M = NO_KEYS, L = 0.f;
   f32x4 o = {0, 0, 0, 0};
   constexpr int U = 4;                         // items whose loads are in flight together
@@ -1139,7 +1145,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = fmaf(y[e], k, o[e]);
   }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const float inv = inverse(L, n - a.s + qi);
 #pragma unroll
   for (int e = 0; e < 4; ++e) o[e] *= inv;
   store4<T>(a, p.b, hk * a.G + m - qi * a.G, qi, t * 4, o);

@@ -106,3 +106,35 @@ def test_rows_of_the_largest_keys(gpu, D, G, s, n):
         tol = tolerance(want, spread, D, n, torch.bfloat16)
         d = np.abs(np64(got) - want)
         assert np.isfinite(np64(got)).all() and (d <= tol).all(), float((d / tol).max())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,cap,n,s,window", [(128, 128, 70, 3, 0), (64, 8192, 8000, 2, 0), (128, 8192, 8000, 9, 700),
+                                              (256, 4096, 4001, 1, 0), (32, 256, 2, 4, 0)])
+def test_rows_whose_every_score_is_minus_infinity(gpu, D, cap, n, s, window, dtype):
+    """They have no softmax: NaN. Zeros are for rows without keys alone."""
+    from delta_attention import ops
+    g = torch.Generator().manual_seed(n)
+    k = torch.randn(1, n, 1, D, generator=g)
+    k[..., 5] = 1 + torch.rand(1, n, 1, generator=g)
+    c = ops.kv8_empty(1, 1, cap, D)
+    ops.kv8_write(c, k.to(DT[dtype]).cuda(), k.to(DT[dtype]).cuda(), 0)
+    q = torch.randn(1, 4, s, D, generator=g).to(DT[dtype]).cuda()
+    count = torch.tensor([n], dtype=torch.int32, device="cuda")
+    for keys in (n, count):
+        usual = ops.kv8_attention(q, c, n_keys=keys, window=window, sm_scale=0.1)
+        bad = q.clone()
+        bad[0, 2, :, 5] = -float("inf")
+        got = ops.kv8_attention(bad, c, n_keys=keys, window=window, sm_scale=0.1)
+        empty = max(s - n, 0)                             # rows before the sequence's start
+        assert (got[:, :, :empty] == 0).all() and got[0, 2, empty:].isnan().all()
+        for h in (0, 1, 3):
+            assert torch.equal(got[0, h], usual[0, h])
+    # sequences of different lengths, the count of each on the device
+    two = ops.KV8(*(t.expand(3, *t.shape[1:]) for t in c))
+    lens = torch.tensor([n, 1, 0], dtype=torch.int32, device="cuda")
+    got = ops.kv8_attention(bad.expand(3, 4, s, D), two, n_keys=lens, window=window, sm_scale=0.1)
+    for b, m in enumerate((n, 1, 0)):
+        empty = max(s - m, 0)
+        assert (got[b, :, :empty] == 0).all() and got[b, 2, empty:].isnan().all()
+        assert got[b, [0, 1, 3]].isfinite().all()
