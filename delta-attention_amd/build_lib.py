@@ -1,5 +1,5 @@
 """Build libdelta_attn.so (the C-ABI library) for gfx950 with hipcc, and the
-extension module of the 8-bit cache's Python calls with g++.
+extension module of the 8-bit cache's Python calls with a host compiler.
 
 Run as a script or call ``build()``. Both land next to the Python package
 (delta_attention/libdelta_attn.so, _kv8_ext.so) so that they travel with the
@@ -8,12 +8,14 @@ tree.
 
 from __future__ import annotations
 
-import importlib.util
 import os
+import shlex
+import shutil
 import subprocess
 import sys
 import sysconfig
 import tempfile
+import warnings
 from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
@@ -52,9 +54,13 @@ def hipcc() -> str:
     return path if os.path.exists(path) else "hipcc"
 
 
-def torch_dir() -> str:
-    """The installed torch package's folder (found without importing it)."""
-    return importlib.util.find_spec("torch").submodule_search_locations[0]
+def host_cxx() -> list:
+    """The C++ compiler of host code: $CXX, or the first of g++, c++ and ROCm's
+    clang++ that is there."""
+    if os.environ.get("CXX"):
+        return shlex.split(os.environ["CXX"])
+    rocm = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "bin", "amdclang++")
+    return [next((c for c in ("g++", "c++", rocm) if shutil.which(c)), "g++")]
 
 
 def _run(cmd, verbose: bool) -> None:
@@ -70,36 +76,50 @@ def _run(cmd, verbose: bool) -> None:
         print(warn, file=sys.stderr)
 
 
+def _compile_ext(verbose: bool, out: str) -> None:
+    import torch          # (the extension is built against it)
+    t = os.path.dirname(torch.__file__)
+    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
+    _run([*host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+          f"-I{INCLUDE}", f"-I{sysconfig.get_paths()['include']}", "-isystem", os.path.join(t, "include"),
+          "-isystem", os.path.join(t, "include", "torch", "csrc", "api", "include"),
+          "-isystem", os.path.join(rocm, "include"), os.path.join(CSRC, EXT_SOURCE), "-o", out,
+          f"-L{t}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
+          "-L" + os.path.join(rocm, "lib"), "-lamdhip64", f"-Wl,-rpath,{t}/lib"], verbose)
+
+
 def build_ext(verbose: bool = False, out: str = EXT_OUT) -> str:
     """The extension module of the 8-bit cache's calls (host code, against the
     installed torch)."""
-    t = torch_dir()
-    rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-    _run(["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-          f"-I{INCLUDE}", f"-I{sysconfig.get_paths()['include']}", "-isystem", os.path.join(t, "include"),
-          "-isystem", os.path.join(t, "include", "torch", "csrc", "api", "include"),
-          "-isystem", os.path.join(rocm, "include"), os.path.join(CSRC, EXT_SOURCE), "-o", out + ".tmp",
-          f"-L{t}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-lamdhip64",
-          f"-Wl,-rpath,{t}/lib"], verbose)
+    _compile_ext(verbose, out + ".tmp")
     os.replace(out + ".tmp", out)
     return out
 
 
 def build(verbose: bool = False, out: str = OUT) -> str:
     """Every source at once (each an object of its own), then the library; the
-    extension beside it when the library is the package's."""
+    extension beside it when the library is the package's. hipcc is all that the
+    library needs: without a host compiler, Python's headers or torch only the
+    extension is left out, with a warning, and the calls that need it say so."""
     compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
     with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(SOURCES) + 1) as pool:
         objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
         jobs = [pool.submit(_run, [hipcc(), *compile_flags, f"-I{INCLUDE}", f"-I{CSRC}", "-c",
                                    os.path.join(CSRC, s), "-o", o], verbose)
                 for s, o in zip(SOURCES, objs)]
-        if out == OUT:
-            jobs.append(pool.submit(build_ext, verbose))
+        ext = pool.submit(_compile_ext, verbose, EXT_OUT + ".tmp") if out == OUT else None
         for j in jobs:
             j.result()
         _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *objs, "-o", out + ".tmp"], verbose)
     os.replace(out + ".tmp", out)
+    if ext is not None:
+        if ext.exception() is None:
+            os.replace(EXT_OUT + ".tmp", EXT_OUT)
+        else:
+            if os.path.exists(EXT_OUT):      # (an older one's structs need not be this library's)
+                os.remove(EXT_OUT)
+            warnings.warn(f"the 8-bit cache's calls are not built: {ext.exception()}")
     return out
 
 

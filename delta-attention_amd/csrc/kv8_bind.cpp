@@ -38,6 +38,11 @@ struct PythonError {};     // a Python exception is set
 #define REQUIRE(cond, ...) \
   if (!(cond)) throw Refused(c10::str(__VA_ARGS__))
 
+PyObject* new_ref(PyObject* o) {
+  Py_INCREF(o);
+  return o;
+}
+
 const at::Tensor& tensor(PyObject* o, const char* what) {
   REQUIRE(THPVariable_Check(o), what, ": a tensor is needed");
   return THPVariable_Unpack(o);
@@ -213,7 +218,7 @@ PyObject* read(PyObject* const* a) {
     const On on(dev);
     check(g_read(&x, on.stream()), "da_kv8_read");
   }
-  if (given) return Py_NewRef(a[5]);
+  if (given) return new_ref(a[5]);
   PyObject* result = PyTuple_New(2);
   if (!result) throw PythonError();
   PyTuple_SET_ITEM(result, 0, THPVariable_Wrap(std::move(k)));
@@ -278,7 +283,7 @@ PyObject* attention(PyObject* const* a) {
     }
     check(g_attn(&x, on.stream()), "da_kv8_attn_fwd");
   }
-  if (a[6] != Py_None) return Py_NewRef(a[6]);
+  if (a[6] != Py_None) return new_ref(a[6]);
   return THPVariable_Wrap(out);
 }
 
@@ -290,7 +295,7 @@ PyObject* bind(PyObject* const* a) {
   g_read = (decltype(g_read))address(a[1]);
   g_attn = (decltype(g_attn))address(a[2]);
   g_attn_bytes = (decltype(g_attn_bytes))address(a[3]);
-  Py_XSETREF(g_check, Py_NewRef(a[4]));
+  Py_XSETREF(g_check, new_ref(a[4]));
   Py_RETURN_NONE;
 }
 
