@@ -559,7 +559,7 @@ constexpr int WAVES = 4;
 // Waves per SIMD of the rows kernel: what the registers of a block's codes, the
 // sums and MT tiles of probabilities leave room for.
 __host__ __device__ constexpr int rows_waves(int D, int mt) {
-  return D * mt <= 64 ? (mt == 1 ? 4 : mt == 2 ? 3 : 2) : D * mt <= 128 ? 2 : 1;
+  return D * mt <= 64 ? (mt == 1 ? 4 : 3) : D * mt <= 128 ? 2 : 1;
 }
 constexpr int CHUNK = 64;                    // blocks of an item at most, where there are many
 
