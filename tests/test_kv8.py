@@ -123,6 +123,34 @@ def test_ops_refuse_a_cache_without_heads():
             call()
 
 
+def test_the_extension_refuses_what_is_no_cache_or_no_result():
+    """Through its own signature: (cache, start, n, n_keys, dtype, results)."""
+    c = ops.kv8_empty(1, 2, 128, 64, "cpu")
+    read = L.kv8_ext().read
+    k = torch.zeros(1, 2, 5, 64, dtype=torch.bfloat16)
+    for bad in (tuple(c)[:3], None, [*c], c.k):
+        with pytest.raises(AssertionError, match="KV8 cache"):
+            read(bad, 0, 5, None, torch.bfloat16, (k, k.clone()))
+    for bad in (k, (k,), [k, k]):
+        with pytest.raises(AssertionError, match="out: two tensors"):
+            read(c, 0, 5, None, torch.bfloat16, bad)
+    for bad in ((k, None), (None, k)):
+        with pytest.raises(AssertionError, match="a tensor is needed"):
+            read(c, 0, 5, None, torch.bfloat16, bad)
+    for bad in ((k, k[:, :, :4]), (k[:, :1], k[:, :1]), (k, k.half()), (k, k.transpose(2, 3).contiguous().transpose(2, 3))):
+        with pytest.raises(AssertionError, match="the results are two"):
+            read(c, 0, 5, None, torch.bfloat16, bad)
+    with pytest.raises(AssertionError, match="not supported"):
+        read(c, 0, 5, None, torch.bfloat16, (k.float(), k.float()))
+    for bad in (None, "bfloat16", 5):
+        with pytest.raises(AssertionError, match="torch.dtype"):
+            read(c, 0, 5, None, bad, None)
+    with pytest.raises(AssertionError, match="not supported"):
+        read(c, 0, 5, None, torch.float32, None)
+    with pytest.raises(TypeError):
+        read(c, 0, 5, None, k, k, k)
+
+
 # the header's structs, in native alignment
 _CACHE = "4P8q4i"                                # k, v, k_scale, v_scale; {batch, head} strides; B, Hkv, cap, D
 WRITE = struct.Struct(_CACHE + "4P7q4i")         # k, v, pos_dev, counts_dev; strides, pos; S, 2 flags, dtype
