@@ -138,3 +138,39 @@ def test_rows_whose_every_score_is_minus_infinity(gpu, D, cap, n, s, window, dty
         empty = max(s - m, 0)
         assert (got[b, :, :empty] == 0).all() and got[b, 2, empty:].isnan().all()
         assert got[b, [0, 1, 3]].isfinite().all()
+
+
+@pytest.mark.parametrize("D,S", [(64, 1), (256, 1), (64, 3), (256, 2), (64, 16), (256, 4), (128, 90), (32, 200), (256, 64)])
+def test_write_clamps_counts(gpu, D, S):
+    """Counts above S write S tokens, those below zero none, by every kernel of
+    the write: behind rows that were written before, up to the capacity's end,
+    and the rows behind keep their bytes."""
+    from delta_attention import ops
+    B, Hkv, cap = 4, 2, 512
+    c, ref = ops.kv8_empty(B, Hkv, cap, D), K8.new_cache(B, Hkv, cap, D)
+    for t in c[:2]:
+        t.view(torch.uint8).fill_(0x55)                            # 13
+    pos = [0, 64, 37, cap - S]
+    g = torch.Generator().manual_seed(S)
+    first, k, v = (torch.randn(B, n, Hkv, D, generator=g).bfloat16().cuda() for n in (cap, S, S))
+    ops.kv8_write(c, first, -first, 0, counts=torch.tensor(pos, dtype=torch.int32, device="cuda"))
+    K8.write(ref, np64(first), np64(-first), [0] * B, pos)
+    at = torch.tensor(pos, device="cuda")
+    before = [t.clone() for t in c]
+    for low in (torch.tensor([-5, -1, -2 ** 31, 0], dtype=torch.int32, device="cuda"),
+                torch.tensor([-3], dtype=torch.int32, device="cuda")):
+        ops.kv8_write(c, k, v, at, counts=low)
+        for t, u in zip(c, before):
+            assert torch.equal(t.view(torch.uint8), u.view(torch.uint8))
+    ops.kv8_write(c, k, v, at, counts=torch.tensor([1000, S + 1, 2 ** 31 - 1, S + 7], dtype=torch.int32, device="cuda"))
+    K8.write(ref, np64(k), np64(v), pos, [S] * B)
+    got = to_oracle(c)
+    for b in range(B):
+        n = pos[b] + S
+        for x in ("k", "v"):
+            assert np.array_equal(got[x][b, :, :n], ref[x][b, :, :n]), (b, x)
+            assert (got[x][b, :, n:] == 13.0).all(), (b, x)
+        for x in ("ke", "ve"):
+            nb = -(-n // 64)
+            assert np.array_equal(got[x][b, :, :nb], ref[x][b, :, :nb]), (b, x)
+            assert (got[x][b, :, nb:] == K8.E_MIN).all()
