@@ -662,7 +662,14 @@ def kv8_attention(q: torch.Tensor, cache: KV8, *, n_keys, window: int = 0, sink:
     n_keys: an int, or an int32 device tensor of one entry or one per sequence,
     read when the kernels run (a recorded call serves every length; counts are
     clamped to the capacity). add: a tensor like q; rnd(rnd(row) + add). A new
-    result has q's strides where q is dense."""
+    result has q's strides where q is dense.
+
+    Keys and values count as code * scale. Scores and sums are float32, the
+    probabilities float16: each is off by up to 2^-11 of itself, or 2^-33 of the
+    row's largest, below which a key counts for nothing. The sums are right for
+    n |v| < 2^114 (|v| < 2^97 at 131072 keys, 2^90 at 2^24); past that they may
+    be infinite, though the cache stores, and kv8_read returns, bfloat16's whole
+    range."""
     return L.kv8_ext().attention(q, cache, n_keys, window, sink, sm_scale, out, add)
 
 

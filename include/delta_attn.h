@@ -330,10 +330,17 @@ int da_kv8_read(const da_kv8_read_args* args, void* stream);
  * keys, row i of q [B, Hq, s, D] (strides {batch, head, row}) stands at r = n - s
  * + i and sees the keys j <= r, with window > 0 only those with j < sink or
  * j > r - window (the decode rows of da_decode_attn_fwd, window 0: every key).
- * out [B, Hq, s, D] = softmax(sm_scale q k) v in fp32, rounded once (sums of
- * values are held times up to 2^14 a key: right for |v| up to 2^90); rows that
- * see no key (r < 0) are zero. addend (optional, like q): out = rnd(rnd(row) +
- * addend). n is n_keys_dev[b] (or n_keys_dev[0] when n_keys_per_seq is 0) read
+ * out [B, Hq, s, D] = softmax(sm_scale q k) v with fp32 scores, references and
+ * sums, rounded at the end; keys and values count as code * scale, also where
+ * that passes the type's largest (da_kv8_read saturates there). The products with
+ * the values and the rows' weights take the probabilities in fp16, relative to a
+ * reference at or up to 2^6 below the row's largest: each is off by up to 2^-11 of
+ * itself, or 2^-33 of the reference's, below which it counts as none (n keys so
+ * far below the largest lose up to n * 2^-33 of the row). A key's value enters the
+ * fp32 sums times up to 2^14: they are right for n |v| < 2^114 (|v| < 2^90 at 2^24
+ * keys, 2^97 at 131072) and may be infinite past it. Rows that see no key (r < 0)
+ * are zero; a row whose every score is -inf is NaN. addend (optional, like q): out
+ * = rnd(rnd(row) + addend). n is n_keys_dev[b] (or n_keys_dev[0] when n_keys_per_seq is 0) read
  * when the kernels run and clamped to [0, cap], or the host's n_keys.
  * DA_ERR_INVALID_ARG for an out with a zero stride over more than one entry.
  * Workspace: da_kv8_attn_workspace_bytes(..., max_keys = cap with a device

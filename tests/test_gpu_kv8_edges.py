@@ -174,3 +174,28 @@ def test_write_clamps_counts(gpu, D, S):
             nb = -(-n // 64)
             assert np.array_equal(got[x][b, :, :nb], ref[x][b, :, :nb]), (b, x)
             assert (got[x][b, :, nb:] == K8.E_MIN).all()
+
+
+def test_rows_hold_sums_of_large_values(gpu):
+    """Values up to n |v| < 2^114, with keys whose weights run up to 2^14 times
+    what they count: the first blocks of each wave set its reference, and every
+    later score lies 5.9 (log2) above it."""
+    from delta_attention import ops
+    n, D = 2500, 32
+    g = torch.Generator().manual_seed(1)
+    k = torch.zeros(1, n, 1, D)
+    k[0, 256:, 0, 0] = 4.0
+    v = (1 + torch.rand(1, n, 1, D, generator=g) * 0.875) * 2.0 ** 101
+    k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+    assert n * float(v.max()) < 2.0 ** 114
+    q = torch.zeros(1, 2, 1, D, dtype=torch.bfloat16)
+    q[..., 0] = 1
+    scale = 5.9 * float(np.log(2.0)) / 4
+    c, ref = ops.kv8_empty(1, 1, n, D), K8.new_cache(1, 1, 2560, D)
+    ops.kv8_write(c, k.cuda(), v.cuda(), 0)
+    K8.write(ref, np64(k), np64(v), [0])
+    kk, vv = K8.values(ref)
+    want, spread = K8.rows(np64(q), kk, vv, [n], 0, 0, scale)
+    got = np64(ops.kv8_attention(q.cuda(), c, n_keys=n, sm_scale=scale))
+    tol = tolerance(want, spread, D, n, torch.bfloat16)
+    assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
