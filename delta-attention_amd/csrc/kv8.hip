@@ -768,7 +768,7 @@ __device__ __forceinline__ void store4(const RowsArgs& a, int b, int h, int i, i
 // when the first product has read this one's, its values after the second.
 //
 // What bounds it: memory, where there is enough of it (a dense row of 32 / 8 heads
-// over 131072 keys 43.8 us, 6.1 TB/s with the first loads; eight sequences of that
+// over 131072 keys 44.2 us, 6.1 TB/s with the first loads; eight sequences of that
 // length 6.65 TB/s); else a launch (1.9 us) and the loads that wait for each other
 // (arguments, count, codes: 5.2 us for a single block). Registers, not MFMA or
 // conversions, limit the waves (203 at head_dim 128 and one row tile).

@@ -38,9 +38,11 @@ class CachedKeys8(NamedTuple):
 
 # Rows (tokens times query heads per kv head) up to which a pass over an 8-bit
 # cache reads its codes (ops.kv8_attention); more rows read the keys back into
-# 16 bits first and run the rows kernel. 32 query heads over 32768 / 131072
-# keys: 256 rows 66 / 219 us so, 91 / 276 by the read-back; 512 rows 115 / 433
-# us, 115 / 391 by the read-back.
+# 16 bits first and run the rows kernel. One bound for all shapes, taken at 32 /
+# 8 heads of 128 over 32768 / 131072 keys: 256 rows 61 / 229 us so, 90 / 279 by
+# the read-back; 512 rows 116 / 434 us, 117 / 393 by the read-back. It is early
+# for short caches (4096 keys, 512 rows: 32 and 36 us) and head_dim 256 (32768
+# keys, 384 rows of 16 / 8 heads: 183 and 195 us).
 DIRECT_ROWS8 = 256
 
 
