@@ -1159,6 +1159,7 @@ __global__ __launch_bounds__(THREADS) void kv8_join_kernel(RowsArgs a) {
 struct RowsPlan {
   int mt, rows, n_rt;
   int64_t pairs, items;     // (sequence, kv head, row tile) triples; item slots
+  int64_t grid;             // workgroups: several row tiles in multiples of 8 of them, as they are dealt to the XCDs
   int64_t pitch;            // floats of an item's partial sums (a multiple of 4)
   int slots, whole, most;
   FastDiv round;
@@ -1201,6 +1202,8 @@ bool plan_rows(RowsPlan& p, int B, int Hkv, int G, int s, int D, int64_t max_key
       if (budget + p.pairs < p.items) p.items = budget + p.pairs;
     }
   }
+  const int64_t group = p.n_rt > 1 ? 8 * (int64_t)p.n_rt : 1;
+  p.grid = (p.items + group - 1) / group * group;
   p.pitch = (int64_t)p.rows * D + (2 * p.rows + 3) / 4 * 4;
   p.bytes = p.whole > 0 ? 0 : (size_t)(p.items * p.pitch) * sizeof(float);
   return true;
@@ -1221,9 +1224,7 @@ int take_cache(Cache& c, const da_kv8_cache& x, int dtype) {
 
 template <typename T, int D>
 void launch_rows(const RowsArgs& a, const RowsPlan& p, hipStream_t st) {
-  // (with several row tiles a multiple of 8 of them, as the items are dealt to the XCDs)
-  const int64_t group = p.n_rt > 1 ? 8 * (int64_t)p.n_rt : 1;
-  const dim3 grid((unsigned)((p.items + group - 1) / group * group)), block(64 * WAVES);
+  const dim3 grid((unsigned)p.grid), block(64 * WAVES);
   if (p.mt == 1) {
     hipLaunchKernelGGL((kv8_rows_kernel<T, D, 1>), grid, block, 0, st, a);
   } else if (p.mt == 2) {
@@ -1383,7 +1384,7 @@ extern "C" int da_kv8_attn_fwd(const da_kv8_attn_args* x, void* stream) {
   a.sink = x->sink < cap ? x->sink : cap;
   RowsPlan p;
   if (!plan_rows(p, B, Hkv, Hq / Hkv, s, x->cache.D, x->n_keys_dev ? cap : x->n_keys, a.window, a.sink) ||
-      p.items * 256 > 0x7fffffffll || p.pairs * (cap / KB) > 0x70000000ll)
+      p.items * 256 > 0x7fffffffll || p.grid * (64 * WAVES) > 0xffffffffll || p.pairs * (cap / KB) > 0x70000000ll)
     return DA_ERR_INVALID_ARG;
   if (p.bytes > 0 && (!x->workspace || x->workspace_bytes < (int64_t)p.bytes)) return DA_ERR_WORKSPACE;
   if (!aligned16(x->workspace)) return DA_ERR_ALIGNMENT;

@@ -261,3 +261,11 @@ def test_c_results_that_share_their_place(lib):
         assert read(bad, good) == read(good, bad) == L.DA_ERR_INVALID_ARG, bad
         assert rows(bad) == L.DA_ERR_INVALID_ARG, bad
     assert read((0, 0, 0), (0, 0, 0), n=0) == rows((0, 0, 0), s=0) == L.DA_OK
+
+
+def test_c_rows_past_a_grids_threads(lib):
+    """2^22 row tiles, dealt to the XCDs by eights, pass a grid's 2^32 threads."""
+    a = dict(CACHE, Hkv=1, D=32)
+    rc = lib.da_kv8_attn_fwd(ATTN.pack(*_head(a), 16, 16, 0, 0, 0, 0, *((32,) * 6), *((0,) * 3), 1, 1 << 28, 0, 64, 0, 0,
+                                       L.DA_BF16, 0.1), None)
+    assert rc == L.DA_ERR_INVALID_ARG
