@@ -203,9 +203,10 @@ PyObject* read(PyObject* const* a) {
     const at::ScalarType type = ((THPDtype*)a[4])->scalar_type;
     x.dtype = dtype_code(type);
     on_gpu(dev);
-    const at::Tensor both = at::empty({2, B, x.cache.Hkv, n, x.cache.D}, at::TensorOptions().dtype(type).device(dev));
-    k = both.select(0, 0);
-    v = both.select(0, 1);
+    // (two allocations: views of one would share a version, and keep each other's memory)
+    const auto options = at::TensorOptions().dtype(type).device(dev);
+    k = at::empty({B, x.cache.Hkv, n, x.cache.D}, options);
+    v = at::empty({B, x.cache.Hkv, n, x.cache.D}, options);
   }
   x.n_keys_dev = entries<int32_t>(a[3], B, at::kInt, dev, "n_keys", x.n_keys_per_seq);
   if (B > 0 && n > 0) {

@@ -199,3 +199,22 @@ def test_rows_hold_sums_of_large_values(gpu):
     got = np64(ops.kv8_attention(q.cuda(), c, n_keys=n, sm_scale=scale))
     tol = tolerance(want, spread, D, n, torch.bfloat16)
     assert np.isfinite(got).all() and (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+def test_read_results_are_independent(gpu):
+    """Changing one result in place leaves the other as autograd saved it, and
+    neither keeps the other's memory."""
+    from delta_attention import ops
+    c = ops.kv8_empty(1, 2, 128, 64)
+    x = torch.randn(1, 100, 2, 64, device="cuda").bfloat16()
+    ops.kv8_write(c, x, x, 0)
+    k, v = ops.kv8_read(c, 0, 100)
+    p = torch.rand(1, 2, 3, 100, device="cuda", requires_grad=True)
+    y = (p.unsqueeze(-1) * v.float().unsqueeze(2)).sum()
+    w = torch.ones_like(v, requires_grad=True)
+    z = (w * v).sum()                                   # (saves v itself)
+    k.mul_(2)
+    (y + z).backward()
+    assert torch.equal(w.grad, v) and not k._is_view() and not v._is_view()
+    for t in (k, v):
+        assert t.untyped_storage().nbytes() == t.numel() * 2
