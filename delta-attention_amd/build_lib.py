@@ -1,9 +1,10 @@
 """Build libdelta_attn.so (the C-ABI library) for gfx950 with hipcc, and the
-extension module of the 8-bit cache's Python calls with a host compiler.
+extension modules of the 8-bit cache's and the generation's Python calls with a
+host compiler.
 
-Run as a script or call ``build()``. Both land next to the Python package
-(delta_attention/libdelta_attn.so, _kv8_ext.so) so that they travel with the
-tree.
+Run as a script or call ``build()``. All land next to the Python package
+(delta_attention/libdelta_attn.so, _kv8_ext.so, _gen_ext.so) so that they
+travel with the tree.
 """
 
 from __future__ import annotations
@@ -24,10 +25,11 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 OUT = os.path.join(HERE, "delta_attention", "libdelta_attn.so")
 SOURCES = ["attn_kernels.hip", "attn_bwd.hip", "delta_add.hip", "rope.hip", "norm.hip",
-           "anchor_cos.hip", "adapt_loop.hip", "kv8.hip"]
+           "anchor_cos.hip", "adapt_loop.hip", "kv8.hip", "sample.hip"]
 ARCH = "gfx950"
 EXT_SOURCE = "kv8_bind.cpp"
 EXT_OUT = os.path.join(HERE, "delta_attention", "_kv8_ext.so")
+GEN_SOURCE = "gen_bind.cpp"       # beside EXT_OUT as _gen_ext.so
 
 # Packed fp32 VALU ops are disabled: they are not used by hand and must not be
 # formed by the compiler either.
@@ -76,50 +78,61 @@ def _run(cmd, verbose: bool) -> None:
         print(warn, file=sys.stderr)
 
 
-def _compile_ext(verbose: bool, out: str) -> None:
+def _compile_ext(verbose: bool, source: str, out: str) -> None:
     import torch          # (the extension is built against it)
     t = os.path.dirname(torch.__file__)
     rocm = os.environ.get("ROCM_PATH", "/opt/rocm")
-    _run([*host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+    _run([*host_cxx(), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-Wno-unused-function",
+          "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
           f"-I{INCLUDE}", f"-I{sysconfig.get_paths()['include']}", "-isystem", os.path.join(t, "include"),
           "-isystem", os.path.join(t, "include", "torch", "csrc", "api", "include"),
-          "-isystem", os.path.join(rocm, "include"), os.path.join(CSRC, EXT_SOURCE), "-o", out,
+          "-isystem", os.path.join(rocm, "include"), os.path.join(CSRC, source), "-o", out,
           f"-L{t}/lib", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip",
           "-L" + os.path.join(rocm, "lib"), "-lamdhip64", f"-Wl,-rpath,{t}/lib"], verbose)
 
 
-def build_ext(verbose: bool = False, out: str = EXT_OUT) -> str:
-    """The extension module of the 8-bit cache's calls (host code, against the
-    installed torch)."""
-    _compile_ext(verbose, out + ".tmp")
-    os.replace(out + ".tmp", out)
-    return out
+def _extensions() -> list:
+    """(source, module, what it holds) of the extension modules (host code,
+    against the installed torch)."""
+    return [(EXT_SOURCE, EXT_OUT, "the 8-bit cache's calls are"),
+            (GEN_SOURCE, os.path.join(os.path.dirname(EXT_OUT), "_gen_ext.so"), "the generation calls are")]
+
+
+def build_ext(verbose: bool = False) -> list:
+    """The extension modules alone."""
+    outs = []
+    for source, out, _ in _extensions():
+        _compile_ext(verbose, source, out + ".tmp")
+        os.replace(out + ".tmp", out)
+        outs.append(out)
+    return outs
 
 
 def build(verbose: bool = False, out: str = OUT) -> str:
     """Every source at once (each an object of its own), then the library; the
-    extension beside it when the library is the package's. hipcc is all that the
+    extensions beside it when the library is the package's. hipcc is all that the
     library needs: without a host compiler, Python's headers or torch only the
-    extension is left out, with a warning, and the calls that need it say so."""
+    extensions are left out, with a warning, and the calls that need them say so."""
     compile_flags = [f for f in HIPCC_FLAGS if f != "-shared"]
-    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(SOURCES) + 1) as pool:
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(len(SOURCES) + 2) as pool:
         objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
         jobs = [pool.submit(_run, [hipcc(), *compile_flags, f"-I{INCLUDE}", f"-I{CSRC}", "-c",
                                    os.path.join(CSRC, s), "-o", o], verbose)
                 for s, o in zip(SOURCES, objs)]
-        ext = pool.submit(_compile_ext, verbose, EXT_OUT + ".tmp") if out == OUT else None
+        exts = [(pool.submit(_compile_ext, verbose, source, path + ".tmp"), path, what)
+                for source, path, what in (_extensions() if out == OUT else [])]
         for j in jobs:
             j.result()
         _run([hipcc(), f"--offload-arch={ARCH}", "-fPIC", "-shared", *objs, "-o", out + ".tmp"], verbose)
     os.replace(out + ".tmp", out)
-    if ext is not None:
+    for ext, path, what in exts:
         if ext.exception() is None:
-            os.replace(EXT_OUT + ".tmp", EXT_OUT)
+            os.replace(path + ".tmp", path)
         else:
-            if os.path.exists(EXT_OUT):      # (an older one's structs need not be this library's)
-                os.remove(EXT_OUT)
-            warnings.warn(f"the 8-bit cache's calls are not built: {ext.exception()}")
+            if os.path.exists(path):         # (an older one's structs need not be this library's)
+                os.remove(path)
+            warnings.warn(f"{what} not built: {ext.exception()}")
     return out
 
 

@@ -15,6 +15,7 @@ import threading
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libdelta_attn.so")
 EXT_PATH = os.path.join(HERE, "_kv8_ext.so")
+GEN_PATH = os.path.join(HERE, "_gen_ext.so")
 
 DA_OK = 0
 DA_ERR_INVALID_ARG = -1
@@ -27,6 +28,7 @@ DA_ERR_SCRATCH = -7
 
 DA_BF16 = 0
 DA_FP16 = 1
+DA_FP32 = 2
 
 DA_EPI_OUTPUT = 0
 DA_EPI_DELTA = 1
@@ -71,6 +73,8 @@ EXPORTS = (
     "da_kv8_read",
     "da_kv8_attn_workspace_bytes",
     "da_kv8_attn_fwd",
+    "da_sample_workspace_bytes",
+    "da_sample",
 )
 
 _ERR_TEXT = {
@@ -90,6 +94,7 @@ class ExtensionMissing(RuntimeError):
 
 _lib = None
 _kv8_ext = None
+_gen_ext = None
 _lib_lock = threading.Lock()
 
 I64x3 = ctypes.c_int64 * 3
@@ -224,12 +229,14 @@ def _load() -> ctypes.CDLL:
                                      _p3, _p3, _p3, _p3, _i, _i, _i, _f,
                                      _i, _i, _i, _i, _i, _i, _d, _d, _d,
                                      _vp, _vp, _vp, _vp, _i, _vp, _sz, _i, _vp, _vp]
-    # (these take one struct; kv8_ext's functions pack it)
-    for f in (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd):
+    # (these take one struct; the functions of kv8_ext and gen_ext pack it)
+    for f in (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd, L.da_sample):
         f.restype = _i
         f.argtypes = [ctypes.c_char_p, _vp]
     L.da_kv8_attn_workspace_bytes.restype = _sz
     L.da_kv8_attn_workspace_bytes.argtypes = [_i, _i, _i, _i, _i, _i, _i, _i]
+    L.da_sample_workspace_bytes.restype = _sz
+    L.da_sample_workspace_bytes.argtypes = [_i, _i, _i]
     L.da_build_target.restype = ctypes.c_char_p
     L.da_build_target.argtypes = []
     return L
@@ -247,6 +254,24 @@ def check(rc: int, what: str) -> None:
     raise AssertionError(msg)
 
 
+def _extension(name: str, path: str, functions):
+    """An extension module of `path`, bound to the addresses of the library's
+    functions and to check."""
+    import torch  # noqa: F401  (its libraries are the extension's)
+    if not os.path.exists(path):
+        raise ExtensionMissing(
+            f"{path} is not built: run `python delta-attention_amd/build_lib.py` "
+            "(or __graft_entry__.build()) first")
+    loader = importlib.machinery.ExtensionFileLoader(f"{__package__}.{name}", path)
+    try:
+        m = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
+        loader.exec_module(m)
+    except ImportError as e:  # pragma: no cover - depends on the machine
+        raise ExtensionMissing(f"cannot load {path}: {e}") from e
+    m.bind(*(ctypes.cast(f, _vp).value for f in functions), check)
+    return m
+
+
 def kv8_ext():
     """The extension module of the 8-bit cache's calls (csrc/kv8_bind.cpp),
     loaded once and bound to the library's functions."""
@@ -256,21 +281,22 @@ def kv8_ext():
     L = lib()
     with _lib_lock:
         if _kv8_ext is None:
-            import torch  # noqa: F401  (its libraries are the extension's)
-            if not os.path.exists(EXT_PATH):
-                raise ExtensionMissing(
-                    f"{EXT_PATH} is not built: run `python delta-attention_amd/build_lib.py` "
-                    "(or __graft_entry__.build()) first")
-            loader = importlib.machinery.ExtensionFileLoader(f"{__package__}._kv8_ext", EXT_PATH)
-            try:
-                m = importlib.util.module_from_spec(importlib.util.spec_from_loader(loader.name, loader))
-                loader.exec_module(m)
-            except ImportError as e:  # pragma: no cover - depends on the machine
-                raise ExtensionMissing(f"cannot load {EXT_PATH}: {e}") from e
-            m.bind(*(ctypes.cast(f, _vp).value for f in (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd,
-                                                         L.da_kv8_attn_workspace_bytes)), check)
-            _kv8_ext = m
+            _kv8_ext = _extension("_kv8_ext", EXT_PATH, (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd,
+                                                         L.da_kv8_attn_workspace_bytes))
     return _kv8_ext
+
+
+def gen_ext():
+    """The extension module of the generation calls (csrc/gen_bind.cpp), loaded
+    once and bound to the library's functions."""
+    global _gen_ext
+    if _gen_ext is not None:
+        return _gen_ext
+    L = lib()
+    with _lib_lock:
+        if _gen_ext is None:
+            _gen_ext = _extension("_gen_ext", GEN_PATH, (L.da_sample, L.da_sample_workspace_bytes))
+    return _gen_ext
 
 
 def strides3(*s: int):

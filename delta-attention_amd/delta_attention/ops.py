@@ -674,6 +674,33 @@ def kv8_attention(q: torch.Tensor, cache: KV8, *, n_keys, window: int = 0, sink:
 
 
 # ---------------------------------------------------------------------------
+# generation
+
+# (checks and launches: csrc/gen_bind.cpp)
+
+def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0,
+                  min_p=0.0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """One token per row of logits [B, V] (bfloat16, float16, float32), drawn by
+    the given numbers u [B] (float32, in [0, 1)) -> (tokens int64 [B], their
+    log-probabilities float32 [B]) (da_sample).
+
+    A row's tokens are ordered by logit, largest first, equal ones by index. Kept
+    are the first top_k (0: all), of those the shortest run that reaches top_p of
+    their probability, of those the tokens of at least min_p times the largest
+    one's, and always the first one; the token is the first by index at which the
+    kept probabilities' sum passes u times their total. Probabilities are those
+    of logits / temperature; temperature 0 takes the first in order (then, and
+    where one token is kept, the log-probability is 0). Settings are numbers,
+    rounded to float32, or device tensors of one entry or one per row (float32;
+    top_k int32), read when the kernels run.
+
+    NaN and -inf logits are never drawn; where logits are +inf those share the
+    row. A row without any other logit gives token 0 and the log-probability
+    NaN. Sums are exact integers: a row's token does not depend on its batch."""
+    return L.gen_ext().sample(logits, u, temperature, top_k, top_p, min_p)
+
+
+# ---------------------------------------------------------------------------
 # decoder-layer element-wise kernels (full-model prefill)
 
 def _rows2d(t: torch.Tensor) -> Tuple[int, int]:

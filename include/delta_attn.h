@@ -48,6 +48,7 @@ extern "C" {
 
 #define DA_BF16 0
 #define DA_FP16 1
+#define DA_FP32 2                    /* logits of da_sample only */
 
 /* Epilogue modes of da_qsparse_attn_fwd. */
 #define DA_EPI_OUTPUT 0    /* o[b, h, i, :] = attention row i (the plain kernel) */
@@ -361,6 +362,45 @@ typedef struct {
 size_t da_kv8_attn_workspace_bytes(int B, int Hq, int Hkv, int s, int D, int max_keys,
                                    int window, int sink);
 int da_kv8_attn_fwd(const da_kv8_attn_args* args, void* stream);
+
+/*
+ * The next tokens of a batch: one token per row of logits [B, V] (row_stride
+ * elements apart, DA_BF16, DA_FP16 or DA_FP32; V up to 2^24, B up to 2^22 - 1)
+ * from a given number u[b] in [0, 1). No counterpart in the reference, whose
+ * loop is greedy (sample.py:178-179).
+ * Candidates are the logits above -inf that are numbers, ordered by logit,
+ * largest first, equal ones by index. Kept are the first top_k of them (0 and
+ * below: all); of those the shortest run whose weight reaches top_p times
+ * theirs (1 and above, NaN: all); of those the tokens with x >= max +
+ * temperature * ln(min_p); and the first one always. Weights are exp((x - max) /
+ * temperature). The token is the first by index at which the sum of the kept
+ * weights passes u times their total (u below 0 or NaN: as 0; 1 and above: the
+ * last kept one); logprobs[b] is ln(its weight / that total). A temperature of 0
+ * (or below, or NaN) takes the first candidate, log-probability 0; where several
+ * logits are +inf they weigh alike and the others nothing. A row without a
+ * candidate gives token 0 with the log-probability NaN.
+ * Weights are integers in units of 2^-45 of the largest (2^-(62 - ceil(log2 V))
+ * past 2^17 tokens) and summed as such: a token below half a unit is never
+ * drawn, and no result depends on the order of the sums.
+ * A setting comes from its device array (an entry per row where its flag is
+ * set, else one for all), read when the kernels run, or from the host's value.
+ * workspace: da_sample_workspace_bytes(B, V, dtype) bytes, which may be 0.
+ */
+typedef struct {
+  const void* logits;
+  const float* u;
+  const float* temperature_dev;
+  const int32_t* top_k_dev;
+  const float *top_p_dev, *min_p_dev;
+  int64_t* tokens;
+  float* logprobs;
+  void* workspace;
+  int64_t workspace_bytes, row_stride;
+  int32_t B, V, dtype, temperature_per_row, top_k_per_row, top_p_per_row, min_p_per_row, top_k;
+  float temperature, top_p, min_p;
+} da_sample_args;
+size_t da_sample_workspace_bytes(int B, int V, int dtype);
+int da_sample(const da_sample_args* args, void* stream);
 
 /*
  * Kernel (3): delta broadcast-add over rows 0 .. s_p-1.
