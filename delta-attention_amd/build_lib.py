@@ -25,7 +25,8 @@ CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 OUT = os.path.join(HERE, "delta_attention", "libdelta_attn.so")
 SOURCES = ["attn_kernels.hip", "attn_bwd.hip", "delta_add.hip", "rope.hip", "norm.hip",
-           "anchor_cos.hip", "adapt_loop.hip", "kv8.hip", "sample.hip"]
+           "anchor_cos.hip", "adapt_loop.hip", "kv8.hip", "sample.hip",
+           "prefix_attn.hip"]
 ARCH = "gfx950"
 EXT_SOURCE = "kv8_bind.cpp"
 EXT_OUT = os.path.join(HERE, "delta_attention", "_kv8_ext.so")

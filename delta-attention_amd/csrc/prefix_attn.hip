@@ -1,0 +1,520 @@
+// Attention rows of a batch whose sequences share prefixes (gfx950 / CDNA4):
+// sequence b of B reads the keys of prefix b / (B / P) and keys of its own.
+//
+//   o = softmax(scale q [Kp; K]^T) [Vp; V]
+//
+// A softmax over two key sets is the join of the softmaxes over each: with the
+// rows' references m, sums l = sum 2^(x - m) and products a = sum 2^(x - m) v of
+// each set, o = sum a 2^(m - M) / sum l 2^(m - M). So the prefix is one matrix
+// product over the rows of all sequences that share it (n s G rows for n
+// sequences of s rows and G query heads a kv head), read once, and each
+// sequence's own keys are another over its s G rows.
+#include <float.h>
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include "capi_common.h"
+#include "delta_attn.h"
+#include "device_common.h"
+
+namespace da {
+namespace {
+
+constexpr int BN = 64;                       // keys per tile
+constexpr int WAVES = 4;
+constexpr int MAX_KEYS = 1 << 30;
+constexpr float NO_KEYS = -FLT_MAX;          // the reference of a row that has seen no score yet
+// A row's reference may lag its largest score by LAG (log2); fp16 probabilities
+// are held times 2^BIAS, so that they are at most 2^14 and end 2^-32 below it.
+constexpr float LAG = 6.f;
+template <typename T> constexpr float BIAS = std::is_same_v<T, _Float16> ? 8.f : 0.f;
+
+struct PrefixArgs {
+  const void *q, *kp, *vp, *k, *v;
+  void* o;
+  int64_t q_b, q_h, q_s, o_b, o_h, o_s;
+  int64_t kp_b, kp_h, vp_b, vp_h, k_b, k_h, v_b, v_h;
+  uint32_t kp_s, vp_s, k_s, v_s;            // bytes from key to key
+  const int *np_dev, *n_dev;                // key counts on the device, or NULL: np, n
+  int np_step, n_step, np, n, Np, cap;      // (counts are clamped to Np and cap)
+  int B, P, per, Hkv, G, s;                 // per = B / P sequences a prefix
+  int rows;                                 // B * s * G: rows of a kv head
+  int p_rows, p_rt, o_rows, o_rt;           // rows of a prefix's sequences and of a sequence, their row tiles
+  int p_splits, o_splits, p_chunk, o_chunk; // splits of the keys, tiles of each
+  int p_items;                              // items of the prefixes, before the sequences' own
+  FastDiv heads, rows_s, f_prt, f_psp, f_ort, f_osp, f_hkv;   // G, s, p_rt, p_splits, o_rt, o_splits, Hkv
+  float scale2;                             // |sm_scale| log2(e), above zero
+  uint32_t flip;                            // the sign bits of Q where sm_scale is negative
+  float *part, *part_m, *part_l;            // [Hkv, splits, rows, D], [Hkv, splits, rows] twice
+};
+
+template <typename T> struct Mma;
+template <> struct Mma<__bf16> {
+  static constexpr uint32_t inf = 0x7f80, one = 0x3f80;
+  static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <> struct Mma<_Float16> {
+  static constexpr uint32_t inf = 0x7c00, one = 0x3c00;
+  static __device__ __forceinline__ f32x4 dot(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+
+// A K or V tile in LDS: rows of D elements, their 16-byte chunks permuted by the
+// row (chunk ^ swz(row)), so that the 16 rows that a fragment read takes the same
+// chunk of lie in different banks.
+template <int D> struct Tile {
+  static constexpr int RB = 2 * D, CH = D / 8, BYTES = BN * RB;
+  static constexpr int DMAS = BYTES / (1024 * WAVES);     // 1024-byte loads of a wave
+  static __device__ __forceinline__ int swz(int row) { return (RB >= 256 ? row : row / (256 / RB)) & (CH < 16 ? CH - 1 : 15); }
+};
+
+__device__ __forceinline__ float group_max(float x) {      // over the four lanes of a row
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float group_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return sum32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// Two elements' marks: the element one where f(element without sign, sign) holds.
+template <typename T, typename F>
+__device__ __forceinline__ uint32_t marks(uint32_t w, F&& f) {
+  constexpr uint32_t one = Mma<T>::one;
+  return (f(w & 0x7fffu, w >> 15 & 1) ? one : 0u) | (f(w >> 16 & 0x7fffu, w >> 31) ? one << 16 : 0u);
+}
+
+__device__ __forceinline__ int prefix_keys(const PrefixArgs& a, int p) {
+  return min(max(a.np_dev ? a.np_dev[(int64_t)p * a.np_step] : a.np, 0), a.Np);
+}
+__device__ __forceinline__ int own_keys(const PrefixArgs& a, int b) {
+  return min(max(a.n_dev ? a.n_dev[(int64_t)b * a.n_step] : a.n, 0), a.cap);
+}
+
+// One item: a row tile of 16 MT rows a wave against a split's key tiles, which
+// all waves load into LDS together, the next one while this one is computed.
+// S^T = K Q^T leaves a lane (row c = lane % 16, group g = lane / 16) the keys 16 t
+// + 4 g + r of its row, which is the right operand of O^T = V^T P^T as it stands;
+// V^T comes from transposed LDS reads of the same keys.
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefix_rows_kernel(PrefixArgs a) {
+  using E = Elt<T>;
+  using M = Mma<T>;
+  using TL = Tile<D>;
+  constexpr int KS = D / 32, DT = D / 16, BM = 16 * MT * WAVES;
+  __shared__ __align__(1024) char smem[2][2][TL::BYTES];
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int c = lane % 16, g = lane / 16;
+
+  // the item: (prefix or sequence, kv head, split, row tile), the row tiles of a
+  // split beside each other
+  int item = blockIdx.x;
+  const bool own = item >= a.p_items;
+  int hk, split, tile, row0, n_rows, n_keys, key0, chunk;   // row0: of the kv head's rows
+  const char *kb, *vb;
+  uint32_t k_s, v_s;
+  int lim0;                                  // the first row's last key, less what its place adds
+  if (!own) {
+    int x = fdiv(item, a.f_prt);
+    tile = item - x * a.p_rt;
+    int y = fdiv(x, a.f_psp);
+    split = x - y * a.p_splits;
+    const int p = fdiv(y, a.f_hkv);
+    hk = y - p * a.Hkv;
+    n_rows = min(BM, a.p_rows - tile * BM);
+    row0 = p * a.p_rows + tile * BM;
+    n_keys = prefix_keys(a, p);
+    chunk = a.p_chunk;
+    kb = (const char*)a.kp + 2 * (p * a.kp_b + hk * a.kp_h);
+    vb = (const char*)a.vp + 2 * (p * a.vp_b + hk * a.vp_h);
+    k_s = a.kp_s, v_s = a.vp_s;
+    lim0 = n_keys - 1;
+  } else {
+    item -= a.p_items;
+    int x = fdiv(item, a.f_ort);
+    tile = item - x * a.o_rt;
+    int y = fdiv(x, a.f_osp);
+    split = x - y * a.o_splits;
+    const int b = fdiv(y, a.f_hkv);
+    hk = y - b * a.Hkv;
+    n_rows = min(BM, a.o_rows - tile * BM);
+    row0 = b * a.o_rows + tile * BM;
+    n_keys = own_keys(a, b);
+    chunk = a.o_chunk;
+    kb = (const char*)a.k + 2 * (b * a.k_b + hk * a.k_h);
+    vb = (const char*)a.v + 2 * (b * a.v_b + hk * a.v_h);
+    k_s = a.k_s, v_s = a.v_s;
+    lim0 = n_keys - a.s;
+    split += a.p_splits;
+  }
+  n_keys = __builtin_amdgcn_readfirstlane(n_keys);
+  lim0 = __builtin_amdgcn_readfirstlane(lim0);
+  key0 = (own ? split - a.p_splits : split) * chunk * BN;
+
+  // this wave's rows: places in the kv head's rows, and each one's last key
+  const int splits = a.p_splits + a.o_splits;
+  const int64_t slot = ((int64_t)hk * splits + split) * a.rows;
+  const bool active = wave * 16 * MT < n_rows;
+  int lim[MT], lim_lo = lim0, lim_hi = lim0;
+  u32x4 qf[MT][KS];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = row0 + min(wave * 16 * MT + mt * 16 + c, n_rows - 1);   // (past the last: it again)
+    const int x = fdiv(r, a.heads), b = fdiv(x, a.rows_s), i = x - b * a.s;
+    lim[mt] = own ? lim0 + i : lim0;
+    const T* src = (const T*)a.q + b * a.q_b + (int64_t)(hk * a.G + r - x * a.G) * a.q_h + i * a.q_s;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) qf[mt][k] = *(const u32x4*)(src + 32 * k + 8 * g) ^ a.flip;
+  }
+  if (own) {                                 // of the whole row tile
+    const int x0 = fdiv(row0, a.heads), x1 = fdiv(row0 + n_rows - 1, a.heads);
+    lim_lo += x0 - (int)fdiv(x0, a.rows_s) * a.s;
+    lim_hi += x1 - (int)fdiv(x1, a.rows_s) * a.s;
+  }
+  const int end = min(min(key0 + chunk * BN, n_keys), lim_hi + 1);
+  const int nt = end > key0 ? (end - key0 + BN - 1) / BN : 0;
+
+  f32x4 acc[MT][DT];
+  float ref[MT], sum[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    ref[mt] = NO_KEYS;
+    sum[mt] = 0.f;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[mt][t] = (f32x4){0, 0, 0, 0};
+  }
+
+  // loads: lane i of load j of a wave fills chunk i of the wave's 1024 bytes
+  uint32_t koff[TL::DMAS], voff[TL::DMAS];
+#pragma unroll
+  for (int j = 0; j < TL::DMAS; ++j) {
+    const int at = (j * WAVES + wave) * 64 + lane, row = at / TL::CH, ch = (at % TL::CH) ^ TL::swz(row);
+    koff[j] = row * k_s + ch * 16;
+    voff[j] = row * v_s + ch * 16;
+  }
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(DA_LDS char*)&smem[0][0][0];
+  auto issue = [&](int t) __attribute__((always_inline)) {
+    const int first = key0 + t * BN;
+    const int64_t left = n_keys - first;     // keys from here on: the others read as zero
+    const int64_t kr = (left - 1) * k_s + TL::RB, vr = (left - 1) * v_s + TL::RB;
+    const u32x4 rk = rsrc_words(kb + (int64_t)first * k_s, kr >> 32 ? 0xffffffffu : (uint32_t)kr);
+    const u32x4 rv = rsrc_words(vb + (int64_t)first * v_s, vr >> 32 ? 0xffffffffu : (uint32_t)vr);
+    const uint32_t st = lds0 + t % 2 * 2 * TL::BYTES + wave * 1024;
+#pragma unroll
+    for (int j = 0; j < TL::DMAS; ++j) dma16_untracked(rk, st + j * WAVES * 1024, koff[j]);
+#pragma unroll
+    for (int j = 0; j < TL::DMAS; ++j) dma16_untracked(rv, st + TL::BYTES + j * WAVES * 1024, voff[j]);
+  };
+  int kread[KS], vread[DT];
+#pragma unroll
+  for (int k = 0; k < KS; ++k) kread[k] = c * TL::RB + ((4 * k + g) ^ TL::swz(c)) * 16;
+#pragma unroll
+  for (int t = 0; t < DT; ++t) {
+    const int row = 4 * g + c / 4;
+    vread[t] = row * TL::RB + ((2 * t + c % 4 / 2) ^ TL::swz(row)) * 16 + c % 2 * 8;
+  }
+
+  if (nt > 0) issue(0);
+  for (int t = 0; t < nt; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();                           // the tile is there, and the one before is read
+    if (t + 1 < nt) issue(t + 1);
+    if (!active) continue;
+    const DA_LDS char* ks = (const DA_LDS char*)&smem[t % 2][0][0];
+    const DA_LDS char* vs = (const DA_LDS char*)&smem[t % 2][1][0];
+    const int first = key0 + t * BN;
+    const bool whole = first + BN - 1 <= lim_lo;
+    f32x4 s[MT][4];
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 ka = *(const DA_LDS u32x4*)(ks + kread[k] + 16 * i * TL::RB);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) s[mt][i] = M::dot(ka, qf[mt][k], k == 0 ? (f32x4){0, 0, 0, 0} : s[mt][i]);
+      }
+    u32x4 pf[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      if (!whole) {
+        const int hi = lim[mt] - first - 4 * g;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[mt][e / 4][e % 4] = e / 4 * 16 + e % 4 <= hi ? s[mt][e / 4][e % 4] : -INFINITY;
+      }
+      float top = s[mt][0][0];
+#pragma unroll
+      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[mt][e / 4][e % 4]);
+      top = group_max(top);
+      if (__any((top - ref[mt]) * a.scale2 > LAG)) {
+        const float to = fmaxf(ref[mt], top);
+        const float alpha = fast_exp2((ref[mt] - to) * a.scale2);
+        ref[mt] = to;
+        sum[mt] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[mt][d][r] *= alpha;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int i = 2 * u + w / 2, r = w % 2 * 2;
+          auto weight = [&](float y) __attribute__((always_inline)) { return fast_exp2(fmaf(y - ref[mt], a.scale2, BIAS<T>)); };
+          pf[mt][u][w] = E::pack2(weight(s[mt][i][r]), weight(s[mt][i][r + 1]));
+          sum[mt] = E::add_pair(pf[mt][u][w], sum[mt]);   // (the rounded ones: as the product has them)
+        }
+    }
+    auto values = [&](int u, int d) __attribute__((always_inline)) -> u32x4 {
+      const u32x2 v0 = read_tr16(vs + vread[d] + 32 * u * TL::RB), v1 = read_tr16(vs + vread[d] + (32 * u + 16) * TL::RB);
+      return (u32x4){v0[0], v0[1], v1[0], v1[1]};
+    };
+    // An infinity or NaN among the values of a key that one of the rows does not see
+    // must not reach it through 0 * inf (keys past the last one are loaded as zero).
+    bool odd = false;
+    if (!whole && lim_lo < lim_hi) {
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const u32x4 va = values(u, d);
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            odd |= (va[w] & M::inf) == M::inf || (va[w] >> 16 & M::inf) == M::inf;
+        }
+      odd = __any(odd);
+    }
+    if (odd) {
+      // taken as zero, and given to the rows that see them from products of the
+      // values' and the rows' marks
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        u32x4 sees[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int at = first + 32 * u + w / 2 * 16 + 4 * g + w % 2 * 2;
+            sees[mt][w] = (at <= lim[mt] ? M::one : 0u) | (at + 1 <= lim[mt] ? M::one << 16 : 0u);
+          }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          u32x4 va = values(u, d), up, down, none;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            up[w] = marks<T>(va[w], [](uint32_t x, uint32_t neg) { return x == M::inf && !neg; });
+            down[w] = marks<T>(va[w], [](uint32_t x, uint32_t neg) { return x == M::inf && neg; });
+            none[w] = marks<T>(va[w], [](uint32_t x, uint32_t) { return x > M::inf; });
+            va[w] &= ((va[w] & M::inf) == M::inf ? 0u : 0xffffu) | ((va[w] >> 16 & M::inf) == M::inf ? 0u : 0xffff0000u);
+          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const f32x4 zero = {0, 0, 0, 0};
+            const f32x4 a = M::dot(up, sees[mt], zero), b = M::dot(down, sees[mt], zero), c = M::dot(none, sees[mt], zero);
+            acc[mt][d] = M::dot(va, pf[mt][u], acc[mt][d]);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              if (a[r] > 0.f) acc[mt][d][r] += INFINITY;
+              if (b[r] > 0.f) acc[mt][d][r] -= INFINITY;
+              if (c[r] > 0.f) acc[mt][d][r] = __builtin_nanf("");
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          const u32x4 va = values(u, d);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) acc[mt][d] = M::dot(va, pf[mt][u], acc[mt][d]);
+        }
+    }
+  }
+  if (!active) return;
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int r = wave * 16 * MT + mt * 16 + c;
+    const float l = group_sum(sum[mt]);
+    if (r >= n_rows) continue;
+    const int64_t at = slot + row0 + r;
+    if (g == 0) {
+      a.part_m[at] = ref[mt];
+      a.part_l[at] = l;
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) *(f32x4*)(a.part + at * D + 16 * d + 4 * g) = acc[mt][d];
+  }
+}
+
+// Joins a row's splits: D / 4 threads a row.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
+  using E = Elt<T>;
+  constexpr int CT = D / 4, PER = 256 / CT;
+  const int64_t x = (int64_t)blockIdx.x * PER + threadIdx.x / CT;
+  if (x >= (int64_t)a.rows * a.Hkv) return;
+  const int hk = (int)(x / a.rows), row = (int)(x - (int64_t)hk * a.rows), t = threadIdx.x % CT;
+  const int y = fdiv(row, a.heads), b = fdiv(y, a.rows_s), i = y - b * a.s;
+  const int splits = a.p_splits + a.o_splits;
+  const int64_t at = (int64_t)hk * splits * a.rows + row;
+  float m = NO_KEYS, l = 0.f;
+  f32x4 o = {0, 0, 0, 0};
+  for (int j = 0; j < splits; ++j) {
+    const float mj = a.part_m[at + (int64_t)j * a.rows], lj = a.part_l[at + (int64_t)j * a.rows];
+    if (lj == 0.f) continue;
+    const f32x4 z = *(const f32x4*)(a.part + (at + (int64_t)j * a.rows) * D + 4 * t);
+    const float to = fmaxf(m, mj), k0 = fast_exp2((m - to) * a.scale2), k1 = fast_exp2((mj - to) * a.scale2);
+    m = to;
+    l = l * k0 + lj * k1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = o[e] * k0 + z[e] * k1;
+  }
+  // a row without keys is zero; one whose every score is -inf has no softmax: NaN
+  const bool none = prefix_keys(a, b / a.per) == 0 && own_keys(a, b) - a.s + i < 0;
+  const float inv = none ? 0.f : 1.f / l;
+  T* dst = (T*)a.o + b * a.o_b + (int64_t)(hk * a.G + row - y * a.G) * a.o_h + i * a.o_s;
+  *(u32x2*)(dst + 4 * t) = (u32x2){E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
+}
+
+// ---------------------------------------------------------------------------
+// host side
+
+struct Plan {
+  int mt, p_rt, o_rt, p_splits, o_splits, p_chunk, o_chunk;
+  int64_t p_items, items, rows;
+  size_t bytes;
+};
+
+bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, int64_t cap) {
+  constexpr int64_t MOST = 1 << 22;          // items and row tiles of a launch
+  p = Plan{};
+  const int64_t own = (int64_t)s * G;
+  if (own > MOST || (int64_t)B * Hkv > MOST || own * B > MOST) return false;
+  p.rows = own * B;
+  const int64_t p_rows = p.rows / P;
+  p.mt = p_rows <= 64 ? 1 : 2;
+  const int bm = 16 * p.mt * WAVES;
+  const int64_t p_rt = Np > 0 ? (p_rows + bm - 1) / bm : 0, o_rt = cap > 0 ? (own + bm - 1) / bm : 0;
+  const int64_t p_tiles = (Np + BN - 1) / BN, o_tiles = (cap + BN - 1) / BN;
+  const int64_t p_lists = P * Hkv * p_rt, o_lists = (int64_t)B * Hkv * o_rt;
+  if (p_lists > MOST || o_lists > MOST) return false;
+  const int64_t slots = 256 * (D <= 128 ? 2 : 1);
+  int64_t chunk = (p_lists * p_tiles + o_lists * o_tiles + slots - 1) / slots;
+  if (chunk < 4) chunk = 4;
+  p.p_rt = (int)(p_rt > 0 ? p_rt : 1);
+  p.o_rt = (int)(o_rt > 0 ? o_rt : 1);
+  p.p_splits = p_rt > 0 ? (int)((p_tiles + chunk - 1) / chunk) : 0;
+  p.o_splits = o_rt > 0 ? (int)((o_tiles + chunk - 1) / chunk) : 0;
+  p.p_chunk = p.p_splits > 0 ? (int)((p_tiles + p.p_splits - 1) / p.p_splits) : 1;
+  p.o_chunk = p.o_splits > 0 ? (int)((o_tiles + p.o_splits - 1) / p.o_splits) : 1;
+  p.p_items = p_lists * p.p_splits;
+  p.items = p.p_items + o_lists * p.o_splits;
+  if (p.items > MOST || p.rows * Hkv > MOST * 4) return false;
+  p.bytes = (size_t)(p.rows * Hkv * (p.p_splits + p.o_splits)) * (D + 2) * sizeof(float);
+  return true;
+}
+
+template <typename T, int D>
+void launch(const PrefixArgs& a, const Plan& p, hipStream_t st) {
+  const dim3 block(64 * WAVES);
+  if (p.items > 0) {
+    if (p.mt == 1) hipLaunchKernelGGL((prefix_rows_kernel<T, D, 1>), dim3((unsigned)p.items), block, 0, st, a);
+    else hipLaunchKernelGGL((prefix_rows_kernel<T, D, 2>), dim3((unsigned)p.items), block, 0, st, a);
+  }
+  constexpr int PER = 256 / (D / 4);
+  hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((unsigned)((p.rows * a.Hkv + PER - 1) / PER)), dim3(256), 0, st, a);
+}
+
+template <typename T>
+void by_dim(int D, const PrefixArgs& a, const Plan& p, hipStream_t st) {
+  if (D == 32) launch<T, 32>(a, p, st);
+  else if (D == 64) launch<T, 64>(a, p, st);
+  else if (D == 128) launch<T, 128>(a, p, st);
+  else launch<T, 256>(a, p, st);
+}
+
+// Bytes from key to key, at most 2^25 (a tile's offsets stay inside 32 bits).
+bool key_stride(uint32_t& to, int64_t elements, int keys) {
+  if (keys > 1 && (elements < 0 || elements > 1 << 24)) return false;
+  to = keys > 1 ? (uint32_t)(2 * elements) : 0;
+  return true;
+}
+
+}  // namespace
+}  // namespace da
+
+using namespace da;
+
+extern "C" size_t da_prefix_attn_workspace_bytes(int B, int P, int Hq, int Hkv, int s, int D, int max_prefix,
+                                                 int max_keys) {
+  if (B < 1 || P < 1 || B % P != 0 || Hq < 1 || Hkv < 1 || Hq % Hkv != 0 || s < 1 || !head_dim_ok(D) ||
+      max_prefix < 0 || max_prefix > MAX_KEYS || max_keys < 0 || max_keys > MAX_KEYS)
+    return 0;
+  Plan p;
+  return plan_for(p, B, P, Hkv, Hq / Hkv, s, D, max_prefix, max_keys) ? p.bytes : 0;
+}
+
+extern "C" int da_prefix_attn_fwd(const da_prefix_attn_args* x, void* stream) {
+  if (!x) return DA_ERR_INVALID_ARG;
+  if (x->dtype != DA_BF16 && x->dtype != DA_FP16) return DA_ERR_DTYPE;
+  if (!head_dim_ok(x->D)) return DA_ERR_HEAD_DIM;
+  const int B = x->B, P = x->P, Hkv = x->Hkv, Hq = x->Hq, s = x->s, Np = x->max_prefix, cap = x->max_keys;
+  if (B < 0 || P < 1 || B % P != 0 || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || s < 0 || Np < 0 || Np > MAX_KEYS ||
+      cap < 0 || cap > MAX_KEYS)
+    return DA_ERR_INVALID_ARG;
+  if ((!x->n_prefix_dev && (x->n_prefix < 0 || x->n_prefix > Np)) || (!x->n_keys_dev && (x->n_keys < 0 || x->n_keys > cap)))
+    return DA_ERR_INVALID_ARG;
+  if (!(fabsf(x->sm_scale) <= FLT_MAX)) return DA_ERR_INVALID_ARG;
+  if (B == 0 || s == 0) return DA_OK;
+  if (!x->q || !x->out || (Np > 0 && (!x->k_prefix || !x->v_prefix)) || (cap > 0 && (!x->k || !x->v)))
+    return DA_ERR_INVALID_ARG;
+  if ((B > 1 && !x->o_str[0]) || (Hq > 1 && !x->o_str[1]) || (s > 1 && !x->o_str[2])) return DA_ERR_INVALID_ARG;
+  if (!aligned16(x->q) || !aligned16(x->out) || !aligned16(x->k_prefix) || !aligned16(x->v_prefix) || !aligned16(x->k) ||
+      !aligned16(x->v) || !strides8(x->q_str) || !strides8(x->o_str) || !strides8(x->kp_str) || !strides8(x->vp_str) ||
+      !strides8(x->k_str) || !strides8(x->v_str) || ((uintptr_t)x->n_prefix_dev & 3) || ((uintptr_t)x->n_keys_dev & 3))
+    return DA_ERR_ALIGNMENT;
+  PrefixArgs a{};
+  if (!key_stride(a.kp_s, x->kp_str[2], Np) || !key_stride(a.vp_s, x->vp_str[2], Np) ||
+      !key_stride(a.k_s, x->k_str[2], cap) || !key_stride(a.v_s, x->v_str[2], cap))
+    return DA_ERR_INVALID_ARG;
+  const int G = Hq / Hkv;
+  Plan p;
+  if (!plan_for(p, B, P, Hkv, G, s, x->D, Np, cap)) return DA_ERR_INVALID_ARG;
+  if (p.bytes > 0 && (!x->workspace || x->workspace_bytes < (int64_t)p.bytes)) return DA_ERR_WORKSPACE;
+  if (!aligned16(x->workspace)) return DA_ERR_ALIGNMENT;
+  a.q = x->q, a.kp = x->k_prefix, a.vp = x->v_prefix, a.k = x->k, a.v = x->v, a.o = x->out;
+  a.q_b = x->q_str[0], a.q_h = x->q_str[1], a.q_s = x->q_str[2];
+  a.o_b = x->o_str[0], a.o_h = x->o_str[1], a.o_s = x->o_str[2];
+  a.kp_b = x->kp_str[0], a.kp_h = x->kp_str[1], a.vp_b = x->vp_str[0], a.vp_h = x->vp_str[1];
+  a.k_b = x->k_str[0], a.k_h = x->k_str[1], a.v_b = x->v_str[0], a.v_h = x->v_str[1];
+  a.np_dev = x->n_prefix_dev, a.n_dev = x->n_keys_dev;
+  a.np_step = x->n_prefix_per ? 1 : 0, a.n_step = x->n_keys_per_seq ? 1 : 0;
+  a.np = x->n_prefix, a.n = x->n_keys, a.Np = Np, a.cap = cap;
+  a.B = B, a.P = P, a.per = B / P, a.Hkv = Hkv, a.G = G, a.s = s;
+  a.rows = (int)p.rows;
+  a.p_rows = a.rows / P, a.o_rows = s * G;
+  a.p_rt = p.p_rt, a.o_rt = p.o_rt;
+  a.p_splits = p.p_splits, a.o_splits = p.o_splits, a.p_chunk = p.p_chunk, a.o_chunk = p.o_chunk;
+  a.p_items = (int)p.p_items;
+  a.heads = make_fastdiv(G), a.rows_s = make_fastdiv(s);
+  a.f_prt = make_fastdiv(p.p_rt), a.f_ort = make_fastdiv(p.o_rt);
+  a.f_psp = make_fastdiv(p.p_splits > 0 ? p.p_splits : 1), a.f_osp = make_fastdiv(p.o_splits > 0 ? p.o_splits : 1);
+  a.f_hkv = make_fastdiv(Hkv);
+  // (a scale of zero, which weighs every key alike, as the smallest one: a masked
+  // score's -inf stays -inf)
+  a.scale2 = fminf(fmaxf(fabsf(x->sm_scale) * 1.4426950408889634f, FLT_TRUE_MIN), FLT_MAX);
+  a.flip = x->sm_scale < 0.f ? 0x80008000u : 0;
+  a.part = (float*)x->workspace;
+  a.part_m = a.part + p.rows * Hkv * (p.p_splits + p.o_splits) * x->D;
+  a.part_l = a.part_m + p.rows * Hkv * (p.p_splits + p.o_splits);
+  (void)hipGetLastError();
+  if (x->dtype == DA_BF16) by_dim<__bf16>(x->D, a, p, (hipStream_t)stream);
+  else by_dim<_Float16>(x->D, a, p, (hipStream_t)stream);
+  return hipGetLastError() == hipSuccess ? DA_OK : DA_ERR_LAUNCH;
+}

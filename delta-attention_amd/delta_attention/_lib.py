@@ -75,6 +75,8 @@ EXPORTS = (
     "da_kv8_attn_fwd",
     "da_sample_workspace_bytes",
     "da_sample",
+    "da_prefix_attn_workspace_bytes",
+    "da_prefix_attn_fwd",
 )
 
 _ERR_TEXT = {
@@ -230,13 +232,15 @@ def _load() -> ctypes.CDLL:
                                      _i, _i, _i, _i, _i, _i, _d, _d, _d,
                                      _vp, _vp, _vp, _vp, _i, _vp, _sz, _i, _vp, _vp]
     # (these take one struct; the functions of kv8_ext and gen_ext pack it)
-    for f in (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd, L.da_sample):
+    for f in (L.da_kv8_write, L.da_kv8_read, L.da_kv8_attn_fwd, L.da_sample, L.da_prefix_attn_fwd):
         f.restype = _i
         f.argtypes = [ctypes.c_char_p, _vp]
     L.da_kv8_attn_workspace_bytes.restype = _sz
     L.da_kv8_attn_workspace_bytes.argtypes = [_i, _i, _i, _i, _i, _i, _i, _i]
     L.da_sample_workspace_bytes.restype = _sz
     L.da_sample_workspace_bytes.argtypes = [_i, _i, _i]
+    L.da_prefix_attn_workspace_bytes.restype = _sz
+    L.da_prefix_attn_workspace_bytes.argtypes = [_i, _i, _i, _i, _i, _i, _i, _i]
     L.da_build_target.restype = ctypes.c_char_p
     L.da_build_target.argtypes = []
     return L
@@ -295,7 +299,9 @@ def gen_ext():
     L = lib()
     with _lib_lock:
         if _gen_ext is None:
-            _gen_ext = _extension("_gen_ext", GEN_PATH, (L.da_sample, L.da_sample_workspace_bytes))
+            _gen_ext = _extension("_gen_ext", GEN_PATH, (L.da_sample, L.da_sample_workspace_bytes,
+                                                         L.da_prefix_attn_fwd,
+                                                         L.da_prefix_attn_workspace_bytes))
     return _gen_ext
 
 

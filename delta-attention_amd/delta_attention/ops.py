@@ -700,6 +700,25 @@ def sample_tokens(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top
     return L.gen_ext().sample(logits, u, temperature, top_k, top_p, min_p)
 
 
+def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k: torch.Tensor,
+                     v: torch.Tensor, *, n_prefix=None, n_keys=None, sm_scale: float,
+                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The last s rows of each sequence of a batch that shares prefixes
+    (da_prefix_attn_fwd): q [B, H, s, D]; k_prefix / v_prefix [P, Hkv, Np, D], of
+    which every B / P sequences in a row share one; k / v [B, Hkv, n, D], each
+    sequence's own keys (any strides, GQA native) -> [B, H, s, D]. Row i stands
+    at n - s + i of its own keys and sees those up to itself and the whole
+    prefix; a row that sees no key is zero. A prefix's keys are read once for
+    all its sequences.
+
+    n_prefix, n_keys: how many of the prefix's and of the own keys count (None:
+    all), numbers or int32 device tensors of one entry or one per prefix /
+    sequence, read when the kernels run (a recorded call serves every length;
+    counts are clamped to the capacities). A new result has q's strides where q
+    is dense."""
+    return L.gen_ext().prefix(q, k_prefix, v_prefix, k, v, n_prefix, n_keys, sm_scale, out)
+
+
 # ---------------------------------------------------------------------------
 # decoder-layer element-wise kernels (full-model prefill)
 

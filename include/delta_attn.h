@@ -364,6 +364,41 @@ size_t da_kv8_attn_workspace_bytes(int B, int Hq, int Hkv, int s, int D, int max
 int da_kv8_attn_fwd(const da_kv8_attn_args* args, void* stream);
 
 /*
+ * Attention rows of a batch whose sequences share prefixes: sequence b of B reads
+ * the keys of prefix b / (B / P) (P divides B) and keys of its own, as if the two
+ * stood behind each other. No counterpart in the reference, which gives every
+ * sequence a cache of its own.
+ * Row i of the s rows of a sequence sees every key of its prefix and its own keys
+ * j <= n - s + i (its own place among the n own keys):
+ *   out = softmax(sm_scale q [Kp; K]^T) [Vp; V]
+ * with fp32 scores and sums; probabilities are rounded to `dtype` before their
+ * product with the values, and enter the row's sum as rounded. A row that sees no
+ * key is zero; one whose every score is -inf is NaN. Keys and values of places
+ * that a row does not see reach it in no way, whatever they hold.
+ * q, out [B, Hq, s, D] (strides {batch, head, row}); k_prefix, v_prefix
+ * [P, Hkv, max_prefix, D], k, v [B, Hkv, max_keys, D] ({batch, head, key}; at most
+ * 2^24 elements from key to key). n_prefix_dev / n_keys_dev: int32 counts on the
+ * device (an entry per prefix or sequence where the flag is set, else one for
+ * all), read when the kernels run and clamped to the capacities; NULL: the host's
+ * counts. A zero stride of q, k_prefix .. v over batch or heads is an expanded
+ * tensor; of out it is DA_ERR_INVALID_ARG.
+ * workspace: da_prefix_attn_workspace_bytes(...) bytes.
+ */
+typedef struct {
+  const void *q, *k_prefix, *v_prefix, *k, *v;
+  void* out;
+  const int32_t *n_prefix_dev, *n_keys_dev;
+  void* workspace;
+  int64_t workspace_bytes;
+  int64_t q_str[3], kp_str[3], vp_str[3], k_str[3], v_str[3], o_str[3];
+  int32_t B, P, Hq, Hkv, s, D, max_prefix, max_keys, n_prefix, n_keys, n_prefix_per, n_keys_per_seq, dtype;
+  float sm_scale;
+} da_prefix_attn_args;
+size_t da_prefix_attn_workspace_bytes(int B, int P, int Hq, int Hkv, int s, int D, int max_prefix,
+                                      int max_keys);
+int da_prefix_attn_fwd(const da_prefix_attn_args* args, void* stream);
+
+/*
  * The next tokens of a batch: one token per row of logits [B, V] (row_stride
  * elements apart, DA_BF16, DA_FP16 or DA_FP32; V up to 2^24, B up to 2^22 - 1)
  * from a given number u[b] in [0, 1). No counterpart in the reference, whose
