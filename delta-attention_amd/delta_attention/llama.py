@@ -36,6 +36,19 @@ class CachedKeys8(NamedTuple):
     n_keys: Union[int, torch.Tensor]
 
 
+class SharedKeys(NamedTuple):
+    """What a cache whose sequences share their prompts hands to the attention in
+    the place of the key states (the value states are then None): one layer's
+    prompt keys and values [P, Hkv, s, D], each sequence's own [B, Hkv, n, D], and
+    how many of the own ones count (an int, or in recorded decode steps an int32
+    device tensor)."""
+    k_prefix: torch.Tensor
+    v_prefix: torch.Tensor
+    k: torch.Tensor
+    v: torch.Tensor
+    n_keys: Union[int, torch.Tensor]
+
+
 # Rows (tokens times query heads per kv head) up to which a pass over an 8-bit
 # cache reads its codes (ops.kv8_attention); more rows read the keys back into
 # 16 bits first and run the rows kernel. One bound for all shapes, taken at 32 /
@@ -427,14 +440,18 @@ class LlamaAttention(nn.Module):
                                **kwargs):
         """Queries at the end of the KV cache: row i of s attends keys
         0 .. n - s + i (llama.py:498-535) -> ([b, s, h, d], None). One-row
-        steps with decode_mode "sparse" / "delta" go to delta_decode_forward."""
+        steps with decode_mode "sparse" / "delta" go to delta_decode_forward.
+        Sequences that share their prompts (SharedKeys) read them once for all
+        (ops.prefix_attention)."""
         b, h, s, d = query_states.size()
         n_keys = kwargs.get("n_keys")
         if s == 1 and getattr(self.config, "decode_mode", "dense") != "dense":
             return self.delta_decode_forward(module, query_states, key_states, value_states,
                                              scaling=scaling, **kwargs)
         q, k, v = self._half(query_states, key_states, value_states)
-        if s == 1:
+        if isinstance(k, SharedKeys):
+            out = ops.prefix_attention(q, k.k_prefix, k.v_prefix, k.k, k.v, n_keys=k.n_keys, sm_scale=float(scaling))
+        elif s == 1:
             out = self._decode_row(q, k, v, scaling, n_keys=n_keys)
         elif isinstance(k, CachedKeys8) and s * self.num_key_value_groups <= DIRECT_ROWS8:
             out = ops.kv8_attention(q, k.cache, n_keys=k.n_keys, sm_scale=float(scaling))
@@ -452,6 +469,8 @@ class LlamaAttention(nn.Module):
         if q.dtype == torch.float32:
             if isinstance(k, CachedKeys8):
                 return q.to(torch.bfloat16), k, v
+            if isinstance(k, SharedKeys):
+                return q.to(torch.bfloat16), SharedKeys(*(t.to(torch.bfloat16) for t in k[:4]), k.n_keys), v
             return q.to(torch.bfloat16), k.to(torch.bfloat16), v.to(torch.bfloat16)
         return q, k, v
 
@@ -577,7 +596,7 @@ class LlamaAttention(nn.Module):
             qw, kw, eps = self._qk_norm()
             if append is not None:
                 ops.rope_qk_append(q, k, v, cos, sin, append.k[self.layer_idx],
-                                   append.v[self.layer_idx], append.pos, q_norm_w=qw,
+                                   append.v[self.layer_idx], append.row, q_norm_w=qw,
                                    k_norm_w=kw, eps=eps)
                 return q.transpose(1, 2), None, None
             ops.rope_qk(q, k, cos, sin, q_norm_w=qw, k_norm_w=kw, eps=eps)
@@ -591,10 +610,12 @@ class LlamaAttention(nn.Module):
         hidden_shape = (*input_shape, -1, self.head_dim)
         cos, sin = position_embeddings
         timer = kwargs.get("timer")
-        if (self.config._attn_implementation == "window" and getattr(past_key_value, "eight_bit", False)
-                and past_key_value.len[self.layer_idx] > 0):
-            raise NotImplementedError("the delta prefill takes a whole prompt, and the 8-bit cache already "
-                                      "holds tokens (continue with 'sdpa_rectangle')")
+        if self.config._attn_implementation == "window" and past_key_value is not None:
+            kind = ("8-bit" if getattr(past_key_value, "eight_bit", False) else
+                    "shared" if getattr(past_key_value, "shared", False) else None)
+            if kind is not None and past_key_value.len[self.layer_idx] > 0:
+                raise NotImplementedError(f"the delta prefill takes a whole prompt, and the {kind} cache already "
+                                          "holds tokens (continue with 'sdpa_rectangle')")
         static = (past_key_value is not None and getattr(past_key_value, "static", False)
                   and not getattr(past_key_value, "eight_bit", False)
                   and hidden_states.dtype in (torch.bfloat16, torch.float16))

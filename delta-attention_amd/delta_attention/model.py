@@ -22,8 +22,8 @@ import torch
 from torch import nn
 
 from . import ops
-from .llama import (CachedKeys8, LlamaAttention, LlamaRMSNorm, fuse_linears, fused_params,
-                    rope_cos_sin)
+from .llama import (CachedKeys8, LlamaAttention, LlamaRMSNorm, SharedKeys, fuse_linears,
+                    fused_params, rope_cos_sin)
 from .timing import Timer, region as _region
 
 
@@ -79,6 +79,8 @@ class KVCache:
     # whether keys and values are codes (the attention then gets CachedKeys8, and
     # static appends run in a launch of their own, not in RoPE's)
     eight_bit = False
+    # whether its sequences share their prompts (the attention then gets SharedKeys)
+    shared = False
 
     def __init__(self, config, batch: int, max_len: int, device, dtype):
         self._allocate(config, batch, max_len, device, dtype)
@@ -90,6 +92,16 @@ class KVCache:
         self.pos = None        # int64 [1]: row of the next append
         self.n_keys = None     # int32 [1]: keys after that append
         self.anchor = False    # delta decode: whether the recorded step is an anchor step
+
+    @property
+    def row(self):
+        """Static mode: the buffers' row of the next append (int64 [1])."""
+        return self.pos
+
+    def for_samples(self, config, samples: int, max_new: int) -> "KVCache":
+        """The cache of `samples` sequences behind each of this one's, which all
+        layers hold alike, for max_new further tokens each."""
+        return KVCacheShared(self, config, samples, max_new)
 
     def _allocate(self, config, batch, max_len, device, dtype):
         shape = (batch, max_len, config.num_key_value_heads, config.head_dim)
@@ -157,6 +169,21 @@ class KVCache8(KVCache):
         self.k = [c.k for c in self.layers]
         self.v = [c.v for c in self.layers]
 
+    def for_samples(self, config, samples: int, max_new: int) -> "KVCache":
+        """(the codes are copied for every sample: a sequence's own tokens go into
+        the blocks behind its prompt's)"""
+        l0 = self.len[0]
+        out = KVCache8(config, self.layers[0].k.shape[0] * samples, l0 + max_new, self.k[0].device, None)
+        nb = -(-l0 // ops.KV8_BLOCK)
+        for to, c in zip(out.layers, self.layers):
+            to.k[:, :, :nb * ops.KV8_BLOCK].view(torch.uint8).copy_(
+                c.k[:, :, :nb * ops.KV8_BLOCK].view(torch.uint8).repeat_interleave(samples, 0))
+            to.v[:, :, :nb].view(torch.uint8).copy_(c.v[:, :, :nb].view(torch.uint8).repeat_interleave(samples, 0))
+            to.k_scale[:, :, :nb] = c.k_scale[:, :, :nb].repeat_interleave(samples, 0)
+            to.v_scale[:, :, :nb] = c.v_scale[:, :, :nb].repeat_interleave(samples, 0)
+        out.len = list(self.len)
+        return out
+
     def views(self, layer_idx: int):
         assert self.static
         return CachedKeys8(self.layers[layer_idx], self.n_keys), None
@@ -176,6 +203,65 @@ class KVCache8(KVCache):
         ops.kv8_write(c, k.transpose(1, 2), v.transpose(1, 2), l0)
         self.len[layer_idx] = l0 + s
         return (key_states, value_states) if l0 == 0 else (CachedKeys8(c, l0 + s), None)
+
+
+class KVCacheShared(KVCache):
+    """The cache of several samples of each prompt: the prompts' keys and values,
+    held once ([P, s, Hkv, D] a layer, the prefill's own buffers), and each
+    sample's own tokens ([P * samples, max_new, Hkv, D]). Decode steps read a
+    prompt once for all its samples (SharedKeys)."""
+
+    shared = True
+
+    def __init__(self, prompts: KVCache, config, samples: int, max_new: int):
+        n = prompts.len[0]
+        assert samples >= 1 and max_new >= 0 and all(l == n for l in prompts.len), (samples, max_new, prompts.len)
+        self.k_prefix = [k[:, :n].transpose(1, 2) for k in prompts.k]
+        self.v_prefix = [v[:, :n].transpose(1, 2) for v in prompts.v]
+        super().__init__(config, prompts.k[0].shape[0] * samples, max_new, prompts.k[0].device, prompts.k[0].dtype)
+        self.len = [n] * len(self.k)       # with the prompt, as the positions count
+        self.n_prefix, self.max_len = n, n + max_new
+        self._row = None
+
+    @property
+    def row(self):
+        return self._row
+
+    def start_static(self):
+        super().start_static()
+        self._row = self.pos - self.n_prefix
+        self.n_keys.sub_(self.n_prefix)    # the own keys after the append
+
+    def advance_static(self):
+        super().advance_static()
+        self._row.add_(1)
+
+    def stop_static(self, n_appended: int):
+        super().stop_static(n_appended)
+        self._row = None
+
+    def _keys(self, layer_idx: int, n_keys) -> SharedKeys:
+        return SharedKeys(self.k_prefix[layer_idx], self.v_prefix[layer_idx], self.k[layer_idx].transpose(1, 2),
+                          self.v[layer_idx].transpose(1, 2), n_keys)
+
+    def views(self, layer_idx: int):
+        assert self.static
+        return self._keys(layer_idx, self.n_keys), None
+
+    def update(self, key_states, value_states, layer_idx: int, cache_kwargs=None):
+        s = key_states.shape[2]
+        k, v = self.k[layer_idx], self.v[layer_idx]
+        if self.static:
+            assert s == 1, "static mode appends one token per step"
+            k.index_copy_(1, self._row, key_states.transpose(1, 2))
+            v.index_copy_(1, self._row, value_states.transpose(1, 2))
+            return self._keys(layer_idx, self.n_keys), None
+        l0 = self.len[layer_idx] - self.n_prefix
+        assert l0 + s <= k.shape[1], (l0, s, k.shape[1])
+        k[:, l0:l0 + s] = key_states.transpose(1, 2)
+        v[:, l0:l0 + s] = value_states.transpose(1, 2)
+        self.len[layer_idx] += s
+        return self._keys(layer_idx, l0 + s), None
 
 
 def new_cache(config, batch: int, max_len: int, device, dtype) -> KVCache:
@@ -342,15 +428,17 @@ class LlamaForCausalLM(nn.Module):
 
     def _decode_graphed(self, cache: KVCache, tok: torch.Tensor, max_new_tokens: int,
                         step_ms: Optional[list], logits_out: Optional[list],
-                        record: bool = True, eos: Optional[torch.Tensor] = None) -> torch.Tensor:
+                        record: bool = True, eos: Optional[torch.Tensor] = None,
+                        pick=None) -> torch.Tensor:
         """Decode steps 1 .. max_new_tokens-1 as HIP graph replays. The cache
         holds the token's row and key count on the device; each step kind
         (delta decode: anchor steps every min(gamma_dec, gamma_dec_max) steps,
         starting with the first; otherwise one kind) runs eagerly once, then is
         recorded and replayed. Outside the graph per step: the greedy argmax
-        (into the next step's input) and the token copy. record=False runs
-        every step eagerly in the same static form (the replays' reference).
-        eos: stop once every row has produced one of these ids."""
+        (into the next step's input), or pick(logits, step), and the token copy.
+        record=False runs every step eagerly in the same static form (the
+        replays' reference). eos: stop once every row has produced one of these
+        ids."""
         import time
         cfg = self.config
         mode = getattr(cfg, "decode_mode", "dense")
@@ -389,7 +477,10 @@ class LlamaForCausalLM(nn.Module):
                 if logits_out is not None:
                     logits_out.append(logits.float().clone())
                 ran = j + 1
-                torch.argmax(logits, dim=-1, keepdim=True, out=tok_buf)
+                if pick is None:
+                    torch.argmax(logits, dim=-1, keepdim=True, out=tok_buf)
+                else:
+                    tok_buf[:, 0] = pick(logits, j + 1)
                 toks[:, j + 1] = tok_buf[:, 0]
                 if step_ms is not None:
                     torch.cuda.synchronize()
@@ -419,6 +510,46 @@ class LlamaForCausalLM(nn.Module):
         eos_token_id (int or ids): stop once every row has produced one (the
         result then has fewer columns; rows that finished earlier keep
         generating, the caller masks them)."""
+        return self._generate(input_ids, max_new_tokens, timer, step_ms, graph, logits_out, record, eos_token_id)
+
+    @torch.inference_mode()
+    def generate_sampled(self, input_ids: torch.Tensor, max_new_tokens: int, u: torch.Tensor, *,
+                         temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, samples: int = 1,
+                         timer: Optional[Timer] = None, step_ms: Optional[list] = None,
+                         graph: bool = False, logits_out: Optional[list] = None,
+                         logprobs_out: Optional[list] = None, record: bool = True,
+                         eos_token_id=None) -> torch.Tensor:
+        """generate_greedy with tokens drawn by ops.sample_tokens: `samples`
+        sequences of each prompt -> [b * samples, n] token ids, a prompt's
+        samples behind each other. u: float32 [b * samples, max_new_tokens] in
+        [0, 1), the number that draws each token. The settings are
+        ops.sample_tokens' (numbers, or device tensors of one entry or one per
+        sequence). The prompts are prefilled once; with several samples their
+        keys stay where they are, and decode steps read them once for all
+        samples (KVCacheShared; the 8-bit cache's codes are copied instead).
+        logprobs_out: receives each step's log-probabilities [b * samples]."""
+        rows = input_ids.shape[0] * samples
+        assert samples >= 1, samples
+        assert u.dim() == 2 and u.shape[0] == rows and u.shape[1] >= max_new_tokens and u.dtype == torch.float32, (
+            f"u: float32 [{rows}, {max_new_tokens}] is needed, got {u.dtype} {tuple(u.shape)}")
+        if samples > 1 and getattr(self.config, "decode_mode", "dense") != "dense":
+            raise NotImplementedError("several samples of a prompt take dense decode steps "
+                                      f"(decode_mode {self.config.decode_mode!r} runs one sequence)")
+        draws = u.t().contiguous()
+
+        def pick(logits: torch.Tensor, step: int) -> torch.Tensor:
+            tok, logprob = ops.sample_tokens(logits, draws[step], temperature=temperature, top_k=top_k,
+                                             top_p=top_p, min_p=min_p)
+            if logprobs_out is not None:
+                logprobs_out.append(logprob)
+            return tok
+
+        return self._generate(input_ids, max_new_tokens, timer, step_ms, graph, logits_out, record, eos_token_id,
+                              pick, samples)
+
+    def _generate(self, input_ids, max_new_tokens, timer, step_ms, graph, logits_out, record, eos_token_id,
+                  pick=None, samples: int = 1) -> torch.Tensor:
+        """The loop of generate_greedy (pick None) and generate_sampled."""
         import time
         cfg = self.config
         eos = None
@@ -426,30 +557,34 @@ class LlamaForCausalLM(nn.Module):
             ids = [eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id)
             eos = torch.tensor(ids, dtype=torch.int64, device=input_ids.device)
         b, s = input_ids.shape
-        cache = new_cache(cfg, b, s + max_new_tokens, input_ids.device, self.lm_head.weight.dtype)
+        cache = new_cache(cfg, b, s + (max_new_tokens if samples == 1 else 0), input_ids.device,
+                          self.lm_head.weight.dtype)
         self.reset_decode_state()
         impl = cfg._attn_implementation
         out = []
         try:
             h = self.model(input_ids, timer, cache)
             logits = self.lm_head(h[:, -1])
+            if samples > 1:
+                cache = cache.for_samples(cfg, samples, max_new_tokens)
+                logits = logits.repeat_interleave(samples, 0)
             if logits_out is not None:
                 logits_out.append(logits.float().clone())
-            tok = logits.argmax(-1)
+            tok = logits.argmax(-1) if pick is None else pick(logits, 0)
             out.append(tok)
             done = _finished(tok, eos)
             cfg._attn_implementation = "sdpa_rectangle"
             if done is not None and bool(done.all()):
                 return torch.stack(out, dim=1)
             if graph and self.graph_decodable() and max_new_tokens > 1:
-                return self._decode_graphed(cache, tok, max_new_tokens, step_ms, logits_out, record, eos)
-            for _ in range(max_new_tokens - 1):
+                return self._decode_graphed(cache, tok, max_new_tokens, step_ms, logits_out, record, eos, pick)
+            for step in range(1, max_new_tokens):
                 t0 = time.perf_counter()
                 h = self.model(tok[:, None], timer, cache)
                 logits = self.lm_head(h[:, -1])
                 if logits_out is not None:
                     logits_out.append(logits.float().clone())
-                tok = logits.argmax(-1)
+                tok = logits.argmax(-1) if pick is None else pick(logits, step)
                 out.append(tok)
                 if step_ms is not None:
                     torch.cuda.synchronize()
@@ -465,46 +600,72 @@ class LlamaForCausalLM(nn.Module):
     @torch.inference_mode()
     def generate(self, input_ids: torch.Tensor, attention_mask: Optional[torch.Tensor] = None,
                  max_new_tokens: int = 128, do_sample: bool = False, eos_token_id=None,
-                 pad_token_id: Optional[int] = None, graph: bool = False, **unused) -> torch.Tensor:
+                 pad_token_id: Optional[int] = None, graph: bool = False,
+                 generator: Optional[torch.Generator] = None, num_return_sequences: int = 1,
+                 temperature: Optional[float] = None, top_k: Optional[int] = None,
+                 top_p: Optional[float] = None, min_p: Optional[float] = None, **unused) -> torch.Tensor:
         """The call model_wrapper.py:97 makes (HF `generate` with the greedy
         `_sample` loop of sample.py:25-262): -> [b, s + n] token ids, the
         prompt (with its padding) followed by the generated tokens; after a
         row's first eos token its remaining positions hold pad_token_id, and
         generation stops once every row has finished. Left-padded rows
         (attention_mask 0 on the padding) run one at a time over their real
-        tokens: the attention kernels take no padding mask. Only greedy
-        decoding is built (do_sample=True raises); `unused` takes the
-        generation kwargs greedy decoding ignores (temperature, top_k, ...)."""
-        if do_sample:
-            raise NotImplementedError("only greedy decoding (do_sample=False) is built")
+        tokens: the attention kernels take no padding mask. `unused` takes the
+        generation kwargs that are not built.
+
+        do_sample=True draws tokens (generate_sampled) by numbers of `generator`,
+        a torch.Generator on the model's device: without one it raises, nothing
+        is drawn from a hidden state. num_return_sequences of each prompt, behind
+        each other ([b * num_return_sequences, s + n]); temperature, top_k, top_p
+        and min_p default to 1, 50, 1 and 0, Hugging Face's defaults. Greedy
+        decoding ignores all of these."""
+        if do_sample and generator is None:
+            raise NotImplementedError("do_sample=True draws from given random numbers: pass generator= "
+                                      "(a torch.Generator on the model's device)")
         if unused.get("repetition_penalty") not in (None, 1, 1.0):
             raise NotImplementedError("repetition_penalty other than 1 is not built")
         b, s = input_ids.shape
+        n_seq = int(num_return_sequences) if do_sample else 1
+        if n_seq < 1:
+            raise ValueError(f"num_return_sequences {num_return_sequences}: one at least")
+        u = None
+        if do_sample:
+            u = torch.rand(b * n_seq, max_new_tokens, device=input_ids.device, generator=generator)
+
+        def run(ids: torch.Tensor, first: int) -> list:
+            if not do_sample:
+                return list(self.generate_greedy(ids, max_new_tokens, graph=graph,
+                                                 eos_token_id=eos_token_id).unbind(0))
+            mine = u[first * n_seq:(first + ids.shape[0]) * n_seq]
+            return list(self.generate_sampled(
+                ids, max_new_tokens, mine, temperature=1.0 if temperature is None else temperature,
+                top_k=50 if top_k is None else top_k, top_p=1.0 if top_p is None else top_p,
+                min_p=0.0 if min_p is None else min_p, samples=n_seq, graph=graph,
+                eos_token_id=eos_token_id).unbind(0))
+
         if pad_token_id is None:
             pad_token_id = (eos_token_id if isinstance(eos_token_id, int)
                             else (list(eos_token_id)[0] if eos_token_id is not None else 0))
         if attention_mask is None or bool(attention_mask.bool().all()):
-            rows = [self.generate_greedy(input_ids, max_new_tokens, graph=graph,
-                                         eos_token_id=eos_token_id)]
-            rows = list(rows[0].unbind(0))
+            rows = run(input_ids, 0)
         else:
             rows = []
             for i in range(b):
                 keep = attention_mask[i].bool()
                 if not bool(keep.any()):
                     raise ValueError(f"row {i} of the batch has no tokens (attention_mask all 0)")
-                rows.append(self.generate_greedy(input_ids[i:i + 1, keep], max_new_tokens,
-                                                 graph=graph, eos_token_id=eos_token_id)[0])
+                rows.extend(run(input_ids[i:i + 1, keep], i))
         ids = ([eos_token_id] if isinstance(eos_token_id, int) else list(eos_token_id)
                if eos_token_id is not None else [])
         n = max(len(r) for r in rows)
-        new = torch.full((b, n), int(pad_token_id), dtype=input_ids.dtype, device=input_ids.device)
+        new = torch.full((b * n_seq, n), int(pad_token_id), dtype=input_ids.dtype, device=input_ids.device)
         for i, r in enumerate(rows):
             hit = (torch.isin(r, torch.tensor(ids, device=r.device)).nonzero()
                    if ids else torch.empty(0, 1))
             end = int(hit[0, 0]) + 1 if len(hit) else len(r)
             new[i, :end] = r[:end]
-        return torch.cat([input_ids, new], dim=1)
+        prompts = input_ids if n_seq == 1 else input_ids.repeat_interleave(n_seq, 0)
+        return torch.cat([prompts, new], dim=1)
 
 
 def _finished(tok: torch.Tensor, eos: Optional[torch.Tensor]) -> Optional[torch.Tensor]:

@@ -3,8 +3,10 @@
 
 Construction builds the model with `init_model` and copies the pipeline
 knobs onto model.config (model_wrapper.py:22-42); `process_batch` tokenizes,
-generates greedily, decodes, strips the prompt and cuts at the stop words,
-returning [{"text": [completion]}] per prompt (model_wrapper.py:89-136);
+generates, decodes, strips the prompt and cuts at the stop words, returning
+[{"text": [completion]}] per prompt (model_wrapper.py:89-136; with
+num_return_sequences=n, which takes do_sample=True and a generator, n
+completions in each "text");
 after each batch the per-layer drift statistics go to the JSON-lines file
 named by DELTA_DRIFT_LOG (model_wrapper.py:56-84).
 
@@ -93,15 +95,19 @@ class HuggingFaceModel:
                                         **args)
         texts = self.tokenizer.batch_decode(generated, skip_special_tokens=True)
         self._flush_drift_stats()
+        n = len(texts) // max(len(prompts), 1)
         results = []
-        for text, prompt in zip(texts, prompts):
+        for i, prompt in enumerate(prompts):
             # the prompt as the tokenizer round-trips it (it need not reproduce
             # the original string exactly)
             ids = self.tokenizer(prompt, return_tensors="pt").input_ids[0]
             prompt = self.tokenizer.decode(ids, skip_special_tokens=True)
-            if text.startswith(prompt):
-                text = text[len(prompt):]
-            for s in self.stop or ():
-                text = text.split(s)[0]
-            results.append({"text": [text]})
+            completions = []
+            for text in texts[i * n:(i + 1) * n]:
+                if text.startswith(prompt):
+                    text = text[len(prompt):]
+                for s in self.stop or ():
+                    text = text.split(s)[0]
+                completions.append(text)
+            results.append({"text": completions})
         return results
