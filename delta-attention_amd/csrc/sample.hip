@@ -16,7 +16,21 @@
 // a 64-bit integer, in units of 2^-45 of the largest one (fewer bits past 2^17
 // tokens, so that a row's total fits 63), rounded from a 64-bit exponential.
 // Integer sums have no order: a row's token does not depend on how the row is
-// split over threads, and the products u * total and p * total are exact.
+// split over workgroups, and the products u * total and p * total are exact.
+//
+// Long rows are split over workgroups ("parts") and take three or four launches:
+//   top     each part's largest and smallest candidate, and the largest of each of
+//           its groups of lanes
+//   gather  top_k: the k-th largest of a row's group maxima is no larger than its
+//           k-th logit, so the tokens from there on hold the first k and few more:
+//           they are gathered in a list. top_p: the weights' histogram over the
+//           logits
+//   sums    (rows without a list) the kept weight of every tile of 64 vectors;
+//           with top_p the tokens of the one bin at which the histogram reaches p
+//           are gathered in a list, those of larger logits are kept
+//   finish  a workgroup a row: the list sorted, the last token kept, the tile at
+//           which the sum passes u times the total, and the token in it
+// Short rows take the last launch alone, the whole row their list.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -29,10 +43,22 @@ namespace da {
 namespace {
 
 typedef unsigned __int128 u128;
+typedef unsigned long long ull;
 
 constexpr int MAX_V = 1 << 24;               // tokens of a vocabulary
-constexpr int MAX_B = 0x3fffff;              // rows (threads of a grid: below 2^32)
+constexpr int MAX_B = 0x3fffff;              // rows (four parts each: threads of a grid below 2^32)
 constexpr uint32_t KEY_NONE = 0x007fffffu;   // -inf's key: candidates lie above it
+constexpr int PART = 256;                    // threads of a part
+constexpr int LIST = 4096;                   // tokens of a row's list
+constexpr int BINS = 768;                    // of a part's histogram
+constexpr int GROUPS = 2048;                 // group maxima of a row at most
+constexpr int FIN = 512;                     // threads of the finish
+constexpr int SLOTS = 2048;                  // tile sums in LDS; bins of a radix pass
+
+struct Part {
+  uint64_t first;                            // the first place in the order, 0: no candidate
+  uint32_t least, pad;                       // the smallest candidate's key
+};
 
 struct SampleArgs {
   const void* x;
@@ -46,6 +72,16 @@ struct SampleArgs {
   int64_t* token;
   float* logp;
   int B, V, bits;                           // weights in units of 2^-bits
+  int parts, tiles, k_list;                 // parts of a row, tiles of a part, the largest top_k with a list
+  FastDiv f_parts;
+  int groups, lanes;                        // group maxima of a part, lanes of a group
+  // workspace, by row
+  Part* part;                               // [parts]
+  uint32_t* maxima;                         // [parts * groups]
+  uint32_t* count;                          // tokens gathered (also past the list's end)
+  uint64_t* hist;                           // [parts, BINS]
+  uint64_t* list;                           // [LIST] places
+  uint64_t* tile;                           // [parts * tiles] kept weight
 };
 
 // A number's place in the order of floats (-0 beside 0); NaN last.
@@ -60,43 +96,166 @@ __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) {
   return key > KEY_NONE ? (uint64_t)key << 32 | (uint32_t)~i : 0;
 }
 __device__ __forceinline__ int index_of(uint64_t place) { return (int)~(uint32_t)place; }
+__device__ __forceinline__ float logit_of(uint64_t place) { return of_key(place >> 32); }
 
-// 2^t for t <= 0 in units of 2^-bits: the fraction's power by its series to the
-// 13th term (2^-52 of it), the whole one by the exponent.
+// 2^t for t <= 0 in units of 2^-bits (bits <= 45): the fraction's power by its
+// series to the 13th term (2^-52 of it), the whole one by the exponent; rounded
+// to an integer by what 2^52 leaves of it.
 __device__ __forceinline__ uint64_t weight_of(double t, int bits) {
-  t = fmax(t, -200.0);                      // (2^-200 of the largest: none)
+  t = fmax(t, -200.0);                      // (2^-200 of the largest: none; also of what is no number)
   const double n = rint(t), f = (t - n) * 0.693147180559945309417;
   double p = 1.0 / 479001600;
   constexpr double c[] = {1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720,
                           1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0};
 #pragma unroll
   for (int i = 0; i < 12; ++i) p = fma(p, f, c[i]);
-  return (uint64_t)rint(ldexp(p, (int)n + bits));
+  return (uint64_t)__double_as_longlong(ldexp(p, (int)n + bits) + 4503599627370496.0) - 0x4330000000000000ull;
 }
 
-template <typename T> struct Logit;
-template <> struct Logit<__bf16> {
-  static __device__ __forceinline__ float at(const void* p, int i) { return Elt<__bf16>::lo(((const uint16_t*)p)[i]); }
+// What a row asks for.
+struct Setting {
+  float t, p, m;
+  int k;
+  bool greedy, cut, list, run;              // cut: top_k takes some away; list: by a list; run: top_p takes some away
+  __device__ __forceinline__ bool sums() const { return !greedy && !cut; }   // rows of the sums launch
 };
-template <> struct Logit<_Float16> {
-  static __device__ __forceinline__ float at(const void* p, int i) { return (float)((const _Float16*)p)[i]; }
-};
-template <> struct Logit<float> {
-  static __device__ __forceinline__ float at(const void* p, int i) { return ((const float*)p)[i]; }
+__device__ __forceinline__ Setting setting_of(const SampleArgs& a, int b) {
+  Setting s;
+  s.t = a.t_dev ? a.t_dev[b * a.t_step] : a.t;
+  s.k = a.k_dev ? a.k_dev[b * a.k_step] : a.k;
+  s.p = a.p_dev ? a.p_dev[b * a.p_step] : a.p;
+  s.m = a.m_dev ? a.m_dev[b * a.m_step] : a.m;
+  s.greedy = !(s.t > 0.f);
+  s.cut = s.k > 0 && s.k < a.V;
+  s.list = s.cut && s.k <= a.k_list;
+  s.run = s.p < 1.f;
+  return s;
+}
+
+// The weights of a row with a candidate, and the bins of its histogram: linear in
+// the logit, from the largest to where weights vanish or the smallest candidate.
+struct Scale {
+  double top, per, bar;
+  float topf, step;
+  int bits;
+  uint64_t first;
+  __device__ __forceinline__ Scale(const SampleArgs& a, const Setting& s, uint64_t first_, uint32_t least) {
+    first = first_;
+    bits = a.bits;
+    topf = logit_of(first);
+    top = topf;
+    per = 1.44269504088896340736 / (double)s.t;
+    bar = s.m > 0.f ? top + (double)s.t * log((double)s.m) : -INFINITY;
+    const double far = a.bits + 2, all = (top - (double)of_key(least)) * per;
+    const double range = all < far ? all : far;
+    step = range > 0.0 ? (float)(BINS * (1.0 - 1.0 / 1024) / range * per) : 0.f;
+  }
+  // (an infinite top: the tokens at it share the row)
+  __device__ __forceinline__ uint64_t weight(float y) const {
+    return weight_of(y == topf ? 0.0 : ((double)y - top) * per, bits);
+  }
+  __device__ __forceinline__ int bin(float y) const {   // BINS and above: no weight
+    const float f = (topf - y) * step;
+    return y == topf ? 0 : topf == INFINITY ? BINS : (int)fminf(f, (float)BINS);
+  }
+  __device__ __forceinline__ bool clears(float y, uint64_t place) const { return (double)y >= bar || place == first; }
 };
 
-constexpr int THREADS = 1024;
-constexpr int BINS = 2048;
+// A row as 16-byte vectors from the aligned address at or before its start; what
+// lies outside the row counts as -inf.
+template <typename T>
+struct Row {
+  static constexpr int E = 16 / sizeof(T);
+  const u32x4* base;
+  int shift, V, n_vec;
+  __device__ __forceinline__ Row(const SampleArgs& a, int b) {
+    const uintptr_t p = (uintptr_t)((const T*)a.x + (int64_t)b * a.x_b);
+    base = (const u32x4*)(p & ~(uintptr_t)15);
+    shift = (int)(p & 15) / sizeof(T);
+    V = a.V;
+    n_vec = (V + shift + E - 1) / E;
+  }
+  __device__ __forceinline__ int index(int v, int e) const { return v * E + e - shift; }
+  __device__ __forceinline__ u32x4 load(int v) const { return base[min(v, n_vec - 1)]; }
+  __device__ __forceinline__ void unpack(u32x4 w, int v, float (&y)[E]) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if constexpr (sizeof(T) == 4) y[e] = __uint_as_float(w[e]);
+      else y[e] = e % 2 ? Elt<T>::hi(w[e / 2]) : Elt<T>::lo(w[e / 2]);
+    }
+    if (v == 0 || v >= n_vec - 1) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int i = index(v, e);
+        y[e] = i >= 0 && i < V && v < n_vec ? y[e] : -INFINITY;
+      }
+    }
+  }
+  // f(logit, index) of each of the vector's candidates and others
+  template <typename F>
+  __device__ __forceinline__ void each(int v, F&& f) const {
+    float y[E];
+    unpack(load(v), v, y);
+#pragma unroll
+    for (int e = 0; e < E; ++e) f(y[e], index(v, e));
+  }
+};
 
-template <typename F>
+// Sum over the lanes up to this one.
+__device__ __forceinline__ uint64_t scan64(uint64_t x) {
+  auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
+    constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, C, R, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), C, R, 0xf, false);
+    x += (uint64_t)hi << 32 | lo;
+  };
+  using std::integral_constant;
+  step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});   // row_shr 1, 2, 4, 8
+  step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+  step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});   // across the rows of 16
+  step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
+  return x;
+}
+__device__ __forceinline__ uint64_t last_lane(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(x >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((uint32_t)x, 63);
+}
+
+template <int N, typename F>
 __device__ __forceinline__ uint64_t block_reduce(uint64_t v, uint64_t* s, F&& f) {
   for (int d = 32; d > 0; d /= 2) v = f(v, __shfl_xor(v, d));
   __syncthreads();
   if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = v;
   __syncthreads();
   v = s[0];
-  for (int w = 1; w < THREADS / 64; ++w) v = f(v, s[w]);
+#pragma unroll
+  for (int w = 1; w < N / 64; ++w) v = f(v, s[w]);
   return v;
+}
+struct Most {
+  __device__ __forceinline__ uint64_t operator()(uint64_t p, uint64_t q) const { return p > q ? p : q; }
+};
+struct Plus {
+  __device__ __forceinline__ uint64_t operator()(uint64_t p, uint64_t q) const { return p + q; }
+};
+
+// Sums of the threads before this one; `total` of all.
+template <int N>
+__device__ __forceinline__ uint64_t block_before(uint64_t v, uint64_t* s, uint64_t& total) {
+  const uint64_t upto = scan64(v);
+  __syncthreads();
+  if (threadIdx.x % 64 == 63) s[threadIdx.x / 64] = upto;
+  __syncthreads();
+  uint64_t before = upto - v;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < N / 64; ++w) {
+    if (w < (int)threadIdx.x / 64) before += s[w];
+    total += s[w];
+  }
+  return before;
 }
 
 // ceil or floor of f * total for 0 <= f < 1, exactly.
@@ -105,121 +264,561 @@ __device__ __forceinline__ uint64_t part_of(float f, uint64_t total, bool up) {
   if (f != f || (int)b <= 0) return 0;
   const int e = b >> 23;                    // f = mant * 2^(e - 150)
   const uint32_t mant = e ? (b & 0x7fffff) | 0x800000 : b & 0x7fffff;
-  const int shift = 150 - (e ? e : 1);      // 24 at least
+  const int shift = 150 - (e ? e : 1);
   if (shift > 120) return up && total ? 1 : 0;
+  if (shift < 24) return total;             // (1 and above)
   const u128 y = (u128)mant * total;
   return (uint64_t)((y + (up ? ((u128)1 << shift) - 1 : 0)) >> shift);
 }
 
-template <typename T>
-__global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
-  __shared__ uint64_t s_red[THREADS / 64], s_bin[BINS], s_found[3];
-  const int b = blockIdx.x, tid = threadIdx.x;
-  const T* x = (const T*)a.x + (int64_t)b * a.x_b;
-  const auto most = [](uint64_t p, uint64_t q) { return p > q ? p : q; };
-  const auto plus = [](uint64_t p, uint64_t q) { return p + q; };
+// A row's first place and smallest candidate, from its parts'.
+__device__ __forceinline__ void row_ends(const SampleArgs& a, int b, uint64_t& first, uint32_t& least) {
+  const Part* p = a.part + (int64_t)b * a.parts;
+  first = 0, least = ~0u;
+  for (int i = threadIdx.x % 64; i < a.parts; i += 64) {
+    first = p[i].first > first ? p[i].first : first;
+    least = min(least, p[i].least);
+  }
+  for (int d = 32; d > 0; d /= 2) {
+    const uint64_t o = __shfl_xor(first, d);
+    first = o > first ? o : first;
+    least = min(least, (uint32_t)__shfl_xor((int)least, d));
+  }
+}
 
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
+  using R = Row<T>;
+  __shared__ uint64_t s_first[PART / 64];
+  __shared__ uint32_t s_least[PART / 64];
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  if (part == 0 && threadIdx.x == 0) a.count[b] = 0;
+  const R row(a, b);
+  float most = -INFINITY, least = INFINITY;
+  int at = 0;                               // the vector that raised `most` last
+  const int v0 = (part * a.tiles + wave) * 64 + lane;
+#pragma unroll 4
+  for (int j = 0; j < a.tiles; j += PART / 64) {
+    const int v = v0 + j * 64;
+    if (v >= row.n_vec) break;
+    float y[R::E];
+    row.unpack(row.load(v), v, y);
+    float top = y[0];
+#pragma unroll
+    for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);   // (a NaN gives way)
+#pragma unroll
+    for (int e = 0; e < R::E; ++e) least = fminf(least, y[e] > -INFINITY ? y[e] : INFINITY);
+    if (top > most) {
+      most = top;
+      at = v;
+    }
+  }
+  const uint32_t key = key_of(most);
   uint64_t first = 0;
-  for (int i = tid; i < a.V; i += THREADS) first = most(first, place_of(key_of(Logit<T>::at(x, i)), i));
-  first = block_reduce(first, s_red, most);
-  if (first == 0) {
-    if (tid == 0) {
-      a.token[b] = 0;
-      a.logp[b] = __builtin_nanf("");
+  if (key > KEY_NONE)
+    row.each(at, [&](float y, int i) __attribute__((always_inline)) {
+      if (first == 0 && key_of(y) == key) first = place_of(key, i);
+    });
+  uint32_t g = key, low = least < INFINITY ? key_of(least) : key > KEY_NONE ? key : ~0u;
+  for (int d = 1; d < a.lanes; d *= 2) g = max(g, (uint32_t)__shfl_xor((int)g, d));
+  if (threadIdx.x % a.lanes == 0) a.maxima[((int64_t)b * a.parts + part) * a.groups + threadIdx.x / a.lanes] = g;
+  for (int d = 32; d > 0; d /= 2) {
+    const uint64_t o = __shfl_xor(first, d);
+    first = o > first ? o : first;
+    low = min(low, (uint32_t)__shfl_xor((int)low, d));
+  }
+  if (lane == 0) {
+    s_first[wave] = first;
+    s_least[wave] = low;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < PART / 64; ++w) {
+      first = s_first[w] > first ? s_first[w] : first;
+      low = min(low, s_least[w]);
     }
+    a.part[(int64_t)b * a.parts + part] = Part{first, low, 0};
+  }
+}
+
+// Appends the places that the part holds in s_list to the row's list.
+__device__ __forceinline__ void append(const SampleArgs& a, int b, const uint64_t* s_list, uint32_t n, uint32_t* s_at) {
+  __syncthreads();
+  if (threadIdx.x == 0 && n > 0) *s_at = atomicAdd(a.count + b, n);
+  __syncthreads();
+  if (n == 0 || n > LIST) return;
+  for (uint32_t i = threadIdx.x; i < n; i += PART)
+    if (*s_at + i < LIST) a.list[(int64_t)b * LIST + *s_at + i] = s_list[i];
+}
+
+template <typename T>
+__global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
+  using R = Row<T>;
+  __shared__ uint64_t s_mem[LIST];          // the list, or the histogram
+  __shared__ uint32_t s_cnt[2][PART / 64], s_n, s_at;
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const Setting s = setting_of(a, b);
+  const bool hist = s.sums() && s.run;
+  if (s.greedy || (!s.list && !hist)) return;
+  uint64_t first;
+  uint32_t least;
+  row_ends(a, b, first, least);
+  if (first == 0) return;
+  const R row(a, b);
+  const int v0 = (part * a.tiles + wave) * 64 + lane;
+  if (s.list) {
+    // The largest number of 16 bits that is no larger than the k-th group maximum's
+    // first 16: bit by bit, by the count of maxima that reach it.
+    const int n_max = a.parts * a.groups;
+    const uint32_t* mx = a.maxima + (int64_t)b * n_max;
+    uint32_t key[GROUPS / PART], low = 0;
+#pragma unroll
+    for (int i = 0; i < GROUPS / PART; ++i) key[i] = i * PART + (int)threadIdx.x < n_max ? mx[i * PART + threadIdx.x] >> 16 : 0;
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint32_t c = low | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < GROUPS / PART; ++i) n += __popcll(__ballot(key[i] >= c));
+      if (lane == 0) s_cnt[bit % 2][wave] = n;
+      __syncthreads();
+      n = 0;
+#pragma unroll
+      for (int w = 0; w < PART / 64; ++w) n += s_cnt[bit % 2][w];
+      if (n >= s.k) low = c;
+    }
+    const uint32_t from = max(low << 16, KEY_NONE + 1);
+    if (threadIdx.x == 0) s_n = 0;
+    __syncthreads();
+#pragma unroll 4
+    for (int j = 0; j < a.tiles; j += PART / 64) {
+      const int v = v0 + j * 64;
+      if (v >= row.n_vec) break;
+      row.each(v, [&](float y, int i) __attribute__((always_inline)) {
+        const uint32_t k = key_of(y);
+        if (k >= from) {
+          const uint32_t at = atomicAdd(&s_n, 1u);
+          if (at < LIST) s_mem[at] = place_of(k, i);
+        }
+      });
+    }
+    __syncthreads();
+    append(a, b, s_mem, s_n, &s_at);
     return;
   }
-  const float temp = a.t_dev ? a.t_dev[b * a.t_step] : a.t;
-  if (!(temp > 0.f)) {
-    if (tid == 0) {
-      a.token[b] = index_of(first);
-      a.logp[b] = 0.f;
-    }
-    return;
+  const Scale sc(a, s, first, least);
+  for (int i = threadIdx.x; i < BINS; i += PART) s_mem[i] = 0;
+  __syncthreads();
+  for (int j = 0; j < a.tiles; j += PART / 64) {
+    const int v = v0 + j * 64;
+    if (v >= row.n_vec) break;
+    row.each(v, [&](float y, int) __attribute__((always_inline)) {
+      if (!(y > -INFINITY)) return;
+      const int at = sc.bin(y);
+      if (at < BINS) atomicAdd((ull*)&s_mem[at], (ull)sc.weight(y));
+    });
   }
-  const int k = a.k_dev ? a.k_dev[b * a.k_step] : a.k;
-  const float p = a.p_dev ? a.p_dev[b * a.p_step] : a.p, m = a.m_dev ? a.m_dev[b * a.m_step] : a.m;
-  const double top = of_key(first >> 32), per = 1.44269504088896340736 / (double)temp;
-  auto weight = [&](float y) __attribute__((always_inline)) -> uint64_t {
-    // (an infinite one: the tokens at it share the row)
-    return weight_of((double)y == top ? 0.0 : ((double)y - top) * per, a.bits);
-  };
-  uint64_t last = 1;                        // the last place kept
-  // The first place in the order at which the measure, summed, reaches `goal`
-  // (0: none does), eleven bits of the place at a time.
-  auto reach = [&](auto&& measure, uint64_t goal) {
-    uint64_t prefix = 0, before = 0;
-    for (int low = 55; low >= 0; low -= 11) {
-      for (int i = tid; i < BINS; i += THREADS) s_bin[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < a.V; i += THREADS) {
-        const float y = Logit<T>::at(x, i);
-        const uint64_t place = place_of(key_of(y), i);
-        if (place < last || (low < 55 && place >> (low + 11) != prefix)) continue;
-        const uint64_t w = measure(y);
-        if (w) atomicAdd((unsigned long long*)&s_bin[place >> low & (BINS - 1)], (unsigned long long)w);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint64_t sum = before;
-        int i = BINS - 1;
-        for (; i > 0 && sum + s_bin[i] < goal; --i) sum += s_bin[i];
-        s_found[0] = prefix << 11 | i;
-        s_found[1] = sum;
-        s_found[2] = sum + s_bin[i];
-      }
-      __syncthreads();
-      prefix = s_found[0];
-      before = s_found[1];
-      if (s_found[2] < goal) return (uint64_t)0;
-    }
-    return prefix;
-  };
-  if (k > 0 && k < a.V) {
-    const uint64_t at = reach([](float) { return (uint64_t)1; }, k);
-    if (at) last = at;
+  __syncthreads();
+  uint64_t* to = a.hist + ((int64_t)b * a.parts + part) * BINS;
+  for (int i = threadIdx.x; i < BINS; i += PART) to[i] = s_mem[i];
+}
+
+// The bin at which a row's histogram reaches p times its total, the weight of
+// those before it and what is to be reached. s: BINS / 3 + 8 words.
+template <int N>
+__device__ __forceinline__ int border_bin(const SampleArgs& a, int b, float p, uint64_t* s, uint64_t& before, uint64_t& goal) {
+  constexpr int PER = BINS / 256;           // bins of a thread
+  static_assert(BINS % 256 == 0 && N >= 256, "256 threads hold the bins");
+  uint64_t sum[PER] = {}, mine = 0, total;
+  if (threadIdx.x < 256) {
+    const uint64_t* h = a.hist + (int64_t)b * a.parts * BINS + threadIdx.x * PER;
+    for (int i = 0; i < a.parts; ++i)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum[e] += h[(int64_t)i * BINS + e];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) mine += sum[e];
   }
-  if (p < 1.f) {
+  uint64_t upto = block_before<N>(mine, s, total);
+  goal = part_of(p, total, true);
+  if (goal < 1) goal = 1;
+  __syncthreads();
+  if (upto < goal && upto + mine >= goal) {
+    int e = 0;
+#pragma unroll
+    for (int i = 0; i < PER - 1; ++i)
+      if (e == i && upto + sum[i] < goal) {
+        upto += sum[i];
+        e = i + 1;
+      }
+    s[0] = threadIdx.x * PER + e;
+    s[1] = upto;
+  }
+  __syncthreads();
+  before = s[1];
+  return (int)s[0];
+}
+
+template <typename T>
+__global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
+  using R = Row<T>;
+  __shared__ uint64_t s_list[LIST], s_scan[8];
+  __shared__ uint32_t s_n, s_at;
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const Setting s = setting_of(a, b);
+  if (!s.sums()) return;
+  uint64_t first;
+  uint32_t least;
+  row_ends(a, b, first, least);
+  if (first == 0) return;
+  const Scale sc(a, s, first, least);
+  uint64_t before, goal;
+  const int border = s.run ? border_bin<PART>(a, b, s.p, s_scan, before, goal) : BINS;
+  if (threadIdx.x == 0) s_n = 0;
+  __syncthreads();
+  const R row(a, b);
+  for (int j = 0; j < a.tiles; j += PART / 64) {
+    const int tile = part * a.tiles + j + wave, v = tile * 64 + lane;
+    if (tile * 64 >= row.n_vec) break;
     uint64_t sum = 0;
-    for (int i = tid; i < a.V; i += THREADS) {
-      const float y = Logit<T>::at(x, i);
-      if (place_of(key_of(y), i) >= last) sum += weight(y);
+    if (v < row.n_vec)
+      row.each(v, [&](float y, int i) __attribute__((always_inline)) {
+        if (!(y > -INFINITY)) return;
+        const int at = sc.bin(y);
+        if (at > border) return;
+        const uint64_t place = place_of(key_of(y), i);
+        if (at == border && s.run) {
+          const uint32_t n = atomicAdd(&s_n, 1u);
+          if (n < LIST) s_list[n] = place;
+        } else if (at < BINS && sc.clears(y, place)) {
+          sum += sc.weight(y);
+        }
+      });
+    sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
+    if (lane == 0) a.tile[(int64_t)b * a.parts * a.tiles + tile] = sum;
+  }
+  __syncthreads();
+  if (s.run) append(a, b, s_list, s_n, &s_at);
+}
+
+// ---------------------------------------------------------------------------
+// Sorts s[0 .. n2), the largest first (n2 a power of two).
+__device__ __forceinline__ void sort_down(uint64_t* s, int n2) {
+  for (int k = 2; k <= n2; k *= 2)
+    for (int j = k / 2; j > 0; j /= 2) {
+      __syncthreads();
+      for (int t = threadIdx.x; t < n2 / 2; t += FIN) {
+        const int i = (t & ~(j - 1)) * 2 | (t & (j - 1));
+        const uint64_t p = s[i], q = s[i + j];
+        if (((i & k) == 0) == (p < q)) {
+          s[i] = q;
+          s[i + j] = p;
+        }
+      }
     }
-    sum = block_reduce(sum, s_red, plus);
-    const uint64_t goal = part_of(p, sum, true);
-    const uint64_t at = goal <= 1 ? first : reach(weight, goal);
-    if (at) last = at;
+  __syncthreads();
+}
+
+template <typename T, bool SPLIT>
+__global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
+  using R = Row<T>;
+  __shared__ uint64_t s_list[LIST], s_slot[SLOTS], s_scan[16], s_found[3];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
+  const Setting s = setting_of(a, b);
+  const R row(a, b);
+  const uint32_t n_cand = SPLIT ? a.count[b] : 0;
+  uint64_t first;
+  uint32_t least = ~0u;
+  if constexpr (SPLIT) {
+    row_ends(a, b, first, least);
+  } else {
+    first = 0;
+    for (int v = tid; v < row.n_vec; v += FIN)
+      row.each(v, [&](float y, int i) __attribute__((always_inline)) {
+        const uint64_t place = place_of(key_of(y), i);
+        first = place > first ? place : first;
+      });
+    first = block_reduce<FIN>(first, s_scan, Most());
   }
-  const double bar = m > 0.f ? top + (double)temp * log((double)m) : -INFINITY;
-  auto kept = [&](float y, int i) __attribute__((always_inline)) -> uint64_t {
-    const uint64_t place = place_of(key_of(y), i);
-    return place >= last && ((double)y >= bar || place == first) ? weight(y) : 0;
+  auto done = [&](int token, float logp) __attribute__((always_inline)) {
+    a.token[b] = token;
+    a.logp[b] = logp;
   };
-  // a stretch of the row for each thread, then the stretch's own tokens
-  const int len = (a.V + THREADS - 1) / THREADS, from = tid * len, to = min(from + len, a.V);
-  uint64_t sum = 0;
-  for (int i = from; i < to; ++i) sum += kept(Logit<T>::at(x, i), i);
-  __syncthreads();
-  s_bin[tid] = sum;
-  __syncthreads();
-  uint64_t before = 0, total = 0;
-  for (int t = 0; t < THREADS; ++t) {
-    if (t == tid) before = total;
-    total += s_bin[t];
+  if (first == 0 || s.greedy) {
+    if (tid == 0) first == 0 ? done(0, __builtin_nanf("")) : done(index_of(first), 0.f);
+    return;
   }
-  const uint64_t goal = part_of(a.u[b], total, false);
-  const uint64_t aim = goal < total ? goal : total - 1;
-  if (before > aim || before + sum <= aim) return;
-  for (int i = from; i < to; ++i) {
-    const float y = Logit<T>::at(x, i);
-    before += kept(y, i);
-    if (before > aim) {
-      a.token[b] = i;
-      const double d = (double)y == top ? 0.0 : ((double)y - top) / (double)temp;
-      a.logp[b] = (float)(d - log(ldexp((double)total, -a.bits)));
+  const Scale sc(a, s, first, SPLIT ? least : KEY_NONE + 1);
+  auto drawn = [&](float y, int i, uint64_t total) __attribute__((always_inline)) {
+    const double d = y == sc.topf ? 0.0 : ((double)y - sc.top) / (double)s.t;
+    done(i, (float)(d - log(ldexp((double)total, -a.bits))));
+  };
+  auto aim_of = [&](uint64_t total) __attribute__((always_inline)) {
+    const uint64_t aim = part_of(a.u[b], total, false);
+    return aim < total ? aim : total - 1;
+  };
+
+  // the row's kept tokens as a list of their own?
+  const bool whole = SPLIT ? s.list && n_cand <= LIST : a.V <= LIST;
+  if (whole) {
+    int n;
+    if constexpr (SPLIT) {
+      n = (int)n_cand;
+      for (int i = tid; i < n; i += FIN) s_list[i] = a.list[(int64_t)b * LIST + i];
+    } else {
+      n = a.V;
+      for (int v = tid; v < row.n_vec; v += FIN)
+        row.each(v, [&](float y, int i) __attribute__((always_inline)) {
+          if (i >= 0 && i < a.V) s_list[i] = place_of(key_of(y), i);
+        });
+    }
+    int n2 = 2;
+    while (n2 < n) n2 *= 2;
+    for (int i = n + tid; i < n2; i += FIN) s_list[i] = 0;
+    __syncthreads();
+    const int per = (n2 + FIN - 1) / FIN, at0 = tid * per, at1 = min(at0 + per, n2);
+    auto mass = [&](int end) __attribute__((always_inline)) {
+      uint64_t sum = 0;
+      for (int i = at0; i < min(at1, end); ++i) sum += s_list[i] ? sc.weight(logit_of(s_list[i])) : 0;
+      return sum;
+    };
+    const bool filter = s.cut || s.run || s.m > 0.f;
+    uint64_t total;
+    if (filter) {
+      sort_down(s_list, n2);
+      if (s.cut) n = min(n, s.k);
+      uint64_t before = block_before<FIN>(mass(n), s_scan, total);
+      const uint64_t goal = s.run ? part_of(s.p, total, true) : ~0ull;
+      int keep = 0;
+      for (int i = at0; i < min(at1, n); ++i) {
+        const uint64_t place = s_list[i];
+        if (place == 0) break;
+        if (i == 0 || (before < goal && sc.clears(logit_of(place), place))) ++keep;
+        before += sc.weight(logit_of(place));
+      }
+      n = (int)block_reduce<FIN>(keep, s_scan, Plus());
+      // by index: the first one the largest number
+      n2 = 2;
+      while (n2 < n) n2 *= 2;
+      __syncthreads();
+      for (int i = tid; i < n2; i += FIN) {
+        const uint64_t place = s_list[i];
+        s_list[i] = i < n ? place << 32 | place >> 32 : 0;
+      }
+      sort_down(s_list, n2);
+      for (int i = tid; i < n2; i += FIN) {
+        const uint64_t place = s_list[i];
+        s_list[i] = place << 32 | place >> 32;
+      }
+      __syncthreads();
+    }
+    uint64_t before = block_before<FIN>(mass(n), s_scan, total);
+    const uint64_t aim = aim_of(total);
+    for (int i = at0; i < min(at1, n); ++i) {
+      const uint64_t place = s_list[i];
+      const uint64_t upto = before + (place ? sc.weight(logit_of(place)) : 0);
+      if (before <= aim && upto > aim) drawn(logit_of(place), index_of(place), total);
+      before = upto;
+    }
+    return;
+  }
+  if constexpr (!SPLIT) return;             // (rows of one launch fit the list)
+
+  uint64_t last = 1;                        // the last place kept
+  int border = BINS;                        // the bin of `last`: the bins before it are kept whole
+  const int tiles = (row.n_vec + 63) / 64, per = (tiles + SLOTS - 1) / SLOTS;   // tiles of a slot
+  const bool ready = s.sums() && (!s.run || n_cand <= LIST);   // by the launches before
+  for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
+  __syncthreads();
+  if (ready) {
+    const uint64_t* sums = a.tile + (int64_t)b * a.parts * a.tiles;
+    if (s.run) {
+      uint64_t before, goal, total;
+      border = border_bin<FIN>(a, b, s.p, s_scan, before, goal);
+      int n = (int)n_cand, n2 = 2;
+      while (n2 < n) n2 *= 2;
+      for (int i = tid; i < n2; i += FIN) s_list[i] = i < n ? a.list[(int64_t)b * LIST + i] : 0;
+      sort_down(s_list, n2);
+      const int share = (n2 + FIN - 1) / FIN, at0 = tid * share, at1 = min(at0 + share, n);
+      uint64_t sum = 0;
+      for (int i = at0; i < at1; ++i) sum += sc.weight(logit_of(s_list[i]));
+      before += block_before<FIN>(sum, s_scan, total);
+      int keep = 0;
+      for (int i = at0; i < at1; ++i) {
+        const uint64_t place = s_list[i], w = sc.weight(logit_of(place));
+        if (place == first || (before < goal && sc.clears(logit_of(place), place))) {
+          ++keep;
+          atomicAdd((ull*)&s_slot[(index_of(place) + row.shift) / R::E / 64 / per], (ull)w);
+        }
+        before += w;
+      }
+      n = (int)block_reduce<FIN>(keep, s_scan, Plus());
+      last = n > 0 ? s_list[n - 1] : ~0ull;
+    }
+    for (int i = tid; i < tiles; i += FIN) {
+      const uint64_t w = sums[i];
+      if (w) atomicAdd((ull*)&s_slot[i / per], (ull)w);
+    }
+    __syncthreads();
+  } else {
+    // What the lists do not hold (a top_k past k_list, more than LIST tokens at a
+    // border): the border place eleven bits at a time, over the whole row.
+    auto over = [&](auto&& f) {
+      for (int v = tid; v < row.n_vec; v += FIN) row.each(v, f);
+    };
+    auto reach = [&](auto&& measure, uint64_t goal) {
+      uint64_t prefix = 0, before = 0;
+      for (int low = 55; low >= 0; low -= 11) {
+        for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
+        __syncthreads();
+        over([&](float y, int i) __attribute__((always_inline)) {
+          const uint64_t place = place_of(key_of(y), i);
+          if (place < last || (low < 55 && place >> (low + 11) != prefix)) return;
+          const uint64_t w = measure(y);
+          if (w) atomicAdd((ull*)&s_slot[place >> low & (SLOTS - 1)], (ull)w);
+        });
+        __syncthreads();
+        if (tid == 0) {
+          uint64_t sum = before;
+          int i = SLOTS - 1;
+          for (; i > 0 && sum + s_slot[i] < goal; --i) sum += s_slot[i];
+          s_found[0] = prefix << 11 | i;
+          s_found[1] = sum;
+          s_found[2] = sum + s_slot[i];
+        }
+        __syncthreads();
+        prefix = s_found[0];
+        before = s_found[1];
+        if (s_found[2] < goal) return (uint64_t)0;   // (fewer than that)
+      }
+      return prefix;
+    };
+    if (s.cut) {
+      const uint64_t at = reach([](float) { return (uint64_t)1; }, s.k);
+      if (at) last = at;
+    }
+    if (s.run) {
+      uint64_t sum = 0;
+      over([&](float y, int i) __attribute__((always_inline)) {
+        if (place_of(key_of(y), i) >= last) sum += sc.weight(y);
+      });
+      sum = block_reduce<FIN>(sum, s_scan, Plus());
+      const uint64_t goal = part_of(s.p, sum, true);
+      const uint64_t at = goal <= 1 ? first : reach([&](float y) { return sc.weight(y); }, goal);
+      if (at) last = at;
+    }
+    border = -1;                            // (by place alone)
+    for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
+    __syncthreads();
+    for (int v = tid; v < tiles * 64; v += FIN) {
+      uint64_t sum = 0;
+      if (v < row.n_vec)
+        row.each(v, [&](float y, int i) __attribute__((always_inline)) {
+          const uint64_t place = place_of(key_of(y), i);
+          if (place >= last && sc.clears(y, place)) sum += sc.weight(y);
+        });
+      sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
+      if (lane == 0 && sum) atomicAdd((ull*)&s_slot[v / 64 / per], (ull)sum);
+    }
+    __syncthreads();
+  }
+
+  // the slot at which the sum passes the aim, then the tile and the token
+  constexpr int PER = SLOTS / FIN;
+  uint64_t mine = 0, total;
+#pragma unroll
+  for (int e = 0; e < PER; ++e) mine += s_slot[tid * PER + e];
+  uint64_t before = block_before<FIN>(mine, s_scan, total);
+  const uint64_t aim = aim_of(total);
+  if (before <= aim && before + mine > aim) {
+    int e = 0;
+    while (before + s_slot[tid * PER + e] <= aim) before += s_slot[tid * PER + e++];
+    s_found[0] = tid * PER + e;
+    s_found[1] = before;
+  }
+  __syncthreads();
+  if (tid >= 64) return;
+  before = s_found[1];
+  for (int t = (int)s_found[0] * per; t < tiles; ++t) {
+    const int v = t * 64 + lane;
+    float y[R::E];
+    uint64_t w[R::E], sum = 0;
+    row.unpack(row.load(v), v, y);
+#pragma unroll
+    for (int e = 0; e < R::E; ++e) {
+      const uint64_t place = place_of(key_of(y[e]), row.index(v, e));
+      const int at = place ? sc.bin(y[e]) : BINS;
+      w[e] = place && (border < 0 ? place >= last : border == BINS ? at < BINS : at < border || (at == border && place >= last)) &&
+                     sc.clears(y[e], place) ? sc.weight(y[e]) : 0;
+      sum += w[e];
+    }
+    const uint64_t upto = scan64(sum);
+    if (before + last_lane(upto) > aim) {
+      uint64_t sofar = before + upto - sum;
+      if (sofar <= aim && sofar + sum > aim) {
+#pragma unroll
+        for (int e = 0; e < R::E; ++e) {
+          if (sofar <= aim && sofar + w[e] > aim) drawn(y[e], row.index(v, e), total);
+          sofar += w[e];
+        }
+      }
       return;
     }
+    before += last_lane(upto);
   }
+}
+
+// ---------------------------------------------------------------------------
+// host side
+
+struct Plan {
+  int parts, tiles, groups, lanes;          // parts 0: one launch
+  size_t part, maxima, count, hist, list, tile, bytes;   // offsets
+};
+
+void plan_for(Plan& p, int B, int V, int dtype) {
+  p = Plan{};
+  if (V <= LIST) return;
+  const int E = dtype == DA_FP32 ? 4 : 8;
+  const int64_t tiles = ((int64_t)V + 2 * E - 1) / E / 64 + 1;   // whatever the row's alignment
+  // parts: some workgroups for each CU together, 4 tiles (one of each wave) at least
+  int64_t parts = (512 + B - 1) / B;
+  parts = parts < 4 ? 4 : parts > 32 ? 32 : parts;
+  while (parts > 4 && tiles < parts * 4) parts /= 2;
+  p.tiles = (int)(((tiles + parts - 1) / parts + 3) / 4 * 4);
+  p.parts = (int)parts;
+  p.lanes = 1;
+  while (p.parts * (PART / p.lanes) > GROUPS) p.lanes *= 2;
+  p.groups = PART / p.lanes;
+  size_t at = 0;
+  auto room = [&](size_t bytes) {
+    const size_t here = at;
+    at += (bytes * B + 255) / 256 * 256;
+    return here;
+  };
+  p.part = room(sizeof(Part) * p.parts);
+  p.maxima = room(sizeof(uint32_t) * p.parts * p.groups);
+  p.count = room(sizeof(uint32_t));
+  p.hist = room(sizeof(uint64_t) * p.parts * BINS);
+  p.list = room(sizeof(uint64_t) * LIST);
+  p.tile = room(sizeof(uint64_t) * p.parts * p.tiles);
+  p.bytes = at;
+}
+
+template <typename T>
+void launch(const SampleArgs& a, hipStream_t st) {
+  if (a.parts == 0) {
+    hipLaunchKernelGGL((sample_finish_kernel<T, false>), dim3(a.B), dim3(FIN), 0, st, a);
+    return;
+  }
+  const dim3 grid(a.parts * a.B);
+  // (what no row can ask for is not launched)
+  const bool t_on = a.t_dev || a.t > 0.f, k_on = a.k_dev || (a.k > 0 && a.k < a.V);
+  const bool k_all = !a.k_dev && a.k > 0 && a.k < a.V, k_list = a.k_dev || (k_on && a.k <= a.k_list);
+  const bool p_on = a.p_dev || a.p < 1.f;
+  hipLaunchKernelGGL((sample_top_kernel<T>), grid, dim3(PART), 0, st, a);
+  if (t_on && (k_list || (p_on && !k_all))) hipLaunchKernelGGL((sample_gather_kernel<T>), grid, dim3(PART), 0, st, a);
+  if (t_on && !k_all) hipLaunchKernelGGL((sample_sums_kernel<T>), grid, dim3(PART), 0, st, a);
+  hipLaunchKernelGGL((sample_finish_kernel<T, true>), dim3(a.B), dim3(FIN), 0, st, a);
 }
 
 }  // namespace
@@ -227,7 +826,12 @@ __global__ __launch_bounds__(THREADS) void sample_kernel(SampleArgs a) {
 
 using namespace da;
 
-extern "C" size_t da_sample_workspace_bytes(int, int, int) { return 0; }
+extern "C" size_t da_sample_workspace_bytes(int B, int V, int dtype) {
+  if (B < 1 || B > MAX_B || V < 1 || V > MAX_V || (dtype != DA_BF16 && dtype != DA_FP16 && dtype != DA_FP32)) return 0;
+  Plan p;
+  plan_for(p, B, V, dtype);
+  return p.bytes;
+}
 
 extern "C" int da_sample(const da_sample_args* x, void* stream) {
   if (!x) return DA_ERR_INVALID_ARG;
@@ -239,6 +843,10 @@ extern "C" int da_sample(const da_sample_args* x, void* stream) {
       ((uintptr_t)x->logprobs & 3) || ((uintptr_t)x->temperature_dev & 3) || ((uintptr_t)x->top_k_dev & 3) ||
       ((uintptr_t)x->top_p_dev & 3) || ((uintptr_t)x->min_p_dev & 3))
     return DA_ERR_ALIGNMENT;
+  Plan p;
+  plan_for(p, x->B, x->V, x->dtype);
+  if (p.bytes > 0 && (!x->workspace || x->workspace_bytes < (int64_t)p.bytes)) return DA_ERR_WORKSPACE;
+  if (!aligned16(x->workspace)) return DA_ERR_ALIGNMENT;
   SampleArgs a{};
   a.x = x->logits;
   a.x_b = x->row_stride;
@@ -253,11 +861,21 @@ extern "C" int da_sample(const da_sample_args* x, void* stream) {
   a.bits = 62;
   while (1 << (62 - a.bits) < x->V) --a.bits;
   if (a.bits > 45) a.bits = 45;
+  a.parts = p.parts, a.tiles = p.tiles;
+  a.f_parts = make_fastdiv(p.parts > 0 ? p.parts : 1);
+  a.groups = p.groups, a.lanes = p.lanes;
+  a.k_list = p.parts * p.groups / 4 * 3;
+  char* ws = (char*)x->workspace;
+  a.part = (Part*)(ws + p.part);
+  a.maxima = (uint32_t*)(ws + p.maxima);
+  a.count = (uint32_t*)(ws + p.count);
+  a.hist = (uint64_t*)(ws + p.hist);
+  a.list = (uint64_t*)(ws + p.list);
+  a.tile = (uint64_t*)(ws + p.tile);
   (void)hipGetLastError();
-  const dim3 grid(x->B), block(THREADS);
   hipStream_t st = (hipStream_t)stream;
-  if (x->dtype == DA_BF16) hipLaunchKernelGGL((sample_kernel<__bf16>), grid, block, 0, st, a);
-  else if (x->dtype == DA_FP16) hipLaunchKernelGGL((sample_kernel<_Float16>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((sample_kernel<float>), grid, block, 0, st, a);
+  if (x->dtype == DA_BF16) launch<__bf16>(a, st);
+  else if (x->dtype == DA_FP16) launch<_Float16>(a, st);
+  else launch<float>(a, st);
   return hipGetLastError() == hipSuccess ? DA_OK : DA_ERR_LAUNCH;
 }
