@@ -28,8 +28,8 @@
 //   sums    (rows without a list) the kept weight of every tile of 64 vectors;
 //           with top_p the tokens of the one bin at which the histogram reaches p
 //           are gathered in a list, those of larger logits are kept
-//   finish  a workgroup a row: the list sorted, the last token kept, the tile at
-//           which the sum passes u times the total, and the token in it
+//   finish  a workgroup a row: the last token kept, by histograms over the list;
+//           the tile at which the sum passes u times the total, and the token in it
 // Short rows take the last launch alone, the whole row their list.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -49,7 +49,7 @@ constexpr int MAX_V = 1 << 24;               // tokens of a vocabulary
 constexpr int MAX_B = 0x3fffff;              // rows (four parts each: threads of a grid below 2^32)
 constexpr uint32_t KEY_NONE = 0x007fffffu;   // -inf's key: candidates lie above it
 constexpr int PART = 256;                    // threads of a part
-constexpr int LIST = 4096;                   // tokens of a row's list
+constexpr int LIST = 3584;                   // tokens of a row's list (two finishing workgroups' LDS a CU)
 constexpr int BINS = 768;                    // of a part's histogram
 constexpr int GROUPS = 2048;                 // group maxima of a row at most
 constexpr int FIN = 512;                     // threads of the finish
@@ -74,12 +74,13 @@ struct SampleArgs {
   int B, V, bits;                           // weights in units of 2^-bits
   int parts, tiles, k_list;                 // parts of a row, tiles of a part, the largest top_k with a list
   FastDiv f_parts;
+  int runs;                                 // whether rows may take a histogram
   int groups, lanes;                        // group maxima of a part, lanes of a group
   // workspace, by row
   Part* part;                               // [parts]
   uint32_t* maxima;                         // [parts * groups]
   uint32_t* count;                          // tokens gathered (also past the list's end)
-  uint64_t* hist;                           // [parts, BINS]
+  uint64_t* hist;                           // [BINS]
   uint64_t* list;                           // [LIST] places
   uint64_t* tile;                           // [parts * tiles] kept weight
 };
@@ -102,7 +103,7 @@ __device__ __forceinline__ float logit_of(uint64_t place) { return of_key(place 
 // series to the 13th term (2^-52 of it), the whole one by the exponent; rounded
 // to an integer by what 2^52 leaves of it.
 __device__ __forceinline__ uint64_t weight_of(double t, int bits) {
-  t = fmax(t, -200.0);                      // (2^-200 of the largest: none; also of what is no number)
+  t = fmax(t, -200.0);                      // (2^-200 of the largest: none; so is what is no candidate)
   const double n = rint(t), f = (t - n) * 0.693147180559945309417;
   double p = 1.0 / 479001600;
   constexpr double c[] = {1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720,
@@ -125,7 +126,7 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int b) {
   s.k = a.k_dev ? a.k_dev[b * a.k_step] : a.k;
   s.p = a.p_dev ? a.p_dev[b * a.p_step] : a.p;
   s.m = a.m_dev ? a.m_dev[b * a.m_step] : a.m;
-  s.greedy = !(s.t > 0.f);
+  s.greedy = !(s.t > 0.f) || s.m > 1.f;     // (a min_p above 1 leaves the first token alone)
   s.cut = s.k > 0 && s.k < a.V;
   s.list = s.cut && s.k <= a.k_list;
   s.run = s.p < 1.f;
@@ -135,30 +136,34 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int b) {
 // The weights of a row with a candidate, and the bins of its histogram: linear in
 // the logit, from the largest to where weights vanish or the smallest candidate.
 struct Scale {
-  double top, per, bar;
-  float topf, step;
+  double top, per;
+  float topf, step, bar;                    // bar: min_p's, the smallest float at or above it
   int bits;
-  uint64_t first;
-  __device__ __forceinline__ Scale(const SampleArgs& a, const Setting& s, uint64_t first_, uint32_t least) {
-    first = first_;
+  bool inf;                                 // an infinite largest logit: the tokens at it share the row
+  __device__ __forceinline__ Scale(const SampleArgs& a, const Setting& s, uint64_t first, uint32_t least) {
     bits = a.bits;
     topf = logit_of(first);
-    top = topf;
+    inf = topf == INFINITY;
     per = 1.44269504088896340736 / (double)s.t;
-    bar = s.m > 0.f ? top + (double)s.t * log((double)s.m) : -INFINITY;
-    const double far = a.bits + 2, all = (top - (double)of_key(least)) * per;
+    bar = -INFINITY;
+    if (s.m > 0.f) {
+      double y = s.m < 1.f ? (double)topf + (double)s.t * log((double)s.m) : (double)topf;
+      if (y != y) y = topf;                 // (an infinite logit at an infinite temperature)
+      bar = (float)y;
+      if ((double)bar < y) bar = of_key(key_of(bar) + 1);
+    }
+    if (inf) topf = 0.f;
+    top = topf;
+    const double far = a.bits + 2, all = (top - (inf ? 0.0 : (double)of_key(least))) * per;
     const double range = all < far ? all : far;
     step = range > 0.0 ? (float)(BINS * (1.0 - 1.0 / 1024) / range * per) : 0.f;
   }
-  // (an infinite top: the tokens at it share the row)
-  __device__ __forceinline__ uint64_t weight(float y) const {
-    return weight_of(y == topf ? 0.0 : ((double)y - top) * per, bits);
+  // logits as the two below take them
+  __device__ __forceinline__ float at(float y) const { return !inf ? y : y == INFINITY ? 0.f : -INFINITY; }
+  __device__ __forceinline__ uint64_t weight(float z) const { return weight_of(((double)z - top) * per, bits); }
+  __device__ __forceinline__ int bin(float z) const {   // BINS: no weight
+    return (int)fminf((topf - z) * step, (float)BINS);
   }
-  __device__ __forceinline__ int bin(float y) const {   // BINS and above: no weight
-    const float f = (topf - y) * step;
-    return y == topf ? 0 : topf == INFINITY ? BINS : (int)fminf(f, (float)BINS);
-  }
-  __device__ __forceinline__ bool clears(float y, uint64_t place) const { return (double)y >= bar || place == first; }
 };
 
 // A row as 16-byte vectors from the aligned address at or before its start; what
@@ -294,6 +299,8 @@ __global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
   __shared__ uint32_t s_least[PART / 64];
   const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   if (part == 0 && threadIdx.x == 0) a.count[b] = 0;
+  if (a.runs)
+    for (int i = part * PART + threadIdx.x; i < BINS; i += a.parts * PART) a.hist[(int64_t)b * BINS + i] = 0;
   const R row(a, b);
   float most = -INFINITY, least = INFINITY;
   int at = 0;                               // the vector that raised `most` last
@@ -307,8 +314,10 @@ __global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
     float top = y[0];
 #pragma unroll
     for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);   // (a NaN gives way)
+    if (a.runs) {
 #pragma unroll
-    for (int e = 0; e < R::E; ++e) least = fminf(least, y[e] > -INFINITY ? y[e] : INFINITY);
+      for (int e = 0; e < R::E; ++e) least = fminf(least, y[e] > -INFINITY ? y[e] : INFINITY);
+    }
     if (top > most) {
       most = top;
       at = v;
@@ -388,19 +397,25 @@ __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
       if (n >= s.k) low = c;
     }
     const uint32_t from = max(low << 16, KEY_NONE + 1);
+    const float bar = of_key(from);
     if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
 #pragma unroll 4
     for (int j = 0; j < a.tiles; j += PART / 64) {
       const int v = v0 + j * 64;
       if (v >= row.n_vec) break;
-      row.each(v, [&](float y, int i) __attribute__((always_inline)) {
-        const uint32_t k = key_of(y);
-        if (k >= from) {
+      float y[R::E];
+      row.unpack(row.load(v), v, y);
+      float top = y[0];
+#pragma unroll
+      for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);
+      if (!(top >= bar)) continue;          // (most vectors)
+#pragma unroll
+      for (int e = 0; e < R::E; ++e)
+        if (y[e] >= bar) {
           const uint32_t at = atomicAdd(&s_n, 1u);
-          if (at < LIST) s_mem[at] = place_of(k, i);
+          if (at < LIST) s_mem[at] = place_of(key_of(y[e]), row.index(v, e));
         }
-      });
     }
     __syncthreads();
     append(a, b, s_mem, s_n, &s_at);
@@ -412,29 +427,35 @@ __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
   for (int j = 0; j < a.tiles; j += PART / 64) {
     const int v = v0 + j * 64;
     if (v >= row.n_vec) break;
-    row.each(v, [&](float y, int) __attribute__((always_inline)) {
-      if (!(y > -INFINITY)) return;
-      const int at = sc.bin(y);
-      if (at < BINS) atomicAdd((ull*)&s_mem[at], (ull)sc.weight(y));
-    });
+    float y[R::E];
+    uint64_t w[R::E];
+    row.unpack(row.load(v), v, y);
+    // (all weights first: their chains of 64-bit operations run beside each other)
+#pragma unroll
+    for (int e = 0; e < R::E; ++e) w[e] = sc.weight(sc.at(y[e]));
+#pragma unroll
+    for (int e = 0; e < R::E; ++e) {
+      const int at = sc.bin(sc.at(y[e]));
+      if (at < BINS) atomicAdd((ull*)&s_mem[at], (ull)w[e]);
+    }
   }
   __syncthreads();
-  uint64_t* to = a.hist + ((int64_t)b * a.parts + part) * BINS;
-  for (int i = threadIdx.x; i < BINS; i += PART) to[i] = s_mem[i];
+  ull* to = (ull*)a.hist + (int64_t)b * BINS;
+  for (int i = threadIdx.x; i < BINS; i += PART)
+    if (s_mem[i]) atomicAdd(to + i, (ull)s_mem[i]);
 }
 
 // The bin at which a row's histogram reaches p times its total, the weight of
-// those before it and what is to be reached. s: BINS / 3 + 8 words.
+// those before it and what is to be reached.
 template <int N>
 __device__ __forceinline__ int border_bin(const SampleArgs& a, int b, float p, uint64_t* s, uint64_t& before, uint64_t& goal) {
   constexpr int PER = BINS / 256;           // bins of a thread
   static_assert(BINS % 256 == 0 && N >= 256, "256 threads hold the bins");
   uint64_t sum[PER] = {}, mine = 0, total;
   if (threadIdx.x < 256) {
-    const uint64_t* h = a.hist + (int64_t)b * a.parts * BINS + threadIdx.x * PER;
-    for (int i = 0; i < a.parts; ++i)
+    const uint64_t* h = a.hist + (int64_t)b * BINS + threadIdx.x * PER;
 #pragma unroll
-      for (int e = 0; e < PER; ++e) sum[e] += h[(int64_t)i * BINS + e];
+    for (int e = 0; e < PER; ++e) sum[e] = h[e];
 #pragma unroll
     for (int e = 0; e < PER; ++e) mine += sum[e];
   }
@@ -479,20 +500,45 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
   for (int j = 0; j < a.tiles; j += PART / 64) {
     const int tile = part * a.tiles + j + wave, v = tile * 64 + lane;
     if (tile * 64 >= row.n_vec) break;
+    float y[R::E];
     uint64_t sum = 0;
-    if (v < row.n_vec)
-      row.each(v, [&](float y, int i) __attribute__((always_inline)) {
-        if (!(y > -INFINITY)) return;
-        const int at = sc.bin(y);
-        if (at > border) return;
-        const uint64_t place = place_of(key_of(y), i);
-        if (at == border && s.run) {
-          const uint32_t n = atomicAdd(&s_n, 1u);
-          if (n < LIST) s_list[n] = place;
-        } else if (at < BINS && sc.clears(y, place)) {
-          sum += sc.weight(y);
+    row.unpack(row.load(v), v, y);
+    if (s.run) {
+      bool listed = false, any = false;
+      int at[R::E];
+#pragma unroll
+      for (int e = 0; e < R::E; ++e) {
+        at[e] = sc.bin(sc.at(y[e]));
+        listed |= at[e] == border;
+        any |= at[e] < border;
+      }
+      if (__any(any)) {
+#pragma unroll
+        for (int e = 0; e < R::E; ++e) {
+          const uint64_t w = sc.weight(sc.at(y[e]));
+          sum += at[e] < border && y[e] >= sc.bar ? w : 0;
         }
-      });
+      }
+      if (listed) {
+#pragma unroll
+        for (int e = 0; e < R::E; ++e)
+          if (at[e] == border) {
+            const uint32_t n = atomicAdd(&s_n, 1u);
+            if (n < LIST) s_list[n] = place_of(key_of(y[e]), row.index(v, e));
+          }
+      }
+    } else {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < R::E; ++e) any |= y[e] >= sc.bar;
+      if (__any(any)) {
+#pragma unroll
+        for (int e = 0; e < R::E; ++e) {
+          const uint64_t w = sc.weight(sc.at(y[e]));
+          sum += y[e] >= sc.bar ? w : 0;
+        }
+      }
+    }
     sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
     if (lane == 0) a.tile[(int64_t)b * a.parts * a.tiles + tile] = sum;
   }
@@ -501,27 +547,46 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
 }
 
 // ---------------------------------------------------------------------------
-// Sorts s[0 .. n2), the largest first (n2 a power of two).
-__device__ __forceinline__ void sort_down(uint64_t* s, int n2) {
-  for (int k = 2; k <= n2; k *= 2)
-    for (int j = k / 2; j > 0; j /= 2) {
-      __syncthreads();
-      for (int t = threadIdx.x; t < n2 / 2; t += FIN) {
-        const int i = (t & ~(j - 1)) * 2 | (t & (j - 1));
-        const uint64_t p = s[i], q = s[i + j];
-        if (((i & k) == 0) == (p < q)) {
-          s[i] = q;
-          s[i + j] = p;
-        }
-      }
-    }
+// The largest of the n values (each from 1 on, below 2^63 apart from one another) at
+// which the measure, summed from the largest value down, reaches `goal`; 0 if it does
+// nowhere. Nine bits of the values' range at a time, by histograms. s: FIN bins and 16
+// words.
+template <typename V, typename M>
+__device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_t lo, uint64_t hi, uint64_t goal, uint64_t* s) {
+  uint64_t* s_scan = s + FIN;
+  const int tid = threadIdx.x;
   __syncthreads();
+  for (;;) {
+    const int bits = 64 - __clzll((long long)((hi - lo) | 1)), shift = bits > 9 ? bits - 9 : 0;
+    s[tid] = 0;
+    __syncthreads();
+    for (int i = tid; i < n; i += FIN) {
+      const uint64_t x = value(i);
+      if (x >= lo && x <= hi) atomicAdd((ull*)&s[(x - lo) >> shift], (ull)measure(i));
+    }
+    __syncthreads();
+    uint64_t total;
+    const uint64_t mine = s[FIN - 1 - tid], before = block_before<FIN>(mine, s_scan, total);
+    __syncthreads();
+    if (tid == 0) s_scan[8] = 0;
+    __syncthreads();
+    if (before < goal && before + mine >= goal) {
+      s_scan[8] = FIN - tid;                // the bin and 1
+      s_scan[9] = before;
+    }
+    __syncthreads();
+    if (s_scan[8] == 0) return 0;
+    goal -= s_scan[9];
+    lo += (s_scan[8] - 1) << shift;
+    if (shift == 0) return lo;
+    if ((hi - lo) >> shift) hi = lo + ((uint64_t)1 << shift) - 1;
+  }
 }
 
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
   using R = Row<T>;
-  __shared__ uint64_t s_list[LIST], s_slot[SLOTS], s_scan[16], s_found[3];
+  __shared__ uint64_t s_list[LIST], s_w[LIST], s_slot[SPLIT ? SLOTS : 1], s_scan[FIN + 16], s_found[3];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
   const Setting s = setting_of(a, b);
   const R row(a, b);
@@ -535,6 +600,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     for (int v = tid; v < row.n_vec; v += FIN)
       row.each(v, [&](float y, int i) __attribute__((always_inline)) {
         const uint64_t place = place_of(key_of(y), i);
+        if (i >= 0 && i < a.V) s_list[i] = place;
         first = place > first ? place : first;
       });
     first = block_reduce<FIN>(first, s_scan, Most());
@@ -548,8 +614,9 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     return;
   }
   const Scale sc(a, s, first, SPLIT ? least : KEY_NONE + 1);
+  auto weight = [&](uint64_t place) __attribute__((always_inline)) { return sc.weight(sc.at(logit_of(place))); };
   auto drawn = [&](float y, int i, uint64_t total) __attribute__((always_inline)) {
-    const double d = y == sc.topf ? 0.0 : ((double)y - sc.top) / (double)s.t;
+    const double d = ((double)sc.at(y) - sc.top) / (double)s.t;
     done(i, (float)(d - log(ldexp((double)total, -a.bits))));
   };
   auto aim_of = [&](uint64_t total) __attribute__((always_inline)) {
@@ -557,74 +624,44 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     return aim < total ? aim : total - 1;
   };
 
-  // the row's kept tokens as a list of their own?
-  const bool whole = SPLIT ? s.list && n_cand <= LIST : a.V <= LIST;
+  // a list that holds all that is kept?
+  const bool whole = SPLIT ? s.list && n_cand <= LIST : true;
   if (whole) {
-    int n;
-    if constexpr (SPLIT) {
-      n = (int)n_cand;
-      for (int i = tid; i < n; i += FIN) s_list[i] = a.list[(int64_t)b * LIST + i];
-    } else {
-      n = a.V;
-      for (int v = tid; v < row.n_vec; v += FIN)
-        row.each(v, [&](float y, int i) __attribute__((always_inline)) {
-          if (i >= 0 && i < a.V) s_list[i] = place_of(key_of(y), i);
-        });
+    const int n = SPLIT ? (int)n_cand : a.V;
+    for (int i = tid; i < n; i += FIN) {
+      const uint64_t place = SPLIT ? a.list[(int64_t)b * LIST + i] : s_list[i];
+      if constexpr (SPLIT) s_list[i] = place;
+      s_w[i] = place ? weight(place) : 0;
     }
-    int n2 = 2;
-    while (n2 < n) n2 *= 2;
-    for (int i = n + tid; i < n2; i += FIN) s_list[i] = 0;
     __syncthreads();
-    const int per = (n2 + FIN - 1) / FIN, at0 = tid * per, at1 = min(at0 + per, n2);
-    auto mass = [&](int end) __attribute__((always_inline)) {
+    auto place = [&](int i) __attribute__((always_inline)) { return s_list[i]; };
+    auto total_of = [&](auto&& kept) __attribute__((always_inline)) {
       uint64_t sum = 0;
-      for (int i = at0; i < min(at1, end); ++i) sum += s_list[i] ? sc.weight(logit_of(s_list[i])) : 0;
-      return sum;
+      for (int i = tid; i < n; i += FIN) sum += kept(i) ? s_w[i] : 0;
+      return block_reduce<FIN>(sum, s_scan, Plus());
     };
-    const bool filter = s.cut || s.run || s.m > 0.f;
-    uint64_t total;
-    if (filter) {
-      sort_down(s_list, n2);
-      if (s.cut) n = min(n, s.k);
-      uint64_t before = block_before<FIN>(mass(n), s_scan, total);
-      const uint64_t goal = s.run ? part_of(s.p, total, true) : ~0ull;
-      int keep = 0;
-      for (int i = at0; i < min(at1, n); ++i) {
-        const uint64_t place = s_list[i];
-        if (place == 0) break;
-        if (i == 0 || (before < goal && sc.clears(logit_of(place), place))) ++keep;
-        before += sc.weight(logit_of(place));
-      }
-      n = (int)block_reduce<FIN>(keep, s_scan, Plus());
-      // by index: the first one the largest number
-      n2 = 2;
-      while (n2 < n) n2 *= 2;
-      __syncthreads();
-      for (int i = tid; i < n2; i += FIN) {
-        const uint64_t place = s_list[i];
-        s_list[i] = i < n ? place << 32 | place >> 32 : 0;
-      }
-      sort_down(s_list, n2);
-      for (int i = tid; i < n2; i += FIN) {
-        const uint64_t place = s_list[i];
-        s_list[i] = place << 32 | place >> 32;
-      }
-      __syncthreads();
+    uint64_t last = 1;                      // the last place kept
+    if (s.cut) {
+      const uint64_t at = reach(n, place, [](int) { return (uint64_t)1; }, last, first, s.k, s_scan);
+      if (at) last = at;                    // (0: there are fewer)
     }
-    uint64_t before = block_before<FIN>(mass(n), s_scan, total);
-    const uint64_t aim = aim_of(total);
-    for (int i = at0; i < min(at1, n); ++i) {
-      const uint64_t place = s_list[i];
-      const uint64_t upto = before + (place ? sc.weight(logit_of(place)) : 0);
-      if (before <= aim && upto > aim) drawn(logit_of(place), index_of(place), total);
-      before = upto;
+    if (s.run) {
+      const uint64_t goal = part_of(s.p, total_of([&](int i) { return s_list[i] >= last; }), true);
+      last = goal <= 1 ? first : reach(n, place, [&](int i) { return s_w[i]; }, last, first, goal, s_scan);
     }
+    auto kept = [&](int i) __attribute__((always_inline)) { return s_list[i] >= last && logit_of(s_list[i]) >= sc.bar; };
+    const uint64_t total = total_of(kept), aim = aim_of(total);
+    // by index: the first one is the largest number
+    auto turned = [&](int i) __attribute__((always_inline)) { return kept(i) ? (uint64_t)(uint32_t)s_list[i] : 0; };
+    const uint64_t at = reach(n, turned, [&](int i) { return s_w[i]; }, (uint32_t)~(a.V - 1), ~0u, aim + 1, s_scan);
+    for (int i = tid; i < n; i += FIN)
+      if (turned(i) == at) drawn(logit_of(s_list[i]), index_of(s_list[i]), total);
     return;
   }
-  if constexpr (!SPLIT) return;             // (rows of one launch fit the list)
+  if constexpr (SPLIT) {
 
   uint64_t last = 1;                        // the last place kept
-  int border = BINS;                        // the bin of `last`: the bins before it are kept whole
+  int border = BINS;                        // its bin: those before it are kept whole
   const int tiles = (row.n_vec + 63) / 64, per = (tiles + SLOTS - 1) / SLOTS;   // tiles of a slot
   const bool ready = s.sums() && (!s.run || n_cand <= LIST);   // by the launches before
   for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
@@ -632,27 +669,18 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
   if (ready) {
     const uint64_t* sums = a.tile + (int64_t)b * a.parts * a.tiles;
     if (s.run) {
-      uint64_t before, goal, total;
+      uint64_t before, goal;
       border = border_bin<FIN>(a, b, s.p, s_scan, before, goal);
-      int n = (int)n_cand, n2 = 2;
-      while (n2 < n) n2 *= 2;
-      for (int i = tid; i < n2; i += FIN) s_list[i] = i < n ? a.list[(int64_t)b * LIST + i] : 0;
-      sort_down(s_list, n2);
-      const int share = (n2 + FIN - 1) / FIN, at0 = tid * share, at1 = min(at0 + share, n);
-      uint64_t sum = 0;
-      for (int i = at0; i < at1; ++i) sum += sc.weight(logit_of(s_list[i]));
-      before += block_before<FIN>(sum, s_scan, total);
-      int keep = 0;
-      for (int i = at0; i < at1; ++i) {
-        const uint64_t place = s_list[i], w = sc.weight(logit_of(place));
-        if (place == first || (before < goal && sc.clears(logit_of(place), place))) {
-          ++keep;
-          atomicAdd((ull*)&s_slot[(index_of(place) + row.shift) / R::E / 64 / per], (ull)w);
-        }
-        before += w;
+      const int n = (int)n_cand;
+      for (int i = tid; i < n; i += FIN) {
+        s_list[i] = a.list[(int64_t)b * LIST + i];
+        s_w[i] = weight(s_list[i]);
       }
-      n = (int)block_reduce<FIN>(keep, s_scan, Plus());
-      last = n > 0 ? s_list[n - 1] : ~0ull;
+      __syncthreads();
+      last = reach(n, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, last, first, goal - before, s_scan);
+      for (int i = tid; i < n; i += FIN)
+        if (s_list[i] >= last && logit_of(s_list[i]) >= sc.bar)
+          atomicAdd((ull*)&s_slot[(index_of(s_list[i]) + row.shift) / R::E / 64 / per], (ull)s_w[i]);
     }
     for (int i = tid; i < tiles; i += FIN) {
       const uint64_t w = sums[i];
@@ -665,7 +693,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     auto over = [&](auto&& f) {
       for (int v = tid; v < row.n_vec; v += FIN) row.each(v, f);
     };
-    auto reach = [&](auto&& measure, uint64_t goal) {
+    auto far = [&](auto&& measure, uint64_t goal) {
       uint64_t prefix = 0, before = 0;
       for (int low = 55; low >= 0; low -= 11) {
         for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
@@ -689,22 +717,23 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
         prefix = s_found[0];
         before = s_found[1];
         if (s_found[2] < goal) return (uint64_t)0;   // (fewer than that)
+        __syncthreads();
       }
       return prefix;
     };
+    auto mass = [&](float y) __attribute__((always_inline)) { return sc.weight(sc.at(y)); };
     if (s.cut) {
-      const uint64_t at = reach([](float) { return (uint64_t)1; }, s.k);
+      const uint64_t at = far([](float) { return (uint64_t)1; }, s.k);
       if (at) last = at;
     }
     if (s.run) {
       uint64_t sum = 0;
       over([&](float y, int i) __attribute__((always_inline)) {
-        if (place_of(key_of(y), i) >= last) sum += sc.weight(y);
+        if (place_of(key_of(y), i) >= last) sum += mass(y);
       });
       sum = block_reduce<FIN>(sum, s_scan, Plus());
       const uint64_t goal = part_of(s.p, sum, true);
-      const uint64_t at = goal <= 1 ? first : reach([&](float y) { return sc.weight(y); }, goal);
-      if (at) last = at;
+      last = goal <= 1 ? first : far(mass, goal);
     }
     border = -1;                            // (by place alone)
     for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
@@ -713,8 +742,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
       uint64_t sum = 0;
       if (v < row.n_vec)
         row.each(v, [&](float y, int i) __attribute__((always_inline)) {
-          const uint64_t place = place_of(key_of(y), i);
-          if (place >= last && sc.clears(y, place)) sum += sc.weight(y);
+          if (place_of(key_of(y), i) >= last && y >= sc.bar) sum += mass(y);
         });
       sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
       if (lane == 0 && sum) atomicAdd((ull*)&s_slot[v / 64 / per], (ull)sum);
@@ -745,10 +773,10 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     row.unpack(row.load(v), v, y);
 #pragma unroll
     for (int e = 0; e < R::E; ++e) {
-      const uint64_t place = place_of(key_of(y[e]), row.index(v, e));
-      const int at = place ? sc.bin(y[e]) : BINS;
-      w[e] = place && (border < 0 ? place >= last : border == BINS ? at < BINS : at < border || (at == border && place >= last)) &&
-                     sc.clears(y[e], place) ? sc.weight(y[e]) : 0;
+      const uint64_t place = place_of(key_of(y[e]), row.index(v, e)), z = sc.weight(sc.at(y[e]));
+      const int at = sc.bin(sc.at(y[e]));
+      const bool in = border < 0 ? place >= last : border == BINS || at < border || (at == border && place >= last);
+      w[e] = in && y[e] >= sc.bar ? z : 0;
       sum += w[e];
     }
     const uint64_t upto = scan64(sum);
@@ -764,6 +792,8 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
       return;
     }
     before += last_lane(upto);
+  }
+
   }
 }
 
@@ -798,14 +828,14 @@ void plan_for(Plan& p, int B, int V, int dtype) {
   p.part = room(sizeof(Part) * p.parts);
   p.maxima = room(sizeof(uint32_t) * p.parts * p.groups);
   p.count = room(sizeof(uint32_t));
-  p.hist = room(sizeof(uint64_t) * p.parts * BINS);
+  p.hist = room(sizeof(uint64_t) * BINS);
   p.list = room(sizeof(uint64_t) * LIST);
   p.tile = room(sizeof(uint64_t) * p.parts * p.tiles);
   p.bytes = at;
 }
 
 template <typename T>
-void launch(const SampleArgs& a, hipStream_t st) {
+void launch(SampleArgs& a, hipStream_t st) {
   if (a.parts == 0) {
     hipLaunchKernelGGL((sample_finish_kernel<T, false>), dim3(a.B), dim3(FIN), 0, st, a);
     return;
@@ -815,6 +845,7 @@ void launch(const SampleArgs& a, hipStream_t st) {
   const bool t_on = a.t_dev || a.t > 0.f, k_on = a.k_dev || (a.k > 0 && a.k < a.V);
   const bool k_all = !a.k_dev && a.k > 0 && a.k < a.V, k_list = a.k_dev || (k_on && a.k <= a.k_list);
   const bool p_on = a.p_dev || a.p < 1.f;
+  a.runs = t_on && p_on && !k_all;
   hipLaunchKernelGGL((sample_top_kernel<T>), grid, dim3(PART), 0, st, a);
   if (t_on && (k_list || (p_on && !k_all))) hipLaunchKernelGGL((sample_gather_kernel<T>), grid, dim3(PART), 0, st, a);
   if (t_on && !k_all) hipLaunchKernelGGL((sample_sums_kernel<T>), grid, dim3(PART), 0, st, a);

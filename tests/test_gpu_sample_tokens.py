@@ -175,6 +175,42 @@ def test_equal_logits_are_taken_by_index(gpu):
     check(x[:64], uniform(64, 8), sure=False, top_k=13)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_long_rows_of_few_values(gpu, dtype):
+    """More equal logits than a list holds, at the border of top_k, of top_p, of
+    both; by index, exactly."""
+    from delta_attention import ops
+    V, n = 65536, 512
+    x = torch.zeros(1, V, device="cuda", dtype=DT[dtype]).expand(n, V)
+    u = (torch.arange(n, device="cuda").float() + 0.5) / n
+    at = (torch.arange(n, device="cuda").double() + 0.5) / n
+    for kept, s in ((V, dict()), (V, dict(top_k=0, min_p=1.0)), (512, dict(top_k=512)), (16384, dict(top_p=0.25)),
+                    (5000, dict(top_k=5000)), (4096, dict(top_k=8192, top_p=0.5)), (300, dict(top_k=600, top_p=0.5))):
+        t, lp = ops.sample_tokens(x, u, **s)
+        assert torch.equal(t, (at * kept).floor().long()), s
+        assert (lp + math.log(kept)).abs().max().item() <= math.log(kept) * 2.0 ** -24 * 1.001 + 2 * off(V)
+    # two values, the larger one past the list too
+    y = torch.zeros(1, V, device="cuda", dtype=DT[dtype])
+    y[:, ::8] = 1.0
+    check(y.expand(40, V), uniform(40, 21), sure=False, top_p=0.5)
+    check(y.expand(40, V), uniform(40, 22), sure=False, top_k=10000)
+    check(y.expand(40, V), uniform(40, 23), sure=False, top_k=10000, top_p=0.9, temperature=0.5)
+
+
+def test_rows_around_the_list(gpu):
+    """Row lengths at which the launches change, and masks that leave fewer
+    candidates than top_k or than groups."""
+    for V in (3583, 3584, 3585, 4095, 4097, 5000, 9001):
+        x, u = logits(6, V, "bf16", V), uniform(6, V + 2)
+        x[1, 100:] = -math.inf
+        x[2, :] = -math.inf
+        x[2, V - 1] = 3.0
+        x[3, ::2] = math.nan
+        x[4, 7:] = torch.finfo(torch.bfloat16).min
+        for s in SETTINGS + [dict(top_k=700), dict(top_k=3000, top_p=0.9)]:
+            check(x, u, sure=False, **s)
+
+
 @pytest.mark.parametrize("V", [33, 40000])
 def test_the_ends_of_u(gpu, V):
     from delta_attention import ops
