@@ -99,17 +99,23 @@ __device__ __forceinline__ uint64_t place_of(uint32_t key, int i) {
 __device__ __forceinline__ int index_of(uint64_t place) { return (int)~(uint32_t)place; }
 __device__ __forceinline__ float logit_of(uint64_t place) { return of_key(place >> 32); }
 
-// 2^t for t <= 0 in units of 2^-bits (bits <= 45): the fraction's power by its
-// series to the 13th term (2^-52 of it), the whole one by the exponent; rounded
-// to an integer by what 2^52 leaves of it.
+// 2^t for t <= 0 in units of 2^-bits (bits <= 45): the fraction's power by the
+// polynomial of degree 10 that meets 2^f at the Chebyshev nodes of [-1/2, 1/2]
+// (2^-51 of it, rounding included; the series takes two terms more), the whole
+// one by the exponent; rounded to an integer by what 2^52 leaves of it.
 __device__ __forceinline__ uint64_t weight_of(double t, int bits) {
   t = fmax(t, -200.0);                      // (2^-200 of the largest: none; so is what is no candidate)
-  const double n = rint(t), f = (t - n) * 0.693147180559945309417;
-  double p = 1.0 / 479001600;
-  constexpr double c[] = {1.0 / 39916800, 1.0 / 3628800, 1.0 / 362880, 1.0 / 40320, 1.0 / 5040, 1.0 / 720,
-                          1.0 / 120, 1.0 / 24, 1.0 / 6, 0.5, 1.0, 1.0};
+  const double n = rint(t), f = t - n;
+  double p = 7.072585949269223e-09;
+  constexpr double c[] = {1.0208690299958306e-07, 1.321544258792169e-06, 1.5252657260200837e-05, 0.0001540353044173605,
+                          0.0013333558230164974, 0.009618129107606888, 0.05550410866444772, 0.24022650695910097,
+                          0.69314718055995, 1.0};
 #pragma unroll
-  for (int i = 0; i < 12; ++i) p = fma(p, f, c[i]);
+  for (int i = 0; i < 10; ++i) {
+    double k = c[i];
+    asm("" : "+s"(k));                      // (a scalar operand: else each term copies it first)
+    p = fma(p, f, k);
+  }
   return (uint64_t)__double_as_longlong(ldexp(p, (int)n + bits) + 4503599627370496.0) - 0x4330000000000000ull;
 }
 
@@ -164,6 +170,24 @@ struct Scale {
   __device__ __forceinline__ int bin(float z) const {   // BINS: no weight
     return (int)fminf((topf - z) * step, (float)BINS);
   }
+  template <int E>
+  __device__ __forceinline__ void at(const float (&y)[E], float (&z)[E]) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] = y[e];
+    if (inf) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] = at(y[e]);
+    }
+  }
+  // All of a vector's, whatever becomes of them: their chains of 64-bit operations
+  // run beside each other.
+  template <int E>
+  __device__ __forceinline__ void weights(const float (&z)[E], uint64_t (&w)[E]) const {
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = weight(z[e]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) asm("" : "+v"(w[e]));
+  }
 };
 
 // A row as 16-byte vectors from the aligned address at or before its start; what
@@ -174,9 +198,9 @@ struct Row {
   const u32x4* base;
   int shift, V, n_vec;
   __device__ __forceinline__ Row(const SampleArgs& a, int b) {
-    const uintptr_t p = (uintptr_t)((const T*)a.x + (int64_t)b * a.x_b);
-    base = (const u32x4*)(p & ~(uintptr_t)15);
-    shift = (int)(p & 15) / sizeof(T);
+    const T* p = (const T*)a.x + (int64_t)b * a.x_b;
+    shift = (int)((uintptr_t)p & 15) / sizeof(T);
+    base = (const u32x4*)(p - shift);
     V = a.V;
     n_vec = (V + shift + E - 1) / E;
   }
@@ -204,15 +228,35 @@ struct Row {
 #pragma unroll
     for (int e = 0; e < E; ++e) f(y[e], index(v, e));
   }
+  // f(vector, logits) of this lane's vectors of a part's tiles, wave w of W every
+  // W-th tile, U loads ahead
+  template <int W, int U, typename F>
+  __device__ __forceinline__ void sweep(int tile0, int tiles, F&& f) const {
+    const int first = tile0 + (int)(threadIdx.x / 64), n = min(tiles - (int)(threadIdx.x / 64), (n_vec + 63) / 64 - first);
+    for (int j = 0; j < n; j += U * W) {
+      u32x4 w[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) w[u] = load((first + j + u * W) * 64 + (int)(threadIdx.x % 64));
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (j + u * W >= n) break;
+        const int v = (first + j + u * W) * 64 + (int)(threadIdx.x % 64);
+        float y[E];
+        unpack(w[u], v, y);
+        f(v, y);
+      }
+    }
+  }
 };
 
-// Sum over the lanes up to this one.
-__device__ __forceinline__ uint64_t scan64(uint64_t x) {
+// op over the lanes up to this one, with 0 beside them.
+template <typename F>
+__device__ __forceinline__ uint64_t lanes_upto(uint64_t x, F&& op) {
   auto step = [&](auto ctrl, auto rows) __attribute__((always_inline)) {
     constexpr int C = decltype(ctrl)::value, R = decltype(rows)::value;
     const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)x, C, R, 0xf, false);
     const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(x >> 32), C, R, 0xf, false);
-    x += (uint64_t)hi << 32 | lo;
+    x = op(x, (uint64_t)hi << 32 | lo);
   };
   using std::integral_constant;
   step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});   // row_shr 1, 2, 4, 8
@@ -223,28 +267,32 @@ __device__ __forceinline__ uint64_t scan64(uint64_t x) {
   step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
   return x;
 }
-__device__ __forceinline__ uint64_t last_lane(uint64_t x) {
-  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(x >> 32), 63) << 32 |
-         (uint32_t)__builtin_amdgcn_readlane((uint32_t)x, 63);
-}
-
-template <int N, typename F>
-__device__ __forceinline__ uint64_t block_reduce(uint64_t v, uint64_t* s, F&& f) {
-  for (int d = 32; d > 0; d /= 2) v = f(v, __shfl_xor(v, d));
-  __syncthreads();
-  if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = v;
-  __syncthreads();
-  v = s[0];
-#pragma unroll
-  for (int w = 1; w < N / 64; ++w) v = f(v, s[w]);
-  return v;
-}
 struct Most {
   __device__ __forceinline__ uint64_t operator()(uint64_t p, uint64_t q) const { return p > q ? p : q; }
 };
 struct Plus {
   __device__ __forceinline__ uint64_t operator()(uint64_t p, uint64_t q) const { return p + q; }
 };
+__device__ __forceinline__ uint64_t scan64(uint64_t x) { return lanes_upto(x, Plus()); }
+__device__ __forceinline__ uint64_t last_lane(uint64_t x) {
+  return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((uint32_t)(x >> 32), 63) << 32 |
+         (uint32_t)__builtin_amdgcn_readlane((uint32_t)x, 63);
+}
+template <typename F>
+__device__ __forceinline__ uint64_t wave_all(uint64_t x, F&& op) { return last_lane(lanes_upto(x, op)); }
+
+// op over the workgroup's N threads (0 beside them). s: N / 64 words.
+template <int N, typename F>
+__device__ __forceinline__ uint64_t block_all(uint64_t v, uint64_t* s, F&& op) {
+  v = lanes_upto(v, op);
+  __syncthreads();
+  if (threadIdx.x % 64 == 63) s[threadIdx.x / 64] = v;
+  __syncthreads();
+  v = s[0];
+#pragma unroll
+  for (int w = 1; w < N / 64; ++w) v = op(v, s[w]);
+  return v;
+}
 
 // Sums of the threads before this one; `total` of all.
 template <int N>
@@ -284,11 +332,8 @@ __device__ __forceinline__ void row_ends(const SampleArgs& a, int b, uint64_t& f
     first = p[i].first > first ? p[i].first : first;
     least = min(least, p[i].least);
   }
-  for (int d = 32; d > 0; d /= 2) {
-    const uint64_t o = __shfl_xor(first, d);
-    first = o > first ? o : first;
-    least = min(least, (uint32_t)__shfl_xor((int)least, d));
-  }
+  first = wave_all(first, Most());
+  least = ~(uint32_t)wave_all(~least, Most());
 }
 
 // ---------------------------------------------------------------------------
@@ -304,13 +349,7 @@ __global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
   const R row(a, b);
   float most = -INFINITY, least = INFINITY;
   int at = 0;                               // the vector that raised `most` last
-  const int v0 = (part * a.tiles + wave) * 64 + lane;
-#pragma unroll 4
-  for (int j = 0; j < a.tiles; j += PART / 64) {
-    const int v = v0 + j * 64;
-    if (v >= row.n_vec) break;
-    float y[R::E];
-    row.unpack(row.load(v), v, y);
+  row.template sweep<PART / 64, 4>(part * a.tiles, a.tiles, [&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
     float top = y[0];
 #pragma unroll
     for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);   // (a NaN gives way)
@@ -322,7 +361,7 @@ __global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
       most = top;
       at = v;
     }
-  }
+  });
   const uint32_t key = key_of(most);
   uint64_t first = 0;
   if (key > KEY_NONE)
@@ -332,11 +371,8 @@ __global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
   uint32_t g = key, low = least < INFINITY ? key_of(least) : key > KEY_NONE ? key : ~0u;
   for (int d = 1; d < a.lanes; d *= 2) g = max(g, (uint32_t)__shfl_xor((int)g, d));
   if (threadIdx.x % a.lanes == 0) a.maxima[((int64_t)b * a.parts + part) * a.groups + threadIdx.x / a.lanes] = g;
-  for (int d = 32; d > 0; d /= 2) {
-    const uint64_t o = __shfl_xor(first, d);
-    first = o > first ? o : first;
-    low = min(low, (uint32_t)__shfl_xor((int)low, d));
-  }
+  first = wave_all(first, Most());
+  low = ~(uint32_t)wave_all(~low, Most());
   if (lane == 0) {
     s_first[wave] = first;
     s_least[wave] = low;
@@ -370,12 +406,7 @@ __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
   const Setting s = setting_of(a, b);
   const bool hist = s.sums() && s.run;
   if (s.greedy || (!s.list && !hist)) return;
-  uint64_t first;
-  uint32_t least;
-  row_ends(a, b, first, least);
-  if (first == 0) return;
   const R row(a, b);
-  const int v0 = (part * a.tiles + wave) * 64 + lane;
   if (s.list) {
     // The largest number of 16 bits that is no larger than the k-th group maximum's
     // first 16: bit by bit, by the count of maxima that reach it.
@@ -400,45 +431,40 @@ __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
     const float bar = of_key(from);
     if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
-#pragma unroll 4
-    for (int j = 0; j < a.tiles; j += PART / 64) {
-      const int v = v0 + j * 64;
-      if (v >= row.n_vec) break;
-      float y[R::E];
-      row.unpack(row.load(v), v, y);
+    row.template sweep<PART / 64, 4>(part * a.tiles, a.tiles, [&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
       float top = y[0];
 #pragma unroll
       for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);
-      if (!(top >= bar)) continue;          // (most vectors)
+      if (!(top >= bar)) return;            // (most vectors)
 #pragma unroll
       for (int e = 0; e < R::E; ++e)
         if (y[e] >= bar) {
           const uint32_t at = atomicAdd(&s_n, 1u);
           if (at < LIST) s_mem[at] = place_of(key_of(y[e]), row.index(v, e));
         }
-    }
+    });
     __syncthreads();
     append(a, b, s_mem, s_n, &s_at);
     return;
   }
+  uint64_t first;
+  uint32_t least;
+  row_ends(a, b, first, least);
+  if (first == 0) return;
   const Scale sc(a, s, first, least);
   for (int i = threadIdx.x; i < BINS; i += PART) s_mem[i] = 0;
   __syncthreads();
-  for (int j = 0; j < a.tiles; j += PART / 64) {
-    const int v = v0 + j * 64;
-    if (v >= row.n_vec) break;
-    float y[R::E];
+  row.template sweep<PART / 64, 2>(part * a.tiles, a.tiles, [&](int, const float (&y)[R::E]) __attribute__((always_inline)) {
+    float z[R::E];
     uint64_t w[R::E];
-    row.unpack(row.load(v), v, y);
-    // (all weights first: their chains of 64-bit operations run beside each other)
-#pragma unroll
-    for (int e = 0; e < R::E; ++e) w[e] = sc.weight(sc.at(y[e]));
+    sc.at(y, z);
+    sc.weights(z, w);
 #pragma unroll
     for (int e = 0; e < R::E; ++e) {
-      const int at = sc.bin(sc.at(y[e]));
+      const int at = sc.bin(z[e]);
       if (at < BINS) atomicAdd((ull*)&s_mem[at], (ull)w[e]);
     }
-  }
+  });
   __syncthreads();
   ull* to = (ull*)a.hist + (int64_t)b * BINS;
   for (int i = threadIdx.x; i < BINS; i += PART)
@@ -484,7 +510,7 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
   using R = Row<T>;
   __shared__ uint64_t s_list[LIST], s_scan[8];
   __shared__ uint32_t s_n, s_at;
-  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64;
   const Setting s = setting_of(a, b);
   if (!s.sums()) return;
   uint64_t first;
@@ -497,27 +523,23 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
   const R row(a, b);
-  for (int j = 0; j < a.tiles; j += PART / 64) {
-    const int tile = part * a.tiles + j + wave, v = tile * 64 + lane;
-    if (tile * 64 >= row.n_vec) break;
-    float y[R::E];
-    uint64_t sum = 0;
-    row.unpack(row.load(v), v, y);
+  row.template sweep<PART / 64, 2>(part * a.tiles, a.tiles, [&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
+    float z[R::E];
+    uint64_t sum = 0, w[R::E];
+    sc.at(y, z);
     if (s.run) {
       bool listed = false, any = false;
       int at[R::E];
 #pragma unroll
       for (int e = 0; e < R::E; ++e) {
-        at[e] = sc.bin(sc.at(y[e]));
+        at[e] = sc.bin(z[e]);
         listed |= at[e] == border;
         any |= at[e] < border;
       }
       if (__any(any)) {
+        sc.weights(z, w);
 #pragma unroll
-        for (int e = 0; e < R::E; ++e) {
-          const uint64_t w = sc.weight(sc.at(y[e]));
-          sum += at[e] < border && y[e] >= sc.bar ? w : 0;
-        }
+        for (int e = 0; e < R::E; ++e) sum += at[e] < border && y[e] >= sc.bar ? w[e] : 0;
       }
       if (listed) {
 #pragma unroll
@@ -532,61 +554,73 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
 #pragma unroll
       for (int e = 0; e < R::E; ++e) any |= y[e] >= sc.bar;
       if (__any(any)) {
+        sc.weights(z, w);
 #pragma unroll
-        for (int e = 0; e < R::E; ++e) {
-          const uint64_t w = sc.weight(sc.at(y[e]));
-          sum += y[e] >= sc.bar ? w : 0;
-        }
+        for (int e = 0; e < R::E; ++e) sum += y[e] >= sc.bar ? w[e] : 0;
       }
     }
     sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
-    if (lane == 0) a.tile[(int64_t)b * a.parts * a.tiles + tile] = sum;
-  }
+    if (lane == 0) a.tile[(int64_t)b * a.parts * a.tiles + v / 64] = sum;
+  });
   __syncthreads();
   if (s.run) append(a, b, s_list, s_n, &s_at);
 }
 
 // ---------------------------------------------------------------------------
-// The largest of the n values (each from 1 on, below 2^63 apart from one another) at
-// which the measure, summed from the largest value down, reaches `goal`; 0 if it does
-// nowhere. Nine bits of the values' range at a time, by histograms. s: FIN bins and 16
-// words.
+// Of the n values, those in [lo, hi] (lo >= 1): the largest at which the measure,
+// summed from the largest value down, reaches `goal`; 0 if none does. Nine bits of
+// the range at a time, by histograms, until one value is left.
+constexpr int REACH = FIN + FIN / 2 + 24;    // words of s
 template <typename V, typename M>
 __device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_t lo, uint64_t hi, uint64_t goal, uint64_t* s) {
   uint64_t* s_scan = s + FIN;
+  uint32_t* s_cnt = (uint32_t*)(s + FIN + 24);
   const int tid = threadIdx.x;
   __syncthreads();
-  for (;;) {
+  for (int pass = 0; ; ++pass) {
     const int bits = 64 - __clzll((long long)((hi - lo) | 1)), shift = bits > 9 ? bits - 9 : 0;
+    uint64_t* found = s_scan + 8 + pass % 2 * 4;   // (the last pass's may still be read)
     s[tid] = 0;
+    s_cnt[tid] = 0;
+    if (tid == 0) found[0] = 0;
     __syncthreads();
     for (int i = tid; i < n; i += FIN) {
       const uint64_t x = value(i);
-      if (x >= lo && x <= hi) atomicAdd((ull*)&s[(x - lo) >> shift], (ull)measure(i));
+      if (x >= lo && x <= hi) {
+        const int at = (int)((x - lo) >> shift);
+        atomicAdd((ull*)&s[at], (ull)measure(i));
+        atomicAdd(&s_cnt[at], 1u);
+      }
     }
     __syncthreads();
     uint64_t total;
     const uint64_t mine = s[FIN - 1 - tid], before = block_before<FIN>(mine, s_scan, total);
-    __syncthreads();
-    if (tid == 0) s_scan[8] = 0;
-    __syncthreads();
     if (before < goal && before + mine >= goal) {
-      s_scan[8] = FIN - tid;                // the bin and 1
-      s_scan[9] = before;
+      found[0] = FIN - tid;                 // the bin and 1
+      found[1] = before;
+      found[2] = s_cnt[FIN - 1 - tid];
     }
     __syncthreads();
-    if (s_scan[8] == 0) return 0;
-    goal -= s_scan[9];
-    lo += (s_scan[8] - 1) << shift;
+    if (found[0] == 0) return 0;
+    goal -= found[1];
+    lo += (found[0] - 1) << shift;
     if (shift == 0) return lo;
     if ((hi - lo) >> shift) hi = lo + ((uint64_t)1 << shift) - 1;
+    if (found[2] == 1) {
+      for (int i = tid; i < n; i += FIN) {
+        const uint64_t x = value(i);
+        if (x >= lo && x <= hi) s_scan[16] = x;
+      }
+      __syncthreads();
+      return s_scan[16];
+    }
   }
 }
 
 template <typename T, bool SPLIT>
 __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
   using R = Row<T>;
-  __shared__ uint64_t s_list[LIST], s_w[LIST], s_slot[SPLIT ? SLOTS : 1], s_scan[FIN + 16], s_found[3];
+  __shared__ uint64_t s_list[LIST], s_w[LIST], s_slot[SPLIT ? SLOTS : 1], s_scan[REACH], s_found[3];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
   const Setting s = setting_of(a, b);
   const R row(a, b);
@@ -603,7 +637,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
         if (i >= 0 && i < a.V) s_list[i] = place;
         first = place > first ? place : first;
       });
-    first = block_reduce<FIN>(first, s_scan, Most());
+    first = block_all<FIN>(first, s_scan, Most());
   }
   auto done = [&](int token, float logp) __attribute__((always_inline)) {
     a.token[b] = token;
@@ -628,26 +662,28 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
   const bool whole = SPLIT ? s.list && n_cand <= LIST : true;
   if (whole) {
     const int n = SPLIT ? (int)n_cand : a.V;
+    uint64_t most_off = 0;
     for (int i = tid; i < n; i += FIN) {
       const uint64_t place = SPLIT ? a.list[(int64_t)b * LIST + i] : s_list[i];
       if constexpr (SPLIT) s_list[i] = place;
       s_w[i] = place ? weight(place) : 0;
+      most_off = ~place > most_off && place ? ~place : most_off;
     }
-    __syncthreads();
+    const uint64_t least_place = ~block_all<FIN>(most_off, s_scan, Most());
     auto place = [&](int i) __attribute__((always_inline)) { return s_list[i]; };
     auto total_of = [&](auto&& kept) __attribute__((always_inline)) {
       uint64_t sum = 0;
       for (int i = tid; i < n; i += FIN) sum += kept(i) ? s_w[i] : 0;
-      return block_reduce<FIN>(sum, s_scan, Plus());
+      return block_all<FIN>(sum, s_scan, Plus());
     };
     uint64_t last = 1;                      // the last place kept
     if (s.cut) {
-      const uint64_t at = reach(n, place, [](int) { return (uint64_t)1; }, last, first, s.k, s_scan);
+      const uint64_t at = reach(n, place, [](int) { return (uint64_t)1; }, least_place, first, s.k, s_scan);
       if (at) last = at;                    // (0: there are fewer)
     }
     if (s.run) {
       const uint64_t goal = part_of(s.p, total_of([&](int i) { return s_list[i] >= last; }), true);
-      last = goal <= 1 ? first : reach(n, place, [&](int i) { return s_w[i]; }, last, first, goal, s_scan);
+      last = goal <= 1 ? first : reach(n, place, [&](int i) { return s_w[i]; }, last > 1 ? last : least_place, first, goal, s_scan);
     }
     auto kept = [&](int i) __attribute__((always_inline)) { return s_list[i] >= last && logit_of(s_list[i]) >= sc.bar; };
     const uint64_t total = total_of(kept), aim = aim_of(total);
@@ -672,12 +708,17 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
       uint64_t before, goal;
       border = border_bin<FIN>(a, b, s.p, s_scan, before, goal);
       const int n = (int)n_cand;
+      uint64_t least_off = 0, most = 0;
       for (int i = tid; i < n; i += FIN) {
-        s_list[i] = a.list[(int64_t)b * LIST + i];
-        s_w[i] = weight(s_list[i]);
+        const uint64_t place = a.list[(int64_t)b * LIST + i];
+        s_list[i] = place;
+        s_w[i] = weight(place);
+        least_off = ~place > least_off ? ~place : least_off;
+        most = place > most ? place : most;
       }
-      __syncthreads();
-      last = reach(n, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, last, first, goal - before, s_scan);
+      least_off = block_all<FIN>(least_off, s_scan, Most());
+      most = block_all<FIN>(most, s_scan, Most());
+      last = reach(n, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, ~least_off, most, goal - before, s_scan);
       for (int i = tid; i < n; i += FIN)
         if (s_list[i] >= last && logit_of(s_list[i]) >= sc.bar)
           atomicAdd((ull*)&s_slot[(index_of(s_list[i]) + row.shift) / R::E / 64 / per], (ull)s_w[i]);
@@ -731,7 +772,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
       over([&](float y, int i) __attribute__((always_inline)) {
         if (place_of(key_of(y), i) >= last) sum += mass(y);
       });
-      sum = block_reduce<FIN>(sum, s_scan, Plus());
+      sum = block_all<FIN>(sum, s_scan, Plus());
       const uint64_t goal = part_of(s.p, sum, true);
       last = goal <= 1 ? first : far(mass, goal);
     }
