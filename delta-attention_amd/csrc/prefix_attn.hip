@@ -43,7 +43,7 @@ struct PrefixArgs {
   int p_rows, p_rt, o_rows, o_rt;           // rows of a prefix's sequences and of a sequence, their row tiles
   int p_splits, o_splits, p_chunk, o_chunk; // splits of the keys, tiles of each
   int p_items;                              // items of the prefixes, before the sequences' own
-  FastDiv heads, rows_s, f_prt, f_psp, f_ort, f_osp, f_hkv;   // G, s, p_rt, p_splits, o_rt, o_splits, Hkv
+  FastDiv heads, rows_s, f_prt, f_psp, f_ort, f_osp, f_hkv, f_rows, f_per;   // G, s, p_rt, p_splits, o_rt, o_splits, Hkv, rows, per
   float scale2;                             // |sm_scale| log2(e), above zero
   uint32_t flip;                            // the sign bits of Q where sm_scale is negative
   float *part, *part_m, *part_l;            // [Hkv, splits, rows, D], [Hkv, splits, rows] twice
@@ -347,36 +347,73 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefi
       a.part_m[at] = ref[mt];
       a.part_l[at] = l;
     }
+    if (nt == 0) continue;                   // (nothing reads the sums of a split without keys)
 #pragma unroll
     for (int d = 0; d < DT; ++d) *(f32x4*)(a.part + at * D + 16 * d + 4 * g) = acc[mt][d];
   }
 }
 
-// Joins a row's splits: D / 4 threads a row.
+// Joins a row's splits: groups of D / 4 threads, `side` (a power of two) of them a
+// row, take splits side by side, four loads of each in flight, and are joined
+// through LDS.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a) {
+__global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int side) {
   using E = Elt<T>;
-  constexpr int CT = D / 4, PER = 256 / CT;
-  const int64_t x = (int64_t)blockIdx.x * PER + threadIdx.x / CT;
-  if (x >= (int64_t)a.rows * a.Hkv) return;
-  const int hk = (int)(x / a.rows), row = (int)(x - (int64_t)hk * a.rows), t = threadIdx.x % CT;
-  const int y = fdiv(row, a.heads), b = fdiv(y, a.rows_s), i = y - b * a.s;
+  constexpr int CT = D / 4, GROUPS = 256 / CT, U = 4;
+  __shared__ f32x4 s_o[GROUPS][CT];
+  __shared__ float s_m[GROUPS], s_l[GROUPS];
+  const int t = threadIdx.x % CT, group = threadIdx.x / CT, sg = group & (side - 1);
+  const int x = blockIdx.x * (GROUPS / side) + group / side;
+  const bool live = x < a.rows * a.Hkv;
+  const int hk = live ? fdiv(x, a.f_rows) : 0, row = live ? x - hk * a.rows : 0;
   const int splits = a.p_splits + a.o_splits;
   const int64_t at = (int64_t)hk * splits * a.rows + row;
   float m = NO_KEYS, l = 0.f;
   f32x4 o = {0, 0, 0, 0};
-  for (int j = 0; j < splits; ++j) {
-    const float mj = a.part_m[at + (int64_t)j * a.rows], lj = a.part_l[at + (int64_t)j * a.rows];
-    if (lj == 0.f) continue;
-    const f32x4 z = *(const f32x4*)(a.part + (at + (int64_t)j * a.rows) * D + 4 * t);
-    const float to = fmaxf(m, mj), k0 = fast_exp2((m - to) * a.scale2), k1 = fast_exp2((mj - to) * a.scale2);
-    m = to;
-    l = l * k0 + lj * k1;
+  for (int j0 = sg; j0 < splits; j0 += U * side) {
+    float mj[U], lj[U];
+    f32x4 z[U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = o[e] * k0 + z[e] * k1;
+    for (int u = 0; u < U; ++u) {              // (past the last: it again, without weight)
+      const int64_t i = at + (int64_t)min(j0 + u * side, splits - 1) * a.rows;
+      mj[u] = a.part_m[i];
+      lj[u] = a.part_l[i];
+      z[u] = *(const f32x4*)(a.part + i * D + 4 * t);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (lj[u] == 0.f || j0 + u * side >= splits) continue;   // (a split without keys holds no sums)
+      const float to = fmaxf(m, mj[u]), k0 = fast_exp2((m - to) * a.scale2), k1 = fast_exp2((mj[u] - to) * a.scale2);
+      m = to;
+      l = l * k0 + lj[u] * k1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = o[e] * k0 + z[u][e] * k1;
+    }
   }
+  if (side > 1) {
+    s_o[group][t] = o;
+    if (t == 0) {
+      s_m[group] = m;
+      s_l[group] = l;
+    }
+    __syncthreads();
+    if (sg > 0) return;
+    for (int i = 1; i < side; ++i) m = fmaxf(m, s_m[group + i]);
+    l = 0.f;
+    o = (f32x4){0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = 0; i < side; ++i) {
+      const float k = fast_exp2((s_m[group + i] - m) * a.scale2);
+      const f32x4 z = s_o[group + i][t];
+      l = fmaf(s_l[group + i], k, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(z[e], k, o[e]);
+    }
+  }
+  if (!live) return;
   // a row without keys is zero; one whose every score is -inf has no softmax: NaN
-  const bool none = prefix_keys(a, b / a.per) == 0 && own_keys(a, b) - a.s + i < 0;
+  const int y = fdiv(row, a.heads), b = fdiv(y, a.rows_s), i = y - b * a.s;
+  const bool none = prefix_keys(a, fdiv(b, a.f_per)) == 0 && own_keys(a, b) - a.s + i < 0;
   const float inv = none ? 0.f : 1.f / l;
   T* dst = (T*)a.o + b * a.o_b + (int64_t)(hk * a.G + row - y * a.G) * a.o_h + i * a.o_s;
   *(u32x2*)(dst + 4 * t) = (u32x2){E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
@@ -427,8 +464,12 @@ void launch(const PrefixArgs& a, const Plan& p, hipStream_t st) {
     if (p.mt == 1) hipLaunchKernelGGL((prefix_rows_kernel<T, D, 1>), dim3((unsigned)p.items), block, 0, st, a);
     else hipLaunchKernelGGL((prefix_rows_kernel<T, D, 2>), dim3((unsigned)p.items), block, 0, st, a);
   }
-  constexpr int PER = 256 / (D / 4);
-  hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((unsigned)((p.rows * a.Hkv + PER - 1) / PER)), dim3(256), 0, st, a);
+  // four splits a group at once, as long as a workgroup has groups
+  constexpr int GROUPS = 256 / (D / 4);
+  int side = 1;
+  while (side < GROUPS && 4 * side < p.p_splits + p.o_splits) side *= 2;
+  const int per = GROUPS / side;
+  hipLaunchKernelGGL((prefix_join_kernel<T, D>), dim3((unsigned)((p.rows * a.Hkv + per - 1) / per)), dim3(256), 0, st, a, side);
 }
 
 template <typename T>
@@ -505,7 +546,7 @@ extern "C" int da_prefix_attn_fwd(const da_prefix_attn_args* x, void* stream) {
   a.heads = make_fastdiv(G), a.rows_s = make_fastdiv(s);
   a.f_prt = make_fastdiv(p.p_rt), a.f_ort = make_fastdiv(p.o_rt);
   a.f_psp = make_fastdiv(p.p_splits > 0 ? p.p_splits : 1), a.f_osp = make_fastdiv(p.o_splits > 0 ? p.o_splits : 1);
-  a.f_hkv = make_fastdiv(Hkv);
+  a.f_hkv = make_fastdiv(Hkv), a.f_rows = make_fastdiv(a.rows), a.f_per = make_fastdiv(a.per);
   // (a scale of zero, which weighs every key alike, as the smallest one: a masked
   // score's -inf stays -inf)
   a.scale2 = fminf(fmaxf(fabsf(x->sm_scale) * 1.4426950408889634f, FLT_TRUE_MIN), FLT_MAX);
