@@ -100,64 +100,30 @@ __device__ __forceinline__ int own_keys(const PrefixArgs& a, int b) {
 // S^T = K Q^T leaves a lane (row c = lane % 16, group g = lane / 16) the keys 16 t
 // + 4 g + r of its row, which is the right operand of O^T = V^T P^T as it stands;
 // V^T comes from transposed LDS reads of the same keys.
-template <typename T, int D, int MT>
-__global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefix_rows_kernel(PrefixArgs a) {
+template <typename T, int D, int MT, bool OWN>
+__device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&smem)[2][2][Tile<D>::BYTES]) {
   using E = Elt<T>;
   using M = Mma<T>;
   using TL = Tile<D>;
   constexpr int KS = D / 32, DT = D / 16, BM = 16 * MT * WAVES;
-  __shared__ __align__(1024) char smem[2][2][TL::BYTES];
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int c = lane % 16, g = lane / 16;
 
   // the item: (prefix or sequence, kv head, split, row tile), the row tiles of a
   // split beside each other
-  int item = blockIdx.x;
-  const bool own = item >= a.p_items;
-  int hk, split, tile, row0, n_rows, n_keys, key0, chunk;   // row0: of the kv head's rows
-  const char *kb, *vb;
-  uint32_t k_s, v_s;
-  int lim0;                                  // the first row's last key, less what its place adds
-  if (!own) {
-    int x = fdiv(item, a.f_prt);
-    tile = item - x * a.p_rt;
-    int y = fdiv(x, a.f_psp);
-    split = x - y * a.p_splits;
-    const int p = fdiv(y, a.f_hkv);
-    hk = y - p * a.Hkv;
-    n_rows = min(BM, a.p_rows - tile * BM);
-    row0 = p * a.p_rows + tile * BM;
-    n_keys = prefix_keys(a, p);
-    chunk = a.p_chunk;
-    kb = (const char*)a.kp + 2 * (p * a.kp_b + hk * a.kp_h);
-    vb = (const char*)a.vp + 2 * (p * a.vp_b + hk * a.vp_h);
-    k_s = a.kp_s, v_s = a.vp_s;
-    lim0 = n_keys - 1;
-  } else {
-    item -= a.p_items;
-    int x = fdiv(item, a.f_ort);
-    tile = item - x * a.o_rt;
-    int y = fdiv(x, a.f_osp);
-    split = x - y * a.o_splits;
-    const int b = fdiv(y, a.f_hkv);
-    hk = y - b * a.Hkv;
-    n_rows = min(BM, a.o_rows - tile * BM);
-    row0 = b * a.o_rows + tile * BM;
-    n_keys = own_keys(a, b);
-    chunk = a.o_chunk;
-    kb = (const char*)a.k + 2 * (b * a.k_b + hk * a.k_h);
-    vb = (const char*)a.v + 2 * (b * a.v_b + hk * a.v_h);
-    k_s = a.k_s, v_s = a.v_s;
-    lim0 = n_keys - a.s;
-    split += a.p_splits;
-  }
-  n_keys = __builtin_amdgcn_readfirstlane(n_keys);
-  lim0 = __builtin_amdgcn_readfirstlane(lim0);
-  key0 = (own ? split - a.p_splits : split) * chunk * BN;
+  const int x0 = fdiv(item, OWN ? a.f_ort : a.f_prt), tile = item - x0 * (OWN ? a.o_rt : a.p_rt);
+  const int y0 = fdiv(x0, OWN ? a.f_osp : a.f_psp), part = x0 - y0 * (OWN ? a.o_splits : a.p_splits);
+  const int list = fdiv(y0, a.f_hkv), hk = y0 - list * a.Hkv;        // list: the prefix or the sequence
+  const int n_rows = min(BM, (OWN ? a.o_rows : a.p_rows) - tile * BM);
+  const int row0 = list * (OWN ? a.o_rows : a.p_rows) + tile * BM;    // of the kv head's rows
+  const int n_keys = __builtin_amdgcn_readfirstlane(OWN ? own_keys(a, list) : prefix_keys(a, list));
+  const int chunk = OWN ? a.o_chunk : a.p_chunk, split = OWN ? part + a.p_splits : part, key0 = part * chunk * BN;
+  const char* kb = (const char*)(OWN ? a.k : a.kp) + 2 * (OWN ? list * a.k_b + hk * a.k_h : list * a.kp_b + hk * a.kp_h);
+  const char* vb = (const char*)(OWN ? a.v : a.vp) + 2 * (OWN ? list * a.v_b + hk * a.v_h : list * a.vp_b + hk * a.vp_h);
+  const uint32_t k_s = OWN ? a.k_s : a.kp_s, v_s = OWN ? a.v_s : a.vp_s;
 
   // this wave's rows: places in the kv head's rows, and each one's last key
-  const int splits = a.p_splits + a.o_splits;
-  const int64_t slot = ((int64_t)hk * splits + split) * a.rows;
+  const int lim0 = OWN ? n_keys - a.s : n_keys - 1;
   const bool active = wave * 16 * MT < n_rows;
   int lim[MT], lim_lo = lim0, lim_hi = lim0;
   u32x4 qf[MT][KS];
@@ -165,21 +131,21 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefi
   for (int mt = 0; mt < MT; ++mt) {
     const int r = row0 + min(wave * 16 * MT + mt * 16 + c, n_rows - 1);   // (past the last: it again)
     const int x = fdiv(r, a.heads), b = fdiv(x, a.rows_s), i = x - b * a.s;
-    lim[mt] = own ? lim0 + i : lim0;
+    lim[mt] = OWN ? lim0 + i : lim0;
     const T* src = (const T*)a.q + b * a.q_b + (int64_t)(hk * a.G + r - x * a.G) * a.q_h + i * a.q_s;
 #pragma unroll
     for (int k = 0; k < KS; ++k) qf[mt][k] = *(const u32x4*)(src + 32 * k + 8 * g) ^ a.flip;
   }
-  if (own) {                                 // of the whole row tile
-    const int x0 = fdiv(row0, a.heads), x1 = fdiv(row0 + n_rows - 1, a.heads);
-    lim_lo += x0 - (int)fdiv(x0, a.rows_s) * a.s;
-    lim_hi += x1 - (int)fdiv(x1, a.rows_s) * a.s;
+  if (OWN) {                                 // of the whole row tile
+    const int u = fdiv(row0, a.heads), w = fdiv(row0 + n_rows - 1, a.heads);
+    lim_lo += u - (int)fdiv(u, a.rows_s) * a.s;
+    lim_hi += w - (int)fdiv(w, a.rows_s) * a.s;
   }
   const int end = min(min(key0 + chunk * BN, n_keys), lim_hi + 1);
   const int nt = end > key0 ? (end - key0 + BN - 1) / BN : 0;
 
   f32x4 acc[MT][DT];
-  float ref[MT], sum[MT];
+  float ref[MT], sum[MT];                    // ref: scaled, in log2
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     ref[mt] = NO_KEYS;
@@ -237,21 +203,25 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefi
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) s[mt][i] = M::dot(ka, qf[mt][k], k == 0 ? (f32x4){0, 0, 0, 0} : s[mt][i]);
       }
-    u32x4 pf[MT][2];
+    if (!whole) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      if (!whole) {
+      for (int mt = 0; mt < MT; ++mt) {
         const int hi = lim[mt] - first - 4 * g;
 #pragma unroll
         for (int e = 0; e < 16; ++e) s[mt][e / 4][e % 4] = e / 4 * 16 + e % 4 <= hi ? s[mt][e / 4][e % 4] : -INFINITY;
       }
+    }
+    u32x4 pf[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      // (IEEE maximum: it needs no quieting of its operands, and a NaN moves no
+      // reference but reaches the row's sum)
       float top = s[mt][0][0];
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = fmaxf(top, s[mt][e / 4][e % 4]);
-      top = group_max(top);
-      if (__any((top - ref[mt]) * a.scale2 > LAG)) {
-        const float to = fmaxf(ref[mt], top);
-        const float alpha = fast_exp2((ref[mt] - to) * a.scale2);
+      for (int e = 1; e < 16; ++e) top = __builtin_elementwise_maximum(top, s[mt][e / 4][e % 4]);
+      top = group_max(top) * a.scale2;
+      if (__any(top - ref[mt] > LAG)) {
+        const float to = fmaxf(ref[mt], top), alpha = fast_exp2(ref[mt] - to);
         ref[mt] = to;
         sum[mt] *= alpha;
 #pragma unroll
@@ -259,12 +229,13 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefi
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[mt][d][r] *= alpha;
       }
+      const float off = BIAS<T> - ref[mt];
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int i = 2 * u + w / 2, r = w % 2 * 2;
-          auto weight = [&](float y) __attribute__((always_inline)) { return fast_exp2(fmaf(y - ref[mt], a.scale2, BIAS<T>)); };
+          auto weight = [&](float y) __attribute__((always_inline)) { return fast_exp2(fmaf(y, a.scale2, off)); };
           pf[mt][u][w] = E::pack2(weight(s[mt][i][r]), weight(s[mt][i][r + 1]));
           sum[mt] = E::add_pair(pf[mt][u][w], sum[mt]);   // (the rounded ones: as the product has them)
         }
@@ -276,7 +247,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefi
     // An infinity or NaN among the values of a key that one of the rows does not see
     // must not reach it through 0 * inf (keys past the last one are loaded as zero).
     bool odd = false;
-    if (!whole && lim_lo < lim_hi) {
+    if (OWN && !whole && lim_lo < lim_hi) {
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -288,7 +259,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefi
         }
       odd = __any(odd);
     }
-    if (odd) {
+    if (OWN && odd) {
       // taken as zero, and given to the rows that see them from products of the
       // values' and the rows' marks
 #pragma unroll
@@ -337,6 +308,7 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefi
     }
   }
   if (!active) return;
+  const int64_t slot = ((int64_t)hk * (a.p_splits + a.o_splits) + split) * a.rows;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int r = wave * 16 * MT + mt * 16 + c;
@@ -351,6 +323,14 @@ __global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefi
 #pragma unroll
     for (int d = 0; d < DT; ++d) *(f32x4*)(a.part + at * D + 16 * d + 4 * g) = acc[mt][d];
   }
+}
+
+template <typename T, int D, int MT>
+__global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefix_rows_kernel(PrefixArgs a) {
+  __shared__ __align__(1024) char smem[2][2][Tile<D>::BYTES];
+  const int item = blockIdx.x;
+  if (item < a.p_items) rows_item<T, D, MT, false>(a, item, smem);
+  else rows_item<T, D, MT, true>(a, item - a.p_items, smem);
 }
 
 // Joins a row's splits: groups of D / 4 threads, `side` (a power of two) of them a
@@ -383,7 +363,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int side
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (lj[u] == 0.f || j0 + u * side >= splits) continue;   // (a split without keys holds no sums)
-      const float to = fmaxf(m, mj[u]), k0 = fast_exp2((m - to) * a.scale2), k1 = fast_exp2((mj[u] - to) * a.scale2);
+      const float to = fmaxf(m, mj[u]), k0 = fast_exp2(m - to), k1 = fast_exp2(mj[u] - to);
       m = to;
       l = l * k0 + lj[u] * k1;
 #pragma unroll
@@ -403,7 +383,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int side
     o = (f32x4){0, 0, 0, 0};
 #pragma unroll 4
     for (int i = 0; i < side; ++i) {
-      const float k = fast_exp2((s_m[group + i] - m) * a.scale2);
+      const float k = fast_exp2(s_m[group + i] - m);
       const f32x4 z = s_o[group + i][t];
       l = fmaf(s_l[group + i], k, l);
 #pragma unroll
