@@ -42,13 +42,17 @@ struct PrefixArgs {
   int rows;                                 // B * s * G: rows of a kv head
   int p_rows, p_rt, o_rows, o_rt;           // rows of a prefix's sequences and of a sequence, their row tiles
   int p_splits, o_splits, p_chunk, o_chunk; // splits of the keys, tiles of each
-  int p_items;                              // items of the prefixes, before the sequences' own
+  int p_items, p_grid;                      // items of the prefixes; their workgroups, before those of the sequences' own
   FastDiv heads, rows_s, f_prt, f_psp, f_ort, f_osp, f_hkv, f_rows, f_per;   // G, s, p_rt, p_splits, o_rt, o_splits, Hkv, rows, per
   float scale2;                             // |sm_scale| log2(e), above zero
   uint32_t flip;                            // the sign bits of Q where sm_scale is negative
   float *part, *part_m, *part_l;            // [Hkv, splits, rows, D], [Hkv, splits, rows] twice
 };
 
+__device__ __forceinline__ void dma16_nt(u32x4 r, uint32_t lds, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
+               :: "s"(lds), "v"(voff), "s"(r) : "memory");
+}
 template <typename T> struct Mma;
 template <> struct Mma<__bf16> {
   static constexpr uint32_t inf = 0x7f80, one = 0x3f80;
@@ -95,17 +99,20 @@ __device__ __forceinline__ int own_keys(const PrefixArgs& a, int b) {
   return min(max(a.n_dev ? a.n_dev[(int64_t)b * a.n_step] : a.n, 0), a.cap);
 }
 
+// Waves of a SIMD: what the accumulators and two tiles of scores leave room for.
+__host__ __device__ constexpr int waves_of(int D, int mt) { return D == 256 ? 1 : D == 128 ? 2 : D * mt == 128 ? 3 : 4; }
+
 // One item: a row tile of 16 MT rows a wave against a split's key tiles, which
 // all waves load into LDS together, the next one while this one is computed.
 // S^T = K Q^T leaves a lane (row c = lane % 16, group g = lane / 16) the keys 16 t
 // + 4 g + r of its row, which is the right operand of O^T = V^T P^T as it stands;
 // V^T comes from transposed LDS reads of the same keys.
-template <typename T, int D, int MT, bool OWN>
+template <typename T, int D, int MT, bool OWN, bool STREAM>
 __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&smem)[2][2][Tile<D>::BYTES]) {
   using E = Elt<T>;
   using M = Mma<T>;
   using TL = Tile<D>;
-  constexpr int KS = D / 32, DT = D / 16, BM = 16 * MT * WAVES;
+  constexpr int KS = D / 32, DT = D / 16, KG = BN / 16, BM = 16 * MT * WAVES;
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int c = lane % 16, g = lane / 16;
 
@@ -163,17 +170,17 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
     voff[j] = row * v_s + ch * 16;
   }
   const uint32_t lds0 = (uint32_t)(uintptr_t)(DA_LDS char*)&smem[0][0][0];
-  auto issue = [&](int t) __attribute__((always_inline)) {
+  auto issue = [&](bool values, int t) __attribute__((always_inline)) {
     const int first = key0 + t * BN;
-    const int64_t left = n_keys - first;     // keys from here on: the others read as zero
-    const int64_t kr = (left - 1) * k_s + TL::RB, vr = (left - 1) * v_s + TL::RB;
-    const u32x4 rk = rsrc_words(kb + (int64_t)first * k_s, kr >> 32 ? 0xffffffffu : (uint32_t)kr);
-    const u32x4 rv = rsrc_words(vb + (int64_t)first * v_s, vr >> 32 ? 0xffffffffu : (uint32_t)vr);
-    const uint32_t st = lds0 + t % 2 * 2 * TL::BYTES + wave * 1024;
+    const uint32_t step = values ? v_s : k_s;
+    const int64_t left = (int64_t)(n_keys - first - 1) * step + TL::RB;   // what lies behind the last key reads as zero
+    const u32x4 r = rsrc_words((values ? vb : kb) + (int64_t)first * step, left >> 32 ? 0xffffffffu : (uint32_t)left);
+    const uint32_t st = lds0 + (t % 2 * 2 + values) * TL::BYTES + wave * 1024;
 #pragma unroll
-    for (int j = 0; j < TL::DMAS; ++j) dma16_untracked(rk, st + j * WAVES * 1024, koff[j]);
-#pragma unroll
-    for (int j = 0; j < TL::DMAS; ++j) dma16_untracked(rv, st + TL::BYTES + j * WAVES * 1024, voff[j]);
+    for (int j = 0; j < TL::DMAS; ++j) {
+      if (STREAM) dma16_nt(r, st + j * WAVES * 1024, values ? voff[j] : koff[j]);
+      else dma16_untracked(r, st + j * WAVES * 1024, values ? voff[j] : koff[j]);
+    }
   };
   int kread[KS], vread[DT];
 #pragma unroll
@@ -184,41 +191,33 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
     vread[t] = row * TL::RB + ((2 * t + c % 4 / 2) ^ TL::swz(row)) * 16 + c % 2 * 8;
   }
 
-  if (nt > 0) issue(0);
-  for (int t = 0; t < nt; ++t) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    lds_barrier();                           // the tile is there, and the one before is read
-    if (t + 1 < nt) issue(t + 1);
-    if (!active) continue;
+  // scores of tile t (raw), with -inf where a row does not see the key
+  auto scores = [&](int t, f32x4 (&s)[MT][KG]) __attribute__((always_inline)) {
     const DA_LDS char* ks = (const DA_LDS char*)&smem[t % 2][0][0];
-    const DA_LDS char* vs = (const DA_LDS char*)&smem[t % 2][1][0];
-    const int first = key0 + t * BN;
-    const bool whole = first + BN - 1 <= lim_lo;
-    f32x4 s[MT][4];
 #pragma unroll
     for (int k = 0; k < KS; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < KG; ++i) {
         const u32x4 ka = *(const DA_LDS u32x4*)(ks + kread[k] + 16 * i * TL::RB);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) s[mt][i] = M::dot(ka, qf[mt][k], k == 0 ? (f32x4){0, 0, 0, 0} : s[mt][i]);
       }
-    if (!whole) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const int hi = lim[mt] - first - 4 * g;
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[mt][e / 4][e % 4] = e / 4 * 16 + e % 4 <= hi ? s[mt][e / 4][e % 4] : -INFINITY;
-      }
-    }
-    u32x4 pf[MT][2];
+  };
+  // the references move where a row's largest score passes its own by LAG
+  auto follow = [&](int t, f32x4 (&s)[MT][KG]) __attribute__((always_inline)) {
+    const int first = key0 + t * BN;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
+      if (first + BN - 1 > lim_lo) {
+        const int hi = lim[mt] - first - 4 * g;
+#pragma unroll
+        for (int e = 0; e < 4 * KG; ++e) s[mt][e / 4][e % 4] = e / 4 * 16 + e % 4 <= hi ? s[mt][e / 4][e % 4] : -INFINITY;
+      }
       // (IEEE maximum: it needs no quieting of its operands, and a NaN moves no
       // reference but reaches the row's sum)
       float top = s[mt][0][0];
 #pragma unroll
-      for (int e = 1; e < 16; ++e) top = __builtin_elementwise_maximum(top, s[mt][e / 4][e % 4]);
+      for (int e = 1; e < 4 * KG; ++e) top = __builtin_elementwise_maximum(top, s[mt][e / 4][e % 4]);
       top = group_max(top) * a.scale2;
       if (__any(top - ref[mt] > LAG)) {
         const float to = fmaxf(ref[mt], top), alpha = fast_exp2(ref[mt] - to);
@@ -229,9 +228,41 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[mt][d][r] *= alpha;
       }
+    }
+  };
+
+  // Step t: the scores of tile t + 1 are formed beside the probabilities of tile t,
+  // then its products with the values. K(t + 2) and V(t + 1) are on their way: into
+  // the places of K(t) and V(t - 1), which step t - 1 read last.
+  f32x4 s[MT][KG];
+  if (nt > 0) {
+    issue(false, 0);
+    issue(true, 0);
+    if (nt > 1) issue(false, 1);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    if (active) {
+      scores(0, s);
+      follow(0, s);
+    }
+  }
+  for (int t = 0; t < nt; ++t) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    lds_barrier();
+    if (t + 2 < nt) issue(false, t + 2);
+    if (t + 1 < nt) issue(true, t + 1);
+    if (!active) continue;
+    const DA_LDS char* vs = (const DA_LDS char*)&smem[t % 2][1][0];
+    const int first = key0 + t * BN;
+    const bool whole = first + BN - 1 <= lim_lo;
+    u32x4 pf[MT][KG / 2];
+    f32x4 next[MT][KG];
+    scores(t + 1, next);                     // (behind the last tile: of what lies there, not used)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
       const float off = BIAS<T> - ref[mt];
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < KG / 2; ++u)
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const int i = 2 * u + w / 2, r = w % 2 * 2;
@@ -251,7 +282,7 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < KG / 2; ++u) {
           const u32x4 va = values(u, d);
 #pragma unroll
           for (int w = 0; w < 4; ++w)
@@ -263,7 +294,7 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
       // taken as zero, and given to the rows that see them from products of the
       // values' and the rows' marks
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
+      for (int u = 0; u < KG / 2; ++u) {
         u32x4 sees[MT];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -298,7 +329,7 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
       }
     } else {
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < KG / 2; ++u)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
           const u32x4 va = values(u, d);
@@ -306,6 +337,11 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
           for (int mt = 0; mt < MT; ++mt) acc[mt][d] = M::dot(va, pf[mt][u], acc[mt][d]);
         }
     }
+    if (t + 1 < nt) follow(t + 1, next);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < KG; ++i) s[mt][i] = next[mt][i];
   }
   if (!active) return;
   const int64_t slot = ((int64_t)hk * (a.p_splits + a.o_splits) + split) * a.rows;
@@ -326,11 +362,20 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
 }
 
 template <typename T, int D, int MT>
-__global__ __launch_bounds__(64 * WAVES, D <= 128 && MT <= 2 ? 2 : 1) void prefix_rows_kernel(PrefixArgs a) {
+__global__ __launch_bounds__(64 * WAVES, waves_of(D, MT)) void prefix_rows_kernel(PrefixArgs a) {
   __shared__ __align__(1024) char smem[2][2][Tile<D>::BYTES];
-  const int item = blockIdx.x;
-  if (item < a.p_items) rows_item<T, D, MT, false>(a, item, smem);
-  else rows_item<T, D, MT, true>(a, item - a.p_items, smem);
+  int item = blockIdx.x;
+  if (item >= a.p_grid) {
+    rows_item<T, D, 1, true, false>(a, item - a.p_grid, smem);
+  } else if (a.p_rt > 1) {
+    // The row tiles of one split run on one XCD (workgroup x runs on XCD x % 8):
+    // its L2 holds the keys that they share.
+    const int q = item / 8, k = fdiv(q, a.f_prt);
+    item = (k * 8 + item % 8) * a.p_rt + q - k * a.p_rt;
+    if (item < a.p_items) rows_item<T, D, MT, false, false>(a, item, smem);
+  } else {
+    rows_item<T, D, MT, false, true>(a, item, smem);
+  }
 }
 
 // Joins a row's splits: groups of D / 4 threads, `side` (a power of two) of them a
@@ -404,7 +449,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int side
 
 struct Plan {
   int mt, p_rt, o_rt, p_splits, o_splits, p_chunk, o_chunk;
-  int64_t p_items, items, rows;
+  int64_t p_items, p_grid, grid, rows;
   size_t bytes;
 };
 
@@ -417,11 +462,11 @@ bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, i
   const int64_t p_rows = p.rows / P;
   p.mt = p_rows <= 64 ? 1 : 2;
   const int bm = 16 * p.mt * WAVES;
-  const int64_t p_rt = Np > 0 ? (p_rows + bm - 1) / bm : 0, o_rt = cap > 0 ? (own + bm - 1) / bm : 0;
+  const int64_t p_rt = Np > 0 ? (p_rows + bm - 1) / bm : 0, o_rt = cap > 0 ? (own + 16 * WAVES - 1) / (16 * WAVES) : 0;
   const int64_t p_tiles = (Np + BN - 1) / BN, o_tiles = (cap + BN - 1) / BN;
   const int64_t p_lists = P * Hkv * p_rt, o_lists = (int64_t)B * Hkv * o_rt;
   if (p_lists > MOST || o_lists > MOST) return false;
-  const int64_t slots = 256 * (D <= 128 ? 2 : 1);
+  const int64_t slots = 256 * waves_of(D, p.mt);
   int64_t chunk = (p_lists * p_tiles + o_lists * o_tiles + slots - 1) / slots;
   if (chunk < 4) chunk = 4;
   p.p_rt = (int)(p_rt > 0 ? p_rt : 1);
@@ -431,8 +476,10 @@ bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, i
   p.p_chunk = p.p_splits > 0 ? (int)((p_tiles + p.p_splits - 1) / p.p_splits) : 1;
   p.o_chunk = p.o_splits > 0 ? (int)((o_tiles + p.o_splits - 1) / p.o_splits) : 1;
   p.p_items = p_lists * p.p_splits;
-  p.items = p.p_items + o_lists * p.o_splits;
-  if (p.items > MOST || p.rows * Hkv > MOST * 4) return false;
+  const int64_t deal = p.p_rt > 1 ? 8 * (int64_t)p.p_rt : 1;
+  p.p_grid = (p.p_items + deal - 1) / deal * deal;
+  p.grid = p.p_grid + o_lists * p.o_splits;
+  if (p.grid > MOST || p.rows * Hkv > MOST * 4) return false;
   p.bytes = (size_t)(p.rows * Hkv * (p.p_splits + p.o_splits)) * (D + 2) * sizeof(float);
   return true;
 }
@@ -440,9 +487,10 @@ bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, i
 template <typename T, int D>
 void launch(const PrefixArgs& a, const Plan& p, hipStream_t st) {
   const dim3 block(64 * WAVES);
-  if (p.items > 0) {
-    if (p.mt == 1) hipLaunchKernelGGL((prefix_rows_kernel<T, D, 1>), dim3((unsigned)p.items), block, 0, st, a);
-    else hipLaunchKernelGGL((prefix_rows_kernel<T, D, 2>), dim3((unsigned)p.items), block, 0, st, a);
+  if (p.grid > 0) {
+    const dim3 grid((unsigned)p.grid);
+    if (p.mt == 1) hipLaunchKernelGGL((prefix_rows_kernel<T, D, 1>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((prefix_rows_kernel<T, D, 2>), grid, block, 0, st, a);
   }
   // four splits a group at once, as long as a workgroup has groups
   constexpr int GROUPS = 256 / (D / 4);
@@ -522,7 +570,7 @@ extern "C" int da_prefix_attn_fwd(const da_prefix_attn_args* x, void* stream) {
   a.p_rows = a.rows / P, a.o_rows = s * G;
   a.p_rt = p.p_rt, a.o_rt = p.o_rt;
   a.p_splits = p.p_splits, a.o_splits = p.o_splits, a.p_chunk = p.p_chunk, a.o_chunk = p.o_chunk;
-  a.p_items = (int)p.p_items;
+  a.p_items = (int)p.p_items, a.p_grid = (int)p.p_grid;
   a.heads = make_fastdiv(G), a.rows_s = make_fastdiv(s);
   a.f_prt = make_fastdiv(p.p_rt), a.f_ort = make_fastdiv(p.o_rt);
   a.f_psp = make_fastdiv(p.p_splits > 0 ? p.p_splits : 1), a.f_osp = make_fastdiv(p.o_splits > 0 ? p.o_splits : 1);
