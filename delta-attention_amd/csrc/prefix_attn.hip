@@ -467,14 +467,31 @@ bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, i
   const int64_t p_lists = P * Hkv * p_rt, o_lists = (int64_t)B * Hkv * o_rt;
   if (p_lists > MOST || o_lists > MOST) return false;
   const int64_t slots = 256 * waves_of(D, p.mt);
-  int64_t chunk = (p_lists * p_tiles + o_lists * o_tiles + slots - 1) / slots;
-  if (chunk < 4) chunk = 4;
+  // Tiles of an item: the count whose items end first, on a model of a launch. An
+  // item takes its tiles and START more; the prefixes' items start first, the
+  // sequences' own in the places beside or behind them; a split costs its partial
+  // sums' way to memory and back.
+  constexpr double START = 1.5;
+  const int64_t least = (p_lists * p_tiles + o_lists * o_tiles + slots - 1) / slots;
+  double best = 0;
+  for (int64_t c = least < 2 ? 2 : least; c <= least + 40; ++c) {
+    const int64_t ps = p_rt > 0 ? (p_tiles + c - 1) / c : 0, os = o_rt > 0 ? (o_tiles + c - 1) / c : 0;
+    const int64_t pc = ps > 0 ? (p_tiles + ps - 1) / ps : 0, oc = os > 0 ? (o_tiles + os - 1) / os : 0;
+    const int64_t pi = p_lists * ps, oi = o_lists * os, rounds = pi / slots, rest = pi % slots, room = slots - rest;
+    const double tp = START + pc, to = START + oc;
+    const double beside = rest > 0 ? tp : 0, own_beside = (double)((oi + room - 1) / room) * to;
+    const double with = rounds * tp + (beside > own_beside ? beside : own_beside);
+    const double behind = rounds * tp + beside + (double)((oi + slots - 1) / slots) * to;
+    const double t = (with < behind ? with : behind) + (double)(p.rows * Hkv * (ps + os)) / (32 * slots);
+    if (best == 0 || t < best) {
+      best = t;
+      p.p_splits = (int)ps, p.o_splits = (int)os;
+      p.p_chunk = (int)(pc > 0 ? pc : 1), p.o_chunk = (int)(oc > 0 ? oc : 1);
+    }
+    if (c >= p_tiles && c >= o_tiles) break;
+  }
   p.p_rt = (int)(p_rt > 0 ? p_rt : 1);
   p.o_rt = (int)(o_rt > 0 ? o_rt : 1);
-  p.p_splits = p_rt > 0 ? (int)((p_tiles + chunk - 1) / chunk) : 0;
-  p.o_splits = o_rt > 0 ? (int)((o_tiles + chunk - 1) / chunk) : 0;
-  p.p_chunk = p.p_splits > 0 ? (int)((p_tiles + p.p_splits - 1) / p.p_splits) : 1;
-  p.o_chunk = p.o_splits > 0 ? (int)((o_tiles + p.o_splits - 1) / p.o_splits) : 1;
   p.p_items = p_lists * p.p_splits;
   const int64_t deal = p.p_rt > 1 ? 8 * (int64_t)p.p_rt : 1;
   p.p_grid = (p.p_items + deal - 1) / deal * deal;
