@@ -92,12 +92,24 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }
 
-// A token's place in the order: larger is earlier. 0: no candidate.
-__device__ __forceinline__ uint64_t place_of(uint32_t key, int i) {
-  return key > KEY_NONE ? (uint64_t)key << 32 | (uint32_t)~i : 0;
-}
-__device__ __forceinline__ int index_of(uint64_t place) { return (int)~(uint32_t)place; }
-__device__ __forceinline__ float logit_of(uint64_t place) { return of_key(place >> 32); }
+// A token's place in the order: larger is earlier, 0 is no candidate. The key's bits
+// that the type uses, above the index turned round.
+template <typename T>
+struct Order {
+  // low bits of a key that are alike in all of the type's numbers of one sign
+  static constexpr int SPARE = sizeof(T) == 4 ? 0 : std::is_same_v<T, __bf16> ? 16 : 13;
+  int bits;                                 // of an index
+  __device__ __forceinline__ explicit Order(int V) : bits(V > 1 ? 32 - __clz(V - 1) : 1) {}
+  __device__ __forceinline__ uint32_t turned(int i) const { return ~(uint32_t)i & ((1u << bits) - 1); }
+  __device__ __forceinline__ uint64_t place(uint32_t key, int i) const {
+    return key > KEY_NONE ? (uint64_t)(key >> SPARE) << bits | turned(i) : 0;
+  }
+  __device__ __forceinline__ int index(uint64_t place) const { return (int)turned((int)place); }
+  __device__ __forceinline__ float logit(uint64_t place) const {
+    const uint32_t k = (uint32_t)(place >> bits) << SPARE;
+    return of_key(k >> 31 ? k : k | ((1u << SPARE) - 1));
+  }
+};
 
 // 2^t for t <= 0 in units of 2^-bits (bits <= 45): the fraction's power by the
 // polynomial of degree 10 that meets 2^f at the Chebyshev nodes of [-1/2, 1/2]
@@ -146,9 +158,9 @@ struct Scale {
   float topf, step, bar;                    // bar: min_p's, the smallest float at or above it
   int bits;
   bool inf;                                 // an infinite largest logit: the tokens at it share the row
-  __device__ __forceinline__ Scale(const SampleArgs& a, const Setting& s, uint64_t first, uint32_t least) {
+  __device__ __forceinline__ Scale(const SampleArgs& a, const Setting& s, float most, uint32_t least) {
     bits = a.bits;
-    topf = logit_of(first);
+    topf = most;
     inf = topf == INFINITY;
     per = 1.44269504088896340736 / (double)s.t;
     bar = -INFINITY;
@@ -228,22 +240,38 @@ struct Row {
 #pragma unroll
     for (int e = 0; e < E; ++e) f(y[e], index(v, e));
   }
-  // f(vector, logits) of this lane's vectors of a part's tiles, wave w of W every
-  // W-th tile, U loads ahead
-  template <int W, int U, typename F>
-  __device__ __forceinline__ void sweep(int tile0, int tiles, F&& f) const {
-    const int first = tile0 + (int)(threadIdx.x / 64), n = min(tiles - (int)(threadIdx.x / 64), (n_vec + 63) / 64 - first);
-    for (int j = 0; j < n; j += U * W) {
-      u32x4 w[U];
+};
+
+// This lane's vectors of `tiles` tiles from tile0 on, wave w of W every W-th tile, U
+// loads ahead: those of the first vectors are made here.
+template <typename T, int W, int U>
+struct Sweep {
+  using R = Row<T>;
+  const R& row;
+  int first, n;
+  u32x4 w[U];
+  __device__ __forceinline__ Sweep(const R& r, int tile0, int tiles) : row(r) {
+    first = tile0 + (int)(threadIdx.x / 64);
+    n = min(tiles - (int)(threadIdx.x / 64), (r.n_vec + 63) / 64 - first);
 #pragma unroll
-      for (int u = 0; u < U; ++u) w[u] = load((first + j + u * W) * 64 + (int)(threadIdx.x % 64));
+    for (int u = 0; u < U; ++u) w[u] = row.load(vector(u * W));
+  }
+  __device__ __forceinline__ int vector(int j) const { return (first + j) * 64 + (int)(threadIdx.x % 64); }
+  template <typename F>
+  __device__ __forceinline__ void run(F&& f) {   // f(vector, logits)
+    for (int j = 0; j < n; j += U * W) {
+      u32x4 now[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        now[u] = w[u];
+        w[u] = row.load(vector(j + (U + u) * W));
+      }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (j + u * W >= n) break;
-        const int v = (first + j + u * W) * 64 + (int)(threadIdx.x % 64);
-        float y[E];
-        unpack(w[u], v, y);
-        f(v, y);
+        float y[R::E];
+        row.unpack(now[u], vector(j + u * W), y);
+        f(vector(j + u * W), y);
       }
     }
   }
@@ -347,9 +375,10 @@ __global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
   if (a.runs)
     for (int i = part * PART + threadIdx.x; i < BINS; i += a.parts * PART) a.hist[(int64_t)b * BINS + i] = 0;
   const R row(a, b);
+  const Order<T> ord(a.V);
   float most = -INFINITY, least = INFINITY;
   int at = 0;                               // the vector that raised `most` last
-  row.template sweep<PART / 64, 4>(part * a.tiles, a.tiles, [&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
+  Sweep<T, PART / 64, 4>(row, part * a.tiles, a.tiles).run([&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
     float top = y[0];
 #pragma unroll
     for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);   // (a NaN gives way)
@@ -366,7 +395,7 @@ __global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
   uint64_t first = 0;
   if (key > KEY_NONE)
     row.each(at, [&](float y, int i) __attribute__((always_inline)) {
-      if (first == 0 && key_of(y) == key) first = place_of(key, i);
+      if (first == 0 && key_of(y) == key) first = ord.place(key, i);
     });
   uint32_t g = key, low = least < INFINITY ? key_of(least) : key > KEY_NONE ? key : ~0u;
   for (int d = 1; d < a.lanes; d *= 2) g = max(g, (uint32_t)__shfl_xor((int)g, d));
@@ -401,37 +430,48 @@ template <typename T>
 __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
   using R = Row<T>;
   __shared__ uint64_t s_mem[LIST];          // the list, or the histogram
-  __shared__ uint32_t s_cnt[2][PART / 64], s_n, s_at;
-  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  __shared__ uint32_t s_n, s_at;
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64;
   const Setting s = setting_of(a, b);
   const bool hist = s.sums() && s.run;
   if (s.greedy || (!s.list && !hist)) return;
   const R row(a, b);
+  const Order<T> ord(a.V);
   if (s.list) {
-    // The largest number of 16 bits that is no larger than the k-th group maximum's
-    // first 16: bit by bit, by the count of maxima that reach it.
-    const int n_max = a.parts * a.groups;
+    Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
+    // The largest number of 16 bits that is no larger than the k-th largest group
+    // maximum's first 16: bit by bit, by the count of maxima that reach it, each wave
+    // for itself. For a small k the groups of one lane are taken as eight.
+    const int n_max = a.parts * a.groups;   // (a multiple of 4)
     const uint32_t* mx = a.maxima + (int64_t)b * n_max;
-    uint32_t key[GROUPS / PART], low = 0;
+    uint32_t key[GROUPS / 64], low = 0;
 #pragma unroll
-    for (int i = 0; i < GROUPS / PART; ++i) key[i] = i * PART + (int)threadIdx.x < n_max ? mx[i * PART + threadIdx.x] >> 16 : 0;
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t c = low | 1u << bit;
-      int n = 0;
+    for (int i = 0; i < GROUPS / 256; ++i) {
+      const u32x4 w = *(const u32x4*)(mx + min((i * 64 + lane) * 4, n_max - 4));
 #pragma unroll
-      for (int i = 0; i < GROUPS / PART; ++i) n += __popcll(__ballot(key[i] >= c));
-      if (lane == 0) s_cnt[bit % 2][wave] = n;
-      __syncthreads();
-      n = 0;
+      for (int e = 0; e < 4; ++e) key[4 * i + e] = (i * 64 + lane) * 4 < n_max ? w[e] >> 16 : 0;
+    }
+    auto search = [&](auto many) __attribute__((always_inline)) {
+      for (int bit = 15; bit >= 0; --bit) {
+        const uint32_t c = low | 1u << bit;
+        int n = 0;
 #pragma unroll
-      for (int w = 0; w < PART / 64; ++w) n += s_cnt[bit % 2][w];
-      if (n >= s.k) low = c;
+        for (int i = 0; i < decltype(many)::value; ++i) n += __popcll(__ballot(key[i] >= c));
+        if (n >= s.k) low = c;
+      }
+    };
+    if (s.k <= 384) {
+#pragma unroll
+      for (int i = 8; i < GROUPS / 64; ++i) key[i % 8] = max(key[i % 8], key[i]);
+      search(std::integral_constant<int, 8>{});
+    } else {
+      search(std::integral_constant<int, GROUPS / 64>{});
     }
     const uint32_t from = max(low << 16, KEY_NONE + 1);
     const float bar = of_key(from);
     if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
-    row.template sweep<PART / 64, 4>(part * a.tiles, a.tiles, [&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
+    sweep.run([&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
       float top = y[0];
 #pragma unroll
       for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);
@@ -440,7 +480,7 @@ __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
       for (int e = 0; e < R::E; ++e)
         if (y[e] >= bar) {
           const uint32_t at = atomicAdd(&s_n, 1u);
-          if (at < LIST) s_mem[at] = place_of(key_of(y[e]), row.index(v, e));
+          if (at < LIST) s_mem[at] = ord.place(key_of(y[e]), row.index(v, e));
         }
     });
     __syncthreads();
@@ -451,10 +491,10 @@ __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
   uint32_t least;
   row_ends(a, b, first, least);
   if (first == 0) return;
-  const Scale sc(a, s, first, least);
+  const Scale sc(a, s, ord.logit(first), least);
   for (int i = threadIdx.x; i < BINS; i += PART) s_mem[i] = 0;
   __syncthreads();
-  row.template sweep<PART / 64, 2>(part * a.tiles, a.tiles, [&](int, const float (&y)[R::E]) __attribute__((always_inline)) {
+  Sweep<T, PART / 64, 2>(row, part * a.tiles, a.tiles).run([&](int, const float (&y)[R::E]) __attribute__((always_inline)) {
     float z[R::E];
     uint64_t w[R::E];
     sc.at(y, z);
@@ -513,17 +553,19 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
   const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64;
   const Setting s = setting_of(a, b);
   if (!s.sums()) return;
+  const R row(a, b);
+  const Order<T> ord(a.V);
+  Sweep<T, PART / 64, 2> sweep(row, part * a.tiles, a.tiles);
   uint64_t first;
   uint32_t least;
   row_ends(a, b, first, least);
   if (first == 0) return;
-  const Scale sc(a, s, first, least);
+  const Scale sc(a, s, ord.logit(first), least);
   uint64_t before, goal;
   const int border = s.run ? border_bin<PART>(a, b, s.p, s_scan, before, goal) : BINS;
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
-  const R row(a, b);
-  row.template sweep<PART / 64, 2>(part * a.tiles, a.tiles, [&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
+  sweep.run([&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
     float z[R::E];
     uint64_t sum = 0, w[R::E];
     sc.at(y, z);
@@ -546,7 +588,7 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
         for (int e = 0; e < R::E; ++e)
           if (at[e] == border) {
             const uint32_t n = atomicAdd(&s_n, 1u);
-            if (n < LIST) s_list[n] = place_of(key_of(y[e]), row.index(v, e));
+            if (n < LIST) s_list[n] = ord.place(key_of(y[e]), row.index(v, e));
           }
       }
     } else {
@@ -570,36 +612,45 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
 // Of the n values, those in [lo, hi] (lo >= 1): the largest at which the measure,
 // summed from the largest value down, reaches `goal`; 0 if none does. Nine bits of
 // the range at a time, by histograms, until one value is left.
-constexpr int REACH = FIN + FIN / 2 + 24;    // words of s
+constexpr int REACH = 3 * FIN + 64;          // words of s
 template <typename V, typename M>
 __device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_t lo, uint64_t hi, uint64_t goal, uint64_t* s) {
-  uint64_t* s_scan = s + FIN;
-  uint32_t* s_cnt = (uint32_t*)(s + FIN + 24);
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, wave = tid / 64;
+  uint64_t* s_scan = s + 3 * FIN;
+  __syncthreads();
+  s[tid] = 0;
+  ((uint32_t*)(s + 2 * FIN))[tid] = 0;
+  if (tid < 2) s_scan[32 + 4 * tid] = 0;
   __syncthreads();
   for (int pass = 0; ; ++pass) {
+    // the two passes' places take turns: what one leaves is cleared by the next
+    uint64_t *bin = s + pass % 2 * FIN, *sums = s_scan + pass % 2 * 16, *found = s_scan + 32 + pass % 2 * 4;
+    uint32_t* cnt = (uint32_t*)(s + 2 * FIN) + pass % 2 * FIN;
     const int bits = 64 - __clzll((long long)((hi - lo) | 1)), shift = bits > 9 ? bits - 9 : 0;
-    uint64_t* found = s_scan + 8 + pass % 2 * 4;   // (the last pass's may still be read)
-    s[tid] = 0;
-    s_cnt[tid] = 0;
-    if (tid == 0) found[0] = 0;
-    __syncthreads();
     for (int i = tid; i < n; i += FIN) {
       const uint64_t x = value(i);
       if (x >= lo && x <= hi) {
         const int at = (int)((x - lo) >> shift);
-        atomicAdd((ull*)&s[at], (ull)measure(i));
-        atomicAdd(&s_cnt[at], 1u);
+        atomicAdd((ull*)&bin[at], (ull)measure(i));
+        atomicAdd(&cnt[at], 1u);
       }
     }
     __syncthreads();
-    uint64_t total;
-    const uint64_t mine = s[FIN - 1 - tid], before = block_before<FIN>(mine, s_scan, total);
+    const uint64_t mine = bin[FIN - 1 - tid], upto = scan64(mine);
+    const uint32_t many = cnt[FIN - 1 - tid];
+    if (tid % 64 == 63) sums[wave] = upto;
+    s[(pass + 1) % 2 * FIN + tid] = 0;
+    ((uint32_t*)(s + 2 * FIN))[(pass + 1) % 2 * FIN + tid] = 0;
+    __syncthreads();
+    uint64_t before = upto - mine;
+#pragma unroll
+    for (int w = 0; w < FIN / 64; ++w) before += w < wave ? sums[w] : 0;
     if (before < goal && before + mine >= goal) {
       found[0] = FIN - tid;                 // the bin and 1
       found[1] = before;
-      found[2] = s_cnt[FIN - 1 - tid];
+      found[2] = many;
     }
+    if (tid == 0) s_scan[32 + (pass + 1) % 2 * 4] = 0;
     __syncthreads();
     if (found[0] == 0) return 0;
     goal -= found[1];
@@ -609,10 +660,10 @@ __device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_
     if (found[2] == 1) {
       for (int i = tid; i < n; i += FIN) {
         const uint64_t x = value(i);
-        if (x >= lo && x <= hi) s_scan[16] = x;
+        if (x >= lo && x <= hi) s_scan[40] = x;
       }
       __syncthreads();
-      return s_scan[16];
+      return s_scan[40];
     }
   }
 }
@@ -624,6 +675,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
   const Setting s = setting_of(a, b);
   const R row(a, b);
+  const Order<T> ord(a.V);
   const uint32_t n_cand = SPLIT ? a.count[b] : 0;
   uint64_t first;
   uint32_t least = ~0u;
@@ -633,7 +685,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     first = 0;
     for (int v = tid; v < row.n_vec; v += FIN)
       row.each(v, [&](float y, int i) __attribute__((always_inline)) {
-        const uint64_t place = place_of(key_of(y), i);
+        const uint64_t place = ord.place(key_of(y), i);
         if (i >= 0 && i < a.V) s_list[i] = place;
         first = place > first ? place : first;
       });
@@ -644,11 +696,11 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     a.logp[b] = logp;
   };
   if (first == 0 || s.greedy) {
-    if (tid == 0) first == 0 ? done(0, __builtin_nanf("")) : done(index_of(first), 0.f);
+    if (tid == 0) first == 0 ? done(0, __builtin_nanf("")) : done(ord.index(first), 0.f);
     return;
   }
-  const Scale sc(a, s, first, SPLIT ? least : KEY_NONE + 1);
-  auto weight = [&](uint64_t place) __attribute__((always_inline)) { return sc.weight(sc.at(logit_of(place))); };
+  const Scale sc(a, s, ord.logit(first), SPLIT ? least : KEY_NONE + 1);
+  auto weight = [&](uint64_t place) __attribute__((always_inline)) { return sc.weight(sc.at(ord.logit(place))); };
   auto drawn = [&](float y, int i, uint64_t total) __attribute__((always_inline)) {
     const double d = ((double)sc.at(y) - sc.top) / (double)s.t;
     done(i, (float)(d - log(ldexp((double)total, -a.bits))));
@@ -685,13 +737,13 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
       const uint64_t goal = part_of(s.p, total_of([&](int i) { return s_list[i] >= last; }), true);
       last = goal <= 1 ? first : reach(n, place, [&](int i) { return s_w[i]; }, last > 1 ? last : least_place, first, goal, s_scan);
     }
-    auto kept = [&](int i) __attribute__((always_inline)) { return s_list[i] >= last && logit_of(s_list[i]) >= sc.bar; };
+    auto kept = [&](int i) __attribute__((always_inline)) { return s_list[i] >= last && ord.logit(s_list[i]) >= sc.bar; };
     const uint64_t total = total_of(kept), aim = aim_of(total);
     // by index: the first one is the largest number
-    auto turned = [&](int i) __attribute__((always_inline)) { return kept(i) ? (uint64_t)(uint32_t)s_list[i] : 0; };
-    const uint64_t at = reach(n, turned, [&](int i) { return s_w[i]; }, (uint32_t)~(a.V - 1), ~0u, aim + 1, s_scan);
+    auto turned = [&](int i) __attribute__((always_inline)) { return kept(i) ? (uint64_t)ord.turned(ord.index(s_list[i])) + 1 : 0; };
+    const uint64_t at = reach(n, turned, [&](int i) { return s_w[i]; }, 1, (uint64_t)ord.turned(0) + 1, aim + 1, s_scan);
     for (int i = tid; i < n; i += FIN)
-      if (turned(i) == at) drawn(logit_of(s_list[i]), index_of(s_list[i]), total);
+      if (turned(i) == at) drawn(ord.logit(s_list[i]), ord.index(s_list[i]), total);
     return;
   }
   if constexpr (SPLIT) {
@@ -720,8 +772,8 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
       most = block_all<FIN>(most, s_scan, Most());
       last = reach(n, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, ~least_off, most, goal - before, s_scan);
       for (int i = tid; i < n; i += FIN)
-        if (s_list[i] >= last && logit_of(s_list[i]) >= sc.bar)
-          atomicAdd((ull*)&s_slot[(index_of(s_list[i]) + row.shift) / R::E / 64 / per], (ull)s_w[i]);
+        if (s_list[i] >= last && ord.logit(s_list[i]) >= sc.bar)
+          atomicAdd((ull*)&s_slot[(ord.index(s_list[i]) + row.shift) / R::E / 64 / per], (ull)s_w[i]);
     }
     for (int i = tid; i < tiles; i += FIN) {
       const uint64_t w = sums[i];
@@ -736,12 +788,12 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     };
     auto far = [&](auto&& measure, uint64_t goal) {
       uint64_t prefix = 0, before = 0;
-      for (int low = 55; low >= 0; low -= 11) {
+      for (int low = 44; low >= 0; low -= 11) {   // (56 bits at most)
         for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
         __syncthreads();
         over([&](float y, int i) __attribute__((always_inline)) {
-          const uint64_t place = place_of(key_of(y), i);
-          if (place < last || (low < 55 && place >> (low + 11) != prefix)) return;
+          const uint64_t place = ord.place(key_of(y), i);
+          if (place < last || (low < 44 && place >> (low + 11) != prefix)) return;
           const uint64_t w = measure(y);
           if (w) atomicAdd((ull*)&s_slot[place >> low & (SLOTS - 1)], (ull)w);
         });
@@ -770,7 +822,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     if (s.run) {
       uint64_t sum = 0;
       over([&](float y, int i) __attribute__((always_inline)) {
-        if (place_of(key_of(y), i) >= last) sum += mass(y);
+        if (ord.place(key_of(y), i) >= last) sum += mass(y);
       });
       sum = block_all<FIN>(sum, s_scan, Plus());
       const uint64_t goal = part_of(s.p, sum, true);
@@ -783,7 +835,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
       uint64_t sum = 0;
       if (v < row.n_vec)
         row.each(v, [&](float y, int i) __attribute__((always_inline)) {
-          if (place_of(key_of(y), i) >= last && y >= sc.bar) sum += mass(y);
+          if (ord.place(key_of(y), i) >= last && y >= sc.bar) sum += mass(y);
         });
       sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
       if (lane == 0 && sum) atomicAdd((ull*)&s_slot[v / 64 / per], (ull)sum);
@@ -814,7 +866,7 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     row.unpack(row.load(v), v, y);
 #pragma unroll
     for (int e = 0; e < R::E; ++e) {
-      const uint64_t place = place_of(key_of(y[e]), row.index(v, e)), z = sc.weight(sc.at(y[e]));
+      const uint64_t place = ord.place(key_of(y[e]), row.index(v, e)), z = sc.weight(sc.at(y[e]));
       const int at = sc.bin(sc.at(y[e]));
       const bool in = border < 0 ? place >= last : border == BINS || at < border || (at == border && place >= last);
       w[e] = in && y[e] >= sc.bar ? z : 0;
