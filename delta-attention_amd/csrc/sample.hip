@@ -31,6 +31,7 @@
 //   finish  a workgroup a row: the last token kept, by histograms over the list;
 //           the tile at which the sum passes u times the total, and the token in it
 // Short rows take the last launch alone, the whole row their list.
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -52,12 +53,11 @@ constexpr int PART = 256;                    // threads of a part
 constexpr int LIST = 3584;                   // tokens of a row's list (two finishing workgroups' LDS a CU)
 constexpr int BINS = 768;                    // of a part's histogram
 constexpr int GROUPS = 2048;                 // group maxima of a row at most
-constexpr int FIN = 512;                     // threads of the finish
 constexpr int SLOTS = 2048;                  // tile sums in LDS; bins of a radix pass
 
 struct Part {
   uint64_t first;                            // the first place in the order, 0: no candidate
-  uint32_t least, pad;                       // the smallest candidate's key
+  uint32_t low, pad;                         // the smallest candidate's key turned round, 0: no candidate
 };
 
 struct SampleArgs {
@@ -111,13 +111,14 @@ struct Order {
   }
 };
 
-// 2^t for t <= 0 in units of 2^-bits (bits <= 45): the fraction's power by the
-// polynomial of degree 10 that meets 2^f at the Chebyshev nodes of [-1/2, 1/2]
-// (2^-51 of it, rounding included; the series takes two terms more), the whole
-// one by the exponent; rounded to an integer by what 2^52 leaves of it.
+// 2^t for t <= 0 in units of 2^-bits (bits <= 45): the fraction's power by
+// the polynomial of degree 10 that meets 2^f at the Chebyshev nodes of [-1/2, 1/2]
+// (2^-51 of it, rounding included; the series takes two terms more), the whole one
+// by the exponent. Whole numbers come from what 2^52 leaves of a sum: of t, and of
+// the weight, which is rounded so.
 __device__ __forceinline__ uint64_t weight_of(double t, int bits) {
   t = fmax(t, -200.0);                      // (2^-200 of the largest: none; so is what is no candidate)
-  const double n = rint(t), f = t - n;
+  const double whole = t + 6755399441055744.0, f = t - (whole - 6755399441055744.0);   // (1.5 * 2^52)
   double p = 7.072585949269223e-09;
   constexpr double c[] = {1.0208690299958306e-07, 1.321544258792169e-06, 1.5252657260200837e-05, 0.0001540353044173605,
                           0.0013333558230164974, 0.009618129107606888, 0.05550410866444772, 0.24022650695910097,
@@ -128,7 +129,10 @@ __device__ __forceinline__ uint64_t weight_of(double t, int bits) {
     asm("" : "+s"(k));                      // (a scalar operand: else each term copies it first)
     p = fma(p, f, k);
   }
-  return (uint64_t)__double_as_longlong(ldexp(p, (int)n + bits) + 4503599627370496.0) - 0x4330000000000000ull;
+  const uint64_t w = (uint64_t)__double_as_longlong(p);
+  const uint32_t hi = (uint32_t)(w >> 32) + (((uint32_t)__double_as_longlong(whole) + bits) << 20);
+  const double scaled = __longlong_as_double((long long)((uint64_t)hi << 32 | (uint32_t)w));
+  return (uint64_t)__double_as_longlong(scaled + 4503599627370496.0) - 0x4330000000000000ull;
 }
 
 // What a row asks for.
@@ -170,6 +174,7 @@ struct Scale {
       bar = (float)y;
       if ((double)bar < y) bar = of_key(key_of(bar) + 1);
     }
+    bar = inf ? INFINITY : fmaxf(bar, -FLT_MAX);   // (candidates alone pass it)
     if (inf) topf = 0.f;
     top = topf;
     const double far = a.bits + 2, all = (top - (inf ? 0.0 : (double)of_key(least))) * per;
@@ -352,174 +357,159 @@ __device__ __forceinline__ uint64_t part_of(float f, uint64_t total, bool up) {
   return (uint64_t)((y + (up ? ((u128)1 << shift) - 1 : 0)) >> shift);
 }
 
-// A row's first place and smallest candidate, from its parts'.
-__device__ __forceinline__ void row_ends(const SampleArgs& a, int b, uint64_t& first, uint32_t& least) {
-  const Part* p = a.part + (int64_t)b * a.parts;
-  first = 0, least = ~0u;
-  for (int i = threadIdx.x % 64; i < a.parts; i += 64) {
-    first = p[i].first > first ? p[i].first : first;
-    least = min(least, p[i].least);
-  }
-  first = wave_all(first, Most());
-  least = ~(uint32_t)wave_all(~least, Most());
-}
-
 // ---------------------------------------------------------------------------
-template <typename T>
-__global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
-  using R = Row<T>;
-  __shared__ uint64_t s_first[PART / 64];
-  __shared__ uint32_t s_least[PART / 64];
-  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  if (part == 0 && threadIdx.x == 0) a.count[b] = 0;
-  if (a.runs)
-    for (int i = part * PART + threadIdx.x; i < BINS; i += a.parts * PART) a.hist[(int64_t)b * BINS + i] = 0;
-  const R row(a, b);
-  const Order<T> ord(a.V);
-  float most = -INFINITY, least = INFINITY;
-  int at = 0;                               // the vector that raised `most` last
-  Sweep<T, PART / 64, 4>(row, part * a.tiles, a.tiles).run([&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
+// The passes over a row, or a part of one.
+
+// This thread's largest number, the vector that held it first, and (want) its
+// smallest candidate.
+template <typename S>
+__device__ __forceinline__ void ends_of(S& sweep, bool want, float& most, int& at, float& least) {
+  constexpr int E = S::R::E;
+  most = -INFINITY, least = INFINITY, at = 0;
+  sweep.run([&](int v, const float (&y)[E]) __attribute__((always_inline)) {
     float top = y[0];
 #pragma unroll
-    for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);   // (a NaN gives way)
-    if (a.runs) {
+    for (int e = 1; e < E; ++e) top = fmaxf(top, y[e]);   // (a NaN gives way)
+    if (want) {
 #pragma unroll
-      for (int e = 0; e < R::E; ++e) least = fminf(least, y[e] > -INFINITY ? y[e] : INFINITY);
+      for (int e = 0; e < E; ++e) least = fminf(least, y[e] > -INFINITY ? y[e] : INFINITY);
     }
     if (top > most) {
       most = top;
       at = v;
     }
   });
+}
+// Its first place and its smallest candidate's key turned round (0: no candidate).
+template <typename T>
+__device__ __forceinline__ void ends_of(const Row<T>& row, const Order<T>& ord, float most, int at, float least,
+                                        uint64_t& first, uint32_t& low) {
   const uint32_t key = key_of(most);
-  uint64_t first = 0;
+  first = 0;
   if (key > KEY_NONE)
     row.each(at, [&](float y, int i) __attribute__((always_inline)) {
       if (first == 0 && key_of(y) == key) first = ord.place(key, i);
     });
-  uint32_t g = key, low = least < INFINITY ? key_of(least) : key > KEY_NONE ? key : ~0u;
-  for (int d = 1; d < a.lanes; d *= 2) g = max(g, (uint32_t)__shfl_xor((int)g, d));
-  if (threadIdx.x % a.lanes == 0) a.maxima[((int64_t)b * a.parts + part) * a.groups + threadIdx.x / a.lanes] = g;
-  first = wave_all(first, Most());
-  low = ~(uint32_t)wave_all(~low, Most());
-  if (lane == 0) {
-    s_first[wave] = first;
-    s_least[wave] = low;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < PART / 64; ++w) {
-      first = s_first[w] > first ? s_first[w] : first;
-      low = min(low, s_least[w]);
-    }
-    a.part[(int64_t)b * a.parts + part] = Part{first, low, 0};
-  }
+  low = least < INFINITY ? ~key_of(least) : key > KEY_NONE ? ~key : 0u;
 }
 
-// Appends the places that the part holds in s_list to the row's list.
-__device__ __forceinline__ void append(const SampleArgs& a, int b, const uint64_t* s_list, uint32_t n, uint32_t* s_at) {
-  __syncthreads();
-  if (threadIdx.x == 0 && n > 0) *s_at = atomicAdd(a.count + b, n);
-  __syncthreads();
-  if (n == 0 || n > LIST) return;
-  for (uint32_t i = threadIdx.x; i < n; i += PART)
-    if (*s_at + i < LIST) a.list[(int64_t)b * LIST + *s_at + i] = s_list[i];
+// A number that no more than k of the groups' maxima's first 16 bits pass: the
+// largest one of 16 bits that is no larger than the k-th largest maximum, bit by bit,
+// by the count of maxima that reach it. Each wave works for itself on all maxima, M a
+// lane; up to 384 the groups of a lane are taken as eight.
+template <int M>
+__device__ __forceinline__ float list_bar(uint32_t (&key)[M], int k) {
+  uint32_t low = 0;
+  auto search = [&](auto many) __attribute__((always_inline)) {
+    for (int bit = 15; bit >= 0; --bit) {
+      const uint32_t c = low | 1u << bit;
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < decltype(many)::value; ++i) n += __popcll(__ballot(key[i] >> 16 >= c));
+      if (n >= k) low = c;
+    }
+  };
+  if (k <= 384) {
+#pragma unroll
+    for (int i = 8; i < M; ++i) key[i % 8] = max(key[i % 8], key[i]);
+    search(std::integral_constant<int, 8>{});
+  } else {
+    search(std::integral_constant<int, M>{});
+  }
+  return of_key(max(low << 16, KEY_NONE + 1));
 }
 
-template <typename T>
-__global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
-  using R = Row<T>;
-  __shared__ uint64_t s_mem[LIST];          // the list, or the histogram
-  __shared__ uint32_t s_n, s_at;
-  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64;
-  const Setting s = setting_of(a, b);
-  const bool hist = s.sums() && s.run;
-  if (s.greedy || (!s.list && !hist)) return;
-  const R row(a, b);
-  const Order<T> ord(a.V);
-  if (s.list) {
-    Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
-    // The largest number of 16 bits that is no larger than the k-th largest group
-    // maximum's first 16: bit by bit, by the count of maxima that reach it, each wave
-    // for itself. For a small k the groups of one lane are taken as eight.
-    const int n_max = a.parts * a.groups;   // (a multiple of 4)
-    const uint32_t* mx = a.maxima + (int64_t)b * n_max;
-    uint32_t key[GROUPS / 64], low = 0;
+// The places of the logits from `bar` on; n counts them (also past the list's end).
+template <typename S, typename O>
+__device__ __forceinline__ void gather_into(S& sweep, const O& ord, float bar, uint64_t* list, uint32_t* n) {
+  constexpr int E = S::R::E;
+  sweep.run([&](int v, const float (&y)[E]) __attribute__((always_inline)) {
+    float top = y[0];
 #pragma unroll
-    for (int i = 0; i < GROUPS / 256; ++i) {
-      const u32x4 w = *(const u32x4*)(mx + min((i * 64 + lane) * 4, n_max - 4));
+    for (int e = 1; e < E; ++e) top = fmaxf(top, y[e]);
+    if (!(top >= bar)) return;              // (most vectors)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) key[4 * i + e] = (i * 64 + lane) * 4 < n_max ? w[e] >> 16 : 0;
-    }
-    auto search = [&](auto many) __attribute__((always_inline)) {
-      for (int bit = 15; bit >= 0; --bit) {
-        const uint32_t c = low | 1u << bit;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < decltype(many)::value; ++i) n += __popcll(__ballot(key[i] >= c));
-        if (n >= s.k) low = c;
+    for (int e = 0; e < E; ++e)
+      if (y[e] >= bar) {
+        const uint32_t at = atomicAdd(n, 1u);
+        if (at < LIST) list[at] = ord.place(key_of(y[e]), sweep.row.index(v, e));
       }
-    };
-    if (s.k <= 384) {
-#pragma unroll
-      for (int i = 8; i < GROUPS / 64; ++i) key[i % 8] = max(key[i % 8], key[i]);
-      search(std::integral_constant<int, 8>{});
-    } else {
-      search(std::integral_constant<int, GROUPS / 64>{});
-    }
-    const uint32_t from = max(low << 16, KEY_NONE + 1);
-    const float bar = of_key(from);
-    if (threadIdx.x == 0) s_n = 0;
-    __syncthreads();
-    sweep.run([&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
-      float top = y[0];
-#pragma unroll
-      for (int e = 1; e < R::E; ++e) top = fmaxf(top, y[e]);
-      if (!(top >= bar)) return;            // (most vectors)
-#pragma unroll
-      for (int e = 0; e < R::E; ++e)
-        if (y[e] >= bar) {
-          const uint32_t at = atomicAdd(&s_n, 1u);
-          if (at < LIST) s_mem[at] = ord.place(key_of(y[e]), row.index(v, e));
-        }
-    });
-    __syncthreads();
-    append(a, b, s_mem, s_n, &s_at);
-    return;
-  }
-  uint64_t first;
-  uint32_t least;
-  row_ends(a, b, first, least);
-  if (first == 0) return;
-  const Scale sc(a, s, ord.logit(first), least);
-  for (int i = threadIdx.x; i < BINS; i += PART) s_mem[i] = 0;
-  __syncthreads();
-  Sweep<T, PART / 64, 2>(row, part * a.tiles, a.tiles).run([&](int, const float (&y)[R::E]) __attribute__((always_inline)) {
-    float z[R::E];
-    uint64_t w[R::E];
+  });
+}
+
+// The weights' histogram.
+template <typename S>
+__device__ __forceinline__ void hist_into(S& sweep, const Scale& sc, uint64_t* hist) {
+  constexpr int E = S::R::E;
+  sweep.run([&](int, const float (&y)[E]) __attribute__((always_inline)) {
+    float z[E];
+    uint64_t w[E];
     sc.at(y, z);
     sc.weights(z, w);
 #pragma unroll
-    for (int e = 0; e < R::E; ++e) {
+    for (int e = 0; e < E; ++e) {
       const int at = sc.bin(z[e]);
-      if (at < BINS) atomicAdd((ull*)&s_mem[at], (ull)w[e]);
+      if (at < BINS) atomicAdd((ull*)&hist[at], (ull)w[e]);
     }
   });
-  __syncthreads();
-  ull* to = (ull*)a.hist + (int64_t)b * BINS;
-  for (int i = threadIdx.x; i < BINS; i += PART)
-    if (s_mem[i]) atomicAdd(to + i, (ull)s_mem[i]);
+}
+
+// put(tile, kept weight); with a border (below BINS) the tokens of that bin go to the
+// list, and those of the bins before it are kept.
+template <typename S, typename O, typename P>
+__device__ __forceinline__ void sums_into(S& sweep, const O& ord, const Scale& sc, int border, uint64_t* list, uint32_t* n,
+                                          P&& put) {
+  constexpr int E = S::R::E;
+  sweep.run([&](int v, const float (&y)[E]) __attribute__((always_inline)) {
+    float z[E];
+    uint64_t sum = 0, w[E];
+    sc.at(y, z);
+    if (border < BINS) {
+      bool listed = false, any = false;
+      int at[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        at[e] = sc.bin(z[e]);
+        listed |= at[e] == border;
+        any |= at[e] < border;
+      }
+      if (__any(any)) {
+        sc.weights(z, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += at[e] < border && y[e] >= sc.bar ? w[e] : 0;
+      }
+      if (listed) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (at[e] == border) {
+            const uint32_t i = atomicAdd(n, 1u);
+            if (i < LIST) list[i] = ord.place(key_of(y[e]), sweep.row.index(v, e));
+          }
+      }
+    } else {
+      bool any = false;
+#pragma unroll
+      for (int e = 0; e < E; ++e) any |= y[e] >= sc.bar;
+      if (__any(any)) {
+        sc.weights(z, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) sum += y[e] >= sc.bar ? w[e] : 0;
+      }
+    }
+    sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
+    if (threadIdx.x % 64 == 0) put(v / 64, sum);
+  });
 }
 
 // The bin at which a row's histogram reaches p times its total, the weight of
 // those before it and what is to be reached.
 template <int N>
-__device__ __forceinline__ int border_bin(const SampleArgs& a, int b, float p, uint64_t* s, uint64_t& before, uint64_t& goal) {
+__device__ __forceinline__ int border_bin(const uint64_t* hist, float p, uint64_t* s, uint64_t& before, uint64_t& goal) {
   constexpr int PER = BINS / 256;           // bins of a thread
   static_assert(BINS % 256 == 0 && N >= 256, "256 threads hold the bins");
   uint64_t sum[PER] = {}, mine = 0, total;
   if (threadIdx.x < 256) {
-    const uint64_t* h = a.hist + (int64_t)b * BINS + threadIdx.x * PER;
+    const uint64_t* h = hist + threadIdx.x * PER;
 #pragma unroll
     for (int e = 0; e < PER; ++e) sum[e] = h[e];
 #pragma unroll
@@ -545,15 +535,118 @@ __device__ __forceinline__ int border_bin(const SampleArgs& a, int b, float p, u
   return (int)s[0];
 }
 
+// ---------------------------------------------------------------------------
+// A row's parts, a launch a pass.
+
 template <typename T>
-__global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
-  using R = Row<T>;
-  __shared__ uint64_t s_list[LIST], s_scan[8];
+__global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
+  __shared__ uint64_t s_first[PART / 64];
+  __shared__ uint32_t s_low[PART / 64];
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  if (part == 0 && threadIdx.x == 0) a.count[b] = 0;
+  if (a.runs)
+    for (int i = part * PART + threadIdx.x; i < BINS; i += a.parts * PART) a.hist[(int64_t)b * BINS + i] = 0;
+  const Row<T> row(a, b);
+  const Order<T> ord(a.V);
+  Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
+  float most, least;
+  int at;
+  ends_of(sweep, a.runs, most, at, least);
+  uint32_t g = key_of(most), low;
+  for (int d = 1; d < a.lanes; d *= 2) g = max(g, (uint32_t)__shfl_xor((int)g, d));
+  if (threadIdx.x % a.lanes == 0) a.maxima[((int64_t)b * a.parts + part) * a.groups + threadIdx.x / a.lanes] = g;
+  uint64_t first;
+  ends_of(row, ord, most, at, least, first, low);
+  first = wave_all(first, Most());
+  low = (uint32_t)wave_all(low, Most());
+  if (lane == 0) {
+    s_first[wave] = first;
+    s_low[wave] = low;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < PART / 64; ++w) {
+      first = s_first[w] > first ? s_first[w] : first;
+      low = max(low, s_low[w]);
+    }
+    a.part[(int64_t)b * a.parts + part] = Part{first, low, 0};
+  }
+}
+
+// A row's first place and smallest candidate's key, from its parts'.
+__device__ __forceinline__ void row_ends(const SampleArgs& a, int b, uint64_t& first, uint32_t& least) {
+  const Part* p = a.part + (int64_t)b * a.parts;
+  uint32_t low = 0;
+  first = 0;
+  for (int i = threadIdx.x % 64; i < a.parts; i += 64) {
+    first = p[i].first > first ? p[i].first : first;
+    low = max(low, p[i].low);
+  }
+  first = wave_all(first, Most());
+  least = ~(uint32_t)wave_all(low, Most());
+}
+
+// Appends the places that the part holds in s_list to the row's list.
+__device__ __forceinline__ void append(const SampleArgs& a, int b, const uint64_t* s_list, uint32_t n, uint32_t* s_at) {
+  __syncthreads();
+  if (threadIdx.x == 0 && n > 0) *s_at = atomicAdd(a.count + b, n);
+  __syncthreads();
+  if (n == 0 || n > LIST) return;
+  for (uint32_t i = threadIdx.x; i < n; i += PART)
+    if (*s_at + i < LIST) a.list[(int64_t)b * LIST + *s_at + i] = s_list[i];
+}
+
+template <typename T>
+__global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
+  __shared__ uint64_t s_mem[LIST];          // the list, or the histogram
   __shared__ uint32_t s_n, s_at;
   const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64;
   const Setting s = setting_of(a, b);
+  if (s.greedy || (!s.list && !(s.sums() && s.run))) return;
+  const Row<T> row(a, b);
+  const Order<T> ord(a.V);
+  if (s.list) {
+    Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
+    const int n_max = a.parts * a.groups;   // (a multiple of 4)
+    const uint32_t* mx = a.maxima + (int64_t)b * n_max;
+    uint32_t key[GROUPS / 64];
+#pragma unroll
+    for (int i = 0; i < GROUPS / 256; ++i) {
+      const u32x4 w = *(const u32x4*)(mx + min((i * 64 + lane) * 4, n_max - 4));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) key[4 * i + e] = (i * 64 + lane) * 4 < n_max ? w[e] : 0;
+    }
+    const float bar = list_bar(key, s.k);
+    if (threadIdx.x == 0) s_n = 0;
+    __syncthreads();
+    gather_into(sweep, ord, bar, s_mem, &s_n);
+    __syncthreads();
+    append(a, b, s_mem, s_n, &s_at);
+    return;
+  }
+  uint64_t first;
+  uint32_t least;
+  row_ends(a, b, first, least);
+  if (first == 0) return;
+  const Scale sc(a, s, ord.logit(first), least);
+  for (int i = threadIdx.x; i < BINS; i += PART) s_mem[i] = 0;
+  __syncthreads();
+  Sweep<T, PART / 64, 2> sweep(row, part * a.tiles, a.tiles);
+  hist_into(sweep, sc, s_mem);
+  __syncthreads();
+  ull* to = (ull*)a.hist + (int64_t)b * BINS;
+  for (int i = threadIdx.x; i < BINS; i += PART)
+    if (s_mem[i]) atomicAdd(to + i, (ull)s_mem[i]);
+}
+
+template <typename T>
+__global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
+  __shared__ uint64_t s_list[LIST], s_scan[8];
+  __shared__ uint32_t s_n, s_at;
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts;
+  const Setting s = setting_of(a, b);
   if (!s.sums()) return;
-  const R row(a, b);
+  const Row<T> row(a, b);
   const Order<T> ord(a.V);
   Sweep<T, PART / 64, 2> sweep(row, part * a.tiles, a.tiles);
   uint64_t first;
@@ -562,91 +655,56 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
   if (first == 0) return;
   const Scale sc(a, s, ord.logit(first), least);
   uint64_t before, goal;
-  const int border = s.run ? border_bin<PART>(a, b, s.p, s_scan, before, goal) : BINS;
+  const int border = s.run ? border_bin<PART>(a.hist + (int64_t)b * BINS, s.p, s_scan, before, goal) : BINS;
   if (threadIdx.x == 0) s_n = 0;
   __syncthreads();
-  sweep.run([&](int v, const float (&y)[R::E]) __attribute__((always_inline)) {
-    float z[R::E];
-    uint64_t sum = 0, w[R::E];
-    sc.at(y, z);
-    if (s.run) {
-      bool listed = false, any = false;
-      int at[R::E];
-#pragma unroll
-      for (int e = 0; e < R::E; ++e) {
-        at[e] = sc.bin(z[e]);
-        listed |= at[e] == border;
-        any |= at[e] < border;
-      }
-      if (__any(any)) {
-        sc.weights(z, w);
-#pragma unroll
-        for (int e = 0; e < R::E; ++e) sum += at[e] < border && y[e] >= sc.bar ? w[e] : 0;
-      }
-      if (listed) {
-#pragma unroll
-        for (int e = 0; e < R::E; ++e)
-          if (at[e] == border) {
-            const uint32_t n = atomicAdd(&s_n, 1u);
-            if (n < LIST) s_list[n] = ord.place(key_of(y[e]), row.index(v, e));
-          }
-      }
-    } else {
-      bool any = false;
-#pragma unroll
-      for (int e = 0; e < R::E; ++e) any |= y[e] >= sc.bar;
-      if (__any(any)) {
-        sc.weights(z, w);
-#pragma unroll
-        for (int e = 0; e < R::E; ++e) sum += y[e] >= sc.bar ? w[e] : 0;
-      }
-    }
-    sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
-    if (lane == 0) a.tile[(int64_t)b * a.parts * a.tiles + v / 64] = sum;
-  });
+  uint64_t* sums = a.tile + (int64_t)b * a.parts * a.tiles;
+  sums_into(sweep, ord, sc, border, s_list, &s_n, [&](int tile, uint64_t w) __attribute__((always_inline)) { sums[tile] = w; });
   __syncthreads();
   if (s.run) append(a, b, s_list, s_n, &s_at);
 }
 
-// ---------------------------------------------------------------------------
-// Of the n values, those in [lo, hi] (lo >= 1): the largest at which the measure,
-// summed from the largest value down, reaches `goal`; 0 if none does. Nine bits of
-// the range at a time, by histograms, until one value is left.
-constexpr int REACH = 3 * FIN + 64;          // words of s
-template <typename V, typename M>
-__device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_t lo, uint64_t hi, uint64_t goal, uint64_t* s) {
+// Values with a measure: narrows [lo, hi] (lo >= 1) towards the largest value at which
+// the measure, summed from the largest value down, reaches `goal` (then the rest of
+// it), until no more than `few` values are left or one place. -> how many are left, 0
+// if none reaches it. Nine or ten bits of the range at a time, by histograms of N bins.
+// each(f) calls f(value, measure) for the thread's values. s: reach_words(N).
+constexpr int reach_words(int N) { return 3 * N + 64; }
+template <int N, typename F>
+__device__ __forceinline__ uint32_t narrow(F&& each, uint64_t& lo, uint64_t& hi, uint64_t& goal, uint32_t few, uint64_t* s) {
+  constexpr int LOG = N == 1024 ? 10 : 9;
+  static_assert(N == 1 << LOG, "a bin a thread");
   const int tid = threadIdx.x, wave = tid / 64;
-  uint64_t* s_scan = s + 3 * FIN;
+  uint64_t* s_scan = s + 3 * N;
   __syncthreads();
   s[tid] = 0;
-  ((uint32_t*)(s + 2 * FIN))[tid] = 0;
+  ((uint32_t*)(s + 2 * N))[tid] = 0;
   if (tid < 2) s_scan[32 + 4 * tid] = 0;
   __syncthreads();
   for (int pass = 0; ; ++pass) {
     // the two passes' places take turns: what one leaves is cleared by the next
-    uint64_t *bin = s + pass % 2 * FIN, *sums = s_scan + pass % 2 * 16, *found = s_scan + 32 + pass % 2 * 4;
-    uint32_t* cnt = (uint32_t*)(s + 2 * FIN) + pass % 2 * FIN;
-    const int bits = 64 - __clzll((long long)((hi - lo) | 1)), shift = bits > 9 ? bits - 9 : 0;
-    for (int i = tid; i < n; i += FIN) {
-      const uint64_t x = value(i);
+    uint64_t *bin = s + pass % 2 * N, *sums = s_scan + pass % 2 * 16, *found = s_scan + 32 + pass % 2 * 4;
+    uint32_t* cnt = (uint32_t*)(s + 2 * N) + pass % 2 * N;
+    const int bits = 64 - __clzll((long long)((hi - lo) | 1)), shift = bits > LOG ? bits - LOG : 0;
+    each([&](uint64_t x, uint64_t measure) __attribute__((always_inline)) {
       if (x >= lo && x <= hi) {
         const int at = (int)((x - lo) >> shift);
-        atomicAdd((ull*)&bin[at], (ull)measure(i));
+        atomicAdd((ull*)&bin[at], (ull)measure);
         atomicAdd(&cnt[at], 1u);
       }
-    }
+    });
     __syncthreads();
-    const uint64_t mine = bin[FIN - 1 - tid], upto = scan64(mine);
-    const uint32_t many = cnt[FIN - 1 - tid];
+    const uint64_t mine = bin[N - 1 - tid], upto = scan64(mine);
+    const uint32_t many = cnt[N - 1 - tid];
     if (tid % 64 == 63) sums[wave] = upto;
-    s[(pass + 1) % 2 * FIN + tid] = 0;
-    ((uint32_t*)(s + 2 * FIN))[(pass + 1) % 2 * FIN + tid] = 0;
+    s[(pass + 1) % 2 * N + tid] = 0;
+    ((uint32_t*)(s + 2 * N))[(pass + 1) % 2 * N + tid] = 0;
     __syncthreads();
     uint64_t before = upto - mine;
 #pragma unroll
-    for (int w = 0; w < FIN / 64; ++w) before += w < wave ? sums[w] : 0;
+    for (int w = 0; w < N / 64; ++w) before += w < wave ? sums[w] : 0;
     if (before < goal && before + mine >= goal) {
-      found[0] = FIN - tid;                 // the bin and 1
+      found[0] = N - tid;                   // the bin and 1
       found[1] = before;
       found[2] = many;
     }
@@ -655,41 +713,70 @@ __device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_
     if (found[0] == 0) return 0;
     goal -= found[1];
     lo += (found[0] - 1) << shift;
-    if (shift == 0) return lo;
     if ((hi - lo) >> shift) hi = lo + ((uint64_t)1 << shift) - 1;
-    if (found[2] == 1) {
-      for (int i = tid; i < n; i += FIN) {
-        const uint64_t x = value(i);
-        if (x >= lo && x <= hi) s_scan[40] = x;
-      }
-      __syncthreads();
-      return s_scan[40];
-    }
+    if (shift == 0 || found[2] <= few) return (uint32_t)found[2];
   }
 }
 
-template <typename T, bool SPLIT>
-__global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
+// The largest of n values from [lo, hi] at which the measure, summed from the largest
+// down, reaches `goal`; 0 if none does.
+template <int N, typename V, typename M>
+__device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_t lo, uint64_t hi, uint64_t goal, uint64_t* s) {
+  const uint32_t left = narrow<N>([&](auto&& f) __attribute__((always_inline)) {
+    for (int i = threadIdx.x; i < n; i += N) f(value(i), measure(i));
+  }, lo, hi, goal, 1, s);
+  if (left == 0 || lo == hi) return left ? lo : 0;
+  uint64_t* only = s + 3 * N + 40;
+  for (int i = threadIdx.x; i < n; i += N) {
+    const uint64_t x = value(i);
+    if (x >= lo && x <= hi) *only = x;
+  }
+  __syncthreads();
+  return *only;
+}
+
+// ---------------------------------------------------------------------------
+// A workgroup a row: the end of what the parts have begun, a short row, or all of a
+// long one.
+enum { SHORT, PARTS, WHOLE };
+__host__ __device__ constexpr int threads_of(int mode) { return mode == WHOLE ? 1024 : 512; }
+
+template <typename T, int MODE>
+__global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleArgs a) {
   using R = Row<T>;
-  __shared__ uint64_t s_list[LIST], s_w[LIST], s_slot[SPLIT ? SLOTS : 1], s_scan[REACH], s_found[3];
+  constexpr int N = threads_of(MODE);
+  __shared__ uint64_t s_list[LIST], s_w[LIST], s_slot[MODE == SHORT ? 1 : SLOTS], s_scan[reach_words(N)], s_found[2];
+  __shared__ uint64_t s_hist[MODE == WHOLE ? BINS : 1];
+  __shared__ __align__(16) uint32_t s_max[MODE == WHOLE ? N : 4], s_n;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
   const Setting s = setting_of(a, b);
   const R row(a, b);
   const Order<T> ord(a.V);
-  const uint32_t n_cand = SPLIT ? a.count[b] : 0;
+  const int tiles = (row.n_vec + 63) / 64, per = (tiles + SLOTS - 1) / SLOTS;   // tiles of a slot
+  uint32_t n_cand = MODE == PARTS ? a.count[b] : 0;
   uint64_t first;
-  uint32_t least = ~0u;
-  if constexpr (SPLIT) {
+  uint32_t least = KEY_NONE + 1;
+  if constexpr (MODE == PARTS) {
     row_ends(a, b, first, least);
+  } else if constexpr (MODE == WHOLE) {
+    Sweep<T, N / 64, 4> sweep(row, 0, tiles);
+    float most, low;
+    int at;
+    uint32_t turned;
+    ends_of(sweep, a.runs, most, at, low);
+    s_max[tid] = key_of(most);
+    ends_of(row, ord, most, at, low, first, turned);
+    first = block_all<N>(first, s_scan, Most());
+    least = ~(uint32_t)block_all<N>(turned, s_scan, Most());
   } else {
     first = 0;
-    for (int v = tid; v < row.n_vec; v += FIN)
+    for (int v = tid; v < row.n_vec; v += N)
       row.each(v, [&](float y, int i) __attribute__((always_inline)) {
         const uint64_t place = ord.place(key_of(y), i);
         if (i >= 0 && i < a.V) s_list[i] = place;
         first = place > first ? place : first;
       });
-    first = block_all<FIN>(first, s_scan, Most());
+    first = block_all<N>(first, s_scan, Most());
   }
   auto done = [&](int token, float logp) __attribute__((always_inline)) {
     a.token[b] = token;
@@ -699,7 +786,39 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
     if (tid == 0) first == 0 ? done(0, __builtin_nanf("")) : done(ord.index(first), 0.f);
     return;
   }
-  const Scale sc(a, s, ord.logit(first), SPLIT ? least : KEY_NONE + 1);
+  const Scale sc(a, s, ord.logit(first), least);
+  int border = BINS;                        // the bin of the last place kept: those before it are kept whole
+  uint64_t before = 0, goal = 0;
+  if constexpr (MODE == WHOLE) {
+    if (tid == 0) s_n = 0;
+    for (int i = tid; i < SLOTS; i += N) s_slot[i] = 0;
+    for (int i = tid; i < BINS; i += N) s_hist[i] = 0;
+    __syncthreads();
+    if (s.list) {
+      Sweep<T, N / 64, 4> sweep(row, 0, tiles);
+      uint32_t key[N / 64];
+#pragma unroll
+      for (int i = 0; i < N / 256; ++i) {
+        const u32x4 w = *(const u32x4*)&s_max[(i * 64 + lane) * 4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) key[4 * i + e] = w[e];
+      }
+      gather_into(sweep, ord, list_bar(key, s.k), s_list, &s_n);
+    } else if (s.sums()) {
+      if (s.run) {
+        Sweep<T, N / 64, 2> sweep(row, 0, tiles);
+        hist_into(sweep, sc, s_hist);
+        __syncthreads();
+        border = border_bin<N>(s_hist, s.p, s_scan, before, goal);
+      }
+      Sweep<T, N / 64, 2> sweep(row, 0, tiles);
+      sums_into(sweep, ord, sc, border, s_list, &s_n, [&](int tile, uint64_t w) __attribute__((always_inline)) {
+        if (w) atomicAdd((ull*)&s_slot[tile / per], (ull)w);
+      });
+    }
+    __syncthreads();
+    n_cand = s_n;
+  }
   auto weight = [&](uint64_t place) __attribute__((always_inline)) { return sc.weight(sc.at(ord.logit(place))); };
   auto drawn = [&](float y, int i, uint64_t total) __attribute__((always_inline)) {
     const double d = ((double)sc.at(y) - sc.top) / (double)s.t;
@@ -711,108 +830,106 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
   };
 
   // a list that holds all that is kept?
-  const bool whole = SPLIT ? s.list && n_cand <= LIST : true;
+  const bool whole = MODE == SHORT || (s.list && n_cand <= LIST);
   if (whole) {
-    const int n = SPLIT ? (int)n_cand : a.V;
+    const int n = MODE == SHORT ? a.V : (int)n_cand;
     uint64_t most_off = 0;
-    for (int i = tid; i < n; i += FIN) {
-      const uint64_t place = SPLIT ? a.list[(int64_t)b * LIST + i] : s_list[i];
-      if constexpr (SPLIT) s_list[i] = place;
+    for (int i = tid; i < n; i += N) {
+      const uint64_t place = MODE == PARTS ? a.list[(int64_t)b * LIST + i] : s_list[i];
+      if constexpr (MODE == PARTS) s_list[i] = place;
       s_w[i] = place ? weight(place) : 0;
       most_off = ~place > most_off && place ? ~place : most_off;
     }
-    const uint64_t least_place = ~block_all<FIN>(most_off, s_scan, Most());
+    const uint64_t least_place = ~block_all<N>(most_off, s_scan, Most());
     auto place = [&](int i) __attribute__((always_inline)) { return s_list[i]; };
     auto total_of = [&](auto&& kept) __attribute__((always_inline)) {
       uint64_t sum = 0;
-      for (int i = tid; i < n; i += FIN) sum += kept(i) ? s_w[i] : 0;
-      return block_all<FIN>(sum, s_scan, Plus());
+      for (int i = tid; i < n; i += N) sum += kept(i) ? s_w[i] : 0;
+      return block_all<N>(sum, s_scan, Plus());
     };
     uint64_t last = 1;                      // the last place kept
     if (s.cut) {
-      const uint64_t at = reach(n, place, [](int) { return (uint64_t)1; }, least_place, first, s.k, s_scan);
+      const uint64_t at = reach<N>(n, place, [](int) { return (uint64_t)1; }, least_place, first, s.k, s_scan);
       if (at) last = at;                    // (0: there are fewer)
     }
     if (s.run) {
       const uint64_t goal = part_of(s.p, total_of([&](int i) { return s_list[i] >= last; }), true);
-      last = goal <= 1 ? first : reach(n, place, [&](int i) { return s_w[i]; }, last > 1 ? last : least_place, first, goal, s_scan);
+      last = goal <= 1 ? first : reach<N>(n, place, [&](int i) { return s_w[i]; }, last > 1 ? last : least_place, first, goal, s_scan);
     }
     auto kept = [&](int i) __attribute__((always_inline)) { return s_list[i] >= last && ord.logit(s_list[i]) >= sc.bar; };
     const uint64_t total = total_of(kept), aim = aim_of(total);
     // by index: the first one is the largest number
     auto turned = [&](int i) __attribute__((always_inline)) { return kept(i) ? (uint64_t)ord.turned(ord.index(s_list[i])) + 1 : 0; };
-    const uint64_t at = reach(n, turned, [&](int i) { return s_w[i]; }, 1, (uint64_t)ord.turned(0) + 1, aim + 1, s_scan);
-    for (int i = tid; i < n; i += FIN)
+    const uint64_t at = reach<N>(n, turned, [&](int i) { return s_w[i]; }, 1, (uint64_t)ord.turned(0) + 1, aim + 1, s_scan);
+    for (int i = tid; i < n; i += N)
       if (turned(i) == at) drawn(ord.logit(s_list[i]), ord.index(s_list[i]), total);
     return;
   }
-  if constexpr (SPLIT) {
+  if constexpr (MODE != SHORT) {
 
   uint64_t last = 1;                        // the last place kept
-  int border = BINS;                        // its bin: those before it are kept whole
-  const int tiles = (row.n_vec + 63) / 64, per = (tiles + SLOTS - 1) / SLOTS;   // tiles of a slot
-  const bool ready = s.sums() && (!s.run || n_cand <= LIST);   // by the launches before
-  for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
-  __syncthreads();
+  const bool ready = s.sums() && (!s.run || n_cand <= LIST);   // by the passes before
+  if (MODE == PARTS || !ready) {
+    for (int i = tid; i < SLOTS; i += N) s_slot[i] = 0;
+    __syncthreads();
+  }
   if (ready) {
-    const uint64_t* sums = a.tile + (int64_t)b * a.parts * a.tiles;
     if (s.run) {
-      uint64_t before, goal;
-      border = border_bin<FIN>(a, b, s.p, s_scan, before, goal);
+      if constexpr (MODE == PARTS) border = border_bin<N>(a.hist + (int64_t)b * BINS, s.p, s_scan, before, goal);
       const int n = (int)n_cand;
       uint64_t least_off = 0, most = 0;
-      for (int i = tid; i < n; i += FIN) {
-        const uint64_t place = a.list[(int64_t)b * LIST + i];
-        s_list[i] = place;
+      for (int i = tid; i < n; i += N) {
+        const uint64_t place = MODE == PARTS ? a.list[(int64_t)b * LIST + i] : s_list[i];
+        if constexpr (MODE == PARTS) s_list[i] = place;
         s_w[i] = weight(place);
         least_off = ~place > least_off ? ~place : least_off;
         most = place > most ? place : most;
       }
-      least_off = block_all<FIN>(least_off, s_scan, Most());
-      most = block_all<FIN>(most, s_scan, Most());
-      last = reach(n, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, ~least_off, most, goal - before, s_scan);
-      for (int i = tid; i < n; i += FIN)
+      least_off = block_all<N>(least_off, s_scan, Most());
+      most = block_all<N>(most, s_scan, Most());
+      last = reach<N>(n, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, ~least_off, most, goal - before, s_scan);
+      for (int i = tid; i < n; i += N)
         if (s_list[i] >= last && ord.logit(s_list[i]) >= sc.bar)
           atomicAdd((ull*)&s_slot[(ord.index(s_list[i]) + row.shift) / R::E / 64 / per], (ull)s_w[i]);
     }
-    for (int i = tid; i < tiles; i += FIN) {
-      const uint64_t w = sums[i];
-      if (w) atomicAdd((ull*)&s_slot[i / per], (ull)w);
+    if constexpr (MODE == PARTS) {
+      const uint64_t* sums = a.tile + (int64_t)b * a.parts * a.tiles;
+      for (int i = tid; i < tiles; i += N) {
+        const uint64_t w = sums[i];
+        if (w) atomicAdd((ull*)&s_slot[i / per], (ull)w);
+      }
     }
     __syncthreads();
   } else {
     // What the lists do not hold (a top_k past k_list, more than LIST tokens at a
-    // border): the border place eleven bits at a time, over the whole row.
+    // border): the border place by passes over the whole row, until a list holds what
+    // is left.
     auto over = [&](auto&& f) {
-      for (int v = tid; v < row.n_vec; v += FIN) row.each(v, f);
+      for (int v = tid; v < row.n_vec; v += N) row.each(v, f);
     };
-    auto far = [&](auto&& measure, uint64_t goal) {
-      uint64_t prefix = 0, before = 0;
-      for (int low = 44; low >= 0; low -= 11) {   // (56 bits at most)
-        for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
-        __syncthreads();
+    auto far = [&](auto&& measure, uint64_t goal) {   // 0: nothing reaches it
+      uint64_t lo = last, hi = first;
+      const uint32_t left = narrow<N>([&](auto&& f) {
         over([&](float y, int i) __attribute__((always_inline)) {
           const uint64_t place = ord.place(key_of(y), i);
-          if (place < last || (low < 44 && place >> (low + 11) != prefix)) return;
-          const uint64_t w = measure(y);
-          if (w) atomicAdd((ull*)&s_slot[place >> low & (SLOTS - 1)], (ull)w);
+          if (place >= lo && place <= hi) f(place, measure(y));
         });
-        __syncthreads();
-        if (tid == 0) {
-          uint64_t sum = before;
-          int i = SLOTS - 1;
-          for (; i > 0 && sum + s_slot[i] < goal; --i) sum += s_slot[i];
-          s_found[0] = prefix << 11 | i;
-          s_found[1] = sum;
-          s_found[2] = sum + s_slot[i];
+      }, lo, hi, goal, LIST, s_scan);
+      if (left == 0 || lo == hi) return left ? lo : 0;
+      if (tid == 0) s_n = 0;
+      __syncthreads();
+      over([&](float y, int i) __attribute__((always_inline)) {
+        const uint64_t place = ord.place(key_of(y), i);
+        if (place >= lo && place <= hi) {
+          const uint32_t at = atomicAdd(&s_n, 1u);
+          if (at < LIST) {
+            s_list[at] = place;
+            s_w[at] = measure(y);
+          }
         }
-        __syncthreads();
-        prefix = s_found[0];
-        before = s_found[1];
-        if (s_found[2] < goal) return (uint64_t)0;   // (fewer than that)
-        __syncthreads();
-      }
-      return prefix;
+      });
+      __syncthreads();
+      return reach<N>((int)left, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, lo, hi, goal, s_scan);
     };
     auto mass = [&](float y) __attribute__((always_inline)) { return sc.weight(sc.at(y)); };
     if (s.cut) {
@@ -824,14 +941,14 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
       over([&](float y, int i) __attribute__((always_inline)) {
         if (ord.place(key_of(y), i) >= last) sum += mass(y);
       });
-      sum = block_all<FIN>(sum, s_scan, Plus());
+      sum = block_all<N>(sum, s_scan, Plus());
       const uint64_t goal = part_of(s.p, sum, true);
       last = goal <= 1 ? first : far(mass, goal);
     }
     border = -1;                            // (by place alone)
-    for (int i = tid; i < SLOTS; i += FIN) s_slot[i] = 0;
+    for (int i = tid; i < SLOTS; i += N) s_slot[i] = 0;
     __syncthreads();
-    for (int v = tid; v < tiles * 64; v += FIN) {
+    for (int v = tid; v < tiles * 64; v += N) {
       uint64_t sum = 0;
       if (v < row.n_vec)
         row.each(v, [&](float y, int i) __attribute__((always_inline)) {
@@ -844,11 +961,11 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
   }
 
   // the slot at which the sum passes the aim, then the tile and the token
-  constexpr int PER = SLOTS / FIN;
+  constexpr int PER = SLOTS / N;
   uint64_t mine = 0, total;
 #pragma unroll
   for (int e = 0; e < PER; ++e) mine += s_slot[tid * PER + e];
-  uint64_t before = block_before<FIN>(mine, s_scan, total);
+  before = block_before<N>(mine, s_scan, total);
   const uint64_t aim = aim_of(total);
   if (before <= aim && before + mine > aim) {
     int e = 0;
@@ -894,13 +1011,20 @@ __global__ __launch_bounds__(FIN) void sample_finish_kernel(SampleArgs a) {
 // host side
 
 struct Plan {
-  int parts, tiles, groups, lanes;          // parts 0: one launch
+  int parts, tiles, groups, lanes;          // parts 0: a workgroup a row, one launch
   size_t part, maxima, count, hist, list, tile, bytes;   // offsets
 };
 
+// A workgroup takes a whole row where there are rows for most CUs, or short ones. 128256
+// bfloat16 tokens, by workgroups / parts: 128 rows 46 / 37 us (temperature alone), 29 /
+// 29 (top_k 50), 96 / 74 (a flat nucleus); 256 rows 55 / 62, 37 / 43, 101 / 113. 16000
+// tokens: 64 rows 16 / 16, 25 / 23, 29 / 29; 256 rows 17 / 20, 24 / 26, 30 / 37. 5000
+// tokens, one row: 12.1 / 13.3, 19.0 / 18.7, 21.5 / 23.0.
+bool by_rows(int B, int V) { return B >= 160 || V <= 8192; }
+
 void plan_for(Plan& p, int B, int V, int dtype) {
   p = Plan{};
-  if (V <= LIST) return;
+  if (by_rows(B, V)) return;
   const int E = dtype == DA_FP32 ? 4 : 8;
   const int64_t tiles = ((int64_t)V + 2 * E - 1) / E / 64 + 1;   // whatever the row's alignment
   // parts: some workgroups for each CU together, 4 tiles (one of each wave) at least
@@ -929,20 +1053,24 @@ void plan_for(Plan& p, int B, int V, int dtype) {
 
 template <typename T>
 void launch(SampleArgs& a, hipStream_t st) {
-  if (a.parts == 0) {
-    hipLaunchKernelGGL((sample_finish_kernel<T, false>), dim3(a.B), dim3(FIN), 0, st, a);
+  if (a.V <= LIST) {
+    hipLaunchKernelGGL((sample_finish_kernel<T, SHORT>), dim3(a.B), dim3(threads_of(SHORT)), 0, st, a);
     return;
   }
-  const dim3 grid(a.parts * a.B);
   // (what no row can ask for is not launched)
   const bool t_on = a.t_dev || a.t > 0.f, k_on = a.k_dev || (a.k > 0 && a.k < a.V);
   const bool k_all = !a.k_dev && a.k > 0 && a.k < a.V, k_list = a.k_dev || (k_on && a.k <= a.k_list);
   const bool p_on = a.p_dev || a.p < 1.f;
   a.runs = t_on && p_on && !k_all;
+  if (a.parts == 0) {
+    hipLaunchKernelGGL((sample_finish_kernel<T, WHOLE>), dim3(a.B), dim3(threads_of(WHOLE)), 0, st, a);
+    return;
+  }
+  const dim3 grid(a.parts * a.B);
   hipLaunchKernelGGL((sample_top_kernel<T>), grid, dim3(PART), 0, st, a);
   if (t_on && (k_list || (p_on && !k_all))) hipLaunchKernelGGL((sample_gather_kernel<T>), grid, dim3(PART), 0, st, a);
   if (t_on && !k_all) hipLaunchKernelGGL((sample_sums_kernel<T>), grid, dim3(PART), 0, st, a);
-  hipLaunchKernelGGL((sample_finish_kernel<T, true>), dim3(a.B), dim3(FIN), 0, st, a);
+  hipLaunchKernelGGL((sample_finish_kernel<T, PARTS>), dim3(a.B), dim3(threads_of(PARTS)), 0, st, a);
 }
 
 }  // namespace
@@ -988,7 +1116,7 @@ extern "C" int da_sample(const da_sample_args* x, void* stream) {
   a.parts = p.parts, a.tiles = p.tiles;
   a.f_parts = make_fastdiv(p.parts > 0 ? p.parts : 1);
   a.groups = p.groups, a.lanes = p.lanes;
-  a.k_list = p.parts * p.groups / 4 * 3;
+  a.k_list = (p.parts > 0 ? p.parts * p.groups : threads_of(WHOLE)) / 4 * 3;
   char* ws = (char*)x->workspace;
   a.part = (Part*)(ws + p.part);
   a.maxima = (uint32_t*)(ws + p.maxima);

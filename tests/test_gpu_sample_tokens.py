@@ -85,6 +85,9 @@ def test_rows_of_every_length(gpu, V, dtype):
     (1, 131073, "fp32", dict()), (3, 151936, "bf16", dict(top_k=5000, top_p=0.95)),
     (300, 1000, "bf16", dict(temperature=0.8, top_k=40, min_p=0.02)), (1, 1 << 20, "fp16", dict(top_p=0.9)),
     (40, 32000, "fp32", dict(temperature=1.2, top_p=0.9, min_p=0.001)),
+    (160, 20011, "bf16", dict(top_k=50, top_p=0.9)), (161, 9999, "fp32", dict(temperature=1.4, top_p=0.97)),
+    (200, 12345, "fp16", dict(temperature=0.6)), (170, 30000, "bf16", dict(min_p=0.03)),
+    (165, 9000, "fp16", dict(top_k=4000, top_p=0.9)), (159, 9000, "fp16", dict(top_k=4000, top_p=0.9)),
 ])
 def test_long_rows_and_wide_batches(gpu, B, V, dtype, s):
     x, u = logits(B, V, dtype, V + B), uniform(B, V)
@@ -175,12 +178,13 @@ def test_equal_logits_are_taken_by_index(gpu):
     check(x[:64], uniform(64, 8), sure=False, top_k=13)
 
 
+@pytest.mark.parametrize("n", [512, 64])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
-def test_long_rows_of_few_values(gpu, dtype):
+def test_long_rows_of_few_values(gpu, dtype, n):
     """More equal logits than a list holds, at the border of top_k, of top_p, of
     both; by index, exactly."""
     from delta_attention import ops
-    V, n = 65536, 512
+    V = 65536
     x = torch.zeros(1, V, device="cuda", dtype=DT[dtype]).expand(n, V)
     u = (torch.arange(n, device="cuda").float() + 0.5) / n
     at = (torch.arange(n, device="cuda").double() + 0.5) / n
@@ -200,8 +204,8 @@ def test_long_rows_of_few_values(gpu, dtype):
 def test_rows_around_the_list(gpu):
     """Row lengths at which the launches change, and masks that leave fewer
     candidates than top_k or than groups."""
-    for V in (3583, 3584, 3585, 4095, 4097, 5000, 9001):
-        x, u = logits(6, V, "bf16", V), uniform(6, V + 2)
+    for V, B in ((3583, 6), (3584, 6), (3585, 6), (4097, 6), (8192, 6), (8193, 6), (9001, 160), (20000, 6)):
+        x, u = logits(B, V, "bf16", V), uniform(B, V + 2)
         x[1, 100:] = -math.inf
         x[2, :] = -math.inf
         x[2, V - 1] = 3.0
@@ -243,12 +247,12 @@ def test_strides_and_offsets(gpu):
 
 def test_a_row_does_not_depend_on_its_batch(gpu):
     from delta_attention import ops
-    x, u = logits(70, 32000, "bf16", 13), uniform(70, 14)
+    x, u = logits(170, 32000, "bf16", 13), uniform(170, 14)
     for s in (dict(), dict(top_p=0.95), dict(top_k=100, top_p=0.9), dict(top_k=6000), dict(min_p=0.01)):
         t, lp = ops.sample_tokens(x, u, **s)
         again = ops.sample_tokens(x, u, **s)
         assert torch.equal(t, again[0]) and torch.equal(lp, again[1])
-        for b in (0, 33, 69):
+        for b in (0, 33, 169):
             one = ops.sample_tokens(x[b:b + 1], u[b:b + 1], **s)
             assert one[0].item() == t[b].item() and one[1].item() == lp[b].item()
 

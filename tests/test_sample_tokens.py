@@ -97,6 +97,7 @@ def test_c_refusals(lib):
     assert lib.da_sample(None, None) == L.DA_ERR_INVALID_ARG
     ws = lib.da_sample_workspace_bytes
     assert ws(0, 10, L.DA_BF16) == ws(1, 0, L.DA_BF16) == ws(1, 10, 5) == ws(1, 1 << 25, L.DA_BF16) == 0
+    assert ws(1, 8192, L.DA_BF16) == ws(160, 100000, L.DA_FP32) == 0       # a workgroup a row
     need = ws(2, 100000, L.DA_BF16)
     if need:
         assert call(V=100000, rs=100000, ws=16, nb=need - 1) == call(V=100000, rs=100000, nb=need) == L.DA_ERR_WORKSPACE
