@@ -754,6 +754,14 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
   const Order<T> ord(a.V);
   const int tiles = (row.n_vec + 63) / 64, per = (tiles + SLOTS - 1) / SLOTS;   // tiles of a slot
   uint32_t n_cand = MODE == PARTS ? a.count[b] : 0;
+  const float u = a.u[b];
+  // (loads that may turn out to be of nothing, made before it is known)
+  const uint64_t *sums = a.tile + (int64_t)b * a.parts * a.tiles, *listed = a.list + (int64_t)b * LIST;
+  uint64_t early_sum = 0, early_place = 0;
+  if constexpr (MODE == PARTS) {
+    early_sum = sums[min(tid, a.parts * a.tiles - 1)];
+    early_place = listed[tid];
+  }
   uint64_t first;
   uint32_t least = KEY_NONE + 1;
   if constexpr (MODE == PARTS) {
@@ -825,7 +833,7 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
     done(i, (float)(d - log(ldexp((double)total, -a.bits))));
   };
   auto aim_of = [&](uint64_t total) __attribute__((always_inline)) {
-    const uint64_t aim = part_of(a.u[b], total, false);
+    const uint64_t aim = part_of(u, total, false);
     return aim < total ? aim : total - 1;
   };
 
@@ -835,7 +843,7 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
     const int n = MODE == SHORT ? a.V : (int)n_cand;
     uint64_t most_off = 0;
     for (int i = tid; i < n; i += N) {
-      const uint64_t place = MODE == PARTS ? a.list[(int64_t)b * LIST + i] : s_list[i];
+      const uint64_t place = MODE != PARTS ? s_list[i] : i == tid ? early_place : listed[i];
       if constexpr (MODE == PARTS) s_list[i] = place;
       s_w[i] = place ? weight(place) : 0;
       most_off = ~place > most_off && place ? ~place : most_off;
@@ -879,7 +887,7 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
       const int n = (int)n_cand;
       uint64_t least_off = 0, most = 0;
       for (int i = tid; i < n; i += N) {
-        const uint64_t place = MODE == PARTS ? a.list[(int64_t)b * LIST + i] : s_list[i];
+        const uint64_t place = MODE != PARTS ? s_list[i] : i == tid ? early_place : listed[i];
         if constexpr (MODE == PARTS) s_list[i] = place;
         s_w[i] = weight(place);
         least_off = ~place > least_off ? ~place : least_off;
@@ -893,9 +901,8 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
           atomicAdd((ull*)&s_slot[(ord.index(s_list[i]) + row.shift) / R::E / 64 / per], (ull)s_w[i]);
     }
     if constexpr (MODE == PARTS) {
-      const uint64_t* sums = a.tile + (int64_t)b * a.parts * a.tiles;
       for (int i = tid; i < tiles; i += N) {
-        const uint64_t w = sums[i];
+        const uint64_t w = i == tid ? early_sum : sums[i];
         if (w) atomicAdd((ull*)&s_slot[i / per], (ull)w);
       }
     }
