@@ -49,11 +49,11 @@ typedef unsigned long long ull;
 constexpr int MAX_V = 1 << 24;               // tokens of a vocabulary
 constexpr int MAX_B = 0x3fffff;              // rows (four parts each: threads of a grid below 2^32)
 constexpr uint32_t KEY_NONE = 0x007fffffu;   // -inf's key: candidates lie above it
-constexpr int PART = 256;                    // threads of a part
+constexpr int PART = 512;                    // threads of a part
 constexpr int LIST = 3584;                   // tokens of a row's list (two finishing workgroups' LDS a CU)
 constexpr int BINS = 768;                    // of a part's histogram
 constexpr int GROUPS = 2048;                 // group maxima of a row at most
-constexpr int SLOTS = 2048;                  // tile sums in LDS; bins of a radix pass
+constexpr int SLOTS = 1024;                  // tile sums in LDS
 
 struct Part {
   uint64_t first;                            // the first place in the order, 0: no candidate
@@ -74,12 +74,13 @@ struct SampleArgs {
   int B, V, bits;                           // weights in units of 2^-bits
   int parts, tiles, k_list;                 // parts of a row, tiles of a part, the largest top_k with a list
   FastDiv f_parts;
-  int runs;                                 // whether rows may take a histogram
+  int runs, sums;                           // whether rows may take a histogram, and whether the sums are launched
   int groups, lanes;                        // group maxima of a part, lanes of a group
   // workspace, by row
   Part* part;                               // [parts]
   uint32_t* maxima;                         // [parts * groups]
   uint32_t* count;                          // tokens gathered (also past the list's end)
+  uint32_t* ended;                          // parts that are through
   uint64_t* hist;                           // [BINS]
   uint64_t* list;                           // [LIST] places
   uint64_t* tile;                           // [parts * tiles] kept weight
@@ -111,17 +112,19 @@ struct Order {
   }
 };
 
-// 2^t for t <= 0 in units of 2^-bits (bits <= 45): the fraction's power by
-// the polynomial of degree 10 that meets 2^f at the Chebyshev nodes of [-1/2, 1/2]
-// (2^-51 of it, rounding included; the series takes two terms more), the whole one
-// by the exponent. Whole numbers come from what 2^52 leaves of a sum: of t, and of
-// the weight, which is rounded so.
-__device__ __forceinline__ uint64_t weight_of(double t, int bits) {
-  t = fmax(t, -200.0);                      // (2^-200 of the largest: none; so is what is no candidate)
-  const double whole = t + 6755399441055744.0, f = t - (whole - 6755399441055744.0);   // (1.5 * 2^52)
+// Weights in units of 2^-bits (bits <= 45) of one that is 1: 2^(d * per) for d <= 0, the
+// fraction's power by the polynomial of degree 10 that meets 2^f at the Chebyshev nodes
+// of [-1/2, 1/2] (2^-51 of it, rounding included; the series takes two terms more), the
+// whole one by the exponent. Whole numbers come from what 2^52 leaves of a sum: of the
+// exponent, with the unit's `bits` above it, and of the weight, which is rounded so.
+// (RAW is that 2^52 of the weight, for the sums to take off together.)
+constexpr double WHOLE_OF = 6755399441055744.0;   // 1.5 * 2^52
+constexpr uint64_t RAW = 0x4330000000000000ull;
+__device__ __forceinline__ uint64_t raw_weight(double d, double per, double whole_of) {
+  const double whole = fma(d, per, whole_of), f = fma(d, per, whole_of - whole);
   double p = 7.072585949269223e-09;
   constexpr double c[] = {1.0208690299958306e-07, 1.321544258792169e-06, 1.5252657260200837e-05, 0.0001540353044173605,
-                          0.0013333558230164974, 0.009618129107606888, 0.05550410866444772, 0.24022650695910097,
+                          0.0013333558230164974, 0.009618129107606888, 0.05550410866447172, 0.24022650695910097,
                           0.69314718055995, 1.0};
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
@@ -130,9 +133,10 @@ __device__ __forceinline__ uint64_t weight_of(double t, int bits) {
     p = fma(p, f, k);
   }
   const uint64_t w = (uint64_t)__double_as_longlong(p);
-  const uint32_t hi = (uint32_t)(w >> 32) + (((uint32_t)__double_as_longlong(whole) + bits) << 20);
+  uint32_t hi = (uint32_t)(w >> 32) + ((uint32_t)__double_as_longlong(whole) << 20);
+  asm("" : "+v"(hi));                       // (32 bits of it: else the sum takes 64)
   const double scaled = __longlong_as_double((long long)((uint64_t)hi << 32 | (uint32_t)w));
-  return (uint64_t)__double_as_longlong(scaled + 4503599627370496.0) - 0x4330000000000000ull;
+  return (uint64_t)__double_as_longlong(scaled + 4503599627370496.0);
 }
 
 // What a row asks for.
@@ -140,7 +144,6 @@ struct Setting {
   float t, p, m;
   int k;
   bool greedy, cut, list, run;              // cut: top_k takes some away; list: by a list; run: top_p takes some away
-  __device__ __forceinline__ bool sums() const { return !greedy && !cut; }   // rows of the sums launch
 };
 __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int b) {
   Setting s;
@@ -150,7 +153,7 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int b) {
   s.m = a.m_dev ? a.m_dev[b * a.m_step] : a.m;
   s.greedy = !(s.t > 0.f) || s.m > 1.f;     // (a min_p above 1 leaves the first token alone)
   s.cut = s.k > 0 && s.k < a.V;
-  s.list = s.cut && s.k <= a.k_list;
+  s.list = !s.greedy && s.cut && s.k <= a.k_list;
   s.run = s.p < 1.f;
   return s;
 }
@@ -158,15 +161,15 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int b) {
 // The weights of a row with a candidate, and the bins of its histogram: linear in
 // the logit, from the largest to where weights vanish or the smallest candidate.
 struct Scale {
-  double top, per;
+  double top, per, none, whole_of;          // none: a distance from the top of no weight
   float topf, step, bar;                    // bar: min_p's, the smallest float at or above it
-  int bits;
   bool inf;                                 // an infinite largest logit: the tokens at it share the row
   __device__ __forceinline__ Scale(const SampleArgs& a, const Setting& s, float most, uint32_t least) {
-    bits = a.bits;
     topf = most;
     inf = topf == INFINITY;
-    per = 1.44269504088896340736 / (double)s.t;
+    per = fmax(1.44269504088896340736 / (double)s.t, 0x1p-300);   // (an infinite temperature: all weigh 1)
+    none = -200.0 / per;
+    whole_of = WHOLE_OF + a.bits;
     bar = -INFINITY;
     if (s.m > 0.f) {
       double y = s.m < 1.f ? (double)topf + (double)s.t * log((double)s.m) : (double)topf;
@@ -174,18 +177,32 @@ struct Scale {
       bar = (float)y;
       if ((double)bar < y) bar = of_key(key_of(bar) + 1);
     }
-    bar = inf ? INFINITY : fmaxf(bar, -FLT_MAX);   // (candidates alone pass it)
+    bar = inf ? 0.f : fmaxf(bar, -FLT_MAX);   // (candidates alone pass it)
     if (inf) topf = 0.f;
     top = topf;
     const double far = a.bits + 2, all = (top - (inf ? 0.0 : (double)of_key(least))) * per;
     const double range = all < far ? all : far;
     step = range > 0.0 ? (float)(BINS * (1.0 - 1.0 / 1024) / range * per) : 0.f;
   }
-  // logits as the two below take them
+  // logits as the rest takes them, and the bar
   __device__ __forceinline__ float at(float y) const { return !inf ? y : y == INFINITY ? 0.f : -INFINITY; }
-  __device__ __forceinline__ uint64_t weight(float z) const { return weight_of(((double)z - top) * per, bits); }
-  __device__ __forceinline__ int bin(float z) const {   // BINS: no weight
-    return (int)fminf((topf - z) * step, (float)BINS);
+  __device__ __forceinline__ uint64_t raw(float z) const { return raw_weight(fmax((double)z - top, none), per, whole_of); }
+  __device__ __forceinline__ uint64_t weight(float z) const { return raw(z) - RAW; }
+  __device__ __forceinline__ float bin(float z) const {   // its whole part is the bin; BINS: no weight
+    return fminf((topf - z) * step, (float)BINS);
+  }
+  // The smallest logit of the bins before `end` (1 to BINS - 1), found by a wave: each
+  // lane tries one of 64 keys of what is left.
+  __device__ __forceinline__ float low_end(int end) const {
+    uint32_t lo = KEY_NONE + 1, hi = key_of(topf);   // (the bins are of falling logits, the top in the first)
+    while (lo < hi) {
+      const uint32_t stride = (hi - lo) / 64 + 1, off = (threadIdx.x % 64) * stride;
+      const uint64_t in = __ballot(bin(of_key(off < hi - lo ? lo + off : hi)) < (float)end);   // (from some lane on)
+      const uint32_t n = in ? __ffsll((long long)in) - 1 : 64;
+      if (n < 64 && n * stride < hi - lo) hi = lo + n * stride;
+      if (n > 0) lo += (n - 1) * stride + 1;
+    }
+    return of_key(hi);
   }
   template <int E>
   __device__ __forceinline__ void at(const float (&y)[E], float (&z)[E]) const {
@@ -199,9 +216,9 @@ struct Scale {
   // All of a vector's, whatever becomes of them: their chains of 64-bit operations
   // run beside each other.
   template <int E>
-  __device__ __forceinline__ void weights(const float (&z)[E], uint64_t (&w)[E]) const {
+  __device__ __forceinline__ void raws(const float (&z)[E], uint64_t (&w)[E]) const {
 #pragma unroll
-    for (int e = 0; e < E; ++e) w[e] = weight(z[e]);
+    for (int e = 0; e < E; ++e) w[e] = raw(z[e]);
 #pragma unroll
     for (int e = 0; e < E; ++e) asm("" : "+v"(w[e]));
   }
@@ -445,59 +462,66 @@ __device__ __forceinline__ void hist_into(S& sweep, const Scale& sc, uint64_t* h
     float z[E];
     uint64_t w[E];
     sc.at(y, z);
-    sc.weights(z, w);
+    sc.raws(z, w);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int at = sc.bin(z[e]);
-      if (at < BINS) atomicAdd((ull*)&hist[at], (ull)w[e]);
+      const float at = sc.bin(z[e]);
+      if (at < (float)BINS) atomicAdd((ull*)&hist[(int)at], (ull)(w[e] - RAW));
     }
   });
 }
 
-// put(tile, kept weight); with a border (below BINS) the tokens of that bin go to the
-// list, and those of the bins before it are kept.
-template <typename S, typename O, typename P>
-__device__ __forceinline__ void sums_into(S& sweep, const O& ord, const Scale& sc, int border, uint64_t* list, uint32_t* n,
-                                          P&& put) {
-  constexpr int E = S::R::E;
-  sweep.run([&](int v, const float (&y)[E]) __attribute__((always_inline)) {
-    float z[E];
-    uint64_t sum = 0, w[E];
-    sc.at(y, z);
-    if (border < BINS) {
-      bool listed = false, any = false;
-      int at[E];
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        at[e] = sc.bin(z[e]);
-        listed |= at[e] == border;
-        any |= at[e] < border;
-      }
-      if (__any(any)) {
-        sc.weights(z, w);
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += at[e] < border && y[e] >= sc.bar ? w[e] : 0;
-      }
-      if (listed) {
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (at[e] == border) {
-            const uint32_t i = atomicAdd(n, 1u);
-            if (i < LIST) list[i] = ord.place(key_of(y[e]), sweep.row.index(v, e));
-          }
-      }
-    } else {
-      bool any = false;
-#pragma unroll
-      for (int e = 0; e < E; ++e) any |= y[e] >= sc.bar;
-      if (__any(any)) {
-        sc.weights(z, w);
-#pragma unroll
-        for (int e = 0; e < E; ++e) sum += y[e] >= sc.bar ? w[e] : 0;
-      }
+// The bin of a row's last place kept: what lies above it is kept whole.
+struct Border {
+  float low, above;                         // its smallest logit, and the smallest above it
+  // (none: the row is kept whole)
+  __device__ __forceinline__ Border() : low(-INFINITY), above(-INFINITY) {}
+  // (two waves find an end each. s: two words)
+  __device__ __forceinline__ Border(const Scale& sc, int bin, uint64_t* s) {
+    const int wave = threadIdx.x / 64;
+    float* ends = (float*)s;
+    __syncthreads();
+    if (wave < 2) {
+      const float end = wave == 0 ? sc.low_end(bin + 1) : bin > 0 ? sc.low_end(bin) : INFINITY;
+      if (threadIdx.x % 64 == 0) ends[wave] = end;
     }
-    sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
+    __syncthreads();
+    low = ends[0], above = ends[1];
+  }
+};
+
+// put(tile, kept weight) of what lies above the border; the border's go to the list.
+template <typename S, typename O, typename P>
+__device__ __forceinline__ void sums_into(S& sweep, const O& ord, const Scale& sc, const Border& border, uint64_t* list,
+                                          uint32_t* n, P&& put) {
+  constexpr int E = S::R::E;
+  const float from = fmaxf(border.above, sc.bar);
+  sweep.run([&](int v, const float (&y)[E]) __attribute__((always_inline)) {
+    float z[E], most;
+    sc.at(y, z);
+    most = z[0];
+#pragma unroll
+    for (int e = 1; e < E; ++e) most = fmaxf(most, z[e]);
+    uint64_t sum = 0;
+    if (__any(most >= from)) {
+      float kept[E];
+      uint64_t w[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) kept[e] = z[e] >= from ? z[e] : -INFINITY;
+      sc.raws(kept, w);
+#pragma unroll
+      for (int e = 0; e < E; ++e) sum += w[e];
+      sum = last_lane(scan64(sum - E * RAW));
+    }
     if (threadIdx.x % 64 == 0) put(v / 64, sum);
+    if (border.low < border.above && most >= border.low) {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (z[e] >= border.low && z[e] < border.above) {
+          const uint32_t i = atomicAdd(n, 1u);
+          if (i < LIST) list[i] = ord.place(key_of(y[e]), sweep.row.index(v, e));
+        }
+    }
   });
 }
 
@@ -533,135 +557,6 @@ __device__ __forceinline__ int border_bin(const uint64_t* hist, float p, uint64_
   __syncthreads();
   before = s[1];
   return (int)s[0];
-}
-
-// ---------------------------------------------------------------------------
-// A row's parts, a launch a pass.
-
-template <typename T>
-__global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
-  __shared__ uint64_t s_first[PART / 64];
-  __shared__ uint32_t s_low[PART / 64];
-  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  if (part == 0 && threadIdx.x == 0) a.count[b] = 0;
-  if (a.runs)
-    for (int i = part * PART + threadIdx.x; i < BINS; i += a.parts * PART) a.hist[(int64_t)b * BINS + i] = 0;
-  const Row<T> row(a, b);
-  const Order<T> ord(a.V);
-  Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
-  float most, least;
-  int at;
-  ends_of(sweep, a.runs, most, at, least);
-  uint32_t g = key_of(most), low;
-  for (int d = 1; d < a.lanes; d *= 2) g = max(g, (uint32_t)__shfl_xor((int)g, d));
-  if (threadIdx.x % a.lanes == 0) a.maxima[((int64_t)b * a.parts + part) * a.groups + threadIdx.x / a.lanes] = g;
-  uint64_t first;
-  ends_of(row, ord, most, at, least, first, low);
-  first = wave_all(first, Most());
-  low = (uint32_t)wave_all(low, Most());
-  if (lane == 0) {
-    s_first[wave] = first;
-    s_low[wave] = low;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < PART / 64; ++w) {
-      first = s_first[w] > first ? s_first[w] : first;
-      low = max(low, s_low[w]);
-    }
-    a.part[(int64_t)b * a.parts + part] = Part{first, low, 0};
-  }
-}
-
-// A row's first place and smallest candidate's key, from its parts'.
-__device__ __forceinline__ void row_ends(const SampleArgs& a, int b, uint64_t& first, uint32_t& least) {
-  const Part* p = a.part + (int64_t)b * a.parts;
-  uint32_t low = 0;
-  first = 0;
-  for (int i = threadIdx.x % 64; i < a.parts; i += 64) {
-    first = p[i].first > first ? p[i].first : first;
-    low = max(low, p[i].low);
-  }
-  first = wave_all(first, Most());
-  least = ~(uint32_t)wave_all(low, Most());
-}
-
-// Appends the places that the part holds in s_list to the row's list.
-__device__ __forceinline__ void append(const SampleArgs& a, int b, const uint64_t* s_list, uint32_t n, uint32_t* s_at) {
-  __syncthreads();
-  if (threadIdx.x == 0 && n > 0) *s_at = atomicAdd(a.count + b, n);
-  __syncthreads();
-  if (n == 0 || n > LIST) return;
-  for (uint32_t i = threadIdx.x; i < n; i += PART)
-    if (*s_at + i < LIST) a.list[(int64_t)b * LIST + *s_at + i] = s_list[i];
-}
-
-template <typename T>
-__global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
-  __shared__ uint64_t s_mem[LIST];          // the list, or the histogram
-  __shared__ uint32_t s_n, s_at;
-  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64;
-  const Setting s = setting_of(a, b);
-  if (s.greedy || (!s.list && !(s.sums() && s.run))) return;
-  const Row<T> row(a, b);
-  const Order<T> ord(a.V);
-  if (s.list) {
-    Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
-    const int n_max = a.parts * a.groups;   // (a multiple of 4)
-    const uint32_t* mx = a.maxima + (int64_t)b * n_max;
-    uint32_t key[GROUPS / 64];
-#pragma unroll
-    for (int i = 0; i < GROUPS / 256; ++i) {
-      const u32x4 w = *(const u32x4*)(mx + min((i * 64 + lane) * 4, n_max - 4));
-#pragma unroll
-      for (int e = 0; e < 4; ++e) key[4 * i + e] = (i * 64 + lane) * 4 < n_max ? w[e] : 0;
-    }
-    const float bar = list_bar(key, s.k);
-    if (threadIdx.x == 0) s_n = 0;
-    __syncthreads();
-    gather_into(sweep, ord, bar, s_mem, &s_n);
-    __syncthreads();
-    append(a, b, s_mem, s_n, &s_at);
-    return;
-  }
-  uint64_t first;
-  uint32_t least;
-  row_ends(a, b, first, least);
-  if (first == 0) return;
-  const Scale sc(a, s, ord.logit(first), least);
-  for (int i = threadIdx.x; i < BINS; i += PART) s_mem[i] = 0;
-  __syncthreads();
-  Sweep<T, PART / 64, 2> sweep(row, part * a.tiles, a.tiles);
-  hist_into(sweep, sc, s_mem);
-  __syncthreads();
-  ull* to = (ull*)a.hist + (int64_t)b * BINS;
-  for (int i = threadIdx.x; i < BINS; i += PART)
-    if (s_mem[i]) atomicAdd(to + i, (ull)s_mem[i]);
-}
-
-template <typename T>
-__global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
-  __shared__ uint64_t s_list[LIST], s_scan[8];
-  __shared__ uint32_t s_n, s_at;
-  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts;
-  const Setting s = setting_of(a, b);
-  if (!s.sums()) return;
-  const Row<T> row(a, b);
-  const Order<T> ord(a.V);
-  Sweep<T, PART / 64, 2> sweep(row, part * a.tiles, a.tiles);
-  uint64_t first;
-  uint32_t least;
-  row_ends(a, b, first, least);
-  if (first == 0) return;
-  const Scale sc(a, s, ord.logit(first), least);
-  uint64_t before, goal;
-  const int border = s.run ? border_bin<PART>(a.hist + (int64_t)b * BINS, s.p, s_scan, before, goal) : BINS;
-  if (threadIdx.x == 0) s_n = 0;
-  __syncthreads();
-  uint64_t* sums = a.tile + (int64_t)b * a.parts * a.tiles;
-  sums_into(sweep, ord, sc, border, s_list, &s_n, [&](int tile, uint64_t w) __attribute__((always_inline)) { sums[tile] = w; });
-  __syncthreads();
-  if (s.run) append(a, b, s_list, s_n, &s_at);
 }
 
 // Values with a measure: narrows [lo, hi] (lo >= 1) towards the largest value at which
@@ -735,102 +630,70 @@ __device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_
   return *only;
 }
 
-// ---------------------------------------------------------------------------
-// A workgroup a row: the end of what the parts have begun, a short row, or all of a
-// long one.
-enum { SHORT, PARTS, WHOLE };
-__host__ __device__ constexpr int threads_of(int mode) { return mode == WHOLE ? 1024 : 512; }
+// A row's first place and smallest candidate's key, from its parts'.
+__device__ __forceinline__ void row_ends(const SampleArgs& a, int b, uint64_t& first, uint32_t& least) {
+  const Part* p = a.part + (int64_t)b * a.parts;
+  uint32_t low = 0;
+  first = 0;
+  for (int i = threadIdx.x % 64; i < a.parts; i += 64) {
+    first = p[i].first > first ? p[i].first : first;
+    low = max(low, p[i].low);
+  }
+  first = wave_all(first, Most());
+  least = ~(uint32_t)wave_all(low, Most());
+}
 
-template <typename T, int MODE>
-__global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleArgs a) {
+// ---------------------------------------------------------------------------
+// The end of a row: a workgroup draws its token.
+enum { SHORT, PARTS, WHOLE };               // a short row, one whose parts are through, a long one by a single workgroup
+__host__ __device__ constexpr int threads_of(int mode) { return mode == WHOLE ? 1024 : mode == PARTS ? PART : 512; }
+
+template <int MODE>
+struct Room {
+  static constexpr int N = threads_of(MODE);
+  uint64_t list[LIST], w[LIST], slot[MODE == SHORT ? 1 : SLOTS], scan[reach_words(N)], found[2];
+  uint64_t hist[MODE == WHOLE ? BINS : 1];
+  uint32_t max[MODE == WHOLE ? N : 4];
+  uint32_t n, at;
+  float bar;
+};
+
+// A word for a workgroup of the same launch, or of one.
+template <typename W>
+__device__ __forceinline__ void put(W* p, W w) { __hip_atomic_store(p, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename W>
+__device__ __forceinline__ W got(const W* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// A row without a candidate, and one of its first token alone.
+__device__ __forceinline__ void put_first(const SampleArgs& a, int b, uint64_t first, int index) {
+  if (threadIdx.x > 0) return;
+  a.token[b] = first ? index : 0;
+  a.logp[b] = first ? 0.f : __builtin_nanf("");
+}
+
+// What is known of a row: its border, if the kept weight of the tiles was summed, with
+// what the border's bin is to reach. n_cand: the tokens of its list.
+template <int MODE, typename T>
+__device__ __forceinline__ void finish(const SampleArgs& a, int b, const Setting& s, const Row<T>& row, const Order<T>& ord,
+                                       uint64_t first, const Scale& sc, Border border, uint64_t goal, uint32_t n_cand,
+                                       Room<MODE>& m) {
   using R = Row<T>;
   constexpr int N = threads_of(MODE);
-  __shared__ uint64_t s_list[LIST], s_w[LIST], s_slot[MODE == SHORT ? 1 : SLOTS], s_scan[reach_words(N)], s_found[2];
-  __shared__ uint64_t s_hist[MODE == WHOLE ? BINS : 1];
-  __shared__ __align__(16) uint32_t s_max[MODE == WHOLE ? N : 4], s_n;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
-  const Setting s = setting_of(a, b);
-  const R row(a, b);
-  const Order<T> ord(a.V);
+  const int tid = threadIdx.x, lane = tid % 64;
   const int tiles = (row.n_vec + 63) / 64, per = (tiles + SLOTS - 1) / SLOTS;   // tiles of a slot
-  uint32_t n_cand = MODE == PARTS ? a.count[b] : 0;
   const float u = a.u[b];
   // (loads that may turn out to be of nothing, made before it is known)
   const uint64_t *sums = a.tile + (int64_t)b * a.parts * a.tiles, *listed = a.list + (int64_t)b * LIST;
   uint64_t early_sum = 0, early_place = 0;
   if constexpr (MODE == PARTS) {
-    early_sum = sums[min(tid, a.parts * a.tiles - 1)];
-    early_place = listed[tid];
-  }
-  uint64_t first;
-  uint32_t least = KEY_NONE + 1;
-  if constexpr (MODE == PARTS) {
-    row_ends(a, b, first, least);
-  } else if constexpr (MODE == WHOLE) {
-    Sweep<T, N / 64, 4> sweep(row, 0, tiles);
-    float most, low;
-    int at;
-    uint32_t turned;
-    ends_of(sweep, a.runs, most, at, low);
-    s_max[tid] = key_of(most);
-    ends_of(row, ord, most, at, low, first, turned);
-    first = block_all<N>(first, s_scan, Most());
-    least = ~(uint32_t)block_all<N>(turned, s_scan, Most());
-  } else {
-    first = 0;
-    for (int v = tid; v < row.n_vec; v += N)
-      row.each(v, [&](float y, int i) __attribute__((always_inline)) {
-        const uint64_t place = ord.place(key_of(y), i);
-        if (i >= 0 && i < a.V) s_list[i] = place;
-        first = place > first ? place : first;
-      });
-    first = block_all<N>(first, s_scan, Most());
-  }
-  auto done = [&](int token, float logp) __attribute__((always_inline)) {
-    a.token[b] = token;
-    a.logp[b] = logp;
-  };
-  if (first == 0 || s.greedy) {
-    if (tid == 0) first == 0 ? done(0, __builtin_nanf("")) : done(ord.index(first), 0.f);
-    return;
-  }
-  const Scale sc(a, s, ord.logit(first), least);
-  int border = BINS;                        // the bin of the last place kept: those before it are kept whole
-  uint64_t before = 0, goal = 0;
-  if constexpr (MODE == WHOLE) {
-    if (tid == 0) s_n = 0;
-    for (int i = tid; i < SLOTS; i += N) s_slot[i] = 0;
-    for (int i = tid; i < BINS; i += N) s_hist[i] = 0;
-    __syncthreads();
-    if (s.list) {
-      Sweep<T, N / 64, 4> sweep(row, 0, tiles);
-      uint32_t key[N / 64];
-#pragma unroll
-      for (int i = 0; i < N / 256; ++i) {
-        const u32x4 w = *(const u32x4*)&s_max[(i * 64 + lane) * 4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) key[4 * i + e] = w[e];
-      }
-      gather_into(sweep, ord, list_bar(key, s.k), s_list, &s_n);
-    } else if (s.sums()) {
-      if (s.run) {
-        Sweep<T, N / 64, 2> sweep(row, 0, tiles);
-        hist_into(sweep, sc, s_hist);
-        __syncthreads();
-        border = border_bin<N>(s_hist, s.p, s_scan, before, goal);
-      }
-      Sweep<T, N / 64, 2> sweep(row, 0, tiles);
-      sums_into(sweep, ord, sc, border, s_list, &s_n, [&](int tile, uint64_t w) __attribute__((always_inline)) {
-        if (w) atomicAdd((ull*)&s_slot[tile / per], (ull)w);
-      });
-    }
-    __syncthreads();
-    n_cand = s_n;
+    early_sum = got(sums + min(tid, a.parts * a.tiles - 1));
+    early_place = got(listed + tid);
   }
   auto weight = [&](uint64_t place) __attribute__((always_inline)) { return sc.weight(sc.at(ord.logit(place))); };
   auto drawn = [&](float y, int i, uint64_t total) __attribute__((always_inline)) {
     const double d = ((double)sc.at(y) - sc.top) / (double)s.t;
-    done(i, (float)(d - log(ldexp((double)total, -a.bits))));
+    a.token[b] = i;
+    a.logp[b] = (float)(d - log(ldexp((double)total, -a.bits)));
   };
   auto aim_of = [&](uint64_t total) __attribute__((always_inline)) {
     const uint64_t aim = part_of(u, total, false);
@@ -843,67 +706,66 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
     const int n = MODE == SHORT ? a.V : (int)n_cand;
     uint64_t most_off = 0;
     for (int i = tid; i < n; i += N) {
-      const uint64_t place = MODE != PARTS ? s_list[i] : i == tid ? early_place : listed[i];
-      if constexpr (MODE == PARTS) s_list[i] = place;
-      s_w[i] = place ? weight(place) : 0;
+      const uint64_t place = MODE != PARTS ? m.list[i] : i == tid ? early_place : got(listed + i);
+      if constexpr (MODE == PARTS) m.list[i] = place;
+      m.w[i] = place ? weight(place) : 0;
       most_off = ~place > most_off && place ? ~place : most_off;
     }
-    const uint64_t least_place = ~block_all<N>(most_off, s_scan, Most());
-    auto place = [&](int i) __attribute__((always_inline)) { return s_list[i]; };
+    const uint64_t least_place = ~block_all<N>(most_off, m.scan, Most());
+    auto place = [&](int i) __attribute__((always_inline)) { return m.list[i]; };
     auto total_of = [&](auto&& kept) __attribute__((always_inline)) {
       uint64_t sum = 0;
-      for (int i = tid; i < n; i += N) sum += kept(i) ? s_w[i] : 0;
-      return block_all<N>(sum, s_scan, Plus());
+      for (int i = tid; i < n; i += N) sum += kept(i) ? m.w[i] : 0;
+      return block_all<N>(sum, m.scan, Plus());
     };
     uint64_t last = 1;                      // the last place kept
     if (s.cut) {
-      const uint64_t at = reach<N>(n, place, [](int) { return (uint64_t)1; }, least_place, first, s.k, s_scan);
+      const uint64_t at = reach<N>(n, place, [](int) { return (uint64_t)1; }, least_place, first, s.k, m.scan);
       if (at) last = at;                    // (0: there are fewer)
     }
     if (s.run) {
-      const uint64_t goal = part_of(s.p, total_of([&](int i) { return s_list[i] >= last; }), true);
-      last = goal <= 1 ? first : reach<N>(n, place, [&](int i) { return s_w[i]; }, last > 1 ? last : least_place, first, goal, s_scan);
+      const uint64_t goal = part_of(s.p, total_of([&](int i) { return m.list[i] >= last; }), true);
+      last = goal <= 1 ? first : reach<N>(n, place, [&](int i) { return m.w[i]; }, last > 1 ? last : least_place, first, goal, m.scan);
     }
-    auto kept = [&](int i) __attribute__((always_inline)) { return s_list[i] >= last && ord.logit(s_list[i]) >= sc.bar; };
+    auto kept = [&](int i) __attribute__((always_inline)) { return m.list[i] >= last && sc.at(ord.logit(m.list[i])) >= sc.bar; };
     const uint64_t total = total_of(kept), aim = aim_of(total);
     // by index: the first one is the largest number
-    auto turned = [&](int i) __attribute__((always_inline)) { return kept(i) ? (uint64_t)ord.turned(ord.index(s_list[i])) + 1 : 0; };
-    const uint64_t at = reach<N>(n, turned, [&](int i) { return s_w[i]; }, 1, (uint64_t)ord.turned(0) + 1, aim + 1, s_scan);
+    auto turned = [&](int i) __attribute__((always_inline)) { return kept(i) ? (uint64_t)ord.turned(ord.index(m.list[i])) + 1 : 0; };
+    const uint64_t at = reach<N>(n, turned, [&](int i) { return m.w[i]; }, 1, (uint64_t)ord.turned(0) + 1, aim + 1, m.scan);
     for (int i = tid; i < n; i += N)
-      if (turned(i) == at) drawn(ord.logit(s_list[i]), ord.index(s_list[i]), total);
+      if (turned(i) == at) drawn(ord.logit(m.list[i]), ord.index(m.list[i]), total);
     return;
   }
   if constexpr (MODE != SHORT) {
 
   uint64_t last = 1;                        // the last place kept
-  const bool ready = s.sums() && (!s.run || n_cand <= LIST);   // by the passes before
+  const bool ready = !s.cut && (!s.run || n_cand <= LIST);   // by the passes before
   if (MODE == PARTS || !ready) {
-    for (int i = tid; i < SLOTS; i += N) s_slot[i] = 0;
+    for (int i = tid; i < SLOTS; i += N) m.slot[i] = 0;
     __syncthreads();
   }
   if (ready) {
     if (s.run) {
-      if constexpr (MODE == PARTS) border = border_bin<N>(a.hist + (int64_t)b * BINS, s.p, s_scan, before, goal);
       const int n = (int)n_cand;
       uint64_t least_off = 0, most = 0;
       for (int i = tid; i < n; i += N) {
-        const uint64_t place = MODE != PARTS ? s_list[i] : i == tid ? early_place : listed[i];
-        if constexpr (MODE == PARTS) s_list[i] = place;
-        s_w[i] = weight(place);
+        const uint64_t place = MODE != PARTS ? m.list[i] : i == tid ? early_place : got(listed + i);
+        if constexpr (MODE == PARTS) m.list[i] = place;
+        m.w[i] = weight(place);
         least_off = ~place > least_off ? ~place : least_off;
         most = place > most ? place : most;
       }
-      least_off = block_all<N>(least_off, s_scan, Most());
-      most = block_all<N>(most, s_scan, Most());
-      last = reach<N>(n, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, ~least_off, most, goal - before, s_scan);
+      least_off = block_all<N>(least_off, m.scan, Most());
+      most = block_all<N>(most, m.scan, Most());
+      last = reach<N>(n, [&](int i) { return m.list[i]; }, [&](int i) { return m.w[i]; }, ~least_off, most, goal, m.scan);
       for (int i = tid; i < n; i += N)
-        if (s_list[i] >= last && ord.logit(s_list[i]) >= sc.bar)
-          atomicAdd((ull*)&s_slot[(ord.index(s_list[i]) + row.shift) / R::E / 64 / per], (ull)s_w[i]);
+        if (m.list[i] >= last && sc.at(ord.logit(m.list[i])) >= sc.bar)
+          atomicAdd((ull*)&m.slot[(ord.index(m.list[i]) + row.shift) / R::E / 64 / per], (ull)m.w[i]);
     }
     if constexpr (MODE == PARTS) {
       for (int i = tid; i < tiles; i += N) {
-        const uint64_t w = i == tid ? early_sum : sums[i];
-        if (w) atomicAdd((ull*)&s_slot[i / per], (ull)w);
+        const uint64_t w = i == tid ? early_sum : got(sums + i);
+        if (w) atomicAdd((ull*)&m.slot[i / per], (ull)w);
       }
     }
     __syncthreads();
@@ -921,22 +783,22 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
           const uint64_t place = ord.place(key_of(y), i);
           if (place >= lo && place <= hi) f(place, measure(y));
         });
-      }, lo, hi, goal, LIST, s_scan);
+      }, lo, hi, goal, LIST, m.scan);
       if (left == 0 || lo == hi) return left ? lo : 0;
-      if (tid == 0) s_n = 0;
+      if (tid == 0) m.n = 0;
       __syncthreads();
       over([&](float y, int i) __attribute__((always_inline)) {
         const uint64_t place = ord.place(key_of(y), i);
         if (place >= lo && place <= hi) {
-          const uint32_t at = atomicAdd(&s_n, 1u);
+          const uint32_t at = atomicAdd(&m.n, 1u);
           if (at < LIST) {
-            s_list[at] = place;
-            s_w[at] = measure(y);
+            m.list[at] = place;
+            m.w[at] = measure(y);
           }
         }
       });
       __syncthreads();
-      return reach<N>((int)left, [&](int i) { return s_list[i]; }, [&](int i) { return s_w[i]; }, lo, hi, goal, s_scan);
+      return reach<N>((int)left, [&](int i) { return m.list[i]; }, [&](int i) { return m.w[i]; }, lo, hi, goal, m.scan);
     };
     auto mass = [&](float y) __attribute__((always_inline)) { return sc.weight(sc.at(y)); };
     if (s.cut) {
@@ -948,21 +810,21 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
       over([&](float y, int i) __attribute__((always_inline)) {
         if (ord.place(key_of(y), i) >= last) sum += mass(y);
       });
-      sum = block_all<N>(sum, s_scan, Plus());
+      sum = block_all<N>(sum, m.scan, Plus());
       const uint64_t goal = part_of(s.p, sum, true);
       last = goal <= 1 ? first : far(mass, goal);
     }
-    border = -1;                            // (by place alone)
-    for (int i = tid; i < SLOTS; i += N) s_slot[i] = 0;
+    border.above = INFINITY;                // (by place alone)
+    for (int i = tid; i < SLOTS; i += N) m.slot[i] = 0;
     __syncthreads();
     for (int v = tid; v < tiles * 64; v += N) {
       uint64_t sum = 0;
       if (v < row.n_vec)
         row.each(v, [&](float y, int i) __attribute__((always_inline)) {
-          if (ord.place(key_of(y), i) >= last && y >= sc.bar) sum += mass(y);
+          if (ord.place(key_of(y), i) >= last && sc.at(y) >= sc.bar) sum += mass(y);
         });
       sum = __any(sum != 0) ? last_lane(scan64(sum)) : 0;
-      if (lane == 0 && sum) atomicAdd((ull*)&s_slot[v / 64 / per], (ull)sum);
+      if (lane == 0 && sum) atomicAdd((ull*)&m.slot[v / 64 / per], (ull)sum);
     }
     __syncthreads();
   }
@@ -971,34 +833,33 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
   constexpr int PER = SLOTS / N;
   uint64_t mine = 0, total;
 #pragma unroll
-  for (int e = 0; e < PER; ++e) mine += s_slot[tid * PER + e];
-  before = block_before<N>(mine, s_scan, total);
+  for (int e = 0; e < PER; ++e) mine += m.slot[tid * PER + e];
+  uint64_t upto_slot = block_before<N>(mine, m.scan, total);
   const uint64_t aim = aim_of(total);
-  if (before <= aim && before + mine > aim) {
+  if (upto_slot <= aim && upto_slot + mine > aim) {
     int e = 0;
-    while (before + s_slot[tid * PER + e] <= aim) before += s_slot[tid * PER + e++];
-    s_found[0] = tid * PER + e;
-    s_found[1] = before;
+    while (upto_slot + m.slot[tid * PER + e] <= aim) upto_slot += m.slot[tid * PER + e++];
+    m.found[0] = tid * PER + e;
+    m.found[1] = upto_slot;
   }
   __syncthreads();
   if (tid >= 64) return;
-  before = s_found[1];
-  for (int t = (int)s_found[0] * per; t < tiles; ++t) {
+  uint64_t sum_before = m.found[1];
+  for (int t = (int)m.found[0] * per; t < tiles; ++t) {
     const int v = t * 64 + lane;
     float y[R::E];
     uint64_t w[R::E], sum = 0;
     row.unpack(row.load(v), v, y);
 #pragma unroll
     for (int e = 0; e < R::E; ++e) {
-      const uint64_t place = ord.place(key_of(y[e]), row.index(v, e)), z = sc.weight(sc.at(y[e]));
-      const int at = sc.bin(sc.at(y[e]));
-      const bool in = border < 0 ? place >= last : border == BINS || at < border || (at == border && place >= last);
-      w[e] = in && y[e] >= sc.bar ? z : 0;
+      const float z = sc.at(y[e]);
+      const bool in = z >= border.above || ord.place(key_of(y[e]), row.index(v, e)) >= last;
+      w[e] = in && z >= sc.bar ? sc.weight(z) : 0;
       sum += w[e];
     }
     const uint64_t upto = scan64(sum);
-    if (before + last_lane(upto) > aim) {
-      uint64_t sofar = before + upto - sum;
+    if (sum_before + last_lane(upto) > aim) {
+      uint64_t sofar = sum_before + upto - sum;
       if (sofar <= aim && sofar + sum > aim) {
 #pragma unroll
         for (int e = 0; e < R::E; ++e) {
@@ -1008,10 +869,243 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
       }
       return;
     }
-    before += last_lane(upto);
+    sum_before += last_lane(upto);
   }
 
   }
+}
+
+
+// A row by one workgroup.
+template <typename T, int MODE>
+__global__ __launch_bounds__(threads_of(MODE)) void sample_row_kernel(SampleArgs a) {
+  constexpr int N = threads_of(MODE);
+  __shared__ __align__(16) Room<MODE> m;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
+  const Setting s = setting_of(a, b);
+  const Row<T> row(a, b);
+  const Order<T> ord(a.V);
+  const int tiles = (row.n_vec + 63) / 64, per = (tiles + SLOTS - 1) / SLOTS;   // tiles of a slot
+  uint64_t first;
+  uint32_t least = KEY_NONE + 1;
+  if constexpr (MODE == PARTS) {
+    row_ends(a, b, first, least);
+  } else if constexpr (MODE == WHOLE) {
+    Sweep<T, N / 64, 4> sweep(row, 0, tiles);
+    float most, low;
+    int at;
+    uint32_t turned;
+    ends_of(sweep, a.runs, most, at, low);
+    m.max[tid] = key_of(most);
+    ends_of(row, ord, most, at, low, first, turned);
+    first = block_all<N>(first, m.scan, Most());
+    least = ~(uint32_t)block_all<N>(turned, m.scan, Most());
+  } else {
+    first = 0;
+    for (int v = tid; v < row.n_vec; v += N)
+      row.each(v, [&](float y, int i) __attribute__((always_inline)) {
+        const uint64_t place = ord.place(key_of(y), i);
+        if (i >= 0 && i < a.V) m.list[i] = place;
+        first = place > first ? place : first;
+      });
+    first = block_all<N>(first, m.scan, Most());
+  }
+  if (first == 0 || s.greedy) {
+    put_first(a, b, first, ord.index(first));
+    return;
+  }
+  const Scale sc(a, s, ord.logit(first), least);
+  Border border;
+  uint64_t before = 0, goal = 0;
+  uint32_t n_cand = 0;
+  if constexpr (MODE == WHOLE) {
+    if (tid == 0) m.n = 0;
+    for (int i = tid; i < SLOTS; i += N) m.slot[i] = 0;
+    for (int i = tid; i < BINS; i += N) m.hist[i] = 0;
+    __syncthreads();
+    if (s.list) {
+      Sweep<T, N / 64, 4> sweep(row, 0, tiles);
+      if (tid < 64) {                       // (one wave, for all)
+        uint32_t key[N / 64];
+#pragma unroll
+        for (int i = 0; i < N / 256; ++i) {
+          const u32x4 w = *(const u32x4*)&m.max[(i * 64 + lane) * 4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) key[4 * i + e] = w[e];
+        }
+        m.bar = list_bar(key, s.k);
+      }
+      __syncthreads();
+      gather_into(sweep, ord, m.bar, m.list, &m.n);
+    } else if (!s.cut) {
+      if (s.run) {
+        Sweep<T, N / 64, 2> sweep(row, 0, tiles);
+        hist_into(sweep, sc, m.hist);
+        __syncthreads();
+        border = Border(sc, border_bin<N>(m.hist, s.p, m.scan, before, goal), m.scan + 2);
+      }
+      Sweep<T, N / 64, 2> sweep(row, 0, tiles);
+      sums_into(sweep, ord, sc, border, m.list, &m.n, [&](int tile, uint64_t w) __attribute__((always_inline)) {
+        if (w) atomicAdd((ull*)&m.slot[tile / per], (ull)w);
+      });
+    }
+    __syncthreads();
+    n_cand = m.n;
+  }
+  finish<MODE>(a, b, s, row, ord, first, sc, border, goal - before, n_cand, m);
+}
+
+// ---------------------------------------------------------------------------
+// A row's parts, a launch a pass.
+
+template <typename T>
+__global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
+  __shared__ uint64_t s_first[PART / 64];
+  __shared__ uint32_t s_low[PART / 64];
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  if (part == 0 && threadIdx.x == 0) a.count[b] = a.ended[b] = 0;
+  if (a.runs)
+    for (int i = part * PART + threadIdx.x; i < BINS; i += a.parts * PART) a.hist[(int64_t)b * BINS + i] = 0;
+  const Row<T> row(a, b);
+  const Order<T> ord(a.V);
+  Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
+  float most, least;
+  int at;
+  ends_of(sweep, a.runs, most, at, least);
+  uint32_t g = key_of(most), low;
+  for (int d = 1; d < a.lanes; d *= 2) g = max(g, (uint32_t)__shfl_xor((int)g, d));
+  if (threadIdx.x % a.lanes == 0) a.maxima[((int64_t)b * a.parts + part) * a.groups + threadIdx.x / a.lanes] = g;
+  uint64_t first;
+  ends_of(row, ord, most, at, least, first, low);
+  first = wave_all(first, Most());
+  low = (uint32_t)wave_all(low, Most());
+  if (lane == 0) {
+    s_first[wave] = first;
+    s_low[wave] = low;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < PART / 64; ++w) {
+      first = s_first[w] > first ? s_first[w] : first;
+      low = max(low, s_low[w]);
+    }
+    a.part[(int64_t)b * a.parts + part] = Part{first, low, 0};
+  }
+}
+
+// Appends the places that the part holds to the row's list.
+__device__ __forceinline__ void append(const SampleArgs& a, int b, Room<PARTS>& m) {
+  __syncthreads();
+  const uint32_t n = m.n;
+  if (threadIdx.x == 0 && n > 0) m.at = atomicAdd(a.count + b, n);
+  __syncthreads();
+  if (n == 0 || n > LIST) return;
+  for (uint32_t i = threadIdx.x; i < n; i += PART)
+    if (m.at + i < LIST) put(a.list + (int64_t)b * LIST + m.at + i, m.list[i]);
+}
+
+// Whether all of a row's parts are through, for the last of them. What they tell it is
+// put() and got(), at the device's scope: each wave waits until its words are out before
+// its part counts as through, and what the last one reads comes after. Nobody waits for
+// another part.
+__device__ __forceinline__ bool last_part(const SampleArgs& a, int b, Room<PARTS>& m) {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (threadIdx.x == 0) m.at = atomicAdd(a.ended + b, 1u);
+  __syncthreads();
+  return (int)m.at == a.parts - 1;
+}
+
+// top_k's lists, and top_p's histograms. Where no sums follow (all rows have a list), the
+// last part of a row ends it.
+template <typename T>
+__global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
+  __shared__ __align__(16) Room<PARTS> m;
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64;
+  const Setting s = setting_of(a, b);
+  if (a.sums && !(s.cut ? s.list : s.run && !s.greedy)) return;
+  const Row<T> row(a, b);
+  const Order<T> ord(a.V);
+  if (s.list) {
+    Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
+    if (threadIdx.x < 64) {                 // (one wave, for all)
+      const int n_max = a.parts * a.groups; // (a multiple of 4)
+      const uint32_t* mx = a.maxima + (int64_t)b * n_max;
+      uint32_t key[GROUPS / 64];
+#pragma unroll
+      for (int i = 0; i < GROUPS / 256; ++i) {
+        const u32x4 w = *(const u32x4*)(mx + min((i * 64 + lane) * 4, n_max - 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) key[4 * i + e] = (i * 64 + lane) * 4 < n_max ? w[e] : 0;
+      }
+      const float bar = list_bar(key, s.k);
+      if (lane == 0) {
+        m.bar = bar;
+        m.n = 0;
+      }
+    }
+    __syncthreads();
+    const float bar = m.bar;
+    gather_into(sweep, ord, bar, m.list, &m.n);
+    append(a, b, m);
+    if (a.sums || !last_part(a, b, m)) return;
+  } else if (!a.sums && part > 0) {
+    return;                                 // (a greedy row)
+  }
+  uint64_t first;
+  uint32_t least;
+  row_ends(a, b, first, least);
+  if (first == 0 || s.greedy) {
+    if (!a.sums) put_first(a, b, first, ord.index(first));
+    return;
+  }
+  const Scale sc(a, s, ord.logit(first), least);
+  if (!a.sums) {
+    finish<PARTS>(a, b, s, row, ord, first, sc, Border(), 0, got(a.count + b), m);
+    return;
+  }
+  for (int i = threadIdx.x; i < BINS; i += PART) m.w[i] = 0;
+  __syncthreads();
+  Sweep<T, PART / 64, 2> sweep(row, part * a.tiles, a.tiles);
+  hist_into(sweep, sc, m.w);
+  __syncthreads();
+  ull* to = (ull*)a.hist + (int64_t)b * BINS;
+  for (int i = threadIdx.x; i < BINS; i += PART)
+    if (m.w[i]) atomicAdd(to + i, (ull)m.w[i]);
+}
+
+// The kept weight of the tiles; the last part of a row ends it.
+template <typename T>
+__global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
+  __shared__ __align__(16) Room<PARTS> m;
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts;
+  const Setting s = setting_of(a, b);
+  const bool alone = s.greedy || s.cut;     // ended by one part, without sums
+  if (alone && part > 0) return;
+  const Row<T> row(a, b);
+  const Order<T> ord(a.V);
+  Sweep<T, PART / 64, 2> sweep(row, part * a.tiles, a.tiles);
+  uint64_t first;
+  uint32_t least;
+  row_ends(a, b, first, least);
+  if (first == 0 || s.greedy) {
+    if (part == 0) put_first(a, b, first, ord.index(first));
+    return;
+  }
+  const Scale sc(a, s, ord.logit(first), least);
+  uint64_t before = 0, goal = 0;
+  Border border;
+  if (alone) {
+    finish<PARTS>(a, b, s, row, ord, first, sc, border, 0, got(a.count + b), m);
+    return;
+  }
+  if (s.run) border = Border(sc, border_bin<PART>(a.hist + (int64_t)b * BINS, s.p, m.scan, before, goal), m.scan + 2);
+  if (threadIdx.x == 0) m.n = 0;
+  __syncthreads();
+  uint64_t* sums = a.tile + (int64_t)b * a.parts * a.tiles;
+  sums_into(sweep, ord, sc, border, m.list, &m.n, [&](int tile, uint64_t w) __attribute__((always_inline)) { put(sums + tile, w); });
+  if (s.run) append(a, b, m);
+  if (last_part(a, b, m)) finish<PARTS>(a, b, s, row, ord, first, sc, border, goal - before, got(a.count + b), m);
 }
 
 // ---------------------------------------------------------------------------
@@ -1019,7 +1113,7 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_finish_kernel(SampleA
 
 struct Plan {
   int parts, tiles, groups, lanes;          // parts 0: a workgroup a row, one launch
-  size_t part, maxima, count, hist, list, tile, bytes;   // offsets
+  size_t part, maxima, count, ended, hist, list, tile, bytes;   // offsets
 };
 
 // A workgroup takes a whole row where there are rows for most CUs, or short ones. 128256
@@ -1034,11 +1128,11 @@ void plan_for(Plan& p, int B, int V, int dtype) {
   if (by_rows(B, V)) return;
   const int E = dtype == DA_FP32 ? 4 : 8;
   const int64_t tiles = ((int64_t)V + 2 * E - 1) / E / 64 + 1;   // whatever the row's alignment
-  // parts: some workgroups for each CU together, 4 tiles (one of each wave) at least
+  // parts: some workgroups for each CU together, 8 tiles (one of each wave) at least
   int64_t parts = (512 + B - 1) / B;
   parts = parts < 4 ? 4 : parts > 32 ? 32 : parts;
-  while (parts > 4 && tiles < parts * 4) parts /= 2;
-  p.tiles = (int)(((tiles + parts - 1) / parts + 3) / 4 * 4);
+  while (parts > 4 && tiles < parts * 8) parts /= 2;
+  p.tiles = (int)(((tiles + parts - 1) / parts + 7) / 8 * 8);
   p.parts = (int)parts;
   p.lanes = 1;
   while (p.parts * (PART / p.lanes) > GROUPS) p.lanes *= 2;
@@ -1052,6 +1146,7 @@ void plan_for(Plan& p, int B, int V, int dtype) {
   p.part = room(sizeof(Part) * p.parts);
   p.maxima = room(sizeof(uint32_t) * p.parts * p.groups);
   p.count = room(sizeof(uint32_t));
+  p.ended = room(sizeof(uint32_t));
   p.hist = room(sizeof(uint64_t) * BINS);
   p.list = room(sizeof(uint64_t) * LIST);
   p.tile = room(sizeof(uint64_t) * p.parts * p.tiles);
@@ -1061,7 +1156,7 @@ void plan_for(Plan& p, int B, int V, int dtype) {
 template <typename T>
 void launch(SampleArgs& a, hipStream_t st) {
   if (a.V <= LIST) {
-    hipLaunchKernelGGL((sample_finish_kernel<T, SHORT>), dim3(a.B), dim3(threads_of(SHORT)), 0, st, a);
+    hipLaunchKernelGGL((sample_row_kernel<T, SHORT>), dim3(a.B), dim3(threads_of(SHORT)), 0, st, a);
     return;
   }
   // (what no row can ask for is not launched)
@@ -1070,14 +1165,17 @@ void launch(SampleArgs& a, hipStream_t st) {
   const bool p_on = a.p_dev || a.p < 1.f;
   a.runs = t_on && p_on && !k_all;
   if (a.parts == 0) {
-    hipLaunchKernelGGL((sample_finish_kernel<T, WHOLE>), dim3(a.B), dim3(threads_of(WHOLE)), 0, st, a);
+    hipLaunchKernelGGL((sample_row_kernel<T, WHOLE>), dim3(a.B), dim3(threads_of(WHOLE)), 0, st, a);
     return;
   }
   const dim3 grid(a.parts * a.B);
+  a.sums = t_on && !k_all;
+  const bool gather = t_on && (k_list || a.runs);
   hipLaunchKernelGGL((sample_top_kernel<T>), grid, dim3(PART), 0, st, a);
-  if (t_on && (k_list || (p_on && !k_all))) hipLaunchKernelGGL((sample_gather_kernel<T>), grid, dim3(PART), 0, st, a);
-  if (t_on && !k_all) hipLaunchKernelGGL((sample_sums_kernel<T>), grid, dim3(PART), 0, st, a);
-  hipLaunchKernelGGL((sample_finish_kernel<T, PARTS>), dim3(a.B), dim3(threads_of(PARTS)), 0, st, a);
+  if (gather) hipLaunchKernelGGL((sample_gather_kernel<T>), grid, dim3(PART), 0, st, a);
+  if (a.sums) hipLaunchKernelGGL((sample_sums_kernel<T>), grid, dim3(PART), 0, st, a);
+  // (all greedy, or a top_k past the lists)
+  if (!gather && !a.sums) hipLaunchKernelGGL((sample_row_kernel<T, PARTS>), dim3(a.B), dim3(PART), 0, st, a);
 }
 
 }  // namespace
@@ -1128,6 +1226,7 @@ extern "C" int da_sample(const da_sample_args* x, void* stream) {
   a.part = (Part*)(ws + p.part);
   a.maxima = (uint32_t*)(ws + p.maxima);
   a.count = (uint32_t*)(ws + p.count);
+  a.ended = (uint32_t*)(ws + p.ended);
   a.hist = (uint64_t*)(ws + p.hist);
   a.list = (uint64_t*)(ws + p.list);
   a.tile = (uint64_t*)(ws + p.tile);
