@@ -643,6 +643,26 @@ __device__ __forceinline__ void row_ends(const SampleArgs& a, int b, uint64_t& f
   least = ~(uint32_t)wave_all(low, Most());
 }
 
+// A short list's n <= FEW values by pairs, N / FEW threads a value: how many are larger
+// than this thread's, and their weight.
+constexpr int FEW = 128;
+template <int N, typename V>
+__device__ __forceinline__ void above(int n, V&& value, const uint64_t* w, uint64_t mine, uint32_t& many, uint64_t& weight) {
+  constexpr int Q = N / FEW;
+  many = 0, weight = 0;
+#pragma unroll 4
+  for (int j = threadIdx.x % Q; j < n; j += Q) {
+    const bool larger = value(j) > mine;
+    many += larger;
+    weight += larger ? w[j] : 0;
+  }
+#pragma unroll
+  for (int d = 1; d < Q; d *= 2) {
+    many += __shfl_xor((int)many, d);
+    weight += (uint64_t)__shfl_xor((long long)weight, d);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // The end of a row: a workgroup draws its token.
 enum { SHORT, PARTS, WHOLE };               // a short row, one whose parts are through, a long one by a single workgroup
@@ -711,6 +731,28 @@ __device__ __forceinline__ void finish(const SampleArgs& a, int b, const Setting
       m.w[i] = place ? weight(place) : 0;
       most_off = ~place > most_off && place ? ~place : most_off;
     }
+    if (n <= FEW) {
+      constexpr int Q = N / FEW;
+      __syncthreads();
+      const int i = tid / Q;
+      const uint64_t place = i < n ? m.list[i] : 0, w = i < n ? m.w[i] : 0;
+      uint32_t rank;
+      uint64_t sum;
+      above<N>(n, [&](int j) { return m.list[j]; }, m.w, place, rank, sum);
+      bool kept = place && (!s.cut || rank < (uint32_t)s.k);
+      if (s.run) {
+        const uint64_t goal = part_of(s.p, block_all<N>(tid % Q == 0 && kept ? w : 0, m.scan, Plus()), true);
+        kept = kept && (sum < goal || rank == 0);
+      }
+      kept = kept && sc.at(ord.logit(place)) >= sc.bar;
+      const uint64_t total = block_all<N>(tid % Q == 0 && kept ? w : 0, m.scan, Plus()), aim = aim_of(total);
+      if (tid % Q == 0 && i < n) m.w[i] = kept ? w : 0;
+      __syncthreads();
+      auto turned = [&](uint64_t place) { return ord.turned(ord.index(place)); };   // (the first index is the largest)
+      above<N>(n, [&](int j) { return turned(m.list[j]); }, m.w, turned(place), rank, sum);
+      if (tid % Q == 0 && kept && sum <= aim && sum + w > aim) drawn(ord.logit(place), ord.index(place), total);
+      return;
+    }
     const uint64_t least_place = ~block_all<N>(most_off, m.scan, Most());
     auto place = [&](int i) __attribute__((always_inline)) { return m.list[i]; };
     auto total_of = [&](auto&& kept) __attribute__((always_inline)) {
@@ -755,9 +797,23 @@ __device__ __forceinline__ void finish(const SampleArgs& a, int b, const Setting
         least_off = ~place > least_off ? ~place : least_off;
         most = place > most ? place : most;
       }
-      least_off = block_all<N>(least_off, m.scan, Most());
-      most = block_all<N>(most, m.scan, Most());
-      last = reach<N>(n, [&](int i) { return m.list[i]; }, [&](int i) { return m.w[i]; }, ~least_off, most, goal, m.scan);
+      if (n <= FEW) {
+        constexpr int Q = N / FEW;
+        if (tid == 0) m.found[0] = 0;
+        __syncthreads();
+        const int i = tid / Q;
+        const uint64_t place = i < n ? m.list[i] : 0, w = i < n ? m.w[i] : 0;
+        uint32_t rank;
+        uint64_t sum;
+        above<N>(n, [&](int j) { return m.list[j]; }, m.w, place, rank, sum);
+        if (tid % Q == 0 && sum < goal && sum + w >= goal) m.found[0] = place;
+        __syncthreads();
+        last = m.found[0];
+      } else {
+        least_off = block_all<N>(least_off, m.scan, Most());
+        most = block_all<N>(most, m.scan, Most());
+        last = reach<N>(n, [&](int i) { return m.list[i]; }, [&](int i) { return m.w[i]; }, ~least_off, most, goal, m.scan);
+      }
       for (int i = tid; i < n; i += N)
         if (m.list[i] >= last && sc.at(ord.logit(m.list[i])) >= sc.bar)
           atomicAdd((ull*)&m.slot[(ord.index(m.list[i]) + row.shift) / R::E / 64 / per], (ull)m.w[i]);
