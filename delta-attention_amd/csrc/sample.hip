@@ -52,7 +52,7 @@ constexpr uint32_t KEY_NONE = 0x007fffffu;   // -inf's key: candidates lie above
 constexpr int PART = 512;                    // threads of a part
 constexpr int LIST = 3584;                   // tokens of a row's list (two finishing workgroups' LDS a CU)
 constexpr int BINS = 768;                    // of a part's histogram
-constexpr int GROUPS = 2048;                 // group maxima of a row at most
+constexpr int GROUPS = 2048;                 // group maxima of a row
 constexpr int SLOTS = 1024;                  // tile sums in LDS
 
 struct Part {
@@ -75,10 +75,10 @@ struct SampleArgs {
   int parts, tiles, k_list;                 // parts of a row, tiles of a part, the largest top_k with a list
   FastDiv f_parts;
   int runs, sums;                           // whether rows may take a histogram, and whether the sums are launched
-  int groups, lanes;                        // group maxima of a part, lanes of a group
+  int lanes;                                // of a group
   // workspace, by row
   Part* part;                               // [parts]
-  uint32_t* maxima;                         // [parts * groups]
+  uint32_t* maxima;                         // [GROUPS]
   uint32_t* count;                          // tokens gathered (also past the list's end)
   uint32_t* ended;                          // parts that are through
   uint64_t* hist;                           // [BINS]
@@ -269,6 +269,7 @@ struct Row {
 template <typename T, int W, int U>
 struct Sweep {
   using R = Row<T>;
+  static constexpr int WAVES = W;
   const R& row;
   int first, n;
   u32x4 w[U];
@@ -378,11 +379,13 @@ __device__ __forceinline__ uint64_t part_of(float f, uint64_t total, bool up) {
 // The passes over a row, or a part of one.
 
 // This thread's largest number, the vector that held it first, and (want) its
-// smallest candidate.
-template <typename S>
-__device__ __forceinline__ void ends_of(S& sweep, bool want, float& most, int& at, float& least) {
+// smallest candidate. group: the largest of its G groups of vectors (G tiles take turns).
+template <int G, typename S>
+__device__ __forceinline__ void ends_of(S& sweep, bool want, float& most, int& at, float& least, float (&group)[G]) {
   constexpr int E = S::R::E;
   most = -INFINITY, least = INFINITY, at = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) group[g] = -INFINITY;
   sweep.run([&](int v, const float (&y)[E]) __attribute__((always_inline)) {
     float top = y[0];
 #pragma unroll
@@ -395,6 +398,8 @@ __device__ __forceinline__ void ends_of(S& sweep, bool want, float& most, int& a
       most = top;
       at = v;
     }
+#pragma unroll
+    for (int g = 0; g < G; ++g) group[g] = fmaxf(group[g], v / (64 * S::WAVES) % G == g ? top : -INFINITY);
   });
 }
 // Its first place and its smallest candidate's key turned round (0: no candidate).
@@ -673,7 +678,7 @@ struct Room {
   static constexpr int N = threads_of(MODE);
   uint64_t list[LIST], w[LIST], slot[MODE == SHORT ? 1 : SLOTS], scan[reach_words(N)], found[2];
   uint64_t hist[MODE == WHOLE ? BINS : 1];
-  uint32_t max[MODE == WHOLE ? N : 4];
+  uint32_t max[MODE == WHOLE ? GROUPS : 4];
   uint32_t n, at;
   float bar;
 };
@@ -951,8 +956,10 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_row_kernel(SampleArgs
     float most, low;
     int at;
     uint32_t turned;
-    ends_of(sweep, a.runs, most, at, low);
-    m.max[tid] = key_of(most);
+    float group[GROUPS / N];
+    ends_of(sweep, a.runs, most, at, low, group);
+#pragma unroll
+    for (int g = 0; g < GROUPS / N; ++g) m.max[g * N + tid] = key_of(group[g]);
     ends_of(row, ord, most, at, low, first, turned);
     first = block_all<N>(first, m.scan, Most());
     least = ~(uint32_t)block_all<N>(turned, m.scan, Most());
@@ -982,9 +989,9 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_row_kernel(SampleArgs
     if (s.list) {
       Sweep<T, N / 64, 4> sweep(row, 0, tiles);
       if (tid < 64) {                       // (one wave, for all)
-        uint32_t key[N / 64];
+        uint32_t key[GROUPS / 64];
 #pragma unroll
-        for (int i = 0; i < N / 256; ++i) {
+        for (int i = 0; i < GROUPS / 256; ++i) {
           const u32x4 w = *(const u32x4*)&m.max[(i * 64 + lane) * 4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) key[4 * i + e] = w[e];
@@ -1027,10 +1034,11 @@ __global__ __launch_bounds__(PART) void sample_top_kernel(SampleArgs a) {
   Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
   float most, least;
   int at;
-  ends_of(sweep, a.runs, most, at, least);
-  uint32_t g = key_of(most), low;
+  float group[1];
+  ends_of(sweep, a.runs, most, at, least, group);
+  uint32_t g = key_of(group[0]), low;
   for (int d = 1; d < a.lanes; d *= 2) g = max(g, (uint32_t)__shfl_xor((int)g, d));
-  if (threadIdx.x % a.lanes == 0) a.maxima[((int64_t)b * a.parts + part) * a.groups + threadIdx.x / a.lanes] = g;
+  if (threadIdx.x % a.lanes == 0) a.maxima[(int64_t)b * GROUPS + (part * PART + threadIdx.x) / a.lanes] = g;
   uint64_t first;
   ends_of(row, ord, most, at, least, first, low);
   first = wave_all(first, Most());
@@ -1085,14 +1093,13 @@ __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
   if (s.list) {
     Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
     if (threadIdx.x < 64) {                 // (one wave, for all)
-      const int n_max = a.parts * a.groups; // (a multiple of 4)
-      const uint32_t* mx = a.maxima + (int64_t)b * n_max;
+      const uint32_t* mx = a.maxima + (int64_t)b * GROUPS;
       uint32_t key[GROUPS / 64];
 #pragma unroll
       for (int i = 0; i < GROUPS / 256; ++i) {
-        const u32x4 w = *(const u32x4*)(mx + min((i * 64 + lane) * 4, n_max - 4));
+        const u32x4 w = *(const u32x4*)(mx + (i * 64 + lane) * 4);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) key[4 * i + e] = (i * 64 + lane) * 4 < n_max ? w[e] : 0;
+        for (int e = 0; e < 4; ++e) key[4 * i + e] = w[e];
       }
       const float bar = list_bar(key, s.k);
       if (lane == 0) {
@@ -1168,7 +1175,7 @@ __global__ __launch_bounds__(PART) void sample_sums_kernel(SampleArgs a) {
 // host side
 
 struct Plan {
-  int parts, tiles, groups, lanes;          // parts 0: a workgroup a row, one launch
+  int parts, tiles, lanes;                  // parts 0: a workgroup a row, one launch
   size_t part, maxima, count, ended, hist, list, tile, bytes;   // offsets
 };
 
@@ -1177,7 +1184,7 @@ struct Plan {
 // 29 (top_k 50), 96 / 74 (a flat nucleus); 256 rows 55 / 62, 37 / 43, 101 / 113. 16000
 // tokens: 64 rows 16 / 16, 25 / 23, 29 / 29; 256 rows 17 / 20, 24 / 26, 30 / 37. 5000
 // tokens, one row: 12.1 / 13.3, 19.0 / 18.7, 21.5 / 23.0.
-bool by_rows(int B, int V) { return B >= 160 || V <= 8192; }
+bool by_rows(int B, int V) { return B >= 160 || V <= 8192 || (B >= 64 && V <= 32768); }
 
 void plan_for(Plan& p, int B, int V, int dtype, bool differ) {
   p = Plan{};
@@ -1193,7 +1200,6 @@ void plan_for(Plan& p, int B, int V, int dtype, bool differ) {
   p.tiles = (int)(((tiles + parts - 1) / parts + 7) / 8 * 8);
   p.parts = (int)parts;
   p.lanes = p.parts * PART / GROUPS;
-  p.groups = PART / p.lanes;
   size_t at = 0;
   auto room = [&](size_t bytes) {
     const size_t here = at;
@@ -1201,7 +1207,7 @@ void plan_for(Plan& p, int B, int V, int dtype, bool differ) {
     return here;
   };
   p.part = room(sizeof(Part) * p.parts);
-  p.maxima = room(sizeof(uint32_t) * p.parts * p.groups);
+  p.maxima = room(sizeof(uint32_t) * GROUPS);
   p.count = room(sizeof(uint32_t));
   p.ended = room(sizeof(uint32_t));
   p.hist = room(sizeof(uint64_t) * BINS);
@@ -1281,8 +1287,8 @@ extern "C" int da_sample(const da_sample_args* x, void* stream) {
   if (a.bits > 45) a.bits = 45;
   a.parts = p.parts, a.tiles = p.tiles;
   a.f_parts = make_fastdiv(p.parts > 0 ? p.parts : 1);
-  a.groups = p.groups, a.lanes = p.lanes;
-  a.k_list = (p.parts > 0 ? p.parts * p.groups : threads_of(WHOLE)) / 4 * 3;
+  a.lanes = p.lanes;
+  a.k_list = GROUPS / 4 * 3;
   char* ws = (char*)x->workspace;
   a.part = (Part*)(ws + p.part);
   a.maxima = (uint32_t*)(ws + p.maxima);
