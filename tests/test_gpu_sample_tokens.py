@@ -44,7 +44,7 @@ def check(x, u, got=None, sure=True, **settings):
     from delta_attention import ops
     tok, lp = got if got is not None else ops.sample_tokens(x, u, **settings)
     assert tok.dtype == torch.int64 and lp.dtype == torch.float32 and tok.shape == lp.shape == (x.shape[0],)
-    X, U, tok, lp = x.float().cpu().numpy(), u.cpu().numpy(), tok.cpu().numpy(), lp.cpu().numpy()
+    X, U, tok, lp = x.float().cpu().numpy(), u.cpu().numpy(), tok.cpu().numpy(), lp.double().cpu().numpy()
     V, compared = X.shape[1], 0
 
     def entry(v, b):
@@ -308,3 +308,63 @@ def test_recorded_and_on_other_streams(gpu):
             assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1]), (i, s)
             check(x, u, got=got, sure=False, **s)
         assert torch.equal(there[0], want[0][0])
+
+
+@pytest.mark.parametrize("B,V,dtype", [(5, 50021, "bf16"), (21, 20011, "fp32"), (48, 40000, "fp16"), (70, 34000, "bf16"),
+                                       (66, 20000, "fp32"), (161, 33000, "fp16")])
+def test_settings_of_long_rows(gpu, B, V, dtype):
+    """Rows of one call that end in different ways: greedy ones, lists short and
+    long and too long, nuclei, whole rows."""
+    g = torch.Generator().manual_seed(B)
+
+    def choice(vals, dtype):
+        return torch.tensor(vals, dtype=dtype)[torch.randint(0, len(vals), (B,), generator=g)].cuda()
+
+    x, u = logits(B, V, dtype, 40), uniform(B, 41)
+    x[1, 50:] = -math.inf
+    x[2] = math.nan
+    k = [0, 0, 0, 1, 7, 120, 1000, 1536, 1537, 5000, V - 1, V]
+    s = dict(temperature=choice([0.0, 0.3, 0.8, 1.0, 1.5], torch.float32), top_k=choice(k, torch.int32),
+             top_p=choice([0.0, 0.5, 0.9, 1.0, 1.0], torch.float32), min_p=choice([0.0, 0.0, 0.05, 1.0, 3.0], torch.float32))
+    compared = check(x, u, sure=False, **s)
+    assert compared >= 0.9 * B
+    # a top_k for all beside temperatures of the rows (greedy ones among them)
+    for top_k in (40, 127, 128, 129, 1536, 1537, V):
+        check(x, u, sure=False, temperature=s["temperature"], top_k=top_k, top_p=0.9)
+    check(x, u, sure=False, temperature=s["temperature"])
+    check(x, u, sure=False, temperature=0.0, top_k=5)
+
+
+@pytest.mark.parametrize("B,V", [(9, 50021), (72, 12000), (162, 40000)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+def test_long_rows_that_a_mask_leaves_little_of(gpu, dtype, B, V):
+    inf, nan = math.inf, math.nan
+    low = torch.finfo(DT[dtype]).min
+    x, u = logits(B, V, dtype, 43), uniform(B, 44)
+    x[0] = -inf
+    x[1] = nan
+    x[2] = -inf
+    x[2, V - 3] = -5.0
+    x[3, :V - 1] = low
+    x[4] = low
+    x[5, 7] = inf
+    x[5, V - 100] = inf
+    x[6, ::2] = nan
+    x[7, 1:] = -inf
+    x[7, 0] = low
+    x[8] = inf
+    for s in SETTINGS + [dict(top_p=0.3, temperature=20.0), dict(top_p=0.7, min_p=0.01)]:
+        check(x, u, sure=False, **s)
+
+
+@pytest.mark.parametrize("offset", [0.0, -300.0, 1000.0])
+def test_nuclei_of_shifted_and_narrow_rows(gpu, offset):
+    """Logits far from zero, or within a few steps of their type: the border's
+    bin holds few values, or one, or the first."""
+    for dtype, V, B in (("fp32", 30011, 6), ("bf16", 30011, 6), ("fp16", 34001, 80), ("fp32", 20000, 64)):
+        for sigma in (1e-3, 0.05, 6.0):
+            x = (logits(B, V, dtype, 50, sigma=sigma).float() + offset).to(DT[dtype])
+            u = uniform(B, 51)
+            for s in (dict(top_p=0.3), dict(top_p=0.97, temperature=0.6), dict(top_p=2.0 ** -30), dict(top_p=1 - 2.0 ** -24),
+                      dict(top_p=0.9, min_p=0.2)):
+                check(x, u, sure=False, **s)
