@@ -579,7 +579,7 @@ __device__ __forceinline__ uint32_t narrow(F&& each, uint64_t& lo, uint64_t& hi,
   __syncthreads();
   s[tid] = 0;
   ((uint32_t*)(s + 2 * N))[tid] = 0;
-  if (tid < 2) s_scan[32 + 4 * tid] = 0;
+  if (tid < 3) s_scan[32 + 4 * tid] = 0;    // (the third: reach's count)
   __syncthreads();
   for (int pass = 0; ; ++pass) {
     // the two passes' places take turns: what one leaves is cleared by the next
@@ -619,20 +619,30 @@ __device__ __forceinline__ uint32_t narrow(F&& each, uint64_t& lo, uint64_t& hi,
 }
 
 // The largest of n values from [lo, hi] at which the measure, summed from the largest
-// down, reaches `goal`; 0 if none does.
+// down, reaches `goal`; 0 if none does. Each wave ends by itself what a lane a value is
+// left of.
 template <int N, typename V, typename M>
 __device__ __forceinline__ uint64_t reach(int n, V&& value, M&& measure, uint64_t lo, uint64_t hi, uint64_t goal, uint64_t* s) {
   const uint32_t left = narrow<N>([&](auto&& f) __attribute__((always_inline)) {
     for (int i = threadIdx.x; i < n; i += N) f(value(i), measure(i));
-  }, lo, hi, goal, 1, s);
+  }, lo, hi, goal, 64, s);
   if (left == 0 || lo == hi) return left ? lo : 0;
-  uint64_t* only = s + 3 * N + 40;
+  uint32_t* count = (uint32_t*)(s + 3 * N + 40);
   for (int i = threadIdx.x; i < n; i += N) {
     const uint64_t x = value(i);
-    if (x >= lo && x <= hi) *only = x;
+    if (x >= lo && x <= hi) {
+      const uint32_t at = atomicAdd(count, 1u);
+      s[at] = x;                              // (the first histogram's place: 64 of them and their measures)
+      s[64 + at] = measure(i);
+    }
   }
   __syncthreads();
-  return *only;
+  const uint32_t lane = threadIdx.x % 64;
+  const uint64_t mine = lane < left ? s[lane] : 0, weight = lane < left ? s[64 + lane] : 0;
+  uint64_t before = 0;
+  for (uint32_t j = 0; j < left; ++j) before += s[j] > mine ? s[64 + j] : 0;
+  const uint64_t at = __ballot(lane < left && before < goal && before + weight >= goal);
+  return at ? s[__ffsll((long long)at) - 1] : 0;
 }
 
 // A row's first place and smallest candidate's key, from its parts'.
