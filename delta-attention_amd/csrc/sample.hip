@@ -274,10 +274,12 @@ struct Sweep {
   int first, n;
   u32x4 w[U];
   __device__ __forceinline__ Sweep(const R& r, int tile0, int tiles) : row(r) {
-    first = tile0 + (int)(threadIdx.x / 64);
-    n = min(tiles - (int)(threadIdx.x / 64), (r.n_vec + 63) / 64 - first);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    first = tile0 + wave;
+    n = min(tiles - wave, (r.n_vec + 63) / 64 - first);
 #pragma unroll
-    for (int u = 0; u < U; ++u) w[u] = row.load(vector(u * W));
+    for (int u = 0; u < U; ++u)
+      if (u * W < n) w[u] = row.load(vector(u * W));
   }
   __device__ __forceinline__ int vector(int j) const { return (first + j) * 64 + (int)(threadIdx.x % 64); }
   template <typename F>
@@ -287,7 +289,7 @@ struct Sweep {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         now[u] = w[u];
-        w[u] = row.load(vector(j + (U + u) * W));
+        if (j + (U + u) * W < n) w[u] = row.load(vector(j + (U + u) * W));
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
