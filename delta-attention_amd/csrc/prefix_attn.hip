@@ -9,6 +9,13 @@
 // product over the rows of all sequences that share it (n s G rows for n
 // sequences of s rows and G query heads a kv head), read once, and each
 // sequence's own keys are another over its s G rows.
+//
+// What bounds it: up to some 128 rows a kv head the keys' bytes (16 sequences of 32 / 8
+// heads of 128 over 131072 keys 108 us in all, 5.4 TB/s; one sequence alone takes 90), past
+// that the matrix products and the exponentials beside them (128 sequences over 65536 keys
+// 185 us, 740 TFLOP/s; 16 of 128 rows each over 32768 keys 1050), and for short keys two
+// launches (10.5 us for 2711 keys). The rows of a batch over whole caches, each with a copy of the prefix,
+// take 50 us where 16 share 4096 keys in 15, and 324 where 4 share 131072 in 92.
 #include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -27,6 +34,7 @@ constexpr int MAX_KEYS = 1 << 30;
 constexpr float NO_KEYS = -FLT_MAX;          // the reference of a row that has seen no score yet
 // A row's reference may lag its largest score by LAG (log2); fp16 probabilities
 // are held times 2^BIAS, so that they are at most 2^14 and end 2^-32 below it.
+// (With LAG 0 128 sequences over 65536 keys take 193 us for 187.)
 constexpr float LAG = 6.f;
 template <typename T> constexpr float BIAS = std::is_same_v<T, _Float16> ? 8.f : 0.f;
 
@@ -49,6 +57,10 @@ struct PrefixArgs {
   float *part, *part_m, *part_l;            // [Hkv, splits, rows, D], [Hkv, splits, rows] twice
 };
 
+// Loads that are not kept in the caches: where no other row tile reads a split's keys (one
+// row tile a split: 16 sequences over 131072 keys 124 -> 108 us, 3 x 5 over 20011 66 -> 57).
+// Where tiles share them they cost the sharing: 128 sequences over 65536 keys 193 -> 216 us.
+// The sequences' own keys come by ordinary loads (by these 57 -> 59 us).
 __device__ __forceinline__ void dma16_nt(u32x4 r, uint32_t lds, uint32_t voff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen nt lds"
                :: "s"(lds), "v"(voff), "s"(r) : "memory");
@@ -106,7 +118,9 @@ __host__ __device__ constexpr int waves_of(int D, int mt) { return D == 256 ? 1 
 // all waves load into LDS together, the next one while this one is computed.
 // S^T = K Q^T leaves a lane (row c = lane % 16, group g = lane / 16) the keys 16 t
 // + 4 g + r of its row, which is the right operand of O^T = V^T P^T as it stands;
-// V^T comes from transposed LDS reads of the same keys.
+// V^T comes from transposed LDS reads of the same keys. Probabilities are rounded to the
+// inputs' type for that product, half a step of which is within the result's own, and
+// summed as rounded, so that a row's weights add up to one.
 template <typename T, int D, int MT, bool OWN, bool STREAM>
 __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&smem)[2][2][Tile<D>::BYTES]) {
   using E = Elt<T>;
@@ -380,7 +394,9 @@ __global__ __launch_bounds__(64 * WAVES, waves_of(D, MT)) void prefix_rows_kerne
 
 // Joins a row's splits: groups of D / 4 threads, `side` (a power of two) of them a
 // row, take splits side by side, four loads of each in flight, and are joined
-// through LDS.
+// through LDS. One group a row, as first built, walked the splits one after another:
+// 148 us in place of 119 for 16 sequences over 131072 keys, 76 for 48 at 40009 of 256. It
+// takes 4 to 10 us now: its launch, and the partial sums' way through memory.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int side) {
   using E = Elt<T>;
@@ -460,6 +476,10 @@ bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, i
   if (own > MOST || (int64_t)B * Hkv > MOST || own * B > MOST) return false;
   p.rows = own * B;
   const int64_t p_rows = p.rows / P;
+  // 16 rows a wave, 32 where a prefix has more than a workgroup of those: the keys are
+  // read from LDS once for both. By 16 / 32: 4 rows over 2711 keys 10.4 / 11.0 us, 16 over
+  // 40009 at head_dim 256 37.8 / 55.7; 512 rows over 65536 keys 208 / 187, 1536 over 30011
+  // at head_dim 64 146 / 125. (64 rows, as far as registers allow, 220 and 260.)
   p.mt = p_rows <= 64 ? 1 : 2;
   const int bm = 16 * p.mt * WAVES;
   const int64_t p_rt = Np > 0 ? (p_rows + bm - 1) / bm : 0, o_rt = cap > 0 ? (own + 16 * WAVES - 1) / (16 * WAVES) : 0;
@@ -470,7 +490,10 @@ bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, i
   // Tiles of an item: the count whose items end first, on a model of a launch. An
   // item takes its tiles and START more; the prefixes' items start first, the
   // sequences' own in the places beside or behind them; a split costs its partial
-  // sums' way to memory and back.
+  // sums' way to memory and back. (Against one round of equal items: 3 prefixes of 5
+  // sequences with 3008 keys of their own each 82 -> 72 us, 512 at head_dim 256 42 -> 37.
+  // Spreading the own items among the prefixes' in launch order: 128 sequences over 65536
+  // keys 186 -> 211 us, 16 over 131072 108 -> 116.)
   constexpr double START = 1.5;
   const int64_t least = (p_lists * p_tiles + o_lists * o_tiles + slots - 1) / slots;
   double best = 0;

@@ -18,9 +18,9 @@
 // Integer sums have no order: a row's token does not depend on how the row is
 // split over workgroups, and the products u * total and p * total are exact.
 //
-// Long rows are split over workgroups ("parts") and take three or four launches:
+// Long rows are split over workgroups ("parts") and take two or three launches:
 //   top     each part's largest and smallest candidate, and the largest of each of
-//           its groups of lanes
+//           the row's groups of lanes
 //   gather  top_k: the k-th largest of a row's group maxima is no larger than its
 //           k-th logit, so the tokens from there on hold the first k and few more:
 //           they are gathered in a list. top_p: the weights' histogram over the
@@ -28,9 +28,18 @@
 //   sums    (rows without a list) the kept weight of every tile of 64 vectors;
 //           with top_p the tokens of the one bin at which the histogram reaches p
 //           are gathered in a list, those of larger logits are kept
-//   finish  a workgroup a row: the last token kept, by histograms over the list;
-//           the tile at which the sum passes u times the total, and the token in it
-// Short rows take the last launch alone, the whole row their list.
+// The part that is through last ends its row: the last token kept, from the list;
+// the tile at which the sum passes u times the total, and the token in it. Where
+// rows fill most CUs, or are short, one workgroup takes a row through the same
+// passes in one launch; rows up to a list's length are their own list.
+//
+// What bounds it. A few rows: the launches and each one's dependent steps (loads of
+// what the launch before left, a barrier or two, the last part's join): one row of
+// 32000 bfloat16 tokens 12.6 us in two launches, one of 128256 with top_p 20.6 in
+// three (4.1 + 5.8 + 11.2 traced). Many rows: a token's weight, 29 instructions of
+// the vector ALU (two thirds of them in 64 bits) for 2 bytes read; 192 rows of 100003
+// tokens with top_p weigh each token twice: 75 us, 0.5 TB/s. Rows with top_k alone
+// weigh no more than their lists: 256 rows of 128256 tokens 38 us, 1.7 TB/s.
 #include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -50,7 +59,7 @@ constexpr int MAX_V = 1 << 24;               // tokens of a vocabulary
 constexpr int MAX_B = 0x3fffff;              // rows (four parts each: threads of a grid below 2^32)
 constexpr uint32_t KEY_NONE = 0x007fffffu;   // -inf's key: candidates lie above it
 constexpr int PART = 512;                    // threads of a part
-constexpr int LIST = 3584;                   // tokens of a row's list (two finishing workgroups' LDS a CU)
+constexpr int LIST = 3584;                   // tokens of a row's list (LDS for two workgroups a CU)
 constexpr int BINS = 768;                    // of a part's histogram
 constexpr int GROUPS = 2048;                 // group maxima of a row
 constexpr int SLOTS = 1024;                  // tile sums in LDS
@@ -117,7 +126,10 @@ struct Order {
 // of [-1/2, 1/2] (2^-51 of it, rounding included; the series takes two terms more), the
 // whole one by the exponent. Whole numbers come from what 2^52 leaves of a sum: of the
 // exponent, with the unit's `bits` above it, and of the weight, which is rounded so.
-// (RAW is that 2^52 of the weight, for the sums to take off together.)
+// (RAW is that 2^52 of the weight, for the sums to take off together.) A tile's weights
+// are bound by these instructions: with the exponent and the units put in apart, and the
+// weight's 2^52 taken off one by one, 33 for 29 (192 rows of temperature alone 48 us for
+// 46). By count, tables of powers in LDS would save less than their gathers cost.
 constexpr double WHOLE_OF = 6755399441055744.0;   // 1.5 * 2^52
 constexpr uint64_t RAW = 0x4330000000000000ull;
 __device__ __forceinline__ uint64_t raw_weight(double d, double per, double whole_of) {
@@ -191,8 +203,9 @@ struct Scale {
   __device__ __forceinline__ float bin(float z) const {   // its whole part is the bin; BINS: no weight
     return fminf((topf - z) * step, (float)BINS);
   }
-  // The smallest logit of the bins before `end` (1 to BINS - 1), found by a wave: each
-  // lane tries one of 64 keys of what is left.
+  // The smallest logit of the bins before `end` (1 to BINS), found by a wave: each lane
+  // tries one of 64 keys of what is left. (Borders as logits cost the sums one comparison
+  // a token, bins four instructions.)
   __device__ __forceinline__ float low_end(int end) const {
     uint32_t lo = KEY_NONE + 1, hi = key_of(topf);   // (the bins are of falling logits, the top in the first)
     while (lo < hi) {
@@ -265,7 +278,8 @@ struct Row {
 };
 
 // This lane's vectors of `tiles` tiles from tile0 on, wave w of W every W-th tile, U
-// loads ahead: those of the first vectors are made here.
+// loads ahead: those of the first vectors are made here. None is made past the wave's
+// own tiles (64 mixed rows of 151936 tokens 52 -> 47 us).
 template <typename T, int W, int U>
 struct Sweep {
   using R = Row<T>;
@@ -417,10 +431,11 @@ __device__ __forceinline__ void ends_of(const Row<T>& row, const Order<T>& ord, 
   low = least < INFINITY ? ~key_of(least) : key > KEY_NONE ? ~key : 0u;
 }
 
-// A number that no more than k of the groups' maxima's first 16 bits pass: the
+// A number that fewer than k of the groups' maxima's first 16 bits pass: the
 // largest one of 16 bits that is no larger than the k-th largest maximum, bit by bit,
-// by the count of maxima that reach it. Each wave works for itself on all maxima, M a
-// lane; up to 384 the groups of a lane are taken as eight.
+// by the count of maxima that reach it. One wave works on all maxima, M a lane (in each
+// wave of the workgroup it took 3 us more); up to 384 the groups of a lane are taken as
+// eight: a quarter of the counting for a list that is hardly longer.
 template <int M>
 __device__ __forceinline__ float list_bar(uint32_t (&key)[M], int k) {
   uint32_t low = 0;
@@ -461,7 +476,8 @@ __device__ __forceinline__ void gather_into(S& sweep, const O& ord, float bar, u
   });
 }
 
-// The weights' histogram.
+// The weights' histogram. (Its additions in LDS take a fifth of a flat row's time, 18 of
+// 96 us for 192 rows; in 32 bits, or with the waves' priorities apart, they take as long.)
 template <typename S>
 __device__ __forceinline__ void hist_into(S& sweep, const Scale& sc, uint64_t* hist) {
   constexpr int E = S::R::E;
@@ -661,7 +677,9 @@ __device__ __forceinline__ void row_ends(const SampleArgs& a, int b, uint64_t& f
 }
 
 // A short list's n <= FEW values by pairs, N / FEW threads a value: how many are larger
-// than this thread's, and their weight.
+// than this thread's, and their weight. One pass and no barrier for each border, where
+// histograms take one or two with three barriers each: 8 rows with top_k 50 19.4 -> 16.0
+// us. (Up to 256 values it is slower: top_k 150 17 -> 23 us.)
 constexpr int FEW = 128;
 template <int N, typename V>
 __device__ __forceinline__ void above(int n, V&& value, const uint64_t* w, uint64_t mine, uint32_t& many, uint64_t& weight) {
@@ -1083,7 +1101,8 @@ __device__ __forceinline__ void append(const SampleArgs& a, int b, Room<PARTS>& 
 // Whether all of a row's parts are through, for the last of them. What they tell it is
 // put() and got(), at the device's scope: each wave waits until its words are out before
 // its part counts as through, and what the last one reads comes after. Nobody waits for
-// another part.
+// another part. (One launch less: 1 us of a single row. With fences in place of the words'
+// scope, which write back and drop a whole L2 in each workgroup, 8 rows take twice as long.)
 __device__ __forceinline__ bool last_part(const SampleArgs& a, int b, Room<PARTS>& m) {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
@@ -1191,11 +1210,14 @@ struct Plan {
   size_t part, maxima, count, ended, hist, list, tile, bytes;   // offsets
 };
 
-// A workgroup takes a whole row where there are rows for most CUs, or short ones. 128256
-// bfloat16 tokens, by workgroups / parts: 128 rows 46 / 37 us (temperature alone), 29 /
-// 29 (top_k 50), 96 / 74 (a flat nucleus); 256 rows 55 / 62, 37 / 43, 101 / 113. 16000
-// tokens: 64 rows 16 / 16, 25 / 23, 29 / 29; 256 rows 17 / 20, 24 / 26, 30 / 37. 5000
-// tokens, one row: 12.1 / 13.3, 19.0 / 18.7, 21.5 / 23.0.
+// A workgroup takes a whole row where there are rows for most CUs, or short ones. By
+// workgroups / parts, us, bfloat16:
+//                     temperature  top_k 50  top_p 0.9  a flat nucleus
+//   128256 x 128         42 / 32    21 / 23    74 / 50      88 / 63
+//   128256 x 192         45 / 49    24 / 43    78 / 72      90 / 98
+//   32000 x 96           18 / 17    15 / 20    31 / 31      36 / 34
+//   16000 x 16           14 / 12    14 / 16    22 / 22      23 / 23
+//   8192 x 1             11 / 12    13 / 15    18 / 21      19 / 21
 bool by_rows(int B, int V) { return B >= 160 || V <= 8192 || (B >= 64 && V <= 32768); }
 
 void plan_for(Plan& p, int B, int V, int dtype, bool differ) {
@@ -1205,8 +1227,8 @@ void plan_for(Plan& p, int B, int V, int dtype, bool differ) {
   const int64_t tiles = ((int64_t)V + 2 * E - 1) / E / 64 + 1;   // whatever the row's alignment
   // parts: 4 at least; then a workgroup a CU, of 8 tiles (one of each wave) at least.
   // Rows that ask for different things differ in work: two a CU spread it. 64 such rows of
-  // 151936 bfloat16 tokens, 8 / 4 parts: 52 / 56 us, 48 rows 45 / 55; of rows that are alike
-  // 64 with top_k 50 take 22.9 / 19.3, 32 of them 22.9 (16 parts) / 17.7 (8).
+  // 151936 bfloat16 tokens, 8 / 4 parts: 47 / 56 us, 48 rows 44 / 54; of rows that are alike
+  // 64 with top_k 50 take 21.2 / 18.9, 32 of them 20.5 (16 parts) / 17.3 (8).
   int64_t parts = 4;
   while (parts < 32 && tiles >= parts * 2 * 8 && parts * 2 * B <= (differ && parts < 16 ? 512 : 256)) parts *= 2;
   p.tiles = (int)(((tiles + parts - 1) / parts + 7) / 8 * 8);
