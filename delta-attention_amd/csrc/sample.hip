@@ -36,7 +36,7 @@
 // What bounds it. A few rows: the launches and each one's dependent steps (loads of
 // what the launch before left, a barrier or two, the last part's join): one row of
 // 32000 bfloat16 tokens 12.6 us in two launches, one of 128256 with top_p 20.6 in
-// three (4.1 + 5.8 + 11.2 traced). Many rows: a token's weight, 29 instructions of
+// three (4.5 + 5.9 + 11.3 traced). Many rows: a token's weight, 29 instructions of
 // the vector ALU (two thirds of them in 64 bits) for 2 bytes read; 192 rows of 100003
 // tokens with top_p weigh each token twice: 75 us, 0.5 TB/s. Rows with top_k alone
 // weigh no more than their lists: 256 rows of 128256 tokens 38 us, 1.7 TB/s.

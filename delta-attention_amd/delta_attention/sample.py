@@ -14,8 +14,8 @@ the model's sampling loop. Here:
   is refused) straight onto the device, in bf16;
 - the attention names are checked rather than registered: prefill runs
   "window" (the delta path), decode steps "sdpa_rectangle";
-- `LlamaForCausalLM.generate` is the greedy sampling loop itself, so no
-  method is patched in;
+- `LlamaForCausalLM.generate` is the loop itself, greedy or drawing tokens by
+  given random numbers, so no method is patched in;
 - a LoRA adapter directory (`config.checkpoint`, PEFT's file layout) is
   merged as W += (alpha / r) * B @ A (alpha / sqrt(r) with rsLoRA).
 """
