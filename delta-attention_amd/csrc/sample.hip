@@ -174,7 +174,7 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int b) {
 // the logit, from the largest to where weights vanish or the smallest candidate.
 struct Scale {
   double top, per, none, whole_of;          // none: a distance from the top of no weight
-  float topf, step, bar;                    // bar: min_p's, the smallest float at or above it
+  float topf, half, step, bar;              // half of the top; bins a half; bar: min_p's, the smallest float at or above it
   bool inf;                                 // an infinite largest logit: the tokens at it share the row
   __device__ __forceinline__ Scale(const SampleArgs& a, const Setting& s, float most, uint32_t least) {
     topf = most;
@@ -194,15 +194,16 @@ struct Scale {
     top = topf;
     const double far = a.bits + 2, all = (top - (inf ? 0.0 : (double)of_key(least))) * per;
     const double range = all < far ? all : far;
-    step = range > 0.0 ? (float)(BINS * (1.0 - 1.0 / 1024) / range * per) : 0.f;
+    half = 0.5f * topf;
+    step = range > 0.0 ? (float)fmin(2 * BINS * (1.0 - 1.0 / 1024) / range * per, (double)FLT_MAX) : 0.f;
   }
   // logits as the rest takes them, and the bar
   __device__ __forceinline__ float at(float y) const { return !inf ? y : y == INFINITY ? 0.f : -INFINITY; }
   __device__ __forceinline__ uint64_t raw(float z) const { return raw_weight(fmax((double)z - top, none), per, whole_of); }
   __device__ __forceinline__ uint64_t weight(float z) const { return raw(z) - RAW; }
-  __device__ __forceinline__ float bin(float z) const {   // its whole part is the bin; BINS: no weight
-    return fminf((topf - z) * step, (float)BINS);
-  }
+  // Its whole part is the bin; BINS: no weight. (Half the distance: the type's largest and
+  // lowest numbers are further apart than a float.)
+  __device__ __forceinline__ float bin(float z) const { return fminf(fmaf(z, -0.5f, half) * step, (float)BINS); }
   // The smallest logit of the bins before `end` (1 to BINS), found by a wave: each lane
   // tries one of 64 keys of what is left. (Borders as logits cost the sums one comparison
   // a token, bins four instructions.)

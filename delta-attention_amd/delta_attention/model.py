@@ -529,7 +529,7 @@ class LlamaForCausalLM(nn.Module):
         samples (KVCacheShared; the 8-bit cache's codes are copied instead).
         logprobs_out: receives each step's log-probabilities [b * samples]."""
         rows = input_ids.shape[0] * samples
-        assert samples >= 1, samples
+        assert samples >= 1 and max_new_tokens >= 1, (samples, max_new_tokens)
         assert u.dim() == 2 and u.shape[0] == rows and u.shape[1] >= max_new_tokens and u.dtype == torch.float32, (
             f"u: float32 [{rows}, {max_new_tokens}] is needed, got {u.dtype} {tuple(u.shape)}")
         if samples > 1 and getattr(self.config, "decode_mode", "dense") != "dense":

@@ -368,3 +368,19 @@ def test_nuclei_of_shifted_and_narrow_rows(gpu, offset):
             for s in (dict(top_p=0.3), dict(top_p=0.97, temperature=0.6), dict(top_p=2.0 ** -30), dict(top_p=1 - 2.0 ** -24),
                       dict(top_p=0.9, min_p=0.2)):
                 check(x, u, sure=False, **s)
+
+
+@pytest.mark.parametrize("B,V", [(5, 20000), (64, 20000), (3, 3000)])
+def test_the_ends_of_float32(gpu, B, V):
+    """Logits and temperatures near the type's largest and smallest numbers: a
+    nucleus's histogram spans more than a float, or less than its smallest step."""
+    x, u = logits(B, V, "fp32", 60, sigma=1.0), uniform(B, 61)
+    x = x / x.abs().amax(1, keepdim=True)
+    for scale, T in ((3.4e38, 1e38), (3.4e38, 3.4e38), (3.4e38, 1e36), (1e-38, 3e-39), (1e-41, 1e-41), (1.0, 1e-45), (1e-30, 1e30)):
+        y = (x.double() * scale).float()
+        for s in (dict(), dict(top_p=0.6), dict(top_k=300, top_p=0.9), dict(top_p=0.9, min_p=0.3)):
+            check(y, u, sure=False, temperature=torch.tensor([T]).cuda(), **s)
+        # masked by the type's lowest value
+        y[:, ::3] = torch.finfo(torch.float32).min
+        for s in (dict(top_p=0.6), dict(top_k=300, top_p=0.9)):
+            check(y, u, sure=False, temperature=torch.tensor([T]).cuda(), **s)

@@ -102,3 +102,10 @@ def test_c_refusals(lib):
     if need:
         assert call(V=100000, rs=100000, ws=16, nb=need - 1) == call(V=100000, rs=100000, nb=need) == L.DA_ERR_WORKSPACE
         assert call(V=100000, rs=100000, ws=24, nb=need) == L.DA_ERR_ALIGNMENT
+
+
+def test_a_generation_of_no_tokens_is_refused():
+    import torch
+    from delta_attention.model import LlamaForCausalLM
+    with pytest.raises(AssertionError):
+        LlamaForCausalLM.generate_sampled(None, torch.zeros(1, 4, dtype=torch.int64), 0, torch.zeros(1, 0))
