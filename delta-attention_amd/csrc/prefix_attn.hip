@@ -13,8 +13,8 @@
 // What bounds it: up to some 128 rows a kv head the keys' bytes (16 sequences of 32 / 8
 // heads of 128 over 131072 keys 108 us in all, 5.4 TB/s; one sequence alone takes 90), past
 // that the matrix products and the exponentials beside them (128 sequences over 65536 keys
-// 185 us, 740 TFLOP/s; 16 of 128 rows each over 32768 keys 1050), and for short keys two
-// launches (10.5 us for 2711 keys). The rows of a batch over whole caches, each with a copy of the prefix,
+// 185 us, 740 TFLOP/s; 16 of 128 rows each over 32768 keys 1050), and for few keys two
+// launches (10.5 us for 2711) or one (5.7 to 7.2 us up to 256). The rows of a batch over whole caches, each with a copy of the prefix,
 // take 50 us where 16 share 4096 keys in 15, and 324 where 4 share 131072 in 92.
 #include <float.h>
 #include <hip/hip_runtime.h>
@@ -114,66 +114,86 @@ __device__ __forceinline__ int own_keys(const PrefixArgs& a, int b) {
 // Waves of a SIMD: what the accumulators and two tiles of scores leave room for.
 __host__ __device__ constexpr int waves_of(int D, int mt) { return D == 256 ? 1 : D == 128 ? 2 : D * mt == 128 ? 3 : 4; }
 
-// One item: a row tile of 16 MT rows a wave against a split's key tiles, which
-// all waves load into LDS together, the next one while this one is computed.
+// A wave's 16 MT rows (row c = lane % 16 of each): their queries and what they have
+// gathered. ref: scaled, in log2.
+template <typename T, int D, int MT>
+struct Rows {
+  u32x4 q[MT][D / 32];
+  f32x4 acc[MT][D / 16];
+  float ref[MT], sum[MT];
+  int own[MT];                               // the row's place among its sequence's s rows
+  // the rows from row0 on of kv head hk, n_rows of the workgroup
+  __device__ __forceinline__ Rows(const PrefixArgs& a, int hk, int row0, int n_rows) {
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), c = lane % 16, g = lane / 16;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int r = row0 + min(wave * 16 * MT + mt * 16 + c, n_rows - 1);   // (past the last: it again)
+      const int x = fdiv(r, a.heads), b = fdiv(x, a.rows_s), i = x - b * a.s;
+      own[mt] = i;
+      const T* src = (const T*)a.q + b * a.q_b + (int64_t)(hk * a.G + r - x * a.G) * a.q_h + i * a.q_s;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) q[mt][k] = *(const u32x4*)(src + 32 * k + 8 * g) ^ a.flip;
+      ref[mt] = NO_KEYS;
+      sum[mt] = 0.f;
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) acc[mt][t] = (f32x4){0, 0, 0, 0};
+    }
+  }
+};
+
+// A head's keys and values, and the bytes from key to key.
+struct Keys {
+  const char *k, *v;
+  uint32_t k_s, v_s;
+  int n;
+};
+template <bool OWN>
+__device__ __forceinline__ Keys keys_of(const PrefixArgs& a, int list, int hk) {
+  Keys x;
+  x.k = (const char*)(OWN ? a.k : a.kp) + 2 * (OWN ? list * a.k_b + hk * a.k_h : list * a.kp_b + hk * a.kp_h);
+  x.v = (const char*)(OWN ? a.v : a.vp) + 2 * (OWN ? list * a.v_b + hk * a.v_h : list * a.vp_b + hk * a.vp_h);
+  x.k_s = OWN ? a.k_s : a.kp_s;
+  x.v_s = OWN ? a.v_s : a.vp_s;
+  x.n = __builtin_amdgcn_readfirstlane(OWN ? own_keys(a, list) : prefix_keys(a, list));
+  return x;
+}
+
+// The rows against the keys of [key0, stop), in tiles that all waves load into LDS
+// together, the next one while this one is computed. row0, n_rows: the workgroup's.
 // S^T = K Q^T leaves a lane (row c = lane % 16, group g = lane / 16) the keys 16 t
 // + 4 g + r of its row, which is the right operand of O^T = V^T P^T as it stands;
 // V^T comes from transposed LDS reads of the same keys. Probabilities are rounded to the
 // inputs' type for that product, half a step of which is within the result's own, and
 // summed as rounded, so that a row's weights add up to one.
+// -> the number of tiles
 template <typename T, int D, int MT, bool OWN, bool STREAM>
-__device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&smem)[2][2][Tile<D>::BYTES]) {
+__device__ __forceinline__ int walk(const PrefixArgs& a, Rows<T, D, MT>& rows, const Keys& keys, int key0, int stop, int row0,
+                                    int n_rows, bool active, char (&smem)[2][2][Tile<D>::BYTES]) {
   using E = Elt<T>;
   using M = Mma<T>;
   using TL = Tile<D>;
-  constexpr int KS = D / 32, DT = D / 16, KG = BN / 16, BM = 16 * MT * WAVES;
+  constexpr int KS = D / 32, DT = D / 16, KG = BN / 16;
   const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
   const int c = lane % 16, g = lane / 16;
+  const char *kb = keys.k, *vb = keys.v;
+  const uint32_t k_s = keys.k_s, v_s = keys.v_s;
+  const int n_keys = keys.n;
+  auto &acc = rows.acc;
+  auto &ref = rows.ref, &sum = rows.sum;
+  auto &qf = rows.q;
 
-  // the item: (prefix or sequence, kv head, split, row tile), the row tiles of a
-  // split beside each other
-  const int x0 = fdiv(item, OWN ? a.f_ort : a.f_prt), tile = item - x0 * (OWN ? a.o_rt : a.p_rt);
-  const int y0 = fdiv(x0, OWN ? a.f_osp : a.f_psp), part = x0 - y0 * (OWN ? a.o_splits : a.p_splits);
-  const int list = fdiv(y0, a.f_hkv), hk = y0 - list * a.Hkv;        // list: the prefix or the sequence
-  const int n_rows = min(BM, (OWN ? a.o_rows : a.p_rows) - tile * BM);
-  const int row0 = list * (OWN ? a.o_rows : a.p_rows) + tile * BM;    // of the kv head's rows
-  const int n_keys = __builtin_amdgcn_readfirstlane(OWN ? own_keys(a, list) : prefix_keys(a, list));
-  const int chunk = OWN ? a.o_chunk : a.p_chunk, split = OWN ? part + a.p_splits : part, key0 = part * chunk * BN;
-  const char* kb = (const char*)(OWN ? a.k : a.kp) + 2 * (OWN ? list * a.k_b + hk * a.k_h : list * a.kp_b + hk * a.kp_h);
-  const char* vb = (const char*)(OWN ? a.v : a.vp) + 2 * (OWN ? list * a.v_b + hk * a.v_h : list * a.vp_b + hk * a.vp_h);
-  const uint32_t k_s = OWN ? a.k_s : a.kp_s, v_s = OWN ? a.v_s : a.vp_s;
-
-  // this wave's rows: places in the kv head's rows, and each one's last key
+  // each row's last key
   const int lim0 = OWN ? n_keys - a.s : n_keys - 1;
-  const bool active = wave * 16 * MT < n_rows;
   int lim[MT], lim_lo = lim0, lim_hi = lim0;
-  u32x4 qf[MT][KS];
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    const int r = row0 + min(wave * 16 * MT + mt * 16 + c, n_rows - 1);   // (past the last: it again)
-    const int x = fdiv(r, a.heads), b = fdiv(x, a.rows_s), i = x - b * a.s;
-    lim[mt] = OWN ? lim0 + i : lim0;
-    const T* src = (const T*)a.q + b * a.q_b + (int64_t)(hk * a.G + r - x * a.G) * a.q_h + i * a.q_s;
-#pragma unroll
-    for (int k = 0; k < KS; ++k) qf[mt][k] = *(const u32x4*)(src + 32 * k + 8 * g) ^ a.flip;
-  }
+  for (int mt = 0; mt < MT; ++mt) lim[mt] = OWN ? lim0 + rows.own[mt] : lim0;
   if (OWN) {                                 // of the whole row tile
     const int u = fdiv(row0, a.heads), w = fdiv(row0 + n_rows - 1, a.heads);
     lim_lo += u - (int)fdiv(u, a.rows_s) * a.s;
     lim_hi += w - (int)fdiv(w, a.rows_s) * a.s;
   }
-  const int end = min(min(key0 + chunk * BN, n_keys), lim_hi + 1);
+  const int end = min(min(stop, n_keys), lim_hi + 1);
   const int nt = end > key0 ? (end - key0 + BN - 1) / BN : 0;
-
-  f32x4 acc[MT][DT];
-  float ref[MT], sum[MT];                    // ref: scaled, in log2
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
-    ref[mt] = NO_KEYS;
-    sum[mt] = 0.f;
-#pragma unroll
-    for (int t = 0; t < DT; ++t) acc[mt][t] = (f32x4){0, 0, 0, 0};
-  }
 
   // loads: lane i of load j of a wave fills chunk i of the wave's 1024 bytes
   uint32_t koff[TL::DMAS], voff[TL::DMAS];
@@ -357,21 +377,58 @@ __device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&
 #pragma unroll
       for (int i = 0; i < KG; ++i) s[mt][i] = next[mt][i];
   }
+  return nt;
+}
+
+// Writes a kv head's row, four columns from `col` on for each f(col, sums) that `each`
+// calls. A row without keys is zero; one whose every score is -inf has no softmax: NaN.
+template <typename T, int D, typename F>
+__device__ __forceinline__ void put_row(const PrefixArgs& a, int hk, int row, float l, F&& each) {
+  using E = Elt<T>;
+  const int y = fdiv(row, a.heads), b = fdiv(y, a.rows_s), i = y - b * a.s;
+  const bool none = prefix_keys(a, fdiv(b, a.f_per)) == 0 && own_keys(a, b) - a.s + i < 0;
+  const float inv = none ? 0.f : 1.f / l;
+  T* dst = (T*)a.o + b * a.o_b + (int64_t)(hk * a.G + row - y * a.G) * a.o_h + i * a.o_s;
+  each([&](int col, const f32x4& o) __attribute__((always_inline)) {
+    *(u32x2*)(dst + col) = (u32x2){E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
+  });
+}
+
+// One item: a row tile of 16 MT rows a wave against a split's keys.
+template <typename T, int D, int MT, bool OWN, bool STREAM>
+__device__ __forceinline__ void rows_item(const PrefixArgs& a, int item, char (&smem)[2][2][Tile<D>::BYTES]) {
+  constexpr int BM = 16 * MT * WAVES;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int c = lane % 16, g = lane / 16;
+
+  // the item: (prefix or sequence, kv head, split, row tile), the row tiles of a
+  // split beside each other
+  const int x0 = fdiv(item, OWN ? a.f_ort : a.f_prt), tile = item - x0 * (OWN ? a.o_rt : a.p_rt);
+  const int y0 = fdiv(x0, OWN ? a.f_osp : a.f_psp), part = x0 - y0 * (OWN ? a.o_splits : a.p_splits);
+  const int list = fdiv(y0, a.f_hkv), hk = y0 - list * a.Hkv;        // list: the prefix or the sequence
+  const int n_rows = min(BM, (OWN ? a.o_rows : a.p_rows) - tile * BM);
+  const int row0 = list * (OWN ? a.o_rows : a.p_rows) + tile * BM;    // of the kv head's rows
+  const int chunk = OWN ? a.o_chunk : a.p_chunk, split = OWN ? part + a.p_splits : part, key0 = part * chunk * BN;
+  const bool active = wave * 16 * MT < n_rows;
+  const Keys keys = keys_of<OWN>(a, list, hk);
+  Rows<T, D, MT> rows(a, hk, row0, n_rows);
+  const int nt = walk<T, D, MT, OWN, STREAM>(a, rows, keys, key0, key0 + chunk * BN, row0, n_rows, active, smem);
+
   if (!active) return;
   const int64_t slot = ((int64_t)hk * (a.p_splits + a.o_splits) + split) * a.rows;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
     const int r = wave * 16 * MT + mt * 16 + c;
-    const float l = group_sum(sum[mt]);
+    const float l = group_sum(rows.sum[mt]);
     if (r >= n_rows) continue;
     const int64_t at = slot + row0 + r;
     if (g == 0) {
-      a.part_m[at] = ref[mt];
+      a.part_m[at] = rows.ref[mt];
       a.part_l[at] = l;
     }
     if (nt == 0) continue;                   // (nothing reads the sums of a split without keys)
 #pragma unroll
-    for (int d = 0; d < DT; ++d) *(f32x4*)(a.part + at * D + 16 * d + 4 * g) = acc[mt][d];
+    for (int d = 0; d < D / 16; ++d) *(f32x4*)(a.part + at * D + 16 * d + 4 * g) = rows.acc[mt][d];
   }
 }
 
@@ -392,6 +449,32 @@ __global__ __launch_bounds__(64 * WAVES, waves_of(D, MT)) void prefix_rows_kerne
   }
 }
 
+// Short keys: a row tile of a sequence against its prefix and its own keys, and its
+// output, in one launch without partial sums.
+template <typename T, int D>
+__global__ __launch_bounds__(64 * WAVES, waves_of(D, 1)) void prefix_whole_kernel(PrefixArgs a) {
+  __shared__ __align__(1024) char smem[2][2][Tile<D>::BYTES];
+  constexpr int BM = 16 * WAVES;
+  const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const int c = lane % 16, g = lane / 16;
+  const int y0 = fdiv(blockIdx.x, a.f_ort), tile = blockIdx.x - y0 * a.o_rt;
+  const int b = fdiv(y0, a.f_hkv), hk = y0 - b * a.Hkv;
+  const int n_rows = min(BM, a.o_rows - tile * BM), row0 = b * a.o_rows + tile * BM;
+  const bool active = wave * 16 < n_rows;
+  const Keys prefix = keys_of<false>(a, fdiv(b, a.f_per), hk), own = keys_of<true>(a, b, hk);
+  Rows<T, D, 1> rows(a, hk, row0, n_rows);
+  walk<T, D, 1, false, false>(a, rows, prefix, 0, prefix.n, row0, n_rows, active, smem);
+  lds_barrier();                             // (the last tiles are read)
+  walk<T, D, 1, true, false>(a, rows, own, 0, own.n, row0, n_rows, active, smem);
+  const int r = wave * 16 + c;
+  const float l = group_sum(rows.sum[0]);
+  if (r >= n_rows) return;
+  put_row<T, D>(a, hk, row0 + r, l, [&](auto&& at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) at(16 * d + 4 * g, rows.acc[0][d]);
+  });
+}
+
 // Joins a row's splits: groups of D / 4 threads, `side` (a power of two) of them a
 // row, take splits side by side, four loads of each in flight, and are joined
 // through LDS. One group a row, as first built, walked the splits one after another:
@@ -399,7 +482,6 @@ __global__ __launch_bounds__(64 * WAVES, waves_of(D, MT)) void prefix_rows_kerne
 // takes 4 to 10 us now: its launch, and the partial sums' way through memory.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int side) {
-  using E = Elt<T>;
   constexpr int CT = D / 4, GROUPS = 256 / CT, U = 4;
   __shared__ f32x4 s_o[GROUPS][CT];
   __shared__ float s_m[GROUPS], s_l[GROUPS];
@@ -452,12 +534,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int side
     }
   }
   if (!live) return;
-  // a row without keys is zero; one whose every score is -inf has no softmax: NaN
-  const int y = fdiv(row, a.heads), b = fdiv(y, a.rows_s), i = y - b * a.s;
-  const bool none = prefix_keys(a, fdiv(b, a.f_per)) == 0 && own_keys(a, b) - a.s + i < 0;
-  const float inv = none ? 0.f : 1.f / l;
-  T* dst = (T*)a.o + b * a.o_b + (int64_t)(hk * a.G + row - y * a.G) * a.o_h + i * a.o_s;
-  *(u32x2*)(dst + 4 * t) = (u32x2){E::pack2(o[0] * inv, o[1] * inv), E::pack2(o[2] * inv, o[3] * inv)};
+  put_row<T, D>(a, hk, row, l, [&](auto&& at) __attribute__((always_inline)) { at(4 * t, o); });
 }
 
 // ---------------------------------------------------------------------------
@@ -466,6 +543,7 @@ __global__ __launch_bounds__(256) void prefix_join_kernel(PrefixArgs a, int side
 struct Plan {
   int mt, p_rt, o_rt, p_splits, o_splits, p_chunk, o_chunk;
   int64_t p_items, p_grid, grid, rows;
+  bool whole;                                // one launch without splits
   size_t bytes;
 };
 
@@ -486,6 +564,20 @@ bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, i
   const int64_t p_tiles = (Np + BN - 1) / BN, o_tiles = (cap + BN - 1) / BN;
   const int64_t p_lists = P * Hkv * p_rt, o_lists = (int64_t)B * Hkv * o_rt;
   if (p_lists > MOST || o_lists > MOST) return false;
+  // Short keys take one launch: 4.1 us and 0.78 a tile (5 and 1.27 at head_dim 256), where
+  // two take 9 and more with the sums that they pass on. By one launch / two: 4 sequences of
+  // 8 x 4 heads of 128 with 2, 4, 8 tiles 5.7 / 9.3, 7.2 / 8.4, 10.2 / 9.6 us; 64 of 8 x 8
+  // with 8, 12, 16 11.1 / 17.9, 14.2 / 18.3, 17.3 / 19.2; 8 of 20 rows of 64 with 12, 16
+  // 13.7 / 15.1, 16.9 / 17.4; 16 of 4 x 2 heads of 256 with 2, 4, 8 7.7 / 9.1, 10.2 / 10.1,
+  // 15.6 / 11.7.
+  const int64_t sums = (p.rows * Hkv * D) >> 16, most = 6 + (sums < 8 ? sums : 8);
+  p.whole = p_tiles + o_tiles <= (D == 256 ? most / 2 : most);
+  if (p.whole) {
+    p.o_rt = (int)((own + 16 * WAVES - 1) / (16 * WAVES));
+    p.grid = (int64_t)B * Hkv * p.o_rt;
+    p.p_rt = p.p_chunk = p.o_chunk = 1;
+    return p.grid <= MOST;
+  }
   const int64_t slots = 256 * waves_of(D, p.mt);
   // Tiles of an item: the count whose items end first, on a model of a launch. An
   // item takes its tiles and START more; the prefixes' items start first, the
@@ -527,6 +619,10 @@ bool plan_for(Plan& p, int B, int P, int Hkv, int G, int s, int D, int64_t Np, i
 template <typename T, int D>
 void launch(const PrefixArgs& a, const Plan& p, hipStream_t st) {
   const dim3 block(64 * WAVES);
+  if (p.whole) {
+    hipLaunchKernelGGL((prefix_whole_kernel<T, D>), dim3((unsigned)p.grid), block, 0, st, a);
+    return;
+  }
   if (p.grid > 0) {
     const dim3 grid((unsigned)p.grid);
     if (p.mt == 1) hipLaunchKernelGGL((prefix_rows_kernel<T, D, 1>), grid, block, 0, st, a);

@@ -382,7 +382,7 @@ int da_kv8_attn_fwd(const da_kv8_attn_args* args, void* stream);
  * all), read when the kernels run and clamped to the capacities; NULL: the host's
  * counts. A zero stride of q, k_prefix .. v over batch or heads is an expanded
  * tensor; of out it is DA_ERR_INVALID_ARG.
- * workspace: da_prefix_attn_workspace_bytes(...) bytes.
+ * workspace: da_prefix_attn_workspace_bytes(...) bytes, which may be 0 (short keys).
  */
 typedef struct {
   const void *q, *k_prefix, *v_prefix, *k, *v;

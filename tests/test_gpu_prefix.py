@@ -302,3 +302,71 @@ def test_agrees_with_a_cache_that_holds_both(gpu):
     kk, vv = (torch.cat([ts[i].repeat_interleave(B // P, 0), ts[i + 2]], 2) for i in (1, 2))
     ref = ops.decode_attention(ts[0], kk, vv, window=0, sink=0, sm_scale=D ** -0.5)
     assert (got.float() - ref.float()).abs().max().item() <= 6 * 2.0 ** -9 * vv.abs().max().item()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("case", [
+    # B, P, H, Hkv, s, D, Np, cap: keys that count, of larger capacities
+    (1, 1, 1, 1, 1, 32, 1, 1), (2, 1, 2, 1, 1, 64, 63, 2), (3, 3, 4, 2, 1, 128, 64, 65),
+    (4, 2, 10, 2, 1, 128, 65, 64), (5, 1, 8, 8, 1, 256, 129, 30), (40, 2, 8, 1, 1, 128, 300, 7),
+    (2, 1, 4, 2, 3, 128, 200, 3), (4, 2, 6, 2, 17, 64, 333, 130), (1, 1, 8, 2, 70, 128, 100, 200),
+    (3, 1, 4, 4, 5, 256, 90, 64), (6, 1, 5, 1, 40, 32, 150, 41), (24, 1, 8, 1, 2, 256, 70, 9),
+], ids=str)
+def test_short_keys_in_large_caches(gpu, case, dtype):
+    """Few keys of many places: split, where caches of their size are not."""
+    B, P, H, Hkv, s, D, Np, cap = case
+    run((B, P, H, Hkv, s, D, Np + 1300, cap + 900), dtype, [Np] * P, [cap] * B, seed=sum(case))
+    run((B, P, H, Hkv, s, D, Np + 1300, cap), dtype, [Np] * P, [cap] * B, seed=sum(case) + 1)
+    run((B, P, H, Hkv, s, D, Np, cap + 1300), dtype, [Np] * P, [cap] * B, seed=sum(case) + 2)
+
+
+def test_counts_in_large_caches(gpu):
+    for dtype in DT:
+        run((8, 4, 4, 2, 1, 128, 1200, 840), dtype, [1200, 0, 1, 64], [840, 0, 0, 1, 64, 65, 63, 128], 21)
+        run((6, 2, 4, 2, 5, 64, 1130, 70), dtype, [0, 129], [0, 1, 4, 5, 70, 66], 22)
+        run((4, 2, 2, 2, 3, 32, 990, 50), dtype, [-7, 1500], [-1, 3, 99, 50], 23)
+        got, _ = run((4, 2, 2, 2, 3, 256, 990, 50), dtype, [0, 0], [0, 1, 2, 3], 24)
+        assert not got[0].any() and not got[1, :, :2].any() and not got[2, :, :1].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D,s,H", [(32, 6, 4), (64, 6, 4), (128, 6, 4), (256, 6, 4), (64, 40, 8)])
+def test_hidden_places_of_large_caches(gpu, D, s, H, dtype):
+    from delta_attention import ops
+    B, P, Hkv, Np, cap = 4, 2, 2, 1150, 700
+    ts = make(B, P, H, Hkv, s, D, Np, cap, dtype, 26)
+    nps, nks = [130, 64], [490, 67, s, 64]
+    kw = dict(n_prefix=torch.tensor(nps, dtype=torch.int32, device="cuda"),
+              n_keys=torch.tensor(nks, dtype=torch.int32, device="cuda"), sm_scale=D ** -0.5)
+    want = ops.prefix_attention(*ts, **kw)
+    close(want, expect(*ts, nps, nks, D ** -0.5), dtype)
+    q, kp, vp, k, v = (t.clone() for t in ts)
+    for p in range(P):
+        kp[p, :, nps[p]:] = math.nan
+        vp[p, :, nps[p]:] = math.inf
+    for b in range(B):
+        k[b, :, nks[b]:] = math.inf
+        v[b, :, nks[b]:] = math.nan
+        v[b, :, nks[b] - 1, ::3] = -math.inf     # the last row's own place
+        v[b, :, nks[b] - 1, 1] = math.nan
+    got = ops.prefix_attention(q, kp, vp, k, v, **kw)
+    assert torch.equal(got[:, :, :s - 1], want[:, :, :s - 1])
+    assert (got[:, :, s - 1, ::3] == -math.inf).all() and torch.isnan(got[:, :, s - 1, 1]).all()
+    assert torch.equal(got[:, :, s - 1, 2::3], want[:, :, s - 1, 2::3])
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_lengths_around_the_split(gpu, D):
+    """Capacities from one tile past the longest that one launch takes, batches
+    with few sums and with many, the references moving in either set."""
+    from delta_attention import ops
+    for B, H, s in ((2, 2, 1), (64, 16, 1), (4, 8, 9)):
+        for tiles in (1, 2, 3, 4, 6, 7, 8, 12, 13, 14, 15):
+            own = min(64 * (tiles // 2) + s, 64 * tiles)
+            run((B, 2, H, 2, s, D, 64 * tiles - own + 1, own), "bf16", seed=tiles + B)
+    ts = make(4, 2, 4, 2, 2, D, 120, 100, "fp16", 28)
+    for i in (1, 3):
+        kk = list(ts)
+        kk[i] = (kk[i].float() * torch.linspace(0.1, 8, kk[i].shape[2], device="cuda")[:, None]).half()
+        got = ops.prefix_attention(*kk, sm_scale=0.3)
+        close(got, expect(*kk, [120] * 2, [100] * 4, 0.3), "fp16")

@@ -105,7 +105,9 @@ def test_c_refusals_and_workspace(lib):
     for bad in (dict(q=24), dict(kp=24), dict(vp=8), dict(k=20), dict(v=17), dict(out=24), dict(npd=18), dict(nkd=17),
                 dict(qs=(256, 68, 64)), dict(kps=(1281, 640, 64)), dict(vs=(128, 64, 132)), dict(os=(256, 64, 12)), dict(ws=24)):
         assert call(**bad) == L.DA_ERR_ALIGNMENT, bad
-    need = ws(4, 2, 4, 2, 1, 64, 10, 6)
-    assert need > 0 and call(nb=need - 1) == call(ws=0) == L.DA_ERR_WORKSPACE
+    assert ws(4, 2, 4, 2, 1, 64, 10, 6) == 0             # (short keys need none)
+    long = dict(Np=2000, npre=2000)
+    need = ws(4, 2, 4, 2, 1, 64, 2000, 6)
+    assert need > 0 and call(nb=need - 1, **long) == call(ws=0, **long) == L.DA_ERR_WORKSPACE
     assert call(s=0) == call(B=0) == L.DA_OK             # nothing launched
     assert lib.da_prefix_attn_fwd(None, None) == L.DA_ERR_INVALID_ARG
