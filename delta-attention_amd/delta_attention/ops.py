@@ -715,7 +715,7 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     all), numbers or int32 device tensors of one entry or one per prefix /
     sequence, read when the kernels run (a recorded call serves every length;
     counts are clamped to the capacities). A new result has q's strides where q
-    is dense."""
+    is dense; a given one (out) lies apart from the inputs."""
     return L.gen_ext().prefix(q, k_prefix, v_prefix, k, v, n_prefix, n_keys, sm_scale, out)
 
 

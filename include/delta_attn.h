@@ -381,7 +381,7 @@ int da_kv8_attn_fwd(const da_kv8_attn_args* args, void* stream);
  * device (an entry per prefix or sequence where the flag is set, else one for
  * all), read when the kernels run and clamped to the capacities; NULL: the host's
  * counts. A zero stride of q, k_prefix .. v over batch or heads is an expanded
- * tensor; of out it is DA_ERR_INVALID_ARG.
+ * tensor; of out it is DA_ERR_INVALID_ARG. out lies apart from the inputs.
  * workspace: da_prefix_attn_workspace_bytes(...) bytes, which may be 0 (short keys).
  */
 typedef struct {
