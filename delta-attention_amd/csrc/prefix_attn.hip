@@ -13,7 +13,7 @@
 // What bounds it: up to some 128 rows a kv head the keys' bytes (16 sequences of 32 / 8
 // heads of 128 over 131072 keys 108 us in all, 5.4 TB/s; one sequence alone takes 90), past
 // that the matrix products and the exponentials beside them (128 sequences over 65536 keys
-// 185 us, 740 TFLOP/s; 16 of 128 rows each over 32768 keys 1050), and for few keys two
+// 178 us, 775 TFLOP/s; 16 of 128 rows each over 32768 keys 1050), and for few keys two
 // launches (10.5 us for 2711) or one (5.7 to 7.2 us up to 256). The rows of a batch over whole caches, each with a copy of the prefix,
 // take 50 us where 16 share 4096 keys in 15, and 324 where 4 share 131072 in 92.
 #include <float.h>
