@@ -61,7 +61,7 @@ constexpr uint32_t KEY_NONE = 0x007fffffu;   // -inf's key: candidates lie above
 constexpr int PART = 512;                    // threads of a part
 constexpr int LIST = 3584;                   // tokens of a row's list (LDS for two workgroups a CU)
 constexpr int BINS = 768;                    // of a part's histogram
-constexpr int GROUPS = 2048;                 // group maxima of a row
+constexpr int GROUPS = 2048;                 // group maxima of a row (four a thread of a part)
 constexpr int SLOTS = 1024;                  // tile sums in LDS
 
 struct Part {
@@ -433,28 +433,27 @@ __device__ __forceinline__ void ends_of(const Row<T>& row, const Order<T>& ord, 
 }
 
 // A number that fewer than k of the groups' maxima's first 16 bits pass: the
-// largest one of 16 bits that is no larger than the k-th largest maximum, bit by bit,
-// by the count of maxima that reach it. One wave works on all maxima, M a lane (in each
-// wave of the workgroup it took 3 us more); up to 384 the groups of a lane are taken as
-// eight: a quarter of the counting for a list that is hardly longer.
-template <int M>
-__device__ __forceinline__ float list_bar(uint32_t (&key)[M], int k) {
+// largest one of 16 bits that is no larger than the k-th largest maximum, two bits at a
+// time, by the counts of maxima that reach it, the workgroup's together. (By one wave for
+// all maxima, a bit at a time without barriers, top_k 700 took 25 us for 21.) key: the
+// thread's maxima. s: 24 words.
+template <int N>
+__device__ __forceinline__ float list_bar(const uint32_t (&key)[GROUPS / N], int k, uint32_t* s) {
+  const int lane = threadIdx.x % 64;
+  if (threadIdx.x < 24) s[threadIdx.x] = 0;
+  __syncthreads();
   uint32_t low = 0;
-  auto search = [&](auto many) __attribute__((always_inline)) {
-    for (int bit = 15; bit >= 0; --bit) {
-      const uint32_t c = low | 1u << bit;
-      int n = 0;
 #pragma unroll
-      for (int i = 0; i < decltype(many)::value; ++i) n += __popcll(__ballot(key[i] >> 16 >= c));
-      if (n >= k) low = c;
-    }
-  };
-  if (k <= 384) {
+  for (int r = 0; r < 8; ++r) {
+    const int bit = 14 - 2 * r;
+    int n[3] = {};
 #pragma unroll
-    for (int i = 8; i < M; ++i) key[i % 8] = max(key[i % 8], key[i]);
-    search(std::integral_constant<int, 8>{});
-  } else {
-    search(std::integral_constant<int, M>{});
+    for (int j = 0; j < 3; ++j)
+#pragma unroll
+      for (int i = 0; i < GROUPS / N; ++i) n[j] += __popcll(__ballot(key[i] >> 16 >= (low | (j + 1) << bit)));
+    if (lane < 3) atomicAdd(&s[3 * r + lane], (uint32_t)(lane == 0 ? n[0] : lane == 1 ? n[1] : n[2]));
+    __syncthreads();
+    low |= ((s[3 * r] >= (uint32_t)k) + (s[3 * r + 1] >= (uint32_t)k) + (s[3 * r + 2] >= (uint32_t)k)) << bit;
   }
   return of_key(max(low << 16, KEY_NONE + 1));
 }
@@ -709,9 +708,7 @@ struct Room {
   static constexpr int N = threads_of(MODE);
   uint64_t list[LIST], w[LIST], slot[MODE == SHORT ? 1 : SLOTS], scan[reach_words(N)], found[2];
   uint64_t hist[MODE == WHOLE ? BINS : 1];
-  uint32_t max[MODE == WHOLE ? GROUPS : 4];
-  uint32_t n, at;
-  float bar;
+  uint32_t count[MODE == SHORT ? 1 : 24], n, at;
 };
 
 // A word for a workgroup of the same launch, or of one.
@@ -973,13 +970,13 @@ template <typename T, int MODE>
 __global__ __launch_bounds__(threads_of(MODE)) void sample_row_kernel(SampleArgs a) {
   constexpr int N = threads_of(MODE);
   __shared__ __align__(16) Room<MODE> m;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid % 64;
+  const int b = blockIdx.x, tid = threadIdx.x;
   const Setting s = setting_of(a, b);
   const Row<T> row(a, b);
   const Order<T> ord(a.V);
   const int tiles = (row.n_vec + 63) / 64, per = (tiles + SLOTS - 1) / SLOTS;   // tiles of a slot
   uint64_t first;
-  uint32_t least = KEY_NONE + 1;
+  uint32_t least = KEY_NONE + 1, maxima[MODE == WHOLE ? GROUPS / N : 1];
   if constexpr (MODE == PARTS) {
     row_ends(a, b, first, least);
   } else if constexpr (MODE == WHOLE) {
@@ -990,7 +987,7 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_row_kernel(SampleArgs
     float group[GROUPS / N];
     ends_of(sweep, a.runs, most, at, low, group);
 #pragma unroll
-    for (int g = 0; g < GROUPS / N; ++g) m.max[g * N + tid] = key_of(group[g]);
+    for (int g = 0; g < GROUPS / N; ++g) maxima[g] = key_of(group[g]);
     ends_of(row, ord, most, at, low, first, turned);
     first = block_all<N>(first, m.scan, Most());
     least = ~(uint32_t)block_all<N>(turned, m.scan, Most());
@@ -1019,18 +1016,8 @@ __global__ __launch_bounds__(threads_of(MODE)) void sample_row_kernel(SampleArgs
     __syncthreads();
     if (s.list) {
       Sweep<T, N / 64, 4> sweep(row, 0, tiles);
-      if (tid < 64) {                       // (one wave, for all)
-        uint32_t key[GROUPS / 64];
-#pragma unroll
-        for (int i = 0; i < GROUPS / 256; ++i) {
-          const u32x4 w = *(const u32x4*)&m.max[(i * 64 + lane) * 4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) key[4 * i + e] = w[e];
-        }
-        m.bar = list_bar(key, s.k);
-      }
-      __syncthreads();
-      gather_into(sweep, ord, m.bar, m.list, &m.n);
+      const float bar = list_bar<N>(maxima, s.k, m.count);
+      gather_into(sweep, ord, bar, m.list, &m.n);
     } else if (!s.cut) {
       if (s.run) {
         Sweep<T, N / 64, 2> sweep(row, 0, tiles);
@@ -1117,30 +1104,17 @@ __device__ __forceinline__ bool last_part(const SampleArgs& a, int b, Room<PARTS
 template <typename T>
 __global__ __launch_bounds__(PART) void sample_gather_kernel(SampleArgs a) {
   __shared__ __align__(16) Room<PARTS> m;
-  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts, lane = threadIdx.x % 64;
+  const int b = fdiv(blockIdx.x, a.f_parts), part = blockIdx.x - b * a.parts;
   const Setting s = setting_of(a, b);
   if (a.sums && !(s.cut ? s.list : s.run && !s.greedy)) return;
   const Row<T> row(a, b);
   const Order<T> ord(a.V);
   if (s.list) {
     Sweep<T, PART / 64, 4> sweep(row, part * a.tiles, a.tiles);
-    if (threadIdx.x < 64) {                 // (one wave, for all)
-      const uint32_t* mx = a.maxima + (int64_t)b * GROUPS;
-      uint32_t key[GROUPS / 64];
-#pragma unroll
-      for (int i = 0; i < GROUPS / 256; ++i) {
-        const u32x4 w = *(const u32x4*)(mx + (i * 64 + lane) * 4);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) key[4 * i + e] = w[e];
-      }
-      const float bar = list_bar(key, s.k);
-      if (lane == 0) {
-        m.bar = bar;
-        m.n = 0;
-      }
-    }
-    __syncthreads();
-    const float bar = m.bar;
+    const u32x4 mx = *(const u32x4*)(a.maxima + (int64_t)b * GROUPS + threadIdx.x * 4);
+    const uint32_t key[] = {mx[0], mx[1], mx[2], mx[3]};
+    if (threadIdx.x == 0) m.n = 0;
+    const float bar = list_bar<PART>(key, s.k, m.count);
     gather_into(sweep, ord, bar, m.list, &m.n);
     append(a, b, m);
     if (a.sums || !last_part(a, b, m)) return;
