@@ -384,3 +384,23 @@ def test_the_ends_of_float32(gpu, B, V):
         y[:, ::3] = torch.finfo(torch.float32).min
         for s in (dict(top_p=0.6), dict(top_k=300, top_p=0.9)):
             check(y, u, sure=False, temperature=torch.tensor([T]).cuda(), **s)
+
+
+def test_calls_at_once(gpu):
+    """Calls of two streams beside each other, their parts among each other's."""
+    from delta_attention import ops
+    sets = [(logits(48, 60000, "bf16", 70), uniform(48, 71)), (logits(70, 40000, "fp32", 72), uniform(70, 73))]
+    settings = [dict(top_p=0.9), dict(top_k=700, top_p=0.95), dict(), dict(temperature=1.6, top_p=0.99)]
+    want = [[ops.sample_tokens(x, u, **s) for s in settings] for x, u in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(6):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i] += [ops.sample_tokens(*sets[i], **s) for s in settings]
+    torch.cuda.synchronize()
+    for i in (0, 1):
+        for j, (t, lp) in enumerate(got[i]):
+            w = want[i][j % len(settings)]
+            assert torch.equal(t, w[0]) and torch.equal(lp, w[1]), (i, j)
