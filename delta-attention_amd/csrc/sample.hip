@@ -136,7 +136,7 @@ __device__ __forceinline__ uint64_t raw_weight(double d, double per, double whol
   const double whole = fma(d, per, whole_of), f = fma(d, per, whole_of - whole);
   double p = 7.072585949269223e-09;
   constexpr double c[] = {1.0208690299958306e-07, 1.321544258792169e-06, 1.5252657260200837e-05, 0.0001540353044173605,
-                          0.0013333558230164974, 0.009618129107606888, 0.05550410866447172, 0.24022650695910097,
+                          0.0013333558230164974, 0.009618129107606888, 0.05550410866444772, 0.24022650695910097,
                           0.69314718055995, 1.0};
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
