@@ -187,7 +187,7 @@ __device__ __forceinline__ int walk(const PrefixArgs& a, Rows<T, D, MT>& rows, c
   int lim[MT], lim_lo = lim0, lim_hi = lim0;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) lim[mt] = OWN ? lim0 + rows.own[mt] : lim0;
-  if (OWN) {                                 // of the whole row tile
+  if (OWN) {                                 // of the whole row tile (which may be a single row's heads)
     const int u = fdiv(row0, a.heads), w = fdiv(row0 + n_rows - 1, a.heads);
     lim_lo += u - (int)fdiv(u, a.rows_s) * a.s;
     lim_hi += w - (int)fdiv(w, a.rows_s) * a.s;
@@ -207,7 +207,7 @@ __device__ __forceinline__ int walk(const PrefixArgs& a, Rows<T, D, MT>& rows, c
   auto issue = [&](bool values, int t) __attribute__((always_inline)) {
     const int first = key0 + t * BN;
     const uint32_t step = values ? v_s : k_s;
-    const int64_t left = (int64_t)(n_keys - first - 1) * step + TL::RB;   // what lies behind the last key reads as zero
+    const int64_t left = (int64_t)(lim_hi - first) * step + TL::RB;   // what lies behind the last key seen reads as zero
     const u32x4 r = rsrc_words((values ? vb : kb) + (int64_t)first * step, left >> 32 ? 0xffffffffu : (uint32_t)left);
     const uint32_t st = lds0 + (t % 2 * 2 + values) * TL::BYTES + wave * 1024;
 #pragma unroll
@@ -314,7 +314,7 @@ __device__ __forceinline__ int walk(const PrefixArgs& a, Rows<T, D, MT>& rows, c
       return (u32x4){v0[0], v0[1], v1[0], v1[1]};
     };
     // An infinity or NaN among the values of a key that one of the rows does not see
-    // must not reach it through 0 * inf (keys past the last one are loaded as zero).
+    // must not reach it through 0 * inf (keys that none of them sees are loaded as zero).
     bool odd = false;
     if (OWN && !whole && lim_lo < lim_hi) {
 #pragma unroll
