@@ -121,7 +121,11 @@ PyObject* prefix(PyObject* const* a) {
   x.sm_scale = (float)number(a[7], "sm_scale");
   const On on(dev);
   at::Tensor in[5], out, ws;
-  for (int i = 0; i < 5; ++i) in[i] = ready(*t[i]);
+  for (int i = 0; i < 5; ++i) {
+    // (keys that share their places, as one key read as many does, are copied too)
+    const bool apart = i == 0 || t[i]->size(2) <= 1 || t[i]->stride(2) >= D;
+    in[i] = apart ? ready(*t[i]) : t[i]->clone(at::MemoryFormat::Contiguous);
+  }
   if (a[8] == Py_None) {
     out = at::empty_like(in[0]);
   } else {

@@ -649,10 +649,12 @@ void by_dim(int D, const PrefixArgs& a, const Plan& p, hipStream_t st) {
   else launch<T, 256>(a, p, st);
 }
 
-// Bytes from key to key, at most 2^25 (a tile's offsets stay inside 32 bits).
-bool key_stride(uint32_t& to, int64_t elements, int keys) {
-  if (keys > 1 && (elements < 0 || elements > 1 << 24)) return false;
-  to = keys > 1 ? (uint32_t)(2 * elements) : 0;
+// Bytes from key to key: at most 2^25 (a tile's offsets stay inside 32 bits), and a key's
+// own at least, also where there is one key: the places of a tile behind the last key lie
+// behind that key's end, where loads give zero.
+bool key_stride(uint32_t& to, int64_t elements, int keys, int D) {
+  if (keys > 1 && (elements < D || elements > 1 << 24)) return false;
+  to = (uint32_t)(2 * (keys > 1 ? elements : D));
   return true;
 }
 
@@ -690,8 +692,8 @@ extern "C" int da_prefix_attn_fwd(const da_prefix_attn_args* x, void* stream) {
       !strides8(x->k_str) || !strides8(x->v_str) || ((uintptr_t)x->n_prefix_dev & 3) || ((uintptr_t)x->n_keys_dev & 3))
     return DA_ERR_ALIGNMENT;
   PrefixArgs a{};
-  if (!key_stride(a.kp_s, x->kp_str[2], Np) || !key_stride(a.vp_s, x->vp_str[2], Np) ||
-      !key_stride(a.k_s, x->k_str[2], cap) || !key_stride(a.v_s, x->v_str[2], cap))
+  if (!key_stride(a.kp_s, x->kp_str[2], Np, x->D) || !key_stride(a.vp_s, x->vp_str[2], Np, x->D) ||
+      !key_stride(a.k_s, x->k_str[2], cap, x->D) || !key_stride(a.v_s, x->v_str[2], cap, x->D))
     return DA_ERR_INVALID_ARG;
   const int G = Hq / Hkv;
   Plan p;

@@ -706,7 +706,8 @@ def prefix_attention(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Te
     """The last s rows of each sequence of a batch that shares prefixes
     (da_prefix_attn_fwd): q [B, H, s, D]; k_prefix / v_prefix [P, Hkv, Np, D], of
     which every B / P sequences in a row share one; k / v [B, Hkv, n, D], each
-    sequence's own keys (any strides, GQA native) -> [B, H, s, D]. Row i stands
+    sequence's own keys (any strides, GQA native; keys that overlap, as one read
+    as many does, are copied first) -> [B, H, s, D]. Row i stands
     at n - s + i of its own keys and sees those up to itself and the whole
     prefix; a row that sees no key is zero. A prefix's keys are read once for
     all its sequences.

@@ -376,8 +376,8 @@ int da_kv8_attn_fwd(const da_kv8_attn_args* args, void* stream);
  * key is zero; one whose every score is -inf is NaN. Keys and values of places
  * that a row does not see reach it in no way, whatever they hold.
  * q, out [B, Hq, s, D] (strides {batch, head, row}); k_prefix, v_prefix
- * [P, Hkv, max_prefix, D], k, v [B, Hkv, max_keys, D] ({batch, head, key}; at most
- * 2^24 elements from key to key). n_prefix_dev / n_keys_dev: int32 counts on the
+ * [P, Hkv, max_prefix, D], k, v [B, Hkv, max_keys, D] ({batch, head, key}; where there
+ * is more than one key, D to 2^24 elements from key to key). n_prefix_dev / n_keys_dev: int32 counts on the
  * device (an entry per prefix or sequence where the flag is set, else one for
  * all), read when the kernels run and clamped to the capacities; NULL: the host's
  * counts. A zero stride of q, k_prefix .. v over batch or heads is an expanded

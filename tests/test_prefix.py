@@ -111,3 +111,23 @@ def test_c_refusals_and_workspace(lib):
     assert need > 0 and call(nb=need - 1, **long) == call(ws=0, **long) == L.DA_ERR_WORKSPACE
     assert call(s=0) == call(B=0) == L.DA_OK             # nothing launched
     assert lib.da_prefix_attn_fwd(None, None) == L.DA_ERR_INVALID_ARG
+
+
+def test_keys_that_overlap_are_refused_in_c(lib):
+    """Keys nearer each other than a key's own elements: what lies behind the last
+    one would be its own bytes again. (ops.prefix_attention copies such tensors.)"""
+    def call(Np, n, **strides):
+        st = dict(kps=(1280, 640, 64), vps=(1280, 640, 64), ks=(128, 64, 128), vs=(128, 64, 128))
+        st.update(strides)
+        return lib.da_prefix_attn_fwd(ARGS.pack(16, 16, 16, 16, 16, 16, 0, 0, 16, 0, 256, 64, 64, *st["kps"], *st["vps"],
+                                                *st["ks"], *st["vs"], 256, 64, 64, 4, 2, 4, 2, 1, 64, Np, n, Np, n, 0, 0,
+                                                L.DA_BF16, 0.1), None)
+
+    for name in ("kps", "vps", "ks", "vs"):
+        for step in (0, 8, 56, -64, (1 << 24) + 8):
+            assert call(2000, 2000, **{name: (1280, 640, step)}) == L.DA_ERR_INVALID_ARG, (name, step)
+    # (as far as the workspace's check: strides that are taken)
+    for strides in (dict(), dict(ks=(1280, 640, 1 << 24))):
+        assert call(2000, 2000, **strides) == L.DA_ERR_WORKSPACE
+    # a set of one key has no step
+    assert call(1, 2000, kps=(1280, 640, 0), vps=(1280, 640, -8)) == call(2000, 1, ks=(64, 64, 0)) == L.DA_ERR_WORKSPACE
