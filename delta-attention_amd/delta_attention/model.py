@@ -602,8 +602,7 @@ class LlamaForCausalLM(nn.Module):
                  max_new_tokens: int = 128, do_sample: bool = False, eos_token_id=None,
                  pad_token_id: Optional[int] = None, graph: bool = False,
                  generator: Optional[torch.Generator] = None, num_return_sequences: int = 1,
-                 temperature: Optional[float] = None, top_k: Optional[int] = None,
-                 top_p: Optional[float] = None, min_p: Optional[float] = None, **unused) -> torch.Tensor:
+                 temperature=None, top_k=None, top_p=None, min_p=None, **unused) -> torch.Tensor:
         """The call model_wrapper.py:97 makes (HF `generate` with the greedy
         `_sample` loop of sample.py:25-262): -> [b, s + n] token ids, the
         prompt (with its padding) followed by the generated tokens; after a
@@ -617,8 +616,9 @@ class LlamaForCausalLM(nn.Module):
         a torch.Generator on the model's device: without one it raises, nothing
         is drawn from a hidden state. num_return_sequences of each prompt, behind
         each other ([b * num_return_sequences, s + n]); temperature, top_k, top_p
-        and min_p default to 1, 50, 1 and 0, Hugging Face's defaults. Greedy
-        decoding ignores all of these."""
+        and min_p (numbers, or device tensors of one entry or one per sequence)
+        default to 1, 50, 1 and 0, Hugging Face's defaults. Greedy decoding
+        ignores all of these."""
         if do_sample and generator is None:
             raise NotImplementedError("do_sample=True draws from given random numbers: pass generator= "
                                       "(a torch.Generator on the model's device)")
@@ -628,20 +628,23 @@ class LlamaForCausalLM(nn.Module):
         n_seq = int(num_return_sequences) if do_sample else 1
         if n_seq < 1:
             raise ValueError(f"num_return_sequences {num_return_sequences}: one at least")
-        u = None
+        u, settings = None, {}
         if do_sample:
             u = torch.rand(b * n_seq, max_new_tokens, device=input_ids.device, generator=generator)
+            settings = dict(temperature=1.0 if temperature is None else temperature, top_k=50 if top_k is None else top_k,
+                            top_p=1.0 if top_p is None else top_p, min_p=0.0 if min_p is None else min_p)
+            for name, x in settings.items():
+                assert not isinstance(x, torch.Tensor) or x.numel() in (1, b * n_seq), (
+                    f"{name}: {x.numel()} entries for {b * n_seq} sequences")
 
         def run(ids: torch.Tensor, first: int) -> list:
             if not do_sample:
                 return list(self.generate_greedy(ids, max_new_tokens, graph=graph,
                                                  eos_token_id=eos_token_id).unbind(0))
-            mine = u[first * n_seq:(first + ids.shape[0]) * n_seq]
-            return list(self.generate_sampled(
-                ids, max_new_tokens, mine, temperature=1.0 if temperature is None else temperature,
-                top_k=50 if top_k is None else top_k, top_p=1.0 if top_p is None else top_p,
-                min_p=0.0 if min_p is None else min_p, samples=n_seq, graph=graph,
-                eos_token_id=eos_token_id).unbind(0))
+            at = slice(first * n_seq, (first + ids.shape[0]) * n_seq)
+            mine = {name: x[at] if isinstance(x, torch.Tensor) and x.numel() > 1 else x for name, x in settings.items()}
+            return list(self.generate_sampled(ids, max_new_tokens, u[at], samples=n_seq, graph=graph,
+                                              eos_token_id=eos_token_id, **mine).unbind(0))
 
         if pad_token_id is None:
             pad_token_id = (eos_token_id if isinstance(eos_token_id, int)
