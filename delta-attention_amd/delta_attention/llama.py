@@ -446,6 +446,7 @@ class LlamaAttention(nn.Module):
         b, h, s, d = query_states.size()
         n_keys = kwargs.get("n_keys")
         if s == 1 and getattr(self.config, "decode_mode", "dense") != "dense":
+            self._refuse_shared(isinstance(key_states, SharedKeys))
             return self.delta_decode_forward(module, query_states, key_states, value_states,
                                              scaling=scaling, **kwargs)
         q, k, v = self._half(query_states, key_states, value_states)
@@ -463,6 +464,12 @@ class LlamaAttention(nn.Module):
             mask = torch.arange(n - s, n, device=q.device, dtype=torch.int64)[None]
             out = qsa_kernel(q, k, v, mask, float(scaling))
         return out.transpose(1, 2).contiguous().to(query_states.dtype), None
+
+    def _refuse_shared(self, shared: bool):
+        """(the sparse and delta decodes read one sequence's own cache)"""
+        if shared:
+            raise NotImplementedError("sequences that share their prompts take dense decode steps "
+                                      f"(decode_mode {self.config.decode_mode!r} runs one sequence)")
 
     @staticmethod
     def _half(q, k, v):
@@ -616,6 +623,8 @@ class LlamaAttention(nn.Module):
             if kind is not None and past_key_value.len[self.layer_idx] > 0:
                 raise NotImplementedError(f"the delta prefill takes a whole prompt, and the {kind} cache already "
                                           "holds tokens (continue with 'sdpa_rectangle')")
+        elif input_shape[1] == 1 and getattr(self.config, "decode_mode", "dense") != "dense":
+            self._refuse_shared(getattr(past_key_value, "shared", False))
         static = (past_key_value is not None and getattr(past_key_value, "static", False)
                   and not getattr(past_key_value, "eight_bit", False)
                   and hidden_states.dtype in (torch.bfloat16, torch.float16))
