@@ -18,6 +18,7 @@ import sysconfig
 import tempfile
 import warnings
 from concurrent.futures import ThreadPoolExecutor
+from typing import Optional, Union
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -100,14 +101,14 @@ def _extensions() -> list:
             (GEN_SOURCE, os.path.join(os.path.dirname(EXT_OUT), "_gen_ext.so"), "the generation calls are")]
 
 
-def build_ext(verbose: bool = False) -> list:
-    """The extension modules alone."""
-    outs = []
-    for source, out, _ in _extensions():
-        _compile_ext(verbose, source, out + ".tmp")
-        os.replace(out + ".tmp", out)
-        outs.append(out)
-    return outs
+def build_ext(verbose: bool = False, out: Optional[str] = None) -> Union[str, list]:
+    """The extension modules alone -> their paths; or (out) the 8-bit cache's at
+    that path -> it."""
+    todo = [(EXT_SOURCE, out)] if out else [(source, path) for source, path, _ in _extensions()]
+    for source, path in todo:
+        _compile_ext(verbose, source, path + ".tmp")
+        os.replace(path + ".tmp", path)
+    return out or [path for _, path in todo]
 
 
 def build(verbose: bool = False, out: str = OUT) -> str:

@@ -53,3 +53,11 @@ def test_one_that_does_not_compile_is_left_out(built, source, what):
         build_lib.build(out=lib)
     assert read(lib) == "new" and not os.path.exists(paths[source])
     assert all(read(p) == "new" for s, p in paths.items() if s != source)
+
+
+def test_one_module_at_a_given_path(built, tmp_path):
+    """build_ext(out=path): the 8-bit cache's module alone, there."""
+    _, paths, _ = built
+    to = str(tmp_path / "elsewhere.so")
+    assert build_lib.build_ext(out=to) == to and build_lib.build_ext(False, to) == to
+    assert read(to) == "new" and all(read(p) == "old" for p in paths.values())
