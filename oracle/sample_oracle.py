@@ -24,7 +24,9 @@ def weights(x, top, T):
 def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     """-> (token, log-probability, margin): margin is the least distance, relative
     to a total, of a border of the sums from what it is compared with, or of a
-    logit from min_p's bar (inf: no such comparison)."""
+    logit from min_p's bar, in temperatures and past what the bar's own float64
+    may be off by (inf: no such comparison; logits equal to the largest need
+    none, the bar is never above it)."""
     x = np.asarray(x, np.float64)
     order = order_of(x)
     if len(order) == 0:
@@ -48,8 +50,10 @@ def sample(x, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         bar = top + temperature * math.log(min_p)
         rest = x[order[1:]]
         with np.errstate(invalid="ignore"):
-            if math.isfinite(bar) and len(rest) and min_p != 1:     # (ln 1 = 0: the bar is the top, exactly)
-                margin = min(margin, float(np.abs(rest - bar).min() / max(abs(bar), 1.0)))
+            if math.isfinite(bar) and min_p != 1:     # (ln 1 = 0: the bar is the top, exactly)
+                off = (abs(top) + temperature * abs(math.log(min_p))) * 2.0 ** -51
+                far = np.abs(rest[rest != top] - bar).min(initial=math.inf)
+                margin = min(margin, max(float(far - off), 0.0) / temperature)
             order = order[:1 + int((rest >= bar).sum())]
     order = np.sort(order)
     w = weights(x[order], top, temperature)
