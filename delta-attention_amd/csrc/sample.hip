@@ -1193,6 +1193,8 @@ struct Plan {
 //   32000 x 96           18 / 17    15 / 20    31 / 31      36 / 34
 //   16000 x 16           14 / 12    14 / 16    22 / 22      23 / 23
 //   8192 x 1             11 / 12    13 / 15    18 / 21      19 / 21
+// (One rule for all settings: a nucleus of 192 rows is 8 % faster by parts. Past 256 rows
+// there is a second round of workgroups: 257 rows with top_p 0.9 165 us, 256 90, 512 177.)
 bool by_rows(int B, int V) { return B >= 160 || V <= 8192 || (B >= 64 && V <= 32768); }
 
 void plan_for(Plan& p, int B, int V, int dtype, bool differ) {
